@@ -10,8 +10,14 @@ Neighbours of the core in the Qwen3-Next layer (``layer_ops``):
     fused_gdn_gating (differentiable; fused_gdn_gating_bwd), l2norm_fwd,
     causal_conv1d_fn, causal_conv1d_update, rms_norm_gated
 
-All call hand-written HIP kernels through the C ABI in include/gdn.h and
-include/gdn_layer.h (``libgdn.so``, built by ``python -m avelang_amd.build``).
+Linear attention with a decay for each head (``linear_attention``):
+    chunk_linear_attn (differentiable; chunk_linear_attn_bwd),
+    fused_recurrent_linear_attn
+Layer norm (``norm``):
+    layer_norm (differentiable; layer_norm_bwd)
+
+All call hand-written HIP kernels through the C ABI in include/gdn.h,
+include/gdn_layer.h and include/gdn_linear.h (``libgdn.so``, built by ``python -m avelang_amd.build``).
 """
 from .gated_delta_rule import (  # noqa: F401
     chunk_bwd_workspace_bytes,
@@ -31,6 +37,14 @@ from .layer_ops import (  # noqa: F401
     l2norm_fwd,
     rms_norm_gated,
 )
+from .linear_attention import (  # noqa: F401
+    chunk_linear_attn,
+    chunk_linear_attn_bwd,
+    chunk_linear_attn_fwd_save,
+    fused_recurrent_linear_attn,
+    linear_attn_workspace_bytes,
+)
+from .norm import layer_norm, layer_norm_bwd, layer_norm_fwd_save  # noqa: F401
 
 __all__ = [
     "chunk_gated_delta_rule",
@@ -47,4 +61,12 @@ __all__ = [
     "causal_conv1d_fn",
     "causal_conv1d_update",
     "rms_norm_gated",
+    "chunk_linear_attn",
+    "chunk_linear_attn_bwd",
+    "chunk_linear_attn_fwd_save",
+    "fused_recurrent_linear_attn",
+    "linear_attn_workspace_bytes",
+    "layer_norm",
+    "layer_norm_bwd",
+    "layer_norm_fwd_save",
 ]

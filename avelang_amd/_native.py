@@ -44,6 +44,19 @@ EXPORTS = (
 # Declared in include/gdn_rows.h.
 EXPORTS_ROWS = ("gdn_chunk_fwd_rows", "gdn_recurrent_fwd_rows")
 
+# Declared in include/gdn_linear.h.
+EXPORTS_LINEAR = (
+    "gdn_linear_chunk_fwd",
+    "gdn_linear_chunk_workspace_bytes",
+    "gdn_linear_states_bytes",
+    "gdn_linear_chunk_bwd",
+    "gdn_linear_chunk_bwd_workspace_bytes",
+    "gdn_linear_recurrent_fwd",
+    "gdn_layer_norm_fwd",
+    "gdn_layer_norm_bwd",
+    "gdn_layer_norm_bwd_workspace_bytes",
+)
+
 GDN_DTYPE_F32 = 0
 GDN_DTYPE_BF16 = 1
 GDN_DTYPE_F16 = 2
@@ -178,6 +191,38 @@ def lib():
                                          + [_f, _i, _vp, _sz, _vp])
         h.gdn_recurrent_fwd_rows.restype = _i
         h.gdn_recurrent_fwd_rows.argtypes = _rows + [_vp] * 5 + [_i] * 8 + [_f, _i, _vp]
+        # q k v, their token strides, g, its type, one per head
+        _lin = [_vp] * 3 + [_ll] * 3 + [_vp, _i, _i]
+        h.gdn_linear_chunk_workspace_bytes.restype = _sz
+        h.gdn_linear_chunk_workspace_bytes.argtypes = [_i] * 8
+        h.gdn_linear_chunk_bwd_workspace_bytes.restype = _sz
+        h.gdn_linear_chunk_bwd_workspace_bytes.argtypes = [_i] * 8
+        h.gdn_linear_states_bytes.restype = _sz
+        h.gdn_linear_states_bytes.argtypes = [_i] * 7   # B T Hv K V N has_cu_seqlens
+        h.gdn_linear_chunk_fwd.restype = _i
+        h.gdn_linear_chunk_fwd.argtypes = (
+            _lin + [_vp] * 4                  # h0 ht o cu_seqlens
+            + [_i] * 7 + [_f]                 # B T Hqk Hv K V N, scale
+            + [_vp, _vp, _sz, _vp])           # states, ws, ws bytes, stream
+        h.gdn_linear_chunk_bwd.restype = _i
+        h.gdn_linear_chunk_bwd.argtypes = (
+            _lin + [_vp] * 3                  # dO dht states
+            + [_vp] * 6                       # dq dk dv dg dh0 cu_seqlens
+            + [_i] * 7 + [_f] + [_vp, _sz, _vp])
+        h.gdn_linear_recurrent_fwd.restype = _i
+        h.gdn_linear_recurrent_fwd.argtypes = (
+            _lin + [_vp] * 5                  # h0 ht o cu_seqlens state_indices
+            + [_i] * 8 + [_f, _vp])           # ... N num_slots, scale, stream
+        h.gdn_layer_norm_fwd.restype = _i
+        h.gdn_layer_norm_fwd.argtypes = (
+            [_vp] * 5                         # x weight bias y stats
+            + [_ll, _i, _i, _f, _i, _i, _vp])  # rows heads D eps dtype w_dtype stream
+        h.gdn_layer_norm_bwd_workspace_bytes.restype = _sz
+        h.gdn_layer_norm_bwd_workspace_bytes.argtypes = [_ll, _i, _i, _i]
+        h.gdn_layer_norm_bwd.restype = _i
+        h.gdn_layer_norm_bwd.argtypes = (
+            [_vp] * 7                         # x weight dy stats dx dweight dbias
+            + [_ll, _i, _i, _i, _i, _vp, _sz, _vp])
         _lib = h
         return _lib
 

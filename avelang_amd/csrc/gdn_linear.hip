@@ -1,0 +1,611 @@
+// Linear attention with a decay for each head, chunked form for gfx950
+// (declared in gdn_linear.h).  Per v-head, state S [K][V] in fp32:
+//     S_t = e^{g_t} S_{t-1} + k_t v_t^T        o_t = scale S_t^T q_t
+// In chunks of 64 tokens, G the chunk's prefix sums of g and R_j the sum of
+// what follows token j in it:
+//     P_ij = scale e^{G_i - G_j} (q_i . k_j)   (j <= i)
+//     o_i  = sum_j P_ij v_j + scale e^{G_i} S^T q_i
+//     S'   = e^{G_63} S + sum_j k_j (e^{R_j} v_j)^T
+// all products on bf16 MFMA with fp32 accumulation.  e^{R_j} v_j enters as the
+// sum of two bf16 parts (2^-17 relative), so the state keeps fp32's sums to
+// that; P and the state's copy that q reads are single bf16 (2^-9, the size
+// of o's own rounding).  R is summed from the chunk's end, not as G_63 - G_j:
+// its error stays in proportion to the decay it gives.
+//
+// A sequence is cut into segments of L chunks that run at the same time: one
+// launch forms every segment's own contribution to the state (from k, v and
+// g), one joins them along each sequence, one walks every segment from its
+// start state and writes o.  Where a whole sequence fits a segment the first
+// two are left out.
+#include "gdn_linear.h"
+#include "../../include/gdn_linear.h"
+
+namespace gdn {
+
+// ---------------------------------------------------------------- table ----
+// Segments of packed sequences: an entry per segment, the first segment of
+// each sequence, and the check of the cu_seqlens contract (on a violation
+// every sequence is one empty segment).
+__global__ __launch_bounds__(1024) void lin_table_kernel(const int32_t* cu, LinSeg* table,
+                                                         int32_t* soff, int32_t* status, int N,
+                                                         int total, int L, int nseg) {
+  __shared__ int wsum[2][16];
+  const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+  int bad = 0;
+  for (int n = tid; n < N; n += 1024) bad |= cu[n + 1] < cu[n];
+  if (tid == 0) bad |= cu[0] != 0 || cu[N] != total;
+  bad = __syncthreads_or(bad);
+  if (tid == 0) *status = bad;
+  int seg0 = 0, chunk0 = 0;   // of this round's first sequence
+  for (int n0 = 0; n0 < N; n0 += 1024) {
+    const int n = n0 + tid;
+    const int s = n < N && !bad ? cu[n] : 0;
+    const int len = n < N && !bad ? cu[n + 1] - s : 0;
+    const int nc = (len + kChunk - 1) / kChunk;
+    const int ns = n < N ? max(1, (nc + L - 1) / L) : 0;
+    int a = ns, b = nc;
+    for (int off = 1; off < 64; off *= 2) {
+      const int x = __shfl_up(a, off), y = __shfl_up(b, off);
+      if (lane >= off) {
+        a += x;
+        b += y;
+      }
+    }
+    __syncthreads();
+    if (lane == 63) {
+      wsum[0][wave] = a;
+      wsum[1][wave] = b;
+    }
+    __syncthreads();
+    int sa = seg0, sb = chunk0;
+    for (int w = 0; w < 16; ++w) {
+      if (w < wave) {
+        sa += wsum[0][w];
+        sb += wsum[1][w];
+      }
+      seg0 += wsum[0][w];
+      chunk0 += wsum[1][w];
+    }
+    sa += a - ns;
+    sb += b - nc;
+    if (n < N) {
+      soff[n] = sa;
+      for (int i = 0; i < ns && sa + i < nseg; ++i)
+        table[sa + i] = LinSeg{s + i * L * kChunk, min(len - i * L * kChunk, L * kChunk),
+                               sb + i * L, n, i == 0, i == ns - 1};
+    }
+  }
+  if (tid == 0) soff[N] = seg0;
+  for (int i = seg0 + tid; i < nseg; i += 1024) table[i] = LinSeg{0, 0, 0, -1, 0, 0};
+}
+
+// -------------------------------------------------------------- segments ----
+// Contribution of a segment to the state after it: sum over its chunks of
+// X^T (f Y) with x = k, y = v, f = e^R; or (REV) to the gradient of the state
+// before it, chunks last to first, x = q, y = dO, f = scale e^G.  A wave owns
+// 32 columns of Y and all rows of the state.
+template <int K, int V, bool REV>
+__global__ __launch_bounds__(2 * V, 2) void lin_segment_kernel(
+    const uint16_t* __restrict__ x, int x_row, const uint16_t* __restrict__ y, int y_row,
+    LinDecay dec, LinGrid grid, int Hqk, int Hv, float scale, float* __restrict__ segs,
+    float* __restrict__ decay) {
+  constexpr int NT = 2 * V;
+  __shared__ __align__(16) char xs[LinTile<K>::BYTES];
+  __shared__ __align__(16) char ys[LinTile<V>::BYTES];
+  __shared__ __align__(16) float fac[2][64];
+  __shared__ float tot[2];
+  const int item = xcd_item();
+  if (item >= grid.nseg * Hv) return;
+  const int sid = item / Hv, h = item % Hv, hq = h / (Hv / Hqk);
+  const LinSeg sg = lin_seg(grid, sid);
+  if (sg.seq < 0 || (REV ? sg.first : sg.last)) return;
+  const int tid = threadIdx.x, lane = tid % 64, w = tid / 64;
+  const int r16 = lane % 16, grp = lane / 16;
+  const int nc = (sg.ntok + kChunk - 1) / kChunk;
+
+  f32x4 S[K / 16][2];
+#pragma unroll
+  for (int t = 0; t < K / 16; ++t) S[t][0] = S[t][1] = zero4();
+  LinStage<K, NT> sx;
+  LinStage<V, NT> sy;
+  float gsum = 0.f;
+  auto load = [&](int c) {
+    const int n = c >= 0 && c < nc ? sg.ntok - c * kChunk : 0;
+    const size_t t = n > 0 ? (size_t)sg.tok0 + c * kChunk : 0;
+    sx.load(x + t * x_row + hq * K, x_row, min(n, 64), tid);
+    sy.load(y + t * y_row + h * V, y_row, min(n, 64), tid);
+  };
+  auto gates = [&](int c, int buf) {   // one wave
+    const int t = c * kChunk + lane;
+    const float g = c >= 0 && c < nc && t < sg.ntok ? lin_g(dec, sg.tok0 + t, h) : 0.f;
+    const float pre = wave_prefix(g, lane);
+    const float sum = __shfl(pre, 63);
+    fac[buf][lane] = REV ? scale * __expf(pre) : __expf(wave_suffix(g, lane));
+    if (lane == 0) tot[buf] = sum;
+    gsum += sum;
+  };
+  const int c0 = REV ? nc - 1 : 0, step = REV ? -1 : 1;
+  load(c0);
+  if (w == 0) gates(c0, 0);
+  for (int i = 0; i < nc; ++i) {
+    const int c = c0 + i * step, buf = i & 1;
+    sx.store(xs, tid);
+    sy.store(ys, tid);
+    __syncthreads();
+    load(c + step);
+    if (w == 0) gates(c + step, buf ^ 1);
+    const float eC = __expf(tot[buf]);
+#pragma unroll
+    for (int t = 0; t < K / 16; ++t)
+#pragma unroll
+      for (int T = 0; T < 2; ++T) S[t][T] *= eC;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const f32x4 f0 = *reinterpret_cast<const f32x4*>(&fac[buf][32 * kb + 8 * grp]);
+      const f32x4 f1 = *reinterpret_cast<const f32x4*>(&fac[buf][32 * kb + 8 * grp + 4]);
+      u16x8 hi[2], lo[2];
+#pragma unroll
+      for (int T = 0; T < 2; ++T) {
+        const u16x8 yf = LinTile<V>::cols(ys, kb, 2 * w + T, lane);
+        u16x4 h0, l0, h1, l1;
+        split_bf4(f32x4{bf2f(yf[0]), bf2f(yf[1]), bf2f(yf[2]), bf2f(yf[3])} * f0, h0, l0);
+        split_bf4(f32x4{bf2f(yf[4]), bf2f(yf[5]), bf2f(yf[6]), bf2f(yf[7])} * f1, h1, l1);
+        hi[T] = cat8(h0, h1);
+        lo[T] = cat8(l0, l1);
+      }
+#pragma unroll
+      for (int t = 0; t < K / 16; ++t) {
+        const u16x8 a = LinTile<K>::cols(xs, kb, t, lane);
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          S[t][T] = mfma16(a, hi[T], S[t][T]);
+          S[t][T] = mfma16(a, lo[T], S[t][T]);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  float* out = segs + ((size_t)sid * Hv + h) * K * V;
+#pragma unroll
+  for (int t = 0; t < K / 16; ++t)
+#pragma unroll
+    for (int T = 0; T < 2; ++T)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        out[rho_row(t, 4 * grp + r) * V + 32 * w + 8 * (r16 >> 2) + 4 * T + (r16 & 3)] =
+            S[t][T][r];
+  // (wave 0's sum covers one chunk past the last, whose decays are 0)
+  if (tid == 0) decay[(size_t)sid * Hv + h] = __expf(gsum);
+}
+
+// The states at every segment's start (REV: the gradients of the state at
+// every segment's end) in place of the contributions, from `edge` (h0 / dht,
+// nullable).  A lane per element.
+template <bool REV>
+__global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int KV,
+                                                       const float* __restrict__ edge,
+                                                       float* __restrict__ segs,
+                                                       const float* __restrict__ decay) {
+  const int per = KV / 256;
+  const int n = blockIdx.x / (Hv * per), h = blockIdx.x / per % Hv;
+  const int e = blockIdx.x % per * 256 + threadIdx.x;
+  int s0, s1;
+  if (grid.table) {
+    s0 = grid.soff[n];
+    s1 = grid.soff[n + 1];
+  } else {
+    s0 = n * grid.nps;
+    s1 = s0 + grid.nps;
+  }
+  if (s1 - s0 < 2) return;
+  float S = edge ? edge[((size_t)n * Hv + h) * KV + e] : 0.f;
+  const int first = REV ? s1 - 1 : s0, step = REV ? -1 : 1, cnt = s1 - s0 - 1;
+  constexpr int U = 8;   // loads in flight
+  for (int i = 0; i < cnt; i += U) {
+    float c[U], d[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const size_t s = first + min(i + j, cnt - 1) * step;
+      c[j] = segs[(s * Hv + h) * KV + e];
+      d[j] = decay[s * Hv + h];
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      if (i + j < cnt) {
+        const size_t s = first + (i + j) * step;
+        segs[(s * Hv + h) * KV + e] = S;
+        S = d[j] * S + c[j];
+      }
+    }
+  }
+  segs[((size_t)(REV ? s0 : s1 - 1) * Hv + h) * KV + e] = S;
+}
+
+// ------------------------------------------------------------------ walk ----
+// One segment and v-head from its start state, chunk by chunk: o (OUT), the
+// state at every chunk's start (SAVE), ht.  A wave owns 32 columns of V, all
+// of the state's rows for them in its accumulators, whose layout is that of
+// the operand with which S^T q is formed: the state never leaves the registers.
+template <int K, int V, bool OUT, bool SAVE>
+__global__ __launch_bounds__(2 * V, 2) void lin_walk_kernel(
+    const uint16_t* __restrict__ q, const uint16_t* __restrict__ k,
+    const uint16_t* __restrict__ v, TokenStride ts, LinDecay dec, LinGrid grid, int Hqk, int Hv,
+    float scale, const float* h0, float* ht, const float* __restrict__ segs,
+    uint16_t* __restrict__ o, u16x8* __restrict__ states) {
+  constexpr int NT = 2 * V, NW = V / 32;
+  __shared__ __align__(16) char qs[LinTile<K>::BYTES];
+  __shared__ __align__(16) char ks[LinTile<K>::BYTES];
+  __shared__ __align__(16) char vs[LinTile<V>::BYTES];
+  __shared__ __align__(16) char ps[LinTile<64>::BYTES];
+  __shared__ __align__(16) float sG[2][64], sQ[2][64], sK[2][64];   // G, scale e^G, e^R
+  const int tid = threadIdx.x, lane = tid % 64, w = tid / 64;
+  const int r16 = lane % 16, grp = lane / 16;
+  const int item = xcd_item();
+  if (grid.table && *grid.status) {
+    // a cu_seqlens violation: no sequence has a token, o is zero
+    if (OUT) {
+      const size_t n = (size_t)grid.total * Hv * V / 8;
+      for (size_t i = (size_t)blockIdx.x * NT + tid; i < n; i += (size_t)gridDim.x * NT)
+        reinterpret_cast<u32x4*>(o)[i] = u32x4{0, 0, 0, 0};
+    }
+  }
+  if (item >= grid.nseg * Hv) return;
+  const int sid = item / Hv, h = item % Hv, hq = h / (Hv / Hqk);
+  const LinSeg sg = lin_seg(grid, sid);
+  if (sg.seq < 0) return;
+  const int nc = (sg.ntok + kChunk - 1) / kChunk;
+  const int vcol = 32 * w + 8 * (r16 >> 2) + (r16 & 3);   // + 4 T: the state's column
+
+  f32x4 S[K / 16][2];
+  const float* src = sg.first ? (h0 ? h0 + ((size_t)sg.seq * Hv + h) * K * V : nullptr)
+                              : segs + ((size_t)sid * Hv + h) * K * V;
+#pragma unroll
+  for (int t = 0; t < K / 16; ++t)
+#pragma unroll
+    for (int T = 0; T < 2; ++T)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        S[t][T][r] = src ? src[rho_row(t, 4 * grp + r) * V + vcol + 4 * T] : 0.f;
+
+  LinStage<K, NT> sq, sk;
+  LinStage<V, NT> sv;
+  auto load = [&](int c) {
+    const int n = c < nc ? sg.ntok - c * kChunk : 0;
+    const size_t t = n > 0 ? (size_t)sg.tok0 + c * kChunk : 0;
+    if (OUT) sq.load(q + t * ts.q + hq * K, ts.q, min(n, 64), tid);
+    sk.load(k + t * ts.k + hq * K, ts.k, min(n, 64), tid);
+    sv.load(v + t * ts.v + h * V, ts.v, min(n, 64), tid);
+  };
+  auto gates = [&](int c, int buf) {   // one wave
+    const int t = c * kChunk + lane;
+    const float g = c < nc && t < sg.ntok ? lin_g(dec, sg.tok0 + t, h) : 0.f;
+    const float pre = wave_prefix(g, lane);
+    sG[buf][lane] = pre;
+    sQ[buf][lane] = scale * __expf(pre);
+    sK[buf][lane] = __expf(wave_suffix(g, lane));
+  };
+  if (OUT) {
+    // the tiles of P above the diagonal that share a 32-wide block with it
+    for (int i = tid; i < 64; i += NT) {
+      const int r = i / 2 % 16 + (i / 32) * 32, u = 4 * (i / 32) + 2 + i % 2;
+      *reinterpret_cast<u32x4*>(ps + LinTile<64>::off(r, u)) = u32x4{0, 0, 0, 0};
+    }
+  }
+  load(0);
+  if (w == 0) gates(0, 0);
+  for (int c = 0; c < nc; ++c) {
+    const int buf = c & 1;
+    if (OUT) sq.store(qs, tid);
+    sk.store(ks, tid);
+    sv.store(vs, tid);
+    __syncthreads();
+    load(c + 1);
+    if (w == 0) gates(c + 1, buf ^ 1);
+
+    if (OUT) {
+      // P, tile by tile (token block it, source block jt), as bf16 rows
+      for (int n = w; n < 10; n += NW) {
+        const int it = tmat_block_row(n), jt = n - tmat_block(it, 0);
+        f32x4 p = zero4();
+#pragma unroll
+        for (int kb = 0; kb < K / 32; ++kb)
+          p = mfma16(LinTile<K>::rows(ks, jt, kb, lane), LinTile<K>::rows(qs, it, kb, lane), p);
+        const int i = 16 * it + r16, j = 16 * jt + 4 * grp;
+        const f32x4 gj = *reinterpret_cast<const f32x4*>(&sG[buf][j]);
+        const float gi = sG[buf][i];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[r] = j + r <= i ? p[r] * (scale * __expf(gi - gj[r])) : 0.f;
+        *reinterpret_cast<u16x4*>(ps + LinTile<64>::off(i, j / 8) + (grp & 1) * 8) = f2bf4(p);
+      }
+    }
+    // the state as bf16 operands, by rows of 32 keys
+    f32x4 O[4][2];
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) O[tt][0] = O[tt][1] = zero4();
+#pragma unroll
+    for (int b = 0; b < K / 32; ++b) {
+      u16x8 sb[2];
+#pragma unroll
+      for (int T = 0; T < 2; ++T) sb[T] = cat8(f2bf4(S[2 * b][T]), f2bf4(S[2 * b + 1][T]));
+      if (OUT) {
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          const u16x8 qf = LinTile<K>::rows(qs, tt, b, lane);
+#pragma unroll
+          for (int T = 0; T < 2; ++T) O[tt][T] = mfma16(sb[T], qf, O[tt][T]);
+        }
+      }
+      if (SAVE) {
+        // transposed through a product with a selection matrix (exact): lane
+        // (r16, grp) gets key rho_row(t, r16), values 32 w + 8 grp + i
+        u16x8* dst = states + ((size_t)(sg.chunk0 + c) * Hv + h) * (K / 16) * (V / 32) * 64;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          u16x8 sel;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            sel[i] = grp == r16 >> 2 && i == 4 * e + (r16 & 3) ? 0x3F80 : 0;
+          const f32x4 a0 = mfma16(sb[0], sel, zero4()), a1 = mfma16(sb[1], sel, zero4());
+          dst[((2 * b + e) * (V / 32) + w) * 64 + lane] = cat8(f2bf4(a0), f2bf4(a1));
+        }
+      }
+    }
+    if (OUT) {
+      float eq[4];
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) eq[tt] = sQ[buf][16 * tt + r16];
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        O[tt][0] *= eq[tt];
+        O[tt][1] *= eq[tt];
+      }
+      __syncthreads();   // P
+    }
+    const float eC = __expf(sG[buf][63]);
+#pragma unroll
+    for (int t = 0; t < K / 16; ++t)
+#pragma unroll
+      for (int T = 0; T < 2; ++T) S[t][T] *= eC;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const f32x4 f0 = *reinterpret_cast<const f32x4*>(&sK[buf][32 * kb + 8 * grp]);
+      const f32x4 f1 = *reinterpret_cast<const f32x4*>(&sK[buf][32 * kb + 8 * grp + 4]);
+      u16x8 vf[2], hi[2], lo[2];
+#pragma unroll
+      for (int T = 0; T < 2; ++T) {
+        vf[T] = LinTile<V>::cols(vs, kb, 2 * w + T, lane);
+        u16x4 h0_, l0, h1, l1;
+        split_bf4(f32x4{bf2f(vf[T][0]), bf2f(vf[T][1]), bf2f(vf[T][2]), bf2f(vf[T][3])} * f0, h0_, l0);
+        split_bf4(f32x4{bf2f(vf[T][4]), bf2f(vf[T][5]), bf2f(vf[T][6]), bf2f(vf[T][7])} * f1, h1, l1);
+        hi[T] = cat8(h0_, h1);
+        lo[T] = cat8(l0, l1);
+      }
+      if (OUT) {
+#pragma unroll
+        for (int tt = 2 * kb; tt < 4; ++tt) {
+          const u16x8 pf = LinTile<64>::rows(ps, tt, kb, lane);
+#pragma unroll
+          for (int T = 0; T < 2; ++T) O[tt][T] = mfma16(vf[T], pf, O[tt][T]);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < K / 16; ++t) {
+        const u16x8 a = LinTile<K>::cols(ks, kb, t, lane);
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          S[t][T] = mfma16(a, hi[T], S[t][T]);
+          S[t][T] = mfma16(a, lo[T], S[t][T]);
+        }
+      }
+    }
+    if (OUT) {
+      const int n = sg.ntok - c * kChunk;
+      uint16_t* dst = o + ((size_t)(sg.tok0 + c * kChunk) * Hv + h) * V + 32 * w + 8 * grp;
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        const int i = 16 * tt + r16;
+        if (i < n)
+          *reinterpret_cast<u16x8*>(dst + (size_t)i * Hv * V) = cat8(f2bf4(O[tt][0]), f2bf4(O[tt][1]));
+      }
+    }
+    __syncthreads();
+  }
+  if (ht && sg.last) {
+    float* out = ht + ((size_t)sg.seq * Hv + h) * K * V;
+#pragma unroll
+    for (int t = 0; t < K / 16; ++t)
+#pragma unroll
+      for (int T = 0; T < 2; ++T)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) out[rho_row(t, 4 * grp + r) * V + vcol + 4 * T] = S[t][T][r];
+  }
+}
+
+// ------------------------------------------------------------------ host ----
+// Chunks per segment: as many as spread all chunks over two workgroups per CU
+// once, four at least.
+LinPlan lin_plan(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu, bool bwd) {
+  LinPlan p{};
+  const long long tokens = (long long)B * T;
+  const long long per = ((long long)T + kChunk - 1) / kChunk;   // chunks of the longest sequence
+  p.chunks = has_cu ? tokens / kChunk + N : B * per;
+  const long long slots = 2LL * device_cus();
+  long long L = (p.chunks * Hv + slots - 1) / slots;
+  if (L < 4) L = 4;
+  if (L > per) L = per > 0 ? per : 1;
+  p.L = (int)L;
+  p.nps = (int)(per > 0 ? (per + L - 1) / L : 1);
+  p.nseg = (int)(has_cu ? N + tokens / (L * kChunk) : (long long)N * p.nps);
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t r = at;
+    at += (bytes + 255) / 256 * 256;
+    return r;
+  };
+  if (has_cu) {
+    p.table = take((size_t)p.nseg * sizeof(LinSeg));
+    p.soff = take(((size_t)N + 1) * 4);
+    p.status = take(4);
+  }
+  if (p.nps > 1) {
+    p.segs = take((size_t)p.nseg * Hv * K * V * 4);
+    p.decay = take((size_t)p.nseg * Hv * 4);
+  }
+  if (bwd && Hv > Hqk) p.part = take((size_t)tokens * Hv * K * 8);
+  if (bwd) p.dgtok = take((size_t)tokens * Hv * 4);
+  p.total = at;
+  return p;
+}
+
+LinGrid lin_grid(const LinPlan& p, unsigned char* ws, int T, int N, int total, bool has_cu) {
+  LinGrid g{};
+  if (has_cu) {
+    g.table = reinterpret_cast<const LinSeg*>(ws + p.table);
+    g.soff = reinterpret_cast<const int32_t*>(ws + p.soff);
+    g.status = reinterpret_cast<const int32_t*>(ws + p.status);
+  }
+  g.T = T;
+  g.L = p.L;
+  g.nps = p.nps;
+  g.nseg = p.nseg;
+  g.N = N;
+  g.total = total;
+  return g;
+}
+
+void launch_lin_table(const int32_t* cu, const LinPlan& p, unsigned char* ws, int N, int total,
+                      hipStream_t st) {
+  hipLaunchKernelGGL(lin_table_kernel, dim3(1), dim3(1024), 0, st, cu,
+                     reinterpret_cast<LinSeg*>(ws + p.table),
+                     reinterpret_cast<int32_t*>(ws + p.soff),
+                     reinterpret_cast<int32_t*>(ws + p.status), N, total, p.L, p.nseg);
+}
+
+template <int K, int V>
+void launch_lin_segments(const uint16_t* x, int x_row, const uint16_t* y, int y_row,
+                         const LinDecay& d, const LinGrid& g, int Hqk, int Hv, float scale,
+                         bool reverse, const float* edge, float* segs, float* decay,
+                         hipStream_t st) {
+  const dim3 items(xcd_grid((long long)g.nseg * Hv)), elems((unsigned)(g.N * Hv * (K * V / 256)));
+  if (reverse) {
+    hipLaunchKernelGGL((lin_segment_kernel<K, V, true>), items, dim3(2 * V), 0, st, x, x_row, y,
+                       y_row, d, g, Hqk, Hv, scale, segs, decay);
+    hipLaunchKernelGGL(lin_join_kernel<true>, elems, dim3(256), 0, st, g, Hv, K * V, edge, segs, decay);
+  } else {
+    hipLaunchKernelGGL((lin_segment_kernel<K, V, false>), items, dim3(2 * V), 0, st, x, x_row, y,
+                       y_row, d, g, Hqk, Hv, scale, segs, decay);
+    hipLaunchKernelGGL(lin_join_kernel<false>, elems, dim3(256), 0, st, g, Hv, K * V, edge, segs, decay);
+  }
+}
+#define GDN_LS(KK, VV)                                                                        \
+  template void launch_lin_segments<KK, VV>(const uint16_t*, int, const uint16_t*, int,       \
+                                            const LinDecay&, const LinGrid&, int, int, float, \
+                                            bool, const float*, float*, float*, hipStream_t);
+GDN_LS(128, 128) GDN_LS(128, 64) GDN_LS(64, 128) GDN_LS(64, 64)
+#undef GDN_LS
+
+namespace {
+template <int K, int V>
+void launch_walk(const uint16_t* q, const uint16_t* k, const uint16_t* v, TokenStride ts,
+                 const LinDecay& d, const LinGrid& g, int Hqk, int Hv, float scale,
+                 const float* h0, float* ht, float* segs, float* decay, uint16_t* o, u16x8* states,
+                 hipStream_t st) {
+  if (g.nps > 1)
+    launch_lin_segments<K, V>(k, ts.k, v, ts.v, d, g, Hqk, Hv, 1.f, false, h0, segs, decay, st);
+  const dim3 items(xcd_grid((long long)g.nseg * Hv));
+#define GDN_LW(OUT, SAVE)                                                                      \
+  hipLaunchKernelGGL((lin_walk_kernel<K, V, OUT, SAVE>), items, dim3(2 * V), 0, st, q, k, v, ts, \
+                     d, g, Hqk, Hv, scale, h0, ht, segs, o, states)
+  if (o && states) GDN_LW(true, true);
+  else if (o) GDN_LW(true, false);
+  else GDN_LW(false, true);
+#undef GDN_LW
+}
+}  // namespace
+
+}  // namespace gdn
+
+namespace gdn_host {
+int validate_common(const void* q, const void* k, const void* v, const float* g, const float* beta,
+                    const float* h0, const float* ht, const void* o, const int32_t* cu, int B,
+                    int T, int Hqk, int Hv, int K, int V, int N);
+int validate_rows(const char* name, const void* q, const void* k, const void* v, long long q_row,
+                  long long k_row, long long v_row, const void* o, long long tokens, int Hqk,
+                  int Hv, int K, int V, gdn::TokenStride& ts);
+
+int lin_validate(const char* name, const void* q, const void* k, const void* v, long long q_row,
+                 long long k_row, long long v_row, const void* g, int g_dtype, const float* h0,
+                 const float* ht, const void* o, const int32_t* cu, int B, int T, int Hqk, int Hv,
+                 int K, int V, int N, gdn::TokenStride& ts) {
+  const float* gf = static_cast<const float*>(g);
+  int rc = validate_common(q, k, v, gf, gf, h0, ht, o, cu, B, T, Hqk, Hv, K, V, N);
+  if (rc) return rc;
+  if (!gdn::dtype_ok(g_dtype)) return fail(GDN_ERR_SHAPE, std::string(name) + ": unsupported dtype code");
+  // (tokens, segments x heads and join workgroups are counted in 32 bits)
+  const long long tokens = (long long)B * T;
+  if (tokens >= (1LL << 31) - 64 || (tokens / 64 + N) * (long long)Hv >= (1LL << 24) * 64 ||
+      (long long)N * Hv * (K * V / 256) >= (1LL << 31))
+    return fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
+  if (tokens > 0)
+    return validate_rows(name, q, k, v, q_row, k_row, v_row, o, tokens, Hqk, Hv, K, V, ts);
+  ts = gdn::TokenStride{Hqk * K, Hqk * K, Hv * V};
+  return GDN_OK;
+}
+bool lin_sizes_ok(int B, int T, int Hqk, int Hv, int K, int V, int N) {
+  return B >= 0 && T >= 0 && Hqk > 0 && Hv > 0 && Hv % Hqk == 0 && N >= 0 &&
+         (K == 64 || K == 128) && (V == 64 || V == 128);
+}
+}  // namespace gdn_host
+
+extern "C" size_t gdn_linear_chunk_workspace_bytes(int B, int T, int Hqk, int Hv, int K, int V,
+                                                   int N, int has_cu_seqlens) {
+  if (!gdn_host::lin_sizes_ok(B, T, Hqk, Hv, K, V, N)) return 0;
+  return gdn::lin_plan(B, T, Hqk, Hv, K, V, N, has_cu_seqlens != 0, false).total;
+}
+
+extern "C" size_t gdn_linear_states_bytes(int B, int T, int Hv, int K, int V, int N,
+                                          int has_cu_seqlens) {
+  if (!gdn_host::lin_sizes_ok(B, T, Hv, Hv, K, V, N)) return 0;
+  return (size_t)gdn::lin_plan(B, T, Hv, Hv, K, V, N, has_cu_seqlens != 0, false).chunks * Hv * K *
+         V * 2;
+}
+
+extern "C" int gdn_linear_chunk_fwd(const void* q, const void* k, const void* v, long long q_row,
+                                    long long k_row, long long v_row, const void* g, int g_dtype,
+                                    int g_per_head, const float* h0, float* ht, void* o,
+                                    const int32_t* cu_seqlens, int B, int T, int Hqk, int Hv,
+                                    int K, int V, int N, float scale, void* states,
+                                    void* workspace, size_t workspace_bytes, void* stream) {
+  const char* name = "gdn_linear_chunk_fwd";
+  gdn::TokenStride ts;
+  // (without o the checks that name it take q's address: nothing is written there)
+  int rc = gdn_host::lin_validate(name, q, k, v, q_row, k_row, v_row, g, g_dtype, h0, ht,
+                                  o ? o : states, cu_seqlens, B, T, Hqk, Hv, K, V, N, ts);
+  if (rc) return rc;
+  const bool has_cu = cu_seqlens != nullptr;
+  const gdn::LinPlan p = gdn::lin_plan(B, T, Hqk, Hv, K, V, N, has_cu, false);
+  if (p.total > 0 && (!workspace || workspace_bytes < p.total))
+    return gdn_host::fail(GDN_ERR_WORKSPACE, std::string(name) + ": workspace needs " +
+                                                 std::to_string(p.total) + " bytes, got " +
+                                                 std::to_string(workspace_bytes));
+  if (N == 0 || ((long long)B * T == 0 && !ht)) return GDN_OK;
+  gdn_host::launch_begin();
+  auto st = static_cast<hipStream_t>(stream);
+  auto* ws = static_cast<unsigned char*>(workspace);
+  const gdn::LinGrid grid = gdn::lin_grid(p, ws, T, N, B * T, has_cu);
+  if (has_cu) gdn::launch_lin_table(cu_seqlens, p, ws, N, B * T, st);
+  const gdn::LinDecay d{g, g_dtype, g_per_head ? 0 : Hv};
+  auto* segs = reinterpret_cast<float*>(ws + p.segs);
+  auto* decay = reinterpret_cast<float*>(ws + p.decay);
+#define GDN_LIN(KK, VV)                                                                        \
+  if (K == KK && V == VV) {                                                                    \
+    gdn::launch_walk<KK, VV>(static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), \
+                             static_cast<const uint16_t*>(v), ts, d, grid, Hqk, Hv, scale, h0, \
+                             ht, segs, decay, static_cast<uint16_t*>(o),                       \
+                             static_cast<gdn::u16x8*>(states), st);                            \
+    return gdn_host::check_launch(name);                                                       \
+  }
+  GDN_LIN(128, 128) GDN_LIN(128, 64) GDN_LIN(64, 128) GDN_LIN(64, 64)
+#undef GDN_LIN
+  return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": unsupported K/V");
+}

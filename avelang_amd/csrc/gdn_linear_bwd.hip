@@ -1,0 +1,511 @@
+// Backward of linear attention's chunked form for gfx950 (declared in
+// gdn_linear.h).  With S the state at a chunk's start (saved by the forward),
+// D the gradient of the state at its end, G and R as in the forward and
+// gamma_ij = scale e^{G_i - G_j} (j <= i):
+//     P_ij = gamma_ij (q_i . k_j)      dP_ij = gamma_ij (do_i . v_j)
+//     dv_j = sum_i P_ij do_i + e^{R_j} D^T k_j
+//     dk_j = sum_i dP_ij q_i + e^{R_j} D v_j
+//     dq_i = sum_j dP_ij k_j + scale e^{G_i} S do_i
+//     D'   = e^{G_63} D + sum_i q_i (scale e^{G_i} do_i)^T
+// and, from the parts a_i = q_i . (S's part of dq_i), b_j = k_j . (D's part of
+// dk_j), M_ij = P_ij (do_i . v_j),
+//     dg_t = e^{G_63} <S, D> + sum_{i >= t} a_i + sum_{j < t} b_j
+//            + sum_{i >= t > j} M_ij,
+// the last as row sums less column sums of the same fp32 numbers, so nothing
+// but their own rounding is lost where it cancels: dg of a head whose memory
+// is short is as good as that of a long one.
+//
+// Segments as in the forward, walked last chunk to first: a launch for every
+// segment's contribution to D, one that joins them, one for the gradients.
+#include "gdn_linear.h"
+#include "../../include/gdn_linear.h"
+
+namespace gdn {
+
+struct LinBwdArgs {
+  const uint16_t *q, *k, *v, *dO;
+  TokenStride ts;
+  LinDecay dec;
+  LinGrid grid;
+  int Hqk, Hv;
+  float scale;
+  const float* dht;
+  float* dh0;
+  const float* segs;
+  const u16x8* states;
+  uint16_t *dq, *dk, *dv;
+  float *pq, *pk;      // [tokens][Hv][K] partial dq, dk (NULL: one v-head per qk-head)
+  float* dg;           // [tokens][Hv]
+};
+
+// A workgroup walks one segment of one v-head.  V / 32 waves own 32 columns
+// of D each (dv and dh0), K / 32 waves 32 columns of D^T (dk and dq, which
+// reduce over V, and with the saved states' fragments <S, D>): D is kept in
+// both orientations so that neither ever leaves the registers.
+template <int K, int V>
+__global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) {
+  constexpr int NT = 2 * (K + V), NV = V / 32, NK = K / 32, NW = NV + NK;
+  __shared__ __align__(16) char qs[LinTile<K>::BYTES];
+  __shared__ __align__(16) char ks[LinTile<K>::BYTES];
+  __shared__ __align__(16) char vs[LinTile<V>::BYTES];
+  __shared__ __align__(16) char os[LinTile<V>::BYTES];
+  __shared__ __align__(16) char ps[LinTile<64>::BYTES];
+  __shared__ __align__(16) char dps[LinTile<64>::BYTES];
+  __shared__ __align__(16) float sG[2][64], sQ[2][64], sK[2][64];
+  __shared__ __align__(16) float rowM[4][64], colM[4][64], asum[NK][64], bsum[NK][64];
+  __shared__ float csum[NK];
+  const int tid = threadIdx.x, lane = tid % 64, w = tid / 64;
+  const int r16 = lane % 16, grp = lane / 16;
+  const int item = xcd_item();
+  if (a.grid.table && *a.grid.status) {
+    // a cu_seqlens violation: every gradient over the tokens is zero
+    const size_t nv = (size_t)a.grid.total * a.Hv * V / 8, nk = (size_t)a.grid.total * a.Hqk * K / 8;
+    const size_t ng = (size_t)a.grid.total * a.Hv, st = (size_t)gridDim.x * NT;
+    const size_t i0 = (size_t)blockIdx.x * NT + tid;
+    for (size_t i = i0; i < nv; i += st) reinterpret_cast<u32x4*>(a.dv)[i] = u32x4{0, 0, 0, 0};
+    for (size_t i = i0; i < nk; i += st) {
+      reinterpret_cast<u32x4*>(a.dq)[i] = u32x4{0, 0, 0, 0};
+      reinterpret_cast<u32x4*>(a.dk)[i] = u32x4{0, 0, 0, 0};
+    }
+    for (size_t i = i0; i < ng; i += st) a.dg[i] = 0.f;
+  }
+  if (item >= a.grid.nseg * a.Hv) return;
+  const int sid = item / a.Hv, h = item % a.Hv, hq = h / (a.Hv / a.Hqk);
+  const LinSeg sg = lin_seg(a.grid, sid);
+  if (sg.seq < 0) return;
+  const int nc = (sg.ntok + kChunk - 1) / kChunk;
+  const bool vwave = w < NV;
+  const int wk = vwave ? 0 : w - NV, wv = vwave ? w : 0;
+
+  // ST[t][T]: V waves D (key tile t, value tile T); key waves D^T (value tile t, key tile T)
+  constexpr int NTILE = (K > V ? K : V) / 16;
+  f32x4 ST[NTILE][2];
+  const float* src = sg.last ? (a.dht ? a.dht + ((size_t)sg.seq * a.Hv + h) * K * V : nullptr)
+                             : a.segs + ((size_t)sid * a.Hv + h) * K * V;
+  const int c32 = 8 * (r16 >> 2) + (r16 & 3);   // + 4 T: the lane's column of 32
+#pragma unroll
+  for (int t = 0; t < NTILE; ++t)
+#pragma unroll
+    for (int T = 0; T < 2; ++T)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int row = rho_row(t, 4 * grp + r), col = c32 + 4 * T;
+        float x = 0.f;
+        if (src) {
+          if (vwave && t < K / 16) x = src[row * V + 32 * wv + col];
+          if (!vwave && t < V / 16) x = src[(32 * wk + col) * V + row];
+        }
+        ST[t][T][r] = x;
+      }
+
+  LinStage<K, NT> sq, sk;
+  LinStage<V, NT> sv, so;
+  auto load = [&](int c) {
+    const int n = c >= 0 ? sg.ntok - c * kChunk : 0;
+    const size_t t = n > 0 ? (size_t)sg.tok0 + c * kChunk : 0;
+    sq.load(a.q + t * a.ts.q + hq * K, a.ts.q, min(n, 64), tid);
+    sk.load(a.k + t * a.ts.k + hq * K, a.ts.k, min(n, 64), tid);
+    sv.load(a.v + t * a.ts.v + h * V, a.ts.v, min(n, 64), tid);
+    so.load(a.dO + (t * a.Hv + h) * V, a.Hv * V, min(n, 64), tid);
+  };
+  auto gates = [&](int c, int buf) {   // one wave
+    const int t = c * kChunk + lane;
+    const float g = c >= 0 && t < sg.ntok ? lin_g(a.dec, sg.tok0 + t, h) : 0.f;
+    const float pre = wave_prefix(g, lane);
+    sG[buf][lane] = pre;
+    sQ[buf][lane] = a.scale * __expf(pre);
+    sK[buf][lane] = __expf(wave_suffix(g, lane));
+  };
+  // the tiles above the diagonal that share a 32-wide block with it, and the
+  // sums that no tile writes
+  for (int i = tid; i < 64; i += NT) {
+    const int r = i / 2 % 16 + (i / 32) * 32, u = 4 * (i / 32) + 2 + i % 2;
+    *reinterpret_cast<u32x4*>(ps + LinTile<64>::off(r, u)) = u32x4{0, 0, 0, 0};
+    *reinterpret_cast<u32x4*>(dps + LinTile<64>::off(r, u)) = u32x4{0, 0, 0, 0};
+  }
+  for (int i = tid; i < 256; i += NT) rowM[i / 64][i % 64] = colM[i / 64][i % 64] = 0.f;
+  __syncthreads();
+  load(nc - 1);
+  if (w == 0 && nc > 0) gates(nc - 1, 0);
+  for (int it_ = 0; it_ < nc; ++it_) {
+    const int c = nc - 1 - it_, buf = it_ & 1;
+    const int n = sg.ntok - c * kChunk;
+    const size_t tok = (size_t)sg.tok0 + c * kChunk;
+    sq.store(qs, tid);
+    sk.store(ks, tid);
+    sv.store(vs, tid);
+    so.store(os, tid);
+    __syncthreads();
+    load(c - 1);
+    if (w == 0) gates(c - 1, buf ^ 1);
+
+    // P and dP, tile by tile, as bf16 rows, and the sums of M
+    for (int m = w; m < 10; m += NW) {
+      const int it = tmat_block_row(m), jt = m - tmat_block(it, 0);
+      f32x4 p = zero4(), d = zero4();
+#pragma unroll
+      for (int kb = 0; kb < K / 32; ++kb)
+        p = mfma16(LinTile<K>::rows(ks, jt, kb, lane), LinTile<K>::rows(qs, it, kb, lane), p);
+#pragma unroll
+      for (int kb = 0; kb < V / 32; ++kb)
+        d = mfma16(LinTile<V>::rows(vs, jt, kb, lane), LinTile<V>::rows(os, it, kb, lane), d);
+      const int i = 16 * it + r16, j = 16 * jt + 4 * grp;
+      const f32x4 gj = *reinterpret_cast<const f32x4*>(&sG[buf][j]);
+      const float gi = sG[buf][i];
+      f32x4 M;
+      float rs = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float gam = a.scale * __expf(gi - gj[r]);
+        const bool in = j + r <= i;
+        p[r] = in ? p[r] * gam : 0.f;
+        M[r] = in ? p[r] * d[r] : 0.f;
+        d[r] = in ? d[r] * gam : 0.f;
+        rs += M[r];
+      }
+      *reinterpret_cast<u16x4*>(ps + LinTile<64>::off(i, j / 8) + (grp & 1) * 8) = f2bf4(p);
+      *reinterpret_cast<u16x4*>(dps + LinTile<64>::off(i, j / 8) + (grp & 1) * 8) = f2bf4(d);
+      rs += __shfl_xor(rs, 16);
+      rs += __shfl_xor(rs, 32);
+      if (grp == 0) rowM[jt][i] = rs;
+#pragma unroll
+      for (int o = 1; o < 16; o *= 2)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) M[r] += __shfl_xor(M[r], o);
+      if (r16 == 0) *reinterpret_cast<f32x4*>(&colM[it][j]) = M;
+    }
+
+    f32x4 X[4][2], Y[4][2];   // dv; or dk and dq (by token tile)
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) X[tt][0] = X[tt][1] = Y[tt][0] = Y[tt][1] = zero4();
+    const float eC = __expf(sG[buf][63]);
+    if (vwave) {
+#pragma unroll
+      for (int b = 0; b < K / 32; ++b) {
+        u16x8 df[2];
+#pragma unroll
+        for (int T = 0; T < 2; ++T) df[T] = cat8(f2bf4(ST[2 * b][T]), f2bf4(ST[2 * b + 1][T]));
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          const u16x8 kf = LinTile<K>::rows(ks, tt, b, lane);
+#pragma unroll
+          for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(df[T], kf, X[tt][T]);
+        }
+      }
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        const float f = sK[buf][16 * tt + r16];
+        X[tt][0] *= f;
+        X[tt][1] *= f;
+      }
+    } else {
+      const u16x8* sp = a.states + (((size_t)(sg.chunk0 + c) * a.Hv + h) * (K / 16) + 2 * wk) *
+                                       (V / 32) * 64 + lane;
+      float cs = 0.f;
+#pragma unroll
+      for (int b = 0; b < V / 32; ++b) {
+        u16x8 df[2], sf[2];
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          sf[T] = sp[(T * (V / 32) + b) * 64];
+          df[T] = cat8(f2bf4(ST[2 * b][T]), f2bf4(ST[2 * b + 1][T]));
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            cs += bf2f(sf[T][r]) * ST[2 * b][T][r] + bf2f(sf[T][4 + r]) * ST[2 * b + 1][T][r];
+        }
+#pragma unroll
+        for (int tt = 0; tt < 4; ++tt) {
+          const u16x8 vf = LinTile<V>::rows(vs, tt, b, lane), of = LinTile<V>::rows(os, tt, b, lane);
+#pragma unroll
+          for (int T = 0; T < 2; ++T) {
+            X[tt][T] = mfma16(df[T], vf, X[tt][T]);
+            Y[tt][T] = mfma16(sf[T], of, Y[tt][T]);
+          }
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < 64; o *= 2) cs += __shfl_xor(cs, o);
+      if (lane == 0) csum[wk] = cs;
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        const int i = 16 * tt + r16;
+        const float fk = sK[buf][i], fq = sQ[buf][i];
+        const u16x8 kr = *reinterpret_cast<const u16x8*>(ks + LinTile<K>::off(i, 4 * wk + grp));
+        const u16x8 qr = *reinterpret_cast<const u16x8*>(qs + LinTile<K>::off(i, 4 * wk + grp));
+        float sa = 0.f, sb = 0.f;
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          X[tt][T] *= fk;
+          Y[tt][T] *= fq;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            sb += bf2f(kr[4 * T + r]) * X[tt][T][r];
+            sa += bf2f(qr[4 * T + r]) * Y[tt][T][r];
+          }
+        }
+        sa += __shfl_xor(sa, 16);
+        sb += __shfl_xor(sb, 16);
+        sa += __shfl_xor(sa, 32);
+        sb += __shfl_xor(sb, 32);
+        if (grp == 0) {
+          asum[wk][i] = sa;
+          bsum[wk][i] = sb;
+        }
+      }
+    }
+    __syncthreads();   // P, dP and the sums
+
+    if (w == 0) {
+      float x = 0.f, y = 0.f, cs = 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x += rowM[u][lane] - colM[u][lane];
+#pragma unroll
+      for (int u = 0; u < NK; ++u) {
+        x += asum[u][lane];
+        y += bsum[u][lane];
+        cs += csum[u];
+      }
+      const float dg = eC * cs + x + wave_suffix(x, lane) + (wave_prefix(y, lane) - y);
+      if (lane < n) a.dg[(tok + lane) * a.Hv + h] = dg;
+    }
+#pragma unroll
+    for (int t = 0; t < NTILE; ++t) {
+      ST[t][0] *= eC;
+      ST[t][1] *= eC;
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      const f32x4 f0 = *reinterpret_cast<const f32x4*>(&sQ[buf][32 * kb + 8 * grp]);
+      const f32x4 f1 = *reinterpret_cast<const f32x4*>(&sQ[buf][32 * kb + 8 * grp + 4]);
+      auto split = [&](u16x8 y, u16x8& hi, u16x8& lo) {
+        u16x4 h0, l0, h1, l1;
+        split_bf4(f32x4{bf2f(y[0]), bf2f(y[1]), bf2f(y[2]), bf2f(y[3])} * f0, h0, l0);
+        split_bf4(f32x4{bf2f(y[4]), bf2f(y[5]), bf2f(y[6]), bf2f(y[7])} * f1, h1, l1);
+        hi = cat8(h0, h1);
+        lo = cat8(l0, l1);
+      };
+      u16x8 yf[2], hi[2], lo[2];
+      if (vwave) {
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          yf[T] = LinTile<V>::cols(os, kb, 2 * wv + T, lane);
+          split(yf[T], hi[T], lo[T]);
+        }
+#pragma unroll
+        for (int tt = 0; tt < 2 * kb + 2; ++tt) {
+          const u16x8 pf = LinTile<64>::cols16(ps, kb, tt, lane);
+#pragma unroll
+          for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(yf[T], pf, X[tt][T]);
+        }
+#pragma unroll
+        for (int t = 0; t < K / 16; ++t) {
+          const u16x8 f = LinTile<K>::cols(qs, kb, t, lane);
+#pragma unroll
+          for (int T = 0; T < 2; ++T) {
+            ST[t][T] = mfma16(f, hi[T], ST[t][T]);
+            ST[t][T] = mfma16(f, lo[T], ST[t][T]);
+          }
+        }
+      } else {
+        u16x8 kf[2];
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          yf[T] = LinTile<K>::cols(qs, kb, 2 * wk + T, lane);
+          kf[T] = LinTile<K>::cols(ks, kb, 2 * wk + T, lane);
+          split(yf[T], hi[T], lo[T]);
+        }
+#pragma unroll
+        for (int tt = 0; tt < 2 * kb + 2; ++tt) {
+          const u16x8 pf = LinTile<64>::cols16(dps, kb, tt, lane);
+#pragma unroll
+          for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(yf[T], pf, X[tt][T]);
+        }
+#pragma unroll
+        for (int tt = 2 * kb; tt < 4; ++tt) {
+          const u16x8 pf = LinTile<64>::rows(dps, tt, kb, lane);
+#pragma unroll
+          for (int T = 0; T < 2; ++T) Y[tt][T] = mfma16(kf[T], pf, Y[tt][T]);
+        }
+#pragma unroll
+        for (int t = 0; t < V / 16; ++t) {
+          const u16x8 f = LinTile<V>::cols(os, kb, t, lane);
+#pragma unroll
+          for (int T = 0; T < 2; ++T) {
+            ST[t][T] = mfma16(f, hi[T], ST[t][T]);
+            ST[t][T] = mfma16(f, lo[T], ST[t][T]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) {
+      const int i = 16 * tt + r16;
+      if (i >= n) continue;
+      const size_t th = (tok + i) * a.Hv + h;
+      if (vwave) {
+        *reinterpret_cast<u16x8*>(a.dv + th * V + 32 * wv + 8 * grp) =
+            cat8(f2bf4(X[tt][0]), f2bf4(X[tt][1]));
+      } else if (a.pq) {
+        f32x4* pq = reinterpret_cast<f32x4*>(a.pq + th * K + 32 * wk + 8 * grp);
+        f32x4* pk = reinterpret_cast<f32x4*>(a.pk + th * K + 32 * wk + 8 * grp);
+        pq[0] = Y[tt][0];
+        pq[1] = Y[tt][1];
+        pk[0] = X[tt][0];
+        pk[1] = X[tt][1];
+      } else {
+        *reinterpret_cast<u16x8*>(a.dq + th * K + 32 * wk + 8 * grp) =
+            cat8(f2bf4(Y[tt][0]), f2bf4(Y[tt][1]));
+        *reinterpret_cast<u16x8*>(a.dk + th * K + 32 * wk + 8 * grp) =
+            cat8(f2bf4(X[tt][0]), f2bf4(X[tt][1]));
+      }
+    }
+    __syncthreads();
+  }
+  if (a.dh0 && sg.first && vwave) {
+    float* out = a.dh0 + ((size_t)sg.seq * a.Hv + h) * K * V;
+#pragma unroll
+    for (int t = 0; t < K / 16; ++t)
+#pragma unroll
+      for (int T = 0; T < 2; ++T)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          out[rho_row(t, 4 * grp + r) * V + 32 * wv + c32 + 4 * T] = ST[t][T][r];
+  }
+}
+
+// dq, dk of a qk-head: the sum of its v-heads' parts, 8 elements per lane.
+__global__ __launch_bounds__(256) void lin_group_sum_kernel(const float* __restrict__ pq,
+                                                            const float* __restrict__ pk,
+                                                            uint16_t* __restrict__ dq,
+                                                            uint16_t* __restrict__ dk,
+                                                            const int32_t* status, long long rows,
+                                                            int rep, int K) {
+  const long long u = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (u * 8 >= rows * K) return;
+  const long long row = u * 8 / K;
+  const int c = u * 8 % K;
+  const float* p = blockIdx.y ? pk : pq;
+  f32x4 s0 = zero4(), s1 = zero4();
+  if (!status || !*status) {
+    for (int r = 0; r < rep; ++r) {
+      const f32x4* x = reinterpret_cast<const f32x4*>(p + (row * rep + r) * K + c);
+      s0 += x[0];
+      s1 += x[1];
+    }
+  }
+  *reinterpret_cast<u16x8*>((blockIdx.y ? dk : dq) + u * 8) = cat8(f2bf4(s0), f2bf4(s1));
+}
+
+// One decay per head: its gradient, the sum over all tokens (a workgroup per
+// head, a fixed order).
+__global__ __launch_bounds__(1024) void lin_head_sum_kernel(const float* __restrict__ x,
+                                                            float* __restrict__ out, int tokens,
+                                                            int Hv) {
+  __shared__ float red[16];
+  float s = 0.f;
+#pragma unroll 4
+  for (int t = threadIdx.x; t < tokens; t += 1024) s += x[(size_t)t * Hv + blockIdx.x];
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) s += __shfl_xor(s, o);
+  if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int i = 1; i < 16; ++i) s += red[i];
+    out[blockIdx.x] = s;
+  }
+}
+
+namespace {
+template <int K, int V>
+void launch_grad(const LinBwdArgs& a, float* segs, float* decay, hipStream_t st) {
+  if (a.grid.nps > 1)
+    launch_lin_segments<K, V>(a.q, a.ts.q, a.dO, a.Hv * V, a.dec, a.grid, a.Hqk, a.Hv, a.scale,
+                              true, a.dht, segs, decay, st);
+  hipLaunchKernelGGL((lin_grad_kernel<K, V>), dim3(xcd_grid((long long)a.grid.nseg * a.Hv)),
+                     dim3(2 * (K + V)), 0, st, a);
+}
+}  // namespace
+
+}  // namespace gdn
+
+namespace gdn_host {
+int lin_validate(const char* name, const void* q, const void* k, const void* v, long long q_row,
+                 long long k_row, long long v_row, const void* g, int g_dtype, const float* h0,
+                 const float* ht, const void* o, const int32_t* cu, int B, int T, int Hqk, int Hv,
+                 int K, int V, int N, gdn::TokenStride& ts);
+bool lin_sizes_ok(int B, int T, int Hqk, int Hv, int K, int V, int N);
+}  // namespace gdn_host
+
+extern "C" size_t gdn_linear_chunk_bwd_workspace_bytes(int B, int T, int Hqk, int Hv, int K, int V,
+                                                       int N, int has_cu_seqlens) {
+  if (!gdn_host::lin_sizes_ok(B, T, Hqk, Hv, K, V, N)) return 0;
+  return gdn::lin_plan(B, T, Hqk, Hv, K, V, N, has_cu_seqlens != 0, true).total;
+}
+
+extern "C" int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v, long long q_row,
+                                    long long k_row, long long v_row, const void* g, int g_dtype,
+                                    int g_per_head, const void* dO, const float* dht,
+                                    const void* states, void* dq, void* dk, void* dv, float* dg,
+                                    float* dh0, const int32_t* cu_seqlens, int B, int T, int Hqk,
+                                    int Hv, int K, int V, int N, float scale, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  const char* name = "gdn_linear_chunk_bwd";
+  gdn::TokenStride ts;
+  int rc = gdn_host::lin_validate(name, q, k, v, q_row, k_row, v_row, g, g_dtype, dht, dh0, dv,
+                                  cu_seqlens, B, T, Hqk, Hv, K, V, N, ts);
+  if (rc) return rc;
+  const long long tokens = (long long)B * T;
+  if ((tokens > 0 && (!dO || !states || !dq || !dk)) || ((tokens > 0 || g_per_head) && !dg))
+    return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": dO, states, dq, dk and dg must be non-NULL");
+  const bool has_cu = cu_seqlens != nullptr;
+  const gdn::LinPlan p = gdn::lin_plan(B, T, Hqk, Hv, K, V, N, has_cu, true);
+  if (p.total > 0 && (!workspace || workspace_bytes < p.total))
+    return gdn_host::fail(GDN_ERR_WORKSPACE, std::string(name) + ": workspace needs " +
+                                                 std::to_string(p.total) + " bytes, got " +
+                                                 std::to_string(workspace_bytes));
+  gdn_host::launch_begin();
+  auto st = static_cast<hipStream_t>(stream);
+  auto* ws = static_cast<unsigned char*>(workspace);
+  float* dgt = g_per_head ? reinterpret_cast<float*>(ws + p.dgtok) : dg;
+  if (N > 0 && (tokens > 0 || dh0)) {
+    const gdn::LinGrid grid = gdn::lin_grid(p, ws, T, N, B * T, has_cu);
+    if (has_cu) gdn::launch_lin_table(cu_seqlens, p, ws, N, B * T, st);
+    gdn::LinBwdArgs a{};
+    a.q = static_cast<const uint16_t*>(q);
+    a.k = static_cast<const uint16_t*>(k);
+    a.v = static_cast<const uint16_t*>(v);
+    a.dO = static_cast<const uint16_t*>(dO);
+    a.ts = ts;
+    a.dec = gdn::LinDecay{g, g_dtype, g_per_head ? 0 : Hv};
+    a.grid = grid;
+    a.Hqk = Hqk;
+    a.Hv = Hv;
+    a.scale = scale;
+    a.dht = dht;
+    a.dh0 = dh0;
+    a.states = static_cast<const gdn::u16x8*>(states);
+    a.dq = static_cast<uint16_t*>(dq);
+    a.dk = static_cast<uint16_t*>(dk);
+    a.dv = static_cast<uint16_t*>(dv);
+    a.dg = dgt;
+    if (Hv > Hqk) {
+      a.pq = reinterpret_cast<float*>(ws + p.part);
+      a.pk = a.pq + tokens * Hv * K;
+    }
+    float* segs = reinterpret_cast<float*>(ws + p.segs);
+    float* decay = reinterpret_cast<float*>(ws + p.decay);
+    a.segs = segs;
+    if (K == 128 && V == 128) gdn::launch_grad<128, 128>(a, segs, decay, st);
+    else if (K == 128) gdn::launch_grad<128, 64>(a, segs, decay, st);
+    else if (V == 128) gdn::launch_grad<64, 128>(a, segs, decay, st);
+    else gdn::launch_grad<64, 64>(a, segs, decay, st);
+    if (a.pq && tokens > 0)
+      hipLaunchKernelGGL(gdn::lin_group_sum_kernel,
+                         dim3((unsigned)((tokens * Hqk * K / 8 + 255) / 256), 2), dim3(256), 0, st,
+                         a.pq, a.pk, a.dq, a.dk, grid.status, tokens * Hqk, Hv / Hqk, K);
+  }
+  if (g_per_head)
+    hipLaunchKernelGGL(gdn::lin_head_sum_kernel, dim3(Hv), dim3(1024), 0, st, dgt, dg, (int)tokens, Hv);
+  return gdn_host::check_launch(name);
+}
