@@ -45,9 +45,9 @@ struct LinDecay {
 };
 // A decay under e^-150 is e^-150: both are 0 in fp32, and -inf (a reset) stays
 // out of the differences of prefix sums.
+__device__ __forceinline__ float lin_clamp(float x) { return x < -150.f ? -150.f : x; }
 __device__ __forceinline__ float lin_g(const LinDecay& d, long long tok, int h) {
-  const float x = ldp(d.g, tok * d.per_token + h, d.dt);
-  return x < -150.f ? -150.f : x;
+  return lin_clamp(ldp(d.g, tok * d.per_token + h, d.dt));
 }
 
 // A [64][D] bf16 tile in LDS: rows of 2 D bytes, their 16-byte units permuted
@@ -62,37 +62,47 @@ struct LinTile {
     return D == 128 ? (((r & 3) << 2) | ((r >> 2) & 3)) : ((((r >> 1) & 1) << 2) | ((r >> 2) & 3));
   }
   __device__ static constexpr int off(int r, int u) { return r * RS + 16 * (u ^ swz(r)); }
+  // Fragment reads.  Each takes a lane's byte base within a tile; what is left
+  // is a constant per call, in the instruction or one XOR (a kernel hides the
+  // bases from the compiler once per chunk, or it would keep every XORed copy
+  // in a register of its own).
+  //
   // Operand fragment of 16 rows and 32 columns: lane (r16, grp) holds
   // X[16 tt + r16][32 kb + 8 grp + i].
-  static __device__ __forceinline__ u16x8 rows(const char* p, int tt, int kb, int lane) {
+  static __device__ __forceinline__ int row_base(int lane) {
     const int r16 = lane % 16, grp = lane / 16;
-    const int base = r16 * RS + 16 * (grp ^ swz(r16));
-    return *reinterpret_cast<const u16x8*>(p + ((base ^ (kb * 64)) + tt * 16 * RS));
+    return r16 * RS + 16 * (grp ^ swz(r16));
+  }
+  static __device__ __forceinline__ u16x8 rows(const char* p, int base, int tt, int kb) {
+    return *reinterpret_cast<const u16x8*>(p + (base ^ (kb * 64)) + tt * 16 * RS);
   }
   // Operand fragment of X^T: 16 columns and 32 rows, lane (r16, grp) holds
   // X[32 kb + 8 grp + i][c], c = rho_row of tile T: 32 (T / 2) + 8 (r16 / 4) +
   // 4 (T % 2) + r16 % 4.  Two tiles' accumulator rows then hold 8 adjacent
   // columns per lane.
-  static __device__ __forceinline__ u16x8 cols(const char* p, int kb, int T, int lane) {
+  static __device__ __forceinline__ int col_base(int lane) {
     const int r16 = lane % 16, grp = lane / 16;
-    const int m4 = r16 >> 2, q4 = r16 & 3;
-    const int r0 = 8 * grp + m4, r1 = r0 + 4;
-    const int b0 = (r0 * RS + 16 * (q4 ^ swz(r0))) ^ ((T >> 1) * 64);
-    const int b1 = (r1 * RS + 16 * (q4 ^ swz(r1))) ^ ((T >> 1) * 64);
-    const int at = kb * 32 * RS + (T & 1) * 8;
+    const int m4 = r16 >> 2, q4 = r16 & 3, r0 = 8 * grp + m4;
+    return r0 * RS + 16 * (q4 ^ swz(r0));
+  }
+  static __device__ __forceinline__ u16x8 cols(const char* p, int base, int kb, int T) {
+    const int b0 = base ^ ((T >> 1) * 64), at = kb * 32 * RS + (T & 1) * 8;
+    // (four rows on, the unit's lowest bit is the other one)
     const u16x4 lo = lds_tr16(reinterpret_cast<const uint16_t*>(p + b0 + at));
-    const u16x4 hi = lds_tr16(reinterpret_cast<const uint16_t*>(p + b1 + at));
+    const u16x4 hi = lds_tr16(reinterpret_cast<const uint16_t*>(p + (b0 ^ 16) + 4 * RS + at));
     return cat8(lo, hi);
   }
   // The same for 16 adjacent columns: lane (r16, grp) holds
   // X[32 kb + 8 grp + i][16 T + r16].
-  static __device__ __forceinline__ u16x8 cols16(const char* p, int kb, int T, int lane) {
+  static __device__ __forceinline__ int col16_base(int T, int lane) {
     const int r16 = lane % 16, grp = lane / 16;
-    const int m4 = r16 >> 2, q4 = r16 & 3;
-    const int r0 = 8 * grp + m4, r1 = r0 + 4, u = 2 * T + (q4 >> 1);
-    const int at = kb * 32 * RS + (q4 & 1) * 8;
-    const u16x4 lo = lds_tr16(reinterpret_cast<const uint16_t*>(p + off(r0, u) + at));
-    const u16x4 hi = lds_tr16(reinterpret_cast<const uint16_t*>(p + off(r1, u) + at));
+    const int m4 = r16 >> 2, q4 = r16 & 3, r0 = 8 * grp + m4;
+    return off(r0, 2 * T + (q4 >> 1)) + (q4 & 1) * 8;
+  }
+  static __device__ __forceinline__ u16x8 cols16(const char* p, int base, int kb) {
+    const int at = kb * 32 * RS;
+    const u16x4 lo = lds_tr16(reinterpret_cast<const uint16_t*>(p + base + at));
+    const u16x4 hi = lds_tr16(reinterpret_cast<const uint16_t*>(p + (base ^ 16) + 4 * RS + at));
     return cat8(lo, hi);
   }
 };
@@ -101,50 +111,101 @@ struct LinTile {
 // and load, by NT threads: rows at and past `n` are zero.
 template <int D, int NT>
 struct LinStage {
-  static constexpr int ALL = 64 * (D / 8);
-  static constexpr int PER = (ALL + NT - 1) / NT;
+  static constexpr int UNITS = D / 8, ALL = 64 * UNITS, PER = (ALL + NT - 1) / NT;
+  static constexpr int STEP = NT / UNITS;   // rows between a lane's loads
+  static_assert(STEP % 4 == 0, "swizzle by constant offsets");
   u32x4 r[PER];
+  // bytes into the chunk's rows of a lane's first load; and into the tile
+  static __device__ __forceinline__ int from(int row, int tid) {
+    return ((tid / UNITS) * row + tid % UNITS * 8) * 2;
+  }
+  static __device__ __forceinline__ int at(int tid, int i) {
+    return LinTile<D>::off(tid / UNITS + i * STEP, tid % UNITS);
+  }
   // p: the head's columns of the chunk's first token; row: elements per token
-  __device__ __forceinline__ void load(const uint16_t* p, int row, int n, int tid) {
+  __device__ __forceinline__ void load(const uint16_t* p, int row, int n, int from) {
     const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint16_t*>(p), 0, n > 0 ? ((n - 1) * row + D) * 2 : 0, kBufferFlags);
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int u = tid + i * NT;
+    for (int i = 0; i < PER; ++i)
       r[i] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-          rs, ((u / (D / 8)) * row + (u % (D / 8)) * 8) * 2, 0, 0));
-    }
+          rs, from + i * STEP * row * 2, 0, 0));
   }
-  __device__ __forceinline__ void store(char* tile, int tid) const {
+  // base: at(tid, 0)
+  __device__ __forceinline__ void store(char* tile, int base, int tid) const {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int u = tid + i * NT;
-      if (ALL % NT && u >= ALL) break;   // (its load was past row 64: out of range, 0)
-      *reinterpret_cast<u32x4*>(tile + LinTile<D>::off(u / (D / 8), u % (D / 8))) = r[i];
+      if (ALL % NT && tid + i * NT >= ALL) break;   // (its load was past row 64: 0)
+      const int to = STEP % 16 == 0 ? base + i * STEP * LinTile<D>::RS : at(tid, i);
+      *reinterpret_cast<u32x4*>(tile + to) = r[i];
     }
   }
 };
 
-// Inclusive prefix sum over a wave.
-__device__ __forceinline__ float wave_prefix(float x, int lane) {
-#pragma unroll
-  for (int off = 1; off < 64; off *= 2) {
-    const float y = __shfl_up(x, off);
-    if (lane >= off) x += y;
-  }
-  return x;
+// The index of this wave, known to be the same in all its lanes.
+__device__ __forceinline__ int wave_index() {
+  return __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
 }
-// Exclusive suffix sum over a wave (sums of what follows a lane).
-__device__ __forceinline__ float wave_suffix(float x, int lane) {
-  float s = __shfl_down(x, 1);
-  if (lane == 63) s = 0.f;
-#pragma unroll
-  for (int off = 1; off < 64; off *= 2) {
-    const float y = __shfl_down(s, off);
-    if (lane + off < 64) s += y;
-  }
-  return s;
+__device__ __forceinline__ void hide(int& x) { asm volatile("" : "+v"(x)); }
+
+// Inclusive prefix sum over a wave, in its lanes' own adders (no LDS).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_add(float x) {
+  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                 0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
 }
+__device__ __forceinline__ float wave_prefix(float x) {
+  x = dpp_add<0x111, 0xf>(x);   // row_shr 1, 2, 4, 8: within 16 lanes
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);   // lane 15 of a row to the next: rows 1 and 3
+  return dpp_add<0x143, 0xc>(x);   // lane 31 to rows 2 and 3
+}
+
+__device__ __forceinline__ float lane63(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+
+// Eight bf16 values times eight fp32 factors (in LDS) as hi + lo in bf16.
+__device__ __forceinline__ void lin_split(u16x8 y, const float* f, u16x8& hi, u16x8& lo) {
+  const f32x4 f0 = *reinterpret_cast<const f32x4*>(f), f1 = *reinterpret_cast<const f32x4*>(f + 4);
+  u16x4 h0, l0, h1, l1;
+  split_bf4(f32x4{bf2f(y[0]), bf2f(y[1]), bf2f(y[2]), bf2f(y[3])} * f0, h0, l0);
+  split_bf4(f32x4{bf2f(y[4]), bf2f(y[5]), bf2f(y[6]), bf2f(y[7])} * f1, h1, l1);
+  hi = cat8(h0, h1);
+  lo = cat8(l0, l1);
+}
+
+// The decays of a chunk on their way in, by two waves: wave 0's lane l has its
+// own token, wave 1's the token 64 - l, so that the prefix sums and the sums
+// of what follows a token (63 - l) are the same scan.  Loaded a chunk ahead,
+// without a branch, and converted where they are used: a wait for them here
+// would hold up the loads behind them.
+struct LinGates {
+  FlatRaw raw;
+  int n;
+  static __device__ __forceinline__ int token(int w, int lane) { return w == 0 ? lane : 64 - lane; }
+  // tok: the chunk's first token; n: its tokens (0: none); i: token(w, lane)
+  __device__ __forceinline__ void load(const LinDecay& d, size_t tok, int n_, int h, int Hv, int i) {
+    n = n_;
+    const int es = d.dt == GDN_DTYPE_F32 ? 4 : 2;
+    const char* p = static_cast<const char*>(d.g) + tok * d.per_token * es;
+    raw = ldp_flat_raw(p, i * d.per_token + h, d.dt, d.per_token ? n * Hv : (n > 0 ? Hv : 0));
+  }
+  __device__ __forceinline__ float prefix(const LinDecay& d, int i) const {
+    const float x = lin_clamp(flat_value(raw, d.dt));
+    return wave_prefix(i < n ? x : 0.f);
+  }
+};
+
+// A [K][V] fp32 state: a lane's part in one register offset, the tiles' and
+// rows' in scalars; without a state (NULL) the loads give 0.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t lin_state(const float* p, int KV) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(p), 0, p ? KV * 4 : 0, kBufferFlags);
+}
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // Workgroup -> work item so that neighbouring items run on the same XCD
 // (workgroups go round the 8 of them) and share its L2.  The grid is

@@ -79,102 +79,111 @@ __global__ __launch_bounds__(1024) void lin_table_kernel(const int32_t* cu, LinS
   for (int i = seg0 + tid; i < nseg; i += 1024) table[i] = LinSeg{0, 0, 0, -1, 0, 0};
 }
 
+// A wave's 16 columns of a state [K][V] as accumulators: tile t's lane holds
+// rows rho_row(t, 4 grp + r) of column 16 w + r16.
+template <int K, int V>
+__device__ __forceinline__ void lin_load_state(f32x4 (&S)[K / 16], const float* p, int w, int lane) {
+  const __amdgpu_buffer_rsrc_t rs = lin_state(p, K * V);
+  const int at = (8 * (lane / 16) * V + 16 * w + lane % 16) * 4;
+#pragma unroll
+  for (int t = 0; t < K / 16; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      S[t][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+          rs, at, (32 * (t >> 1) + 4 * (t & 1) + r) * V * 4, 0));
+}
+template <int K, int V>
+__device__ __forceinline__ void lin_store_state(const f32x4 (&S)[K / 16], float* p, int w, int lane) {
+  const __amdgpu_buffer_rsrc_t rs = lin_state(p, K * V);
+  const int at = (8 * (lane / 16) * V + 16 * w + lane % 16) * 4;
+#pragma unroll
+  for (int t = 0; t < K / 16; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(S[t][r]), rs, at,
+                                            (32 * (t >> 1) + 4 * (t & 1) + r) * V * 4, 0);
+}
+
 // -------------------------------------------------------------- segments ----
 // Contribution of a segment to the state after it: sum over its chunks of
 // X^T (f Y) with x = k, y = v, f = e^R; or (REV) to the gradient of the state
 // before it, chunks last to first, x = q, y = dO, f = scale e^G.  A wave owns
-// 32 columns of Y and all rows of the state.
+// 16 columns of Y and all rows of the state.
 template <int K, int V, bool REV>
-__global__ __launch_bounds__(2 * V, 2) void lin_segment_kernel(
+__global__ __launch_bounds__(4 * V, 4) void lin_segment_kernel(
     const uint16_t* __restrict__ x, int x_row, const uint16_t* __restrict__ y, int y_row,
     LinDecay dec, LinGrid grid, int Hqk, int Hv, float scale, float* __restrict__ segs,
     float* __restrict__ decay) {
-  constexpr int NT = 2 * V;
+  constexpr int NT = 4 * V;
   __shared__ __align__(16) char xs[LinTile<K>::BYTES];
   __shared__ __align__(16) char ys[LinTile<V>::BYTES];
-  __shared__ __align__(16) float fac[2][64];
-  __shared__ float tot[2];
+  __shared__ __align__(16) float fac[64];
+  __shared__ float tot;
   const int item = xcd_item();
   if (item >= grid.nseg * Hv) return;
   const int sid = item / Hv, h = item % Hv, hq = h / (Hv / Hqk);
   const LinSeg sg = lin_seg(grid, sid);
   if (sg.seq < 0 || (REV ? sg.first : sg.last)) return;
-  const int tid = threadIdx.x, lane = tid % 64, w = tid / 64;
+  const int tid = threadIdx.x, lane = tid % 64, w = wave_index();
   const int r16 = lane % 16, grp = lane / 16;
   const int nc = (sg.ntok + kChunk - 1) / kChunk;
 
-  f32x4 S[K / 16][2];
+  f32x4 S[K / 16];
 #pragma unroll
-  for (int t = 0; t < K / 16; ++t) S[t][0] = S[t][1] = zero4();
+  for (int t = 0; t < K / 16; ++t) S[t] = zero4();
   LinStage<K, NT> sx;
   LinStage<V, NT> sy;
+  LinGates lg;
+  int gi = LinGates::token(w, lane);
   float gsum = 0.f;
+  int xf = LinStage<K, NT>::from(x_row, tid), yf = LinStage<V, NT>::from(y_row, tid);
+  int xt = LinStage<K, NT>::at(tid, 0), yt = LinStage<V, NT>::at(tid, 0);
   auto load = [&](int c) {
     const int n = c >= 0 && c < nc ? sg.ntok - c * kChunk : 0;
     const size_t t = n > 0 ? (size_t)sg.tok0 + c * kChunk : 0;
-    sx.load(x + t * x_row + hq * K, x_row, min(n, 64), tid);
-    sy.load(y + t * y_row + h * V, y_row, min(n, 64), tid);
-  };
-  auto gates = [&](int c, int buf) {   // one wave
-    const int t = c * kChunk + lane;
-    const float g = c >= 0 && c < nc && t < sg.ntok ? lin_g(dec, sg.tok0 + t, h) : 0.f;
-    const float pre = wave_prefix(g, lane);
-    const float sum = __shfl(pre, 63);
-    fac[buf][lane] = REV ? scale * __expf(pre) : __expf(wave_suffix(g, lane));
-    if (lane == 0) tot[buf] = sum;
-    gsum += sum;
+    if (w < 2) lg.load(dec, t, min(n, 64), h, Hv, gi);
+    sx.load(x + t * x_row + hq * K, x_row, min(n, 64), xf);
+    sy.load(y + t * y_row + h * V, y_row, min(n, 64), yf);
   };
   const int c0 = REV ? nc - 1 : 0, step = REV ? -1 : 1;
+  int xb = LinTile<K>::col_base(lane), yb = LinTile<V>::col16_base(w, lane);
   load(c0);
-  if (w == 0) gates(c0, 0);
   for (int i = 0; i < nc; ++i) {
-    const int c = c0 + i * step, buf = i & 1;
-    sx.store(xs, tid);
-    sy.store(ys, tid);
+    hide(xb);
+    hide(xf);
+    hide(yf);
+    hide(gi);
+    sx.store(xs, xt, tid);
+    sy.store(ys, yt, tid);
+    if (w < 2) {
+      const float pre = lg.prefix(dec, gi);
+      if (w == 1) {
+        if (!REV) fac[63 - lane] = __expf(pre);
+      } else {
+        if (REV) fac[lane] = scale * __expf(pre);
+        if (lane == 63) tot = pre;
+        gsum += lane63(pre);
+      }
+    }
     __syncthreads();
-    load(c + step);
-    if (w == 0) gates(c + step, buf ^ 1);
-    const float eC = __expf(tot[buf]);
+    load(c0 + (i + 1) * step);
+    const float eC = __expf(tot);
 #pragma unroll
-    for (int t = 0; t < K / 16; ++t)
-#pragma unroll
-      for (int T = 0; T < 2; ++T) S[t][T] *= eC;
+    for (int t = 0; t < K / 16; ++t) S[t] *= eC;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      const f32x4 f0 = *reinterpret_cast<const f32x4*>(&fac[buf][32 * kb + 8 * grp]);
-      const f32x4 f1 = *reinterpret_cast<const f32x4*>(&fac[buf][32 * kb + 8 * grp + 4]);
-      u16x8 hi[2], lo[2];
-#pragma unroll
-      for (int T = 0; T < 2; ++T) {
-        const u16x8 yf = LinTile<V>::cols(ys, kb, 2 * w + T, lane);
-        u16x4 h0, l0, h1, l1;
-        split_bf4(f32x4{bf2f(yf[0]), bf2f(yf[1]), bf2f(yf[2]), bf2f(yf[3])} * f0, h0, l0);
-        split_bf4(f32x4{bf2f(yf[4]), bf2f(yf[5]), bf2f(yf[6]), bf2f(yf[7])} * f1, h1, l1);
-        hi[T] = cat8(h0, h1);
-        lo[T] = cat8(l0, l1);
-      }
+      u16x8 hi, lo;
+      lin_split(LinTile<V>::cols16(ys, yb, kb), fac + 32 * kb + 8 * grp, hi, lo);
 #pragma unroll
       for (int t = 0; t < K / 16; ++t) {
-        const u16x8 a = LinTile<K>::cols(xs, kb, t, lane);
-#pragma unroll
-        for (int T = 0; T < 2; ++T) {
-          S[t][T] = mfma16(a, hi[T], S[t][T]);
-          S[t][T] = mfma16(a, lo[T], S[t][T]);
-        }
+        const u16x8 a = LinTile<K>::cols(xs, xb, kb, t);
+        S[t] = mfma16(a, hi, S[t]);
+        S[t] = mfma16(a, lo, S[t]);
       }
     }
     __syncthreads();
   }
-  float* out = segs + ((size_t)sid * Hv + h) * K * V;
-#pragma unroll
-  for (int t = 0; t < K / 16; ++t)
-#pragma unroll
-    for (int T = 0; T < 2; ++T)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        out[rho_row(t, 4 * grp + r) * V + 32 * w + 8 * (r16 >> 2) + 4 * T + (r16 & 3)] =
-            S[t][T][r];
-  // (wave 0's sum covers one chunk past the last, whose decays are 0)
+  lin_store_state<K, V>(S, segs + ((size_t)sid * Hv + h) * K * V, w, lane);
   if (tid == 0) decay[(size_t)sid * Hv + h] = __expf(gsum);
 }
 
@@ -223,22 +232,22 @@ __global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int
 
 // ------------------------------------------------------------------ walk ----
 // One segment and v-head from its start state, chunk by chunk: o (OUT), the
-// state at every chunk's start (SAVE), ht.  A wave owns 32 columns of V, all
+// state at every chunk's start (SAVE), ht.  A wave owns 16 columns of V, all
 // of the state's rows for them in its accumulators, whose layout is that of
 // the operand with which S^T q is formed: the state never leaves the registers.
 template <int K, int V, bool OUT, bool SAVE>
-__global__ __launch_bounds__(2 * V, 2) void lin_walk_kernel(
+__global__ __launch_bounds__(4 * V, 4) void lin_walk_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k,
     const uint16_t* __restrict__ v, TokenStride ts, LinDecay dec, LinGrid grid, int Hqk, int Hv,
     float scale, const float* h0, float* ht, const float* __restrict__ segs,
-    uint16_t* __restrict__ o, u16x8* __restrict__ states) {
-  constexpr int NT = 2 * V, NW = V / 32;
+    uint16_t* __restrict__ o, u16x4* __restrict__ states) {
+  constexpr int NT = 4 * V, NW = V / 16;
   __shared__ __align__(16) char qs[LinTile<K>::BYTES];
   __shared__ __align__(16) char ks[LinTile<K>::BYTES];
   __shared__ __align__(16) char vs[LinTile<V>::BYTES];
   __shared__ __align__(16) char ps[LinTile<64>::BYTES];
-  __shared__ __align__(16) float sG[2][64], sQ[2][64], sK[2][64];   // G, scale e^G, e^R
-  const int tid = threadIdx.x, lane = tid % 64, w = tid / 64;
+  __shared__ __align__(16) float sG[64], sQ[64], sK[64];   // G log2(e), scale e^G, e^R
+  const int tid = threadIdx.x, lane = tid % 64, w = wave_index();
   const int r16 = lane % 16, grp = lane / 16;
   const int item = xcd_item();
   if (grid.table && *grid.status) {
@@ -254,35 +263,27 @@ __global__ __launch_bounds__(2 * V, 2) void lin_walk_kernel(
   const LinSeg sg = lin_seg(grid, sid);
   if (sg.seq < 0) return;
   const int nc = (sg.ntok + kChunk - 1) / kChunk;
-  const int vcol = 32 * w + 8 * (r16 >> 2) + (r16 & 3);   // + 4 T: the state's column
 
-  f32x4 S[K / 16][2];
+  f32x4 S[K / 16];   // rows rho_row(t, 4 grp + r), column 16 w + r16
   const float* src = sg.first ? (h0 ? h0 + ((size_t)sg.seq * Hv + h) * K * V : nullptr)
                               : segs + ((size_t)sid * Hv + h) * K * V;
-#pragma unroll
-  for (int t = 0; t < K / 16; ++t)
-#pragma unroll
-    for (int T = 0; T < 2; ++T)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        S[t][T][r] = src ? src[rho_row(t, 4 * grp + r) * V + vcol + 4 * T] : 0.f;
+  lin_load_state<K, V>(S, src, w, lane);
 
   LinStage<K, NT> sq, sk;
   LinStage<V, NT> sv;
+  LinGates lg;
+  int gi = LinGates::token(w, lane);
+  int qf = LinStage<K, NT>::from(ts.q, tid), kf = LinStage<K, NT>::from(ts.k, tid);
+  int vr = LinStage<V, NT>::from(ts.v, tid);
+  const int kt = LinStage<K, NT>::at(tid, 0), vt = LinStage<V, NT>::at(tid, 0);
+  int oat = (r16 * Hv * V + 16 * w + 4 * grp) * 2;   // bytes into the chunk's rows of o
   auto load = [&](int c) {
     const int n = c < nc ? sg.ntok - c * kChunk : 0;
     const size_t t = n > 0 ? (size_t)sg.tok0 + c * kChunk : 0;
-    if (OUT) sq.load(q + t * ts.q + hq * K, ts.q, min(n, 64), tid);
-    sk.load(k + t * ts.k + hq * K, ts.k, min(n, 64), tid);
-    sv.load(v + t * ts.v + h * V, ts.v, min(n, 64), tid);
-  };
-  auto gates = [&](int c, int buf) {   // one wave
-    const int t = c * kChunk + lane;
-    const float g = c < nc && t < sg.ntok ? lin_g(dec, sg.tok0 + t, h) : 0.f;
-    const float pre = wave_prefix(g, lane);
-    sG[buf][lane] = pre;
-    sQ[buf][lane] = scale * __expf(pre);
-    sK[buf][lane] = __expf(wave_suffix(g, lane));
+    if (w < 2) lg.load(dec, t, min(n, 64), h, Hv, gi);
+    if (OUT) sq.load(q + t * ts.q + hq * K, ts.q, min(n, 64), qf);
+    sk.load(k + t * ts.k + hq * K, ts.k, min(n, 64), kf);
+    sv.load(v + t * ts.v + h * V, ts.v, min(n, 64), vr);
   };
   if (OUT) {
     // the tiles of P above the diagonal that share a 32-wide block with it
@@ -291,16 +292,39 @@ __global__ __launch_bounds__(2 * V, 2) void lin_walk_kernel(
       *reinterpret_cast<u32x4*>(ps + LinTile<64>::off(r, u)) = u32x4{0, 0, 0, 0};
     }
   }
+  int rb = LinTile<K>::row_base(lane), kcb = LinTile<K>::col_base(lane);
+  int vb = LinTile<V>::col16_base(w, lane), pb = LinTile<64>::row_base(lane);
+  int pw = LinTile<64>::off(r16, grp >> 1) + (grp & 1) * 8;
   load(0);
-  if (w == 0) gates(0, 0);
   for (int c = 0; c < nc; ++c) {
-    const int buf = c & 1;
-    if (OUT) sq.store(qs, tid);
-    sk.store(ks, tid);
-    sv.store(vs, tid);
+    // (nothing derived from these is kept from one chunk for the next)
+    int ln = lane;
+    hide(ln);
+    const int r16 = ln % 16, grp = ln / 16;
+    hide(vb);
+    hide(pb);
+    hide(pw);
+    hide(rb);
+    hide(kcb);
+    hide(qf);
+    hide(gi);
+    hide(kf);
+    hide(vr);
+    hide(oat);
+    if (OUT) sq.store(qs, kt, tid);
+    sk.store(ks, kt, tid);
+    sv.store(vs, vt, tid);
+    if (w < 2) {
+      const float pre = lg.prefix(dec, gi) * kLog2e, e = exp2_(pre);
+      if (w == 1) {
+        sK[63 - lane] = e;
+      } else {
+        sG[lane] = pre;
+        sQ[lane] = scale * e;
+      }
+    }
     __syncthreads();
     load(c + 1);
-    if (w == 0) gates(c + 1, buf ^ 1);
 
     if (OUT) {
       // P, tile by tile (token block it, source block jt), as bf16 rows
@@ -309,116 +333,85 @@ __global__ __launch_bounds__(2 * V, 2) void lin_walk_kernel(
         f32x4 p = zero4();
 #pragma unroll
         for (int kb = 0; kb < K / 32; ++kb)
-          p = mfma16(LinTile<K>::rows(ks, jt, kb, lane), LinTile<K>::rows(qs, it, kb, lane), p);
+          p = mfma16(LinTile<K>::rows(ks, rb, jt, kb), LinTile<K>::rows(qs, rb, it, kb), p);
         const int i = 16 * it + r16, j = 16 * jt + 4 * grp;
-        const f32x4 gj = *reinterpret_cast<const f32x4*>(&sG[buf][j]);
-        const float gi = sG[buf][i];
+        const f32x4 gj = *reinterpret_cast<const f32x4*>(&sG[j]);
+        const float gi = sG[i];
+        // (a select on each side of the product: no branch around the exponential,
+        // and what is masked may be infinite or NaN)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[r] = j + r <= i ? p[r] * (scale * __expf(gi - gj[r])) : 0.f;
-        *reinterpret_cast<u16x4*>(ps + LinTile<64>::off(i, j / 8) + (grp & 1) * 8) = f2bf4(p);
+        for (int r = 0; r < 4; ++r) {
+          const bool in = j + r <= i;
+          p[r] = (in ? p[r] * scale : 0.f) * exp2_(in ? gi - gj[r] : 0.f);
+        }
+        *reinterpret_cast<u16x4*>(ps + (pw ^ (32 * jt)) + it * 2048) = f2bf4(p);
       }
     }
     // the state as bf16 operands, by rows of 32 keys
-    f32x4 O[4][2];
+    f32x4 O[4];   // columns 16 w + 4 grp + r of token 16 tt + r16
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt) O[tt][0] = O[tt][1] = zero4();
+    for (int tt = 0; tt < 4; ++tt) O[tt] = zero4();
 #pragma unroll
     for (int b = 0; b < K / 32; ++b) {
-      u16x8 sb[2];
-#pragma unroll
-      for (int T = 0; T < 2; ++T) sb[T] = cat8(f2bf4(S[2 * b][T]), f2bf4(S[2 * b + 1][T]));
+      const u16x8 sb = cat8(f2bf4(S[2 * b]), f2bf4(S[2 * b + 1]));
       if (OUT) {
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-          const u16x8 qf = LinTile<K>::rows(qs, tt, b, lane);
-#pragma unroll
-          for (int T = 0; T < 2; ++T) O[tt][T] = mfma16(sb[T], qf, O[tt][T]);
-        }
+        for (int tt = 0; tt < 4; ++tt) O[tt] = mfma16(sb, LinTile<K>::rows(qs, rb, tt, b), O[tt]);
       }
       if (SAVE) {
         // transposed through a product with a selection matrix (exact): lane
-        // (r16, grp) gets key rho_row(t, r16), values 32 w + 8 grp + i
-        u16x8* dst = states + ((size_t)(sg.chunk0 + c) * Hv + h) * (K / 16) * (V / 32) * 64;
+        // (r16, grp) gets key rho_row(t, r16), values 16 w + 4 grp + r, which
+        // are half a lane's share of the backward's fragment
+        u16x4* dst = states + ((size_t)(sg.chunk0 + c) * Hv + h) * (K / 16) * (V / 32) * 128 +
+                     (w >> 1) * 128 + (r16 + 16 * (2 * (w & 1) + (grp >> 1))) * 2 + (grp & 1);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           u16x8 sel;
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             sel[i] = grp == r16 >> 2 && i == 4 * e + (r16 & 3) ? 0x3F80 : 0;
-          const f32x4 a0 = mfma16(sb[0], sel, zero4()), a1 = mfma16(sb[1], sel, zero4());
-          dst[((2 * b + e) * (V / 32) + w) * 64 + lane] = cat8(f2bf4(a0), f2bf4(a1));
+          dst[(2 * b + e) * (V / 32) * 128] = f2bf4(mfma16(sb, sel, zero4()));
         }
       }
     }
     if (OUT) {
-      float eq[4];
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) eq[tt] = sQ[buf][16 * tt + r16];
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        O[tt][0] *= eq[tt];
-        O[tt][1] *= eq[tt];
-      }
+      for (int tt = 0; tt < 4; ++tt) O[tt] *= sQ[16 * tt + r16];
       __syncthreads();   // P
     }
-    const float eC = __expf(sG[buf][63]);
+    const float eC = exp2_(sG[63]);
 #pragma unroll
-    for (int t = 0; t < K / 16; ++t)
-#pragma unroll
-      for (int T = 0; T < 2; ++T) S[t][T] *= eC;
+    for (int t = 0; t < K / 16; ++t) S[t] *= eC;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      const f32x4 f0 = *reinterpret_cast<const f32x4*>(&sK[buf][32 * kb + 8 * grp]);
-      const f32x4 f1 = *reinterpret_cast<const f32x4*>(&sK[buf][32 * kb + 8 * grp + 4]);
-      u16x8 vf[2], hi[2], lo[2];
-#pragma unroll
-      for (int T = 0; T < 2; ++T) {
-        vf[T] = LinTile<V>::cols(vs, kb, 2 * w + T, lane);
-        u16x4 h0_, l0, h1, l1;
-        split_bf4(f32x4{bf2f(vf[T][0]), bf2f(vf[T][1]), bf2f(vf[T][2]), bf2f(vf[T][3])} * f0, h0_, l0);
-        split_bf4(f32x4{bf2f(vf[T][4]), bf2f(vf[T][5]), bf2f(vf[T][6]), bf2f(vf[T][7])} * f1, h1, l1);
-        hi[T] = cat8(h0_, h1);
-        lo[T] = cat8(l0, l1);
-      }
+      const u16x8 vf = LinTile<V>::cols16(vs, vb, kb);
       if (OUT) {
 #pragma unroll
-        for (int tt = 2 * kb; tt < 4; ++tt) {
-          const u16x8 pf = LinTile<64>::rows(ps, tt, kb, lane);
-#pragma unroll
-          for (int T = 0; T < 2; ++T) O[tt][T] = mfma16(vf[T], pf, O[tt][T]);
-        }
+        for (int tt = 2 * kb; tt < 4; ++tt)
+          O[tt] = mfma16(vf, LinTile<64>::rows(ps, pb, tt, kb), O[tt]);
       }
+      u16x8 hi, lo;
+      lin_split(vf, sK + 32 * kb + 8 * grp, hi, lo);
 #pragma unroll
       for (int t = 0; t < K / 16; ++t) {
-        const u16x8 a = LinTile<K>::cols(ks, kb, t, lane);
-#pragma unroll
-        for (int T = 0; T < 2; ++T) {
-          S[t][T] = mfma16(a, hi[T], S[t][T]);
-          S[t][T] = mfma16(a, lo[T], S[t][T]);
-        }
+        const u16x8 a = LinTile<K>::cols(ks, kcb, kb, t);
+        S[t] = mfma16(a, hi, S[t]);
+        S[t] = mfma16(a, lo, S[t]);
       }
     }
     if (OUT) {
-      const int n = sg.ntok - c * kChunk;
-      uint16_t* dst = o + ((size_t)(sg.tok0 + c * kChunk) * Hv + h) * V + 32 * w + 8 * grp;
+      // (stores past the segment's last token are dropped)
+      const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(
+          o + ((size_t)(sg.tok0 + c * kChunk) * Hv + h) * V, 0,
+          ((min(sg.ntok - c * kChunk, 64) - 1) * Hv + 1) * V * 2, kBufferFlags);
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        const int i = 16 * tt + r16;
-        if (i < n)
-          *reinterpret_cast<u16x8*>(dst + (size_t)i * Hv * V) = cat8(f2bf4(O[tt][0]), f2bf4(O[tt][1]));
-      }
+      for (int tt = 0; tt < 4; ++tt)
+        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2p, f2bf4(O[tt])), ro,
+                                              oat + tt * 16 * Hv * V * 2, 0, 0);
     }
     __syncthreads();
   }
-  if (ht && sg.last) {
-    float* out = ht + ((size_t)sg.seq * Hv + h) * K * V;
-#pragma unroll
-    for (int t = 0; t < K / 16; ++t)
-#pragma unroll
-      for (int T = 0; T < 2; ++T)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) out[rho_row(t, 4 * grp + r) * V + vcol + 4 * T] = S[t][T][r];
-  }
+  if (ht && sg.last) lin_store_state<K, V>(S, ht + ((size_t)sg.seq * Hv + h) * K * V, w, lane);
 }
 
 // ------------------------------------------------------------------ host ----
@@ -488,11 +481,11 @@ void launch_lin_segments(const uint16_t* x, int x_row, const uint16_t* y, int y_
                          hipStream_t st) {
   const dim3 items(xcd_grid((long long)g.nseg * Hv)), elems((unsigned)(g.N * Hv * (K * V / 256)));
   if (reverse) {
-    hipLaunchKernelGGL((lin_segment_kernel<K, V, true>), items, dim3(2 * V), 0, st, x, x_row, y,
+    hipLaunchKernelGGL((lin_segment_kernel<K, V, true>), items, dim3(4 * V), 0, st, x, x_row, y,
                        y_row, d, g, Hqk, Hv, scale, segs, decay);
     hipLaunchKernelGGL(lin_join_kernel<true>, elems, dim3(256), 0, st, g, Hv, K * V, edge, segs, decay);
   } else {
-    hipLaunchKernelGGL((lin_segment_kernel<K, V, false>), items, dim3(2 * V), 0, st, x, x_row, y,
+    hipLaunchKernelGGL((lin_segment_kernel<K, V, false>), items, dim3(4 * V), 0, st, x, x_row, y,
                        y_row, d, g, Hqk, Hv, scale, segs, decay);
     hipLaunchKernelGGL(lin_join_kernel<false>, elems, dim3(256), 0, st, g, Hv, K * V, edge, segs, decay);
   }
@@ -508,13 +501,13 @@ namespace {
 template <int K, int V>
 void launch_walk(const uint16_t* q, const uint16_t* k, const uint16_t* v, TokenStride ts,
                  const LinDecay& d, const LinGrid& g, int Hqk, int Hv, float scale,
-                 const float* h0, float* ht, float* segs, float* decay, uint16_t* o, u16x8* states,
+                 const float* h0, float* ht, float* segs, float* decay, uint16_t* o, u16x4* states,
                  hipStream_t st) {
   if (g.nps > 1)
     launch_lin_segments<K, V>(k, ts.k, v, ts.v, d, g, Hqk, Hv, 1.f, false, h0, segs, decay, st);
   const dim3 items(xcd_grid((long long)g.nseg * Hv));
 #define GDN_LW(OUT, SAVE)                                                                      \
-  hipLaunchKernelGGL((lin_walk_kernel<K, V, OUT, SAVE>), items, dim3(2 * V), 0, st, q, k, v, ts, \
+  hipLaunchKernelGGL((lin_walk_kernel<K, V, OUT, SAVE>), items, dim3(4 * V), 0, st, q, k, v, ts, \
                      d, g, Hqk, Hv, scale, h0, ht, segs, o, states)
   if (o && states) GDN_LW(true, true);
   else if (o) GDN_LW(true, false);
@@ -602,7 +595,7 @@ extern "C" int gdn_linear_chunk_fwd(const void* q, const void* k, const void* v,
     gdn::launch_walk<KK, VV>(static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), \
                              static_cast<const uint16_t*>(v), ts, d, grid, Hqk, Hv, scale, h0, \
                              ht, segs, decay, static_cast<uint16_t*>(o),                       \
-                             static_cast<gdn::u16x8*>(states), st);                            \
+                             static_cast<gdn::u16x4*>(states), st);                            \
     return gdn_host::check_launch(name);                                                       \
   }
   GDN_LIN(128, 128) GDN_LIN(128, 64) GDN_LIN(64, 128) GDN_LIN(64, 64)

@@ -51,10 +51,10 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
   __shared__ __align__(16) char os[LinTile<V>::BYTES];
   __shared__ __align__(16) char ps[LinTile<64>::BYTES];
   __shared__ __align__(16) char dps[LinTile<64>::BYTES];
-  __shared__ __align__(16) float sG[2][64], sQ[2][64], sK[2][64];
+  __shared__ __align__(16) float sG[64], sQ[64], sK[64];   // G log2(e), scale e^G, e^R
   __shared__ __align__(16) float rowM[4][64], colM[4][64], asum[NK][64], bsum[NK][64];
   __shared__ float csum[NK];
-  const int tid = threadIdx.x, lane = tid % 64, w = tid / 64;
+  const int tid = threadIdx.x, lane = tid % 64, w = wave_index();
   const int r16 = lane % 16, grp = lane / 16;
   const int item = xcd_item();
   if (a.grid.table && *a.grid.status) {
@@ -82,6 +82,8 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
   f32x4 ST[NTILE][2];
   const float* src = sg.last ? (a.dht ? a.dht + ((size_t)sg.seq * a.Hv + h) * K * V : nullptr)
                              : a.segs + ((size_t)sid * a.Hv + h) * K * V;
+  const __amdgpu_buffer_rsrc_t rst = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<float*>(src), 0, src ? K * V * 4 : 0, kBufferFlags);
   const int c32 = 8 * (r16 >> 2) + (r16 & 3);   // + 4 T: the lane's column of 32
 #pragma unroll
   for (int t = 0; t < NTILE; ++t)
@@ -90,31 +92,27 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int row = rho_row(t, 4 * grp + r), col = c32 + 4 * T;
-        float x = 0.f;
-        if (src) {
-          if (vwave && t < K / 16) x = src[row * V + 32 * wv + col];
-          if (!vwave && t < V / 16) x = src[(32 * wk + col) * V + row];
-        }
-        ST[t][T][r] = x;
+        // (a tile the wave does not have is read out of range: 0)
+        const int in = vwave ? (t < K / 16 ? row * V + 32 * wv + col : K * V)
+                             : (t < V / 16 ? (32 * wk + col) * V + row : K * V);
+        ST[t][T][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rst, in * 4, 0, 0));
       }
 
   LinStage<K, NT> sq, sk;
   LinStage<V, NT> sv, so;
+  LinGates lg;
+  int gi = LinGates::token(w, lane);
+  int qf = LinStage<K, NT>::from(a.ts.q, tid), kf = LinStage<K, NT>::from(a.ts.k, tid);
+  int vf = LinStage<V, NT>::from(a.ts.v, tid), of = LinStage<V, NT>::from(a.Hv * V, tid);
+  const int kt = LinStage<K, NT>::at(tid, 0), vt = LinStage<V, NT>::at(tid, 0);
   auto load = [&](int c) {
     const int n = c >= 0 ? sg.ntok - c * kChunk : 0;
     const size_t t = n > 0 ? (size_t)sg.tok0 + c * kChunk : 0;
-    sq.load(a.q + t * a.ts.q + hq * K, a.ts.q, min(n, 64), tid);
-    sk.load(a.k + t * a.ts.k + hq * K, a.ts.k, min(n, 64), tid);
-    sv.load(a.v + t * a.ts.v + h * V, a.ts.v, min(n, 64), tid);
-    so.load(a.dO + (t * a.Hv + h) * V, a.Hv * V, min(n, 64), tid);
-  };
-  auto gates = [&](int c, int buf) {   // one wave
-    const int t = c * kChunk + lane;
-    const float g = c >= 0 && t < sg.ntok ? lin_g(a.dec, sg.tok0 + t, h) : 0.f;
-    const float pre = wave_prefix(g, lane);
-    sG[buf][lane] = pre;
-    sQ[buf][lane] = a.scale * __expf(pre);
-    sK[buf][lane] = __expf(wave_suffix(g, lane));
+    if (w < 2) lg.load(a.dec, t, min(n, 64), h, a.Hv, gi);
+    sq.load(a.q + t * a.ts.q + hq * K, a.ts.q, min(n, 64), qf);
+    sk.load(a.k + t * a.ts.k + hq * K, a.ts.k, min(n, 64), kf);
+    sv.load(a.v + t * a.ts.v + h * V, a.ts.v, min(n, 64), vf);
+    so.load(a.dO + (t * a.Hv + h) * V, a.Hv * V, min(n, 64), of);
   };
   // the tiles above the diagonal that share a 32-wide block with it, and the
   // sums that no tile writes
@@ -125,19 +123,37 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
   }
   for (int i = tid; i < 256; i += NT) rowM[i / 64][i % 64] = colM[i / 64][i % 64] = 0.f;
   __syncthreads();
+  int krb = LinTile<K>::row_base(lane), vrb = LinTile<V>::row_base(lane);
+  int kcb = LinTile<K>::col_base(lane), vcb = LinTile<V>::col_base(lane);
+  const int pb = LinTile<64>::row_base(lane);
   load(nc - 1);
-  if (w == 0 && nc > 0) gates(nc - 1, 0);
-  for (int it_ = 0; it_ < nc; ++it_) {
-    const int c = nc - 1 - it_, buf = it_ & 1;
+  for (int c = nc - 1; c >= 0; --c) {
+    hide(krb);
+    hide(vrb);
+    hide(kcb);
+    hide(vcb);
+    hide(qf);
+    hide(gi);
+    hide(kf);
+    hide(vf);
+    hide(of);
     const int n = sg.ntok - c * kChunk;
     const size_t tok = (size_t)sg.tok0 + c * kChunk;
-    sq.store(qs, tid);
-    sk.store(ks, tid);
-    sv.store(vs, tid);
-    so.store(os, tid);
+    sq.store(qs, kt, tid);
+    sk.store(ks, kt, tid);
+    sv.store(vs, vt, tid);
+    so.store(os, vt, tid);
+    if (w < 2) {
+      const float pre = lg.prefix(a.dec, gi) * kLog2e, e = exp2_(pre);
+      if (w == 1) {
+        sK[63 - lane] = e;
+      } else {
+        sG[lane] = pre;
+        sQ[lane] = a.scale * e;
+      }
+    }
     __syncthreads();
     load(c - 1);
-    if (w == 0) gates(c - 1, buf ^ 1);
 
     // P and dP, tile by tile, as bf16 rows, and the sums of M
     for (int m = w; m < 10; m += NW) {
@@ -145,22 +161,23 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
       f32x4 p = zero4(), d = zero4();
 #pragma unroll
       for (int kb = 0; kb < K / 32; ++kb)
-        p = mfma16(LinTile<K>::rows(ks, jt, kb, lane), LinTile<K>::rows(qs, it, kb, lane), p);
+        p = mfma16(LinTile<K>::rows(ks, krb, jt, kb), LinTile<K>::rows(qs, krb, it, kb), p);
 #pragma unroll
       for (int kb = 0; kb < V / 32; ++kb)
-        d = mfma16(LinTile<V>::rows(vs, jt, kb, lane), LinTile<V>::rows(os, it, kb, lane), d);
+        d = mfma16(LinTile<V>::rows(vs, vrb, jt, kb), LinTile<V>::rows(os, vrb, it, kb), d);
       const int i = 16 * it + r16, j = 16 * jt + 4 * grp;
-      const f32x4 gj = *reinterpret_cast<const f32x4*>(&sG[buf][j]);
-      const float gi = sG[buf][i];
+      const f32x4 gj = *reinterpret_cast<const f32x4*>(&sG[j]);
+      const float gi = sG[i];
       f32x4 M;
       float rs = 0.f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float gam = a.scale * __expf(gi - gj[r]);
         const bool in = j + r <= i;
-        p[r] = in ? p[r] * gam : 0.f;
-        M[r] = in ? p[r] * d[r] : 0.f;
-        d[r] = in ? d[r] * gam : 0.f;
+        const float gam = a.scale * exp2_(in ? gi - gj[r] : 0.f);
+        d[r] = in ? d[r] : 0.f;
+        p[r] = (in ? p[r] : 0.f) * gam;
+        M[r] = p[r] * d[r];
+        d[r] *= gam;
         rs += M[r];
       }
       *reinterpret_cast<u16x4*>(ps + LinTile<64>::off(i, j / 8) + (grp & 1) * 8) = f2bf4(p);
@@ -178,7 +195,7 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
     f32x4 X[4][2], Y[4][2];   // dv; or dk and dq (by token tile)
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) X[tt][0] = X[tt][1] = Y[tt][0] = Y[tt][1] = zero4();
-    const float eC = __expf(sG[buf][63]);
+    const float eC = exp2_(sG[63]);
     if (vwave) {
 #pragma unroll
       for (int b = 0; b < K / 32; ++b) {
@@ -187,14 +204,14 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
         for (int T = 0; T < 2; ++T) df[T] = cat8(f2bf4(ST[2 * b][T]), f2bf4(ST[2 * b + 1][T]));
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
-          const u16x8 kf = LinTile<K>::rows(ks, tt, b, lane);
+          const u16x8 kf = LinTile<K>::rows(ks, krb, tt, b);
 #pragma unroll
           for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(df[T], kf, X[tt][T]);
         }
       }
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
-        const float f = sK[buf][16 * tt + r16];
+        const float f = sK[16 * tt + r16];
         X[tt][0] *= f;
         X[tt][1] *= f;
       }
@@ -215,7 +232,7 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
         }
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
-          const u16x8 vf = LinTile<V>::rows(vs, tt, b, lane), of = LinTile<V>::rows(os, tt, b, lane);
+          const u16x8 vf = LinTile<V>::rows(vs, vrb, tt, b), of = LinTile<V>::rows(os, vrb, tt, b);
 #pragma unroll
           for (int T = 0; T < 2; ++T) {
             X[tt][T] = mfma16(df[T], vf, X[tt][T]);
@@ -229,7 +246,7 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
         const int i = 16 * tt + r16;
-        const float fk = sK[buf][i], fq = sQ[buf][i];
+        const float fk = sK[i], fq = sQ[i];
         const u16x8 kr = *reinterpret_cast<const u16x8*>(ks + LinTile<K>::off(i, 4 * wk + grp));
         const u16x8 qr = *reinterpret_cast<const u16x8*>(qs + LinTile<K>::off(i, 4 * wk + grp));
         float sa = 0.f, sb = 0.f;
@@ -265,7 +282,12 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
         y += bsum[u][lane];
         cs += csum[u];
       }
-      const float dg = eC * cs + x + wave_suffix(x, lane) + (wave_prefix(y, lane) - y);
+      // prefix sums of y before the token, and of x from it on (the total less
+      // what is before it)
+      const float px = wave_prefix(x);
+      const float tx = __builtin_bit_cast(
+          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, px), 63));
+      const float dg = eC * cs + (tx - px + x) + (wave_prefix(y) - y);
       if (lane < n) a.dg[(tok + lane) * a.Hv + h] = dg;
     }
 #pragma unroll
@@ -275,8 +297,8 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
     }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      const f32x4 f0 = *reinterpret_cast<const f32x4*>(&sQ[buf][32 * kb + 8 * grp]);
-      const f32x4 f1 = *reinterpret_cast<const f32x4*>(&sQ[buf][32 * kb + 8 * grp + 4]);
+      const f32x4 f0 = *reinterpret_cast<const f32x4*>(&sQ[32 * kb + 8 * grp]);
+      const f32x4 f1 = *reinterpret_cast<const f32x4*>(&sQ[32 * kb + 8 * grp + 4]);
       auto split = [&](u16x8 y, u16x8& hi, u16x8& lo) {
         u16x4 h0, l0, h1, l1;
         split_bf4(f32x4{bf2f(y[0]), bf2f(y[1]), bf2f(y[2]), bf2f(y[3])} * f0, h0, l0);
@@ -288,18 +310,18 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
       if (vwave) {
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
-          yf[T] = LinTile<V>::cols(os, kb, 2 * wv + T, lane);
+          yf[T] = LinTile<V>::cols(os, vcb, kb, 2 * wv + T);
           split(yf[T], hi[T], lo[T]);
         }
 #pragma unroll
         for (int tt = 0; tt < 2 * kb + 2; ++tt) {
-          const u16x8 pf = LinTile<64>::cols16(ps, kb, tt, lane);
+          const u16x8 pf = LinTile<64>::cols16(ps, LinTile<64>::col16_base(tt, lane), kb);
 #pragma unroll
           for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(yf[T], pf, X[tt][T]);
         }
 #pragma unroll
         for (int t = 0; t < K / 16; ++t) {
-          const u16x8 f = LinTile<K>::cols(qs, kb, t, lane);
+          const u16x8 f = LinTile<K>::cols(qs, kcb, kb, t);
 #pragma unroll
           for (int T = 0; T < 2; ++T) {
             ST[t][T] = mfma16(f, hi[T], ST[t][T]);
@@ -310,25 +332,25 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
         u16x8 kf[2];
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
-          yf[T] = LinTile<K>::cols(qs, kb, 2 * wk + T, lane);
-          kf[T] = LinTile<K>::cols(ks, kb, 2 * wk + T, lane);
+          yf[T] = LinTile<K>::cols(qs, kcb, kb, 2 * wk + T);
+          kf[T] = LinTile<K>::cols(ks, kcb, kb, 2 * wk + T);
           split(yf[T], hi[T], lo[T]);
         }
 #pragma unroll
         for (int tt = 0; tt < 2 * kb + 2; ++tt) {
-          const u16x8 pf = LinTile<64>::cols16(dps, kb, tt, lane);
+          const u16x8 pf = LinTile<64>::cols16(dps, LinTile<64>::col16_base(tt, lane), kb);
 #pragma unroll
           for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(yf[T], pf, X[tt][T]);
         }
 #pragma unroll
         for (int tt = 2 * kb; tt < 4; ++tt) {
-          const u16x8 pf = LinTile<64>::rows(dps, tt, kb, lane);
+          const u16x8 pf = LinTile<64>::rows(dps, pb, tt, kb);
 #pragma unroll
           for (int T = 0; T < 2; ++T) Y[tt][T] = mfma16(kf[T], pf, Y[tt][T]);
         }
 #pragma unroll
         for (int t = 0; t < V / 16; ++t) {
-          const u16x8 f = LinTile<V>::cols(os, kb, t, lane);
+          const u16x8 f = LinTile<V>::cols(os, vcb, kb, t);
 #pragma unroll
           for (int T = 0; T < 2; ++T) {
             ST[t][T] = mfma16(f, hi[T], ST[t][T]);
