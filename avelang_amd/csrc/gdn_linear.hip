@@ -79,12 +79,12 @@ __global__ __launch_bounds__(1024) void lin_table_kernel(const int32_t* cu, LinS
   for (int i = seg0 + tid; i < nseg; i += 1024) table[i] = LinSeg{0, 0, 0, -1, 0, 0};
 }
 
-// A wave's 16 columns of a state [K][V] as accumulators: tile t's lane holds
-// rows rho_row(t, 4 grp + r) of column 16 w + r16.
+// 16 columns (ct) of a state [K][V] as accumulators: tile t's lane holds rows
+// rho_row(t, 4 grp + r) of column 16 ct + r16.
 template <int K, int V>
-__device__ __forceinline__ void lin_load_state(f32x4 (&S)[K / 16], const float* p, int w, int lane) {
+__device__ __forceinline__ void lin_load_state(f32x4 (&S)[K / 16], const float* p, int ct, int lane) {
   const __amdgpu_buffer_rsrc_t rs = lin_state(p, K * V);
-  const int at = (8 * (lane / 16) * V + 16 * w + lane % 16) * 4;
+  const int at = (8 * (lane / 16) * V + 16 * ct + lane % 16) * 4;
 #pragma unroll
   for (int t = 0; t < K / 16; ++t)
 #pragma unroll
@@ -93,9 +93,9 @@ __device__ __forceinline__ void lin_load_state(f32x4 (&S)[K / 16], const float* 
           rs, at, (32 * (t >> 1) + 4 * (t & 1) + r) * V * 4, 0));
 }
 template <int K, int V>
-__device__ __forceinline__ void lin_store_state(const f32x4 (&S)[K / 16], float* p, int w, int lane) {
+__device__ __forceinline__ void lin_store_state(const f32x4 (&S)[K / 16], float* p, int ct, int lane) {
   const __amdgpu_buffer_rsrc_t rs = lin_state(p, K * V);
-  const int at = (8 * (lane / 16) * V + 16 * w + lane % 16) * 4;
+  const int at = (8 * (lane / 16) * V + 16 * ct + lane % 16) * 4;
 #pragma unroll
   for (int t = 0; t < K / 16; ++t)
 #pragma unroll
@@ -108,13 +108,13 @@ __device__ __forceinline__ void lin_store_state(const f32x4 (&S)[K / 16], float*
 // Contribution of a segment to the state after it: sum over its chunks of
 // X^T (f Y) with x = k, y = v, f = e^R; or (REV) to the gradient of the state
 // before it, chunks last to first, x = q, y = dO, f = scale e^G.  A wave owns
-// 16 columns of Y and all rows of the state.
-template <int K, int V, bool REV>
-__global__ __launch_bounds__(4 * V, 4) void lin_segment_kernel(
+// 16 CT columns of Y and all rows of the state.
+template <int K, int V, int CT, bool REV>
+__global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_segment_kernel(
     const uint16_t* __restrict__ x, int x_row, const uint16_t* __restrict__ y, int y_row,
     LinDecay dec, LinGrid grid, int Hqk, int Hv, float scale, float* __restrict__ segs,
     float* __restrict__ decay) {
-  constexpr int NT = 4 * V;
+  constexpr int NT = 4 * V / CT;
   __shared__ __align__(16) char xs[LinTile<K>::BYTES];
   __shared__ __align__(16) char ys[LinTile<V>::BYTES];
   __shared__ __align__(16) float fac[64];
@@ -128,9 +128,11 @@ __global__ __launch_bounds__(4 * V, 4) void lin_segment_kernel(
   const int r16 = lane % 16, grp = lane / 16;
   const int nc = (sg.ntok + kChunk - 1) / kChunk;
 
-  f32x4 S[K / 16];
+  f32x4 S[CT][K / 16];
 #pragma unroll
-  for (int t = 0; t < K / 16; ++t) S[t] = zero4();
+  for (int T = 0; T < CT; ++T)
+#pragma unroll
+    for (int t = 0; t < K / 16; ++t) S[T][t] = zero4();
   LinStage<K, NT> sx;
   LinStage<V, NT> sy;
   LinGates lg;
@@ -146,7 +148,7 @@ __global__ __launch_bounds__(4 * V, 4) void lin_segment_kernel(
     sy.load(y + t * y_row + h * V, y_row, min(n, 64), yf);
   };
   const int c0 = REV ? nc - 1 : 0, step = REV ? -1 : 1;
-  int xb = LinTile<K>::col_base(lane), yb = LinTile<V>::col16_base(w, lane);
+  int xb = LinTile<K>::col_base(lane), yb = LinTile<V>::col16_base(CT * w, lane);
   load(c0);
   for (int i = 0; i < nc; ++i) {
     hide(xb);
@@ -169,21 +171,29 @@ __global__ __launch_bounds__(4 * V, 4) void lin_segment_kernel(
     load(c0 + (i + 1) * step);
     const float eC = __expf(tot);
 #pragma unroll
-    for (int t = 0; t < K / 16; ++t) S[t] *= eC;
+    for (int T = 0; T < CT; ++T)
+#pragma unroll
+      for (int t = 0; t < K / 16; ++t) S[T][t] *= eC;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      u16x8 hi, lo;
-      lin_split(LinTile<V>::cols16(ys, yb, kb), fac + 32 * kb + 8 * grp, hi, lo);
+      u16x8 hi[CT], lo[CT];
+#pragma unroll
+      for (int T = 0; T < CT; ++T)
+        lin_split(LinTile<V>::cols16(ys, yb ^ (32 * T), kb), fac + 32 * kb + 8 * grp, hi[T], lo[T]);
 #pragma unroll
       for (int t = 0; t < K / 16; ++t) {
         const u16x8 a = LinTile<K>::cols(xs, xb, kb, t);
-        S[t] = mfma16(a, hi, S[t]);
-        S[t] = mfma16(a, lo, S[t]);
+#pragma unroll
+        for (int T = 0; T < CT; ++T) S[T][t] = mfma16(a, hi[T], S[T][t]);
+#pragma unroll
+        for (int T = 0; T < CT; ++T) S[T][t] = mfma16(a, lo[T], S[T][t]);
       }
     }
     __syncthreads();
   }
-  lin_store_state<K, V>(S, segs + ((size_t)sid * Hv + h) * K * V, w, lane);
+#pragma unroll
+  for (int T = 0; T < CT; ++T)
+    lin_store_state<K, V>(S[T], segs + ((size_t)sid * Hv + h) * K * V, CT * w + T, lane);
   if (tid == 0) decay[(size_t)sid * Hv + h] = __expf(gsum);
 }
 
@@ -232,16 +242,16 @@ __global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int
 
 // ------------------------------------------------------------------ walk ----
 // One segment and v-head from its start state, chunk by chunk: o (OUT), the
-// state at every chunk's start (SAVE), ht.  A wave owns 16 columns of V, all
+// state at every chunk's start (SAVE), ht.  A wave owns 16 CT columns of V, all
 // of the state's rows for them in its accumulators, whose layout is that of
 // the operand with which S^T q is formed: the state never leaves the registers.
-template <int K, int V, bool OUT, bool SAVE>
-__global__ __launch_bounds__(4 * V, 4) void lin_walk_kernel(
+template <int K, int V, int CT, bool OUT, bool SAVE>
+__global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k,
     const uint16_t* __restrict__ v, TokenStride ts, LinDecay dec, LinGrid grid, int Hqk, int Hv,
     float scale, const float* h0, float* ht, const float* __restrict__ segs,
     uint16_t* __restrict__ o, u16x4* __restrict__ states) {
-  constexpr int NT = 4 * V, NW = V / 16;
+  constexpr int NT = 4 * V / CT, NW = V / 16 / CT;
   __shared__ __align__(16) char qs[LinTile<K>::BYTES];
   __shared__ __align__(16) char ks[LinTile<K>::BYTES];
   __shared__ __align__(16) char vs[LinTile<V>::BYTES];
@@ -264,10 +274,11 @@ __global__ __launch_bounds__(4 * V, 4) void lin_walk_kernel(
   if (sg.seq < 0) return;
   const int nc = (sg.ntok + kChunk - 1) / kChunk;
 
-  f32x4 S[K / 16];   // rows rho_row(t, 4 grp + r), column 16 w + r16
+  f32x4 S[CT][K / 16];   // rows rho_row(t, 4 grp + r), column 16 (CT w + T) + r16
   const float* src = sg.first ? (h0 ? h0 + ((size_t)sg.seq * Hv + h) * K * V : nullptr)
                               : segs + ((size_t)sid * Hv + h) * K * V;
-  lin_load_state<K, V>(S, src, w, lane);
+#pragma unroll
+  for (int T = 0; T < CT; ++T) lin_load_state<K, V>(S[T], src, CT * w + T, lane);
 
   LinStage<K, NT> sq, sk;
   LinStage<V, NT> sv;
@@ -276,7 +287,7 @@ __global__ __launch_bounds__(4 * V, 4) void lin_walk_kernel(
   int qf = LinStage<K, NT>::from(ts.q, tid), kf = LinStage<K, NT>::from(ts.k, tid);
   int vr = LinStage<V, NT>::from(ts.v, tid);
   const int kt = LinStage<K, NT>::at(tid, 0), vt = LinStage<V, NT>::at(tid, 0);
-  int oat = (r16 * Hv * V + 16 * w + 4 * grp) * 2;   // bytes into the chunk's rows of o
+  int oat = (r16 * Hv * V + 16 * CT * w + 4 * grp) * 2;   // bytes into the chunk's rows of o
   auto load = [&](int c) {
     const int n = c < nc ? sg.ntok - c * kChunk : 0;
     const size_t t = n > 0 ? (size_t)sg.tok0 + c * kChunk : 0;
@@ -293,8 +304,23 @@ __global__ __launch_bounds__(4 * V, 4) void lin_walk_kernel(
     }
   }
   int rb = LinTile<K>::row_base(lane), kcb = LinTile<K>::col_base(lane);
-  int vb = LinTile<V>::col16_base(w, lane), pb = LinTile<64>::row_base(lane);
+  int vb = LinTile<V>::col16_base(CT * w, lane), pb = LinTile<64>::row_base(lane);
   int pw = LinTile<64>::off(r16, grp >> 1) + (grp & 1) * 8;
+  // o of a chunk leaves ahead of the loads issued in the next: the wait for
+  // loads counts stores too, and behind them it would wait out every store
+  // (64 packed prompts: 1091 us so)
+  u32x2p held[4][CT];
+  auto store_o = [&](int c) {
+    // (stores past the segment's last token are dropped)
+    const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(
+        o + ((size_t)(sg.tok0 + c * kChunk) * Hv + h) * V, 0,
+        ((min(sg.ntok - c * kChunk, 64) - 1) * Hv + 1) * V * 2, kBufferFlags);
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int T = 0; T < CT; ++T)
+        __builtin_amdgcn_raw_buffer_store_b64(held[tt][T], ro, oat + (tt * 16 * Hv * V + 16 * T) * 2, 0, 0);
+  };
   load(0);
   for (int c = 0; c < nc; ++c) {
     // (nothing derived from these is kept from one chunk for the next)
@@ -324,6 +350,7 @@ __global__ __launch_bounds__(4 * V, 4) void lin_walk_kernel(
       }
     }
     __syncthreads();
+    if (OUT && c > 0) store_o(c - 1);
     load(c + 1);
 
     if (OUT) {
@@ -348,71 +375,100 @@ __global__ __launch_bounds__(4 * V, 4) void lin_walk_kernel(
       }
     }
     // the state as bf16 operands, by rows of 32 keys
-    f32x4 O[4];   // columns 16 w + 4 grp + r of token 16 tt + r16
+    f32x4 O[4][CT];   // columns 16 (CT w + T) + 4 grp + r of token 16 tt + r16
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt) O[tt] = zero4();
+    for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+      for (int T = 0; T < CT; ++T) O[tt][T] = zero4();
 #pragma unroll
     for (int b = 0; b < K / 32; ++b) {
-      const u16x8 sb = cat8(f2bf4(S[2 * b]), f2bf4(S[2 * b + 1]));
+      u16x8 sb[CT];
+#pragma unroll
+      for (int T = 0; T < CT; ++T) sb[T] = cat8(f2bf4(S[T][2 * b]), f2bf4(S[T][2 * b + 1]));
       if (OUT) {
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt) O[tt] = mfma16(sb, LinTile<K>::rows(qs, rb, tt, b), O[tt]);
+        for (int tt = 0; tt < 4; ++tt) {
+          const u16x8 f = LinTile<K>::rows(qs, rb, tt, b);
+#pragma unroll
+          for (int T = 0; T < CT; ++T) O[tt][T] = mfma16(sb[T], f, O[tt][T]);
+        }
       }
       if (SAVE) {
         // transposed through a product with a selection matrix (exact): lane
-        // (r16, grp) gets key rho_row(t, r16), values 16 w + 4 grp + r, which
+        // (r16, grp) gets key rho_row(t, r16), values 16 ct + 4 grp + r, which
         // are half a lane's share of the backward's fragment
-        u16x4* dst = states + ((size_t)(sg.chunk0 + c) * Hv + h) * (K / 16) * (V / 32) * 128 +
-                     (w >> 1) * 128 + (r16 + 16 * (2 * (w & 1) + (grp >> 1))) * 2 + (grp & 1);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          u16x8 sel;
+        for (int T = 0; T < CT; ++T) {
+          const int ct = CT * w + T;
+          u16x4* dst = states + ((size_t)(sg.chunk0 + c) * Hv + h) * (K / 16) * (V / 32) * 128 +
+                       (ct >> 1) * 128 + (r16 + 16 * (2 * (ct & 1) + (grp >> 1))) * 2 + (grp & 1);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            sel[i] = grp == r16 >> 2 && i == 4 * e + (r16 & 3) ? 0x3F80 : 0;
-          dst[(2 * b + e) * (V / 32) * 128] = f2bf4(mfma16(sb, sel, zero4()));
+          for (int e = 0; e < 2; ++e) {
+            u16x8 sel;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              sel[i] = grp == r16 >> 2 && i == 4 * e + (r16 & 3) ? 0x3F80 : 0;
+            dst[(2 * b + e) * (V / 32) * 128] = f2bf4(mfma16(sb[T], sel, zero4()));
+          }
         }
       }
     }
     if (OUT) {
 #pragma unroll
-      for (int tt = 0; tt < 4; ++tt) O[tt] *= sQ[16 * tt + r16];
+      for (int tt = 0; tt < 4; ++tt) {
+        const float eq = sQ[16 * tt + r16];
+#pragma unroll
+        for (int T = 0; T < CT; ++T) O[tt][T] *= eq;
+      }
       __syncthreads();   // P
     }
     const float eC = exp2_(sG[63]);
 #pragma unroll
-    for (int t = 0; t < K / 16; ++t) S[t] *= eC;
+    for (int T = 0; T < CT; ++T)
+#pragma unroll
+      for (int t = 0; t < K / 16; ++t) S[T][t] *= eC;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      const u16x8 vf = LinTile<V>::cols16(vs, vb, kb);
+      u16x8 vf[CT], hi[CT], lo[CT];
+#pragma unroll
+      for (int T = 0; T < CT; ++T) {
+        vf[T] = LinTile<V>::cols16(vs, vb ^ (32 * T), kb);
+        lin_split(vf[T], sK + 32 * kb + 8 * grp, hi[T], lo[T]);
+      }
       if (OUT) {
 #pragma unroll
-        for (int tt = 2 * kb; tt < 4; ++tt)
-          O[tt] = mfma16(vf, LinTile<64>::rows(ps, pb, tt, kb), O[tt]);
+        for (int tt = 2 * kb; tt < 4; ++tt) {
+          const u16x8 f = LinTile<64>::rows(ps, pb, tt, kb);
+#pragma unroll
+          for (int T = 0; T < CT; ++T) O[tt][T] = mfma16(vf[T], f, O[tt][T]);
+        }
       }
-      u16x8 hi, lo;
-      lin_split(vf, sK + 32 * kb + 8 * grp, hi, lo);
 #pragma unroll
       for (int t = 0; t < K / 16; ++t) {
-        const u16x8 a = LinTile<K>::cols(ks, kcb, kb, t);
-        S[t] = mfma16(a, hi, S[t]);
-        S[t] = mfma16(a, lo, S[t]);
+        const u16x8 f = LinTile<K>::cols(ks, kcb, kb, t);
+#pragma unroll
+        for (int T = 0; T < CT; ++T) S[T][t] = mfma16(f, hi[T], S[T][t]);
+#pragma unroll
+        for (int T = 0; T < CT; ++T) S[T][t] = mfma16(f, lo[T], S[T][t]);
       }
     }
     if (OUT) {
-      // (stores past the segment's last token are dropped)
-      const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(
-          o + ((size_t)(sg.tok0 + c * kChunk) * Hv + h) * V, 0,
-          ((min(sg.ntok - c * kChunk, 64) - 1) * Hv + 1) * V * 2, kBufferFlags);
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt)
-        __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2p, f2bf4(O[tt])), ro,
-                                              oat + tt * 16 * Hv * V * 2, 0, 0);
+#pragma unroll
+        for (int T = 0; T < CT; ++T) held[tt][T] = __builtin_bit_cast(u32x2p, f2bf4(O[tt][T]));
     }
     __syncthreads();
   }
-  if (ht && sg.last) lin_store_state<K, V>(S, ht + ((size_t)sg.seq * Hv + h) * K * V, w, lane);
+  if (OUT && nc > 0) store_o(nc - 1);
+  if (ht && sg.last) {
+#pragma unroll
+    for (int T = 0; T < CT; ++T)
+      lin_store_state<K, V>(S[T], ht + ((size_t)sg.seq * Hv + h) * K * V, CT * w + T, lane);
+  }
 }
+
+constexpr int kColTiles = 2;
 
 // ------------------------------------------------------------------ host ----
 // Chunks per segment: as many as spread all chunks over two workgroups per CU
@@ -481,11 +537,11 @@ void launch_lin_segments(const uint16_t* x, int x_row, const uint16_t* y, int y_
                          hipStream_t st) {
   const dim3 items(xcd_grid((long long)g.nseg * Hv)), elems((unsigned)(g.N * Hv * (K * V / 256)));
   if (reverse) {
-    hipLaunchKernelGGL((lin_segment_kernel<K, V, true>), items, dim3(4 * V), 0, st, x, x_row, y,
+    hipLaunchKernelGGL((lin_segment_kernel<K, V, kColTiles, true>), items, dim3(4 * V / kColTiles), 0, st, x, x_row, y,
                        y_row, d, g, Hqk, Hv, scale, segs, decay);
     hipLaunchKernelGGL(lin_join_kernel<true>, elems, dim3(256), 0, st, g, Hv, K * V, edge, segs, decay);
   } else {
-    hipLaunchKernelGGL((lin_segment_kernel<K, V, false>), items, dim3(4 * V), 0, st, x, x_row, y,
+    hipLaunchKernelGGL((lin_segment_kernel<K, V, kColTiles, false>), items, dim3(4 * V / kColTiles), 0, st, x, x_row, y,
                        y_row, d, g, Hqk, Hv, scale, segs, decay);
     hipLaunchKernelGGL(lin_join_kernel<false>, elems, dim3(256), 0, st, g, Hv, K * V, edge, segs, decay);
   }
@@ -507,7 +563,7 @@ void launch_walk(const uint16_t* q, const uint16_t* k, const uint16_t* v, TokenS
     launch_lin_segments<K, V>(k, ts.k, v, ts.v, d, g, Hqk, Hv, 1.f, false, h0, segs, decay, st);
   const dim3 items(xcd_grid((long long)g.nseg * Hv));
 #define GDN_LW(OUT, SAVE)                                                                      \
-  hipLaunchKernelGGL((lin_walk_kernel<K, V, OUT, SAVE>), items, dim3(4 * V), 0, st, q, k, v, ts, \
+  hipLaunchKernelGGL((lin_walk_kernel<K, V, kColTiles, OUT, SAVE>), items, dim3(4 * V / kColTiles), 0, st, q, k, v, ts, \
                      d, g, Hqk, Hv, scale, h0, ht, segs, o, states)
   if (o && states) GDN_LW(true, true);
   else if (o) GDN_LW(true, false);
