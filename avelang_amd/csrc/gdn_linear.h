@@ -20,8 +20,11 @@ struct LinGrid {
   const LinSeg* table;      // [nseg], NULL: equal lengths
   const int32_t* soff;      // [N + 1] first segment of each sequence (with table)
   const int32_t* status;    // != 0: a cu_seqlens violation (with table)
+  const int32_t* order;     // [nseg] segments, longest first (with table)
+  const int32_t* joins;     // [1 + nlong] how many sequences have several segments, which (table)
   int T, L, nps;            // tokens and segments per sequence (without table), chunks per segment
   int nseg;                 // segments at most
+  int nlong;                // sequences of several segments at most
   int N, total;             // sequences, tokens of all
 };
 
@@ -207,19 +210,28 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t lin_state(const float* p, int 
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Workgroup -> work item so that neighbouring items run on the same XCD
-// (workgroups go round the 8 of them) and share its L2.  The grid is
-// xcd_grid(n); items at and past n are for nobody.
-inline unsigned xcd_grid(long long n) { return (unsigned)((n + 7) / 8 * 8); }
-__device__ __forceinline__ int xcd_item() {
-  return (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
+// Workgroup -> (segment, v-head): the v-heads of a qk-head run on one XCD
+// (workgroups go round the 8 of them) one after another and share q and k in
+// its L2; a segment's qk-heads, and so segments of different lengths, are
+// spread over the XCDs.  Packed segments start longest first.  The grid is
+// lin_items(...) workgroups; false: none for this one.
+inline unsigned lin_items(int nseg, int Hqk, int Hv) {
+  return (unsigned)(((long long)nseg * Hqk + 7) / 8 * 8 * (Hv / Hqk));
+}
+__device__ __forceinline__ bool lin_item(const LinGrid& g, int nseg, int Hqk, int Hv, int& s,
+                                         int& h) {
+  const int rep = Hv / Hqk, i = blockIdx.x / 8, u = i / rep * 8 + blockIdx.x % 8;
+  s = u / Hqk;
+  h = u % Hqk * rep + i % rep;
+  return s < nseg;
 }
 
 // Host: how a call is cut (byte offsets into the workspace).
 struct LinPlan {
   int L, nps, nseg;          // as LinGrid
   long long chunks;          // chunks of all sequences at most (chunk-start states)
-  size_t table, soff, status, segs, decay, total;
+  int nlong;                 // sequences of several segments at most (0: no join)
+  size_t table, soff, status, order, joins, segs, decay, total;
   // backward
   size_t part;               // fp32 partial dq, dk per v-head (Hv > Hqk)
   size_t dgtok;              // fp32 dg per token and v-head (one decay per head)

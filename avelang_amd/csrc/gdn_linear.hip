@@ -27,15 +27,24 @@ namespace gdn {
 // each sequence, and the check of the cu_seqlens contract (on a violation
 // every sequence is one empty segment).
 __global__ __launch_bounds__(1024) void lin_table_kernel(const int32_t* cu, LinSeg* table,
-                                                         int32_t* soff, int32_t* status, int N,
-                                                         int total, int L, int nseg) {
-  __shared__ int wsum[2][16];
+                                                         int32_t* soff, int32_t* status,
+                                                         int32_t* order, int32_t* joins, int N,
+                                                         int total, int L, int nseg, int nlong) {
+  constexpr int BINS = 256;   // of lengths, for the order
+  __shared__ int wsum[2][16], bin[BINS], nj;
   const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
   int bad = 0;
   for (int n = tid; n < N; n += 1024) bad |= cu[n + 1] < cu[n];
   if (tid == 0) bad |= cu[0] != 0 || cu[N] != total;
   bad = __syncthreads_or(bad);
-  if (tid == 0) *status = bad;
+  if (tid == 0) {
+    *status = bad;
+    nj = 0;
+  }
+  if (tid < BINS) bin[tid] = 0;
+  auto bin_of = [&](int ntok) {   // longer ones first
+    return BINS - 1 - (int)((long long)(ntok + kChunk - 1) / kChunk * (BINS - 1) / L);
+  };
   int seg0 = 0, chunk0 = 0;   // of this round's first sequence
   for (int n0 = 0; n0 < N; n0 += 1024) {
     const int n = n0 + tid;
@@ -70,13 +79,35 @@ __global__ __launch_bounds__(1024) void lin_table_kernel(const int32_t* cu, LinS
     sb += b - nc;
     if (n < N) {
       soff[n] = sa;
-      for (int i = 0; i < ns && sa + i < nseg; ++i)
-        table[sa + i] = LinSeg{s + i * L * kChunk, min(len - i * L * kChunk, L * kChunk),
-                               sb + i * L, n, i == 0, i == ns - 1};
+      for (int i = 0; i < ns && sa + i < nseg; ++i) {
+        const int ntok = min(len - i * L * kChunk, L * kChunk);
+        table[sa + i] = LinSeg{s + i * L * kChunk, ntok, sb + i * L, n, i == 0, i == ns - 1};
+        atomicAdd(&bin[bin_of(ntok)], 1);
+      }
+      if (ns > 1) {
+        const int j = atomicAdd(&nj, 1);
+        if (j < nlong) joins[1 + j] = n;
+      }
     }
   }
-  if (tid == 0) soff[N] = seg0;
-  for (int i = seg0 + tid; i < nseg; i += 1024) table[i] = LinSeg{0, 0, 0, -1, 0, 0};
+  for (int i = seg0 + tid; i < nseg; i += 1024) {
+    table[i] = LinSeg{0, 0, 0, -1, 0, 0};
+    order[i] = i;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    soff[N] = seg0;
+    if (nlong > 0) joins[0] = min(nj, nlong);
+    int at = 0;
+    for (int i = 0; i < BINS; ++i) {
+      const int x = bin[i];
+      bin[i] = at;
+      at += x;
+    }
+  }
+  __syncthreads();
+  // (which of equal lengths comes first changes when a segment runs, nothing else)
+  for (int i = tid; i < min(seg0, nseg); i += 1024) order[atomicAdd(&bin[bin_of(table[i].ntok)], 1)] = i;
 }
 
 // 16 columns (ct) of a state [K][V] as accumulators: tile t's lane holds rows
@@ -119,9 +150,16 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_segment_kernel(
   __shared__ __align__(16) char ys[LinTile<V>::BYTES];
   __shared__ __align__(16) float fac[64];
   __shared__ float tot;
-  const int item = xcd_item();
-  if (item >= grid.nseg * Hv) return;
-  const int sid = item / Hv, h = item % Hv, hq = h / (Hv / Hqk);
+  int sid, h;
+  if (grid.table) {
+    if (!lin_item(grid, grid.nseg, Hqk, Hv, sid, h)) return;
+    sid = grid.order[sid];
+  } else {   // every segment but one of each sequence
+    const int per = grid.nps - 1;
+    if (!lin_item(grid, grid.N * per, Hqk, Hv, sid, h)) return;
+    sid = sid / per * grid.nps + sid % per + (REV ? 1 : 0);
+  }
+  const int hq = h / (Hv / Hqk);
   const LinSeg sg = lin_seg(grid, sid);
   if (sg.seq < 0 || (REV ? sg.first : sg.last)) return;
   const int tid = threadIdx.x, lane = tid % 64, w = wave_index();
@@ -206,17 +244,18 @@ __global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int
                                                        float* __restrict__ segs,
                                                        const float* __restrict__ decay) {
   const int per = KV / 256;
-  const int n = blockIdx.x / (Hv * per), h = blockIdx.x / per % Hv;
-  const int e = blockIdx.x % per * 256 + threadIdx.x;
+  int n = blockIdx.x / (Hv * per);
+  const int h = blockIdx.x / per % Hv, e = blockIdx.x % per * 256 + threadIdx.x;
   int s0, s1;
   if (grid.table) {
+    if (n >= grid.joins[0]) return;
+    n = grid.joins[1 + n];
     s0 = grid.soff[n];
     s1 = grid.soff[n + 1];
   } else {
     s0 = n * grid.nps;
     s1 = s0 + grid.nps;
   }
-  if (s1 - s0 < 2) return;
   float S = edge ? edge[((size_t)n * Hv + h) * KV + e] : 0.f;
   const int first = REV ? s1 - 1 : s0, step = REV ? -1 : 1, cnt = s1 - s0 - 1;
   constexpr int U = 8;   // loads in flight
@@ -259,7 +298,6 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
   __shared__ __align__(16) float sG[64], sQ[64], sK[64];   // G log2(e), scale e^G, e^R
   const int tid = threadIdx.x, lane = tid % 64, w = wave_index();
   const int r16 = lane % 16, grp = lane / 16;
-  const int item = xcd_item();
   if (grid.table && *grid.status) {
     // a cu_seqlens violation: no sequence has a token, o is zero
     if (OUT) {
@@ -268,8 +306,10 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
         reinterpret_cast<u32x4*>(o)[i] = u32x4{0, 0, 0, 0};
     }
   }
-  if (item >= grid.nseg * Hv) return;
-  const int sid = item / Hv, h = item % Hv, hq = h / (Hv / Hqk);
+  int sid, h;
+  if (!lin_item(grid, grid.nseg, Hqk, Hv, sid, h)) return;
+  if (grid.table) sid = grid.order[sid];
+  const int hq = h / (Hv / Hqk);
   const LinSeg sg = lin_seg(grid, sid);
   if (sg.seq < 0) return;
   const int nc = (sg.ntok + kChunk - 1) / kChunk;
@@ -485,6 +525,8 @@ LinPlan lin_plan(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu
   p.L = (int)L;
   p.nps = (int)(per > 0 ? (per + L - 1) / L : 1);
   p.nseg = (int)(has_cu ? N + tokens / (L * kChunk) : (long long)N * p.nps);
+  // a sequence of several segments has more than L chunks
+  p.nlong = (int)(p.nps < 2 ? 0 : has_cu ? tokens / (L * kChunk) : N);
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t r = at;
@@ -495,8 +537,10 @@ LinPlan lin_plan(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu
     p.table = take((size_t)p.nseg * sizeof(LinSeg));
     p.soff = take(((size_t)N + 1) * 4);
     p.status = take(4);
+    p.order = take((size_t)p.nseg * 4);
+    p.joins = take(((size_t)p.nlong + 1) * 4);
   }
-  if (p.nps > 1) {
+  if (p.nlong > 0) {
     p.segs = take((size_t)p.nseg * Hv * K * V * 4);
     p.decay = take((size_t)p.nseg * Hv * 4);
   }
@@ -512,11 +556,14 @@ LinGrid lin_grid(const LinPlan& p, unsigned char* ws, int T, int N, int total, b
     g.table = reinterpret_cast<const LinSeg*>(ws + p.table);
     g.soff = reinterpret_cast<const int32_t*>(ws + p.soff);
     g.status = reinterpret_cast<const int32_t*>(ws + p.status);
+    g.order = reinterpret_cast<const int32_t*>(ws + p.order);
+    g.joins = reinterpret_cast<const int32_t*>(ws + p.joins);
   }
   g.T = T;
   g.L = p.L;
   g.nps = p.nps;
   g.nseg = p.nseg;
+  g.nlong = p.nlong;
   g.N = N;
   g.total = total;
   return g;
@@ -527,7 +574,9 @@ void launch_lin_table(const int32_t* cu, const LinPlan& p, unsigned char* ws, in
   hipLaunchKernelGGL(lin_table_kernel, dim3(1), dim3(1024), 0, st, cu,
                      reinterpret_cast<LinSeg*>(ws + p.table),
                      reinterpret_cast<int32_t*>(ws + p.soff),
-                     reinterpret_cast<int32_t*>(ws + p.status), N, total, p.L, p.nseg);
+                     reinterpret_cast<int32_t*>(ws + p.status),
+                     reinterpret_cast<int32_t*>(ws + p.order),
+                     reinterpret_cast<int32_t*>(ws + p.joins), N, total, p.L, p.nseg, p.nlong);
 }
 
 template <int K, int V>
@@ -535,7 +584,8 @@ void launch_lin_segments(const uint16_t* x, int x_row, const uint16_t* y, int y_
                          const LinDecay& d, const LinGrid& g, int Hqk, int Hv, float scale,
                          bool reverse, const float* edge, float* segs, float* decay,
                          hipStream_t st) {
-  const dim3 items(xcd_grid((long long)g.nseg * Hv)), elems((unsigned)(g.N * Hv * (K * V / 256)));
+  const dim3 items(lin_items(g.table ? g.nseg : g.N * (g.nps - 1), Hqk, Hv));
+  const dim3 elems((unsigned)(g.nlong * Hv * (K * V / 256)));
   if (reverse) {
     hipLaunchKernelGGL((lin_segment_kernel<K, V, kColTiles, true>), items, dim3(4 * V / kColTiles), 0, st, x, x_row, y,
                        y_row, d, g, Hqk, Hv, scale, segs, decay);
@@ -559,9 +609,9 @@ void launch_walk(const uint16_t* q, const uint16_t* k, const uint16_t* v, TokenS
                  const LinDecay& d, const LinGrid& g, int Hqk, int Hv, float scale,
                  const float* h0, float* ht, float* segs, float* decay, uint16_t* o, u16x4* states,
                  hipStream_t st) {
-  if (g.nps > 1)
+  if (g.nlong > 0)
     launch_lin_segments<K, V>(k, ts.k, v, ts.v, d, g, Hqk, Hv, 1.f, false, h0, segs, decay, st);
-  const dim3 items(xcd_grid((long long)g.nseg * Hv));
+  const dim3 items(lin_items(g.nseg, Hqk, Hv));
 #define GDN_LW(OUT, SAVE)                                                                      \
   hipLaunchKernelGGL((lin_walk_kernel<K, V, kColTiles, OUT, SAVE>), items, dim3(4 * V / kColTiles), 0, st, q, k, v, ts, \
                      d, g, Hqk, Hv, scale, h0, ht, segs, o, states)

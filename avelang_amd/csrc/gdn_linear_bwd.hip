@@ -56,7 +56,6 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
   __shared__ float csum[NK];
   const int tid = threadIdx.x, lane = tid % 64, w = wave_index();
   const int r16 = lane % 16, grp = lane / 16;
-  const int item = xcd_item();
   if (a.grid.table && *a.grid.status) {
     // a cu_seqlens violation: every gradient over the tokens is zero
     const size_t nv = (size_t)a.grid.total * a.Hv * V / 8, nk = (size_t)a.grid.total * a.Hqk * K / 8;
@@ -69,8 +68,10 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
     }
     for (size_t i = i0; i < ng; i += st) a.dg[i] = 0.f;
   }
-  if (item >= a.grid.nseg * a.Hv) return;
-  const int sid = item / a.Hv, h = item % a.Hv, hq = h / (a.Hv / a.Hqk);
+  int sid, h;
+  if (!lin_item(a.grid, a.grid.nseg, a.Hqk, a.Hv, sid, h)) return;
+  if (a.grid.table) sid = a.grid.order[sid];
+  const int hq = h / (a.Hv / a.Hqk);
   const LinSeg sg = lin_seg(a.grid, sid);
   if (sg.seq < 0) return;
   const int nc = (sg.ntok + kChunk - 1) / kChunk;
@@ -441,10 +442,10 @@ __global__ __launch_bounds__(1024) void lin_head_sum_kernel(const float* __restr
 namespace {
 template <int K, int V>
 void launch_grad(const LinBwdArgs& a, float* segs, float* decay, hipStream_t st) {
-  if (a.grid.nps > 1)
+  if (a.grid.nlong > 0)
     launch_lin_segments<K, V>(a.q, a.ts.q, a.dO, a.Hv * V, a.dec, a.grid, a.Hqk, a.Hv, a.scale,
                               true, a.dht, segs, decay, st);
-  hipLaunchKernelGGL((lin_grad_kernel<K, V>), dim3(xcd_grid((long long)a.grid.nseg * a.Hv)),
+  hipLaunchKernelGGL((lin_grad_kernel<K, V>), dim3(lin_items(a.grid.nseg, a.Hqk, a.Hv)),
                      dim3(2 * (K + V)), 0, st, a);
 }
 }  // namespace
