@@ -38,66 +38,58 @@ struct LinBwdArgs {
   float* dg;           // [tokens][Hv]
 };
 
+template <int K, int V>
+struct LinGradLds {
+  char qs[LinTile<K>::BYTES], ks[LinTile<K>::BYTES];
+  char vs[LinTile<V>::BYTES], os[LinTile<V>::BYTES];
+  char ps[LinTile<64>::BYTES], dps[LinTile<64>::BYTES];
+  float sG[64], sQ[64], sK[64];   // G log2(e), scale e^G, e^R
+  float rowM[4][64], colM[4][64], asum[K / 32][64], bsum[K / 32][64];
+  float csum[K / 32];
+};
+
 // A workgroup walks one segment of one v-head.  V / 32 waves own 32 columns
 // of D each (dv and dh0), K / 32 waves 32 columns of D^T (dk and dq, which
 // reduce over V, and with the saved states' fragments <S, D>): D is kept in
-// both orientations so that neither ever leaves the registers.
-template <int K, int V>
-__global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) {
+// both orientations so that neither ever leaves the registers.  This is one
+// wave's walk, VW: of the first kind.  Both kinds meet the same barriers.
+template <int K, int V, bool VW>
+__device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg& sg, int sid, int h,
+                                              int w, LinGradLds<K, V>& lds) {
   constexpr int NT = 2 * (K + V), NV = V / 32, NK = K / 32, NW = NV + NK;
-  __shared__ __align__(16) char qs[LinTile<K>::BYTES];
-  __shared__ __align__(16) char ks[LinTile<K>::BYTES];
-  __shared__ __align__(16) char vs[LinTile<V>::BYTES];
-  __shared__ __align__(16) char os[LinTile<V>::BYTES];
-  __shared__ __align__(16) char ps[LinTile<64>::BYTES];
-  __shared__ __align__(16) char dps[LinTile<64>::BYTES];
-  __shared__ __align__(16) float sG[64], sQ[64], sK[64];   // G log2(e), scale e^G, e^R
-  __shared__ __align__(16) float rowM[4][64], colM[4][64], asum[NK][64], bsum[NK][64];
-  __shared__ float csum[NK];
-  const int tid = threadIdx.x, lane = tid % 64, w = wave_index();
-  const int r16 = lane % 16, grp = lane / 16;
-  if (a.grid.table && *a.grid.status) {
-    // a cu_seqlens violation: every gradient over the tokens is zero
-    const size_t nv = (size_t)a.grid.total * a.Hv * V / 8, nk = (size_t)a.grid.total * a.Hqk * K / 8;
-    const size_t ng = (size_t)a.grid.total * a.Hv, st = (size_t)gridDim.x * NT;
-    const size_t i0 = (size_t)blockIdx.x * NT + tid;
-    for (size_t i = i0; i < nv; i += st) reinterpret_cast<u32x4*>(a.dv)[i] = u32x4{0, 0, 0, 0};
-    for (size_t i = i0; i < nk; i += st) {
-      reinterpret_cast<u32x4*>(a.dq)[i] = u32x4{0, 0, 0, 0};
-      reinterpret_cast<u32x4*>(a.dk)[i] = u32x4{0, 0, 0, 0};
-    }
-    for (size_t i = i0; i < ng; i += st) a.dg[i] = 0.f;
-  }
-  int sid, h;
-  if (!lin_item(a.grid, a.grid.nseg, a.Hqk, a.Hv, sid, h)) return;
-  if (a.grid.table) sid = a.grid.order[sid];
+  constexpr int NTILE = (VW ? K : V) / 16;
+  char *qs = lds.qs, *ks = lds.ks, *vs = lds.vs, *os = lds.os, *ps = lds.ps, *dps = lds.dps;
+  float *sG = lds.sG, *sQ = lds.sQ, *sK = lds.sK;
+  auto &rowM = lds.rowM, &colM = lds.colM;
+  auto &asum = lds.asum, &bsum = lds.bsum;
+  float* csum = lds.csum;
+  const int tid = threadIdx.x, lane = tid % 64;
   const int hq = h / (a.Hv / a.Hqk);
-  const LinSeg sg = lin_seg(a.grid, sid);
-  if (sg.seq < 0) return;
   const int nc = (sg.ntok + kChunk - 1) / kChunk;
-  const bool vwave = w < NV;
-  const int wk = vwave ? 0 : w - NV, wv = vwave ? w : 0;
+  const int wk = VW ? 0 : w - NV, wv = VW ? w : 0;   // the wave's 32 columns
 
-  // ST[t][T]: V waves D (key tile t, value tile T); key waves D^T (value tile t, key tile T)
-  constexpr int NTILE = (K > V ? K : V) / 16;
+  // ST[t][T]: D (key tile t, value tile T), or D^T (value tile t, key tile T)
   f32x4 ST[NTILE][2];
   const float* src = sg.last ? (a.dht ? a.dht + ((size_t)sg.seq * a.Hv + h) * K * V : nullptr)
                              : a.segs + ((size_t)sid * a.Hv + h) * K * V;
-  const __amdgpu_buffer_rsrc_t rst = __builtin_amdgcn_make_buffer_rsrc(
-      const_cast<float*>(src), 0, src ? K * V * 4 : 0, kBufferFlags);
-  const int c32 = 8 * (r16 >> 2) + (r16 & 3);   // + 4 T: the lane's column of 32
+  // a lane's part of the state's address, V waves: row 8 grp (+ the tile's and
+  // r), column of value tile T; key waves with rows and columns exchanged
+  auto state_at = [&](int lane, int T) {
+    const int r16 = lane % 16, grp = lane / 16, c = 8 * (r16 >> 2) + (r16 & 3) + 4 * T;
+    return (VW ? 8 * grp * V + 32 * wv + c : (32 * wk + c) * V + 8 * grp) * 4;
+  };
+  auto tile_at = [&](int t, int r) {
+    return (32 * (t >> 1) + 4 * (t & 1) + r) * (VW ? V : 1) * 4;
+  };
+  const __amdgpu_buffer_rsrc_t rst = lin_state(src, K * V);
 #pragma unroll
   for (int t = 0; t < NTILE; ++t)
 #pragma unroll
     for (int T = 0; T < 2; ++T)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int row = rho_row(t, 4 * grp + r), col = c32 + 4 * T;
-        // (a tile the wave does not have is read out of range: 0)
-        const int in = vwave ? (t < K / 16 ? row * V + 32 * wv + col : K * V)
-                             : (t < V / 16 ? (32 * wk + col) * V + row : K * V);
-        ST[t][T][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rst, in * 4, 0, 0));
-      }
+      for (int r = 0; r < 4; ++r)
+        ST[t][T][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+            rst, state_at(lane, T), tile_at(t, r), 0));
 
   LinStage<K, NT> sq, sk;
   LinStage<V, NT> sv, so;
@@ -126,18 +118,80 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
   __syncthreads();
   int krb = LinTile<K>::row_base(lane), vrb = LinTile<V>::row_base(lane);
   int kcb = LinTile<K>::col_base(lane), vcb = LinTile<V>::col_base(lane);
-  const int pb = LinTile<64>::row_base(lane);
+  int pb = LinTile<64>::row_base(lane);
+  int pcb = LinTile<64>::col16_base(0, lane);
+  int pw = LinTile<64>::off(lane % 16, lane / 32) + (lane / 16 & 1) * 8;
+  // the chunk's gradients leave ahead of the loads issued in the next one: the
+  // wait for loads counts stores too
+  f32x4 X[4][2], Y[4][2];   // dv; or dk and dq (by token tile)
+  auto store_grads = [&](int c) {
+    int ln = lane;
+    hide(ln);
+    const int r16 = ln % 16, grp = ln / 16;
+    const int n = min(sg.ntok - c * kChunk, 64);
+    const size_t tok = (size_t)sg.tok0 + c * kChunk;
+    // (stores past the segment's last token are dropped)
+    if constexpr (VW) {
+      const int row = a.Hv * V * 2, at = r16 * row + (32 * wv + 8 * grp) * 2;
+      const __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc(
+          a.dv + (tok * a.Hv + h) * V, 0, (n - 1) * row + V * 2, kBufferFlags);
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt)
+        __builtin_amdgcn_raw_buffer_store_b128(
+            __builtin_bit_cast(u32x4, cat8(f2bf4(X[tt][0]), f2bf4(X[tt][1]))), rd,
+            at + tt * 16 * row, 0, 0);
+    } else if (a.pq) {
+      const int row = a.Hv * K * 4, at = r16 * row + (32 * wk + 8 * grp) * 4;
+      const size_t from = (tok * a.Hv + h) * K;
+      const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(
+          a.pq + from, 0, (n - 1) * row + K * 4, kBufferFlags);
+      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+          a.pk + from, 0, (n - 1) * row + K * 4, kBufferFlags);
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+        for (int T = 0; T < 2; ++T) {
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, Y[tt][T]), rq,
+                                                 at + tt * 16 * row + 16 * T, 0, 0);
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, X[tt][T]), rk,
+                                                 at + tt * 16 * row + 16 * T, 0, 0);
+        }
+    } else {
+      const int row = a.Hv * K * 2, at = r16 * row + (32 * wk + 8 * grp) * 2;
+      const size_t from = (tok * a.Hv + h) * K;
+      const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(
+          a.dq + from, 0, (n - 1) * row + K * 2, kBufferFlags);
+      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+          a.dk + from, 0, (n - 1) * row + K * 2, kBufferFlags);
+#pragma unroll
+      for (int tt = 0; tt < 4; ++tt) {
+        __builtin_amdgcn_raw_buffer_store_b128(
+            __builtin_bit_cast(u32x4, cat8(f2bf4(Y[tt][0]), f2bf4(Y[tt][1]))), rq,
+            at + tt * 16 * row, 0, 0);
+        __builtin_amdgcn_raw_buffer_store_b128(
+            __builtin_bit_cast(u32x4, cat8(f2bf4(X[tt][0]), f2bf4(X[tt][1]))), rk,
+            at + tt * 16 * row, 0, 0);
+      }
+    }
+  };
   load(nc - 1);
   for (int c = nc - 1; c >= 0; --c) {
+    // (nothing derived from these is kept from one chunk for the next)
+    int ln = lane;
+    hide(ln);
+    const int lane = ln, r16 = ln % 16, grp = ln / 16;
     hide(krb);
     hide(vrb);
     hide(kcb);
     hide(vcb);
+    hide(pb);
+    hide(pw);
+    hide(pcb);
     hide(qf);
-    hide(gi);
     hide(kf);
     hide(vf);
     hide(of);
+    hide(gi);
     const int n = sg.ntok - c * kChunk;
     const size_t tok = (size_t)sg.tok0 + c * kChunk;
     sq.store(qs, kt, tid);
@@ -154,6 +208,7 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
       }
     }
     __syncthreads();
+    if (c < nc - 1) store_grads(c + 1);
     load(c - 1);
 
     // P and dP, tile by tile, as bf16 rows, and the sums of M
@@ -181,8 +236,8 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
         d[r] *= gam;
         rs += M[r];
       }
-      *reinterpret_cast<u16x4*>(ps + LinTile<64>::off(i, j / 8) + (grp & 1) * 8) = f2bf4(p);
-      *reinterpret_cast<u16x4*>(dps + LinTile<64>::off(i, j / 8) + (grp & 1) * 8) = f2bf4(d);
+      *reinterpret_cast<u16x4*>(ps + (pw ^ (32 * jt)) + it * 2048) = f2bf4(p);
+      *reinterpret_cast<u16x4*>(dps + (pw ^ (32 * jt)) + it * 2048) = f2bf4(d);
       rs += __shfl_xor(rs, 16);
       rs += __shfl_xor(rs, 32);
       if (grp == 0) rowM[jt][i] = rs;
@@ -193,11 +248,10 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
       if (r16 == 0) *reinterpret_cast<f32x4*>(&colM[it][j]) = M;
     }
 
-    f32x4 X[4][2], Y[4][2];   // dv; or dk and dq (by token tile)
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) X[tt][0] = X[tt][1] = Y[tt][0] = Y[tt][1] = zero4();
     const float eC = exp2_(sG[63]);
-    if (vwave) {
+    if constexpr (VW) {
 #pragma unroll
       for (int b = 0; b < K / 32; ++b) {
         u16x8 df[2];
@@ -308,7 +362,7 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
         lo = cat8(l0, l1);
       };
       u16x8 yf[2], hi[2], lo[2];
-      if (vwave) {
+      if constexpr (VW) {
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
           yf[T] = LinTile<V>::cols(os, vcb, kb, 2 * wv + T);
@@ -316,7 +370,7 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
         }
 #pragma unroll
         for (int tt = 0; tt < 2 * kb + 2; ++tt) {
-          const u16x8 pf = LinTile<64>::cols16(ps, LinTile<64>::col16_base(tt, lane), kb);
+          const u16x8 pf = LinTile<64>::cols16(ps, pcb ^ (32 * tt), kb);
 #pragma unroll
           for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(yf[T], pf, X[tt][T]);
         }
@@ -339,7 +393,7 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
         }
 #pragma unroll
         for (int tt = 0; tt < 2 * kb + 2; ++tt) {
-          const u16x8 pf = LinTile<64>::cols16(dps, LinTile<64>::col16_base(tt, lane), kb);
+          const u16x8 pf = LinTile<64>::cols16(dps, pcb ^ (32 * tt), kb);
 #pragma unroll
           for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(yf[T], pf, X[tt][T]);
         }
@@ -360,40 +414,46 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
         }
       }
     }
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt) {
-      const int i = 16 * tt + r16;
-      if (i >= n) continue;
-      const size_t th = (tok + i) * a.Hv + h;
-      if (vwave) {
-        *reinterpret_cast<u16x8*>(a.dv + th * V + 32 * wv + 8 * grp) =
-            cat8(f2bf4(X[tt][0]), f2bf4(X[tt][1]));
-      } else if (a.pq) {
-        f32x4* pq = reinterpret_cast<f32x4*>(a.pq + th * K + 32 * wk + 8 * grp);
-        f32x4* pk = reinterpret_cast<f32x4*>(a.pk + th * K + 32 * wk + 8 * grp);
-        pq[0] = Y[tt][0];
-        pq[1] = Y[tt][1];
-        pk[0] = X[tt][0];
-        pk[1] = X[tt][1];
-      } else {
-        *reinterpret_cast<u16x8*>(a.dq + th * K + 32 * wk + 8 * grp) =
-            cat8(f2bf4(Y[tt][0]), f2bf4(Y[tt][1]));
-        *reinterpret_cast<u16x8*>(a.dk + th * K + 32 * wk + 8 * grp) =
-            cat8(f2bf4(X[tt][0]), f2bf4(X[tt][1]));
-      }
-    }
     __syncthreads();
   }
-  if (a.dh0 && sg.first && vwave) {
-    float* out = a.dh0 + ((size_t)sg.seq * a.Hv + h) * K * V;
+  if (nc > 0) store_grads(0);
+  if (a.dh0 && sg.first && VW) {
+    const __amdgpu_buffer_rsrc_t rd = lin_state(a.dh0 + ((size_t)sg.seq * a.Hv + h) * K * V, K * V);
 #pragma unroll
     for (int t = 0; t < K / 16; ++t)
 #pragma unroll
       for (int T = 0; T < 2; ++T)
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          out[rho_row(t, 4 * grp + r) * V + 32 * wv + c32 + 4 * T] = ST[t][T][r];
+          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(ST[t][T][r]), rd, state_at(lane, T),
+                                                tile_at(t, r), 0);
   }
+}
+
+template <int K, int V>
+__global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) {
+  constexpr int NT = 2 * (K + V);
+  __shared__ __align__(16) LinGradLds<K, V> lds;
+  if (a.grid.table && *a.grid.status) {
+    // a cu_seqlens violation: every gradient over the tokens is zero
+    const size_t nv = (size_t)a.grid.total * a.Hv * V / 8, nk = (size_t)a.grid.total * a.Hqk * K / 8;
+    const size_t ng = (size_t)a.grid.total * a.Hv, st = (size_t)gridDim.x * NT;
+    const size_t i0 = (size_t)blockIdx.x * NT + threadIdx.x;
+    for (size_t i = i0; i < nv; i += st) reinterpret_cast<u32x4*>(a.dv)[i] = u32x4{0, 0, 0, 0};
+    for (size_t i = i0; i < nk; i += st) {
+      reinterpret_cast<u32x4*>(a.dq)[i] = u32x4{0, 0, 0, 0};
+      reinterpret_cast<u32x4*>(a.dk)[i] = u32x4{0, 0, 0, 0};
+    }
+    for (size_t i = i0; i < ng; i += st) a.dg[i] = 0.f;
+  }
+  int sid, h;
+  if (!lin_item(a.grid, a.grid.nseg, a.Hqk, a.Hv, sid, h)) return;
+  if (a.grid.table) sid = a.grid.order[sid];
+  const LinSeg sg = lin_seg(a.grid, sid);
+  if (sg.seq < 0) return;
+  const int w = wave_index();
+  if (w < V / 32) lin_grad_walk<K, V, true>(a, sg, sid, h, w, lds);
+  else lin_grad_walk<K, V, false>(a, sg, sid, h, w, lds);
 }
 
 // dq, dk of a qk-head: the sum of its v-heads' parts, 8 elements per lane.
