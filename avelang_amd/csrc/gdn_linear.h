@@ -170,14 +170,25 @@ __device__ __forceinline__ float lane63(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
 
-// Eight bf16 values times eight fp32 factors (in LDS) as hi + lo in bf16.
-__device__ __forceinline__ void lin_split(u16x8 y, const float* f, u16x8& hi, u16x8& lo) {
+// Eight bf16 values times eight fp32 factors (in LDS) as a sum of NP bf16
+// parts: 2^-8 per part.
+template <int NP>
+__device__ __forceinline__ void lin_split(u16x8 y, const float* f, u16x8 (&part)[NP]) {
   const f32x4 f0 = *reinterpret_cast<const f32x4*>(f), f1 = *reinterpret_cast<const f32x4*>(f + 4);
-  u16x4 h0, l0, h1, l1;
-  split_bf4(f32x4{bf2f(y[0]), bf2f(y[1]), bf2f(y[2]), bf2f(y[3])} * f0, h0, l0);
-  split_bf4(f32x4{bf2f(y[4]), bf2f(y[5]), bf2f(y[6]), bf2f(y[7])} * f1, h1, l1);
-  hi = cat8(h0, h1);
-  lo = cat8(l0, l1);
+  f32x4 x0 = f32x4{bf2f(y[0]), bf2f(y[1]), bf2f(y[2]), bf2f(y[3])} * f0;
+  f32x4 x1 = f32x4{bf2f(y[4]), bf2f(y[5]), bf2f(y[6]), bf2f(y[7])} * f1;
+#pragma unroll
+  for (int p = 0; p < NP; ++p) {
+    const u16x4 h0 = f2bf4(x0), h1 = f2bf4(x1);
+    part[p] = cat8(h0, h1);
+    if (p + 1 < NP) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        x0[i] -= bf2f(h0[i]);
+        x1[i] -= bf2f(h1[i]);
+      }
+    }
+  }
 }
 
 // The decays of a chunk on their way in, by two waves: wave 0's lane l has its
@@ -245,7 +256,7 @@ void launch_lin_table(const int32_t* cu, const LinPlan& p, unsigned char* ws, in
 template <int K, int V>
 void launch_lin_segments(const uint16_t* x, int x_row, const uint16_t* y, int y_row,
                          const LinDecay& d, const LinGrid& g, int Hqk, int Hv, float scale,
-                         bool reverse, const float* edge, float* segs, float* decay,
-                         hipStream_t st);
+                         bool reverse, bool full, const float* edge, float* segs,
+                         float* decay, float* end, hipStream_t st);
 
 }  // namespace gdn

@@ -6,10 +6,10 @@
 //     P_ij = scale e^{G_i - G_j} (q_i . k_j)   (j <= i)
 //     o_i  = sum_j P_ij v_j + scale e^{G_i} S^T q_i
 //     S'   = e^{G_63} S + sum_j k_j (e^{R_j} v_j)^T
-// all products on bf16 MFMA with fp32 accumulation.  e^{R_j} v_j enters as the
-// sum of two bf16 parts (2^-17 relative), so the state keeps fp32's sums to
-// that; P and the state's copy that q reads are single bf16 (2^-9, the size
-// of o's own rounding).  R is summed from the chunk's end, not as G_63 - G_j:
+// all products on bf16 MFMA with fp32 accumulation.  e^{R_j} v_j enters as a
+// sum of bf16 parts: three (2^-24) where a state is returned or saved, two
+// (2^-16) where it serves o alone; P and the state's copy that q reads are
+// single bf16 (2^-8, the size of o's own rounding).  R is summed from the chunk's end, not as G_63 - G_j:
 // its error stays in proportion to the decay it gives.
 //
 // A sequence is cut into segments of L chunks that run at the same time: one
@@ -140,11 +140,11 @@ __device__ __forceinline__ void lin_store_state(const f32x4 (&S)[K / 16], float*
 // X^T (f Y) with x = k, y = v, f = e^R; or (REV) to the gradient of the state
 // before it, chunks last to first, x = q, y = dO, f = scale e^G.  A wave owns
 // 16 CT columns of Y and all rows of the state.
-template <int K, int V, int CT, bool REV>
+template <int K, int V, int CT, int NP, bool REV>
 __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_segment_kernel(
     const uint16_t* __restrict__ x, int x_row, const uint16_t* __restrict__ y, int y_row,
-    LinDecay dec, LinGrid grid, int Hqk, int Hv, float scale, float* __restrict__ segs,
-    float* __restrict__ decay) {
+    LinDecay dec, LinGrid grid, int Hqk, int Hv, float scale, bool all,
+    float* __restrict__ segs, float* __restrict__ decay) {
   constexpr int NT = 4 * V / CT;
   __shared__ __align__(16) char xs[LinTile<K>::BYTES];
   __shared__ __align__(16) char ys[LinTile<V>::BYTES];
@@ -154,16 +154,16 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_segment_kernel(
   if (grid.table) {
     if (!lin_item(grid, grid.nseg, Hqk, Hv, sid, h)) return;
     sid = grid.order[sid];
-  } else {   // every segment but one of each sequence
-    const int per = grid.nps - 1;
+  } else {   // every segment, or every one but one of each sequence
+    const int per = all ? grid.nps : grid.nps - 1;
     if (!lin_item(grid, grid.N * per, Hqk, Hv, sid, h)) return;
-    sid = sid / per * grid.nps + sid % per + (REV ? 1 : 0);
+    sid = sid / per * grid.nps + sid % per + (REV && !all ? 1 : 0);
   }
   const int hq = h / (Hv / Hqk);
   const LinSeg sg = lin_seg(grid, sid);
-  if (sg.seq < 0 || (REV ? sg.first : sg.last)) return;
+  if (sg.seq < 0 || (!all && (REV ? sg.first : sg.last))) return;
   const int tid = threadIdx.x, lane = tid % 64, w = wave_index();
-  const int r16 = lane % 16, grp = lane / 16;
+  const int grp = lane / 16;
   const int nc = (sg.ntok + kChunk - 1) / kChunk;
 
   f32x4 S[CT][K / 16];
@@ -214,17 +214,17 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_segment_kernel(
       for (int t = 0; t < K / 16; ++t) S[T][t] *= eC;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      u16x8 hi[CT], lo[CT];
+      u16x8 part[CT][NP];
 #pragma unroll
       for (int T = 0; T < CT; ++T)
-        lin_split(LinTile<V>::cols16(ys, yb ^ (32 * T), kb), fac + 32 * kb + 8 * grp, hi[T], lo[T]);
+        lin_split(LinTile<V>::cols16(ys, yb ^ (32 * T), kb), fac + 32 * kb + 8 * grp, part[T]);
 #pragma unroll
       for (int t = 0; t < K / 16; ++t) {
         const u16x8 a = LinTile<K>::cols(xs, xb, kb, t);
 #pragma unroll
-        for (int T = 0; T < CT; ++T) S[T][t] = mfma16(a, hi[T], S[T][t]);
+        for (int p = 0; p < NP; ++p)
 #pragma unroll
-        for (int T = 0; T < CT; ++T) S[T][t] = mfma16(a, lo[T], S[T][t]);
+          for (int T = 0; T < CT; ++T) S[T][t] = mfma16(a, part[T][p], S[T][t]);
       }
     }
     __syncthreads();
@@ -237,12 +237,14 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_segment_kernel(
 
 // The states at every segment's start (REV: the gradients of the state at
 // every segment's end) in place of the contributions, from `edge` (h0 / dht,
-// nullable).  A lane per element.
+// nullable); into `end` (nullable) the state after the last.  A lane per
+// element.
 template <bool REV>
 __global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int KV,
-                                                       const float* __restrict__ edge,
+                                                       const float* edge,
                                                        float* __restrict__ segs,
-                                                       const float* __restrict__ decay) {
+                                                       const float* __restrict__ decay,
+                                                       float* end) {
   const int per = KV / 256;
   int n = blockIdx.x / (Hv * per);
   const int h = blockIdx.x / per % Hv, e = blockIdx.x % per * 256 + threadIdx.x;
@@ -276,7 +278,10 @@ __global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int
       }
     }
   }
-  segs[((size_t)(REV ? s0 : s1 - 1) * Hv + h) * KV + e] = S;
+  const size_t at = (size_t)(REV ? s0 : s1 - 1) * Hv + h;
+  const float last = end ? decay[at] * S + segs[at * KV + e] : 0.f;
+  segs[at * KV + e] = S;
+  if (end) end[((size_t)n * Hv + h) * KV + e] = last;
 }
 
 // ------------------------------------------------------------------ walk ----
@@ -284,7 +289,7 @@ __global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int
 // state at every chunk's start (SAVE), ht.  A wave owns 16 CT columns of V, all
 // of the state's rows for them in its accumulators, whose layout is that of
 // the operand with which S^T q is formed: the state never leaves the registers.
-template <int K, int V, int CT, bool OUT, bool SAVE>
+template <int K, int V, int CT, int NP, bool OUT, bool SAVE>
 __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k,
     const uint16_t* __restrict__ v, TokenStride ts, LinDecay dec, LinGrid grid, int Hqk, int Hv,
@@ -315,7 +320,8 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
   const int nc = (sg.ntok + kChunk - 1) / kChunk;
 
   f32x4 S[CT][K / 16];   // rows rho_row(t, 4 grp + r), column 16 (CT w + T) + r16
-  const float* src = sg.first ? (h0 ? h0 + ((size_t)sg.seq * Hv + h) * K * V : nullptr)
+  // (several segments: the first one's from the join too, since ht may be h0)
+  const float* src = sg.first && sg.last ? (h0 ? h0 + ((size_t)sg.seq * Hv + h) * K * V : nullptr)
                               : segs + ((size_t)sid * Hv + h) * K * V;
 #pragma unroll
   for (int T = 0; T < CT; ++T) lin_load_state<K, V>(S[T], src, CT * w + T, lane);
@@ -469,11 +475,11 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
       for (int t = 0; t < K / 16; ++t) S[T][t] *= eC;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      u16x8 vf[CT], hi[CT], lo[CT];
+      u16x8 vf[CT], part[CT][NP];
 #pragma unroll
       for (int T = 0; T < CT; ++T) {
         vf[T] = LinTile<V>::cols16(vs, vb ^ (32 * T), kb);
-        lin_split(vf[T], sK + 32 * kb + 8 * grp, hi[T], lo[T]);
+        lin_split(vf[T], sK + 32 * kb + 8 * grp, part[T]);
       }
       if (OUT) {
 #pragma unroll
@@ -487,9 +493,9 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
       for (int t = 0; t < K / 16; ++t) {
         const u16x8 f = LinTile<K>::cols(ks, kcb, kb, t);
 #pragma unroll
-        for (int T = 0; T < CT; ++T) S[T][t] = mfma16(f, hi[T], S[T][t]);
+        for (int p = 0; p < NP; ++p)
 #pragma unroll
-        for (int T = 0; T < CT; ++T) S[T][t] = mfma16(f, lo[T], S[T][t]);
+          for (int T = 0; T < CT; ++T) S[T][t] = mfma16(f, part[T][p], S[T][t]);
       }
     }
     if (OUT) {
@@ -508,11 +514,15 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
   }
 }
 
-constexpr int kColTiles = 2;
+// 16-column tiles per wave.  Two in the walk read half of what one reads from
+// LDS (packed prompts 873 us against 920); one in the segments leaves room for
+// four waves per SIMD (8192 tokens, both launches: 111 us against 115).
+constexpr int kColTiles = 2, kSegTiles = 1;
 
 // ------------------------------------------------------------------ host ----
 // Chunks per segment: as many as spread all chunks over two workgroups per CU
-// once, four at least.
+// once.  (8192 tokens, 32 v-heads: L = 8 111 us; 4 127, 16 122, 32 213.  449
+// tokens: L = 1 28 us; 2 31, 4 38, all 8 chunks in one walk 38.)
 LinPlan lin_plan(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu, bool bwd) {
   LinPlan p{};
   const long long tokens = (long long)B * T;
@@ -520,7 +530,7 @@ LinPlan lin_plan(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu
   p.chunks = has_cu ? tokens / kChunk + N : B * per;
   const long long slots = 2LL * device_cus();
   long long L = (p.chunks * Hv + slots - 1) / slots;
-  if (L < 4) L = 4;
+  if (L < 1) L = 1;
   if (L > per) L = per > 0 ? per : 1;
   p.L = (int)L;
   p.nps = (int)(per > 0 ? (per + L - 1) / L : 1);
@@ -582,24 +592,27 @@ void launch_lin_table(const int32_t* cu, const LinPlan& p, unsigned char* ws, in
 template <int K, int V>
 void launch_lin_segments(const uint16_t* x, int x_row, const uint16_t* y, int y_row,
                          const LinDecay& d, const LinGrid& g, int Hqk, int Hv, float scale,
-                         bool reverse, const float* edge, float* segs, float* decay,
-                         hipStream_t st) {
-  const dim3 items(lin_items(g.table ? g.nseg : g.N * (g.nps - 1), Hqk, Hv));
+                         bool reverse, bool full, const float* edge, float* segs, float* decay,
+                         float* end, hipStream_t st) {
+  const dim3 items(lin_items(g.table ? g.nseg : g.N * (g.nps - (end ? 0 : 1)), Hqk, Hv));
   const dim3 elems((unsigned)(g.nlong * Hv * (K * V / 256)));
+#define GDN_SEG(NP, REV)                                                                        \
+  hipLaunchKernelGGL((lin_segment_kernel<K, V, kSegTiles, NP, REV>), items,                     \
+                     dim3(4 * V / kSegTiles), 0, st, x, x_row, y, y_row, d, g, Hqk, Hv, scale,  \
+                     end != nullptr, segs, decay);                                              \
+  hipLaunchKernelGGL(lin_join_kernel<REV>, elems, dim3(256), 0, st, g, Hv, K * V, edge, segs, decay, end)
   if (reverse) {
-    hipLaunchKernelGGL((lin_segment_kernel<K, V, kColTiles, true>), items, dim3(4 * V / kColTiles), 0, st, x, x_row, y,
-                       y_row, d, g, Hqk, Hv, scale, segs, decay);
-    hipLaunchKernelGGL(lin_join_kernel<true>, elems, dim3(256), 0, st, g, Hv, K * V, edge, segs, decay);
+    if (full) { GDN_SEG(3, true); } else { GDN_SEG(2, true); }
   } else {
-    hipLaunchKernelGGL((lin_segment_kernel<K, V, kColTiles, false>), items, dim3(4 * V / kColTiles), 0, st, x, x_row, y,
-                       y_row, d, g, Hqk, Hv, scale, segs, decay);
-    hipLaunchKernelGGL(lin_join_kernel<false>, elems, dim3(256), 0, st, g, Hv, K * V, edge, segs, decay);
+    if (full) { GDN_SEG(3, false); } else { GDN_SEG(2, false); }
   }
+#undef GDN_SEG
 }
 #define GDN_LS(KK, VV)                                                                        \
   template void launch_lin_segments<KK, VV>(const uint16_t*, int, const uint16_t*, int,       \
                                             const LinDecay&, const LinGrid&, int, int, float, \
-                                            bool, const float*, float*, float*, hipStream_t);
+                                            bool, bool, const float*, float*, float*, float*,  \
+                                            hipStream_t);
 GDN_LS(128, 128) GDN_LS(128, 64) GDN_LS(64, 128) GDN_LS(64, 64)
 #undef GDN_LS
 
@@ -609,15 +622,26 @@ void launch_walk(const uint16_t* q, const uint16_t* k, const uint16_t* v, TokenS
                  const LinDecay& d, const LinGrid& g, int Hqk, int Hv, float scale,
                  const float* h0, float* ht, float* segs, float* decay, uint16_t* o, u16x4* states,
                  hipStream_t st) {
-  if (g.nlong > 0)
-    launch_lin_segments<K, V>(k, ts.k, v, ts.v, d, g, Hqk, Hv, 1.f, false, h0, segs, decay, st);
+  // (the saved states have the same bits whether they are formed with o and ht
+  // or again)
+  const bool full = ht || states;
+  if (g.nlong > 0) {
+    // equal lengths without saved states: the final states come from the segments'
+    // contributions, and the walk, for o alone, takes two parts
+    const bool end = ht && !states && !g.table;
+    launch_lin_segments<K, V>(k, ts.k, v, ts.v, d, g, Hqk, Hv, 1.f, false, full, h0, segs, decay,
+                              end ? ht : nullptr, st);
+    if (end) ht = nullptr;
+  }
   const dim3 items(lin_items(g.nseg, Hqk, Hv));
-#define GDN_LW(OUT, SAVE)                                                                      \
-  hipLaunchKernelGGL((lin_walk_kernel<K, V, kColTiles, OUT, SAVE>), items, dim3(4 * V / kColTiles), 0, st, q, k, v, ts, \
-                     d, g, Hqk, Hv, scale, h0, ht, segs, o, states)
-  if (o && states) GDN_LW(true, true);
-  else if (o) GDN_LW(true, false);
-  else GDN_LW(false, true);
+#define GDN_LW(NP, OUT, SAVE)                                                                   \
+  hipLaunchKernelGGL((lin_walk_kernel<K, V, kColTiles, NP, OUT, SAVE>), items,                  \
+                     dim3(4 * V / kColTiles), 0, st, q, k, v, ts, d, g, Hqk, Hv, scale, h0, ht, \
+                     segs, o, states)
+  if (o && states) GDN_LW(3, true, true);
+  else if (!o) GDN_LW(3, false, true);
+  else if (ht) GDN_LW(3, true, false);
+  else GDN_LW(2, true, false);
 #undef GDN_LW
 }
 }  // namespace

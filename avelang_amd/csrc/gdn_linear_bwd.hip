@@ -53,7 +53,7 @@ struct LinGradLds {
 // reduce over V, and with the saved states' fragments <S, D>): D is kept in
 // both orientations so that neither ever leaves the registers.  This is one
 // wave's walk, VW: of the first kind.  Both kinds meet the same barriers.
-template <int K, int V, bool VW>
+template <int K, int V, bool VW, int NP>
 __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg& sg, int sid, int h,
                                               int w, LinGradLds<K, V>& lds) {
   constexpr int NT = 2 * (K + V), NV = V / 32, NK = K / 32, NW = NV + NK;
@@ -70,7 +70,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
 
   // ST[t][T]: D (key tile t, value tile T), or D^T (value tile t, key tile T)
   f32x4 ST[NTILE][2];
-  const float* src = sg.last ? (a.dht ? a.dht + ((size_t)sg.seq * a.Hv + h) * K * V : nullptr)
+  const float* src = sg.first && sg.last ? (a.dht ? a.dht + ((size_t)sg.seq * a.Hv + h) * K * V : nullptr)
                              : a.segs + ((size_t)sid * a.Hv + h) * K * V;
   // a lane's part of the state's address, V waves: row 8 grp (+ the tile's and
   // r), column of value tile T; key waves with rows and columns exchanged
@@ -352,21 +352,12 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
     }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
-      const f32x4 f0 = *reinterpret_cast<const f32x4*>(&sQ[32 * kb + 8 * grp]);
-      const f32x4 f1 = *reinterpret_cast<const f32x4*>(&sQ[32 * kb + 8 * grp + 4]);
-      auto split = [&](u16x8 y, u16x8& hi, u16x8& lo) {
-        u16x4 h0, l0, h1, l1;
-        split_bf4(f32x4{bf2f(y[0]), bf2f(y[1]), bf2f(y[2]), bf2f(y[3])} * f0, h0, l0);
-        split_bf4(f32x4{bf2f(y[4]), bf2f(y[5]), bf2f(y[6]), bf2f(y[7])} * f1, h1, l1);
-        hi = cat8(h0, h1);
-        lo = cat8(l0, l1);
-      };
-      u16x8 yf[2], hi[2], lo[2];
+      u16x8 yf[2], part[2][NP];
       if constexpr (VW) {
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
           yf[T] = LinTile<V>::cols(os, vcb, kb, 2 * wv + T);
-          split(yf[T], hi[T], lo[T]);
+          lin_split(yf[T], sQ + 32 * kb + 8 * grp, part[T]);
         }
 #pragma unroll
         for (int tt = 0; tt < 2 * kb + 2; ++tt) {
@@ -378,10 +369,9 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
         for (int t = 0; t < K / 16; ++t) {
           const u16x8 f = LinTile<K>::cols(qs, kcb, kb, t);
 #pragma unroll
-          for (int T = 0; T < 2; ++T) {
-            ST[t][T] = mfma16(f, hi[T], ST[t][T]);
-            ST[t][T] = mfma16(f, lo[T], ST[t][T]);
-          }
+          for (int p = 0; p < NP; ++p)
+#pragma unroll
+            for (int T = 0; T < 2; ++T) ST[t][T] = mfma16(f, part[T][p], ST[t][T]);
         }
       } else {
         u16x8 kf[2];
@@ -389,7 +379,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
         for (int T = 0; T < 2; ++T) {
           yf[T] = LinTile<K>::cols(qs, kcb, kb, 2 * wk + T);
           kf[T] = LinTile<K>::cols(ks, kcb, kb, 2 * wk + T);
-          split(yf[T], hi[T], lo[T]);
+          lin_split(yf[T], sQ + 32 * kb + 8 * grp, part[T]);
         }
 #pragma unroll
         for (int tt = 0; tt < 2 * kb + 2; ++tt) {
@@ -407,10 +397,9 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
         for (int t = 0; t < V / 16; ++t) {
           const u16x8 f = LinTile<V>::cols(os, vcb, kb, t);
 #pragma unroll
-          for (int T = 0; T < 2; ++T) {
-            ST[t][T] = mfma16(f, hi[T], ST[t][T]);
-            ST[t][T] = mfma16(f, lo[T], ST[t][T]);
-          }
+          for (int p = 0; p < NP; ++p)
+#pragma unroll
+            for (int T = 0; T < 2; ++T) ST[t][T] = mfma16(f, part[T][p], ST[t][T]);
         }
       }
     }
@@ -430,7 +419,8 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
   }
 }
 
-template <int K, int V>
+// NP: the parts of dO's products on the way to dh0 (three where it is wanted).
+template <int K, int V, int NP>
 __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) {
   constexpr int NT = 2 * (K + V);
   __shared__ __align__(16) LinGradLds<K, V> lds;
@@ -452,8 +442,8 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
   const LinSeg sg = lin_seg(a.grid, sid);
   if (sg.seq < 0) return;
   const int w = wave_index();
-  if (w < V / 32) lin_grad_walk<K, V, true>(a, sg, sid, h, w, lds);
-  else lin_grad_walk<K, V, false>(a, sg, sid, h, w, lds);
+  if (w < V / 32) lin_grad_walk<K, V, true, NP>(a, sg, sid, h, w, lds);
+  else lin_grad_walk<K, V, false, 2>(a, sg, sid, h, w, lds);
 }
 
 // dq, dk of a qk-head: the sum of its v-heads' parts, 8 elements per lane.
@@ -504,9 +494,10 @@ template <int K, int V>
 void launch_grad(const LinBwdArgs& a, float* segs, float* decay, hipStream_t st) {
   if (a.grid.nlong > 0)
     launch_lin_segments<K, V>(a.q, a.ts.q, a.dO, a.Hv * V, a.dec, a.grid, a.Hqk, a.Hv, a.scale,
-                              true, a.dht, segs, decay, st);
-  hipLaunchKernelGGL((lin_grad_kernel<K, V>), dim3(lin_items(a.grid.nseg, a.Hqk, a.Hv)),
-                     dim3(2 * (K + V)), 0, st, a);
+                              true, a.dh0 != nullptr, a.dht, segs, decay, nullptr, st);
+  const dim3 items(lin_items(a.grid.nseg, a.Hqk, a.Hv));
+  if (a.dh0) hipLaunchKernelGGL((lin_grad_kernel<K, V, 3>), items, dim3(2 * (K + V)), 0, st, a);
+  else hipLaunchKernelGGL((lin_grad_kernel<K, V, 2>), items, dim3(2 * (K + V)), 0, st, a);
 }
 }  // namespace
 

@@ -292,3 +292,22 @@ def test_on_another_stream(rocm_device):
         got = ave.chunk_linear_attn(t["q"], t["k"], t["v"], t["g"])[0]
     st.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("packed", [False, True])
+def test_final_state_over_the_initial_one(rocm_device, packed):
+    """Sequences of several segments with final_state = initial_state: nothing reads it after it
+    is written."""
+    import avelang_amd as ave
+    lens = [700, 0, 30, 570]
+    shape = (1, 1300, 1, 2, 64, 64) if packed else (2, 700, 2, 4, 128, 128)
+    t = to(make(*shape, seed=11, lens=lens if packed else None), rocm_device)
+    cu = torch.tensor(cu_of(lens), device=rocm_device) if packed else None
+    args = (t["q"], t["k"], t["v"], t["g"])
+    o, s = ave.chunk_linear_attn(*args, initial_state=t["h0"], output_final_state=True, cu_seqlens=cu)
+    for _ in range(5):
+        state = t["h0"].clone()
+        o2, s2 = ave.chunk_linear_attn(*args, initial_state=state, output_final_state=True,
+                                       cu_seqlens=cu, final_state=state)
+        assert s2 is state and torch.equal(s2, s) and torch.equal(o2, o)
