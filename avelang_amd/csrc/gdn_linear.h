@@ -79,31 +79,30 @@ struct LinTile {
   static __device__ __forceinline__ u16x8 rows(const char* p, int base, int tt, int kb) {
     return *reinterpret_cast<const u16x8*>(p + (base ^ (kb * 64)) + tt * 16 * RS);
   }
-  // Operand fragment of X^T: 16 columns and 32 rows, lane (r16, grp) holds
-  // X[32 kb + 8 grp + i][c], c = rho_row of tile T: 32 (T / 2) + 8 (r16 / 4) +
-  // 4 (T % 2) + r16 % 4.  Two tiles' accumulator rows then hold 8 adjacent
-  // columns per lane.
-  static __device__ __forceinline__ int col_base(int lane) {
+  // The same rows, with the columns in the order in which two 16-row tiles of
+  // accumulators hold theirs: element i < 4 is column 32 kb + 4 grp + i, the
+  // others 16 further on (the operand that meets a state kept in accumulators).
+  static __device__ __forceinline__ int row4_base(int lane) {
     const int r16 = lane % 16, grp = lane / 16;
-    const int m4 = r16 >> 2, q4 = r16 & 3, r0 = 8 * grp + m4;
-    return r0 * RS + 16 * (q4 ^ swz(r0));
+    return off(r16, grp >> 1) + (grp & 1) * 8;
   }
-  static __device__ __forceinline__ u16x8 cols(const char* p, int base, int kb, int T) {
-    const int b0 = base ^ ((T >> 1) * 64), at = kb * 32 * RS + (T & 1) * 8;
-    // (four rows on, the unit's lowest bit is the other one)
-    const u16x4 lo = lds_tr16(reinterpret_cast<const uint16_t*>(p + b0 + at));
-    const u16x4 hi = lds_tr16(reinterpret_cast<const uint16_t*>(p + (b0 ^ 16) + 4 * RS + at));
-    return cat8(lo, hi);
+  static __device__ __forceinline__ u16x8 rows4(const char* p, int base, int tt, int kb) {
+    const int b = base ^ (kb * 64);
+    return cat8(*reinterpret_cast<const u16x4*>(p + b + tt * 16 * RS),
+                *reinterpret_cast<const u16x4*>(p + (b ^ 32) + tt * 16 * RS));
   }
-  // The same for 16 adjacent columns: lane (r16, grp) holds
+  // Operand fragment of X^T, 16 columns and 32 rows: lane (r16, grp) holds
   // X[32 kb + 8 grp + i][16 T + r16].
-  static __device__ __forceinline__ int col16_base(int T, int lane) {
+  static __device__ __forceinline__ int col_base(int T, int lane) {
     const int r16 = lane % 16, grp = lane / 16;
     const int m4 = r16 >> 2, q4 = r16 & 3, r0 = 8 * grp + m4;
     return off(r0, 2 * T + (q4 >> 1)) + (q4 & 1) * 8;
   }
-  static __device__ __forceinline__ u16x8 cols16(const char* p, int base, int kb) {
+  // (base: of tile T0, for tile T0 ^ T)
+  static __device__ __forceinline__ u16x8 cols(const char* p, int base, int kb, int T) {
     const int at = kb * 32 * RS;
+    base ^= 32 * T;
+    // (four rows on, the unit's lowest bit is the other one)
     const u16x4 lo = lds_tr16(reinterpret_cast<const uint16_t*>(p + base + at));
     const u16x4 hi = lds_tr16(reinterpret_cast<const uint16_t*>(p + (base ^ 16) + 4 * RS + at));
     return cat8(lo, hi);
@@ -145,6 +144,19 @@ struct LinStage {
   }
 };
 
+// Sum over 16 lanes (lane 15 of each 16 has it).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float dpp_add(float x) {
+  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
+                 0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float row16_sum(float x) {
+  x = dpp_add<0x111, 0xf>(x);   // row_shr 1, 2, 4, 8
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  return dpp_add<0x118, 0xf>(x);
+}
+
 // The index of this wave, known to be the same in all its lanes.
 __device__ __forceinline__ int wave_index() {
   return __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
@@ -152,16 +164,8 @@ __device__ __forceinline__ int wave_index() {
 __device__ __forceinline__ void hide(int& x) { asm volatile("" : "+v"(x)); }
 
 // Inclusive prefix sum over a wave, in its lanes' own adders (no LDS).
-template <int CTRL, int ROWS>
-__device__ __forceinline__ float dpp_add(float x) {
-  return x + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(
-                 0, __builtin_bit_cast(int, x), CTRL, ROWS, 0xf, false));
-}
 __device__ __forceinline__ float wave_prefix(float x) {
-  x = dpp_add<0x111, 0xf>(x);   // row_shr 1, 2, 4, 8: within 16 lanes
-  x = dpp_add<0x112, 0xf>(x);
-  x = dpp_add<0x114, 0xf>(x);
-  x = dpp_add<0x118, 0xf>(x);
+  x = row16_sum(x);             // (a prefix sum within the 16 lanes)
   x = dpp_add<0x142, 0xa>(x);   // lane 15 of a row to the next: rows 1 and 3
   return dpp_add<0x143, 0xc>(x);   // lane 31 to rows 2 and 3
 }

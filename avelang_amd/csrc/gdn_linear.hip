@@ -111,28 +111,28 @@ __global__ __launch_bounds__(1024) void lin_table_kernel(const int32_t* cu, LinS
 }
 
 // 16 columns (ct) of a state [K][V] as accumulators: tile t's lane holds rows
-// rho_row(t, 4 grp + r) of column 16 ct + r16.
+// 16 t + 4 grp + r of column 16 ct + r16.
 template <int K, int V>
 __device__ __forceinline__ void lin_load_state(f32x4 (&S)[K / 16], const float* p, int ct, int lane) {
   const __amdgpu_buffer_rsrc_t rs = lin_state(p, K * V);
-  const int at = (8 * (lane / 16) * V + 16 * ct + lane % 16) * 4;
+  const int at = (4 * (lane / 16) * V + 16 * ct + lane % 16) * 4;
 #pragma unroll
   for (int t = 0; t < K / 16; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       S[t][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
-          rs, at, (32 * (t >> 1) + 4 * (t & 1) + r) * V * 4, 0));
+          rs, at, (16 * t + r) * V * 4, 0));
 }
 template <int K, int V>
 __device__ __forceinline__ void lin_store_state(const f32x4 (&S)[K / 16], float* p, int ct, int lane) {
   const __amdgpu_buffer_rsrc_t rs = lin_state(p, K * V);
-  const int at = (8 * (lane / 16) * V + 16 * ct + lane % 16) * 4;
+  const int at = (4 * (lane / 16) * V + 16 * ct + lane % 16) * 4;
 #pragma unroll
   for (int t = 0; t < K / 16; ++t)
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(S[t][r]), rs, at,
-                                            (32 * (t >> 1) + 4 * (t & 1) + r) * V * 4, 0);
+                                            (16 * t + r) * V * 4, 0);
 }
 
 // -------------------------------------------------------------- segments ----
@@ -186,7 +186,7 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_segment_kernel(
     sy.load(y + t * y_row + h * V, y_row, min(n, 64), yf);
   };
   const int c0 = REV ? nc - 1 : 0, step = REV ? -1 : 1;
-  int xb = LinTile<K>::col_base(lane), yb = LinTile<V>::col16_base(CT * w, lane);
+  int xb = LinTile<K>::col_base(0, lane), yb = LinTile<V>::col_base(CT * w, lane);
   load(c0);
   for (int i = 0; i < nc; ++i) {
     hide(xb);
@@ -217,7 +217,7 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_segment_kernel(
       u16x8 part[CT][NP];
 #pragma unroll
       for (int T = 0; T < CT; ++T)
-        lin_split(LinTile<V>::cols16(ys, yb ^ (32 * T), kb), fac + 32 * kb + 8 * grp, part[T]);
+        lin_split(LinTile<V>::cols(ys, yb, kb, T), fac + 32 * kb + 8 * grp, part[T]);
 #pragma unroll
       for (int t = 0; t < K / 16; ++t) {
         const u16x8 a = LinTile<K>::cols(xs, xb, kb, t);
@@ -319,7 +319,7 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
   if (sg.seq < 0) return;
   const int nc = (sg.ntok + kChunk - 1) / kChunk;
 
-  f32x4 S[CT][K / 16];   // rows rho_row(t, 4 grp + r), column 16 (CT w + T) + r16
+  f32x4 S[CT][K / 16];   // rows 16 t + 4 grp + r, column 16 (CT w + T) + r16
   // (several segments: the first one's from the join too, since ht may be h0)
   const float* src = sg.first && sg.last ? (h0 ? h0 + ((size_t)sg.seq * Hv + h) * K * V : nullptr)
                               : segs + ((size_t)sid * Hv + h) * K * V;
@@ -349,8 +349,9 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
       *reinterpret_cast<u32x4*>(ps + LinTile<64>::off(r, u)) = u32x4{0, 0, 0, 0};
     }
   }
-  int rb = LinTile<K>::row_base(lane), kcb = LinTile<K>::col_base(lane);
-  int vb = LinTile<V>::col16_base(CT * w, lane), pb = LinTile<64>::row_base(lane);
+  int rb = LinTile<K>::row_base(lane), r4b = LinTile<K>::row4_base(lane);
+  int kcb = LinTile<K>::col_base(0, lane);
+  int vb = LinTile<V>::col_base(CT * w, lane), pb = LinTile<64>::row_base(lane);
   int pw = LinTile<64>::off(r16, grp >> 1) + (grp & 1) * 8;
   // o of a chunk leaves ahead of the loads issued in the next: the wait for
   // loads counts stores too, and behind them it would wait out every store
@@ -377,6 +378,7 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
     hide(pb);
     hide(pw);
     hide(rb);
+    hide(r4b);
     hide(kcb);
     hide(qf);
     hide(gi);
@@ -434,28 +436,29 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
       if (OUT) {
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
-          const u16x8 f = LinTile<K>::rows(qs, rb, tt, b);
+          const u16x8 f = LinTile<K>::rows4(qs, r4b, tt, b);
 #pragma unroll
           for (int T = 0; T < CT; ++T) O[tt][T] = mfma16(sb[T], f, O[tt][T]);
         }
       }
       if (SAVE) {
         // transposed through a product with a selection matrix (exact): lane
-        // (r16, grp) gets key rho_row(t, r16), values 16 ct + 4 grp + r, which
-        // are half a lane's share of the backward's fragment
+        // (r16, grp) gets key 16 t + r16, values 16 ct + 4 grp + r, half of its
+        // share of the backward's fragment (rows4's order)
+        u16x4* dst = states + ((size_t)(sg.chunk0 + c) * Hv + h) * (K / 16) * (V / 32) * 128 +
+                     ((CT * w) >> 1) * 128 + lane * 2 + (CT * w & 1);
 #pragma unroll
-        for (int T = 0; T < CT; ++T) {
-          const int ct = CT * w + T;
-          u16x4* dst = states + ((size_t)(sg.chunk0 + c) * Hv + h) * (K / 16) * (V / 32) * 128 +
-                       (ct >> 1) * 128 + (r16 + 16 * (2 * (ct & 1) + (grp >> 1))) * 2 + (grp & 1);
+        for (int e = 0; e < 2; ++e) {
+          u16x8 sel;
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            u16x8 sel;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              sel[i] = grp == r16 >> 2 && i == 4 * e + (r16 & 3) ? 0x3F80 : 0;
-            dst[(2 * b + e) * (V / 32) * 128] = f2bf4(mfma16(sb[T], sel, zero4()));
-          }
+          for (int i = 0; i < 8; ++i)
+            sel[i] = grp == r16 >> 2 && i == 4 * e + (r16 & 3) ? 0x3F80 : 0;
+          u16x4* at = dst + (2 * b + e) * (V / 32) * 128;
+          const u16x4 x = f2bf4(mfma16(sb[0], sel, zero4()));
+          if constexpr (CT == 2)
+            *reinterpret_cast<u16x8*>(at) = cat8(x, f2bf4(mfma16(sb[1], sel, zero4())));
+          else
+            *at = x;
         }
       }
     }
@@ -478,7 +481,7 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
       u16x8 vf[CT], part[CT][NP];
 #pragma unroll
       for (int T = 0; T < CT; ++T) {
-        vf[T] = LinTile<V>::cols16(vs, vb ^ (32 * T), kb);
+        vf[T] = LinTile<V>::cols(vs, vb, kb, T);
         lin_split(vf[T], sK + 32 * kb + 8 * grp, part[T]);
       }
       if (OUT) {
@@ -514,10 +517,12 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
   }
 }
 
-// 16-column tiles per wave.  Two in the walk read half of what one reads from
+// 16-column tiles per wave.  Two in the walk of a 128-column state read half of what one reads from
 // LDS (packed prompts 873 us against 920); one in the segments leaves room for
 // four waves per SIMD (8192 tokens, both launches: 111 us against 115).
-constexpr int kColTiles = 2, kSegTiles = 1;
+template <int V>
+constexpr int kColTiles = V == 128 ? 2 : 1;
+constexpr int kSegTiles = 1;
 
 // ------------------------------------------------------------------ host ----
 // Chunks per segment: as many as spread all chunks over two workgroups per CU
@@ -635,8 +640,8 @@ void launch_walk(const uint16_t* q, const uint16_t* k, const uint16_t* v, TokenS
   }
   const dim3 items(lin_items(g.nseg, Hqk, Hv));
 #define GDN_LW(NP, OUT, SAVE)                                                                   \
-  hipLaunchKernelGGL((lin_walk_kernel<K, V, kColTiles, NP, OUT, SAVE>), items,                  \
-                     dim3(4 * V / kColTiles), 0, st, q, k, v, ts, d, g, Hqk, Hv, scale, h0, ht, \
+  hipLaunchKernelGGL((lin_walk_kernel<K, V, kColTiles<V>, NP, OUT, SAVE>), items,                  \
+                     dim3(4 * V / kColTiles<V>), 0, st, q, k, v, ts, d, g, Hqk, Hv, scale, h0, ht, \
                      segs, o, states)
   if (o && states) GDN_LW(3, true, true);
   else if (!o) GDN_LW(3, false, true);

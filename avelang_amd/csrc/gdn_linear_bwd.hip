@@ -44,7 +44,9 @@ struct LinGradLds {
   char vs[LinTile<V>::BYTES], os[LinTile<V>::BYTES];
   char ps[LinTile<64>::BYTES], dps[LinTile<64>::BYTES];
   float sG[64], sQ[64], sK[64];   // G log2(e), scale e^G, e^R
-  float rowM[4][64], colM[4][64], asum[K / 32][64], bsum[K / 32][64];
+  // (slots that their writers own and the reader adds up: M's row sums by source
+  // block and lane group, its column sums by token block; a and b by wave and group)
+  float rowM[16][64], colM[4][64], asum[K / 8][64], bsum[K / 8][64];
   float csum[K / 32];
 };
 
@@ -60,7 +62,8 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
   constexpr int NTILE = (VW ? K : V) / 16;
   char *qs = lds.qs, *ks = lds.ks, *vs = lds.vs, *os = lds.os, *ps = lds.ps, *dps = lds.dps;
   float *sG = lds.sG, *sQ = lds.sQ, *sK = lds.sK;
-  auto &rowM = lds.rowM, &colM = lds.colM;
+  auto &rowM = lds.rowM;
+  auto &colM = lds.colM;
   auto &asum = lds.asum, &bsum = lds.bsum;
   float* csum = lds.csum;
   const int tid = threadIdx.x, lane = tid % 64;
@@ -72,14 +75,14 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
   f32x4 ST[NTILE][2];
   const float* src = sg.first && sg.last ? (a.dht ? a.dht + ((size_t)sg.seq * a.Hv + h) * K * V : nullptr)
                              : a.segs + ((size_t)sid * a.Hv + h) * K * V;
-  // a lane's part of the state's address, V waves: row 8 grp (+ the tile's and
+  // a lane's part of the state's address, V waves: row 4 grp (+ the tile's and
   // r), column of value tile T; key waves with rows and columns exchanged
   auto state_at = [&](int lane, int T) {
-    const int r16 = lane % 16, grp = lane / 16, c = 8 * (r16 >> 2) + (r16 & 3) + 4 * T;
-    return (VW ? 8 * grp * V + 32 * wv + c : (32 * wk + c) * V + 8 * grp) * 4;
+    const int r16 = lane % 16, grp = lane / 16, c = 16 * T + r16;
+    return (VW ? 4 * grp * V + 32 * wv + c : (32 * wk + c) * V + 4 * grp) * 4;
   };
   auto tile_at = [&](int t, int r) {
-    return (32 * (t >> 1) + 4 * (t & 1) + r) * (VW ? V : 1) * 4;
+    return (16 * t + r) * (VW ? V : 1) * 4;
   };
   const __amdgpu_buffer_rsrc_t rst = lin_state(src, K * V);
 #pragma unroll
@@ -114,12 +117,14 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
     *reinterpret_cast<u32x4*>(ps + LinTile<64>::off(r, u)) = u32x4{0, 0, 0, 0};
     *reinterpret_cast<u32x4*>(dps + LinTile<64>::off(r, u)) = u32x4{0, 0, 0, 0};
   }
-  for (int i = tid; i < 256; i += NT) rowM[i / 64][i % 64] = colM[i / 64][i % 64] = 0.f;
+  for (int i = tid; i < 1024; i += NT) rowM[i / 64][i % 64] = 0.f;
+  for (int i = tid; i < 256; i += NT) colM[i / 64][i % 64] = 0.f;
   __syncthreads();
   int krb = LinTile<K>::row_base(lane), vrb = LinTile<V>::row_base(lane);
-  int kcb = LinTile<K>::col_base(lane), vcb = LinTile<V>::col_base(lane);
+  int kr4 = LinTile<K>::row4_base(lane), vr4 = LinTile<V>::row4_base(lane);
+  int kcb = LinTile<K>::col_base(0, lane), vcb = LinTile<V>::col_base(0, lane);
   int pb = LinTile<64>::row_base(lane);
-  int pcb = LinTile<64>::col16_base(0, lane);
+  int pcb = LinTile<64>::col_base(0, lane);
   int pw = LinTile<64>::off(lane % 16, lane / 32) + (lane / 16 & 1) * 8;
   // the chunk's gradients leave ahead of the loads issued in the next one: the
   // wait for loads counts stores too
@@ -131,47 +136,32 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
     const int n = min(sg.ntok - c * kChunk, 64);
     const size_t tok = (size_t)sg.tok0 + c * kChunk;
     // (stores past the segment's last token are dropped)
-    if constexpr (VW) {
-      const int row = a.Hv * V * 2, at = r16 * row + (32 * wv + 8 * grp) * 2;
+    // columns 16 T + 4 grp + r of the wave's 32, token 16 tt + r16
+    auto put = [&](void* p, size_t from, int es, int width, const f32x4 (&x)[4][2]) {
+      const int row = a.Hv * width * es, at = r16 * row + (32 * (VW ? wv : wk) + 4 * grp) * es;
       const __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc(
-          a.dv + (tok * a.Hv + h) * V, 0, (n - 1) * row + V * 2, kBufferFlags);
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt)
-        __builtin_amdgcn_raw_buffer_store_b128(
-            __builtin_bit_cast(u32x4, cat8(f2bf4(X[tt][0]), f2bf4(X[tt][1]))), rd,
-            at + tt * 16 * row, 0, 0);
-    } else if (a.pq) {
-      const int row = a.Hv * K * 4, at = r16 * row + (32 * wk + 8 * grp) * 4;
-      const size_t from = (tok * a.Hv + h) * K;
-      const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(
-          a.pq + from, 0, (n - 1) * row + K * 4, kBufferFlags);
-      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-          a.pk + from, 0, (n - 1) * row + K * 4, kBufferFlags);
+          static_cast<char*>(p) + from * width * es, 0, (n - 1) * row + width * es, kBufferFlags);
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, Y[tt][T]), rq,
-                                                 at + tt * 16 * row + 16 * T, 0, 0);
-          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, X[tt][T]), rk,
-                                                 at + tt * 16 * row + 16 * T, 0, 0);
+          if (es == 4)
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, x[tt][T]), rd,
+                                                   at + tt * 16 * row + 64 * T, 0, 0);
+          else
+            __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2p, f2bf4(x[tt][T])), rd,
+                                                  at + tt * 16 * row + 32 * T, 0, 0);
         }
+    };
+    const size_t from = tok * a.Hv + h;
+    if constexpr (VW) {
+      put(a.dv, from, 2, V, X);
+    } else if (a.pq) {
+      put(a.pq, from, 4, K, Y);
+      put(a.pk, from, 4, K, X);
     } else {
-      const int row = a.Hv * K * 2, at = r16 * row + (32 * wk + 8 * grp) * 2;
-      const size_t from = (tok * a.Hv + h) * K;
-      const __amdgpu_buffer_rsrc_t rq = __builtin_amdgcn_make_buffer_rsrc(
-          a.dq + from, 0, (n - 1) * row + K * 2, kBufferFlags);
-      const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-          a.dk + from, 0, (n - 1) * row + K * 2, kBufferFlags);
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        __builtin_amdgcn_raw_buffer_store_b128(
-            __builtin_bit_cast(u32x4, cat8(f2bf4(Y[tt][0]), f2bf4(Y[tt][1]))), rq,
-            at + tt * 16 * row, 0, 0);
-        __builtin_amdgcn_raw_buffer_store_b128(
-            __builtin_bit_cast(u32x4, cat8(f2bf4(X[tt][0]), f2bf4(X[tt][1]))), rk,
-            at + tt * 16 * row, 0, 0);
-      }
+      put(a.dq, from, 2, K, Y);
+      put(a.dk, from, 2, K, X);
     }
   };
   load(nc - 1);
@@ -181,6 +171,8 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
     hide(ln);
     const int lane = ln, r16 = ln % 16, grp = ln / 16;
     hide(krb);
+    hide(kr4);
+    hide(vr4);
     hide(vrb);
     hide(kcb);
     hide(vcb);
@@ -238,14 +230,10 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
       }
       *reinterpret_cast<u16x4*>(ps + (pw ^ (32 * jt)) + it * 2048) = f2bf4(p);
       *reinterpret_cast<u16x4*>(dps + (pw ^ (32 * jt)) + it * 2048) = f2bf4(d);
-      rs += __shfl_xor(rs, 16);
-      rs += __shfl_xor(rs, 32);
-      if (grp == 0) rowM[jt][i] = rs;
+      rowM[4 * jt + grp][i] = rs;
 #pragma unroll
-      for (int o = 1; o < 16; o *= 2)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) M[r] += __shfl_xor(M[r], o);
-      if (r16 == 0) *reinterpret_cast<f32x4*>(&colM[it][j]) = M;
+      for (int r = 0; r < 4; ++r) M[r] = row16_sum(M[r]);
+      if (r16 == 15) *reinterpret_cast<f32x4*>(&colM[it][j]) = M;
     }
 
 #pragma unroll
@@ -259,7 +247,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
         for (int T = 0; T < 2; ++T) df[T] = cat8(f2bf4(ST[2 * b][T]), f2bf4(ST[2 * b + 1][T]));
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
-          const u16x8 kf = LinTile<K>::rows(ks, krb, tt, b);
+          const u16x8 kf = LinTile<K>::rows4(ks, kr4, tt, b);
 #pragma unroll
           for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(df[T], kf, X[tt][T]);
         }
@@ -287,7 +275,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
         }
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
-          const u16x8 vf = LinTile<V>::rows(vs, vrb, tt, b), of = LinTile<V>::rows(os, vrb, tt, b);
+          const u16x8 vf = LinTile<V>::rows4(vs, vr4, tt, b), of = LinTile<V>::rows4(os, vr4, tt, b);
 #pragma unroll
           for (int T = 0; T < 2; ++T) {
             X[tt][T] = mfma16(df[T], vf, X[tt][T]);
@@ -295,34 +283,28 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
           }
         }
       }
-#pragma unroll
-      for (int o = 1; o < 64; o *= 2) cs += __shfl_xor(cs, o);
-      if (lane == 0) csum[wk] = cs;
+      cs = wave_prefix(cs);
+      if (lane == 63) csum[wk] = cs;
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt) {
         const int i = 16 * tt + r16;
         const float fk = sK[i], fq = sQ[i];
-        const u16x8 kr = *reinterpret_cast<const u16x8*>(ks + LinTile<K>::off(i, 4 * wk + grp));
-        const u16x8 qr = *reinterpret_cast<const u16x8*>(qs + LinTile<K>::off(i, 4 * wk + grp));
         float sa = 0.f, sb = 0.f;
 #pragma unroll
         for (int T = 0; T < 2; ++T) {
+          const int at = LinTile<K>::off(i, 4 * wk + 2 * T + (grp >> 1)) + (grp & 1) * 8;
+          const u16x4 kr = *reinterpret_cast<const u16x4*>(ks + at);
+          const u16x4 qr = *reinterpret_cast<const u16x4*>(qs + at);
           X[tt][T] *= fk;
           Y[tt][T] *= fq;
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            sb += bf2f(kr[4 * T + r]) * X[tt][T][r];
-            sa += bf2f(qr[4 * T + r]) * Y[tt][T][r];
+            sb += bf2f(kr[r]) * X[tt][T][r];
+            sa += bf2f(qr[r]) * Y[tt][T][r];
           }
         }
-        sa += __shfl_xor(sa, 16);
-        sb += __shfl_xor(sb, 16);
-        sa += __shfl_xor(sa, 32);
-        sb += __shfl_xor(sb, 32);
-        if (grp == 0) {
-          asum[wk][i] = sa;
-          bsum[wk][i] = sb;
-        }
+        asum[4 * wk + grp][i] = sa;
+        bsum[4 * wk + grp][i] = sb;
       }
     }
     __syncthreads();   // P, dP and the sums
@@ -330,13 +312,16 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
     if (w == 0) {
       float x = 0.f, y = 0.f, cs = 0.f;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) x += rowM[u][lane] - colM[u][lane];
+      for (int u = 0; u < 16; ++u) x += rowM[u][lane];
 #pragma unroll
-      for (int u = 0; u < NK; ++u) {
+      for (int u = 0; u < 4; ++u) x -= colM[u][lane];
+#pragma unroll
+      for (int u = 0; u < 4 * NK; ++u) {
         x += asum[u][lane];
         y += bsum[u][lane];
-        cs += csum[u];
       }
+#pragma unroll
+      for (int u = 0; u < NK; ++u) cs += csum[u];
       // prefix sums of y before the token, and of x from it on (the total less
       // what is before it)
       const float px = wave_prefix(x);
@@ -361,7 +346,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
         }
 #pragma unroll
         for (int tt = 0; tt < 2 * kb + 2; ++tt) {
-          const u16x8 pf = LinTile<64>::cols16(ps, pcb ^ (32 * tt), kb);
+          const u16x8 pf = LinTile<64>::cols(ps, pcb, kb, tt);
 #pragma unroll
           for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(yf[T], pf, X[tt][T]);
         }
@@ -383,7 +368,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
         }
 #pragma unroll
         for (int tt = 0; tt < 2 * kb + 2; ++tt) {
-          const u16x8 pf = LinTile<64>::cols16(dps, pcb ^ (32 * tt), kb);
+          const u16x8 pf = LinTile<64>::cols(dps, pcb, kb, tt);
 #pragma unroll
           for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(yf[T], pf, X[tt][T]);
         }
