@@ -107,6 +107,18 @@ struct LinTile {
     const u16x4 hi = lds_tr16(reinterpret_cast<const uint16_t*>(p + (base ^ 16) + 4 * RS + at));
     return cat8(lo, hi);
   }
+  // The same with the rows in rows4's order: i < 4 row 32 kb + 4 grp + i, the
+  // others 16 further on.
+  static __device__ __forceinline__ int col4_base(int T, int lane) {
+    const int r16 = lane % 16, grp = lane / 16;
+    const int m4 = r16 >> 2, q4 = r16 & 3;
+    return off(4 * grp + m4, 2 * T + (q4 >> 1)) + (q4 & 1) * 8;
+  }
+  static __device__ __forceinline__ u16x8 cols4(const char* p, int base, int kb, int T) {
+    const char* x = p + (base ^ (32 * T)) + kb * 32 * RS;
+    return cat8(lds_tr16(reinterpret_cast<const uint16_t*>(x)),
+                lds_tr16(reinterpret_cast<const uint16_t*>(x + 16 * RS)));
+  }
 };
 
 // The 64 rows of a chunk on their way from HBM to a tile, 16 bytes per lane
@@ -248,9 +260,11 @@ struct LinPlan {
   int nlong;                 // sequences of several segments at most (0: no join)
   size_t table, soff, status, order, joins, segs, decay, total;
   // backward
-  size_t part;               // fp32 partial dq, dk per v-head (Hv > Hqk)
+  size_t part;               // fp32 partial dq, dk (several per qk-head)
   size_t dgtok;              // fp32 dg per token and v-head (one decay per head)
 };
+// Whether the backward takes two v-heads of a qk-head at a time.
+inline bool lin_pair(int Hqk, int Hv) { return Hv / Hqk % 2 == 0; }
 LinPlan lin_plan(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu, bool bwd);
 LinGrid lin_grid(const LinPlan& p, unsigned char* ws, int T, int N, int total, bool has_cu);
 void launch_lin_table(const int32_t* cu, const LinPlan& p, unsigned char* ws, int N, int total,

@@ -559,7 +559,8 @@ LinPlan lin_plan(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu
     p.segs = take((size_t)p.nseg * Hv * K * V * 4);
     p.decay = take((size_t)p.nseg * Hv * 4);
   }
-  if (bwd && Hv > Hqk) p.part = take((size_t)tokens * Hv * K * 8);
+  const int parts = Hv / Hqk / (lin_pair(Hqk, Hv) ? 2 : 1);
+  if (bwd && parts > 1) p.part = take((size_t)tokens * Hqk * parts * K * 8);
   if (bwd) p.dgtok = take((size_t)tokens * Hv * 4);
   p.total = at;
   return p;

@@ -17,6 +17,8 @@
 //
 // Segments as in the forward, walked last chunk to first: a launch for every
 // segment's contribution to D, one that joins them, one for the gradients.
+#include <type_traits>
+
 #include "gdn_linear.h"
 #include "../../include/gdn_linear.h"
 
@@ -34,7 +36,7 @@ struct LinBwdArgs {
   const float* segs;
   const u16x8* states;
   uint16_t *dq, *dk, *dv;
-  float *pq, *pk;      // [tokens][Hv][K] partial dq, dk (NULL: one v-head per qk-head)
+  float *pq, *pk;      // [tokens][Hv / HP][K] partial dq, dk (NULL: none needed)
   float* dg;           // [tokens][Hv]
 };
 
@@ -43,6 +45,7 @@ struct LinGradLds {
   char qs[LinTile<K>::BYTES], ks[LinTile<K>::BYTES];
   char vs[LinTile<V>::BYTES], os[LinTile<V>::BYTES];
   char ps[LinTile<64>::BYTES], dps[LinTile<64>::BYTES];
+  char ds[2 * V * K];             // D^T as bf16, rows of K
   float sG[64], sQ[64], sK[64];   // G log2(e), scale e^G, e^R
   // (slots that their writers own and the reader adds up: M's row sums by source
   // block and lane group, its column sums by token block; a and b by wave and group)
@@ -50,63 +53,64 @@ struct LinGradLds {
   float csum[K / 32];
 };
 
-// A workgroup walks one segment of one v-head.  V / 32 waves own 32 columns
-// of D each (dv and dh0), K / 32 waves 32 columns of D^T (dk and dq, which
-// reduce over V, and with the saved states' fragments <S, D>): D is kept in
-// both orientations so that neither ever leaves the registers.  This is one
-// wave's walk, VW: of the first kind.  Both kinds meet the same barriers.
-template <int K, int V, bool VW, int NP>
-__device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg& sg, int sid, int h,
+// What one wave of lin_grad_kernel does (see there).
+template <int K, int V, int HP, int NP, bool VW>
+__device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg& sg, int sid, int hp,
                                               int w, LinGradLds<K, V>& lds) {
-  constexpr int NT = 2 * (K + V), NV = V / 32, NK = K / 32, NW = NV + NK;
-  constexpr int NTILE = (VW ? K : V) / 16;
+  constexpr int NT = 2 * (K + V), NV = V / 32, NK = K / 32;
+  // who brings the tiles in: with four key waves those alone (two heads' D leave
+  // the V waves no registers for it), else all
+  constexpr bool BY_KEYS = NK == 4, BRINGS = !BY_KEYS || !VW;
+  constexpr int NS = BY_KEYS ? 64 * NK : NT;
   char *qs = lds.qs, *ks = lds.ks, *vs = lds.vs, *os = lds.os, *ps = lds.ps, *dps = lds.dps;
+  char* ds = lds.ds;
   float *sG = lds.sG, *sQ = lds.sQ, *sK = lds.sK;
-  auto &rowM = lds.rowM;
-  auto &colM = lds.colM;
-  auto &asum = lds.asum, &bsum = lds.bsum;
-  float* csum = lds.csum;
   const int tid = threadIdx.x, lane = tid % 64;
-  const int hq = h / (a.Hv / a.Hqk);
+  const int h0 = hp * HP, hq = h0 / (a.Hv / a.Hqk);
   const int nc = (sg.ntok + kChunk - 1) / kChunk;
   const int wk = VW ? 0 : w - NV, wv = VW ? w : 0;   // the wave's 32 columns
 
-  // ST[t][T]: D (key tile t, value tile T), or D^T (value tile t, key tile T)
-  f32x4 ST[NTILE][2];
-  const float* src = sg.first && sg.last ? (a.dht ? a.dht + ((size_t)sg.seq * a.Hv + h) * K * V : nullptr)
-                             : a.segs + ((size_t)sid * a.Hv + h) * K * V;
-  // a lane's part of the state's address, V waves: row 4 grp (+ the tile's and
-  // r), column of value tile T; key waves with rows and columns exchanged
+  // V waves: D of each head, rows (keys) 16 t + 4 grp + r, columns 32 wv + 16 T + r16
+  f32x4 ST[HP][K / 16][2];
   auto state_at = [&](int lane, int T) {
-    const int r16 = lane % 16, grp = lane / 16, c = 16 * T + r16;
-    return (VW ? 4 * grp * V + 32 * wv + c : (32 * wk + c) * V + 4 * grp) * 4;
+    return (4 * (lane / 16) * V + 32 * wv + 16 * T + lane % 16) * 4;
   };
-  auto tile_at = [&](int t, int r) {
-    return (16 * t + r) * (VW ? V : 1) * 4;
-  };
-  const __amdgpu_buffer_rsrc_t rst = lin_state(src, K * V);
+  if constexpr (VW) {
 #pragma unroll
-  for (int t = 0; t < NTILE; ++t)
+    for (int hh = 0; hh < HP; ++hh) {
+      const int h = h0 + hh;
+      const float* src =
+          sg.first && sg.last ? (a.dht ? a.dht + ((size_t)sg.seq * a.Hv + h) * K * V : nullptr)
+                              : a.segs + ((size_t)sid * a.Hv + h) * K * V;
+      const __amdgpu_buffer_rsrc_t rst = lin_state(src, K * V);
 #pragma unroll
-    for (int T = 0; T < 2; ++T)
+      for (int t = 0; t < K / 16; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        ST[t][T][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
-            rst, state_at(lane, T), tile_at(t, r), 0));
+        for (int T = 0; T < 2; ++T)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            ST[hh][t][T][r] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(
+                rst, state_at(lane, T), (16 * t + r) * V * 4, 0));
+    }
+  }
 
-  LinStage<K, NT> sq, sk;
-  LinStage<V, NT> sv, so;
+  LinStage<K, NS> sq, sk;
+  LinStage<V, NS> sv, so;
   LinGates lg;
+  const int st = BY_KEYS ? tid - 64 * NV : tid;
   int gi = LinGates::token(w, lane);
-  int qf = LinStage<K, NT>::from(a.ts.q, tid), kf = LinStage<K, NT>::from(a.ts.k, tid);
-  int vf = LinStage<V, NT>::from(a.ts.v, tid), of = LinStage<V, NT>::from(a.Hv * V, tid);
-  const int kt = LinStage<K, NT>::at(tid, 0), vt = LinStage<V, NT>::at(tid, 0);
-  auto load = [&](int c) {
-    const int n = c >= 0 ? sg.ntok - c * kChunk : 0;
+  int qf = LinStage<K, NS>::from(a.ts.q, st), kf = LinStage<K, NS>::from(a.ts.k, st);
+  int vf = LinStage<V, NS>::from(a.ts.v, st), of = LinStage<V, NS>::from(a.Hv * V, st);
+  const int kt = LinStage<K, NS>::at(st, 0), vt = LinStage<V, NS>::at(st, 0);
+  auto load = [&](int c, int hh) {
+    const int n = c >= 0 ? sg.ntok - c * kChunk : 0, h = h0 + hh;
     const size_t t = n > 0 ? (size_t)sg.tok0 + c * kChunk : 0;
     if (w < 2) lg.load(a.dec, t, min(n, 64), h, a.Hv, gi);
-    sq.load(a.q + t * a.ts.q + hq * K, a.ts.q, min(n, 64), qf);
-    sk.load(a.k + t * a.ts.k + hq * K, a.ts.k, min(n, 64), kf);
+    if constexpr (!BRINGS) return;
+    if (hh == 0) {
+      sq.load(a.q + t * a.ts.q + hq * K, a.ts.q, min(n, 64), qf);
+      sk.load(a.k + t * a.ts.k + hq * K, a.ts.k, min(n, 64), kf);
+    }
     sv.load(a.v + t * a.ts.v + h * V, a.ts.v, min(n, 64), vf);
     so.load(a.dO + (t * a.Hv + h) * V, a.Hv * V, min(n, 64), of);
   };
@@ -117,30 +121,33 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
     *reinterpret_cast<u32x4*>(ps + LinTile<64>::off(r, u)) = u32x4{0, 0, 0, 0};
     *reinterpret_cast<u32x4*>(dps + LinTile<64>::off(r, u)) = u32x4{0, 0, 0, 0};
   }
-  for (int i = tid; i < 1024; i += NT) rowM[i / 64][i % 64] = 0.f;
-  for (int i = tid; i < 256; i += NT) colM[i / 64][i % 64] = 0.f;
+  for (int i = tid; i < 1024; i += NT) lds.rowM[i / 64][i % 64] = 0.f;
+  for (int i = tid; i < 256; i += NT) lds.colM[i / 64][i % 64] = 0.f;
   __syncthreads();
+
   int krb = LinTile<K>::row_base(lane), vrb = LinTile<V>::row_base(lane);
   int kr4 = LinTile<K>::row4_base(lane), vr4 = LinTile<V>::row4_base(lane);
   int kcb = LinTile<K>::col_base(0, lane), vcb = LinTile<V>::col_base(0, lane);
-  int pb = LinTile<64>::row_base(lane);
-  int pcb = LinTile<64>::col_base(0, lane);
+  int pb = LinTile<64>::row_base(lane), pcb = LinTile<64>::col_base(0, lane);
   int pw = LinTile<64>::off(lane % 16, lane / 32) + (lane / 16 & 1) * 8;
-  // the chunk's gradients leave ahead of the loads issued in the next one: the
-  // wait for loads counts stores too
-  f32x4 X[4][2], Y[4][2];   // dv; or dk and dq (by token tile)
-  auto store_grads = [&](int c) {
+  int dcb = LinTile<K>::col4_base(2 * wk, lane);            // key waves: D^T read
+  int dwb = LinTile<K>::row4_base(lane) + 32 * wv * 2 * K;   // V waves: D^T written
+  // A chunk's gradients leave ahead of the loads issued after it: the wait for
+  // loads counts stores too.
+  f32x4 X[4][2], Y[4][2];   // dv; or dk and dq, over the heads (by token tile)
+  auto store_grads = [&](int c, int h) {
     int ln = lane;
     hide(ln);
     const int r16 = ln % 16, grp = ln / 16;
     const int n = min(sg.ntok - c * kChunk, 64);
     const size_t tok = (size_t)sg.tok0 + c * kChunk;
-    // (stores past the segment's last token are dropped)
-    // columns 16 T + 4 grp + r of the wave's 32, token 16 tt + r16
-    auto put = [&](void* p, size_t from, int es, int width, const f32x4 (&x)[4][2]) {
-      const int row = a.Hv * width * es, at = r16 * row + (32 * (VW ? wv : wk) + 4 * grp) * es;
+    // columns 16 T + 4 grp + r of the wave's 32, token 16 tt + r16 (stores past
+    // the segment's last token are dropped)
+    auto put = [&](void* p, int heads, int hd, int es, int width, const f32x4 (&x)[4][2]) {
+      const int row = heads * width * es, at = r16 * row + (32 * (VW ? wv : wk) + 4 * grp) * es;
       const __amdgpu_buffer_rsrc_t rd = __builtin_amdgcn_make_buffer_rsrc(
-          static_cast<char*>(p) + from * width * es, 0, (n - 1) * row + width * es, kBufferFlags);
+          static_cast<char*>(p) + (tok * heads + hd) * width * es, 0, (n - 1) * row + width * es,
+          kBufferFlags);
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
@@ -153,43 +160,62 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
                                                   at + tt * 16 * row + 32 * T, 0, 0);
         }
     };
-    const size_t from = tok * a.Hv + h;
     if constexpr (VW) {
-      put(a.dv, from, 2, V, X);
+      put(a.dv, a.Hv, h, 2, V, X);
     } else if (a.pq) {
-      put(a.pq, from, 4, K, Y);
-      put(a.pk, from, 4, K, X);
+      put(a.pq, a.Hv / HP, hp, 4, K, Y);
+      put(a.pk, a.Hv / HP, hp, 4, K, X);
     } else {
-      put(a.dq, from, 2, K, Y);
-      put(a.dk, from, 2, K, X);
+      put(a.dq, a.Hqk, hq, 2, K, Y);
+      put(a.dk, a.Hqk, hq, 2, K, X);
     }
   };
-  load(nc - 1);
-  for (int c = nc - 1; c >= 0; --c) {
-    // (nothing derived from these is kept from one chunk for the next)
+  // key waves: the saved state's fragments of their keys, an iteration ahead
+  u16x8 SF[2][V / 32];
+  auto load_states = [&](int c, int hh) {
+    const u16x8* sp = a.states + (((size_t)(sg.chunk0 + max(c, 0)) * a.Hv + h0 + hh) * (K / 16) +
+                                  2 * wk) * (V / 32) * 64 + lane;
+#pragma unroll
+    for (int T = 0; T < 2; ++T)
+#pragma unroll
+      for (int b = 0; b < V / 32; ++b) SF[T][b] = sp[(T * (V / 32) + b) * 64];
+  };
+  auto zero = [](f32x4 (&x)[4][2]) {
+#pragma unroll
+    for (int tt = 0; tt < 4; ++tt) x[tt][0] = x[tt][1] = zero4();
+  };
+
+  auto iterate = [&](int c, auto head) {
+    constexpr int hh = decltype(head)::value;
+    const int h = h0 + hh;
+    // (nothing derived from these is kept from one iteration for the next)
     int ln = lane;
     hide(ln);
     const int lane = ln, r16 = ln % 16, grp = ln / 16;
     hide(krb);
+    hide(vrb);
     hide(kr4);
     hide(vr4);
-    hide(vrb);
     hide(kcb);
     hide(vcb);
     hide(pb);
     hide(pw);
     hide(pcb);
+    hide(dcb);
+    hide(dwb);
     hide(qf);
     hide(kf);
     hide(vf);
     hide(of);
     hide(gi);
-    const int n = sg.ntok - c * kChunk;
-    const size_t tok = (size_t)sg.tok0 + c * kChunk;
-    sq.store(qs, kt, tid);
-    sk.store(ks, kt, tid);
-    sv.store(vs, vt, tid);
-    so.store(os, vt, tid);
+    if constexpr (BRINGS) {
+      if (hh == 0) {
+        sq.store(qs, kt, st);
+        sk.store(ks, kt, st);
+      }
+      sv.store(vs, vt, st);
+      so.store(os, vt, st);
+    }
     if (w < 2) {
       const float pre = lg.prefix(a.dec, gi) * kLog2e, e = exp2_(pre);
       if (w == 1) {
@@ -199,57 +225,34 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
         sQ[lane] = a.scale * e;
       }
     }
-    __syncthreads();
-    if (c < nc - 1) store_grads(c + 1);
-    load(c - 1);
-
-    // P and dP, tile by tile, as bf16 rows, and the sums of M
-    for (int m = w; m < 10; m += NW) {
-      const int it = tmat_block_row(m), jt = m - tmat_block(it, 0);
-      f32x4 p = zero4(), d = zero4();
+    if constexpr (VW) {
 #pragma unroll
-      for (int kb = 0; kb < K / 32; ++kb)
-        p = mfma16(LinTile<K>::rows(ks, krb, jt, kb), LinTile<K>::rows(qs, krb, it, kb), p);
+      for (int t = 0; t < K / 16; ++t)
 #pragma unroll
-      for (int kb = 0; kb < V / 32; ++kb)
-        d = mfma16(LinTile<V>::rows(vs, vrb, jt, kb), LinTile<V>::rows(os, vrb, it, kb), d);
-      const int i = 16 * it + r16, j = 16 * jt + 4 * grp;
-      const f32x4 gj = *reinterpret_cast<const f32x4*>(&sG[j]);
-      const float gi = sG[i];
-      f32x4 M;
-      float rs = 0.f;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const bool in = j + r <= i;
-        const float gam = a.scale * exp2_(in ? gi - gj[r] : 0.f);
-        d[r] = in ? d[r] : 0.f;
-        p[r] = (in ? p[r] : 0.f) * gam;
-        M[r] = p[r] * d[r];
-        d[r] *= gam;
-        rs += M[r];
-      }
-      *reinterpret_cast<u16x4*>(ps + (pw ^ (32 * jt)) + it * 2048) = f2bf4(p);
-      *reinterpret_cast<u16x4*>(dps + (pw ^ (32 * jt)) + it * 2048) = f2bf4(d);
-      rowM[4 * jt + grp][i] = rs;
-#pragma unroll
-      for (int r = 0; r < 4; ++r) M[r] = row16_sum(M[r]);
-      if (r16 == 15) *reinterpret_cast<f32x4*>(&colM[it][j]) = M;
+        for (int T = 0; T < 2; ++T)
+          *reinterpret_cast<u16x4*>(ds + (dwb ^ (32 * t)) + T * 16 * 2 * K) = f2bf4(ST[hh][t][T]);
     }
+    __syncthreads();
+    if (VW ? c < nc - 1 || hh > 0 : c < nc - 1 && hh == 0)
+      store_grads(hh > 0 ? c : c + 1, VW ? (hh > 0 ? h - 1 : h0 + HP - 1) : h0);
+    if (hh + 1 < HP) load(c, hh + 1);
+    else load(c - 1, 0);
 
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt) X[tt][0] = X[tt][1] = Y[tt][0] = Y[tt][1] = zero4();
     const float eC = exp2_(sG[63]);
     if constexpr (VW) {
+      // dv's part of D, then D of the chunk before
+      zero(X);
 #pragma unroll
       for (int b = 0; b < K / 32; ++b) {
         u16x8 df[2];
 #pragma unroll
-        for (int T = 0; T < 2; ++T) df[T] = cat8(f2bf4(ST[2 * b][T]), f2bf4(ST[2 * b + 1][T]));
+        for (int T = 0; T < 2; ++T)
+          df[T] = cat8(f2bf4(ST[hh][2 * b][T]), f2bf4(ST[hh][2 * b + 1][T]));
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
-          const u16x8 kf = LinTile<K>::rows4(ks, kr4, tt, b);
+          const u16x8 f = LinTile<K>::rows4(ks, kr4, tt, b);
 #pragma unroll
-          for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(df[T], kf, X[tt][T]);
+          for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(df[T], f, X[tt][T]);
         }
       }
 #pragma unroll
@@ -258,154 +261,197 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
         X[tt][0] *= f;
         X[tt][1] *= f;
       }
-    } else {
-      const u16x8* sp = a.states + (((size_t)(sg.chunk0 + c) * a.Hv + h) * (K / 16) + 2 * wk) *
-                                       (V / 32) * 64 + lane;
-      float cs = 0.f;
 #pragma unroll
-      for (int b = 0; b < V / 32; ++b) {
-        u16x8 df[2], sf[2];
-#pragma unroll
-        for (int T = 0; T < 2; ++T) {
-          sf[T] = sp[(T * (V / 32) + b) * 64];
-          df[T] = cat8(f2bf4(ST[2 * b][T]), f2bf4(ST[2 * b + 1][T]));
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            cs += bf2f(sf[T][r]) * ST[2 * b][T][r] + bf2f(sf[T][4 + r]) * ST[2 * b + 1][T][r];
-        }
-#pragma unroll
-        for (int tt = 0; tt < 4; ++tt) {
-          const u16x8 vf = LinTile<V>::rows4(vs, vr4, tt, b), of = LinTile<V>::rows4(os, vr4, tt, b);
-#pragma unroll
-          for (int T = 0; T < 2; ++T) {
-            X[tt][T] = mfma16(df[T], vf, X[tt][T]);
-            Y[tt][T] = mfma16(sf[T], of, Y[tt][T]);
-          }
-        }
-      }
-      cs = wave_prefix(cs);
-      if (lane == 63) csum[wk] = cs;
-#pragma unroll
-      for (int tt = 0; tt < 4; ++tt) {
-        const int i = 16 * tt + r16;
-        const float fk = sK[i], fq = sQ[i];
-        float sa = 0.f, sb = 0.f;
-#pragma unroll
-        for (int T = 0; T < 2; ++T) {
-          const int at = LinTile<K>::off(i, 4 * wk + 2 * T + (grp >> 1)) + (grp & 1) * 8;
-          const u16x4 kr = *reinterpret_cast<const u16x4*>(ks + at);
-          const u16x4 qr = *reinterpret_cast<const u16x4*>(qs + at);
-          X[tt][T] *= fk;
-          Y[tt][T] *= fq;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            sb += bf2f(kr[r]) * X[tt][T][r];
-            sa += bf2f(qr[r]) * Y[tt][T][r];
-          }
-        }
-        asum[4 * wk + grp][i] = sa;
-        bsum[4 * wk + grp][i] = sb;
-      }
-    }
-    __syncthreads();   // P, dP and the sums
-
-    if (w == 0) {
-      float x = 0.f, y = 0.f, cs = 0.f;
-#pragma unroll
-      for (int u = 0; u < 16; ++u) x += rowM[u][lane];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) x -= colM[u][lane];
-#pragma unroll
-      for (int u = 0; u < 4 * NK; ++u) {
-        x += asum[u][lane];
-        y += bsum[u][lane];
+      for (int t = 0; t < K / 16; ++t) {
+        ST[hh][t][0] *= eC;
+        ST[hh][t][1] *= eC;
       }
 #pragma unroll
-      for (int u = 0; u < NK; ++u) cs += csum[u];
-      // prefix sums of y before the token, and of x from it on (the total less
-      // what is before it)
-      const float px = wave_prefix(x);
-      const float tx = __builtin_bit_cast(
-          float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, px), 63));
-      const float dg = eC * cs + (tx - px + x) + (wave_prefix(y) - y);
-      if (lane < n) a.dg[(tok + lane) * a.Hv + h] = dg;
-    }
+      for (int kb = 0; kb < 2; ++kb) {
+        u16x8 part[2][NP];
 #pragma unroll
-    for (int t = 0; t < NTILE; ++t) {
-      ST[t][0] *= eC;
-      ST[t][1] *= eC;
-    }
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      u16x8 yf[2], part[2][NP];
-      if constexpr (VW) {
-#pragma unroll
-        for (int T = 0; T < 2; ++T) {
-          yf[T] = LinTile<V>::cols(os, vcb, kb, 2 * wv + T);
-          lin_split(yf[T], sQ + 32 * kb + 8 * grp, part[T]);
-        }
-#pragma unroll
-        for (int tt = 0; tt < 2 * kb + 2; ++tt) {
-          const u16x8 pf = LinTile<64>::cols(ps, pcb, kb, tt);
-#pragma unroll
-          for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(yf[T], pf, X[tt][T]);
-        }
+        for (int T = 0; T < 2; ++T)
+          lin_split(LinTile<V>::cols(os, vcb, kb, 2 * wv + T), sQ + 32 * kb + 8 * grp, part[T]);
 #pragma unroll
         for (int t = 0; t < K / 16; ++t) {
           const u16x8 f = LinTile<K>::cols(qs, kcb, kb, t);
 #pragma unroll
           for (int p = 0; p < NP; ++p)
 #pragma unroll
-            for (int T = 0; T < 2; ++T) ST[t][T] = mfma16(f, part[T][p], ST[t][T]);
+            for (int T = 0; T < 2; ++T) ST[hh][t][T] = mfma16(f, part[T][p], ST[hh][t][T]);
         }
-      } else {
-        u16x8 kf[2];
+      }
+    } else {
+      // P and dP, tile by tile, as bf16 rows, and the sums of M
+      for (int m = wk; m < 10; m += NK) {
+        const int it = tmat_block_row(m), jt = m - tmat_block(it, 0);
+        f32x4 p = zero4(), d = zero4();
 #pragma unroll
-        for (int T = 0; T < 2; ++T) {
-          yf[T] = LinTile<K>::cols(qs, kcb, kb, 2 * wk + T);
-          kf[T] = LinTile<K>::cols(ks, kcb, kb, 2 * wk + T);
-          lin_split(yf[T], sQ + 32 * kb + 8 * grp, part[T]);
+        for (int kb = 0; kb < K / 32; ++kb)
+          p = mfma16(LinTile<K>::rows(ks, krb, jt, kb), LinTile<K>::rows(qs, krb, it, kb), p);
+#pragma unroll
+        for (int kb = 0; kb < V / 32; ++kb)
+          d = mfma16(LinTile<V>::rows(vs, vrb, jt, kb), LinTile<V>::rows(os, vrb, it, kb), d);
+        const int i = 16 * it + r16, j = 16 * jt + 4 * grp;
+        const f32x4 gj = *reinterpret_cast<const f32x4*>(&sG[j]);
+        const float gi = sG[i];
+        f32x4 M;
+        float rs = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool in = j + r <= i;
+          const float gam = a.scale * exp2_(in ? gi - gj[r] : 0.f);
+          d[r] = in ? d[r] : 0.f;
+          p[r] = (in ? p[r] : 0.f) * gam;
+          M[r] = p[r] * d[r];
+          d[r] *= gam;
+          rs += M[r];
+        }
+        *reinterpret_cast<u16x4*>(ps + (pw ^ (32 * jt)) + it * 2048) = f2bf4(p);
+        *reinterpret_cast<u16x4*>(dps + (pw ^ (32 * jt)) + it * 2048) = f2bf4(d);
+        lds.rowM[4 * jt + grp][i] = rs;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) M[r] = row16_sum(M[r]);
+        if (r16 == 15) *reinterpret_cast<f32x4*>(&lds.colM[it][j]) = M;
+      }
+      if (hh == 0) {
+        zero(X);
+        zero(Y);
+      }
+      // the parts of dk from D and of dq from S: products, then the tokens' factors
+      auto inter = [&](f32x4 (&out)[4][2], const float* fac, const char* own, auto sums, auto&& op,
+                       auto&& rows) {
+        f32x4 Z[4][2];
+        zero(Z);
+#pragma unroll
+        for (int b = 0; b < V / 32; ++b) {
+          u16x8 f[2];
+#pragma unroll
+          for (int T = 0; T < 2; ++T) f[T] = op(T, b);
+#pragma unroll
+          for (int tt = 0; tt < 4; ++tt) {
+            const u16x8 x = rows(tt, b);
+#pragma unroll
+            for (int T = 0; T < 2; ++T) Z[tt][T] = mfma16(f[T], x, Z[tt][T]);
+          }
         }
 #pragma unroll
-        for (int tt = 0; tt < 2 * kb + 2; ++tt) {
-          const u16x8 pf = LinTile<64>::cols(dps, pcb, kb, tt);
+        for (int tt = 0; tt < 4; ++tt) {
+          const int i = 16 * tt + r16;
+          const float e = fac[i];
+          float s = 0.f;
 #pragma unroll
-          for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(yf[T], pf, X[tt][T]);
+          for (int T = 0; T < 2; ++T) {
+            Z[tt][T] *= e;
+            out[tt][T] += Z[tt][T];
+            const u16x4 x = *reinterpret_cast<const u16x4*>(
+                own + LinTile<K>::off(i, 4 * wk + 2 * T + (grp >> 1)) + (grp & 1) * 8);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s += bf2f(x[r]) * Z[tt][T][r];
+          }
+          sums[4 * wk + grp][i] = s;
         }
+      };
+      float cs = 0.f;
+      inter(X, sK, ks, lds.bsum,
+            [&](int T, int b) {
+              const u16x8 f = LinTile<K>::cols4(ds, dcb, b, T);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) cs += bf2f(f[i]) * bf2f(SF[T][b][i]);
+              return f;
+            },
+            [&](int tt, int b) { return LinTile<V>::rows4(vs, vr4, tt, b); });
+      inter(Y, sQ, qs, lds.asum, [&](int T, int b) { return SF[T][b]; },
+            [&](int tt, int b) { return LinTile<V>::rows4(os, vr4, tt, b); });
+      if (hh + 1 < HP) load_states(c, hh + 1);
+      else load_states(c - 1, 0);
+      cs = wave_prefix(cs);
+      if (lane == 63) lds.csum[wk] = cs;
+    }
+    __syncthreads();   // P, dP and the sums
+
+    if (VW && w == 0) {
+      float x = 0.f, y = 0.f, cs = 0.f;
+#pragma unroll
+      for (int u = 0; u < 16; ++u) x += lds.rowM[u][lane];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) x -= lds.colM[u][lane];
+#pragma unroll
+      for (int u = 0; u < 4 * NK; ++u) {
+        x += lds.asum[u][lane];
+        y += lds.bsum[u][lane];
+      }
+#pragma unroll
+      for (int u = 0; u < NK; ++u) cs += lds.csum[u];
+      // prefix sums of y before the token, and of x from it on (the total less
+      // what is before it)
+      const float px = wave_prefix(x);
+      const float dg = eC * cs + (lane63(px) - px + x) + (wave_prefix(y) - y);
+      const int n = sg.ntok - c * kChunk;
+      if (lane < n) a.dg[((size_t)sg.tok0 + c * kChunk + lane) * a.Hv + h] = dg;
+    }
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      u16x8 f[2];
+#pragma unroll
+      for (int T = 0; T < 2; ++T)
+        f[T] = VW ? LinTile<V>::cols(os, vcb, kb, 2 * wv + T) : LinTile<K>::cols(qs, kcb, kb, 2 * wk + T);
+#pragma unroll
+      for (int tt = 0; tt < 2 * kb + 2; ++tt) {
+        const u16x8 pf = LinTile<64>::cols(VW ? ps : dps, pcb, kb, tt);
+#pragma unroll
+        for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(f[T], pf, X[tt][T]);
+      }
+      if constexpr (!VW) {
+#pragma unroll
+        for (int T = 0; T < 2; ++T) f[T] = LinTile<K>::cols(ks, kcb, kb, 2 * wk + T);
 #pragma unroll
         for (int tt = 2 * kb; tt < 4; ++tt) {
           const u16x8 pf = LinTile<64>::rows(dps, pb, tt, kb);
 #pragma unroll
-          for (int T = 0; T < 2; ++T) Y[tt][T] = mfma16(kf[T], pf, Y[tt][T]);
-        }
-#pragma unroll
-        for (int t = 0; t < V / 16; ++t) {
-          const u16x8 f = LinTile<V>::cols(os, vcb, kb, t);
-#pragma unroll
-          for (int p = 0; p < NP; ++p)
-#pragma unroll
-            for (int T = 0; T < 2; ++T) ST[t][T] = mfma16(f, part[T][p], ST[t][T]);
+          for (int T = 0; T < 2; ++T) Y[tt][T] = mfma16(f[T], pf, Y[tt][T]);
         }
       }
     }
     __syncthreads();
+  };
+
+  if constexpr (!VW) {
+    if (nc > 0) load_states(nc - 1, 0);
   }
-  if (nc > 0) store_grads(0);
-  if (a.dh0 && sg.first && VW) {
-    const __amdgpu_buffer_rsrc_t rd = lin_state(a.dh0 + ((size_t)sg.seq * a.Hv + h) * K * V, K * V);
+  load(nc - 1, 0);
+  for (int c = nc - 1; c >= 0; --c) {
+    iterate(c, std::integral_constant<int, 0>{});
+    if constexpr (HP == 2) iterate(c, std::integral_constant<int, 1>{});
+  }
+  if (nc > 0) store_grads(0, VW ? h0 + HP - 1 : h0);
+  if constexpr (VW) {
+    if (a.dh0 && sg.first) {
 #pragma unroll
-    for (int t = 0; t < K / 16; ++t)
+      for (int hh = 0; hh < HP; ++hh) {
+        const __amdgpu_buffer_rsrc_t rd =
+            lin_state(a.dh0 + ((size_t)sg.seq * a.Hv + h0 + hh) * K * V, K * V);
 #pragma unroll
-      for (int T = 0; T < 2; ++T)
+        for (int t = 0; t < K / 16; ++t)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(ST[t][T][r]), rd, state_at(lane, T),
-                                                tile_at(t, r), 0);
+          for (int T = 0; T < 2; ++T)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(ST[hh][t][T][r]), rd,
+                                                    state_at(lane, T), (16 * t + r) * V * 4, 0);
+      }
+    }
   }
 }
 
-// NP: the parts of dO's products on the way to dh0 (three where it is wanted).
-template <int K, int V, int NP>
+// A workgroup walks one segment of HP v-heads of one qk-head, chunk by chunk
+// and in each chunk head by head: q and k are staged once, dk and dq add up
+// over the heads in registers.  V / 32 waves own 32 columns of every D (dv,
+// dh0) and leave it as bf16 in LDS for the K / 32 waves that own 32 key columns
+// (dk, dq, P, dP and with the saved states' fragments <S, D>, all of which
+// reduce over V).  NP: the parts of dO's products on the way to dh0 (three
+// where it is wanted).
+template <int K, int V, int HP, int NP>
 __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) {
   constexpr int NT = 2 * (K + V);
   __shared__ __align__(16) LinGradLds<K, V> lds;
@@ -421,17 +467,17 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
     }
     for (size_t i = i0; i < ng; i += st) a.dg[i] = 0.f;
   }
-  int sid, h;
-  if (!lin_item(a.grid, a.grid.nseg, a.Hqk, a.Hv, sid, h)) return;
+  int sid, hp;
+  if (!lin_item(a.grid, a.grid.nseg, a.Hqk, a.Hv / HP, sid, hp)) return;
   if (a.grid.table) sid = a.grid.order[sid];
   const LinSeg sg = lin_seg(a.grid, sid);
   if (sg.seq < 0) return;
   const int w = wave_index();
-  if (w < V / 32) lin_grad_walk<K, V, true, NP>(a, sg, sid, h, w, lds);
-  else lin_grad_walk<K, V, false, 2>(a, sg, sid, h, w, lds);
+  if (w < V / 32) lin_grad_walk<K, V, HP, NP, true>(a, sg, sid, hp, w, lds);
+  else lin_grad_walk<K, V, HP, NP, false>(a, sg, sid, hp, w, lds);
 }
 
-// dq, dk of a qk-head: the sum of its v-heads' parts, 8 elements per lane.
+// dq, dk of a qk-head: the sum of its rep parts, 8 elements per lane.
 __global__ __launch_bounds__(256) void lin_group_sum_kernel(const float* __restrict__ pq,
                                                             const float* __restrict__ pk,
                                                             uint16_t* __restrict__ dq,
@@ -480,9 +526,17 @@ void launch_grad(const LinBwdArgs& a, float* segs, float* decay, hipStream_t st)
   if (a.grid.nlong > 0)
     launch_lin_segments<K, V>(a.q, a.ts.q, a.dO, a.Hv * V, a.dec, a.grid, a.Hqk, a.Hv, a.scale,
                               true, a.dh0 != nullptr, a.dht, segs, decay, nullptr, st);
-  const dim3 items(lin_items(a.grid.nseg, a.Hqk, a.Hv));
-  if (a.dh0) hipLaunchKernelGGL((lin_grad_kernel<K, V, 3>), items, dim3(2 * (K + V)), 0, st, a);
-  else hipLaunchKernelGGL((lin_grad_kernel<K, V, 2>), items, dim3(2 * (K + V)), 0, st, a);
+#define GDN_LG(HP, NP)                                                                       \
+  hipLaunchKernelGGL((lin_grad_kernel<K, V, HP, NP>),                                        \
+                     dim3(lin_items(a.grid.nseg, a.Hqk, a.Hv / HP)), dim3(2 * (K + V)), 0, st, a)
+  if (lin_pair(a.Hqk, a.Hv)) {
+    if (a.dh0) GDN_LG(2, 3);
+    else GDN_LG(2, 2);
+  } else {
+    if (a.dh0) GDN_LG(1, 3);
+    else GDN_LG(1, 2);
+  }
+#undef GDN_LG
 }
 }  // namespace
 
@@ -548,9 +602,10 @@ extern "C" int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v,
     a.dk = static_cast<uint16_t*>(dk);
     a.dv = static_cast<uint16_t*>(dv);
     a.dg = dgt;
-    if (Hv > Hqk) {
+    const int parts = Hv / Hqk / (gdn::lin_pair(Hqk, Hv) ? 2 : 1);   // of a qk-head's gradients
+    if (parts > 1) {
       a.pq = reinterpret_cast<float*>(ws + p.part);
-      a.pk = a.pq + tokens * Hv * K;
+      a.pk = a.pq + tokens * Hqk * parts * K;
     }
     float* segs = reinterpret_cast<float*>(ws + p.segs);
     float* decay = reinterpret_cast<float*>(ws + p.decay);
@@ -562,7 +617,7 @@ extern "C" int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v,
     if (a.pq && tokens > 0)
       hipLaunchKernelGGL(gdn::lin_group_sum_kernel,
                          dim3((unsigned)((tokens * Hqk * K / 8 + 255) / 256), 2), dim3(256), 0, st,
-                         a.pq, a.pk, a.dq, a.dk, grid.status, tokens * Hqk, Hv / Hqk, K);
+                         a.pq, a.pk, a.dq, a.dk, grid.status, tokens * Hqk, parts, K);
   }
   if (g_per_head)
     hipLaunchKernelGGL(gdn::lin_head_sum_kernel, dim3(Hv), dim3(1024), 0, st, dgt, dg, (int)tokens, Hv);
