@@ -58,10 +58,11 @@ template <int K, int V, int HP, int NP, bool VW>
 __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg& sg, int sid, int hp,
                                               int w, LinGradLds<K, V>& lds) {
   constexpr int NT = 2 * (K + V), NV = V / 32, NK = K / 32;
-  // who brings the tiles in: with four key waves those alone (two heads' D leave
-  // the V waves no registers for it), else all
-  constexpr bool BY_KEYS = NK == 4, BRINGS = !BY_KEYS || !VW;
-  constexpr int NS = BY_KEYS ? 64 * NK : NT;
+  // who brings the tiles in: with four waves of each kind the key waves (two
+  // heads' D leave the V waves few registers), but q the V waves; else all
+  constexpr bool SPLIT = NK == 4 && NV == 4, KEYS = NK == 4 && NV == 2;
+  constexpr bool BRINGS = !SPLIT && (!KEYS || !VW);   // all of them
+  constexpr int NS = SPLIT || KEYS ? 256 : NT;
   char *qs = lds.qs, *ks = lds.ks, *vs = lds.vs, *os = lds.os, *ps = lds.ps, *dps = lds.dps;
   char* ds = lds.ds;
   float *sG = lds.sG, *sQ = lds.sQ, *sK = lds.sK;
@@ -97,7 +98,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
   LinStage<K, NS> sq, sk;
   LinStage<V, NS> sv, so;
   LinGates lg;
-  const int st = BY_KEYS ? tid - 64 * NV : tid;
+  const int st = (SPLIT || KEYS) && !VW ? tid - 64 * NV : tid;
   int gi = LinGates::token(w, lane);
   int qf = LinStage<K, NS>::from(a.ts.q, st), kf = LinStage<K, NS>::from(a.ts.k, st);
   int vf = LinStage<V, NS>::from(a.ts.v, st), of = LinStage<V, NS>::from(a.Hv * V, st);
@@ -106,13 +107,14 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
     const int n = c >= 0 ? sg.ntok - c * kChunk : 0, h = h0 + hh;
     const size_t t = n > 0 ? (size_t)sg.tok0 + c * kChunk : 0;
     if (w < 2) lg.load(a.dec, t, min(n, 64), h, a.Hv, gi);
-    if constexpr (!BRINGS) return;
     if (hh == 0) {
-      sq.load(a.q + t * a.ts.q + hq * K, a.ts.q, min(n, 64), qf);
-      sk.load(a.k + t * a.ts.k + hq * K, a.ts.k, min(n, 64), kf);
+      if (BRINGS || (SPLIT && VW)) sq.load(a.q + t * a.ts.q + hq * K, a.ts.q, min(n, 64), qf);
+      if (BRINGS || (SPLIT && !VW)) sk.load(a.k + t * a.ts.k + hq * K, a.ts.k, min(n, 64), kf);
     }
-    sv.load(a.v + t * a.ts.v + h * V, a.ts.v, min(n, 64), vf);
-    so.load(a.dO + (t * a.Hv + h) * V, a.Hv * V, min(n, 64), of);
+    if (BRINGS || (SPLIT && !VW)) {
+      sv.load(a.v + t * a.ts.v + h * V, a.ts.v, min(n, 64), vf);
+      so.load(a.dO + (t * a.Hv + h) * V, a.Hv * V, min(n, 64), of);
+    }
   };
   // the tiles above the diagonal that share a 32-wide block with it, and the
   // sums that no tile writes
@@ -125,13 +127,6 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
   for (int i = tid; i < 256; i += NT) lds.colM[i / 64][i % 64] = 0.f;
   __syncthreads();
 
-  int krb = LinTile<K>::row_base(lane), vrb = LinTile<V>::row_base(lane);
-  int kr4 = LinTile<K>::row4_base(lane), vr4 = LinTile<V>::row4_base(lane);
-  int kcb = LinTile<K>::col_base(0, lane), vcb = LinTile<V>::col_base(0, lane);
-  int pb = LinTile<64>::row_base(lane), pcb = LinTile<64>::col_base(0, lane);
-  int pw = LinTile<64>::off(lane % 16, lane / 32) + (lane / 16 & 1) * 8;
-  int dcb = LinTile<K>::col4_base(2 * wk, lane);            // key waves: D^T read
-  int dwb = LinTile<K>::row4_base(lane) + 32 * wv * 2 * K;   // V waves: D^T written
   // A chunk's gradients leave ahead of the loads issued after it: the wait for
   // loads counts stores too.
   f32x4 X[4][2], Y[4][2];   // dv; or dk and dq, over the heads (by token tile)
@@ -192,27 +187,23 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
     int ln = lane;
     hide(ln);
     const int lane = ln, r16 = ln % 16, grp = ln / 16;
-    hide(krb);
-    hide(vrb);
-    hide(kr4);
-    hide(vr4);
-    hide(kcb);
-    hide(vcb);
-    hide(pb);
-    hide(pw);
-    hide(pcb);
-    hide(dcb);
-    hide(dwb);
+    const int krb = LinTile<K>::row_base(lane), vrb = LinTile<V>::row_base(lane);
+    const int kr4 = LinTile<K>::row4_base(lane), vr4 = LinTile<V>::row4_base(lane);
+    const int kcb = LinTile<K>::col_base(0, lane), vcb = LinTile<V>::col_base(0, lane);
+    const int pb = LinTile<64>::row_base(lane), pcb = LinTile<64>::col_base(0, lane);
+    const int pw = LinTile<64>::off(r16, grp >> 1) + (grp & 1) * 8;
+    const int dcb = LinTile<K>::col4_base(2 * wk, lane);   // key waves: D^T read
+    const int dwb = kr4 + 32 * wv * 2 * K;                 // V waves: D^T written
     hide(qf);
     hide(kf);
     hide(vf);
     hide(of);
     hide(gi);
-    if constexpr (BRINGS) {
-      if (hh == 0) {
-        sq.store(qs, kt, st);
-        sk.store(ks, kt, st);
-      }
+    if (hh == 0) {
+      if (BRINGS || (SPLIT && VW)) sq.store(qs, kt, st);
+      if (BRINGS || (SPLIT && !VW)) sk.store(ks, kt, st);
+    }
+    if (BRINGS || (SPLIT && !VW)) {
       sv.store(vs, vt, st);
       so.store(os, vt, st);
     }
