@@ -45,7 +45,7 @@ struct LinGradLds {
   char qs[LinTile<K>::BYTES], ks[LinTile<K>::BYTES];
   char vs[LinTile<V>::BYTES], os[LinTile<V>::BYTES];
   char ps[LinTile<64>::BYTES], dps[LinTile<64>::BYTES];
-  char ds[2 * V * K];             // D^T as bf16, rows of K
+  char ds[2][2 * V * K];          // D^T in two bf16 parts, rows of K
   float sG[64], sQ[64], sK[64];   // G log2(e), scale e^G, e^R
   // (slots that their writers own and the reader adds up: M's row sums by source
   // block and lane group, its column sums by token block; a and b by wave and group)
@@ -64,7 +64,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
   constexpr bool BRINGS = !SPLIT && (!KEYS || !VW);   // all of them
   constexpr int NS = SPLIT || KEYS ? 256 : NT;
   char *qs = lds.qs, *ks = lds.ks, *vs = lds.vs, *os = lds.os, *ps = lds.ps, *dps = lds.dps;
-  char* ds = lds.ds;
+  char *ds = lds.ds[0], *dl = lds.ds[1];
   float *sG = lds.sG, *sQ = lds.sQ, *sK = lds.sK;
   const int tid = threadIdx.x, lane = tid % 64;
   const int h0 = hp * HP, hq = h0 / (a.Hv / a.Hqk);
@@ -221,7 +221,12 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
       for (int t = 0; t < K / 16; ++t)
 #pragma unroll
         for (int T = 0; T < 2; ++T)
-          *reinterpret_cast<u16x4*>(ds + (dwb ^ (32 * t)) + T * 16 * 2 * K) = f2bf4(ST[hh][t][T]);
+        {
+          u16x4 hi, lo;
+          split_bf4(ST[hh][t][T], hi, lo);
+          *reinterpret_cast<u16x4*>(ds + (dwb ^ (32 * t)) + T * 16 * 2 * K) = hi;
+          *reinterpret_cast<u16x4*>(dl + (dwb ^ (32 * t)) + T * 16 * 2 * K) = lo;
+        }
     }
     __syncthreads();
     if (VW ? c < nc - 1 || hh > 0 : c < nc - 1 && hh == 0)
@@ -346,9 +351,12 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
       float cs = 0.f;
       inter(X, sK, ks, lds.bsum,
             [&](int T, int b) {
+              // <S, D> from both parts of D: it is most of dg where the memory is
+              // long, and the sum of K V products would show their rounding
               const u16x8 f = LinTile<K>::cols4(ds, dcb, b, T);
+              const u16x8 l = LinTile<K>::cols4(dl, dcb, b, T);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) cs += bf2f(f[i]) * bf2f(SF[T][b][i]);
+              for (int i = 0; i < 8; ++i) cs += (bf2f(f[i]) + bf2f(l[i])) * bf2f(SF[T][b][i]);
               return f;
             },
             [&](int tt, int b) { return LinTile<V>::rows4(vs, vr4, tt, b); });
@@ -438,7 +446,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
 // A workgroup walks one segment of HP v-heads of one qk-head, chunk by chunk
 // and in each chunk head by head: q and k are staged once, dk and dq add up
 // over the heads in registers.  V / 32 waves own 32 columns of every D (dv,
-// dh0) and leave it as bf16 in LDS for the K / 32 waves that own 32 key columns
+// dh0) and leave it in LDS, in two bf16 parts, for the K / 32 waves that own 32 key columns
 // (dk, dq, P, dP and with the saved states' fragments <S, D>, all of which
 // reduce over V).  NP: the parts of dO's products on the way to dh0 (three
 // where it is wanted).

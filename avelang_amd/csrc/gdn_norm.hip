@@ -15,25 +15,28 @@ namespace gdn {
 // 16 bytes at an element-aligned address (rows of odd length, sliced bases)
 typedef uint32_t u32x4e __attribute__((ext_vector_type(4), aligned(2)));
 
+// the elements of 16 bytes, as floats
+template <int DT>
+__device__ __forceinline__ void unpack(u32x4e raw, float* f) {
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if constexpr (DT == GDN_DTYPE_F32) {
+      f[w] = __uint_as_float(raw[w]);
+    } else {
+      f[2 * w] = Elt<DT>::to_f(static_cast<uint16_t>(raw[w]));
+      f[2 * w + 1] = Elt<DT>::to_f(static_cast<uint16_t>(raw[w] >> 16));
+    }
+  }
+}
 // N elements of type DT at p (element-aligned), as floats
 template <int DT, int N>
 __device__ __forceinline__ void ldn(const void* p, long long i, float (&f)[N]) {
   constexpr int VEC = Elt<DT>::VEC;
   static_assert(N % VEC == 0, "whole vectors");
 #pragma unroll
-  for (int u = 0; u < N / VEC; ++u) {
-    const auto* src = static_cast<const typename Elt<DT>::T*>(p) + i + u * VEC;
-    const u32x4e raw = *reinterpret_cast<const u32x4e*>(src);
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if constexpr (DT == GDN_DTYPE_F32) {
-        f[u * VEC + w] = __uint_as_float(raw[w]);
-      } else {
-        f[u * VEC + 2 * w] = Elt<DT>::to_f(static_cast<uint16_t>(raw[w]));
-        f[u * VEC + 2 * w + 1] = Elt<DT>::to_f(static_cast<uint16_t>(raw[w] >> 16));
-      }
-    }
-  }
+  for (int u = 0; u < N / VEC; ++u)
+    unpack<DT>(*reinterpret_cast<const u32x4e*>(static_cast<const typename Elt<DT>::T*>(p) + i + u * VEC),
+               f + u * VEC);
 }
 template <int DT, int N>
 __device__ __forceinline__ void stn(void* p, long long i, const float (&f)[N]) {
@@ -77,6 +80,21 @@ __device__ __forceinline__ void ld_row(const void* p, long long base, int c, int
 #pragma unroll
     for (int j = 0; j < VEC; ++j) f[j] = c + j < D ? lde<DT>(p, base + c + j) : 0.f;
   }
+}
+// The same as raw bits.
+template <int DT>
+__device__ __forceinline__ u32x4e ld_raw(const void* p, long long base, int c, int D) {
+  constexpr int VEC = Elt<DT>::VEC;
+  const auto* src = static_cast<const typename Elt<DT>::T*>(p) + base + c;
+  if (c + VEC <= D) return *reinterpret_cast<const u32x4e*>(src);
+  u32x4e r = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    if (c + j >= D) break;
+    if constexpr (DT == GDN_DTYPE_F32) r[j] = __float_as_uint(src[j]);
+    else r[j / 2] |= static_cast<uint32_t>(src[j]) << (16 * (j % 2));
+  }
+  return r;
 }
 template <int DT, int VEC>
 __device__ __forceinline__ void st_row(void* p, long long base, int c, int D,
@@ -259,20 +277,30 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormBwdArgs a) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) dw[i][j] = db[i][j] = 0.f;
   }
-  float x[VPT][VEC], dy[VPT][VEC], mean = 0.f, rstd = 0.f;
+  // the next row's bits, on their way while this one is reduced
+  u32x4e rx[VPT], ry[VPT];
+  float nm = 0.f, nr = 0.f;
   auto load = [&](long long r) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
-      ld_row<DT, VEC>(a.x, r * a.D, (l + LPR * i) * VEC, a.D, x[i]);
-      ld_row<DT, VEC>(a.dy, r * a.D, (l + LPR * i) * VEC, a.D, dy[i]);
+      rx[i] = ld_raw<DT>(a.x, r * a.D, (l + LPR * i) * VEC, a.D);
+      ry[i] = ld_raw<DT>(a.dy, r * a.D, (l + LPR * i) * VEC, a.D);
     }
-    mean = a.stats[2 * r];
-    rstd = a.stats[2 * r + 1];
+    nm = a.stats[2 * r];
+    nr = a.stats[2 * r + 1];
   };
   const float inv_d = 1.f / a.D;
   int ph = 0;
+  if (live && gid < a.rows) load(gid);
   for (long long r = live ? gid : a.rows; r < a.rows; r += a.groups, ph ^= 1) {
-    load(r);
+    float x[VPT][VEC], dy[VPT][VEC];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      unpack<DT>(rx[i], x[i]);
+      unpack<DT>(ry[i], dy[i]);
+    }
+    const float mean = nm, rstd = nr;
+    if (r + a.groups < a.rows) load(r + a.groups);
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
