@@ -17,6 +17,8 @@
 // g), one joins them along each sequence, one walks every segment from its
 // start state and writes o.  Where a whole sequence fits a segment the first
 // two are left out.
+#include <initializer_list>
+
 #include "gdn_linear.h"
 #include "../../include/gdn_linear.h"
 
@@ -290,7 +292,7 @@ __global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int
 // of the state's rows for them in its accumulators, whose layout is that of
 // the operand with which S^T q is formed: the state never leaves the registers.
 template <int K, int V, int CT, int NP, bool OUT, bool SAVE>
-__global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
+__global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k,
     const uint16_t* __restrict__ v, TokenStride ts, LinDecay dec, LinGrid grid, int Hqk, int Hv,
     float scale, const float* h0, float* ht, const float* __restrict__ segs,
@@ -472,6 +474,7 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
       __syncthreads();   // P
     }
     const float eC = exp2_(sG[63]);
+    const u16x8 ones = {0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80};
 #pragma unroll
     for (int T = 0; T < CT; ++T)
 #pragma unroll
@@ -485,11 +488,50 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_walk_kernel(
         lin_split(vf[T], sK + 32 * kb + 8 * grp, part[T]);
       }
       if (OUT) {
+        // The block's sums by column show a value that is not finite.  It must not
+        // meet the zeros of P before its token: it is left out of the product, and
+        // its column is NaN from its token on.
+        bool finite = true;
+#pragma unroll
+        for (int T = 0; T < CT; ++T) {
+          const f32x4 sum = mfma16(vf[T], ones, zero4());
+#pragma unroll
+          for (int r = 0; r < 4; ++r) finite = finite && fabsf(sum[r]) < INFINITY;
+        }
+        const bool clean = __all(finite);
+        u16x8 vm[CT];
+        int from[CT];   // the first such token of column r16 (64: none)
+#pragma unroll
+        for (int T = 0; T < CT; ++T) {
+          vm[T] = vf[T];
+          from[T] = 64;
+          if (!clean) {
+#pragma unroll
+            for (int i = 7; i >= 0; --i)
+              if ((vf[T][i] & 0x7F80) == 0x7F80) {
+                vm[T][i] = 0;
+                from[T] = 32 * kb + 8 * grp + i;
+              }
+            from[T] = min(from[T], __shfl_xor(from[T], 16));
+            from[T] = min(from[T], __shfl_xor(from[T], 32));
+          }
+        }
 #pragma unroll
         for (int tt = 2 * kb; tt < 4; ++tt) {
           const u16x8 f = LinTile<64>::rows(ps, pb, tt, kb);
 #pragma unroll
-          for (int T = 0; T < CT; ++T) O[tt][T] = mfma16(vf[T], f, O[tt][T]);
+          for (int T = 0; T < CT; ++T) O[tt][T] = mfma16(vm[T], f, O[tt][T]);
+        }
+        if (!clean) {
+#pragma unroll
+          for (int T = 0; T < CT; ++T)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const int at = __shfl(from[T], 4 * grp + r);
+#pragma unroll
+              for (int tt = 2 * kb; tt < 4; ++tt)
+                if (16 * tt + r16 >= at) O[tt][T][r] = NAN;
+            }
         }
       }
 #pragma unroll
@@ -670,14 +712,22 @@ int lin_validate(const char* name, const void* q, const void* k, const void* v, 
   int rc = validate_common(q, k, v, gf, gf, h0, ht, o, cu, B, T, Hqk, Hv, K, V, N);
   if (rc) return rc;
   if (!gdn::dtype_ok(g_dtype)) return fail(GDN_ERR_SHAPE, std::string(name) + ": unsupported dtype code");
-  // (tokens, segments x heads and join workgroups are counted in 32 bits)
+  // (tokens, segments x heads and join workgroups are counted in 32 bits, and so
+  // are the bytes of a chunk's rows)
   const long long tokens = (long long)B * T;
   if (tokens >= (1LL << 31) - 64 || (tokens / 64 + N) * (long long)Hv >= (1LL << 24) * 64 ||
-      (long long)N * Hv * (K * V / 256) >= (1LL << 31))
+      (long long)N * Hv * (K * V / 256) >= (1LL << 31) || Hv >= (1 << 15))
     return fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
   if (tokens > 0)
     return validate_rows(name, q, k, v, q_row, k_row, v_row, o, tokens, Hqk, Hv, K, V, ts);
   ts = gdn::TokenStride{Hqk * K, Hqk * K, Hv * V};
+  return GDN_OK;
+}
+// 16-byte aligned (rows are read and written in vectors).
+int lin_aligned(const char* name, std::initializer_list<const void*> ptrs) {
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % 16)
+      return fail(GDN_ERR_SHAPE, std::string(name) + ": outputs and gradients must be 16-byte aligned");
   return GDN_OK;
 }
 bool lin_sizes_ok(int B, int T, int Hqk, int Hv, int K, int V, int N) {
@@ -707,9 +757,10 @@ extern "C" int gdn_linear_chunk_fwd(const void* q, const void* k, const void* v,
                                     void* workspace, size_t workspace_bytes, void* stream) {
   const char* name = "gdn_linear_chunk_fwd";
   gdn::TokenStride ts;
-  // (without o the checks that name it take q's address: nothing is written there)
+  // (without o its checks look at the states, which are larger)
   int rc = gdn_host::lin_validate(name, q, k, v, q_row, k_row, v_row, g, g_dtype, h0, ht,
                                   o ? o : states, cu_seqlens, B, T, Hqk, Hv, K, V, N, ts);
+  if (!rc) rc = gdn_host::lin_aligned(name, {o, states, workspace});
   if (rc) return rc;
   const bool has_cu = cu_seqlens != nullptr;
   const gdn::LinPlan p = gdn::lin_plan(B, T, Hqk, Hv, K, V, N, has_cu, false);

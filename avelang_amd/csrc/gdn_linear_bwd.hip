@@ -17,6 +17,7 @@
 //
 // Segments as in the forward, walked last chunk to first: a launch for every
 // segment's contribution to D, one that joins them, one for the gradients.
+#include <initializer_list>
 #include <type_traits>
 
 #include "gdn_linear.h"
@@ -547,6 +548,7 @@ int lin_validate(const char* name, const void* q, const void* k, const void* v, 
                  const float* ht, const void* o, const int32_t* cu, int B, int T, int Hqk, int Hv,
                  int K, int V, int N, gdn::TokenStride& ts);
 bool lin_sizes_ok(int B, int T, int Hqk, int Hv, int K, int V, int N);
+int lin_aligned(const char* name, std::initializer_list<const void*> ptrs);
 }  // namespace gdn_host
 
 extern "C" size_t gdn_linear_chunk_bwd_workspace_bytes(int B, int T, int Hqk, int Hv, int K, int V,
@@ -566,6 +568,7 @@ extern "C" int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v,
   gdn::TokenStride ts;
   int rc = gdn_host::lin_validate(name, q, k, v, q_row, k_row, v_row, g, g_dtype, dht, dh0, dv,
                                   cu_seqlens, B, T, Hqk, Hv, K, V, N, ts);
+  if (!rc) rc = gdn_host::lin_aligned(name, {dO, states, dq, dk, dv, workspace});
   if (rc) return rc;
   const long long tokens = (long long)B * T;
   if ((tokens > 0 && (!dO || !states || !dq || !dk)) || ((tokens > 0 || g_per_head) && !dg))
@@ -576,11 +579,13 @@ extern "C" int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v,
     return gdn_host::fail(GDN_ERR_WORKSPACE, std::string(name) + ": workspace needs " +
                                                  std::to_string(p.total) + " bytes, got " +
                                                  std::to_string(workspace_bytes));
+  const bool walk = N > 0 && (tokens > 0 || dh0);
+  if (!walk && !g_per_head) return GDN_OK;
   gdn_host::launch_begin();
   auto st = static_cast<hipStream_t>(stream);
   auto* ws = static_cast<unsigned char*>(workspace);
   float* dgt = g_per_head ? reinterpret_cast<float*>(ws + p.dgtok) : dg;
-  if (N > 0 && (tokens > 0 || dh0)) {
+  if (walk) {
     const gdn::LinGrid grid = gdn::lin_grid(p, ws, T, N, B * T, has_cu);
     if (has_cu) gdn::launch_lin_table(cu_seqlens, p, ws, N, B * T, st);
     gdn::LinBwdArgs a{};

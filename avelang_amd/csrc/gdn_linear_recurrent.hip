@@ -10,6 +10,8 @@
 // they are cut into tiles of 16 columns.  A lane holds float4 columns of K /
 // ROWG rows; a persistent grid walks the tiles, the next tile's state loaded
 // while the current one is advanced, in 16-byte streaming loads.
+#include <initializer_list>
+
 #include "gdn_linear.h"
 #include "../../include/gdn_linear.h"
 
@@ -163,6 +165,7 @@ int lin_validate(const char* name, const void* q, const void* k, const void* v, 
                  long long k_row, long long v_row, const void* g, int g_dtype, const float* h0,
                  const float* ht, const void* o, const int32_t* cu, int B, int T, int Hqk, int Hv,
                  int K, int V, int N, gdn::TokenStride& ts);
+int lin_aligned(const char* name, std::initializer_list<const void*> ptrs);
 }
 
 extern "C" int gdn_linear_recurrent_fwd(const void* q, const void* k, const void* v,
@@ -174,9 +177,10 @@ extern "C" int gdn_linear_recurrent_fwd(const void* q, const void* k, const void
                                         int num_slots, float scale, void* stream) {
   const char* name = "gdn_linear_recurrent_fwd";
   gdn::TokenStride ts;
-  const int rc = gdn_host::lin_validate(name, q, k, v, q_row, k_row, v_row, g, g_dtype,
+  int rc = gdn_host::lin_validate(name, q, k, v, q_row, k_row, v_row, g, g_dtype,
                                         state_indices ? nullptr : h0, state_indices ? nullptr : ht,
                                         o, cu_seqlens, B, T, Hqk, Hv, K, V, N, ts);
+  if (!rc) rc = gdn_host::lin_aligned(name, {o, h0, ht});
   if (rc) return rc;
   if (num_slots < 0 || (!state_indices && num_slots != N))
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": num_slots must be >= 0, and N without state_indices");

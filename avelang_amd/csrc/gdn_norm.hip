@@ -569,6 +569,7 @@ extern "C" int gdn_layer_norm_bwd(const void* x, const void* weight, const void*
       pb = dbias ? static_cast<float*>(workspace) + p.parts * C : nullptr;
     }
   }
+  if (rows == 0 && !sums) return GDN_OK;
   gdn_host::launch_begin();
   if (rows > 0) {
     const gdn::NormBwdArgs a{x,  weight, dy,    stats, dx, pw, pb,

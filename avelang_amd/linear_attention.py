@@ -43,10 +43,11 @@ __all__ = [
 def _inputs(q, k, v, g, cu_seqlens, name, out=None):
     """Checked q, k, v (as the kernels take them), g, cu_seqlens on the device,
     the token strides and the sizes (B, T, Hqk, Hv, K, V, N)."""
+    bf16 = torch.bfloat16
     for nm, t in (("q", q), ("k", k), ("v", v)):
         if not isinstance(t, torch.Tensor):
             raise ValueError(f"{name}: {nm} must be a torch.Tensor")
-        if t.dtype != torch.bfloat16:
+        if t.dtype is not bf16:
             raise ValueError(f"{name}: {nm} must have dtype torch.bfloat16, got {t.dtype}.")
         if t.dim() != 4:
             raise ValueError(f"{name}: {nm} must be 4-D [B, T, H, D], got {tuple(t.shape)}.")
@@ -62,8 +63,9 @@ def _inputs(q, k, v, g, cu_seqlens, name, out=None):
         raise ValueError(f"{name}: head sizes K={K}, V={V} unsupported (each in {_HEAD_SIZES}).")
     if not isinstance(g, torch.Tensor) or not g.is_floating_point():
         raise ValueError(f"{name}: g must be a floating point torch.Tensor")
-    if tuple(g.shape) not in ((B, T, Hv), (Hv,)):
-        raise ValueError(f"{name}: g must have shape {(B, T, Hv)} or {(Hv,)}, got {tuple(g.shape)}.")
+    gs = g.shape
+    if gs != (B, T, Hv) and gs != (Hv,):
+        raise ValueError(f"{name}: g must have shape {(B, T, Hv)} or {(Hv,)}, got {tuple(gs)}.")
     dev = q.device
     if dev.type != "cuda":
         raise ValueError(f"{name}: tensors must be on a ROCm (cuda) device, got {dev}.")
@@ -77,7 +79,8 @@ def _inputs(q, k, v, g, cu_seqlens, name, out=None):
     q, k, v, rows = _in_place(q, k, v, out)
     if rows is None:
         rows = (Hqk * K, Hqk * K, Hv * V)
-        q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q, k, v))
+        if (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+            q, k, v = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (q, k, v))
     return q, k, v, g.contiguous(), cu, rows, (B, T, Hqk, Hv, K, V, N)
 
 
@@ -100,7 +103,7 @@ def _cu(cu_seqlens, B, T, dev, name):
 
 
 def _state(t, shape, dev, what, name):
-    if (not isinstance(t, torch.Tensor) or tuple(t.shape) != shape or t.dtype != torch.float32
+    if (not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not torch.float32
             or t.device != dev):
         raise ValueError(f"{name}: {what} must be torch.float32 of shape {shape} on {dev}.")
     return t.contiguous()
@@ -197,8 +200,7 @@ def chunk_linear_attn_bwd(
             or do.device != dev):
         raise ValueError(f"{name}: do must be a bf16 tensor of shape {tuple(v.shape)} on {dev}.")
     do = do.contiguous()
-    if do.data_ptr() % 16:
-        do = do.clone()
+    do = do if do.data_ptr() % 16 == 0 else do.clone()
     if dht is not None:
         dht = _state(dht, (N, Hv, K, V), dev, "dht", name)
     if initial_state is not None:
@@ -276,7 +278,9 @@ def chunk_linear_attn(
     B = 1) packs N sequences; on the CPU a violation of its contract raises,
     on the device it empties every sequence.  ``workspace`` (uint8, of
     ``linear_attn_workspace_bytes(...)``), ``out`` and ``final_state`` (which
-    may be ``initial_state`` itself) avoid allocation.
+    may be ``initial_state`` itself) avoid allocation.  Infinities and NaN in
+    a token's inputs reach its own and later outputs only (padding behind a
+    batch's rows may hold anything); in the gradients they may reach others.
 
     Differentiable in q, k, v, g and initial_state (``chunk_linear_attn_bwd``).
     The forward then keeps the state at every chunk's start for the backward

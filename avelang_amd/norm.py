@@ -18,7 +18,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .layer_ops import _DTYPES, _dt, _on, _ptr, _stream
+from .layer_ops import _dt, _ptr, _stream
 
 __all__ = ["layer_norm", "layer_norm_fwd_save", "layer_norm_bwd"]
 
@@ -28,32 +28,42 @@ def _args(x, weight, bias, name):
     if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{name}: x must be a tensor with a last axis of at least 1.")
     dt = _dt(x, name, "x")
-    D, heads, p = x.shape[-1], 1, None
-    for nm, t in (("weight", weight), ("bias", bias)):
-        if t is None:
-            continue
-        if not isinstance(t, torch.Tensor):
-            raise ValueError(f"{name}: {nm} must be a torch.Tensor or None.")
-        if tuple(t.shape) != (D,) and (x.dim() < 2 or t.shape != x.shape[-2:]):
-            raise ValueError(f"{name}: {nm} must have the shape of x's last axis or last two axes, "
-                             f"got {tuple(t.shape)} for x {tuple(x.shape)}.")
-        if t.device != x.device:
-            raise ValueError(f"{name}: {nm} must be on {x.device}, got {t.device}.")
-        if p is not None and (t.shape != p.shape or t.dtype != p.dtype):
-            raise ValueError(f"{name}: weight and bias must share a shape and a dtype.")
-        p = t
-    wdt = dt
+    dev = x.device
+    if dev.type != "cuda":
+        raise ValueError(f"{name}: tensors must be on a ROCm (cuda) device, got {dev}.")
+    D, heads, wdt = x.shape[-1], 1, dt
+    p = bias if weight is None else weight
     if p is not None:
+        for nm, t in (("weight", weight), ("bias", bias)):
+            if t is None:
+                continue
+            if not isinstance(t, torch.Tensor):
+                raise ValueError(f"{name}: {nm} must be a torch.Tensor or None.")
+            if t.dim() == 1:
+                ok = t.shape[0] == D
+            else:
+                ok = t.dim() == 2 <= x.dim() and t.shape == x.shape[-2:]
+            if not ok:
+                raise ValueError(f"{name}: {nm} must have the shape of x's last axis or last two "
+                                 f"axes, got {tuple(t.shape)} for x {tuple(x.shape)}.")
+            if t.device != dev:
+                raise ValueError(f"{name}: {nm} must be on {dev}, got {t.device}.")
+        if bias is not None and p is not bias and (bias.dtype != p.dtype or bias.dim() != p.dim()):
+            raise ValueError(f"{name}: weight and bias must share a shape and a dtype.")
         wdt = _dt(p, name, "weight")
         if p.dim() == 2:
             heads = p.shape[0]
             if heads < 1:
                 raise ValueError(f"{name}: x must have at least one head.")
-    _on(x.device, name)
-    x = x.contiguous()
-    weight = weight.contiguous() if weight is not None else None
-    bias = bias.contiguous() if bias is not None else None
-    return x, weight, bias, x.numel() // D, heads, D, dt, wdt
+        if weight is not None:
+            weight = weight.contiguous()
+        if bias is not None:
+            bias = bias.contiguous()
+    return x.contiguous(), weight, bias, x.numel() // D, heads, D, dt, wdt
+
+
+def _grad(t):
+    return isinstance(t, torch.Tensor) and t.requires_grad
 
 
 def _fwd(x, weight, bias, eps, name, out=None, save=False):
@@ -129,10 +139,10 @@ class _LayerNorm(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, bias, stats = ctx.saved_tensors
         x, weight, bias, rows, heads, D, dt, wdt = _args(x, weight, bias, "layer_norm")
-        dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
-        db = torch.empty_like(bias) if bias is not None and ctx.needs_input_grad[2] else None
-        dx, dw, db = _bwd(x, weight, dy.to(x.dtype), stats, rows, heads, D, dt, wdt, dw, db,
-                          "layer_norm")
+        _, want_w, want_b, _ = ctx.needs_input_grad
+        dw = torch.empty_like(weight) if want_w and weight is not None else None
+        db = torch.empty_like(bias) if want_b and bias is not None else None
+        dx, dw, db = _bwd(x, weight, dy, stats, rows, heads, D, dt, wdt, dw, db, "layer_norm")
         return dx, dw, db, None
 
 
@@ -147,8 +157,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     Differentiable in x, weight and bias (``layer_norm_bwd``); the forward then
     keeps 8 bytes per row.
     """
-    if torch.is_grad_enabled() and any(
-            isinstance(t, torch.Tensor) and t.requires_grad for t in (x, weight, bias)):
+    if torch.is_grad_enabled() and (_grad(x) or _grad(weight) or _grad(bias)):
         if out is not None:
             raise ValueError("layer_norm: out is not supported when gradients are required.")
         return _LayerNorm.apply(x, weight, bias, eps)

@@ -9,11 +9,13 @@
  * h / (Hv / Hqk)):
  *     S_t = e^{g_t} S_{t-1} + k_t v_t^T        o_t = scale S_t^T q_t
  *   q, k [B, T, Hqk, K], v, o [B, T, Hv, V]  bf16, K and V in {64, 128}
- *   g    [B, T, Hv], or (g_per_head) [Hv], the same decay at every token
+ *   g    [B, T, Hv], or (g_per_head) [Hv], the same decay at every token; a
+ *        decay under -150 (-inf: a reset) counts as -150, e^-150 = 0 in fp32
  *   h0, ht [N, Hv, K, V] fp32 (nullable: zeros, not written; ht may be h0)
  *   q_row, k_row, v_row: elements from one token's rows to the next's (a
  *   token's heads contiguous): a multiple of 8, at least the heads' width and
- *   under 2^23; q, k, v 16-byte aligned.  o is contiguous.
+ *   under 2^23.  o is contiguous.  All tensors but g and cu_seqlens are
+ *   16-byte aligned.  Under 2^15 v-heads.
  *   cu_seqlens [N + 1] int32 (B == 1) or NULL (N == B), under gdn.h's
  *   contract; a violation found on the device empties every sequence: o (or
  *   the gradients) is zero and ht is h0.

@@ -311,3 +311,28 @@ def test_final_state_over_the_initial_one(rocm_device, packed):
         o2, s2 = ave.chunk_linear_attn(*args, initial_state=state, output_final_state=True,
                                        cu_seqlens=cu, final_state=state)
         assert s2 is state and torch.equal(s2, s) and torch.equal(o2, o)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 100, 1, 2, 64, 128), (2, 300, 1, 1, 128, 64), (1, 70, 2, 2, 128, 128)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_not_finite_stays_behind(rocm_device, shape, bad):
+    """What is not finite in a token's q, k, v or g leaves every earlier token's output alone, and
+    a token's own q all others'."""
+    import avelang_amd as ave
+    t = to(make(*shape, seed=12), rocm_device)
+    want = ave.chunk_linear_attn(t["q"], t["k"], t["v"], t["g"], initial_state=t["h0"])[0]
+    T = shape[1]
+    for n in ("q", "k", "v", "g"):
+        if n == "g" and bad < 0:
+            continue   # a reset
+        for at in (0, 13, 31, 33, T - 1):
+            x = t[n].clone()
+            x[0, at] = bad
+            got = ave.chunk_linear_attn(*(x if m == n else t[m] for m in ("q", "k", "v", "g")),
+                                        initial_state=t["h0"])[0]
+            assert torch.equal(got[0, :at], want[0, :at]), (n, at)
+            assert torch.equal(got[1:], want[1:])
+            assert not got[0, at].isfinite().all()
+            if n == "q":
+                assert torch.equal(got[0, at + 1:], want[0, at + 1:])
