@@ -14,14 +14,18 @@ struct LinSeg {
   int first, last;   // first / last segment of its sequence
 };
 
+// A sequence of several segments (seq < 0: no more of them): s0 .. s1 - 1.
+struct LinJoin {
+  int seq, s0, s1;
+};
+
 // Where a segment's data comes from: equal lengths by arithmetic, cu_seqlens
 // through the table the table kernel wrote.
 struct LinGrid {
   const LinSeg* table;      // [nseg], NULL: equal lengths
-  const int32_t* soff;      // [N + 1] first segment of each sequence (with table)
   const int32_t* status;    // != 0: a cu_seqlens violation (with table)
   const int32_t* order;     // [nseg] segments, longest first (with table)
-  const int32_t* joins;     // [1 + nlong] how many sequences have several segments, which (table)
+  const LinJoin* joins;     // [nlong] the sequences of several segments (with table)
   int T, L, nps;            // tokens and segments per sequence (without table), chunks per segment
   int nseg;                 // segments at most
   int nlong;                // sequences of several segments at most
@@ -258,7 +262,7 @@ struct LinPlan {
   int L, nps, nseg;          // as LinGrid
   long long chunks;          // chunks of all sequences at most (chunk-start states)
   int nlong;                 // sequences of several segments at most (0: no join)
-  size_t table, soff, status, order, joins, segs, decay, total;
+  size_t table, status, order, joins, segs, decay, total;
   // backward
   size_t part;               // fp32 partial dq, dk (several per qk-head)
   size_t dgtok;              // fp32 dg per token and v-head (one decay per head)

@@ -25,12 +25,12 @@
 namespace gdn {
 
 // ---------------------------------------------------------------- table ----
-// Segments of packed sequences: an entry per segment, the first segment of
-// each sequence, and the check of the cu_seqlens contract (on a violation
+// Segments of packed sequences: an entry per segment, the sequences of several
+// segments, and the check of the cu_seqlens contract (on a violation
 // every sequence is one empty segment).
 __global__ __launch_bounds__(1024) void lin_table_kernel(const int32_t* cu, LinSeg* table,
-                                                         int32_t* soff, int32_t* status,
-                                                         int32_t* order, int32_t* joins, int N,
+                                                         LinJoin* joins, int32_t* status,
+                                                         int32_t* order, int N,
                                                          int total, int L, int nseg, int nlong) {
   constexpr int BINS = 256;   // of lengths, for the order
   __shared__ int wsum[2][16], bin[BINS], nj;
@@ -80,7 +80,6 @@ __global__ __launch_bounds__(1024) void lin_table_kernel(const int32_t* cu, LinS
     sa += a - ns;
     sb += b - nc;
     if (n < N) {
-      soff[n] = sa;
       for (int i = 0; i < ns && sa + i < nseg; ++i) {
         const int ntok = min(len - i * L * kChunk, L * kChunk);
         table[sa + i] = LinSeg{s + i * L * kChunk, ntok, sb + i * L, n, i == 0, i == ns - 1};
@@ -88,7 +87,7 @@ __global__ __launch_bounds__(1024) void lin_table_kernel(const int32_t* cu, LinS
       }
       if (ns > 1) {
         const int j = atomicAdd(&nj, 1);
-        if (j < nlong) joins[1 + j] = n;
+        if (j < nlong) joins[j] = LinJoin{n, sa, min(sa + ns, nseg)};
       }
     }
   }
@@ -97,14 +96,23 @@ __global__ __launch_bounds__(1024) void lin_table_kernel(const int32_t* cu, LinS
     order[i] = i;
   }
   __syncthreads();
-  if (tid == 0) {
-    soff[N] = seg0;
-    if (nlong > 0) joins[0] = min(nj, nlong);
-    int at = 0;
-    for (int i = 0; i < BINS; ++i) {
-      const int x = bin[i];
-      bin[i] = at;
-      at += x;
+  for (int i = nj + tid; i < nlong; i += 1024) joins[i] = LinJoin{-1, 0, 0};
+  if (wave == 0) {   // where each bin's segments start
+    constexpr int PER = BINS / 64;
+    int x[PER], sum = 0;
+    for (int i = 0; i < PER; ++i) {
+      x[i] = bin[PER * lane + i];
+      sum += x[i];
+    }
+    int at = sum;
+    for (int off = 1; off < 64; off *= 2) {
+      const int y = __shfl_up(at, off);
+      if (lane >= off) at += y;
+    }
+    at -= sum;
+    for (int i = 0; i < PER; ++i) {
+      bin[PER * lane + i] = at;
+      at += x[i];
     }
   }
   __syncthreads();
@@ -239,51 +247,57 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_segment_kernel(
 
 // The states at every segment's start (REV: the gradients of the state at
 // every segment's end) in place of the contributions, from `edge` (h0 / dht,
-// nullable); into `end` (nullable) the state after the last.  A lane per
-// element.
-template <bool REV>
+// nullable); into `end` (nullable) the state after the last.  A lane per E
+// adjacent elements: four where that still gives every CU two workgroups, else
+// one, with as many segments' loads in flight.
+template <bool REV, int E>
 __global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int KV,
                                                        const float* edge,
                                                        float* __restrict__ segs,
                                                        const float* __restrict__ decay,
                                                        float* end) {
-  const int per = KV / 256;
+  typedef float vec __attribute__((ext_vector_type(E)));
+  const int per = KV / (256 * E);
   int n = blockIdx.x / (Hv * per);
-  const int h = blockIdx.x / per % Hv, e = blockIdx.x % per * 256 + threadIdx.x;
+  const int h = blockIdx.x / per % Hv, e = (blockIdx.x % per * 256 + threadIdx.x) * E;
   int s0, s1;
   if (grid.table) {
-    if (n >= grid.joins[0]) return;
-    n = grid.joins[1 + n];
-    s0 = grid.soff[n];
-    s1 = grid.soff[n + 1];
+    const LinJoin j = grid.joins[n];
+    if (j.seq < 0) return;
+    n = j.seq;
+    s0 = j.s0;
+    s1 = j.s1;
   } else {
     s0 = n * grid.nps;
     s1 = s0 + grid.nps;
   }
-  float S = edge ? edge[((size_t)n * Hv + h) * KV + e] : 0.f;
+  auto at = [&](size_t s) { return reinterpret_cast<vec*>(segs + (s * Hv + h) * KV + e); };
+  vec S = {};
+  if (edge) S = *reinterpret_cast<const vec*>(edge + ((size_t)n * Hv + h) * KV + e);
   const int first = REV ? s1 - 1 : s0, step = REV ? -1 : 1, cnt = s1 - s0 - 1;
-  constexpr int U = 8;   // loads in flight
+  constexpr int U = E == 1 ? 16 : 8;   // loads in flight
   for (int i = 0; i < cnt; i += U) {
-    float c[U], d[U];
+    vec c[U];
+    float d[U];
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       const size_t s = first + min(i + j, cnt - 1) * step;
-      c[j] = segs[(s * Hv + h) * KV + e];
+      c[j] = *at(s);
       d[j] = decay[s * Hv + h];
     }
 #pragma unroll
     for (int j = 0; j < U; ++j) {
       if (i + j < cnt) {
-        const size_t s = first + (i + j) * step;
-        segs[(s * Hv + h) * KV + e] = S;
+        *at(first + (i + j) * step) = S;
         S = d[j] * S + c[j];
       }
     }
   }
-  const size_t at = (size_t)(REV ? s0 : s1 - 1) * Hv + h;
-  const float last = end ? decay[at] * S + segs[at * KV + e] : 0.f;
-  segs[at * KV + e] = S;
-  if (end) end[((size_t)n * Hv + h) * KV + e] = last;
+  const size_t last = REV ? s0 : s1 - 1;
+  vec x = {};
+  if (end) x = decay[last * Hv + h] * S + *at(last);
+  *at(last) = S;
+  if (end) *reinterpret_cast<vec*>(end + ((size_t)n * Hv + h) * KV + e) = x;
 }
 
 // ------------------------------------------------------------------ walk ----
@@ -592,10 +606,9 @@ LinPlan lin_plan(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu
   };
   if (has_cu) {
     p.table = take((size_t)p.nseg * sizeof(LinSeg));
-    p.soff = take(((size_t)N + 1) * 4);
     p.status = take(4);
     p.order = take((size_t)p.nseg * 4);
-    p.joins = take(((size_t)p.nlong + 1) * 4);
+    p.joins = take((size_t)p.nlong * sizeof(LinJoin));
   }
   if (p.nlong > 0) {
     p.segs = take((size_t)p.nseg * Hv * K * V * 4);
@@ -612,10 +625,9 @@ LinGrid lin_grid(const LinPlan& p, unsigned char* ws, int T, int N, int total, b
   LinGrid g{};
   if (has_cu) {
     g.table = reinterpret_cast<const LinSeg*>(ws + p.table);
-    g.soff = reinterpret_cast<const int32_t*>(ws + p.soff);
     g.status = reinterpret_cast<const int32_t*>(ws + p.status);
     g.order = reinterpret_cast<const int32_t*>(ws + p.order);
-    g.joins = reinterpret_cast<const int32_t*>(ws + p.joins);
+    g.joins = reinterpret_cast<const LinJoin*>(ws + p.joins);
   }
   g.T = T;
   g.L = p.L;
@@ -631,10 +643,9 @@ void launch_lin_table(const int32_t* cu, const LinPlan& p, unsigned char* ws, in
                       hipStream_t st) {
   hipLaunchKernelGGL(lin_table_kernel, dim3(1), dim3(1024), 0, st, cu,
                      reinterpret_cast<LinSeg*>(ws + p.table),
-                     reinterpret_cast<int32_t*>(ws + p.soff),
+                     reinterpret_cast<LinJoin*>(ws + p.joins),
                      reinterpret_cast<int32_t*>(ws + p.status),
-                     reinterpret_cast<int32_t*>(ws + p.order),
-                     reinterpret_cast<int32_t*>(ws + p.joins), N, total, p.L, p.nseg, p.nlong);
+                     reinterpret_cast<int32_t*>(ws + p.order), N, total, p.L, p.nseg, p.nlong);
 }
 
 template <int K, int V>
@@ -643,12 +654,19 @@ void launch_lin_segments(const uint16_t* x, int x_row, const uint16_t* y, int y_
                          bool reverse, bool full, const float* edge, float* segs, float* decay,
                          float* end, hipStream_t st) {
   const dim3 items(lin_items(g.table ? g.nseg : g.N * (g.nps - (end ? 0 : 1)), Hqk, Hv));
-  const dim3 elems((unsigned)(g.nlong * Hv * (K * V / 256)));
+  const long long waves = (long long)g.nlong * Hv * (K * V / 256);   // workgroups of one per lane
+  const bool four = waves >= 8LL * device_cus();
+  const dim3 elems((unsigned)(four ? waves / 4 : waves));
 #define GDN_SEG(NP, REV)                                                                        \
   hipLaunchKernelGGL((lin_segment_kernel<K, V, kSegTiles, NP, REV>), items,                     \
                      dim3(4 * V / kSegTiles), 0, st, x, x_row, y, y_row, d, g, Hqk, Hv, scale,  \
                      end != nullptr, segs, decay);                                              \
-  hipLaunchKernelGGL(lin_join_kernel<REV>, elems, dim3(256), 0, st, g, Hv, K * V, edge, segs, decay, end)
+  if (four)                                                                                     \
+    hipLaunchKernelGGL((lin_join_kernel<REV, 4>), elems, dim3(256), 0, st, g, Hv, K * V, edge,   \
+                       segs, decay, end);                                                       \
+  else                                                                                          \
+    hipLaunchKernelGGL((lin_join_kernel<REV, 1>), elems, dim3(256), 0, st, g, Hv, K * V, edge,   \
+                       segs, decay, end)
   if (reverse) {
     if (full) { GDN_SEG(3, true); } else { GDN_SEG(2, true); }
   } else {
@@ -727,7 +745,7 @@ int lin_validate(const char* name, const void* q, const void* k, const void* v, 
 int lin_aligned(const char* name, std::initializer_list<const void*> ptrs) {
   for (const void* p : ptrs)
     if (reinterpret_cast<uintptr_t>(p) % 16)
-      return fail(GDN_ERR_SHAPE, std::string(name) + ": outputs and gradients must be 16-byte aligned");
+      return fail(GDN_ERR_SHAPE, std::string(name) + ": tensors must be 16-byte aligned");
   return GDN_OK;
 }
 bool lin_sizes_ok(int B, int T, int Hqk, int Hv, int K, int V, int N) {
@@ -760,7 +778,7 @@ extern "C" int gdn_linear_chunk_fwd(const void* q, const void* k, const void* v,
   // (without o its checks look at the states, which are larger)
   int rc = gdn_host::lin_validate(name, q, k, v, q_row, k_row, v_row, g, g_dtype, h0, ht,
                                   o ? o : states, cu_seqlens, B, T, Hqk, Hv, K, V, N, ts);
-  if (!rc) rc = gdn_host::lin_aligned(name, {o, states, workspace});
+  if (!rc) rc = gdn_host::lin_aligned(name, {o, h0, ht, states, workspace});
   if (rc) return rc;
   const bool has_cu = cu_seqlens != nullptr;
   const gdn::LinPlan p = gdn::lin_plan(B, T, Hqk, Hv, K, V, N, has_cu, false);

@@ -38,8 +38,15 @@ struct LinBwdArgs {
   const u16x8* states;
   uint16_t *dq, *dk, *dv;
   float *pq, *pk;      // [tokens][Hv / HP][K] partial dq, dk (NULL: none needed)
-  float* dg;           // [tokens][Hv]
+  void* dg;            // [tokens][Hv], of type dgt
+  int dgt;
 };
+
+__device__ __forceinline__ void lin_put(void* p, size_t i, float x, int dt) {
+  if (dt == GDN_DTYPE_F32) ste<GDN_DTYPE_F32>(p, i, x);
+  else if (dt == GDN_DTYPE_BF16) ste<GDN_DTYPE_BF16>(p, i, x);
+  else ste<GDN_DTYPE_F16>(p, i, x);
+}
 
 template <int K, int V>
 struct LinGradLds {
@@ -388,7 +395,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
       const float px = wave_prefix(x);
       const float dg = eC * cs + (lane63(px) - px + x) + (wave_prefix(y) - y);
       const int n = sg.ntok - c * kChunk;
-      if (lane < n) a.dg[((size_t)sg.tok0 + c * kChunk + lane) * a.Hv + h] = dg;
+      if (lane < n) lin_put(a.dg, ((size_t)sg.tok0 + c * kChunk + lane) * a.Hv + h, dg, a.dgt);
     }
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
@@ -465,7 +472,7 @@ __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) 
       reinterpret_cast<u32x4*>(a.dq)[i] = u32x4{0, 0, 0, 0};
       reinterpret_cast<u32x4*>(a.dk)[i] = u32x4{0, 0, 0, 0};
     }
-    for (size_t i = i0; i < ng; i += st) a.dg[i] = 0.f;
+    for (size_t i = i0; i < ng; i += st) lin_put(a.dg, i, 0.f, a.dgt);
   }
   int sid, hp;
   if (!lin_item(a.grid, a.grid.nseg, a.Hqk, a.Hv / HP, sid, hp)) return;
@@ -503,8 +510,8 @@ __global__ __launch_bounds__(256) void lin_group_sum_kernel(const float* __restr
 // One decay per head: its gradient, the sum over all tokens (a workgroup per
 // head, a fixed order).
 __global__ __launch_bounds__(1024) void lin_head_sum_kernel(const float* __restrict__ x,
-                                                            float* __restrict__ out, int tokens,
-                                                            int Hv) {
+                                                            void* __restrict__ out, int tokens,
+                                                            int Hv, int dt) {
   __shared__ float red[16];
   float s = 0.f;
 #pragma unroll 4
@@ -516,7 +523,7 @@ __global__ __launch_bounds__(1024) void lin_head_sum_kernel(const float* __restr
   if (threadIdx.x == 0) {
 #pragma unroll
     for (int i = 1; i < 16; ++i) s += red[i];
-    out[blockIdx.x] = s;
+    lin_put(out, blockIdx.x, s, dt);
   }
 }
 
@@ -560,7 +567,7 @@ extern "C" size_t gdn_linear_chunk_bwd_workspace_bytes(int B, int T, int Hqk, in
 extern "C" int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v, long long q_row,
                                     long long k_row, long long v_row, const void* g, int g_dtype,
                                     int g_per_head, const void* dO, const float* dht,
-                                    const void* states, void* dq, void* dk, void* dv, float* dg,
+                                    const void* states, void* dq, void* dk, void* dv, void* dg,
                                     float* dh0, const int32_t* cu_seqlens, int B, int T, int Hqk,
                                     int Hv, int K, int V, int N, float scale, void* workspace,
                                     size_t workspace_bytes, void* stream) {
@@ -568,7 +575,7 @@ extern "C" int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v,
   gdn::TokenStride ts;
   int rc = gdn_host::lin_validate(name, q, k, v, q_row, k_row, v_row, g, g_dtype, dht, dh0, dv,
                                   cu_seqlens, B, T, Hqk, Hv, K, V, N, ts);
-  if (!rc) rc = gdn_host::lin_aligned(name, {dO, states, dq, dk, dv, workspace});
+  if (!rc) rc = gdn_host::lin_aligned(name, {dO, dht, states, dq, dk, dv, dh0, workspace});
   if (rc) return rc;
   const long long tokens = (long long)B * T;
   if ((tokens > 0 && (!dO || !states || !dq || !dk)) || ((tokens > 0 || g_per_head) && !dg))
@@ -584,7 +591,7 @@ extern "C" int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v,
   gdn_host::launch_begin();
   auto st = static_cast<hipStream_t>(stream);
   auto* ws = static_cast<unsigned char*>(workspace);
-  float* dgt = g_per_head ? reinterpret_cast<float*>(ws + p.dgtok) : dg;
+  void* dgt = g_per_head ? ws + p.dgtok : dg;   // (one decay per head: fp32, summed below)
   if (walk) {
     const gdn::LinGrid grid = gdn::lin_grid(p, ws, T, N, B * T, has_cu);
     if (has_cu) gdn::launch_lin_table(cu_seqlens, p, ws, N, B * T, st);
@@ -606,6 +613,7 @@ extern "C" int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v,
     a.dk = static_cast<uint16_t*>(dk);
     a.dv = static_cast<uint16_t*>(dv);
     a.dg = dgt;
+    a.dgt = g_per_head ? GDN_DTYPE_F32 : g_dtype;
     const int parts = Hv / Hqk / (gdn::lin_pair(Hqk, Hv) ? 2 : 1);   // of a qk-head's gradients
     if (parts > 1) {
       a.pq = reinterpret_cast<float*>(ws + p.part);
@@ -624,6 +632,7 @@ extern "C" int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v,
                          a.pq, a.pk, a.dq, a.dk, grid.status, tokens * Hqk, parts, K);
   }
   if (g_per_head)
-    hipLaunchKernelGGL(gdn::lin_head_sum_kernel, dim3(Hv), dim3(1024), 0, st, dgt, dg, (int)tokens, Hv);
+    hipLaunchKernelGGL(gdn::lin_head_sum_kernel, dim3(Hv), dim3(1024), 0, st,
+                       static_cast<const float*>(dgt), dg, (int)tokens, Hv, g_dtype);
   return gdn_host::check_launch(name);
 }

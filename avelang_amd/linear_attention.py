@@ -106,7 +106,8 @@ def _state(t, shape, dev, what, name):
     if (not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not torch.float32
             or t.device != dev):
         raise ValueError(f"{name}: {what} must be torch.float32 of shape {shape} on {dev}.")
-    return t.contiguous()
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
 def linear_attn_workspace_bytes(B: int, T: int, Hqk: int, Hv: int, K: int, V: int, N: int,
@@ -136,7 +137,7 @@ def _chunk_fwd(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens,
         else:
             ht = final_state
             if _state(ht, (N, Hv, K, V), dev, "final_state", name) is not ht:
-                raise ValueError(f"{name}: final_state must be contiguous.")
+                raise ValueError(f"{name}: final_state must be contiguous and 16-byte aligned.")
     states = None
     if save:
         states = torch.empty(max(1, lib.gdn_linear_states_bytes(B, T, Hv, K, V, N, cu is not None)),
@@ -187,7 +188,7 @@ def chunk_linear_attn_bwd(
     workspace: Optional[torch.Tensor] = None,
 ):
     """Gradients of ``chunk_linear_attn``: ``(dq, dk, dv, dg, dh0)``, dq, dk, dv
-    in bf16, dg in fp32 with g's shape, dh0 fp32 (None without
+    in bf16, dg with g's shape and type, dh0 fp32 (None without
     ``initial_state``).  ``do`` is dL/do (bf16, v's shape), ``dht`` (nullable)
     dL/d(final state).  Without ``states`` (``chunk_linear_attn_fwd_save``) the
     forward's states are formed again.  Deterministic.
@@ -216,7 +217,7 @@ def chunk_linear_attn_bwd(
     bf = dict(dtype=torch.bfloat16, device=dev)
     dq, dk = torch.empty((B, T, Hqk, K), **bf), torch.empty((B, T, Hqk, K), **bf)
     dv = torch.empty((B, T, Hv, V), **bf)
-    dg = torch.empty(g.shape, dtype=torch.float32, device=dev)
+    dg = torch.empty_like(g)
     dh0 = None
     if initial_state is not None:
         dh0 = torch.empty((N, Hv, K, V), dtype=torch.float32, device=dev)
@@ -252,8 +253,8 @@ class _ChunkLinearAttn(torch.autograd.Function):
         if do is None:
             do = torch.zeros_like(v)
         dq, dk, dv, dg, dh0 = chunk_linear_attn_bwd(
-            q, k, v, g, do.to(torch.bfloat16), dht, ctx.scale, h0, cu, states=states)
-        return dq, dk, dv, dg.to(g.dtype), None, dh0, None, None, None
+            q, k, v, g, do, dht, ctx.scale, h0, cu, states=states)
+        return dq, dk, dv, dg if dg.dtype is g.dtype else dg.to(g.dtype), None, dh0, None, None, None
 
 
 def chunk_linear_attn(
@@ -351,9 +352,10 @@ def fused_recurrent_linear_attn(
     if h0 is not None:
         h0 = _state(h0, (slots,) + state, dev, "initial_state", name)
         if output_final_state and inplace_final_state and h0 is not initial_state:
-            raise ValueError(f"{name}: an in-place initial_state must be contiguous.")
+            raise ValueError(f"{name}: an in-place initial_state must be contiguous and "
+                             "16-byte aligned.")
         if idx is not None and h0 is not initial_state:
-            raise ValueError(f"{name}: the state pool must be contiguous.")
+            raise ValueError(f"{name}: the state pool must be contiguous and 16-byte aligned.")
     if output_final_state:
         ht = h0
         if h0 is None or not inplace_final_state:

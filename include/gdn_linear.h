@@ -51,8 +51,8 @@ int gdn_linear_chunk_fwd(const void* q, const void* k, const void* v,
 
 /*
  * Its gradients: dO [B, T, Hv, V] bf16 contiguous, dht nullable; dq, dk, dv
- * bf16 contiguous (q's, k's, v's shapes), dg fp32 [B, T, Hv], dh0 (nullable).
- * With g_per_head dg is fp32 [Hv], the sum over all tokens in a fixed order.
+ * bf16 contiguous (q's, k's, v's shapes), dg (g's shape and type), dh0 (nullable).
+ * With g_per_head dg is the sum over all tokens, in fp32 and in a fixed order.
  * states: what gdn_linear_chunk_fwd left for these same inputs.
  * Deterministic; workspace: gdn_linear_chunk_bwd_workspace_bytes bytes.
  */
@@ -62,7 +62,7 @@ int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v,
                          long long q_row, long long k_row, long long v_row,
                          const void* g, int g_dtype, int g_per_head,
                          const void* dO, const float* dht, const void* states,
-                         void* dq, void* dk, void* dv, float* dg, float* dh0,
+                         void* dq, void* dk, void* dv, void* dg, float* dh0,
                          const int32_t* cu_seqlens,
                          int B, int T, int Hqk, int Hv, int K, int V, int N, float scale,
                          void* workspace, size_t workspace_bytes, void* stream);

@@ -336,3 +336,29 @@ def test_not_finite_stays_behind(rocm_device, shape, bad):
             assert not got[0, at].isfinite().all()
             if n == "q":
                 assert torch.equal(got[0, at + 1:], want[0, at + 1:])
+
+
+@pytest.mark.gpu
+def test_odd_addresses(rocm_device):
+    """States, slices and gradients at addresses off 16 bytes are copied, in-place ones refused."""
+    import avelang_amd as ave
+    t = to(make(1, 70, 1, 2, 64, 64, seed=13), rocm_device)
+    args = (t["q"], t["k"], t["v"], t["g"])
+
+    def odd(x):
+        y = torch.empty(x.numel() + 1, dtype=x.dtype, device=rocm_device)[1:].view(x.shape)
+        return y.copy_(x)
+    kw = dict(output_final_state=True)
+    for op, more in ((ave.chunk_linear_attn, {}), (ave.fused_recurrent_linear_attn, dict(inplace_final_state=False))):
+        want = op(*args, initial_state=t["h0"], **kw, **more)
+        got = op(*map(odd, args), initial_state=odd(t["h0"]), **kw, **more)
+        assert all(torch.equal(x, y) for x, y in zip(want, got))
+    want = ave.chunk_linear_attn_bwd(*args, t["do"], t["dht"], initial_state=t["h0"])
+    got = ave.chunk_linear_attn_bwd(*map(odd, args), odd(t["do"]), odd(t["dht"]), initial_state=odd(t["h0"]))
+    assert all(torch.equal(x, y) for x, y in zip(want, got))
+    with pytest.raises(ValueError, match="aligned"):
+        ave.fused_recurrent_linear_attn(*args, initial_state=odd(t["h0"]), output_final_state=True)
+    with pytest.raises(ValueError, match="aligned"):
+        ave.chunk_linear_attn(*args, initial_state=t["h0"], final_state=odd(t["h0"]), output_final_state=True)
+    with pytest.raises(ValueError, match="aligned"):
+        ave.chunk_linear_attn(*args, out=odd(t["v"]))
