@@ -119,10 +119,10 @@ def linear_attn_workspace_bytes(B: int, T: int, Hqk: int, Hv: int, K: int, V: in
     return int(f(B, T, Hqk, Hv, K, V, N, int(has_cu_seqlens)))
 
 
-def _chunk_fwd(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, name,
-               workspace=None, out=None, final_state=None, save=False, want_o=True):
-    """gdn_linear_chunk_fwd: (o, final state, saved states)."""
-    q, k, v, g, cu, rows, dims = _inputs(q, k, v, g, cu_seqlens, name, out)
+def _chunk_fwd(inputs, scale, initial_state, output_final_state, name, workspace=None, out=None,
+               final_state=None, save=False, want_o=True):
+    """gdn_linear_chunk_fwd on ``_inputs``' result: (o, final state, saved states)."""
+    q, k, v, g, cu, rows, dims = inputs
     B, T, Hqk, Hv, K, V, N = dims
     dev = q.device
     lib = _native.lib()
@@ -169,8 +169,9 @@ def chunk_linear_attn_fwd_save(
     """Training forward: ``(o, final_state, states)``, ``states`` (the bf16
     state at every chunk's start, 2 K V bytes per 64 tokens and v-head) being
     what ``chunk_linear_attn_bwd`` takes for these same inputs."""
-    return _chunk_fwd(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens,
-                      "chunk_linear_attn_fwd_save", save=True)
+    name = "chunk_linear_attn_fwd_save"
+    return _chunk_fwd(_inputs(q, k, v, g, cu_seqlens, name), scale, initial_state,
+                      output_final_state, name, save=True)
 
 
 def chunk_linear_attn_bwd(
@@ -194,7 +195,12 @@ def chunk_linear_attn_bwd(
     forward's states are formed again.  Deterministic.
     """
     name = "chunk_linear_attn_bwd"
-    q, k, v, g, cu, rows, dims = _inputs(q, k, v, g, cu_seqlens, name)
+    return _chunk_bwd(_inputs(q, k, v, g, cu_seqlens, name), do, dht, scale, initial_state, states,
+                      workspace, name)
+
+
+def _chunk_bwd(inputs, do, dht, scale, initial_state, states, workspace, name):
+    q, k, v, g, cu, rows, dims = inputs
     B, T, Hqk, Hv, K, V, N = dims
     dev = q.device
     if (not isinstance(do, torch.Tensor) or do.shape != v.shape or do.dtype != torch.bfloat16
@@ -208,7 +214,7 @@ def chunk_linear_attn_bwd(
         _state(initial_state, (N, Hv, K, V), dev, "initial_state", name)
     lib = _native.lib()
     if states is None:
-        _, _, states = _chunk_fwd(q, k, v, g, scale, initial_state, False, cu, name, save=True,
+        _, _, states = _chunk_fwd(inputs, scale, initial_state, False, name, save=True,
                                   want_o=False)
     else:
         need = lib.gdn_linear_states_bytes(B, T, Hv, K, V, N, cu is not None)
@@ -239,22 +245,24 @@ def chunk_linear_attn_bwd(
 class _ChunkLinearAttn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, scale, initial_state, output_final_state, cu_seqlens, save):
-        o, ht, states = _chunk_fwd(q, k, v, g, scale, initial_state, output_final_state,
-                                   cu_seqlens, "chunk_linear_attn", save=save)
-        ctx.save_for_backward(q, k, v, g, initial_state, cu_seqlens, states)
-        ctx.scale = scale
+        name = "chunk_linear_attn"
+        inputs = _inputs(q, k, v, g, cu_seqlens, name)
+        o, ht, states = _chunk_fwd(inputs, scale, initial_state, output_final_state, name, save=save)
+        ctx.save_for_backward(*inputs[:5], initial_state, states)
+        ctx.rest = inputs[5:] + (scale, g.dtype)
         ctx.set_materialize_grads(False)
         return (o, ht) if output_final_state else o
 
     @staticmethod
     @once_differentiable
     def backward(ctx, do, dht=None):
-        q, k, v, g, h0, cu, states = ctx.saved_tensors
+        q, k, v, g, cu, h0, states = ctx.saved_tensors
+        rows, dims, scale, g_type = ctx.rest
         if do is None:
-            do = torch.zeros_like(v)
-        dq, dk, dv, dg, dh0 = chunk_linear_attn_bwd(
-            q, k, v, g, do, dht, ctx.scale, h0, cu, states=states)
-        return dq, dk, dv, dg if dg.dtype is g.dtype else dg.to(g.dtype), None, dh0, None, None, None
+            do = torch.zeros(v.shape, dtype=v.dtype, device=v.device)
+        dq, dk, dv, dg, dh0 = _chunk_bwd((q, k, v, g, cu, rows, dims), do, dht, scale, h0, states,
+                                         None, "chunk_linear_attn")
+        return dq, dk, dv, dg if dg.dtype is g_type else dg.to(g_type), None, dh0, None, None, None
 
 
 def chunk_linear_attn(
@@ -297,8 +305,9 @@ def chunk_linear_attn(
         res = _ChunkLinearAttn.apply(q, k, v, g, scale, initial_state, bool(output_final_state),
                                      cu_seqlens, bool(save_for_backward))
         return res if output_final_state else (res, None)
-    o, ht, _ = _chunk_fwd(q, k, v, g, scale, initial_state, output_final_state, cu_seqlens,
-                          "chunk_linear_attn", workspace, out, final_state)
+    name = "chunk_linear_attn"
+    o, ht, _ = _chunk_fwd(_inputs(q, k, v, g, cu_seqlens, name, out), scale, initial_state,
+                          output_final_state, name, workspace, out, final_state)
     return o, ht
 
 

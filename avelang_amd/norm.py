@@ -62,12 +62,12 @@ def _args(x, weight, bias, name):
     return x.contiguous(), weight, bias, x.numel() // D, heads, D, dt, wdt
 
 
-def _grad(t):
+def _grad(t) -> bool:
     return isinstance(t, torch.Tensor) and t.requires_grad
 
 
-def _fwd(x, weight, bias, eps, name, out=None, save=False):
-    x, weight, bias, rows, heads, D, dt, wdt = _args(x, weight, bias, name)
+def _fwd(args, eps, name, out=None, save=False):
+    x, weight, bias, rows, heads, D, dt, wdt = args
     if out is None:
         y = torch.empty_like(x)
     else:
@@ -88,7 +88,8 @@ def layer_norm_fwd_save(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                         eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor]:
     """Training forward: ``(y, stats)``, ``stats`` fp32 [rows, 2] holding each
     row's mean and 1 / sqrt(var + eps) for ``layer_norm_bwd``."""
-    return _fwd(x, weight, bias, eps, "layer_norm_fwd_save", save=True)
+    name = "layer_norm_fwd_save"
+    return _fwd(_args(x, weight, bias, name), eps, name, save=True)
 
 
 def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Tensor,
@@ -130,19 +131,20 @@ def _bwd(x, weight, dy, stats, rows, heads, D, dt, wdt, dw, db, name):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, stats = _fwd(x, weight, bias, eps, "layer_norm", save=True)
-        ctx.save_for_backward(x, weight, bias, stats)
+        args = _args(x, weight, bias, "layer_norm")
+        y, stats = _fwd(args, eps, "layer_norm", save=True)
+        ctx.save_for_backward(args[0], args[1], args[2], stats)
+        ctx.sizes = args[3:]
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, weight, bias, stats = ctx.saved_tensors
-        x, weight, bias, rows, heads, D, dt, wdt = _args(x, weight, bias, "layer_norm")
         _, want_w, want_b, _ = ctx.needs_input_grad
         dw = torch.empty_like(weight) if want_w and weight is not None else None
         db = torch.empty_like(bias) if want_b and bias is not None else None
-        dx, dw, db = _bwd(x, weight, dy, stats, rows, heads, D, dt, wdt, dw, db, "layer_norm")
+        dx, dw, db = _bwd(x, weight, dy, stats, *ctx.sizes, dw, db, "layer_norm")
         return dx, dw, db, None
 
 
@@ -161,4 +163,4 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
         if out is not None:
             raise ValueError("layer_norm: out is not supported when gradients are required.")
         return _LayerNorm.apply(x, weight, bias, eps)
-    return _fwd(x, weight, bias, eps, "layer_norm", out)[0]
+    return _fwd(_args(x, weight, bias, "layer_norm"), eps, "layer_norm", out)[0]
