@@ -146,6 +146,33 @@ __device__ __forceinline__ void lin_store_state(const f32x4 (&S)[K / 16], float*
 }
 
 // -------------------------------------------------------------- segments ----
+// A chunk's step of the state: S' = eC S + X^T (f Y), X and Y the tiles in xs and
+// ys (bases xb, yb), f per token in LDS.
+template <int K, int V, int CT, int NP>
+__device__ __forceinline__ void lin_step(f32x4 (&S)[CT][K / 16], const char* xs, int xb,
+                                         const char* ys, int yb, const float* f, float eC,
+                                         int grp) {
+#pragma unroll
+  for (int T = 0; T < CT; ++T)
+#pragma unroll
+    for (int t = 0; t < K / 16; ++t) S[T][t] *= eC;
+#pragma unroll
+  for (int kb = 0; kb < 2; ++kb) {
+    u16x8 part[CT][NP];
+#pragma unroll
+    for (int T = 0; T < CT; ++T)
+      lin_split(LinTile<V>::cols(ys, yb, kb, T), f + 32 * kb + 8 * grp, part[T]);
+#pragma unroll
+    for (int t = 0; t < K / 16; ++t) {
+      const u16x8 a = LinTile<K>::cols(xs, xb, kb, t);
+#pragma unroll
+      for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int T = 0; T < CT; ++T) S[T][t] = mfma16(a, part[T][p], S[T][t]);
+    }
+  }
+}
+
 // Contribution of a segment to the state after it: sum over its chunks of
 // X^T (f Y) with x = k, y = v, f = e^R; or (REV) to the gradient of the state
 // before it, chunks last to first, x = q, y = dO, f = scale e^G.  A wave owns
@@ -218,26 +245,7 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_segment_kernel(
     }
     __syncthreads();
     load(c0 + (i + 1) * step);
-    const float eC = __expf(tot);
-#pragma unroll
-    for (int T = 0; T < CT; ++T)
-#pragma unroll
-      for (int t = 0; t < K / 16; ++t) S[T][t] *= eC;
-#pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-      u16x8 part[CT][NP];
-#pragma unroll
-      for (int T = 0; T < CT; ++T)
-        lin_split(LinTile<V>::cols(ys, yb, kb, T), fac + 32 * kb + 8 * grp, part[T]);
-#pragma unroll
-      for (int t = 0; t < K / 16; ++t) {
-        const u16x8 a = LinTile<K>::cols(xs, xb, kb, t);
-#pragma unroll
-        for (int p = 0; p < NP; ++p)
-#pragma unroll
-          for (int T = 0; T < CT; ++T) S[T][t] = mfma16(a, part[T][p], S[T][t]);
-      }
-    }
+    lin_step<K, V, CT, NP>(S, xs, xb, ys, yb, fac, __expf(tot), grp);
     __syncthreads();
   }
 #pragma unroll
@@ -311,7 +319,10 @@ __global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int
 // ahead); what bounds a walk is the sum of a chunk's latencies (LDS reads, three
 // barriers) over the two workgroups that a CU holds: 8192 tokens, 32 v-heads
 // 59 us for 204 MB, 3.5 TB/s; 64 packed prompts in three parts 1035 us, 3.4 TB/s.
-template <int K, int V, int CT, int NP, bool OUT, bool SAVE>
+//
+// ALONE: no launch has formed the segments' start states; each segment first
+// steps the state through the chunks before it.
+template <int K, int V, int CT, int NP, bool OUT, bool SAVE, bool ALONE>
 __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k,
     const uint16_t* __restrict__ v, TokenStride ts, LinDecay dec, LinGrid grid, int Hqk, int Hv,
@@ -337,13 +348,20 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
   if (!lin_item(grid, grid.nseg, Hqk, Hv, sid, h)) return;
   if (grid.table) sid = grid.order[sid];
   const int hq = h / (Hv / Hqk);
-  const LinSeg sg = lin_seg(grid, sid);
+  LinSeg sg = lin_seg(grid, sid);
   if (sg.seq < 0) return;
+  int own = 0;   // the segment's first chunk
+  if (ALONE) {
+    own = sid % grid.nps * grid.L;
+    sg.tok0 -= own * kChunk;
+    sg.ntok += own * kChunk;
+    sg.chunk0 -= own;
+  }
   const int nc = (sg.ntok + kChunk - 1) / kChunk;
 
   f32x4 S[CT][K / 16];   // rows 16 t + 4 grp + r, column 16 (CT w + T) + r16
   // (several segments: the first one's from the join too, since ht may be h0)
-  const float* src = sg.first && sg.last ? (h0 ? h0 + ((size_t)sg.seq * Hv + h) * K * V : nullptr)
+  const float* src = ALONE || (sg.first && sg.last) ? (h0 ? h0 + ((size_t)sg.seq * Hv + h) * K * V : nullptr)
                               : segs + ((size_t)sid * Hv + h) * K * V;
 #pragma unroll
   for (int T = 0; T < CT; ++T) lin_load_state<K, V>(S[T], src, CT * w + T, lane);
@@ -360,7 +378,7 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
     const int n = c < nc ? sg.ntok - c * kChunk : 0;
     const size_t t = n > 0 ? (size_t)sg.tok0 + c * kChunk : 0;
     if (w < 2) lg.load(dec, t, min(n, 64), h, Hv, gi);
-    if (OUT) sq.load(q + t * ts.q + hq * K, ts.q, min(n, 64), qf);
+    if (OUT && c >= own) sq.load(q + t * ts.q + hq * K, ts.q, min(n, 64), qf);
     sk.load(k + t * ts.k + hq * K, ts.k, min(n, 64), kf);
     sv.load(v + t * ts.v + h * V, ts.v, min(n, 64), vr);
   };
@@ -375,8 +393,30 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
   int kcb = LinTile<K>::col_base(0, lane);
   int vb = LinTile<V>::col_base(CT * w, lane), pb = LinTile<64>::row_base(lane);
   int pw = LinTile<64>::off(r16, grp >> 1) + (grp & 1) * 8;
+  auto decays = [&]() {   // two waves
+    const float pre = lg.prefix(dec, gi) * kLog2e, e = exp2_(pre);
+    if (w == 1) {
+      sK[63 - lane] = e;
+    } else {
+      sG[lane] = pre;
+      sQ[lane] = scale * e;
+    }
+  };
   load(0);
-  for (int c = 0; c < nc; ++c) {
+  if constexpr (ALONE) {
+    for (int c = 0; c < own; ++c) {
+      hide(kcb);
+      hide(vb);
+      sk.store(ks, kt, tid);
+      sv.store(vs, vt, tid);
+      if (w < 2) decays();
+      __syncthreads();
+      load(c + 1);
+      lin_step<K, V, CT, NP>(S, ks, kcb, vs, vb, sK, exp2_(sG[63]), grp);
+      __syncthreads();
+    }
+  }
+  for (int c = own; c < nc; ++c) {
     // (nothing derived from these is kept from one chunk for the next)
     int ln = lane;
     hide(ln);
@@ -395,15 +435,7 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
     if (OUT) sq.store(qs, kt, tid);
     sk.store(ks, kt, tid);
     sv.store(vs, vt, tid);
-    if (w < 2) {
-      const float pre = lg.prefix(dec, gi) * kLog2e, e = exp2_(pre);
-      if (w == 1) {
-        sK[63 - lane] = e;
-      } else {
-        sG[lane] = pre;
-        sQ[lane] = scale * e;
-      }
-    }
+    if (w < 2) decays();
     __syncthreads();
     if (!OUT) load(c + 1);
 
@@ -568,6 +600,12 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
   }
 }
 
+__global__ __launch_bounds__(256) void lin_copy_kernel(const f32x4* __restrict__ from,
+                                                       f32x4* __restrict__ to, size_t n) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) to[i] = from[i];
+}
+
 // 16-column tiles per wave.  Two in the walk of a 128-column state read half of
 // what one reads from LDS (64 packed prompts 1082 us against 1297, 8192 tokens
 // 113 against 123); a walk of 64 columns has room for twice the waves with one.
@@ -576,6 +614,15 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
 template <int V>
 constexpr int kColTiles = V == 128 ? 2 : 1;
 constexpr int kSegTiles = 1;
+// Whether each chunk's workgroup steps through those before it by itself.  One
+// launch of 9 us and 2 per chunk stands against three of 16 (4 v-heads) to 19 us
+// and up to 1 per chunk (32 v-heads): 16 -> 32 heads, 192 tokens 13.5 us against
+// 21.0, 449 23.3 against 25.3, 640 32.0 both, 1024 49.5 against 38.5; 2 -> 4
+// heads, 512 tokens 22.4 against 17.7.
+inline bool lin_alone(const LinGrid& g, int Hv) {
+  return !g.table && g.nps > 1 && g.L == 1 &&
+         (g.nps <= 4 || (g.nps <= 9 && (long long)g.nseg * Hv >= device_cus()));
+}
 
 // ------------------------------------------------------------------ host ----
 // Chunks per segment: as many as spread all chunks over two workgroups per CU
@@ -689,7 +736,15 @@ void launch_walk(const uint16_t* q, const uint16_t* k, const uint16_t* v, TokenS
   // (the saved states have the same bits whether they are formed with o and ht
   // or again)
   const bool full = ht || states;
-  if (g.nlong > 0) {
+  // (ht over h0, which the other workgroups still read: they read a copy)
+  const bool alone = lin_alone(g, Hv);
+  if (alone && ht && ht == h0) {
+    const size_t n = (size_t)g.N * Hv * K * V / 4;
+    hipLaunchKernelGGL(lin_copy_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st,
+                       reinterpret_cast<const f32x4*>(h0), reinterpret_cast<f32x4*>(segs), n);
+    h0 = segs;
+  }
+  if (g.nlong > 0 && !alone) {
     // equal lengths without saved states: the final states come from the segments'
     // contributions, and the walk, for o alone, takes two parts
     const bool end = ht && !states && !g.table;
@@ -698,14 +753,23 @@ void launch_walk(const uint16_t* q, const uint16_t* k, const uint16_t* v, TokenS
     if (end) ht = nullptr;
   }
   const dim3 items(lin_items(g.nseg, Hqk, Hv));
-#define GDN_LW(NP, OUT, SAVE)                                                                   \
-  hipLaunchKernelGGL((lin_walk_kernel<K, V, kColTiles<V>, NP, OUT, SAVE>), items,                  \
-                     dim3(4 * V / kColTiles<V>), 0, st, q, k, v, ts, d, g, Hqk, Hv, scale, h0, ht, \
-                     segs, o, states)
-  if (o && states) GDN_LW(3, true, true);
-  else if (!o) GDN_LW(3, false, true);
-  else if (ht) GDN_LW(3, true, false);
-  else GDN_LW(2, true, false);
+#define GDN_LW(NP, OUT, SAVE, ALONE)                                                            \
+  hipLaunchKernelGGL((lin_walk_kernel<K, V, kColTiles<V>, NP, OUT, SAVE, ALONE>), items,        \
+                     dim3(4 * V / kColTiles<V>), 0, st, q, k, v, ts, d, g, Hqk, Hv, scale, h0,  \
+                     ht, segs, o, states)
+  if (o && states) {
+    if (alone) GDN_LW(3, true, true, true);
+    else GDN_LW(3, true, true, false);
+  } else if (!o) {
+    if (alone) GDN_LW(3, false, true, true);
+    else GDN_LW(3, false, true, false);
+  } else if (ht) {
+    if (alone) GDN_LW(3, true, false, true);
+    else GDN_LW(3, true, false, false);
+  } else {
+    if (alone) GDN_LW(2, true, false, true);
+    else GDN_LW(2, true, false, false);
+  }
 #undef GDN_LW
 }
 }  // namespace

@@ -362,3 +362,26 @@ def test_odd_addresses(rocm_device):
         ave.chunk_linear_attn(*args, initial_state=t["h0"], final_state=odd(t["h0"]), output_final_state=True)
     with pytest.raises(ValueError, match="aligned"):
         ave.chunk_linear_attn(*args, out=odd(t["v"]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 130, 2, 4, 128, 128), (2, 256, 1, 1, 64, 64), (3, 500, 16, 32, 128, 64),
+                                   (1, 570, 16, 32, 64, 128), (1, 600, 16, 32, 128, 128)])
+def test_short_prompts(rocm_device, shape):
+    """Prompts of a few chunks, each chunk's workgroup by itself, and just beyond them: o, the
+    final state, also over the initial one, and the gradients' states."""
+    import avelang_amd as ave
+    d = make(*shape, seed=21)
+    o, ht = linear_ref.linear_attn(d["q"], d["k"], d["v"], d["g"], h0=d["h0"])
+    t = to(d, rocm_device)
+    args = (t["q"], t["k"], t["v"], t["g"])
+    got, s = ave.chunk_linear_attn(*args, initial_state=t["h0"], output_final_state=True)
+    assert far(got, o) <= 2 ** -8 and far(s, ht) <= 2 ** -20
+    state = t["h0"].clone()
+    got2, _ = ave.chunk_linear_attn(*args, initial_state=state, output_final_state=True, final_state=state)
+    assert torch.equal(got, got2) and torch.equal(state, s)
+    _, _, states = ave.chunk_linear_attn_fwd_save(*args, initial_state=t["h0"])
+    kw = dict(initial_state=t["h0"])
+    a = ave.chunk_linear_attn_bwd(*args, t["do"], t["dht"], states=states, **kw)
+    b = ave.chunk_linear_attn_bwd(*args, t["do"], t["dht"], **kw)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
