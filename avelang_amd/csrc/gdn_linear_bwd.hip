@@ -323,20 +323,22 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
         zero(Y);
       }
       // the parts of dk from D and of dq from S: products, then the tokens' factors
-      auto inter = [&](f32x4 (&out)[4][2], const float* fac, const char* own, auto sums, auto&& op,
-                       auto&& rows) {
+      auto inter = [&](auto parts, f32x4 (&out)[4][2], const float* fac, const char* own, auto sums,
+                       auto&& op, auto&& rows) {
         f32x4 Z[4][2];
         zero(Z);
 #pragma unroll
         for (int b = 0; b < V / 32; ++b) {
-          u16x8 f[2];
+          u16x8 f[2][parts];
 #pragma unroll
-          for (int T = 0; T < 2; ++T) f[T] = op(T, b);
+          for (int T = 0; T < 2; ++T) op(T, b, f[T]);
 #pragma unroll
           for (int tt = 0; tt < 4; ++tt) {
             const u16x8 x = rows(tt, b);
 #pragma unroll
-            for (int T = 0; T < 2; ++T) Z[tt][T] = mfma16(f[T], x, Z[tt][T]);
+            for (int p = 0; p < parts; ++p)
+#pragma unroll
+              for (int T = 0; T < 2; ++T) Z[tt][T] = mfma16(f[T][p], x, Z[tt][T]);
           }
         }
 #pragma unroll
@@ -357,18 +359,22 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
         }
       };
       float cs = 0.f;
-      inter(X, sK, ks, lds.bsum,
-            [&](int T, int b) {
-              // <S, D> from both parts of D: it is most of dg where the memory is
-              // long, and the sum of K V products would show their rounding
+      inter(std::integral_constant<int, 2>{}, X, sK, ks, lds.bsum,
+            [&](int T, int b, u16x8 (&out)[2]) {
+              // both parts of D: <S, D> and b are sums of random signs in dg, which
+              // show their rounding in full (dg's error against 64 bits over 28 shapes,
+              // in its own rounding: 90 % within 1.46, at most 1.73; 1.73 and 1.88 with
+              // one part for b; the step at 8192 tokens 3 % more)
               const u16x8 f = LinTile<K>::cols4(ds, dcb, b, T);
               const u16x8 l = LinTile<K>::cols4(dl, dcb, b, T);
 #pragma unroll
               for (int i = 0; i < 8; ++i) cs += (bf2f(f[i]) + bf2f(l[i])) * bf2f(SF[T][b][i]);
-              return f;
+              out[0] = f;
+              out[1] = l;
             },
             [&](int tt, int b) { return LinTile<V>::rows4(vs, vr4, tt, b); });
-      inter(Y, sQ, qs, lds.asum, [&](int T, int b) { return SF[T][b]; },
+      inter(std::integral_constant<int, 1>{}, Y, sQ, qs, lds.asum,
+            [&](int T, int b, u16x8 (&out)[1]) { out[0] = SF[T][b]; },
             [&](int tt, int b) { return LinTile<V>::rows4(os, vr4, tt, b); });
       if (hh + 1 < HP) load_states(c, hh + 1);
       else load_states(c - 1, 0);
@@ -458,7 +464,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
 // (dk, dq, P, dP and with the saved states' fragments <S, D>, all of which
 // reduce over V).  NP: the parts of dO's products on the way to dh0 (three
 // where it is wanted).  8192 tokens, 16 -> 32 heads: 163 us, 403 MB read and
-// written at least (one head at a time, with fp32 parts of dq and dk summed by
+// written at least, 172 with both parts of D in dk (one head at a time, with fp32 parts of dq and dk summed by
 // a launch of their own, 226 + 59); bound by registers and LDS (157 KiB: one
 // workgroup of two waves per SIMD), whose latencies three barriers per head and
 // chunk expose.
