@@ -258,7 +258,7 @@ __global__ __launch_bounds__(4 * V / CT, 4 / CT) void lin_segment_kernel(
 // every segment's end) in place of the contributions, from `edge` (h0 / dht,
 // nullable); into `end` (nullable) the state after the last.  Bound by HBM: a
 // lane per E adjacent elements, four where that still gives every CU two
-// workgroups (449 tokens 26 us for all three launches against 31 with one, 8192
+// workgroups (449 tokens 26 us for three launches against 31 with one, 8192
 // tokens 101 against 105), else one, with as many segments' loads in flight.
 template <bool REV, int E>
 __global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int KV,
@@ -614,20 +614,22 @@ __global__ __launch_bounds__(256) void lin_copy_kernel(const f32x4* __restrict__
 template <int V>
 constexpr int kColTiles = V == 128 ? 2 : 1;
 constexpr int kSegTiles = 1;
-// Whether each chunk's workgroup steps through those before it by itself.  One
-// launch of 9 us and 2 per chunk stands against three of 16 (4 v-heads) to 19 us
-// and up to 1 per chunk (32 v-heads): 16 -> 32 heads, 192 tokens 13.5 us against
-// 21.0, 449 23.3 against 25.3, 640 32.0 both, 1024 49.5 against 38.5; 2 -> 4
-// heads, 512 tokens 22.4 against 17.7.
+// Whether each chunk's workgroup steps through those before it by itself, its
+// waves with one tile each (a workgroup has a CU to itself: 16 -> 32 heads, 100
+// tokens 10.1 us against 11.4 with two, 449 20.4 against 22.7).  One launch of 7
+// us and 1.7 per chunk stands against three of 16 (4 v-heads) to 19 us and up to
+// 1 per chunk (32 v-heads): 16 -> 32 heads, 256 tokens 13.7 us against 23.1, 449
+// 20.4 against 25.3, 768 37.6 against 33.6; 8 -> 16, 500 20.2 against 25.2; 2 ->
+// 4, 384 16.5 against 17.3, 500 19.5 against 17.6.
 inline bool lin_alone(const LinGrid& g, int Hv) {
   return !g.table && g.nps > 1 && g.L == 1 &&
-         (g.nps <= 4 || (g.nps <= 9 && (long long)g.nseg * Hv >= device_cus()));
+         (g.nps <= 6 || (g.nps <= 10 && 2LL * g.nseg * Hv >= device_cus()));
 }
 
 // ------------------------------------------------------------------ host ----
 // Chunks per segment: as many as spread all chunks over two workgroups per CU
-// once.  (8192 tokens, 32 v-heads: L = 8 101 us; 4 122, 16 111.  449 tokens:
-// L = 1 26 us; 2 30, 4 37, all 8 chunks in one walk 39.  20011 tokens, 4
+// once.  (8192 tokens, 32 v-heads: L = 8 101 us; 4 122, 16 111.  449 tokens, in
+// three launches: L = 1 26 us; 2 30, 4 37, all 8 chunks in one walk 39.  20011 tokens, 4
 // v-heads: L = 3 58 us; 2 70, 4 61, 16 103.)
 LinPlan lin_plan(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu, bool bwd) {
   LinPlan p{};
@@ -754,9 +756,9 @@ void launch_walk(const uint16_t* q, const uint16_t* k, const uint16_t* v, TokenS
   }
   const dim3 items(lin_items(g.nseg, Hqk, Hv));
 #define GDN_LW(NP, OUT, SAVE, ALONE)                                                            \
-  hipLaunchKernelGGL((lin_walk_kernel<K, V, kColTiles<V>, NP, OUT, SAVE, ALONE>), items,        \
-                     dim3(4 * V / kColTiles<V>), 0, st, q, k, v, ts, d, g, Hqk, Hv, scale, h0,  \
-                     ht, segs, o, states)
+  hipLaunchKernelGGL((lin_walk_kernel<K, V, ALONE ? 1 : kColTiles<V>, NP, OUT, SAVE, ALONE>),    \
+                     items, dim3(4 * V / (ALONE ? 1 : kColTiles<V>)), 0, st, q, k, v, ts, d, g,  \
+                     Hqk, Hv, scale, h0, ht, segs, o, states)
   if (o && states) {
     if (alone) GDN_LW(3, true, true, true);
     else GDN_LW(3, true, true, false);

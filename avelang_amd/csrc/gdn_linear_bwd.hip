@@ -463,8 +463,8 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
 // dh0) and leave it in LDS, in two bf16 parts, for the K / 32 waves that own 32 key columns
 // (dk, dq, P, dP and with the saved states' fragments <S, D>, all of which
 // reduce over V).  NP: the parts of dO's products on the way to dh0 (three
-// where it is wanted).  8192 tokens, 16 -> 32 heads: 163 us, 403 MB read and
-// written at least, 172 with both parts of D in dk (one head at a time, with fp32 parts of dq and dk summed by
+// where it is wanted).  8192 tokens, 16 -> 32 heads: 175 us, 403 MB read and
+// written at least, 163 with one part of D in dk (one head at a time, then, with fp32 parts of dq and dk summed by
 // a launch of their own, 226 + 59); bound by registers and LDS (157 KiB: one
 // workgroup of two waves per SIMD), whose latencies three barriers per head and
 // chunk expose.

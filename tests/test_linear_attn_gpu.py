@@ -366,7 +366,8 @@ def test_odd_addresses(rocm_device):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(1, 130, 2, 4, 128, 128), (2, 256, 1, 1, 64, 64), (3, 500, 16, 32, 128, 64),
-                                   (1, 570, 16, 32, 64, 128), (1, 600, 16, 32, 128, 128)])
+                                   (1, 640, 16, 32, 64, 128), (1, 650, 16, 32, 128, 128),
+                                   (1, 384, 2, 4, 128, 128), (1, 385, 2, 4, 128, 128)])
 def test_short_prompts(rocm_device, shape):
     """Prompts of a few chunks, each chunk's workgroup by itself, and just beyond them: o, the
     final state, also over the initial one, and the gradients' states."""
