@@ -30,6 +30,7 @@ struct LinGrid {
   int nseg;                 // segments at most
   int nlong;                // sequences of several segments at most
   int N, total;             // sequences, tokens of all
+  bool one;                 // one workgroup per CU
 };
 
 __device__ __forceinline__ LinSeg lin_seg(const LinGrid& g, int s) {
@@ -262,6 +263,7 @@ __device__ __forceinline__ bool lin_item(const LinGrid& g, int nseg, int Hqk, in
 // Host: how a call is cut (byte offsets into the workspace).
 struct LinPlan {
   int L, nps, nseg;          // as LinGrid
+  bool one;                  // as LinGrid
   long long chunks;          // chunks of all sequences at most (chunk-start states)
   int nlong;                 // sequences of several segments at most (0: no join)
   size_t table, status, order, joins, segs, decay, total;

@@ -608,35 +608,50 @@ __global__ __launch_bounds__(256) void lin_copy_kernel(const f32x4* __restrict__
 
 // 16-column tiles per wave.  Two in the walk of a 128-column state read half of
 // what one reads from LDS (64 packed prompts 1082 us against 1297, 8192 tokens
-// 113 against 123); a walk of 64 columns has room for twice the waves with one.
+// 113 against 123); a walk of 64 columns has room for twice the waves with one,
+// and where a workgroup has a CU to itself one is better for both (100 tokens of
+// 32 v-heads 10.1 us against 11.4, 3000 54.1 against 56.9).
 // In the segments both take the same time, and one leaves registers for four
 // waves per SIMD.
 template <int V>
 constexpr int kColTiles = V == 128 ? 2 : 1;
 constexpr int kSegTiles = 1;
-// Whether each chunk's workgroup steps through those before it by itself, its
-// waves with one tile each (a workgroup has a CU to itself: 16 -> 32 heads, 100
-// tokens 10.1 us against 11.4 with two, 449 20.4 against 22.7).  One launch of 7
-// us and 1.7 per chunk stands against three of 16 (4 v-heads) to 19 us and up to
-// 1 per chunk (32 v-heads): 16 -> 32 heads, 256 tokens 13.7 us against 23.1, 449
-// 20.4 against 25.3, 768 37.6 against 33.6; 8 -> 16, 500 20.2 against 25.2; 2 ->
-// 4, 384 16.5 against 17.3, 500 19.5 against 17.6.
+// Whether each chunk's workgroup steps through those before it by itself.  One
+// launch of 7 us and 1.7 per chunk stands against three of 15 (4 v-heads) to 18
+// us and up to 0.9 per chunk (32 v-heads): 16 -> 32 heads, 256 tokens 13.7 us
+// against 22.2, 449 20.7 against 24.4; 8 -> 16, 500 20.1 against 24.4; 16 -> 16,
+// 768 26.9 against 24.4; 2 -> 4, 384 16.4 both, 449 19.4 against 16.8.
 inline bool lin_alone(const LinGrid& g, int Hv) {
   return !g.table && g.nps > 1 && g.L == 1 &&
          (g.nps <= 6 || (g.nps <= 10 && 2LL * g.nseg * Hv >= device_cus()));
 }
 
 // ------------------------------------------------------------------ host ----
-// Chunks per segment: as many as spread all chunks over two workgroups per CU
-// once.  (8192 tokens, 32 v-heads: L = 8 101 us; 4 122, 16 111.  449 tokens, in
-// three launches: L = 1 26 us; 2 30, 4 37, all 8 chunks in one walk 39.  20011 tokens, 4
-// v-heads: L = 3 58 us; 2 70, 4 61, 16 103.)
+// Chunks per segment: as many as give every workgroup that the CUs hold one
+// segment.
+//
+// Forward: one workgroup per CU, of a wave per 16 columns, against two of a wave
+// per 32 (V = 64: 16), which has fewer contributions to write, join and read, but
+// also fewer latencies side by side.  K = V = 128 (us): 20011 tokens of 4
+// v-heads, 4.9 chunks per CU, 49.7 against 59.4; of 32 v-heads 1024 tokens, 2 per
+// CU, 30.0 and 38.8, 4096, 8 per CU, 67.4 and 71.0, 6000, 12 per CU, 87.0 and
+// 88.2, 8192, 16 per CU, 113 and 107.  K = 64, V = 128: 2048 tokens 32.9 and 36.3,
+// 4096 50.8 and 50.5, 6000 67.7 and 64.4.  V = 64: 8192 tokens of 4 v-heads, 2 per
+// CU, 29.5 and 33.3, 2048 of 32, 4 per CU, 34.0 and 33.5, 3000 43.2 and 40.5.
+//
+// Backward: a workgroup of the gradients has a CU to itself, or half (K = V = 64),
+// and one or two v-heads.  (Training steps in us: 16 -> 16 heads of 128, 4096
+// tokens 119, with twice the segments 132; 16 -> 32 of 64, 8192 tokens 153, with
+// half 180; 16 -> 32 of 128, 8192 tokens 333, with half 467.)
 LinPlan lin_plan(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu, bool bwd) {
   LinPlan p{};
   const long long tokens = (long long)B * T;
   const long long per = ((long long)T + kChunk - 1) / kChunk;   // chunks of the longest sequence
   p.chunks = has_cu ? tokens / kChunk + N : B * per;
-  const long long slots = 2LL * device_cus();
+  const long long cus = device_cus();
+  p.one = !bwd && p.chunks * Hv < (V == 64 ? 4 : K == 64 ? 8 : 12) * cus;
+  const long long slots = cus * (bwd ? (K + V == 128 ? 2 : 1) * (lin_pair(Hqk, Hv) ? 2 : 1)
+                                     : p.one ? 1 : 2);
   long long L = (p.chunks * Hv + slots - 1) / slots;
   if (L < 1) L = 1;
   if (L > per) L = per > 0 ? per : 1;
@@ -679,6 +694,7 @@ LinGrid lin_grid(const LinPlan& p, unsigned char* ws, int T, int N, int total, b
   g.T = T;
   g.L = p.L;
   g.nps = p.nps;
+  g.one = p.one;
   g.nseg = p.nseg;
   g.nlong = p.nlong;
   g.N = N;
@@ -755,23 +771,23 @@ void launch_walk(const uint16_t* q, const uint16_t* k, const uint16_t* v, TokenS
     if (end) ht = nullptr;
   }
   const dim3 items(lin_items(g.nseg, Hqk, Hv));
-#define GDN_LW(NP, OUT, SAVE, ALONE)                                                            \
-  hipLaunchKernelGGL((lin_walk_kernel<K, V, ALONE ? 1 : kColTiles<V>, NP, OUT, SAVE, ALONE>),    \
-                     items, dim3(4 * V / (ALONE ? 1 : kColTiles<V>)), 0, st, q, k, v, ts, d, g,  \
-                     Hqk, Hv, scale, h0, ht, segs, o, states)
-  if (o && states) {
-    if (alone) GDN_LW(3, true, true, true);
-    else GDN_LW(3, true, true, false);
-  } else if (!o) {
-    if (alone) GDN_LW(3, false, true, true);
-    else GDN_LW(3, false, true, false);
-  } else if (ht) {
-    if (alone) GDN_LW(3, true, false, true);
-    else GDN_LW(3, true, false, false);
+#define GDN_LW(CT, NP, OUT, SAVE, ALONE)                                                     \
+  hipLaunchKernelGGL((lin_walk_kernel<K, V, CT, NP, OUT, SAVE, ALONE>), items,               \
+                     dim3(4 * V / CT), 0, st, q, k, v, ts, d, g, Hqk, Hv, scale, h0, ht, segs, \
+                     o, states)
+#define GDN_LWS(CT, ALONE)                         \
+  if (o && states) GDN_LW(CT, 3, true, true, ALONE); \
+  else if (!o) GDN_LW(CT, 3, false, true, ALONE);  \
+  else if (ht) GDN_LW(CT, 3, true, false, ALONE);  \
+  else GDN_LW(CT, 2, true, false, ALONE)
+  if (alone) {
+    GDN_LWS(1, true);
+  } else if (g.one) {
+    GDN_LWS(1, false);
   } else {
-    if (alone) GDN_LW(2, true, false, true);
-    else GDN_LW(2, true, false, false);
+    GDN_LWS(kColTiles<V>, false);
   }
+#undef GDN_LWS
 #undef GDN_LW
 }
 }  // namespace
