@@ -12,6 +12,7 @@ namespace gdn {
 struct LinSeg {
   int tok0, ntok, chunk0, seq;
   int first, last;   // first / last segment of its sequence
+  int before;        // chunks of its sequence before it
 };
 
 // A sequence of several segments (seq < 0: no more of them): s0 .. s1 - 1.
@@ -43,6 +44,7 @@ __device__ __forceinline__ LinSeg lin_seg(const LinGrid& g, int s) {
   r.chunk0 = r.seq * ((g.T + kChunk - 1) / kChunk) + i * g.L;
   r.first = i == 0;
   r.last = i == g.nps - 1;
+  r.before = i * g.L;
   return r;
 }
 

@@ -9,14 +9,14 @@
 // all products on bf16 MFMA with fp32 accumulation.  e^{R_j} v_j enters as a
 // sum of bf16 parts: three (2^-24) where a state is returned or saved, two
 // (2^-16) where it serves o alone; P and the state's copy that q reads are
-// single bf16 (2^-8, the size of o's own rounding).  R is summed from the chunk's end, not as G_63 - G_j:
-// its error stays in proportion to the decay it gives.
+// single bf16 (2^-8, the size of o's own rounding).  R is summed from the chunk's
+// end, not as G_63 - G_j: its error stays in proportion to the decay it gives.
 //
 // A sequence is cut into segments of L chunks that run at the same time: one
 // launch forms every segment's own contribution to the state (from k, v and
 // g), one joins them along each sequence, one walks every segment from its
-// start state and writes o.  Where a whole sequence fits a segment the first
-// two are left out.
+// start state and writes o.  Where a whole sequence fits a segment, and where a
+// few chunks are stepped through again faster, the first two are left out.
 #include <initializer_list>
 
 #include "gdn_linear.h"
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(1024) void lin_table_kernel(const int32_t* cu, LinS
     if (n < N) {
       for (int i = 0; i < ns && sa + i < nseg; ++i) {
         const int ntok = min(len - i * L * kChunk, L * kChunk);
-        table[sa + i] = LinSeg{s + i * L * kChunk, ntok, sb + i * L, n, i == 0, i == ns - 1};
+        table[sa + i] = LinSeg{s + i * L * kChunk, ntok, sb + i * L, n, i == 0, i == ns - 1, i * L};
         atomicAdd(&bin[bin_of(ntok)], 1);
       }
       if (ns > 1) {
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(1024) void lin_table_kernel(const int32_t* cu, LinS
     }
   }
   for (int i = seg0 + tid; i < nseg; i += 1024) {
-    table[i] = LinSeg{0, 0, 0, -1, 0, 0};
+    table[i] = LinSeg{0, 0, 0, -1, 0, 0, 0};
     order[i] = i;
   }
   __syncthreads();
@@ -352,7 +352,7 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
   if (sg.seq < 0) return;
   int own = 0;   // the segment's first chunk
   if (ALONE) {
-    own = sid % grid.nps * grid.L;
+    own = sg.before;
     sg.tok0 -= own * kChunk;
     sg.ntok += own * kChunk;
     sg.chunk0 -= own;
@@ -616,13 +616,15 @@ __global__ __launch_bounds__(256) void lin_copy_kernel(const f32x4* __restrict__
 template <int V>
 constexpr int kColTiles = V == 128 ? 2 : 1;
 constexpr int kSegTiles = 1;
-// Whether each chunk's workgroup steps through those before it by itself.  One
+// Whether each chunk's workgroup steps through those before it by itself (packed
+// sequences: nps is of one that had all tokens).  One
 // launch of 7 us and 1.7 per chunk stands against three of 15 (4 v-heads) to 18
 // us and up to 0.9 per chunk (32 v-heads): 16 -> 32 heads, 256 tokens 13.7 us
 // against 22.2, 449 20.7 against 24.4; 8 -> 16, 500 20.1 against 24.4; 16 -> 16,
-// 768 26.9 against 24.4; 2 -> 4, 384 16.4 both, 449 19.4 against 16.8.
+// 768 26.9 against 24.4; 2 -> 4, 384 16.4 both, 449 19.4 against 16.8; packed, 16
+// -> 32, two of 100 tokens 16.1 against 27.0.
 inline bool lin_alone(const LinGrid& g, int Hv) {
-  return !g.table && g.nps > 1 && g.L == 1 &&
+  return g.nps > 1 && g.L == 1 &&
          (g.nps <= 6 || (g.nps <= 10 && 2LL * g.nseg * Hv >= device_cus()));
 }
 

@@ -386,3 +386,27 @@ def test_short_prompts(rocm_device, shape):
     a = ave.chunk_linear_attn_bwd(*args, t["do"], t["dht"], states=states, **kw)
     b = ave.chunk_linear_attn_bwd(*args, t["do"], t["dht"], **kw)
     assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[100, 0, 200], [384], [385, 1], [64, 128, 1, 65, 130]])
+def test_short_packed_prompts(rocm_device, lens):
+    """Packed prompts of few tokens in all: each as by itself, the state also over the initial
+    one, and the gradients' states formed again."""
+    import avelang_amd as ave
+    cu = cu_of(lens)
+    d = make(1, cu[-1], 2, 4, 128, 128, seed=31, lens=lens)
+    t = to(d, rocm_device)
+    o, ht = linear_ref.linear_attn(d["q"], d["k"], d["v"], d["g"], h0=d["h0"], cu=cu)
+    args, c = (t["q"], t["k"], t["v"], t["g"]), torch.tensor(cu, device=rocm_device)
+    got, s = ave.chunk_linear_attn(*args, initial_state=t["h0"], output_final_state=True, cu_seqlens=c)
+    assert far(got, o) <= 2 ** -8 and far(s, ht) <= 2 ** -20
+    state = t["h0"].clone()
+    got2, _ = ave.chunk_linear_attn(*args, initial_state=state, output_final_state=True, cu_seqlens=c,
+                                    final_state=state)
+    assert torch.equal(got, got2) and torch.equal(state, s)
+    kw = dict(initial_state=t["h0"], cu_seqlens=c)
+    _, _, states = ave.chunk_linear_attn_fwd_save(*args, **kw)
+    a = ave.chunk_linear_attn_bwd(*args, t["do"], t["dht"], states=states, **kw)
+    b = ave.chunk_linear_attn_bwd(*args, t["do"], t["dht"], **kw)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
