@@ -8,8 +8,8 @@
 //     S'   = e^{G_63} S + sum_j k_j (e^{R_j} v_j)^T
 // all products on bf16 MFMA with fp32 accumulation.  e^{R_j} v_j enters as a
 // sum of bf16 parts: three (2^-24) where a state is returned or saved, two
-// (2^-16) where it serves o alone; P and the state's copy that q reads are
-// single bf16 (2^-8, the size of o's own rounding).  R is summed from the chunk's
+// (2^-16) where it serves o alone; P two; the state's copy that q reads is single
+// bf16 (2^-8, the size of o's own rounding).  R is summed from the chunk's
 // end, not as G_63 - G_j: its error stays in proportion to the decay it gives.
 //
 // A sequence is cut into segments of L chunks that run at the same time: one
@@ -318,7 +318,7 @@ __global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int
 // K, q and v come from HBM once (registers to swizzled LDS tiles, a chunk
 // ahead); what bounds a walk is the sum of a chunk's latencies (LDS reads, three
 // barriers) over the two workgroups that a CU holds: 8192 tokens, 32 v-heads
-// 59 us for 204 MB, 3.5 TB/s; 64 packed prompts in three parts 1035 us, 3.4 TB/s.
+// 64 us for 204 MB, 3.2 TB/s; 64 packed prompts in three parts 1069 us, 3.3 TB/s.
 //
 // ALONE: no launch has formed the segments' start states; each segment first
 // steps the state through the chunks before it.
@@ -332,7 +332,7 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
   __shared__ __align__(16) char qs[LinTile<K>::BYTES];
   __shared__ __align__(16) char ks[LinTile<K>::BYTES];
   __shared__ __align__(16) char vs[LinTile<V>::BYTES];
-  __shared__ __align__(16) char ps[LinTile<64>::BYTES];
+  __shared__ __align__(16) char ps[LinTile<64>::BYTES], pl[LinTile<64>::BYTES];   // P in two parts
   __shared__ __align__(16) float sG[64], sQ[64], sK[64];   // G log2(e), scale e^G, e^R
   const int tid = threadIdx.x, lane = tid % 64, w = wave_index();
   const int r16 = lane % 16, grp = lane / 16;
@@ -387,6 +387,7 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
     for (int i = tid; i < 64; i += NT) {
       const int r = i / 2 % 16 + (i / 32) * 32, u = 4 * (i / 32) + 2 + i % 2;
       *reinterpret_cast<u32x4*>(ps + LinTile<64>::off(r, u)) = u32x4{0, 0, 0, 0};
+      *reinterpret_cast<u32x4*>(pl + LinTile<64>::off(r, u)) = u32x4{0, 0, 0, 0};
     }
   }
   int rb = LinTile<K>::row_base(lane), r4b = LinTile<K>::row4_base(lane);
@@ -440,7 +441,10 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
     if (!OUT) load(c + 1);
 
     if (OUT) {
-      // P, tile by tile (token block it, source block jt), as bf16 rows
+      // P, tile by tile (token block it, source block jt), as rows of two bf16 parts:
+      // one's rounding is the same for all of a value's columns, which the first
+      // token after an empty state shows in full (1.73 of o's own; 449 tokens 1 %
+      // more, 8192 2 %, 64 packed prompts 4 %)
       for (int n = w; n < 10; n += NW) {
         const int it = tmat_block_row(n), jt = n - tmat_block(it, 0);
         f32x4 p = zero4();
@@ -457,7 +461,10 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
           const bool in = j + r <= i;
           p[r] = (in ? p[r] * scale : 0.f) * exp2_(in ? gi - gj[r] : 0.f);
         }
-        *reinterpret_cast<u16x4*>(ps + (pw ^ (32 * jt)) + it * 2048) = f2bf4(p);
+        u16x4 hi, lo;
+        split_bf4(p, hi, lo);
+        *reinterpret_cast<u16x4*>(ps + (pw ^ (32 * jt)) + it * 2048) = hi;
+        *reinterpret_cast<u16x4*>(pl + (pw ^ (32 * jt)) + it * 2048) = lo;
       }
     }
     if (OUT) load(c + 1);
@@ -556,6 +563,9 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
           const u16x8 f = LinTile<64>::rows(ps, pb, tt, kb);
 #pragma unroll
           for (int T = 0; T < CT; ++T) O[tt][T] = mfma16(vm[T], f, O[tt][T]);
+          const u16x8 fl = LinTile<64>::rows(pl, pb, tt, kb);
+#pragma unroll
+          for (int T = 0; T < CT; ++T) O[tt][T] = mfma16(vm[T], fl, O[tt][T]);
         }
         if (!clean) {
 #pragma unroll
