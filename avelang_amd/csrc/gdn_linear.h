@@ -195,8 +195,8 @@ __device__ __forceinline__ float lane63(float x) {
 
 // Eight bf16 values times eight fp32 factors (in LDS) as a sum of NP bf16
 // parts, 2^-8 per part.  Three where a state is returned or saved (its error
-// then is fp32's, 2e-7 of it; two leave 3e-6 and cost 64 packed prompts 944 us
-// in place of 1037, 8192 tokens 100 of 105), two where it serves bf16 outputs.
+// then is fp32's, 2e-7 of it; two leave 3e-6 and cost 64 packed prompts 957 us
+// in place of 1067, 8192 tokens 100 of 105), two where it serves bf16 outputs.
 template <int NP>
 __device__ __forceinline__ void lin_split(u16x8 y, const float* f, u16x8 (&part)[NP]) {
   const f32x4 f0 = *reinterpret_cast<const f32x4*>(f), f1 = *reinterpret_cast<const f32x4*>(f + 4);

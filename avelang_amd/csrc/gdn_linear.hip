@@ -47,7 +47,7 @@ __global__ __launch_bounds__(1024) void lin_table_kernel(const int32_t* cu, LinS
   auto bin_of = [&](int ntok) {   // longer ones first
     return BINS - 1 - (int)((long long)(ntok + kChunk - 1) / kChunk * (BINS - 1) / L);
   };
-  int seg0 = 0, chunk0 = 0;   // of this round's first sequence
+  int seg0 = 0, chunk0 = 0;   // of these 1024 sequences' first
   for (int n0 = 0; n0 < N; n0 += 1024) {
     const int n = n0 + tid;
     const int s = n < N && !bad ? cu[n] : 0;
