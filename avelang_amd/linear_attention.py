@@ -220,6 +220,7 @@ def _chunk_bwd(inputs, do, dht, scale, initial_state, states, workspace, name):
         need = lib.gdn_linear_states_bytes(B, T, Hv, K, V, N, cu is not None)
         if states.device != dev or states.numel() * states.element_size() < need:
             raise ValueError(f"{name}: states must hold {need} bytes on {dev}.")
+        states = states.contiguous()
     bf = dict(dtype=torch.bfloat16, device=dev)
     dq, dk = torch.empty((B, T, Hqk, K), **bf), torch.empty((B, T, Hqk, K), **bf)
     dv = torch.empty((B, T, Hv, V), **bf)
@@ -249,7 +250,7 @@ class _ChunkLinearAttn(torch.autograd.Function):
         inputs = _inputs(q, k, v, g, cu_seqlens, name)
         o, ht, states = _chunk_fwd(inputs, scale, initial_state, output_final_state, name, save=save)
         ctx.save_for_backward(*inputs[:5], initial_state, states)
-        ctx.rest = inputs[5:] + (scale, g.dtype)
+        ctx.rest = scale, g.dtype
         ctx.set_materialize_grads(False)
         return (o, ht) if output_final_state else o
 
@@ -257,11 +258,14 @@ class _ChunkLinearAttn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, do, dht=None):
         q, k, v, g, cu, h0, states = ctx.saved_tensors
-        rows, dims, scale, g_type = ctx.rest
+        scale, g_type = ctx.rest
         if do is None:
             do = torch.zeros(v.shape, dtype=v.dtype, device=v.device)
-        dq, dk, dv, dg, dh0 = _chunk_bwd((q, k, v, g, cu, rows, dims), do, dht, scale, h0, states,
-                                         None, "chunk_linear_attn")
+        # (token strides and alignment as they are now: a hook on saved tensors, one
+        # that offloads them say, returns others of another layout)
+        name = "chunk_linear_attn"
+        dq, dk, dv, dg, dh0 = _chunk_bwd(_inputs(q, k, v, g, cu, name), do, dht, scale, h0, states,
+                                         None, name)
         return dq, dk, dv, dg if dg.dtype is g_type else dg.to(g_type), None, dh0, None, None, None
 
 

@@ -1,0 +1,94 @@
+"""What linear attention's and layer norm's autograd forms keep for the backward: saved tensors
+come back from hooks (offloading to the host, say) in another layout than they went in with.
+
+Tolerances: none, the same bits with a hook as without.
+"""
+import pytest
+import torch
+
+from avelang_amd import linear_attention as L
+
+BF = torch.bfloat16
+
+
+def _slices(B, T, Hqk, Hv, K, V, device="cpu", seed=0):
+    """q, k, v as column slices of one tensor, which are read in place, and g."""
+    gen = torch.Generator().manual_seed(seed)
+    widths = [Hqk * K, Hqk * K, Hv * V]
+    y = torch.randn((B, T, sum(widths) + 16), generator=gen).to(BF).to(device)
+    q, k, v = (x.reshape(B, T, h, d) for x, h, d in zip(y[..., :-16].split(widths, -1),
+                                                       (Hqk, Hqk, Hv), (K, K, V)))
+    return q, k, v, -torch.rand((B, T, Hv), generator=gen).to(device)
+
+
+def _odd(x):
+    """x at an address off 16 bytes (contiguous otherwise)."""
+    if x.dtype is not BF:
+        return x
+    return torch.empty(x.numel() + 1, dtype=x.dtype, device=x.device)[1:].view(x.shape).copy_(x)
+
+
+def _strided(x):
+    """x's values with its last two axes stored the other way round."""
+    return x if x.dim() < 2 else x.transpose(-1, -2).contiguous().transpose(-1, -2)
+
+
+HOOKS = {"contiguous": lambda x: x.contiguous(), "odd": _odd, "strided": _strided}
+
+
+@pytest.mark.parametrize("hook", sorted(HOOKS) + ["cpu"])
+def test_strides_of_what_comes_back(monkeypatch, hook):
+    """The backward is given the strides of the tensors it reads, not of those that were saved."""
+    seen = {}
+
+    def inputs(q, k, v, g, cu, name, out=None):   # the checks of devices left out
+        q, k, v, rows = L._in_place(q, k, v, out)
+        if rows is None:
+            rows = tuple(x.shape[2] * x.shape[3] for x in (q, k, v))
+            q, k, v = (x if x.data_ptr() % 16 == 0 else x.clone() for x in (q, k, v))
+        dims = (*q.shape[:3], v.shape[2], q.shape[3], v.shape[3], q.shape[0])
+        return q, k, v, g.contiguous(), cu, rows, dims
+
+    def bwd(inputs, do, dht, scale, h0, states, *rest):
+        seen["inputs"] = inputs
+        q, k, v, g = inputs[:4]
+        return torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), torch.zeros_like(g), None
+    monkeypatch.setattr(L, "_inputs", inputs)
+    monkeypatch.setattr(L, "_chunk_fwd", lambda inputs, *a, **kw: (inputs[2].contiguous(), None, None))
+    monkeypatch.setattr(L, "_chunk_bwd", bwd)
+    args = [x.requires_grad_() for x in _slices(2, 5, 2, 4, 64, 128)]
+    around = (torch.autograd.graph.save_on_cpu() if hook == "cpu" else
+              torch.autograd.graph.saved_tensors_hooks(HOOKS[hook], lambda x: x))
+    with around:
+        o, _ = L.chunk_linear_attn(*args)
+    o.sum().backward()
+    q, k, v, g, _, rows, _ = seen["inputs"]
+    for x, want, row in zip((q, k, v), args, rows):
+        assert torch.equal(x, want)
+        assert x.data_ptr() % 16 == 0
+        assert x.stride() == (5 * row, row, x.shape[3], 1)
+    assert g.is_contiguous()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hook", sorted(HOOKS) + ["cpu"])
+@pytest.mark.parametrize("save", [True, False])
+@pytest.mark.parametrize("packed", [False, True])
+def test_gradients_through_hooks(rocm_device, hook, save, packed):
+    import avelang_amd as ave
+    B, T = (1, 150) if packed else (2, 75)
+    cu = torch.tensor([0, 70, 150], dtype=torch.int32, device=rocm_device) if packed else None
+    gen = torch.Generator().manual_seed(3)
+    h0 = torch.randn((2, 4, 64, 128), generator=gen).to(rocm_device).requires_grad_()
+    do = torch.randn((B, T, 4, 128), generator=gen).to(BF).to(rocm_device)
+
+    def grads(around):
+        leaves = [x.requires_grad_() for x in _slices(B, T, 2, 4, 64, 128, rocm_device)] + [h0]
+        with around:
+            o, ht = ave.chunk_linear_attn(*leaves[:4], initial_state=h0, output_final_state=True,
+                                          cu_seqlens=cu, save_for_backward=save)
+        return torch.autograd.grad([o, ht], leaves, [do, torch.ones_like(ht)])
+    want = grads(torch.autograd.graph.saved_tensors_hooks(lambda x: x, lambda x: x))
+    got = grads(torch.autograd.graph.save_on_cpu() if hook == "cpu" else
+                torch.autograd.graph.saved_tensors_hooks(HOOKS[hook], lambda x: x))
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
