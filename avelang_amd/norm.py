@@ -102,29 +102,29 @@ def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Te
     """
     name = "layer_norm_bwd"
     x, weight, _, rows, heads, D, dt, wdt = _args(x, weight, None, name)
+    return _bwd(x, weight, dy, stats, rows, heads, D, dt, wdt if weight is not None else 0,
+                torch.empty_like(weight) if weight is not None else None,
+                None if not has_bias else torch.empty_like(weight) if weight is not None
+                else torch.empty(D, dtype=torch.float32, device=x.device), name)
+
+
+def _bwd(x, weight, dy, stats, rows, heads, D, dt, wdt, dw, db, name):
     dev = x.device
     if not isinstance(dy, torch.Tensor) or dy.shape != x.shape or dy.dtype != x.dtype or dy.device != dev:
         raise ValueError(f"{name}: dy must be a {x.dtype} tensor of shape {tuple(x.shape)} on {dev}.")
     if (not isinstance(stats, torch.Tensor) or tuple(stats.shape) != (rows, 2) or stats.device != dev
-            or stats.dtype != torch.float32 or not stats.is_contiguous()):
-        raise ValueError(f"{name}: stats must be contiguous torch.float32 of shape {(rows, 2)} on {dev}.")
-    return _bwd(x, weight, dy, stats, rows, heads, D, dt, wdt if weight is not None else 0,
-                torch.empty_like(weight) if weight is not None else None,
-                None if not has_bias else torch.empty_like(weight) if weight is not None
-                else torch.empty(D, dtype=torch.float32, device=dev), name)
-
-
-def _bwd(x, weight, dy, stats, rows, heads, D, dt, wdt, dw, db, name):
-    dy = dy.contiguous()
+            or stats.dtype != torch.float32):
+        raise ValueError(f"{name}: stats must be torch.float32 of shape {(rows, 2)} on {dev}.")
+    dy, stats = dy.contiguous(), stats.contiguous()
     dx = torch.empty_like(x)
     lib = _native.lib()
     ws, nbytes = None, 0
     if dw is not None or db is not None:
         nbytes = lib.gdn_layer_norm_bwd_workspace_bytes(rows, heads, D, dt)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _native.check(lib.gdn_layer_norm_bwd(
         x.data_ptr(), _ptr(weight), dy.data_ptr(), stats.data_ptr(), dx.data_ptr(), _ptr(dw),
-        _ptr(db), rows, heads, D, dt, wdt, _ptr(ws), nbytes, _stream(x.device)), name)
+        _ptr(db), rows, heads, D, dt, wdt, _ptr(ws), nbytes, _stream(dev)), name)
     return dx, dw, db
 
 
@@ -134,17 +134,18 @@ class _LayerNorm(torch.autograd.Function):
         args = _args(x, weight, bias, "layer_norm")
         y, stats = _fwd(args, eps, "layer_norm", save=True)
         ctx.save_for_backward(args[0], args[1], args[2], stats)
-        ctx.sizes = args[3:]
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         x, weight, bias, stats = ctx.saved_tensors
+        # (checked again: a hook on saved tensors may return others of another layout)
+        x, weight, bias, *sizes = _args(x, weight, bias, "layer_norm")
         _, want_w, want_b, _ = ctx.needs_input_grad
         dw = torch.empty_like(weight) if want_w and weight is not None else None
         db = torch.empty_like(bias) if want_b and bias is not None else None
-        dx, dw, db = _bwd(x, weight, dy, stats, *ctx.sizes, dw, db, "layer_norm")
+        dx, dw, db = _bwd(x, weight, dy, stats, *sizes, dw, db, "layer_norm")
         return dx, dw, db, None
 
 

@@ -3,10 +3,13 @@ come back from hooks (offloading to the host, say) in another layout than they w
 
 Tolerances: none, the same bits with a hook as without.
 """
+import ctypes
+
 import pytest
 import torch
 
 from avelang_amd import linear_attention as L
+from avelang_amd import norm as N
 
 BF = torch.bfloat16
 
@@ -92,3 +95,55 @@ def test_gradients_through_hooks(rocm_device, hook, save, packed):
     got = grads(torch.autograd.graph.save_on_cpu() if hook == "cpu" else
                 torch.autograd.graph.saved_tensors_hooks(HOOKS[hook], lambda x: x))
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+@pytest.mark.parametrize("hook", ["contiguous", "strided"])
+def test_layout_of_what_comes_back_to_the_norm(monkeypatch, hook):
+    """The kernels are given rows that follow one another, whatever a hook returns."""
+    def args(x, weight, bias, name):   # the checks of devices left out
+        return x.contiguous(), weight.contiguous(), bias.contiguous(), 15, 3, 8, 1, 0
+
+    class Lib:
+        def gdn_layer_norm_fwd(self, *a):
+            return 0
+
+        def gdn_layer_norm_bwd_workspace_bytes(self, *a):
+            return 8
+
+        def gdn_layer_norm_bwd(self, x, w, dy, stats, *a):
+            self.seen = [torch.frombuffer((ctypes.c_float * n).from_address(p), dtype=torch.float32).clone()
+                         for p, n in ((x, 120), (w, 24), (dy, 120), (stats, 30))]
+            return 0
+    lib = Lib()
+    monkeypatch.setattr(N, "_args", args)
+    monkeypatch.setattr(N, "_stream", lambda dev: 0)
+    monkeypatch.setattr(N._native, "lib", lambda: lib)
+    gen = torch.Generator().manual_seed(1)
+    x, w, b, dy = (torch.randn(s, generator=gen) for s in ((5, 3, 8), (3, 8), (3, 8), (5, 3, 8)))
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: (kept.append(t), HOOKS[hook](t))[1], lambda t: t):
+        y = N.layer_norm(x.requires_grad_(), w.requires_grad_(), b.requires_grad_())
+    y.backward(_strided(dy))
+    assert len(kept) == 4
+    for got, want in zip(lib.seen, (x, w, dy, kept[3])):
+        assert torch.equal(got.nan_to_num(), want.detach().reshape(-1).nan_to_num())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hook", sorted(HOOKS) + ["cpu"])
+@pytest.mark.parametrize("heads", [0, 3])
+def test_norm_gradients_through_hooks(rocm_device, hook, heads):
+    import avelang_amd as ave
+    par = (heads, 40) if heads else (40,)
+    gen = torch.Generator().manual_seed(2)
+    x, w, b, dy = (torch.randn(s, generator=gen).to(rocm_device) for s in ((50,) + par, par, par, (50,) + par))
+
+    def grads(around):
+        leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+        with around:
+            y = ave.layer_norm(*leaves)
+        return torch.autograd.grad(y, leaves, dy)
+    want = grads(torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t))
+    got = grads(torch.autograd.graph.save_on_cpu() if hook == "cpu" else
+                torch.autograd.graph.saved_tensors_hooks(HOOKS[hook], lambda t: t))
+    assert all(torch.equal(g, r) for g, r in zip(got, want))
