@@ -276,6 +276,8 @@ struct LinPlan {
 // Whether the backward takes two v-heads of a qk-head at a time.
 inline bool lin_pair(int Hqk, int Hv) { return Hv / Hqk % 2 == 0; }
 LinPlan lin_plan(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu, bool bwd);
+// The workspace that the caller is asked for.
+size_t lin_bytes(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu, bool bwd);
 LinGrid lin_grid(const LinPlan& p, unsigned char* ws, int T, int N, int total, bool has_cu);
 void launch_lin_table(const int32_t* cu, const LinPlan& p, unsigned char* ws, int N, int total,
                       hipStream_t st);

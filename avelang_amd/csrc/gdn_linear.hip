@@ -655,15 +655,17 @@ inline bool lin_alone(const LinGrid& g, int Hv) {
 // and one or two v-heads.  (Training steps in us: 16 -> 16 heads of 128, 4096
 // tokens 119, with twice the segments 132; 16 -> 32 of 64, 8192 tokens 153, with
 // half 180; 16 -> 32 of 128, 8192 tokens 333, with half 467.)
+long long lin_slots(int Hqk, int Hv, int K, int V, bool bwd, bool one) {
+  if (bwd) return (long long)device_cus() * (K + V == 128 ? 2 : 1) * (lin_pair(Hqk, Hv) ? 2 : 1);
+  return (long long)device_cus() * (one ? 1 : 2);
+}
 LinPlan lin_plan(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu, bool bwd) {
   LinPlan p{};
   const long long tokens = (long long)B * T;
   const long long per = ((long long)T + kChunk - 1) / kChunk;   // chunks of the longest sequence
   p.chunks = has_cu ? tokens / kChunk + N : B * per;
-  const long long cus = device_cus();
-  p.one = !bwd && p.chunks * Hv < (V == 64 ? 4 : K == 64 ? 8 : 12) * cus;
-  const long long slots = cus * (bwd ? (K + V == 128 ? 2 : 1) * (lin_pair(Hqk, Hv) ? 2 : 1)
-                                     : p.one ? 1 : 2);
+  p.one = !bwd && p.chunks * Hv < (V == 64 ? 4 : K == 64 ? 8 : 12) * (long long)device_cus();
+  const long long slots = lin_slots(Hqk, Hv, K, V, bwd, p.one);
   long long L = (p.chunks * Hv + slots - 1) / slots;
   if (L < 1) L = 1;
   if (L > per) L = per > 0 ? per : 1;
@@ -693,6 +695,40 @@ LinPlan lin_plan(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu
   if (bwd) p.dgtok = take((size_t)tokens * Hv * 4);
   p.total = at;
   return p;
+}
+
+// Bytes that hold this call and every other of these heads whose B, T and N are
+// no larger.  (lin_plan's own need is not monotone: 16 -> 32 heads of 128, 512
+// tokens are 8 segments, 576 tokens 5.)  Of n sequences that are cut there are
+// at most c = slots / Hv segments more than n less one (packed: c more than n),
+// and none is cut where n * Hv reaches the slots (packed: where (chunks + n) *
+// Hv / slots reaches the chunks).
+size_t lin_bytes(int B, int T, int Hqk, int Hv, int K, int V, int N, bool has_cu, bool bwd) {
+  const long long tokens = (long long)B * T, full = T / kChunk;
+  const long long per = ((long long)T + kChunk - 1) / kChunk;
+  const long long slots = lin_slots(Hqk, Hv, K, V, bwd, false), c = (slots + Hv - 1) / Hv;
+  long long rows = 0;   // segments whose states are kept
+  size_t at = 0;
+  auto take = [&](long long bytes) { at += (size_t)(bytes + 255) / 256 * 256; };
+  if (has_cu) {
+    const long long more = full < c ? full : c;
+    take((N + more) * (long long)sizeof(LinSeg));
+    take(4);
+    take((N + more) * 4LL);
+    take(more * (long long)sizeof(LinJoin));
+    const long long most = slots > Hv ? (per - 1) * (slots - Hv) / Hv : 0;
+    const long long n = N < most ? N : most;
+    rows = n > 0 ? n + more : 0;
+  } else if (per > 1) {
+    const long long n = N < (slots - 1) / Hv ? N : (slots - 1) / Hv;
+    rows = n > 0 ? (n * per < c + n - 1 ? n * per : c + n - 1) : 0;
+  }
+  take(rows * Hv * K * V * 4);
+  take(rows * Hv * 4);
+  const int parts = Hv / Hqk / (lin_pair(Hqk, Hv) ? 2 : 1);
+  if (bwd && parts > 1) take(tokens * Hqk * parts * K * 8);
+  if (bwd) take(tokens * Hv * 4);
+  return at;
 }
 
 LinGrid lin_grid(const LinPlan& p, unsigned char* ws, int T, int N, int total, bool has_cu) {
@@ -849,7 +885,7 @@ bool lin_sizes_ok(int B, int T, int Hqk, int Hv, int K, int V, int N) {
 extern "C" size_t gdn_linear_chunk_workspace_bytes(int B, int T, int Hqk, int Hv, int K, int V,
                                                    int N, int has_cu_seqlens) {
   if (!gdn_host::lin_sizes_ok(B, T, Hqk, Hv, K, V, N)) return 0;
-  return gdn::lin_plan(B, T, Hqk, Hv, K, V, N, has_cu_seqlens != 0, false).total;
+  return gdn::lin_bytes(B, T, Hqk, Hv, K, V, N, has_cu_seqlens != 0, false);
 }
 
 extern "C" size_t gdn_linear_states_bytes(int B, int T, int Hv, int K, int V, int N,

@@ -571,7 +571,7 @@ int lin_aligned(const char* name, std::initializer_list<const void*> ptrs);
 extern "C" size_t gdn_linear_chunk_bwd_workspace_bytes(int B, int T, int Hqk, int Hv, int K, int V,
                                                        int N, int has_cu_seqlens) {
   if (!gdn_host::lin_sizes_ok(B, T, Hqk, Hv, K, V, N)) return 0;
-  return gdn::lin_plan(B, T, Hqk, Hv, K, V, N, has_cu_seqlens != 0, true).total;
+  return gdn::lin_bytes(B, T, Hqk, Hv, K, V, N, has_cu_seqlens != 0, true);
 }
 
 extern "C" int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v, long long q_row,

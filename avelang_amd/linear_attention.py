@@ -112,7 +112,8 @@ def _state(t, shape, dev, what, name):
 
 def linear_attn_workspace_bytes(B: int, T: int, Hqk: int, Hv: int, K: int, V: int, N: int,
                                 has_cu_seqlens: bool, backward: bool = False) -> int:
-    """Device scratch bytes ``chunk_linear_attn`` (or its backward) needs."""
+    """Device scratch bytes ``chunk_linear_attn`` (or its backward) needs for these sizes, or
+    for others of the same heads with B, T and N no larger."""
     lib = _native.lib()
     f = (lib.gdn_linear_chunk_bwd_workspace_bytes if backward
          else lib.gdn_linear_chunk_workspace_bytes)
@@ -290,10 +291,11 @@ def chunk_linear_attn(
     ``scale`` defaults to ``K ** -0.5``.  ``cu_seqlens`` (int32 / int64 [N + 1],
     B = 1) packs N sequences; on the CPU a violation of its contract raises,
     on the device it empties every sequence.  ``workspace`` (uint8, of
-    ``linear_attn_workspace_bytes(...)``), ``out`` and ``final_state`` (which
-    may be ``initial_state`` itself) avoid allocation.  Infinities and NaN in
-    a token's inputs reach its own and later outputs only (padding behind a
-    batch's rows may hold anything); in the gradients they may reach others.
+    ``linear_attn_workspace_bytes(...)`` for this problem or any larger one),
+    ``out`` and ``final_state`` (which may be ``initial_state`` itself) avoid
+    allocation.  Infinities and NaN in a token's inputs reach its own and later
+    outputs only (padding behind a batch's rows may hold anything); in the
+    gradients they may reach others.
 
     Differentiable in q, k, v, g and initial_state (``chunk_linear_attn_bwd``).
     The forward then keeps the state at every chunk's start for the backward

@@ -35,7 +35,8 @@ extern "C" {
 
 /*
  * Chunked form (prompts, training).  workspace: gdn_linear_chunk_workspace_bytes
- * bytes.  states (nullable): gdn_linear_states_bytes bytes that receive what
+ * bytes, for these sizes or for others of the same heads with B, T and N no
+ * smaller.  states (nullable): gdn_linear_states_bytes bytes that receive what
  * gdn_linear_chunk_bwd reads of this forward (the state at every chunk's
  * start, bf16); o may then be NULL (states only).
  */
@@ -54,7 +55,7 @@ int gdn_linear_chunk_fwd(const void* q, const void* k, const void* v,
  * bf16 contiguous (q's, k's, v's shapes), dg (g's shape and type), dh0 (nullable).
  * With g_per_head dg is the sum over all tokens, in fp32 and in a fixed order.
  * states: what gdn_linear_chunk_fwd left for these same inputs.
- * Deterministic; workspace: gdn_linear_chunk_bwd_workspace_bytes bytes.
+ * Deterministic; workspace: gdn_linear_chunk_bwd_workspace_bytes bytes, likewise.
  */
 size_t gdn_linear_chunk_bwd_workspace_bytes(int B, int T, int Hqk, int Hv, int K, int V, int N,
                                             int has_cu_seqlens);
