@@ -93,6 +93,16 @@ def _in_place(q, k, v, out=None):
     return q, k, v, rows
 
 
+def _cu_on_device(c32: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """A checked int32 cu_seqlens of the CPU on ``dev``.  The copy of a pinned one is
+    still to come when the call returns: it is made from a copy of its own, so that
+    the caller may refill the buffer at once.  (Under capture from the caller's:
+    each replay reads what is there.)"""
+    if c32.is_pinned() and not torch.cuda.is_current_stream_capturing():
+        c32 = torch.empty_like(c32, pin_memory=True).copy_(c32)
+    return c32.to(device=dev, non_blocking=True)
+
+
 def _check_inputs(q, k, v, g, beta, initial_state, cu_seqlens, name, convert_gates=True,
                   contiguous=True):
     for nm, t in (("q", q), ("k", k), ("v", v)):
@@ -143,9 +153,11 @@ def _check_inputs(q, k, v, g, beta, initial_state, cu_seqlens, name, convert_gat
             lib = _native.lib()
             if lib.gdn_cu_seqlens_check(c32.data_ptr(), N, T) != 0:
                 raise ValueError(f"{name}: {lib.gdn_last_error().decode()} (T={T}).")
+            cu = _cu_on_device(c32, dev)
         elif cu_seqlens.device != dev:
             raise ValueError(f"{name}: cu_seqlens must be on {dev} or the CPU.")
-        cu = cu_seqlens.to(device=dev, dtype=torch.int32, non_blocking=True).contiguous()
+        else:
+            cu = cu_seqlens.to(dtype=torch.int32).contiguous()
     else:
         N = B
         cu = None

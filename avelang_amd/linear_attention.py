@@ -28,7 +28,8 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .gated_delta_rule import _HEAD_SIZES, _check_distinct_slots, _in_place, _out, _ptr, _stream_ptr
+from .gated_delta_rule import (_HEAD_SIZES, _check_distinct_slots, _cu_on_device, _in_place, _out,
+                               _ptr, _stream_ptr)
 from .layer_ops import _DTYPES
 
 __all__ = [
@@ -97,9 +98,10 @@ def _cu(cu_seqlens, B, T, dev, name):
         lib = _native.lib()
         if lib.gdn_cu_seqlens_check(c32.data_ptr(), N, T) != 0:
             raise ValueError(f"{name}: {lib.gdn_last_error().decode()} (T={T}).")
-    elif cu_seqlens.device != dev:
+        return _cu_on_device(c32, dev), N
+    if cu_seqlens.device != dev:
         raise ValueError(f"{name}: cu_seqlens must be on {dev} or the CPU.")
-    return cu_seqlens.to(device=dev, dtype=torch.int32, non_blocking=True).contiguous(), N
+    return cu_seqlens.to(dtype=torch.int32).contiguous(), N
 
 
 def _state(t, shape, dev, what, name):
