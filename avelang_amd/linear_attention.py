@@ -334,7 +334,8 @@ def fused_recurrent_linear_attn(
     out: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """Token by token (decode): every state is read once, advanced through its
-    sequence's tokens and written once.  Not differentiable.
+    sequence's tokens and written once.  Not differentiable.  ``cu_seqlens`` as in
+    ``chunk_linear_attn``.
 
     With ``output_final_state`` and ``inplace_final_state`` (and an
     ``initial_state``) the final state overwrites ``initial_state`` and that
