@@ -198,11 +198,11 @@ def chunk_linear_attn_bwd(
     forward's states are formed again.  Deterministic.
     """
     name = "chunk_linear_attn_bwd"
-    return _chunk_bwd(_inputs(q, k, v, g, cu_seqlens, name), do, dht, scale, initial_state, states,
-                      workspace, name)
+    return _chunk_bwd(_inputs(q, k, v, g, cu_seqlens, name), do, dht, scale, initial_state,
+                      initial_state is not None, states, workspace, name)
 
 
-def _chunk_bwd(inputs, do, dht, scale, initial_state, states, workspace, name):
+def _chunk_bwd(inputs, do, dht, scale, initial_state, want_dh0, states, workspace, name):
     q, k, v, g, cu, rows, dims = inputs
     B, T, Hqk, Hv, K, V, N = dims
     dev = q.device
@@ -229,7 +229,7 @@ def _chunk_bwd(inputs, do, dht, scale, initial_state, states, workspace, name):
     dv = torch.empty((B, T, Hv, V), **bf)
     dg = torch.empty_like(g)
     dh0 = None
-    if initial_state is not None:
+    if want_dh0:
         dh0 = torch.empty((N, Hv, K, V), dtype=torch.float32, device=dev)
     if workspace is None:
         nbytes = lib.gdn_linear_chunk_bwd_workspace_bytes(*dims, cu is not None)
@@ -252,7 +252,8 @@ class _ChunkLinearAttn(torch.autograd.Function):
         name = "chunk_linear_attn"
         inputs = _inputs(q, k, v, g, cu_seqlens, name)
         o, ht, states = _chunk_fwd(inputs, scale, initial_state, output_final_state, name, save=save)
-        ctx.save_for_backward(*inputs[:5], initial_state, states)
+        # (of a state that the backward has no need to form again only the shape counts)
+        ctx.save_for_backward(*inputs[:5], None if save else initial_state, states)
         ctx.rest = scale, g.dtype
         ctx.set_materialize_grads(False)
         return (o, ht) if output_final_state else o
@@ -267,8 +268,8 @@ class _ChunkLinearAttn(torch.autograd.Function):
         # (token strides and alignment as they are now: a hook on saved tensors, one
         # that offloads them say, returns others of another layout)
         name = "chunk_linear_attn"
-        dq, dk, dv, dg, dh0 = _chunk_bwd(_inputs(q, k, v, g, cu, name), do, dht, scale, h0, states,
-                                         None, name)
+        dq, dk, dv, dg, dh0 = _chunk_bwd(_inputs(q, k, v, g, cu, name), do, dht, scale, h0,
+                                         ctx.needs_input_grad[5], states, None, name)
         return dq, dk, dv, dg if dg.dtype is g_type else dg.to(g_type), None, dh0, None, None, None
 
 

@@ -147,3 +147,50 @@ def test_norm_gradients_through_hooks(rocm_device, hook, heads):
     got = grads(torch.autograd.graph.save_on_cpu() if hook == "cpu" else
                 torch.autograd.graph.saved_tensors_hooks(HOOKS[hook], lambda t: t))
     assert all(torch.equal(g, r) for g, r in zip(got, want))
+
+
+@pytest.mark.parametrize("save", [True, False])
+@pytest.mark.parametrize("wanted", [True, False])
+def test_what_the_backward_asks_for(monkeypatch, save, wanted):
+    """A carried state without a gradient gets none, and is held only to form the states again."""
+    seen = {}
+
+    def fwd(inputs, scale, initial_state, output_final_state, name, save=False):
+        return inputs[2].clone(), None, torch.zeros(8, dtype=torch.uint8) if save else None
+
+    def bwd(inputs, do, dht, scale, initial_state, want_dh0, states, workspace, name):
+        seen.update(h0=initial_state, want=want_dh0, states=states)
+        return *(torch.zeros_like(x) for x in inputs[:4]), state * 0 if want_dh0 else None
+    monkeypatch.setattr(L, "_inputs", lambda q, k, v, g, cu, name, out=None: (q, k, v, g, cu, None, None))
+    monkeypatch.setattr(L, "_chunk_fwd", fwd)
+    monkeypatch.setattr(L, "_chunk_bwd", bwd)
+    args = [x.contiguous().requires_grad_() for x in _slices(1, 5, 2, 4, 64, 64)]
+    state = torch.zeros(1, 4, 64, 64, requires_grad=wanted)
+    o, _ = L.chunk_linear_attn(*args, initial_state=state, save_for_backward=save)
+    if save:
+        with torch.no_grad():
+            state.fill_(1.0)   # the next step's state
+    o.sum().backward()
+    assert seen["want"] == wanted and (seen["h0"] is None) == save and (seen["states"] is None) != save
+    assert (state.grad is not None) == wanted
+
+
+@pytest.mark.gpu
+def test_state_carried_in_place(rocm_device):
+    import avelang_amd as ave
+    gen = torch.Generator().manual_seed(6)
+    h0 = torch.randn((1, 4, 64, 128), generator=gen).to(rocm_device)
+    do = torch.randn((1, 300, 4, 128), generator=gen).to(BF).to(rocm_device)
+
+    def grads(overwrite, wanted):
+        leaves = [x.requires_grad_() for x in _slices(1, 300, 2, 4, 64, 128, rocm_device)]
+        state = h0.clone().requires_grad_(wanted)
+        o, ht = ave.chunk_linear_attn(*leaves, initial_state=state, output_final_state=True)
+        if overwrite:
+            with torch.no_grad():
+                state.copy_(ht)
+        return torch.autograd.grad(o, leaves + [state] * wanted, do)
+    want = grads(False, False)
+    assert all(torch.equal(x, y) for x, y in zip(grads(True, False), want))
+    for x, y in zip(grads(True, True), grads(False, True)):
+        assert torch.equal(x, y)
