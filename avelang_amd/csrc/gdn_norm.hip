@@ -309,14 +309,15 @@ __global__ __launch_bounds__(256) void norm_bwd_kernel(NormBwdArgs a) {
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        x[i][j] = (x[i][j] - mean) * rstd;
+        // (past the row's end 0, and so is dy: the mean of a near-constant row
+        // times rstd may be infinite)
+        x[i][j] = (l + LPR * i) * VEC + j < a.D ? (x[i][j] - mean) * rstd : 0.f;
         dw[i][j] += dy[i][j] * x[i][j];
         db[i][j] += dy[i][j];
         dy[i][j] *= w[i][j];
         s1 += dy[i][j];
         s2 += dy[i][j] * x[i][j];
       }
-    // (a lane past the row's end holds dy = 0: nothing of it enters the sums)
     s1 = row_sum<LPR>(s1, red[ph][0]) * inv_d;
     s2 = row_sum<LPR>(s2, red[ph][1]) * inv_d;
 #pragma unroll
@@ -372,7 +373,7 @@ __global__ __launch_bounds__(256) void norm_bwd_long_kernel(NormBwdArgs a) {
     if (a.w) ld_par<VEC>(a.w, hb, c, a.D, a.wt, w);
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-      x[j] = (x[j] - mean) * rstd;
+      x[j] = c + j < a.D ? (x[j] - mean) * rstd : 0.f;   // (as above)
       if (a.w) dy[j] *= w[j];
     }
   };
