@@ -493,10 +493,16 @@ int check_norm(const char* name, long long rows, int heads, int D, int dtype, in
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": rows must be >= 0, heads and D >= 1");
   if (!gdn::dtype_ok(dtype) || !gdn::dtype_ok(w_dtype))
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": unsupported dtype code");
-  // (a grid of at most 2^31 - 1 workgroups, columns counted in int where a row is walked)
+  // (rows' workgroups and columns of a row are counted in int)
   if (rows >= (1LL << 31) || (long long)heads * D >= (1LL << 31) || D > (1 << 30))
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
   return GDN_OK;
+}
+
+// A launch has under 2^32 lanes in a dimension.
+int check_lanes(const char* name, long long workgroups, int lanes) {
+  if (workgroups * lanes < (1LL << 32)) return GDN_OK;
+  return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large for one launch");
 }
 
 }  // namespace
@@ -513,10 +519,12 @@ extern "C" int gdn_layer_norm_fwd(const void* x, const void* weight, const void*
   if (rc) return rc;
   if (rows == 0) return GDN_OK;
   if (!x || !y) return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": x and y must be non-NULL");
+  const RowForm f = row_form(D, dtype);
+  const int per = f.lpr ? 256 / f.lpr : 1;   // rows per workgroup
+  if (const int fit = check_lanes(name, (rows + per - 1) / per, 256)) return fit;
   gdn_host::launch_begin();
   auto st = static_cast<hipStream_t>(stream);
   const gdn::NormArgs a{x, weight, bias, y, stats, rows, heads, D, eps, w_dtype};
-  const RowForm f = row_form(D, dtype);
 #define GDN_NF(TT, LL, VV)                                                                      \
   if (dtype == TT && f.lpr == LL && f.vpt == VV) {                                              \
     constexpr int GPW = 256 / LL;                                                               \
@@ -558,11 +566,15 @@ extern "C" int gdn_layer_norm_bwd(const void* x, const void* weight, const void*
   const long long C = (long long)heads * D;
   auto st = static_cast<hipStream_t>(stream);
   const bool sums = dweight || dbias;
+  if (sums)
+    if (const int fit = check_lanes(name, (C + 63) / 64, 1024)) return fit;
   BwdPlan p{};
   float* pw = nullptr;
   float* pb = nullptr;
   if (rows > 0) {
     p = bwd_plan(rows, heads, D, dtype);
+    if (!p.f.lpr)
+      if (const int fit = check_lanes(name, rows, 256)) return fit;
     if (sums) {
       const size_t need = (size_t)p.parts * C * 2 * sizeof(float);
       if (!workspace || workspace_bytes < need)

@@ -88,7 +88,9 @@ int gdn_linear_recurrent_fwd(const void* q, const void* k, const void* v,
  *     y = (x - mean) / sqrt(var + eps) * weight + bias
  * with the biased variance, in fp32.  Row r uses row r % heads of weight and
  * bias [heads, D] (w_dtype; each nullable).  stats (nullable, fp32 [rows, 2])
- * receives the mean and 1 / sqrt(var + eps) for gdn_layer_norm_bwd.
+ * receives the mean and 1 / sqrt(var + eps) for gdn_layer_norm_bwd.  Rows times
+ * the lanes of one (16 to 64 for rows of up to 2048 16-bit or 1024 32-bit
+ * elements, else 256) under 2^32.
  */
 int gdn_layer_norm_fwd(const void* x, const void* weight, const void* bias, void* y, float* stats,
                        long long rows, int heads, int D, float eps, int dtype, int w_dtype,
@@ -96,7 +98,8 @@ int gdn_layer_norm_fwd(const void* x, const void* weight, const void* bias, void
 
 /*
  * Its gradients: dx (x's type) and, each nullable, dweight / dbias [heads, D]
- * (w_dtype), summed over the rows in a fixed order.
+ * (w_dtype), summed over the rows in a fixed order; heads * D under 2^28 with
+ * either of these.
  */
 size_t gdn_layer_norm_bwd_workspace_bytes(long long rows, int heads, int D, int dtype);
 int gdn_layer_norm_bwd(const void* x, const void* weight, const void* dy, const float* stats,

@@ -1,0 +1,29 @@
+"""Sizes beyond what a launch can have are refused as such, before anything is enqueued.
+
+Every call here is refused: the addresses belong to nothing.
+"""
+import pytest
+
+from avelang_amd import _native
+
+P = [(i + 1) << 42 for i in range(16)]
+
+
+@pytest.mark.parametrize("rows,D,dt", [(1 << 28, 8, 1), ((1 << 28) - 15, 128, 2), (1 << 28, 64, 0),
+                                       (1 << 27, 256, 1), (1 << 26, 2048, 1), (1 << 24, 4096, 1),
+                                       ((1 << 24) + 1, 20001, 0)])
+def test_norm_rows(rows, D, dt):
+    lib = _native.lib()
+    assert lib.gdn_layer_norm_fwd(P[0], None, None, P[1], None, rows, 1, D, 1e-5, dt, 0, None) == -2
+    assert "too large" in _native.last_error()
+
+
+def test_norm_backward():
+    lib = _native.lib()
+
+    def bwd(rows, heads, D, dw):
+        return lib.gdn_layer_norm_bwd(P[0], None, P[1], P[2], P[3], dw, None, rows, heads, D, 1, 0, P[4],
+                                      1 << 60, None)
+    assert bwd(1 << 24, 1, 20001, None) == -2      # a workgroup per row
+    assert bwd(4, 1 << 20, 256, P[5]) == -2        # a lane per column and slice of the sums
+    assert bwd(0, 1 << 20, 256, P[5]) == -2
