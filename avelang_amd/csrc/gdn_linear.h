@@ -251,8 +251,8 @@ __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(
 // its L2; a segment's qk-heads, and so segments of different lengths, are
 // spread over the XCDs.  Packed segments start longest first.  The grid is
 // lin_items(...) workgroups; false: none for this one.
-inline unsigned lin_items(int nseg, int Hqk, int Hv) {
-  return (unsigned)(((long long)nseg * Hqk + 7) / 8 * 8 * (Hv / Hqk));
+inline long long lin_items(int nseg, int Hqk, int Hv) {
+  return ((long long)nseg * Hqk + 7) / 8 * 8 * (Hv / Hqk);
 }
 __device__ __forceinline__ bool lin_item(const LinGrid& g, int nseg, int Hqk, int Hv, int& s,
                                          int& h) {

@@ -764,7 +764,7 @@ void launch_lin_segments(const uint16_t* x, int x_row, const uint16_t* y, int y_
                          const LinDecay& d, const LinGrid& g, int Hqk, int Hv, float scale,
                          bool reverse, bool full, const float* edge, float* segs, float* decay,
                          float* end, hipStream_t st) {
-  const dim3 items(lin_items(g.table ? g.nseg : g.N * (g.nps - (end ? 0 : 1)), Hqk, Hv));
+  const dim3 items((unsigned)lin_items(g.table ? g.nseg : g.N * (g.nps - (end ? 0 : 1)), Hqk, Hv));
   const long long waves = (long long)g.nlong * Hv * (K * V / 256);   // workgroups of one per lane
   const bool four = waves >= 8LL * device_cus();
   const dim3 elems((unsigned)(four ? waves / 4 : waves));
@@ -818,7 +818,7 @@ void launch_walk(const uint16_t* q, const uint16_t* k, const uint16_t* v, TokenS
                               end ? ht : nullptr, st);
     if (end) ht = nullptr;
   }
-  const dim3 items(lin_items(g.nseg, Hqk, Hv));
+  const dim3 items((unsigned)lin_items(g.nseg, Hqk, Hv));
 #define GDN_LW(CT, NP, OUT, SAVE, ALONE)                                                     \
   hipLaunchKernelGGL((lin_walk_kernel<K, V, CT, NP, OUT, SAVE, ALONE>), items,               \
                      dim3(4 * V / CT), 0, st, q, k, v, ts, d, g, Hqk, Hv, scale, h0, ht, segs, \
@@ -859,7 +859,7 @@ int lin_validate(const char* name, const void* q, const void* k, const void* v, 
   if (rc) return rc;
   if (!gdn::dtype_ok(g_dtype)) return fail(GDN_ERR_SHAPE, std::string(name) + ": unsupported dtype code");
   // (tokens, segments x heads and join workgroups are counted in 32 bits, and so
-  // are the bytes of a chunk's rows)
+  // are the bytes of a chunk's rows; the lanes of a launch: lin_lanes)
   const long long tokens = (long long)B * T;
   if (tokens >= (1LL << 31) - 64 || (tokens / 64 + N) * (long long)Hv >= (1LL << 24) * 64 ||
       (long long)N * Hv * (K * V / 256) >= (1LL << 31) || Hv >= (1 << 15))
@@ -875,6 +875,11 @@ int lin_aligned(const char* name, std::initializer_list<const void*> ptrs) {
     if (reinterpret_cast<uintptr_t>(p) % 16)
       return fail(GDN_ERR_SHAPE, std::string(name) + ": tensors must be 16-byte aligned");
   return GDN_OK;
+}
+// A launch has under 2^32 lanes in a dimension.
+int lin_lanes(const char* name, long long lanes) {
+  if (lanes < (1LL << 32)) return GDN_OK;
+  return fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large for one launch");
 }
 bool lin_sizes_ok(int B, int T, int Hqk, int Hv, int K, int V, int N) {
   return B >= 0 && T >= 0 && Hqk > 0 && Hv > 0 && Hv % Hqk == 0 && N >= 0 &&
@@ -910,6 +915,8 @@ extern "C" int gdn_linear_chunk_fwd(const void* q, const void* k, const void* v,
   if (rc) return rc;
   const bool has_cu = cu_seqlens != nullptr;
   const gdn::LinPlan p = gdn::lin_plan(B, T, Hqk, Hv, K, V, N, has_cu, false);
+  rc = gdn_host::lin_lanes(name, gdn::lin_items(p.nseg, Hqk, Hv) * (p.nlong > 0 || p.one ? 4 * V : 256));
+  if (rc) return rc;
   if (p.total > 0 && (!workspace || workspace_bytes < p.total))
     return gdn_host::fail(GDN_ERR_WORKSPACE, std::string(name) + ": workspace needs " +
                                                  std::to_string(p.total) + " bytes, got " +

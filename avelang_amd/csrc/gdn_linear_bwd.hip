@@ -545,7 +545,7 @@ void launch_grad(const LinBwdArgs& a, float* segs, float* decay, hipStream_t st)
                               true, a.dh0 != nullptr, a.dht, segs, decay, nullptr, st);
 #define GDN_LG(HP, NP)                                                                       \
   hipLaunchKernelGGL((lin_grad_kernel<K, V, HP, NP>),                                        \
-                     dim3(lin_items(a.grid.nseg, a.Hqk, a.Hv / HP)), dim3(2 * (K + V)), 0, st, a)
+                     dim3((unsigned)lin_items(a.grid.nseg, a.Hqk, a.Hv / HP)), dim3(2 * (K + V)), 0, st, a)
   if (lin_pair(a.Hqk, a.Hv)) {
     if (a.dh0) GDN_LG(2, 3);
     else GDN_LG(2, 2);
@@ -565,6 +565,7 @@ int lin_validate(const char* name, const void* q, const void* k, const void* v, 
                  const float* ht, const void* o, const int32_t* cu, int B, int T, int Hqk, int Hv,
                  int K, int V, int N, gdn::TokenStride& ts);
 bool lin_sizes_ok(int B, int T, int Hqk, int Hv, int K, int V, int N);
+int lin_lanes(const char* name, long long lanes);
 int lin_aligned(const char* name, std::initializer_list<const void*> ptrs);
 }  // namespace gdn_host
 
@@ -592,6 +593,11 @@ extern "C" int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v,
     return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": dO, states, dq, dk and dg must be non-NULL");
   const bool has_cu = cu_seqlens != nullptr;
   const gdn::LinPlan p = gdn::lin_plan(B, T, Hqk, Hv, K, V, N, has_cu, true);
+  const int hp = gdn::lin_pair(Hqk, Hv) ? 2 : 1;
+  rc = gdn_host::lin_lanes(name, gdn::lin_items(p.nseg, Hqk, Hv / hp) * 2 * (K + V));
+  if (!rc && p.nlong > 0) rc = gdn_host::lin_lanes(name, gdn::lin_items(p.nseg, Hqk, Hv) * 4 * V);
+  if (!rc && Hv / Hqk / hp > 1) rc = gdn_host::lin_lanes(name, tokens * Hqk * K / 8 + 255);
+  if (rc) return rc;
   if (p.total > 0 && (!workspace || workspace_bytes < p.total))
     return gdn_host::fail(GDN_ERR_WORKSPACE, std::string(name) + ": workspace needs " +
                                                  std::to_string(p.total) + " bytes, got " +
@@ -624,7 +630,7 @@ extern "C" int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v,
     a.dv = static_cast<uint16_t*>(dv);
     a.dg = dgt;
     a.dgt = g_per_head ? GDN_DTYPE_F32 : g_dtype;
-    const int parts = Hv / Hqk / (gdn::lin_pair(Hqk, Hv) ? 2 : 1);   // of a qk-head's gradients
+    const int parts = Hv / Hqk / hp;   // of a qk-head's gradients
     if (parts > 1) {
       a.pq = reinterpret_cast<float*>(ws + p.part);
       a.pk = a.pq + tokens * Hqk * parts * K;

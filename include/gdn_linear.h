@@ -15,7 +15,8 @@
  *   q_row, k_row, v_row: elements from one token's rows to the next's (a
  *   token's heads contiguous): a multiple of 8, at least the heads' width and
  *   under 2^23.  o is contiguous.  All tensors but g and cu_seqlens are
- *   16-byte aligned.  Under 2^15 v-heads.
+ *   16-byte aligned.  Under 2^15 v-heads; chunked, segments (a sequence is one
+ *   at least) times v-heads times lanes (4 V, backward 2 (K + V)) under 2^32.
  *   cu_seqlens [N + 1] int32 (B == 1) or NULL (N == B), under gdn.h's
  *   contract; a violation found on the device empties every sequence: o (or
  *   the gradients) is zero and ht is h0.

@@ -27,3 +27,20 @@ def test_norm_backward():
     assert bwd(1 << 24, 1, 20001, None) == -2      # a workgroup per row
     assert bwd(4, 1 << 20, 256, P[5]) == -2        # a lane per column and slice of the sums
     assert bwd(0, 1 << 20, 256, P[5]) == -2
+
+
+@pytest.mark.parametrize("N,Hqk,Hv,K,V", [(1 << 20, 16, 16, 64, 64), (1 << 20, 8, 16, 64, 128),
+                                          (1 << 19, 32, 32, 128, 128)])
+def test_many_sequences(N, Hqk, Hv, K, V):
+    """A workgroup per sequence and v-head (backward: pair of them)."""
+    lib = _native.lib()
+    rows = (Hqk * K, Hqk * K, Hv * V)
+    assert lib.gdn_linear_chunk_fwd(P[0], P[1], P[2], *rows, P[3], 0, 0, None, None, P[5], P[4], 1, N, Hqk,
+                                    Hv, K, V, N, 0.1, None, P[11], 1 << 60, None) == -2
+    assert "too large" in _native.last_error()
+    # (a pair of v-heads per workgroup: twice as many sequences)
+    M = N * (Hv // Hqk)
+    assert lib.gdn_linear_chunk_bwd(P[0], P[1], P[2], *rows, P[3], 0, 0, P[5], None, P[6], P[7], P[8], P[9],
+                                    P[10], None, P[4], 1, M, Hqk, Hv, K, V, M, 0.1, P[11], 1 << 60,
+                                    None) == -2
+    assert "too large" in _native.last_error()
