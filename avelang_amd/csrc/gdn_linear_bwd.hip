@@ -591,6 +591,26 @@ extern "C" int gdn_linear_chunk_bwd(const void* q, const void* k, const void* v,
   const long long tokens = (long long)B * T;
   if ((tokens > 0 && (!dO || !states || !dq || !dk)) || ((tokens > 0 || g_per_head) && !dg))
     return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": dO, states, dq, dk and dg must be non-NULL");
+  // the gradients leave while the inputs (whole rows where they are slices) are read
+  auto span = [&](int row, int width) { return tokens > 0 ? (size_t)((tokens - 1) * row + width) * 2 : 0; };
+  const int es = g_dtype == GDN_DTYPE_F32 ? 4 : 2;
+  const size_t nqk = (size_t)tokens * Hqk * K * 2, nvo = (size_t)tokens * Hv * V * 2;
+  const size_t ng = (size_t)(g_per_head ? 1 : tokens) * Hv * es, nst = (size_t)N * Hv * K * V * 4;
+  const void* in[] = {q, k, v, g, dO, states, cu_seqlens};
+  const size_t nin[] = {span(ts.q, Hqk * K), span(ts.k, Hqk * K), span(ts.v, Hv * V), ng, nvo,
+                        gdn_linear_states_bytes(B, T, Hv, K, V, N, cu_seqlens != nullptr), (N + 1) * 4ull};
+  const void* out[] = {dq, dk, dv, dg, dh0};
+  const size_t nout[] = {nqk, nqk, nvo, ng, nst};
+  auto meet = [](const void* a, size_t na, const void* b, size_t nb) {
+    return a && b && na && nb && gdn_host::overlaps(a, na, b, nb);
+  };
+  for (int i = 0; i < 5; ++i) {
+    bool bad = i < 4 && meet(out[i], nout[i], dht, nst);   // (dh0 may be dht)
+    for (int j = 0; j < 7; ++j) bad |= meet(out[i], nout[i], in[j], nin[j]);
+    for (int j = i + 1; j < 5; ++j) bad |= meet(out[i], nout[i], out[j], nout[j]);
+    if (bad)
+      return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": a gradient overlaps an input or another gradient");
+  }
   const bool has_cu = cu_seqlens != nullptr;
   const gdn::LinPlan p = gdn::lin_plan(B, T, Hqk, Hv, K, V, N, has_cu, true);
   const int hp = gdn::lin_pair(Hqk, Hv) ? 2 : 1;

@@ -1,4 +1,5 @@
-"""Sizes beyond what a launch can have are refused as such, before anything is enqueued.
+"""Sizes beyond what a launch can have, and gradients written over what is still read, are refused
+as such, before anything is enqueued.
 
 Every call here is refused: the addresses belong to nothing.
 """
@@ -44,3 +45,25 @@ def test_many_sequences(N, Hqk, Hv, K, V):
                                     P[10], None, P[4], 1, M, Hqk, Hv, K, V, M, 0.1, P[11], 1 << 60,
                                     None) == -2
     assert "too large" in _native.last_error()
+
+
+NAMES = ("q", "k", "v", "g", "dO", "states", "cu", "dht", "dq", "dk", "dv", "dg", "dh0")
+OUT = NAMES[8:]
+
+
+@pytest.mark.parametrize("out", OUT)
+@pytest.mark.parametrize("other", NAMES)
+@pytest.mark.parametrize("sliced", [False, True])
+def test_gradients_apart(out, other, sliced):
+    if out == other or (out, other) == ("dh0", "dht"):
+        return
+    lib = _native.lib()
+    at = dict(zip(NAMES, P))
+    at[out] = at[other] + 16   # within both, at these sizes
+    if sliced and other in "qkv":   # beyond a contiguous tensor's end, within the slices' rows
+        at[out] = at[other] + 99 * 1024 * 2
+    rows = (1024,) * 3 if sliced else (128, 128, 256)
+    rc = lib.gdn_linear_chunk_bwd(at["q"], at["k"], at["v"], *rows, at["g"], 0, 0, at["dO"], at["dht"],
+                                  at["states"], at["dq"], at["dk"], at["dv"], at["dg"], at["dh0"], at["cu"],
+                                  1, 100, 2, 4, 64, 64, 7, 0.1, P[14], 1 << 60, None)
+    assert rc == -5 and len(_native.last_error()) > 0
