@@ -37,3 +37,29 @@ def test_constant_rows(rocm_device, D, xt):
     if D > 5:   # (shorter rows' terms cancel to eps' share)
         assert (dx[[0, 2]] - want[0][[0, 2]]).norm() <= (half + 2 ** -18) * want[0][[0, 2]].norm()
         assert (dw - want[1]).norm() <= 2 ** -18 * want[1].norm()
+
+
+@pytest.mark.parametrize("rows,D,xt", [(1500, 4096, torch.bfloat16), (1601, 8192, torch.bfloat16),
+                                       (1301, 8000, torch.float32), (1100, 2049, torch.float32),
+                                       (5000, 2048, torch.float16)])
+@pytest.mark.parametrize("heads", [0, 3])
+def test_several_rows_per_workgroup(rocm_device, rows, D, xt, heads):
+    """More rows than the groups that walk them: each takes two and more, the next on its way."""
+    import avelang_amd as ave
+    gen = torch.Generator(device=rocm_device).manual_seed(rows)
+    r = lambda *s: torch.randn(s, generator=gen, device=rocm_device)  # noqa: E731
+    par = (heads, D) if heads else (D,)
+    x = (r(rows, *par) * (0.5 + r(rows, *par[:-1], 1).abs()) + r(rows, *par[:-1], 1)).to(xt)
+    w, b, dy = 1 + 0.2 * r(*par), 0.1 * r(*par), r(rows, *par).to(xt)
+    leaves = [t.double().requires_grad_() for t in (x, w, b)]
+    ref = linear_ref.layer_norm(*leaves)
+    want = torch.autograd.grad(ref, leaves, dy.double())
+    mine = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = ave.layer_norm(*mine)
+    got = torch.autograd.grad(y, mine, dy)
+    half = torch.finfo(xt).eps / 2
+    assert (y.detach().double() - ref.detach()).norm() <= (half + 2 ** -18) * ref.detach().norm()
+    for g, want_g, h in zip(got, want, (half, 0, 0)):
+        assert (g.double() - want_g).norm() <= (h + 2 ** -18) * want_g.norm()
+    again = torch.autograd.grad(ave.layer_norm(*mine), mine, dy)
+    assert all(torch.equal(g, a) for g, a in zip(got, again))
