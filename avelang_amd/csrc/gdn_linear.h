@@ -216,6 +216,37 @@ __device__ __forceinline__ void lin_split(u16x8 y, const float* f, u16x8 (&part)
   }
 }
 
+// A saved state, 16 bits per value: four neighbours of one key's row as fp16
+// with nine bits after the leading one, under a common factor 2^(16 e - 126)
+// whose e is in their lowest bits.  (In bf16, seven bits, its rounding was what
+// was wrong with dg: 2.0e-3 of it where dg's own is 1.7e-3, three times that for
+// a few tokens behind an initial state.)  The largest of the four lies in
+// [2^-1, 2^15), so that one 2^15 times smaller still has bf16's precision.  What
+// is cut off is 2^-10 on average, 0.7 of which the factor makes up for; values of
+// nine bits and less stay what they are, and so do infinities and NaN.
+__device__ __forceinline__ u16x4 lin_pack(f32x4 x) {
+  constexpr uint32_t M = 0x00010001;
+  const float m = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+  const uint32_t e = __float_as_uint(m) & 0x78000000u;
+  x *= __uint_as_float(0x7E800000u - e) * 1.000671f;
+  const uint32_t a = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));
+  const uint32_t b = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x[2], x[3]));
+  const uint32_t u = (e >> 27) | (e >> 12);   // bits 0, 1 of e / 2^27 in 0 and 16, bits 2, 3 in 2 and 18
+  return __builtin_bit_cast(u16x4, u32x2p{(u & M) | (a & ~M), ((u >> 2) & M) | (b & ~M)});
+}
+__device__ __forceinline__ f32x4 lin_unpack(u16x4 p) {
+  constexpr uint32_t M = 0x00010001;
+  const u32x2p d = __builtin_bit_cast(u32x2p, p);
+  uint32_t u = (d[0] & M) | ((d[1] & M) << 2);
+  u |= u >> 15;
+  const float s = __uint_as_float((u << 27) + 0x00800000u);
+  const u16x4 h = __builtin_bit_cast(u16x4, u32x2p{d[0] & ~M, d[1] & ~M});
+  f32x4 x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(h[i])));
+  return x * s;
+}
+
 // The decays of a chunk on their way in, by two waves: wave 0's lane l has its
 // own token, wave 1's the token 64 - l, so that the prefix sums and the sums
 // of what follows a token (63 - l) are the same scan.  Loaded a chunk ahead,

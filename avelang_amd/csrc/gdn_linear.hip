@@ -476,9 +476,19 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
       for (int T = 0; T < CT; ++T) O[tt][T] = zero4();
 #pragma unroll
     for (int b = 0; b < K / 32; ++b) {
-      u16x8 sb[CT];
+      u16x8 sb[CT], sl[CT];   // (sl: what sb leaves, for the saved copy)
 #pragma unroll
-      for (int T = 0; T < CT; ++T) sb[T] = cat8(f2bf4(S[T][2 * b]), f2bf4(S[T][2 * b + 1]));
+      for (int T = 0; T < CT; ++T) {
+        if constexpr (SAVE) {
+          u16x4 h0, h1, l0, l1;
+          split_bf4(S[T][2 * b], h0, l0);
+          split_bf4(S[T][2 * b + 1], h1, l1);
+          sb[T] = cat8(h0, h1);
+          sl[T] = cat8(l0, l1);
+        } else {
+          sb[T] = cat8(f2bf4(S[T][2 * b]), f2bf4(S[T][2 * b + 1]));
+        }
+      }
       if (OUT) {
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt) {
@@ -488,7 +498,7 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
         }
       }
       if (SAVE) {
-        // transposed through a product with a selection matrix (exact): lane
+        // transposed through products with a selection matrix (exact): lane
         // (r16, grp) gets key 16 t + r16, values 16 ct + 4 grp + r, half of its
         // share of the backward's fragment (rows4's order)
         u16x4* dst = states + ((size_t)(sg.chunk0 + c) * Hv + h) * (K / 16) * (V / 32) * 128 +
@@ -500,9 +510,10 @@ __global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
           for (int i = 0; i < 8; ++i)
             sel[i] = grp == r16 >> 2 && i == 4 * e + (r16 & 3) ? 0x3F80 : 0;
           u16x4* at = dst + (2 * b + e) * (V / 32) * 128;
-          const u16x4 x = f2bf4(mfma16(sb[0], sel, zero4()));
+          const u16x4 x = lin_pack(mfma16(sl[0], sel, mfma16(sb[0], sel, zero4())));
           if constexpr (CT == 2)
-            *reinterpret_cast<u16x8*>(at) = cat8(x, f2bf4(mfma16(sb[1], sel, zero4())));
+            *reinterpret_cast<u16x8*>(at) =
+                cat8(x, lin_pack(mfma16(sl[1], sel, mfma16(sb[1], sel, zero4()))));
           else
             *at = x;
         }

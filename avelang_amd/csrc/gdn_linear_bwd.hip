@@ -13,7 +13,8 @@
 //            + sum_{i >= t > j} M_ij,
 // the last as row sums less column sums of the same fp32 numbers, so nothing
 // but their own rounding is lost where it cancels: dg of a head whose memory
-// is short is as good as that of a long one.
+// is short is as good as that of a long one.  The saved states enter dq and dg
+// whole (they are two bf16 parts), D in two parts into dk, dg and <S, D>.
 //
 // Segments as in the forward, walked last chunk to first: a launch for every
 // segment's contribution to D, one that joins them, one for the gradients.
@@ -35,7 +36,7 @@ struct LinBwdArgs {
   const float* dht;
   float* dh0;
   const float* segs;
-  const u16x8* states;
+  const u16x8* states;   // lin_pack's
   uint16_t *dq, *dk, *dv;
   float *pq, *pk;      // [tokens][Hv / HP][K] partial dq, dk (NULL: none needed)
   void* dg;            // [tokens][Hv], of type dgt
@@ -358,24 +359,32 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
           sums[4 * wk + grp][i] = s;
         }
       };
-      float cs = 0.f;
       inter(std::integral_constant<int, 2>{}, X, sK, ks, lds.bsum,
             [&](int T, int b, u16x8 (&out)[2]) {
-              // both parts of D: <S, D> and b are sums of random signs in dg, which
-              // show their rounding in full (dg's error against 64 bits over 28 shapes,
-              // in its own rounding: 90 % within 1.46, at most 1.73; 1.73 and 1.88 with
-              // one part for b; the step at 8192 tokens 3 % more)
-              const u16x8 f = LinTile<K>::cols4(ds, dcb, b, T);
-              const u16x8 l = LinTile<K>::cols4(dl, dcb, b, T);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) cs += (bf2f(f[i]) + bf2f(l[i])) * bf2f(SF[T][b][i]);
-              out[0] = f;
-              out[1] = l;
+              out[0] = LinTile<K>::cols4(ds, dcb, b, T);
+              out[1] = LinTile<K>::cols4(dl, dcb, b, T);
             },
             [&](int tt, int b) { return LinTile<V>::rows4(vs, vr4, tt, b); });
-      inter(std::integral_constant<int, 1>{}, Y, sQ, qs, lds.asum,
-            [&](int T, int b, u16x8 (&out)[1]) { out[0] = SF[T][b]; },
+      // both parts of S and of D: <S, D>, a and b are sums of random signs in dg,
+      // which show every rounding in full.  <S, D> of 16 keys is the trace of a
+      // product of fragments.
+      f32x4 SD = zero4();
+      inter(std::integral_constant<int, 2>{}, Y, sQ, qs, lds.asum,
+            [&](int T, int b, u16x8 (&out)[2]) {
+              u16x4 h0, h1, l0, l1;
+              split_bf4(lin_unpack(u16x4{SF[T][b][0], SF[T][b][1], SF[T][b][2], SF[T][b][3]}), h0, l0);
+              split_bf4(lin_unpack(u16x4{SF[T][b][4], SF[T][b][5], SF[T][b][6], SF[T][b][7]}), h1, l1);
+              out[0] = cat8(h0, h1);
+              out[1] = cat8(l0, l1);
+              const u16x8 f = LinTile<K>::cols4(ds, dcb, b, T);
+              SD = mfma16(f, out[0], SD);
+              SD = mfma16(f, out[1], SD);
+              SD = mfma16(LinTile<K>::cols4(dl, dcb, b, T), out[0], SD);
+            },
             [&](int tt, int b) { return LinTile<V>::rows4(os, vr4, tt, b); });
+      float cs = 0.f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) cs += 4 * grp + r == r16 ? SD[r] : 0.f;
       if (hh + 1 < HP) load_states(c, hh + 1);
       else load_states(c - 1, 0);
       cs = wave_prefix(cs);

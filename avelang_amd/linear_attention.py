@@ -169,8 +169,8 @@ def chunk_linear_attn_fwd_save(
     output_final_state: bool = False,
     cu_seqlens: Optional[torch.Tensor] = None,
 ):
-    """Training forward: ``(o, final_state, states)``, ``states`` (the bf16
-    state at every chunk's start, 2 K V bytes per 64 tokens and v-head) being
+    """Training forward: ``(o, final_state, states)``, ``states`` (the state at
+    every chunk's start in 16 bits, 2 K V bytes per 64 tokens and v-head) being
     what ``chunk_linear_attn_bwd`` takes for these same inputs."""
     name = "chunk_linear_attn_fwd_save"
     return _chunk_fwd(_inputs(q, k, v, g, cu_seqlens, name), scale, initial_state,
@@ -192,8 +192,8 @@ def chunk_linear_attn_bwd(
     workspace: Optional[torch.Tensor] = None,
 ):
     """Gradients of ``chunk_linear_attn``: ``(dq, dk, dv, dg, dh0)``, dq, dk, dv
-    in bf16, dg with g's shape and type, dh0 fp32 (None without
-    ``initial_state``).  ``do`` is dL/do (bf16, v's shape), ``dht`` (nullable)
+    in bf16, dg with g's shape and type (an fp32 dg too holds the saved states'
+    rounding, a few 10^-4 of it), dh0 fp32 (None without ``initial_state``).  ``do`` is dL/do (bf16, v's shape), ``dht`` (nullable)
     dL/d(final state).  Without ``states`` (``chunk_linear_attn_fwd_save``) the
     forward's states are formed again.  Deterministic.
     """

@@ -39,7 +39,8 @@ extern "C" {
  * bytes, for these sizes or for others of the same heads with B, T and N no
  * smaller.  states (nullable): gdn_linear_states_bytes bytes that receive what
  * gdn_linear_chunk_bwd reads of this forward (the state at every chunk's
- * start, bf16); o may then be NULL (states only).
+ * start, 16 bits per value: nine after the leading one); o may then be NULL
+ * (states only).
  */
 size_t gdn_linear_chunk_workspace_bytes(int B, int T, int Hqk, int Hv, int K, int V, int N,
                                         int has_cu_seqlens);
@@ -55,6 +56,8 @@ int gdn_linear_chunk_fwd(const void* q, const void* k, const void* v,
  * Its gradients: dO [B, T, Hv, V] bf16 contiguous, dht nullable; dq, dk, dv
  * bf16 contiguous (q's, k's, v's shapes), dg (g's shape and type), dh0 (nullable).
  * None of them may overlap an input or another (dh0 may be dht).
+ * dg is formed in fp32, of whatever type, but from these states: 2^-9 of its
+ * terms each, a few 10^-4 of it altogether.
  * With g_per_head dg is the sum over all tokens, in fp32 and in a fixed order.
  * states: what gdn_linear_chunk_fwd left for these same inputs.
  * Deterministic; workspace: gdn_linear_chunk_bwd_workspace_bytes bytes, likewise.
