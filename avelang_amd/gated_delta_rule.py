@@ -98,7 +98,7 @@ def _cu_on_device(c32: torch.Tensor, dev: torch.device) -> torch.Tensor:
     still to come when the call returns: it is made from a copy of its own, so that
     the caller may refill the buffer at once.  (Under capture from the caller's:
     each replay reads what is there.)"""
-    if c32.is_pinned() and not torch.cuda.is_current_stream_capturing():
+    if not torch.cuda.is_current_stream_capturing() and c32.is_pinned():
         c32 = torch.empty_like(c32, pin_memory=True).copy_(c32)
     return c32.to(device=dev, non_blocking=True)
 

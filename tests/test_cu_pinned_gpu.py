@@ -39,3 +39,23 @@ def test_refilled_at_once(rocm_device, op, dtype):
     torch.cuda.synchronize()
     for x, y in zip(got, want):
         assert all(torch.equal(a, b) for a, b in zip(x, y))
+
+
+def test_captured(rocm_device):
+    """In a graph every replay reads the buffer as it is then."""
+    import avelang_amd as ave
+    gen = torch.Generator().manual_seed(5)
+    q, k, v = (torch.randn((1, 200, h, 64), generator=gen).to(rocm_device).bfloat16() for h in (2, 2, 4))
+    g = -torch.rand((1, 200, 4), generator=gen).to(rocm_device)
+    offsets = [torch.tensor(c, dtype=torch.int32) for c in ([0, 30, 130, 200], [0, 100, 150, 200])]
+    want = [ave.chunk_linear_attn(q, k, v, g, output_final_state=True, cu_seqlens=c) for c in offsets]
+    staging = torch.empty(4, dtype=torch.int32, pin_memory=True).copy_(offsets[0])
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = ave.chunk_linear_attn(q, k, v, g, output_final_state=True, cu_seqlens=staging)
+    for i in (0, 1, 0, 1):
+        staging.copy_(offsets[i])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(held, want[i]))

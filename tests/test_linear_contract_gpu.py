@@ -38,3 +38,22 @@ def test_violation_empties_every_sequence(rocm_device, case, heads, K, V):
     b = ave.fused_recurrent_linear_attn(q, k, v, g, initial_state=h0, output_final_state=True,
                                         inplace_final_state=False, cu_seqlens=cu.cpu())
     assert all(torch.equal(x, y) for x, y in zip(a, b)) and a[0].any()
+
+
+@pytest.mark.parametrize("B,T,cu", [(2, 0, None), (0, 5, None), (1, 0, [0, 0, 0])])
+@pytest.mark.parametrize("per_head", [False, True])
+def test_no_tokens(rocm_device, B, T, cu, per_head):
+    """Nothing to read: the states stay, and the decays' gradients over no tokens are zero."""
+    import avelang_amd as ave
+    N = B if cu is None else 2
+    z = lambda *s: torch.zeros(s, device=rocm_device, dtype=torch.bfloat16)  # noqa: E731
+    q, k, v = z(B, T, 2, 64), z(B, T, 2, 64), z(B, T, 4, 64)
+    g = -torch.ones(4, device=rocm_device) if per_head else torch.zeros(B, T, 4, device=rocm_device)
+    h0, dht = (torch.randn(N, 4, 64, 64, device=rocm_device) for _ in range(2))
+    c = None if cu is None else torch.tensor(cu, dtype=torch.int32, device=rocm_device)
+    for op, kw in ((ave.chunk_linear_attn, {}), (ave.fused_recurrent_linear_attn, dict(inplace_final_state=False))):
+        o, ht = op(q, k, v, g, initial_state=h0, output_final_state=True, cu_seqlens=c, **kw)
+        assert o.shape == v.shape and torch.equal(ht, h0)
+    dq, dk, dv, dg, dh0 = ave.chunk_linear_attn_bwd(q, k, v, g, v, dht, initial_state=h0, cu_seqlens=c)
+    assert dq.shape == q.shape and dv.shape == v.shape and torch.equal(dh0, dht)
+    assert dg.shape == g.shape and not dg.any()
