@@ -54,11 +54,13 @@ struct LinGradLds {
   char qs[LinTile<K>::BYTES], ks[LinTile<K>::BYTES];
   char vs[LinTile<V>::BYTES], os[LinTile<V>::BYTES];
   char ps[LinTile<64>::BYTES], dps[LinTile<64>::BYTES];
+  char pd[4][512], dpd[4][512];   // what bf16 leaves of their tiles on the diagonal, rows of 16
   char ds[2][2 * V * K];          // D^T in two bf16 parts, rows of K
   float sG[64], sQ[64], sK[64];   // G log2(e), scale e^G, e^R
   // (slots that their writers own and the reader adds up: M's row sums by source
-  // block and lane group, its column sums by token block; a and b by wave and group)
-  float rowM[16][64], colM[4][64], asum[K / 8][64], bsum[K / 8][64];
+  // block and pair of lane groups, its column sums by token block; a and b by wave
+  // and group)
+  float rowM[8][64], colM[4][64], asum[K / 8][64], bsum[K / 8][64];
   float csum[K / 32];
 };
 
@@ -132,7 +134,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
     *reinterpret_cast<u32x4*>(ps + LinTile<64>::off(r, u)) = u32x4{0, 0, 0, 0};
     *reinterpret_cast<u32x4*>(dps + LinTile<64>::off(r, u)) = u32x4{0, 0, 0, 0};
   }
-  for (int i = tid; i < 1024; i += NT) lds.rowM[i / 64][i % 64] = 0.f;
+  for (int i = tid; i < 512; i += NT) lds.rowM[i / 64][i % 64] = 0.f;
   for (int i = tid; i < 256; i += NT) lds.colM[i / 64][i % 64] = 0.f;
   __syncthreads();
 
@@ -203,6 +205,8 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
     const int pw = LinTile<64>::off(r16, grp >> 1) + (grp & 1) * 8;
     const int dcb = LinTile<K>::col4_base(2 * wk, lane);   // key waves: D^T read
     const int dwb = kr4 + 32 * wv * 2 * K;                 // V waves: D^T written
+    const int kc4 = LinTile<K>::col4_base(0, lane), vc4 = LinTile<V>::col4_base(0, lane);
+    const int dtr = (4 * grp + (r16 >> 2)) * 32 + (r16 & 3) * 8;   // pd, dpd transposed
     hide(qf);
     hide(kf);
     hide(vf);
@@ -240,9 +244,13 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
     __syncthreads();
     if (VW ? c < nc - 1 || hh > 0 : c < nc - 1 && hh == 0)
       store_grads(hh > 0 ? c : c + 1, VW ? (hh > 0 ? h - 1 : h0 + HP - 1) : h0);
-    if (hh + 1 < HP) load(c, hh + 1);
-    else load(c - 1, 0);
-
+    // the next iteration's tiles: on their way through the products behind the
+    // next barrier alone, long enough (from the start of the iteration on they
+    // took 48 registers, which two heads' gradients do not leave: scratch)
+    auto load_next = [&]() {
+      if (hh + 1 < HP) load(c, hh + 1);
+      else load(c - 1, 0);
+    };
     const float eC = exp2_(sG[63]);
     if constexpr (VW) {
       // dv's part of D, then D of the chunk before
@@ -286,8 +294,10 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
             for (int T = 0; T < 2; ++T) ST[hh][t][T] = mfma16(f, part[T][p], ST[hh][t][T]);
         }
       }
+      load_next();
     } else {
-      // P and dP, tile by tile, as bf16 rows, and the sums of M
+      // P and dP, tile by tile, as bf16 rows, what these leave of the tiles on the
+      // diagonal, and the sums of M
       for (int m = wk; m < 10; m += NK) {
         const int it = tmat_block_row(m), jt = m - tmat_block(it, 0);
         f32x4 p = zero4(), d = zero4();
@@ -312,9 +322,17 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
           d[r] *= gam;
           rs += M[r];
         }
-        *reinterpret_cast<u16x4*>(ps + (pw ^ (32 * jt)) + it * 2048) = f2bf4(p);
-        *reinterpret_cast<u16x4*>(dps + (pw ^ (32 * jt)) + it * 2048) = f2bf4(d);
-        lds.rowM[4 * jt + grp][i] = rs;
+        u16x4 ph, pl, dh, dl;
+        split_bf4(p, ph, pl);
+        split_bf4(d, dh, dl);
+        *reinterpret_cast<u16x4*>(ps + (pw ^ (32 * jt)) + it * 2048) = ph;
+        *reinterpret_cast<u16x4*>(dps + (pw ^ (32 * jt)) + it * 2048) = dh;
+        if (it == jt) {
+          *reinterpret_cast<u16x4*>(lds.pd[it] + r16 * 32 + grp * 8) = pl;
+          *reinterpret_cast<u16x4*>(lds.dpd[it] + r16 * 32 + grp * 8) = dl;
+        }
+        rs += __shfl_xor(rs, 16);
+        if (grp % 2 == 0) lds.rowM[2 * jt + grp / 2][i] = rs;
 #pragma unroll
         for (int r = 0; r < 4; ++r) M[r] = row16_sum(M[r]);
         if (r16 == 15) *reinterpret_cast<f32x4*>(&lds.colM[it][j]) = M;
@@ -324,20 +342,20 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
         zero(Y);
       }
       // the parts of dk from D and of dq from S: products, then the tokens' factors
-      auto inter = [&](auto parts, f32x4 (&out)[4][2], const float* fac, const char* own, auto sums,
+      auto inter = [&](f32x4 (&out)[4][2], const float* fac, const char* own, auto sums,
                        auto&& op, auto&& rows) {
         f32x4 Z[4][2];
         zero(Z);
 #pragma unroll
         for (int b = 0; b < V / 32; ++b) {
-          u16x8 f[2][parts];
+          u16x8 f[2][2];
 #pragma unroll
           for (int T = 0; T < 2; ++T) op(T, b, f[T]);
 #pragma unroll
           for (int tt = 0; tt < 4; ++tt) {
             const u16x8 x = rows(tt, b);
 #pragma unroll
-            for (int p = 0; p < parts; ++p)
+            for (int p = 0; p < 2; ++p)
 #pragma unroll
               for (int T = 0; T < 2; ++T) Z[tt][T] = mfma16(f[T][p], x, Z[tt][T]);
           }
@@ -359,7 +377,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
           sums[4 * wk + grp][i] = s;
         }
       };
-      inter(std::integral_constant<int, 2>{}, X, sK, ks, lds.bsum,
+      inter(X, sK, ks, lds.bsum,
             [&](int T, int b, u16x8 (&out)[2]) {
               out[0] = LinTile<K>::cols4(ds, dcb, b, T);
               out[1] = LinTile<K>::cols4(dl, dcb, b, T);
@@ -369,7 +387,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
       // which show every rounding in full.  <S, D> of 16 keys is the trace of a
       // product of fragments.
       f32x4 SD = zero4();
-      inter(std::integral_constant<int, 2>{}, Y, sQ, qs, lds.asum,
+      inter(Y, sQ, qs, lds.asum,
             [&](int T, int b, u16x8 (&out)[2]) {
               u16x4 h0, h1, l0, l1;
               split_bf4(lin_unpack(u16x4{SF[T][b][0], SF[T][b][1], SF[T][b][2], SF[T][b][3]}), h0, l0);
@@ -385,6 +403,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
       float cs = 0.f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) cs += 4 * grp + r == r16 ? SD[r] : 0.f;
+      load_next();
       if (hh + 1 < HP) load_states(c, hh + 1);
       else load_states(c - 1, 0);
       cs = wave_prefix(cs);
@@ -395,7 +414,7 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
     if (VW && w == 0) {
       float x = 0.f, y = 0.f, cs = 0.f;
 #pragma unroll
-      for (int u = 0; u < 16; ++u) x += lds.rowM[u][lane];
+      for (int u = 0; u < 8; ++u) x += lds.rowM[u][lane];
 #pragma unroll
       for (int u = 0; u < 4; ++u) x -= lds.colM[u][lane];
 #pragma unroll
@@ -424,6 +443,26 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
 #pragma unroll
         for (int T = 0; T < 2; ++T) X[tt][T] = mfma16(f[T], pf, X[tt][T]);
       }
+      // what bf16 leaves of P's (dP's) diagonal tiles: where a gradient is a few
+      // tokens' sum their rounding is the same for all of its columns and shows in
+      // full
+      auto diagonal = [&](f32x4 (&out)[4][2], auto&& columns, auto&& tile) {
+        const u16x4 none = {0, 0, 0, 0};
+        const u16x8 x0 = columns(0), x1 = columns(1);
+#pragma unroll
+        for (int t = 2 * kb; t < 2 * kb + 2; ++t) {
+          const u16x4 lo = tile(t);
+          const u16x8 y = t % 2 ? cat8(none, lo) : cat8(lo, none);
+          out[t][0] = mfma16(x0, y, out[t][0]);
+          out[t][1] = mfma16(x1, y, out[t][1]);
+        }
+      };
+      diagonal(X, [&](int T) { return VW ? LinTile<V>::cols4(os, vc4, kb, 2 * wv + T)
+                                         : LinTile<K>::cols4(qs, kc4, kb, 2 * wk + T); },
+               [&](int t) { return lds_tr16(reinterpret_cast<const uint16_t*>((VW ? lds.pd : lds.dpd)[t] + dtr)); });
+      if constexpr (!VW)
+        diagonal(Y, [&](int T) { return LinTile<K>::cols4(ks, kc4, kb, 2 * wk + T); },
+                 [&](int t) { return *reinterpret_cast<const u16x4*>(lds.dpd[t] + r16 * 32 + grp * 8); });
       if constexpr (!VW) {
 #pragma unroll
         for (int T = 0; T < 2; ++T) f[T] = LinTile<K>::cols(ks, kcb, kb, 2 * wk + T);

@@ -91,3 +91,17 @@ def test_states_that_are_not_finite(rocm_device, bad):
         at = torch.tensor(keep, device=rocm_device)
         assert torch.equal(x.index_select(d, at), y.index_select(d, at))
     assert not got[0][0, :, 1].isfinite().all() and not got[3][0, :, 1].isfinite().all()
+
+
+@pytest.mark.parametrize("T", [1, 2, 4, 9, 16])
+@pytest.mark.parametrize("heads", [(16, 32), (16, 16), (4, 12)])
+@pytest.mark.parametrize("K,V", [(128, 128), (64, 64), (128, 64), (64, 128)])
+def test_few_tokens(rocm_device, T, heads, K, V):
+    """Gradients that are sums of a few terms show their own rounding alone: P and dP enter in two
+    parts within a tile of 16 tokens (2^-16 of them left, 2^-12 allowed)."""
+    import avelang_amd as ave
+    t = make(rocm_device, 2, T, *heads, K, V, seed=T)
+    want = linear_ref.linear_attn_chunked(t["q"], t["k"], t["v"], t["g"], t["do"])
+    got = ave.chunk_linear_attn_bwd(t["q"], t["k"], t["v"], t["g"], t["do"])
+    for x, ref in zip(got[:3], want[2:5]):
+        assert far(x, ref) <= (far(ref.to(BF), ref) ** 2 + 2.0 ** -24) ** 0.5
