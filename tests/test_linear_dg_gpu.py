@@ -96,12 +96,15 @@ def test_states_that_are_not_finite(rocm_device, bad):
 @pytest.mark.parametrize("T", [1, 2, 4, 9, 16])
 @pytest.mark.parametrize("heads", [(16, 32), (16, 16), (4, 12)])
 @pytest.mark.parametrize("K,V", [(128, 128), (64, 64), (128, 64), (64, 128)])
-def test_few_tokens(rocm_device, T, heads, K, V):
+@pytest.mark.parametrize("end", [False, True])
+def test_few_tokens(rocm_device, T, heads, K, V, end):
     """Gradients that are sums of a few terms show their own rounding alone: P and dP enter in two
-    parts within a tile of 16 tokens (2^-16 of them left, 2^-12 allowed)."""
+    parts within a tile of 16 tokens, and so does the final state's gradient (2^-16 of them left,
+    2^-12 allowed)."""
     import avelang_amd as ave
     t = make(rocm_device, 2, T, *heads, K, V, seed=T)
-    want = linear_ref.linear_attn_chunked(t["q"], t["k"], t["v"], t["g"], t["do"])
-    got = ave.chunk_linear_attn_bwd(t["q"], t["k"], t["v"], t["g"], t["do"])
+    dht = t["dht"] if end else None
+    want = linear_ref.linear_attn_chunked(t["q"], t["k"], t["v"], t["g"], t["do"], dht)
+    got = ave.chunk_linear_attn_bwd(t["q"], t["k"], t["v"], t["g"], t["do"], dht)
     for x, ref in zip(got[:3], want[2:5]):
         assert far(x, ref) <= (far(ref.to(BF), ref) ** 2 + 2.0 ** -24) ** 0.5
