@@ -322,8 +322,10 @@ __global__ __launch_bounds__(256) void lin_join_kernel(LinGrid grid, int Hv, int
 //
 // ALONE: no launch has formed the segments' start states; each segment first
 // steps the state through the chunks before it.
+// (Two waves per SIMD is what LDS, or V / 16 waves of 128 registers and more,
+// leave all forms but the smallest.)
 template <int K, int V, int CT, int NP, bool OUT, bool SAVE, bool ALONE>
-__global__ __launch_bounds__(4 * V / CT, CT == 1 ? 3 : 2) void lin_walk_kernel(
+__global__ __launch_bounds__(4 * V / CT, CT == 1 && K + V == 128 ? 3 : 2) void lin_walk_kernel(
     const uint16_t* __restrict__ q, const uint16_t* __restrict__ k,
     const uint16_t* __restrict__ v, TokenStride ts, LinDecay dec, LinGrid grid, int Hqk, int Hv,
     float scale, const float* h0, float* ht, const float* __restrict__ segs,
