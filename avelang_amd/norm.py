@@ -102,29 +102,34 @@ def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Te
     """
     name = "layer_norm_bwd"
     x, weight, _, rows, heads, D, dt, wdt = _args(x, weight, None, name)
-    return _bwd(x, weight, dy, stats, rows, heads, D, dt, wdt if weight is not None else 0,
-                torch.empty_like(weight) if weight is not None else None,
-                None if not has_bias else torch.empty_like(weight) if weight is not None
-                else torch.empty(D, dtype=torch.float32, device=x.device), name)
-
-
-def _bwd(x, weight, dy, stats, rows, heads, D, dt, wdt, dw, db, name):
     dev = x.device
     if not isinstance(dy, torch.Tensor) or dy.shape != x.shape or dy.dtype != x.dtype or dy.device != dev:
         raise ValueError(f"{name}: dy must be a {x.dtype} tensor of shape {tuple(x.shape)} on {dev}.")
-    if (not isinstance(stats, torch.Tensor) or tuple(stats.shape) != (rows, 2) or stats.device != dev
-            or stats.dtype != torch.float32):
+    stats = _stats(stats, rows, dev, name)
+    return _bwd(x, weight, dy, stats, rows, heads, D, dt, wdt if weight is not None else 0,
+                torch.empty_like(weight) if weight is not None else None,
+                None if not has_bias else torch.empty_like(weight) if weight is not None
+                else torch.empty(D, dtype=torch.float32, device=dev), name)
+
+
+def _stats(stats, rows, dev, name):
+    if (not isinstance(stats, torch.Tensor) or stats.shape != (rows, 2) or stats.device != dev
+            or stats.dtype is not torch.float32):
         raise ValueError(f"{name}: stats must be torch.float32 of shape {(rows, 2)} on {dev}.")
-    dy, stats = dy.contiguous(), stats.contiguous()
+    return stats.contiguous()
+
+
+def _bwd(x, weight, dy, stats, rows, heads, D, dt, wdt, dw, db, name):
+    dy = dy.contiguous()
     dx = torch.empty_like(x)
     lib = _native.lib()
     ws, nbytes = None, 0
     if dw is not None or db is not None:
         nbytes = lib.gdn_layer_norm_bwd_workspace_bytes(rows, heads, D, dt)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     _native.check(lib.gdn_layer_norm_bwd(
         x.data_ptr(), _ptr(weight), dy.data_ptr(), stats.data_ptr(), dx.data_ptr(), _ptr(dw),
-        _ptr(db), rows, heads, D, dt, wdt, _ptr(ws), nbytes, _stream(dev)), name)
+        _ptr(db), rows, heads, D, dt, wdt, _ptr(ws), nbytes, _stream(x.device)), name)
     return dx, dw, db
 
 
@@ -140,12 +145,17 @@ class _LayerNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         x, weight, bias, stats = ctx.saved_tensors
-        # (checked again: a hook on saved tensors may return others of another layout)
-        x, weight, bias, *sizes = _args(x, weight, bias, "layer_norm")
+        # (checked again: a hook on saved tensors may return others of another layout;
+        # dy is as autograd checked it, like the output)
+        name = "layer_norm"
+        x, weight, bias, *sizes = _args(x, weight, bias, name)
+        stats = _stats(stats, sizes[0], x.device, name)
+        if x.shape != dy.shape or x.dtype is not dy.dtype:
+            raise ValueError(f"{name}: x must be saved as it was.")
         _, want_w, want_b, _ = ctx.needs_input_grad
         dw = torch.empty_like(weight) if want_w and weight is not None else None
         db = torch.empty_like(bias) if want_b and bias is not None else None
-        dx, dw, db = _bwd(x, weight, dy, stats, *sizes, dw, db, "layer_norm")
+        dx, dw, db = _bwd(x, weight, dy, stats, *sizes, dw, db, name)
         return dx, dw, db, None
 
 
