@@ -515,11 +515,12 @@ __device__ __forceinline__ void lin_grad_walk(const LinBwdArgs& a, const LinSeg&
 // dh0) and leave it in LDS, in two bf16 parts, for the K / 32 waves that own 32 key columns
 // (dk, dq, P, dP and with the saved states' fragments <S, D>, all of which
 // reduce over V).  NP: the parts of dO's products on the way to dh0 (three
-// where it is wanted).  8192 tokens, 16 -> 32 heads: 175 us, 403 MB read and
-// written at least, 163 with one part of D in dk (one head at a time, then, with fp32 parts of dq and dk summed by
-// a launch of their own, 226 + 59); bound by registers and LDS (157 KiB: one
-// workgroup of two waves per SIMD), whose latencies three barriers per head and
-// chunk expose.
+// where it is wanted).  8192 tokens, 16 -> 32 heads: 188 us (178 at the highest
+// clock) for 403 MB read and written at least (one head at a time, with fp32 parts of
+// dq and dk summed by a launch of their own, 226 + 59 where two at a time took 175).
+// Bound by latencies: registers (up to 256, none in scratch) and LDS (160 KiB)
+// leave one workgroup, two waves per SIMD, whose waves wait half of their time,
+// at three barriers per head and chunk and for LDS; MFMA is busy a quarter of it.
 template <int K, int V, int HP, int NP>
 __global__ __launch_bounds__(2 * (K + V), 2) void lin_grad_kernel(LinBwdArgs a) {
   constexpr int NT = 2 * (K + V);
