@@ -56,8 +56,9 @@ int gdn_linear_chunk_fwd(const void* q, const void* k, const void* v,
  * Its gradients: dO [B, T, Hv, V] bf16 contiguous, dht nullable; dq, dk, dv
  * bf16 contiguous (q's, k's, v's shapes), dg (g's shape and type), dh0 (nullable).
  * None of them may overlap an input or another (dh0 may be dht).
- * dg is formed in fp32, of whatever type, but from these states: 2^-9 of its
- * terms each, a few 10^-4 of it altogether.
+ * dg is formed in fp32, of whatever type, but from these states: up to 2^-9 of
+ * its terms each, a few 10^-4 of it over many heads and tokens, more of a single
+ * number whose terms cancel.
  * With g_per_head dg is the sum over all tokens, in fp32 and in a fixed order.
  * states: what gdn_linear_chunk_fwd left for these same inputs.
  * Deterministic; workspace: gdn_linear_chunk_bwd_workspace_bytes bytes, likewise.
