@@ -193,7 +193,8 @@ def chunk_linear_attn_bwd(
 ):
     """Gradients of ``chunk_linear_attn``: ``(dq, dk, dv, dg, dh0)``, dq, dk, dv
     in bf16, dg with g's shape and type (an fp32 dg too holds the saved states'
-    rounding, up to 2^-9 of each of its terms), dh0 fp32 (None without ``initial_state``).  ``do`` is dL/do (bf16, v's shape), ``dht`` (nullable)
+    rounding, up to 2^-9 of each of its terms), dh0 fp32 (None without
+    ``initial_state``).  ``do`` is dL/do (bf16, v's shape), ``dht`` (nullable)
     dL/d(final state).  Without ``states`` (``chunk_linear_attn_fwd_save``) the
     forward's states are formed again.  Deterministic.
     """
