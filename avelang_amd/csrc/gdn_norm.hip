@@ -10,132 +10,10 @@
 // forward 8192 x 4096 bf16 26.5 us (5.1 TB/s), 262144 rows of 128 27.7 us (4.8);
 // backward 8192 x 4096 36.8 us (5.5 TB/s; 56 to 61 without the next row on its
 // way) and 4.1 us for the sums of the partial weight gradients.
-#include "gdn_chunk.h"
+#include "gdn_norm_rows.h"
 #include "../../include/gdn_linear.h"
 
 namespace gdn {
-
-// 16 bytes at an element-aligned address (rows of odd length, sliced bases)
-typedef uint32_t u32x4e __attribute__((ext_vector_type(4), aligned(2)));
-
-// the elements of 16 bytes, as floats
-template <int DT>
-__device__ __forceinline__ void unpack(u32x4e raw, float* f) {
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if constexpr (DT == GDN_DTYPE_F32) {
-      f[w] = __uint_as_float(raw[w]);
-    } else {
-      f[2 * w] = Elt<DT>::to_f(static_cast<uint16_t>(raw[w]));
-      f[2 * w + 1] = Elt<DT>::to_f(static_cast<uint16_t>(raw[w] >> 16));
-    }
-  }
-}
-// N elements of type DT at p (element-aligned), as floats
-template <int DT, int N>
-__device__ __forceinline__ void ldn(const void* p, long long i, float (&f)[N]) {
-  constexpr int VEC = Elt<DT>::VEC;
-  static_assert(N % VEC == 0, "whole vectors");
-#pragma unroll
-  for (int u = 0; u < N / VEC; ++u)
-    unpack<DT>(*reinterpret_cast<const u32x4e*>(static_cast<const typename Elt<DT>::T*>(p) + i + u * VEC),
-               f + u * VEC);
-}
-template <int DT, int N>
-__device__ __forceinline__ void stn(void* p, long long i, const float (&f)[N]) {
-  constexpr int VEC = Elt<DT>::VEC;
-#pragma unroll
-  for (int u = 0; u < N / VEC; ++u) {
-    u32x4e raw;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      if constexpr (DT == GDN_DTYPE_F32)
-        raw[w] = __float_as_uint(f[u * VEC + w]);
-      else
-        raw[w] = Elt<DT>::from_f(f[u * VEC + 2 * w]) |
-                 (static_cast<uint32_t>(Elt<DT>::from_f(f[u * VEC + 2 * w + 1])) << 16);
-    }
-    *reinterpret_cast<u32x4e*>(static_cast<typename Elt<DT>::T*>(p) + i + u * VEC) = raw;
-  }
-}
-
-// N parameters from element i of a tensor of runtime type wt
-template <int N>
-__device__ __forceinline__ void ldw(const void* p, long long i, int wt, float (&f)[N]) {
-  if (wt == GDN_DTYPE_F32) {
-    ldn<GDN_DTYPE_F32, N>(p, i, f);
-  } else if constexpr (N % 8 == 0) {
-    if (wt == GDN_DTYPE_BF16) ldn<GDN_DTYPE_BF16, N>(p, i, f);
-    else ldn<GDN_DTYPE_F16, N>(p, i, f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = ldp(p, i + j, wt);
-  }
-}
-
-// Elements c .. c + VEC - 1 of a row of D at p + base (0 past its end).
-template <int DT, int VEC>
-__device__ __forceinline__ void ld_row(const void* p, long long base, int c, int D,
-                                       float (&f)[VEC]) {
-  if (c + VEC <= D) {
-    ldn<DT, VEC>(p, base + c, f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) f[j] = c + j < D ? lde<DT>(p, base + c + j) : 0.f;
-  }
-}
-// The same as raw bits.
-template <int DT>
-__device__ __forceinline__ u32x4e ld_raw(const void* p, long long base, int c, int D) {
-  constexpr int VEC = Elt<DT>::VEC;
-  const auto* src = static_cast<const typename Elt<DT>::T*>(p) + base + c;
-  if (c + VEC <= D) return *reinterpret_cast<const u32x4e*>(src);
-  u32x4e r = {0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < VEC; ++j) {
-    if (c + j >= D) break;
-    if constexpr (DT == GDN_DTYPE_F32) r[j] = __float_as_uint(src[j]);
-    else r[j / 2] |= static_cast<uint32_t>(src[j]) << (16 * (j % 2));
-  }
-  return r;
-}
-template <int DT, int VEC>
-__device__ __forceinline__ void st_row(void* p, long long base, int c, int D,
-                                       const float (&f)[VEC]) {
-  if (c + VEC <= D) {
-    stn<DT, VEC>(p, base + c, f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j)
-      if (c + j < D) ste<DT>(p, base + c + j, f[j]);
-  }
-}
-template <int VEC>
-__device__ __forceinline__ void ld_par(const void* p, long long base, int c, int D, int wt,
-                                       float (&f)[VEC]) {
-  if (c + VEC <= D) {
-    ldw<VEC>(p, base + c, wt, f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) f[j] = c + j < D ? ldp(p, base + c + j, wt) : 0.f;
-  }
-}
-
-// Sum over the LPR lanes of a row: a wave's shuffles, and across the four
-// waves of a 256-lane row through `red` (a buffer per call in flight).
-template <int LPR>
-__device__ __forceinline__ float row_sum(float x, float* red) {
-#pragma unroll
-  for (int off = 1; off < (LPR < 64 ? LPR : 64); off *= 2) x += __shfl_xor(x, off);
-  if constexpr (LPR > 64) {
-    if (threadIdx.x % 64 == 0) red[threadIdx.x / 64] = x;
-    __syncthreads();
-    x = red[0];
-#pragma unroll
-    for (int w = 1; w < LPR / 64; ++w) x += red[w];
-  }
-  return x;
-}
 
 struct NormArgs {
   const void* x;
@@ -445,33 +323,14 @@ __global__ __launch_bounds__(1024) void norm_sum_kernel(const float* pw, const f
 
 namespace {
 
-// Lanes and vectors per row: the fewest lanes that hold it, a workgroup from
-// four vectors per lane of a wave on; lpr 0: longer than a workgroup holds.
-struct RowForm {
-  int lpr, vpt;
-};
-RowForm row_form(int D, int dtype) {
-  const int vec = dtype == GDN_DTYPE_F32 ? 4 : 8;
-  const int n = (D + vec - 1) / vec;
-  if (n <= 16) return {16, 1};
-  if (n <= 32) return {32, 1};
-  if (n <= 64) return {64, 1};
-  if (n <= 128) return {64, 2};
-  if (n <= 256) return {64, 4};
-  if (n <= 512) return {256, 2};
-  if (n <= 1024) return {256, 4};
-  if (vec == 4 && n <= 2048) return {256, 8};
-  return {0, 0};
-}
-
 // Groups that walk the rows of the backward, and the partial sums they leave:
 // two workgroups per CU, a multiple of the heads, no more than rows.
 struct BwdPlan {
-  RowForm f;
+  gdn::RowForm f;
   long long groups, parts, span;
 };
 BwdPlan bwd_plan(long long rows, int heads, int D, int dtype) {
-  BwdPlan p{row_form(D, dtype), 0, 0, 0};
+  BwdPlan p{gdn::row_form(D, dtype), 0, 0, 0};
   const long long per = (rows + heads - 1) / heads;   // rows of a head at most
   if (!p.f.lpr) {
     p.parts = per < 64 ? (per ? per : 1) : 64;
@@ -499,12 +358,6 @@ int check_norm(const char* name, long long rows, int heads, int D, int dtype, in
   return GDN_OK;
 }
 
-// A launch has under 2^32 lanes in a dimension.
-int check_lanes(const char* name, long long workgroups, int lanes) {
-  if (workgroups * lanes < (1LL << 32)) return GDN_OK;
-  return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large for one launch");
-}
-
 }  // namespace
 
 #define GDN_NORM_FORMS(CALL, TT)                                                                 \
@@ -519,9 +372,9 @@ extern "C" int gdn_layer_norm_fwd(const void* x, const void* weight, const void*
   if (rc) return rc;
   if (rows == 0) return GDN_OK;
   if (!x || !y) return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": x and y must be non-NULL");
-  const RowForm f = row_form(D, dtype);
+  const gdn::RowForm f = gdn::row_form(D, dtype);
   const int per = f.lpr ? 256 / f.lpr : 1;   // rows per workgroup
-  if (const int fit = check_lanes(name, (rows + per - 1) / per, 256)) return fit;
+  if (const int fit = gdn_host::check_lanes(name, (rows + per - 1) / per, 256)) return fit;
   gdn_host::launch_begin();
   auto st = static_cast<hipStream_t>(stream);
   const gdn::NormArgs a{x, weight, bias, y, stats, rows, heads, D, eps, w_dtype};
@@ -567,14 +420,14 @@ extern "C" int gdn_layer_norm_bwd(const void* x, const void* weight, const void*
   auto st = static_cast<hipStream_t>(stream);
   const bool sums = dweight || dbias;
   if (sums)
-    if (const int fit = check_lanes(name, (C + 63) / 64, 1024)) return fit;
+    if (const int fit = gdn_host::check_lanes(name, (C + 63) / 64, 1024)) return fit;
   BwdPlan p{};
   float* pw = nullptr;
   float* pb = nullptr;
   if (rows > 0) {
     p = bwd_plan(rows, heads, D, dtype);
     if (!p.f.lpr)
-      if (const int fit = check_lanes(name, rows, 256)) return fit;
+      if (const int fit = gdn_host::check_lanes(name, rows, 256)) return fit;
     if (sums) {
       const size_t need = (size_t)p.parts * C * 2 * sizeof(float);
       if (!workspace || workspace_bytes < need)
