@@ -44,7 +44,23 @@ from .linear_attention import (  # noqa: F401
     fused_recurrent_linear_attn,
     linear_attn_workspace_bytes,
 )
-from .norm import layer_norm, layer_norm_bwd, layer_norm_fwd_save  # noqa: F401
+from .norm import (  # noqa: F401
+    layer_norm,
+    layer_norm_bwd,
+    layer_norm_fwd_save,
+    rms_norm,
+    rms_norm_bwd,
+    rms_norm_fwd_save,
+    rms_norm_quant,
+)
+from .paged_attention import (  # noqa: F401
+    PagedKVCache,
+    paged_attention,
+    paged_attention_workspace_bytes,
+    paged_cache_read,
+    paged_cache_write,
+)
+from .rotary import rotary_embedding, rotary_frequencies  # noqa: F401
 
 __all__ = [
     "chunk_gated_delta_rule",
@@ -69,4 +85,15 @@ __all__ = [
     "layer_norm",
     "layer_norm_bwd",
     "layer_norm_fwd_save",
+    "rms_norm",
+    "rms_norm_bwd",
+    "rms_norm_fwd_save",
+    "rms_norm_quant",
+    "rotary_embedding",
+    "rotary_frequencies",
+    "PagedKVCache",
+    "paged_cache_write",
+    "paged_cache_read",
+    "paged_attention",
+    "paged_attention_workspace_bytes",
 ]

@@ -57,9 +57,23 @@ EXPORTS_LINEAR = (
     "gdn_layer_norm_bwd_workspace_bytes",
 )
 
+# Declared in include/gdn_attn.h.
+EXPORTS_ATTN = (
+    "gdn_rms_norm_fwd",
+    "gdn_rms_norm_bwd",
+    "gdn_rms_norm_bwd_workspace_bytes",
+    "gdn_rotary",
+    "gdn_paged_write",
+    "gdn_paged_read",
+    "gdn_paged_attn_fwd",
+    "gdn_paged_attn_workspace_bytes",
+)
+
 GDN_DTYPE_F32 = 0
 GDN_DTYPE_BF16 = 1
 GDN_DTYPE_F16 = 2
+GDN_DTYPE_E4M3 = 3
+GDN_DTYPE_I8 = 4
 
 GDN_OK = 0
 GDN_ERR_NULL = -1
@@ -223,8 +237,48 @@ def lib():
         h.gdn_layer_norm_bwd.argtypes = (
             [_vp] * 7                         # x weight dy stats dx dweight dbias
             + [_ll, _i, _i, _i, _i, _vp, _sz, _vp])
+        h.gdn_rms_norm_fwd.restype = _i
+        h.gdn_rms_norm_fwd.argtypes = (
+            [_vp] * 7                         # x residual weight y h rstd scale
+            + [_ll, _i, _f, _f, _i, _i, _i, _i, _vp])   # rows D eps offset types stream
+        h.gdn_rms_norm_bwd_workspace_bytes.restype = _sz
+        h.gdn_rms_norm_bwd_workspace_bytes.argtypes = [_ll, _i, _i]
+        h.gdn_rms_norm_bwd.restype = _i
+        h.gdn_rms_norm_bwd.argtypes = (
+            [_vp] * 8                         # h weight dy dh rstd dx dr dweight
+            + [_ll, _i, _f, _i, _i, _i, _vp, _sz, _vp])
+        h.gdn_rotary.restype = _i
+        h.gdn_rotary.argtypes = (
+            [_vp] * 6                         # x y and their strides, heads, positions
+            + [_i, _ll, _vp]                  # int64, batch stride, inv_freq
+            + [_i] * 4 + [_f, _i, _i, _i, _vp])   # B T D R magnitude near inverse dtype stream
+        h.gdn_paged_write.restype = _i
+        h.gdn_paged_write.argtypes = (
+            [_vp, _vp] + [_ll] * 4 + [_vp, _i]   # k v strides slots int64
+            + [_vp] * 4                       # caches and scales
+            + [_i] * 7 + [_vp])               # T H D pages page dtypes stream
+        h.gdn_paged_read.restype = _i
+        h.gdn_paged_read.argtypes = [_vp] * 5 + [_i] + [_vp] * 2 + [_i] * 7 + [_vp]
+        h.gdn_paged_attn_workspace_bytes.restype = _sz
+        h.gdn_paged_attn_workspace_bytes.argtypes = [_i] * 6
+        h.gdn_paged_attn_fwd.restype = _i
+        h.gdn_paged_attn_fwd.argtypes = (
+            [_vp] + [_ll] * 3                 # q and its strides
+            + [_vp] * 5 + [_ll]               # caches, scales, block table and its stride
+            + [_vp] * 3                       # lengths o lse
+            + [_i] * 9 + [_f, _i, _i]         # N L Hq Hkv D pages page max_length window scale types
+            + [_vp, _sz, _vp])
         _lib = h
         return _lib
+
+
+def on_device(dev, fn, *args):
+    """``fn(*args)`` with ``dev`` as the current device (the entry points launch on it and
+    size their grids for it)."""
+    if torch._C._cuda_getDevice() == dev.index:
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
 
 
 def last_error() -> str:

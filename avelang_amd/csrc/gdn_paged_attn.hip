@@ -1,0 +1,695 @@
+// Attention of a sequence's newest tokens over a paged key-value cache, for
+// gfx950 (declared in gdn_attn.h): per kv-head and row (token, q-head of its
+// group)
+//     o = sum_t e^{s_t - m} v_t / sum_t e^{s_t - m},   s_t = scale q . k_t
+// over the tokens t that the row sees, with the running maximum m, sum and o of
+// one pass (in base 2).
+//
+// The path reads the cache once (2 D elements per token and kv-head against 4 D
+// flops per row: up to 16 rows share a read) and is bound by HBM.  A wave takes
+// 32 tokens at a time straight from HBM into the registers of its MFMA operands,
+// no LDS in between: S^T = K Q^T with tokens as rows leaves P^T in the layout in
+// which it is the operand of O^T = V^T P^T, whose V^T a lane forms in its own
+// registers from eight tokens' 16-byte pieces (one v_perm per word).  The next
+// tokens' K is on its way while these' softmax and V are worked on, and the other
+// way round.
+//
+// Work: every (sequence, kv-head) is as many units of 128 tokens as its length
+// has; all units in a row are cut into equal shares, one per workgroup, whatever
+// the lengths (read on the device: nothing here depends on a host copy of them).
+// A share that holds a whole (sequence, kv-head) writes its output; parts leave
+// m, the sum and o in the workspace and a second launch joins them.
+#include "gdn_bits8.h"
+#include "gdn_norm_rows.h"
+
+namespace gdn {
+
+constexpr int kUnit = 128;   // tokens of a unit of work
+
+struct PagedAttnArgs {
+  const void* q;
+  long long sn, sl, sh;   // q's strides of sequence, token and head
+  const void* kc;
+  const void* vc;
+  const float* ks;
+  const float* vs;
+  const int32_t* table;
+  long long table_stride;
+  const int32_t* lens;
+  void* o;
+  float* lse;
+  float* part;
+  int4* desc;
+  int N, L, Hq, Hkv, G, R, RG, rows;   // R = L G rows per kv-head in RG groups of at most `rows`
+  int num_pages, page, cap, window;
+  float scale2;   // scale log2(e)
+};
+
+// Tokens [lo, hi) that a sequence's rows see, and their units (one at least).
+struct Span {
+  int lo, hi, units;
+};
+__device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int n) {
+  Span s;
+  s.hi = min(max(a.lens[n], 0), a.cap);
+  s.lo = a.window > 0 ? max(0, s.hi - a.L + 1 - a.window) & ~15 : 0;
+  s.units = max(1, (s.hi - s.lo + kUnit - 1) / kUnit);
+  return s;
+}
+
+__device__ __forceinline__ float xmax16(float x) {
+  x = fmaxf(x, __shfl_xor(x, 16));
+  return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float xsum16(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+// What the MFMAs run in: bf16 over a bf16 cache; fp16 else (8-bit codes are
+// exact there, and two conversions cheaper than in bf16).
+template <bool BF>
+__device__ __forceinline__ f32x4 mfma_t(u16x8 a, u16x8 b, f32x4 c) {
+  if constexpr (BF) return mfma16(a, b, c);
+  else return mfma16h(a, b, c);
+}
+template <bool BF>
+__device__ __forceinline__ uint16_t from_f(float f) {
+  if constexpr (BF) return f2bf(f);
+  else return f2h(f);
+}
+template <bool BF>
+__device__ __forceinline__ float to_f(uint16_t h) {
+  if constexpr (BF) return bf2f(h);
+  else return static_cast<float>(__builtin_bit_cast(_Float16, h));
+}
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4w __attribute__((ext_vector_type(4)));
+
+// Two codes in the halves of a word as fp16.  Integers: the byte (biased by 128)
+// as an fp16 denormal u 2^-24, times 2^15, less 128 2^-9: the value times 2^-9,
+// exactly.
+constexpr float kI8 = 512.f;
+__device__ __forceinline__ uint32_t i8_pair(uint32_t u) {
+  const f16x2 x = __builtin_bit_cast(f16x2, u);
+  const f16x2 k = {(_Float16)32768.f, (_Float16)32768.f}, b = {(_Float16)-0.25f, (_Float16)-0.25f};
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(x, k, b));
+}
+template <bool HI>
+__device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI));
+}
+
+// Eight codes as an operand.
+template <int CT>
+__device__ __forceinline__ u16x8 codes_operand(uint32_t w0, uint32_t w1) {
+  u32x4w r;
+  if constexpr (CT == GDN_DTYPE_E4M3) {
+    r = u32x4w{e4m3_pair<false>(w0), e4m3_pair<true>(w0), e4m3_pair<false>(w1), e4m3_pair<true>(w1)};
+  } else {
+    w0 ^= 0x80808080u;
+    w1 ^= 0x80808080u;
+    r = u32x4w{i8_pair(__builtin_amdgcn_perm(0, w0, 0x0c010c00u)), i8_pair(__builtin_amdgcn_perm(0, w0, 0x0c030c02u)),
+               i8_pair(__builtin_amdgcn_perm(0, w1, 0x0c010c00u)), i8_pair(__builtin_amdgcn_perm(0, w1, 0x0c030c02u))};
+  }
+  return __builtin_bit_cast(u16x8, r);
+}
+
+// RW: waves of a workgroup that take rows apart (16 each); the others take tokens apart.
+template <int QT, int CT, int D, int RW>
+__global__ __launch_bounds__(256, D == 256 && (CT == GDN_DTYPE_BF16 || CT == GDN_DTYPE_F16) ? 1 : 2)
+void paged_attn_kernel(PagedAttnArgs a) {
+  constexpr bool BF = CT == GDN_DTYPE_BF16;                        // bf16 products
+  constexpr bool C8 = CT == GDN_DTYPE_E4M3 || CT == GDN_DTYPE_I8;  // codes with scales
+  constexpr int ES = C8 ? 1 : 2, ROW = D * ES;                     // bytes of an element, of a row
+  constexpr int TW = 4 / RW;                                       // waves that take tokens apart
+  constexpr int KL = ROW / 64;                                     // 16-byte pieces of K per lane and 16 tokens
+  constexpr int E = D / 16;                                        // elements of V per lane and token
+  constexpr int VD = E * ES / 4;                                   // words of them
+  constexpr int CH = E * ES > 16 ? 16 / ES : E;                    // elements of one piece
+  constexpr bool LO = BF || QT == GDN_DTYPE_F16;   // P in two parts: 2^-9 (bf16), 2^-12 of one would show in o
+  __shared__ float buf[4][16][D + 4];
+  __shared__ float sm[4][16], sl[4][16];
+  __shared__ int wave_sum[4];
+  __shared__ int found[2];
+  const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+  const int c16 = lane % 16, g = lane / 16;
+  const int ts = wave / RW, rw = wave % RW;
+  const char* const kc = static_cast<const char*>(a.kc);
+  const char* const vc = static_cast<const char*>(a.vc);
+
+  // this workgroup's share of all units
+  const int HG = a.Hkv * a.RG;
+  int total, u0, u1, share, n, prefix;
+  {
+    const int per = (a.N + 255) / 256, first = tid * per, last = min(first + per, a.N);
+    int sum = 0;
+    for (int i = first; i < last; ++i) sum += span_of(a, i).units;
+    int incl = sum;
+#pragma unroll
+    for (int off = 1; off < 64; off *= 2) {
+      const int x = __shfl_up(incl, off);
+      if (lane >= off) incl += x;
+    }
+    if (lane == 63) wave_sum[wave] = incl;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < wave) incl += wave_sum[w];
+      total += wave_sum[w];
+    }
+    total = __builtin_amdgcn_readfirstlane(total) * HG;
+    share = (total + gridDim.x - 1) / gridDim.x;
+    u0 = min((int)blockIdx.x * share, total);
+    u1 = min(u0 + share, total);
+    if (tid == 0) a.desc[blockIdx.x] = int4{0, 0, 0, 0};
+    if (u0 >= u1) return;
+    int at = incl - sum;
+    if (at * HG <= u0 && u0 < incl * HG) {
+      int i = first;
+      for (;; ++i) {
+        const int un = span_of(a, i).units;
+        if (u0 < (at + un) * HG) break;
+        at += un;
+      }
+      found[0] = i;
+      found[1] = at;
+    }
+    __syncthreads();
+    n = __builtin_amdgcn_readfirstlane(found[0]);
+    prefix = __builtin_amdgcn_readfirstlane(found[1]);
+  }
+
+  for (int u = u0; u < u1;) {
+    const Span sp = span_of(a, n);
+    const int rel = u - prefix * HG, item = rel / sp.units, start = rel % sp.units;
+    const int len = min(sp.units - start, u1 - u);
+    const int kvh = item / a.RG, rg = item % a.RG;
+    const int t0 = sp.lo + start * kUnit, t1 = min(t0 + len * kUnit, sp.hi);
+
+    // the rows' queries: column c16 of the operand is row 16 (rg RW + rw) + c16
+    const int rr = 16 * (rg * RW + rw) + c16, l = rr / a.G;
+    const int pos = sp.hi - a.L + l;   // its own place in the sequence
+    u16x8 qf[D / 32];
+    float qscale = a.scale2;
+    {
+      float f[D / 32][8];
+      uint32_t m = 0;
+      const long long base = n * a.sn + l * a.sl + (kvh * a.G + rr % a.G) * a.sh;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) {
+        const int d = C8 ? 64 * (k / 2) + 16 * g + 8 * (k % 2) : 32 * k + 8 * g;
+        if (rr < a.R) {
+          if constexpr (C8) ldn<QT, 8>(a.q, base + d, f[k]);
+          else qf[k] = *reinterpret_cast<const u16x8*>(static_cast<const uint16_t*>(a.q) + base + d);
+        } else {
+          qf[k] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[k][j] = 0.f;
+        }
+        if constexpr (C8) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) m = max(m, abs_bits(f[k][j]));
+        }
+      }
+      if constexpr (C8) {
+        // in fp16, with a power of two that brings the row's largest value to
+        // [2^14, 2^15): a bf16 value down to 2^-31 of it stays exact
+        m = max(m, (uint32_t)__shfl_xor((int)m, 16));
+        m = max(m, (uint32_t)__shfl_xor((int)m, 32));
+        const int e = min(max((int)(m >> 23), 64), 254) - 127;
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) qf[k][j] = f2h(ldexpf(f[k][j], 14 - e));
+        qscale = ldexpf(a.scale2 * (CT == GDN_DTYPE_I8 ? kI8 : 1.f), e - 14);
+      }
+    }
+
+    // rows (in the cache) of the next 64 sixteens of this wave's tokens, one per lane
+    const int step = 32 * TW;
+    const int tiles = t1 > t0 + 32 * ts ? (t1 - t0 - 32 * ts + step - 1) / step : 0;
+    long long row64 = 0;
+    auto look_up = [&](int it) {
+      int t = t0 + 32 * ts + (it + lane / 2) * step + 16 * (lane % 2);
+      t = min(t, (t1 - 1) & ~15);
+      const int pg = a.table[n * a.table_stride + t / a.page];
+      const bool ok = pg >= 0 && pg < a.num_pages;
+      row64 = ok ? ((long long)pg * a.Hkv + kvh) * a.page + t % a.page : -1;
+    };
+    auto row_at = [&](int it, int s) {
+      const int i = 2 * (it % 32) + s;
+      const uint32_t lo = __builtin_amdgcn_readlane((int)row64, i);
+      const uint32_t hi = __builtin_amdgcn_readlane((int)(row64 >> 32), i);
+      return (long long)((uint64_t)hi << 32 | lo);
+    };
+
+    u32x4w kr[2][KL];
+    uint32_t vr[8][VD];
+    f32x4 kscale[2], vscale[2];
+    long long rows[2];   // of the tile whose K is loaded
+    auto valid = [&](int it, int s) {   // tokens of a sixteen that there are
+      return min(max(t1 - (t0 + 32 * ts + it * step + 16 * s), 1), 16);
+    };
+    auto load_k = [&](int it) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        rows[s] = row_at(it, s);
+        const long long row = max(rows[s], 0ll);
+        const char* p = kc + row * ROW;
+        const int off = min(c16, valid(it, s) - 1) * ROW + 16 * g;
+#pragma unroll
+        for (int k = 0; k < KL; ++k) kr[s][k] = *reinterpret_cast<const u32x4w*>(p + (off + 64 * k));
+        if constexpr (C8) kscale[s] = *reinterpret_cast<const f32x4*>(a.ks + row + 4 * g);
+      }
+    };
+    auto load_v = [&](const long long (&rv)[2], int it) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const long long row = max(rv[s], 0ll);
+        const char* p = vc + row * ROW;
+        const int most = valid(it, s) - 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int off = min(4 * g + i, most) * ROW + c16 * CH * ES;
+          uint32_t* dst = vr[4 * s + i];
+          if constexpr (VD == 1) {
+            dst[0] = *reinterpret_cast<const uint32_t*>(p + off);
+          } else if constexpr (VD == 2) {
+            const u32x2p x = *reinterpret_cast<const u32x2p*>(p + off);
+            dst[0] = x[0];
+            dst[1] = x[1];
+          } else {
+#pragma unroll
+            for (int j = 0; j < VD / 4; ++j) {
+              const u32x4w x = *reinterpret_cast<const u32x4w*>(p + (off + 256 * j));
+#pragma unroll
+              for (int w = 0; w < 4; ++w) dst[4 * j + w] = x[w];
+            }
+          }
+        }
+        if constexpr (C8) vscale[s] = *reinterpret_cast<const f32x4*>(a.vs + row + 4 * g);
+      }
+    };
+
+    f32x4 acc[E];
+#pragma unroll
+    for (int j = 0; j < E; ++j) acc[j] = zero4();
+    float m = -INFINITY, sum = 0.f, vref = 0.f, vinv = 1.f;
+    long long rv[2];
+    if (tiles > 0) {
+      look_up(0);
+      load_k(0);
+      rv[0] = rows[0];
+      rv[1] = rows[1];
+      load_v(rv, 0);
+    }
+    for (int it = 0; it < tiles; ++it) {
+      const int tb = t0 + 32 * ts + it * step;
+      f32x4 S[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        S[s] = zero4();
+#pragma unroll
+        for (int k = 0; k < D / 32; ++k) {
+          u16x8 kf;
+          if constexpr (C8) kf = codes_operand<CT>(kr[s][k / 2][2 * (k % 2)], kr[s][k / 2][2 * (k % 2) + 1]);
+          else kf = __builtin_bit_cast(u16x8, kr[s][k]);
+          S[s] = mfma_t<BF>(kf, qf[k], S[s]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) S[s][r] *= C8 ? qscale * kscale[s][r] : qscale;
+      }
+      const bool bad = rows[0] < 0 || rows[1] < 0;
+      const bool here[2] = {rows[0] < 0, rows[1] < 0};
+      if (it + 1 < tiles) {
+        if ((it + 1) % 32 == 0) look_up(it + 1);
+        load_k(it + 1);
+      }
+      // tokens that some row of this wave does not see
+      const bool mixed = (a.L > 1 && tb + 31 > sp.hi - a.L) || (a.window > 0 && tb <= sp.hi - 1 - a.window);
+      const bool part = mixed || bad || tb + 32 > t1;
+      bool seen[2][4];
+      if (part) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int t = tb + 16 * s + 4 * g + r;
+            seen[s][r] = t < t1 && t <= pos && (a.window == 0 || t > pos - a.window);
+            if (here[s]) S[s][r] = __builtin_nanf("");
+            if (!seen[s][r]) S[s][r] = -INFINITY;
+          }
+      }
+      float mx = S[0][0];
+#pragma unroll
+      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, S[i / 4][i % 4]);
+      mx = fmaxf(m, xmax16(mx));
+      const float ref = mx == -INFINITY ? 0.f : mx;
+      float grow = 1.f;
+      if constexpr (C8) {
+        // V's scales over a power of two no smaller than any so far: P stays in
+        // fp16's range
+        float big = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (part && !(tb + 16 * (i / 4) + 4 * g + i % 4 < t1)) vscale[i / 4][i % 4] = 0.f;
+          big = fmaxf(big, vscale[i / 4][i % 4]);
+        }
+        big = xmax16(big);
+        if (big > vref) {
+          const float next = __uint_as_float(min((__float_as_uint(big) & 0x7f800000u) + 0x800000u, 0x7e800000u));
+          grow = vref * (1.f / next);
+          vref = next;
+          vinv = 1.f / next;
+        }
+      }
+      if (__any(mx > m) || (C8 && grow != 1.f)) {
+        const float f = exp2f(m - ref);   // (m = -inf: 0)
+        sum *= f;
+#pragma unroll
+        for (int j = 0; j < E; ++j) acc[j] *= f * grow;
+        m = mx;
+      }
+      u16x8 hi, lo;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        float p = exp2f(S[i / 4][i % 4] - ref);
+        sum += p;
+        if constexpr (C8) {
+          p *= vscale[i / 4][i % 4] * vinv;
+          if (part && !seen[i / 4][i % 4]) p = 0.f;
+        }
+        hi[i] = from_f<BF>(p);
+        if constexpr (LO) lo[i] = from_f<BF>(p - to_f<BF>(hi[i]));
+      }
+      u16x8 ones;
+      if (mixed) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ones[i] = seen[i / 4][i % 4] ? from_f<BF>(1.f) : (uint16_t)0;
+      }
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        u32x4w vf;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          if constexpr (CT == GDN_DTYPE_E4M3) {
+            const uint32_t w = __builtin_amdgcn_perm(vr[2 * t + 1][j / 4], vr[2 * t][j / 4],
+                                                     j % 4 < 2 ? 0x05010400u : 0x07030602u);
+            vf[t] = j % 2 ? e4m3_pair<true>(w) : e4m3_pair<false>(w);
+          } else if constexpr (CT == GDN_DTYPE_I8) {
+            constexpr uint32_t sel[4] = {0x0c040c00u, 0x0c050c01u, 0x0c060c02u, 0x0c070c03u};
+            vf[t] = i8_pair(__builtin_amdgcn_perm(vr[2 * t + 1][j / 4] ^ 0x80808080u,
+                                                  vr[2 * t][j / 4] ^ 0x80808080u, sel[j % 4]));
+          } else {
+            vf[t] = __builtin_amdgcn_perm(vr[2 * t + 1][j / 2], vr[2 * t][j / 2],
+                                          j % 2 ? 0x07060302u : 0x05040100u);
+          }
+        }
+        u16x8 v = __builtin_bit_cast(u16x8, vf);
+        if (mixed) {
+          // a value that is not finite reaches only the rows that see its token
+          constexpr uint16_t kExp = BF ? 0x7f80 : 0x7c00;
+          u16x8 ind;
+          bool any = false;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const bool x = (v[i] & kExp) == kExp;
+            any |= x;
+            ind[i] = x ? from_f<BF>(1.f) : (uint16_t)0;
+            v[i] = x ? (uint16_t)0 : v[i];
+          }
+          if (__any(any)) {
+            const f32x4 hit = mfma_t<BF>(ind, ones, zero4());
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (hit[r] > 0.f) acc[j][r] = __builtin_nanf("");
+          }
+        }
+        acc[j] = mfma_t<BF>(v, hi, acc[j]);
+        if constexpr (LO) acc[j] = mfma_t<BF>(v, lo, acc[j]);
+      }
+      if (it + 1 < tiles) {
+        rv[0] = rows[0];
+        rv[1] = rows[1];
+        load_v(rv, it + 1);
+      }
+    }
+    sum = xsum16(sum);
+    if constexpr (C8) {
+#pragma unroll
+      for (int j = 0; j < E; ++j) acc[j] *= vref * (CT == GDN_DTYPE_I8 ? kI8 : 1.f);
+    }
+
+    // the waves' parts joined: D's element of lane (c16, g), r of acc[j] is
+    // (j / CH) 16 CH + (4 g + r) CH + j % CH of row c16
+    if (g == 0) {
+      sm[wave][c16] = m;
+      sl[wave][c16] = sum;
+    }
+    if (rr < a.R) {
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) buf[wave][c16][(j / CH) * 16 * CH + (4 * g + r) * CH + j % CH] = acc[j][r];
+    }
+    __syncthreads();
+    const bool whole = len == sp.units;
+    const int slot = u == u0 ? 2 * blockIdx.x : 2 * blockIdx.x + 1;
+    float* const part = a.part + (size_t)slot * a.rows * (D + 2);
+    const int here = min(a.R - 16 * RW * rg, 16 * RW);   // rows of this group
+    for (int i = tid; i < here * (D / 4); i += 256) {
+      const int row = i / (D / 4), d = 4 * (i % (D / 4)), w0 = row / 16, c = row % 16;
+      float M = sm[w0][c];
+#pragma unroll
+      for (int w = 1; w < TW; ++w) M = fmaxf(M, sm[w0 + w * RW][c]);
+      const float ref = M == -INFINITY ? 0.f : M;
+      float s = 0.f;
+      f32x4 o = zero4();
+#pragma unroll
+      for (int w = 0; w < TW; ++w) {
+        const float f = exp2f(sm[w0 + w * RW][c] - ref);
+        s += f * sl[w0 + w * RW][c];
+        o += f * *reinterpret_cast<const f32x4*>(&buf[w0 + w * RW][c][d]);
+      }
+      const int orow = 16 * RW * rg + row;
+      const long long at = ((long long)n * a.L + orow / a.G) * a.Hq + kvh * a.G + orow % a.G;
+      if (whole) {
+        o *= s == 0.f ? 0.f : 1.f / s;
+        u16x4 h;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) h[j] = Elt<QT>::from_f(o[j]);
+        *reinterpret_cast<u16x4*>(static_cast<uint16_t*>(a.o) + at * D + d) = h;
+        if (a.lse && d == 0) a.lse[at] = s == 0.f ? -INFINITY : (M + log2f(s)) * 0.69314718055994530942f;
+      } else {
+        *reinterpret_cast<f32x4*>(part + row * D + d) = o;
+        if (d == 0) {
+          part[a.rows * D + row] = M;
+          part[a.rows * (D + 1) + row] = s;
+        }
+      }
+    }
+    if (!whole && start == 0 && tid == 0)
+      a.desc[blockIdx.x] = int4{n, item, slot, 1 + (sp.units - len + share - 1) / share};
+    u += len;
+    if (item == HG - 1 && start + len == sp.units) {
+      prefix += sp.units;
+      ++n;
+    }
+    __syncthreads();
+  }
+}
+
+// Parts of one (sequence, kv-head) joined: block (w, row, 64 columns) takes the one
+// that begins in workgroup w's share and ends in another's.
+template <int QT, int D>
+__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
+  __shared__ float red[4];
+  __shared__ float acc[4][64];
+  const int4 ds = a.desc[blockIdx.x];
+  const int pieces = ds.w;
+  if (pieces == 0) return;
+  const int kvh = ds.y / a.RG, rg = ds.y % a.RG, row = blockIdx.y;
+  const int orow = rg * a.rows + row;
+  if (orow >= a.R) return;
+  const int tid = threadIdx.x, col = tid % 64, grp = tid / 64, d = blockIdx.z * 64 + col;
+  const size_t each = (size_t)a.rows * (D + 2);
+  // piece p's part: its workgroup's first, but for the one that begins here
+  auto at = [&](int p) { return a.part + (p == 0 ? ds.z : 2 * (blockIdx.x + p)) * each; };
+  float M = -INFINITY;
+  for (int p = tid; p < pieces; p += 256) M = fmaxf(M, at(p)[a.rows * D + row]);
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) M = fmaxf(M, __shfl_xor(M, off));
+  if (col == 0) red[grp] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float ref = M == -INFINITY ? 0.f : M;
+  float s = 0.f, o = 0.f;
+#pragma unroll 4
+  for (int p = grp; p < pieces; p += 4) {
+    const float* x = at(p);
+    const float f = exp2f(x[a.rows * D + row] - ref);
+    s += f * x[a.rows * (D + 1) + row];
+    o += f * x[row * D + d];
+  }
+  acc[grp][col] = o;
+  __syncthreads();
+  if (col == 0) red[grp] = s;
+  __syncthreads();
+  if (grp) return;
+  o = acc[0][col] + acc[1][col] + acc[2][col] + acc[3][col];
+  s = red[0] + red[1] + red[2] + red[3];
+  const long long out = ((long long)ds.x * a.L + orow / a.G) * a.Hq + kvh * a.G + orow % a.G;
+  ste<QT>(a.o, out * D + d, s == 0.f ? 0.f : o / s);
+  if (a.lse && d == 0) a.lse[out] = s == 0.f ? -INFINITY : (M + log2f(s)) * 0.69314718055994530942f;
+}
+
+}  // namespace gdn
+
+namespace gdn_host {
+int check_cache(const char* name, const void* k_cache, const void* v_cache, const float* k_scale,
+                const float* v_scale, int H, int D, int num_pages, int page_size, int cache_dtype);
+}
+
+namespace {
+
+// Workgroups, and how the rows of a kv-head are laid over their waves.
+struct AttnPlan {
+  int rw, rg, rows;
+  long long wgs;
+  size_t desc, bytes;
+};
+int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_length, AttnPlan& p) {
+  if (N < 0 || L < 1 || Hq < 1 || Hkv < 1 || max_length < 0)
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": sizes must be non-negative (L, Hq, Hkv > 0)");
+  if (Hq % Hkv)
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": Hq must be a multiple of Hkv");
+  if (D != 64 && D != 128 && D != 256)
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": D must be 64, 128 or 256");
+  const long long R = (long long)L * (Hq / Hkv);
+  if (R > (1 << 20) || max_length > (1 << 30) || Hq > (1 << 20))
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
+  p.rw = R <= 16 ? 1 : R <= 32 ? 2 : 4;
+  p.rg = (int)((R + 16 * p.rw - 1) / (16 * p.rw));
+  p.rows = (int)(R < 16 * p.rw ? R : 16 * p.rw);
+  const long long units = ((long long)max_length + gdn::kUnit - 1) / gdn::kUnit;
+  const long long most = (units ? units : 1) * N * Hkv * p.rg;
+  if (most >= (1LL << 30))
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
+  p.wgs = 2LL * gdn::device_cus();
+  if (p.wgs > most) p.wgs = most;
+  p.desc = (size_t)p.wgs * 16;
+  p.bytes = p.desc + (size_t)p.wgs * 2 * p.rows * (D + 2) * sizeof(float);
+  p.bytes = (p.bytes + 255) / 256 * 256;
+  return GDN_OK;
+}
+
+}  // namespace
+
+extern "C" size_t gdn_paged_attn_workspace_bytes(int N, int L, int Hq, int Hkv, int D, int max_length) {
+  AttnPlan p{};
+  if (attn_plan("gdn_paged_attn_workspace_bytes", N, L, Hq, Hkv, D, max_length, p)) return 0;
+  return p.bytes;
+}
+
+extern "C" int gdn_paged_attn_fwd(const void* q, long long q_seq, long long q_token, long long q_head,
+                                  const void* k_cache, const void* v_cache, const float* k_scale,
+                                  const float* v_scale, const int32_t* block_table,
+                                  long long table_row, const int32_t* lengths, void* o, float* lse,
+                                  int N, int L, int Hq, int Hkv, int D, int num_pages,
+                                  int page_size, int max_length, int window, float scale,
+                                  int dtype, int cache_dtype, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  const char* name = "gdn_paged_attn_fwd";
+  AttnPlan p{};
+  if (const int rc = attn_plan(name, N, L, Hq, Hkv, D, max_length, p)) return rc;
+  if (const int rc = gdn_host::check_cache(name, k_cache, v_cache, k_scale, v_scale, Hkv, D, num_pages, page_size,
+                                           cache_dtype))
+    return rc;
+  if (page_size % 16)
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": page_size must be a multiple of 16");
+  if (num_pages < 1)
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": the cache must have a page");
+  if (window < 0 || table_row < 0 || (max_length && table_row < (max_length - 1) / page_size + 1))
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": window must be >= 0, and a table's row hold the "
+                                                             "pages of max_length tokens");
+  if (dtype != GDN_DTYPE_BF16 && dtype != GDN_DTYPE_F16)
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": unsupported dtype code");
+  if (N == 0) return GDN_OK;
+  if (!q || !o || !lengths || (max_length && !block_table))
+    return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": q, o, block_table and lengths must be non-NULL");
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(o)) % 16 || (q_seq | q_token | q_head) % 8 ||
+      q_seq < 0 || q_token < 0 || q_head < 0)
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": q and o must be 16-byte aligned, q's strides "
+                                                             "non-negative multiples of 8");
+  if ((reinterpret_cast<uintptr_t>(k_scale) | reinterpret_cast<uintptr_t>(v_scale)) % 16)
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": scales must be 16-byte aligned");
+  const size_t ob = (size_t)N * L * Hq * D * 2;
+  const size_t qb = ((size_t)(N - 1) * q_seq + (size_t)(L - 1) * q_token + (size_t)(Hq - 1) * q_head + D) * 2;
+  if (gdn_host::overlaps(o, ob, q, qb))
+    return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": o must not overlap q");
+  if (!workspace || workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(workspace) % 16)
+    return gdn_host::fail(GDN_ERR_WORKSPACE, std::string(name) + ": workspace needs " + std::to_string(p.bytes) +
+                                                 " bytes, 16-byte aligned, got " + std::to_string(workspace_bytes));
+  const long long R = (long long)L * (Hq / Hkv);
+  gdn::PagedAttnArgs a{};
+  a.q = q;
+  a.sn = q_seq;
+  a.sl = q_token;
+  a.sh = q_head;
+  a.kc = k_cache;
+  a.vc = v_cache;
+  a.ks = k_scale;
+  a.vs = v_scale;
+  a.table = block_table;
+  a.table_stride = table_row;
+  a.lens = lengths;
+  a.o = o;
+  a.lse = lse;
+  a.desc = static_cast<int4*>(workspace);
+  a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.desc);
+  a.N = N;
+  a.L = L;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.G = Hq / Hkv;
+  a.R = (int)R;
+  a.RG = p.rg;
+  a.rows = p.rows;
+  a.num_pages = num_pages;
+  a.page = page_size;
+  a.cap = max_length;
+  a.window = window > (1 << 30) ? 1 << 30 : window;
+  a.scale2 = scale * 1.44269504088896340736f;
+  auto st = static_cast<hipStream_t>(stream);
+  gdn_host::launch_begin();
+  bool done = false;
+#define GDN_PA(QQ, CC, DD, WW)                                                                    \
+  if (dtype == QQ && cache_dtype == CC && D == DD && p.rw == WW) {                                \
+    hipLaunchKernelGGL((gdn::paged_attn_kernel<QQ, CC, DD, WW>), dim3((unsigned)p.wgs), dim3(256), 0, st, a); \
+    done = true;                                                                                  \
+  }
+#define GDN_PA_W(QQ, CC, DD) GDN_PA(QQ, CC, DD, 1) GDN_PA(QQ, CC, DD, 2) GDN_PA(QQ, CC, DD, 4)
+#define GDN_PA_D(QQ, CC) GDN_PA_W(QQ, CC, 64) GDN_PA_W(QQ, CC, 128) GDN_PA_W(QQ, CC, 256)
+  GDN_PA_D(GDN_DTYPE_BF16, GDN_DTYPE_BF16)
+  GDN_PA_D(GDN_DTYPE_F16, GDN_DTYPE_F16)
+  GDN_PA_D(GDN_DTYPE_BF16, GDN_DTYPE_E4M3)
+  GDN_PA_D(GDN_DTYPE_F16, GDN_DTYPE_E4M3)
+  GDN_PA_D(GDN_DTYPE_BF16, GDN_DTYPE_I8)
+  GDN_PA_D(GDN_DTYPE_F16, GDN_DTYPE_I8)
+#undef GDN_PA_D
+#undef GDN_PA_W
+#undef GDN_PA
+  if (!done)
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": the cache must be of q's type or have 8 bits");
+  const dim3 grid((unsigned)p.wgs, (unsigned)p.rows, (unsigned)(D / 64));
+#define GDN_PJ(QQ, DD)                                                                            \
+  if (dtype == QQ && D == DD)                                                                     \
+    hipLaunchKernelGGL((gdn::paged_attn_join_kernel<QQ, DD>), grid, dim3(256), 0, st, a);
+  GDN_PJ(GDN_DTYPE_BF16, 64) GDN_PJ(GDN_DTYPE_BF16, 128) GDN_PJ(GDN_DTYPE_BF16, 256)
+  GDN_PJ(GDN_DTYPE_F16, 64) GDN_PJ(GDN_DTYPE_F16, 128) GDN_PJ(GDN_DTYPE_F16, 256)
+#undef GDN_PJ
+  return gdn_host::check_launch(name);
+}

@@ -1,0 +1,210 @@
+// Rotary positions for gfx950 (declared in gdn_attn.h):
+//     (a, b) -> m (a cos t - b sin t, b cos t + a sin t),  t = p f_j
+// of the pairs of a head's first R elements, the rest copied.
+//
+// The path reads and writes every element once and is bound by HBM.  A lane
+// owns a unit of 2 VEC elements of a head (VEC pairs, or 2 VEC elements of the
+// copied part), forms its pairs' sines and cosines once and turns that unit of
+// several heads.  There is no table of angles: a position's turns p f / 2 pi are
+// formed in 64 bits and reduced there, so far positions lose nothing, and no
+// position is out of a table's range.
+#include "gdn_norm_rows.h"
+#include "../../include/gdn_attn.h"
+
+namespace gdn {
+
+struct RotaryArgs {
+  const void* x[2];
+  void* y[2];
+  long long xs[2][3], ys[2][3];
+  const void* pos;
+  const double* freq;
+  long long pos_batch;
+  int heads[2];
+  int T, R, units, per_wg, rows, split, inplace;   // rows: B T;  split: lanes' groups per token
+  float mag, sign;
+  int pos64;
+};
+
+// VEC elements at p + i: 16 bytes, or fewer where VEC is not a whole vector.
+template <int DT, int VEC>
+__device__ __forceinline__ void ld_unit(const void* p, long long i, float (&f)[VEC]) {
+  if constexpr (VEC % Elt<DT>::VEC == 0) {
+    ldn<DT, VEC>(p, i, f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[j] = lde<DT>(p, i + j);
+  }
+}
+template <int DT, int VEC>
+__device__ __forceinline__ void st_unit(void* p, long long i, const float (&f)[VEC]) {
+  if constexpr (VEC % Elt<DT>::VEC == 0) {
+    stn<DT, VEC>(p, i, f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) ste<DT>(p, i + j, f[j]);
+  }
+}
+
+template <int DT, int VEC, bool NEAR>
+__global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
+  const int slot = threadIdx.x / a.units, u = threadIdx.x % a.units;
+  const long long id = (long long)blockIdx.x * a.per_wg + slot;
+  if (slot >= a.per_wg || id >= (long long)a.rows * a.split) return;
+  const int row = (int)(id / a.split), h0 = (int)(id % a.split);
+  const int b = row / a.T, t = row % a.T;
+  const bool turn = 2 * VEC * u < a.R;
+  if (!turn && a.inplace) return;
+  // offsets of the unit's two halves in a head
+  const int lo = NEAR || !turn ? 2 * VEC * u : VEC * u;
+  const int hi = NEAR || !turn ? lo + VEC : lo + a.R / 2;
+  float c[VEC], s[VEC];
+  if (turn) {
+    const long long pi = b * a.pos_batch + t;
+    const double p = a.pos64 ? (double)static_cast<const long long*>(a.pos)[pi]
+                             : (double)static_cast<const int*>(a.pos)[pi];
+    double f[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) f[j] = a.freq[VEC * u + j];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+      double w = p * f[j] * 0.15915494309189533577;   // turns: 1 / (2 pi)
+      w -= rint(w);
+      sincospif(2.f * (float)w, &s[j], &c[j]);
+      c[j] *= a.mag;
+      s[j] *= a.mag * a.sign;
+    }
+  }
+  const int total = a.heads[0] + a.heads[1];
+  for (int h = h0; h < total; h += a.split) {
+    const int k = h >= a.heads[0], hh = k ? h - a.heads[0] : h;
+    const long long in = b * a.xs[k][0] + t * a.xs[k][1] + hh * a.xs[k][2];
+    const long long out = b * a.ys[k][0] + t * a.ys[k][1] + hh * a.ys[k][2];
+    float x[VEC], y[VEC];
+    ld_unit<DT, VEC>(a.x[k], in + lo, x);
+    ld_unit<DT, VEC>(a.x[k], in + hi, y);
+    if (turn) {
+      if constexpr (NEAR) {
+        // neighbours: pair j is elements 2 j and 2 j + 1 of x and y together
+        float z[2 * VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          z[j] = x[j];
+          z[VEC + j] = y[j];
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float p = z[2 * j], q = z[2 * j + 1];
+          z[2 * j] = p * c[j] - q * s[j];
+          z[2 * j + 1] = q * c[j] + p * s[j];
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          x[j] = z[j];
+          y[j] = z[VEC + j];
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float p = x[j], q = y[j];
+          x[j] = p * c[j] - q * s[j];
+          y[j] = q * c[j] + p * s[j];
+        }
+      }
+    }
+    st_unit<DT, VEC>(a.y[k], out + lo, x);
+    st_unit<DT, VEC>(a.y[k], out + hi, y);
+  }
+}
+
+}  // namespace gdn
+
+extern "C" int gdn_rotary(const void* const* x, void* const* y, const long long* xs,
+                          const long long* ys, const int* heads, const void* positions,
+                          int pos_int64, long long pos_batch, const double* inv_freq, int B, int T,
+                          int D, int R, float magnitude, int interleaved, int inverse, int dtype,
+                          void* stream) {
+  const char* name = "gdn_rotary";
+  if (!x || !y || !xs || !ys || !heads)
+    return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": x, y, their strides and heads must be non-NULL");
+  if (B < 0 || T < 0 || heads[0] < 1 || heads[1] < 0)
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": sizes must be non-negative (heads[0] > 0)");
+  if (D < 2 || D > 512 || D % 2 || R < 2 || R > D || R % 2)
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": D and R must be even, 2 <= R <= D <= 512");
+  if (!gdn::dtype_ok(dtype))
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": unsupported dtype code");
+  if ((long long)heads[0] + heads[1] > (1 << 20) || (long long)B * T >= (1LL << 31))
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
+  if ((long long)B * T == 0) return GDN_OK;
+  if (!positions || !inv_freq || !x[0] || !y[0] || (heads[1] && (!x[1] || !y[1])))
+    return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": x, y, positions and inv_freq must be non-NULL");
+  const int two = heads[1] > 0 ? 2 : 1;
+  bool inplace = true;
+  for (int k = 0; k < two; ++k) {
+    const bool same = x[k] == y[k];
+    for (int i = 0; i < 3; ++i) {
+      if (xs[3 * k + i] < 0 || ys[3 * k + i] < 0)
+        return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": strides must be non-negative");
+      if (same && xs[3 * k + i] != ys[3 * k + i])
+        return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": in place x and y must have the same strides");
+    }
+    inplace = inplace && same;
+    if (same != (x[0] == y[0]))
+      return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": both tensors in place, or none");
+  }
+  if (two == 2 && y[0] == y[1])
+    return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": the two outputs must not be one");
+  // the widest units that divide both parts of a head: 16 bytes of each half, 2
+  // elements, or 1
+  const int full = dtype == GDN_DTYPE_F32 ? 4 : 8;
+  int vec = 1;
+  for (const int v : {full, 2})
+    if (vec == 1 && R % (2 * v) == 0 && D % (2 * v) == 0) vec = v;
+  gdn::RotaryArgs a{};
+  for (int k = 0; k < two; ++k) {
+    a.x[k] = x[k];
+    a.y[k] = y[k];
+    a.heads[k] = heads[k];
+    for (int i = 0; i < 3; ++i) {
+      a.xs[k][i] = xs[3 * k + i];
+      a.ys[k][i] = ys[3 * k + i];
+    }
+  }
+  a.pos = positions;
+  a.pos64 = pos_int64;
+  a.pos_batch = pos_batch;
+  a.freq = inv_freq;
+  a.T = T;
+  a.R = R;
+  a.units = D / (2 * vec);
+  a.per_wg = 256 / a.units;
+  a.rows = B * T;
+  a.inplace = inplace;
+  a.mag = magnitude;
+  a.sign = inverse ? -1.f : 1.f;
+  // groups of lanes per token: as many heads to a group as leave every CU eight
+  // workgroups, eight at most
+  const int total = heads[0] + heads[1];
+  const long long want = 8LL * gdn::device_cus() * a.per_wg;
+  long long split = (want + a.rows - 1) / a.rows;
+  if (split < (total + 7) / 8) split = (total + 7) / 8;
+  a.split = (int)(split < total ? split : total);
+  const long long wgs = ((long long)a.rows * a.split + a.per_wg - 1) / a.per_wg;
+  if (const int fit = gdn_host::check_lanes(name, wgs, 256)) return fit;
+  gdn_host::launch_begin();
+  auto st = static_cast<hipStream_t>(stream);
+#define GDN_ROT(TT, VV, NN)                                                                   \
+  if (dtype == TT && vec == VV && !interleaved == !NN) {                                      \
+    hipLaunchKernelGGL((gdn::rotary_kernel<TT, VV, NN>), dim3((unsigned)wgs), dim3(256), 0, st, a); \
+    return gdn_host::check_launch(name);                                                      \
+  }
+#define GDN_ROT_V(TT, FULL)                                                                   \
+  GDN_ROT(TT, FULL, false) GDN_ROT(TT, FULL, true) GDN_ROT(TT, 2, false) GDN_ROT(TT, 2, true) \
+  GDN_ROT(TT, 1, false) GDN_ROT(TT, 1, true)
+  GDN_ROT_V(GDN_DTYPE_BF16, 8)
+  GDN_ROT_V(GDN_DTYPE_F16, 8)
+  GDN_ROT_V(GDN_DTYPE_F32, 4)
+#undef GDN_ROT
+#undef GDN_ROT_V
+  return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": unsupported configuration");
+}

@@ -1,12 +1,15 @@
-"""Layer norm for MI355X (gfx950), forward and backward.
+"""Layer norm and root-mean-square norm for MI355X (gfx950), forward and backward.
 
-    y = (x - mean) / sqrt(var + eps) * weight + bias
+    layer_norm   y = (x - mean) / sqrt(var + eps) * weight + bias
+    rms_norm     y = h / sqrt(mean(h^2) + eps) * (weight + offset),  h = x [+ residual]
 
 over the last axis with the biased variance, in fp32 whatever x's type.  The
-weight and bias have the last axis' shape, or the last two's: every head's
-row by itself with parameters of its own (the norm of an attention's output).
-HIP kernels of ``csrc/gdn_norm.hip`` behind ``include/gdn_linear.h``; there is
-no fallback path.  The reference repository has no counterpart; the wrappers
+layer norm's weight and bias have the last axis' shape, or the last two's: every
+head's row by itself with parameters of its own (the norm of an attention's
+output).  The RMS norm also adds the residual stream and can leave its output in
+8 bits with a scale per row (``rms_norm_quant``).
+HIP kernels of ``csrc/gdn_norm.hip`` behind ``include/gdn_linear.h`` and of
+``csrc/gdn_rms.hip`` behind ``include/gdn_attn.h``; there is no fallback path.  The reference repository has no counterpart; the wrappers
 follow its kernel-library convention
 (python/avelang_kernels/amdgpu_gemm.py:458-494).
 """
@@ -18,9 +21,12 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .layer_ops import _dt, _ptr, _stream
+from .layer_ops import _DTYPES, _dt, _ptr, _stream
 
-__all__ = ["layer_norm", "layer_norm_fwd_save", "layer_norm_bwd"]
+_CODES = {torch.float8_e4m3fn: _native.GDN_DTYPE_E4M3, torch.int8: _native.GDN_DTYPE_I8}
+
+__all__ = ["layer_norm", "layer_norm_fwd_save", "layer_norm_bwd",
+           "rms_norm", "rms_norm_quant", "rms_norm_fwd_save", "rms_norm_bwd"]
 
 
 def _args(x, weight, bias, name):
@@ -175,3 +181,184 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
             raise ValueError("layer_norm: out is not supported when gradients are required.")
         return _LayerNorm.apply(x, weight, bias, eps)
     return _fwd(_args(x, weight, bias, "layer_norm"), eps, "layer_norm", out)[0]
+
+
+def _rms_args(x, weight, residual, name):
+    """Checked, contiguous x, weight and residual, with rows, D and type codes."""
+    if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"{name}: x must be a tensor with a last axis of at least 1.")
+    dt = rdt = _dt(x, name, "x")
+    wdt, dev, D = dt, x.device, x.shape[-1]
+    if dev.type != "cuda":
+        raise ValueError(f"{name}: tensors must be on a ROCm (cuda) device, got {dev}.")
+    if weight is not None:
+        if not isinstance(weight, torch.Tensor) or weight.shape != (D,) or weight.device != dev:
+            raise ValueError(f"{name}: weight must be a tensor of shape ({D},) on {dev}.")
+        wdt = _dt(weight, name, "weight")
+        weight = weight.contiguous()
+    if residual is not None:
+        if (not isinstance(residual, torch.Tensor) or residual.shape != x.shape
+                or residual.device != dev or residual.dtype not in (x.dtype, torch.float32)):
+            raise ValueError(f"{name}: residual must be a tensor of x's shape {tuple(x.shape)} and "
+                             f"type or torch.float32 on {dev}.")
+        rdt = _DTYPES[residual.dtype]
+        residual = residual.contiguous()
+    return x.contiguous(), weight, residual, x.numel() // D, D, dt, rdt, wdt
+
+
+def _rms_out(t, like, name, what):
+    if t is None:
+        return torch.empty_like(like)
+    if (not isinstance(t, torch.Tensor) or t.shape != like.shape or t.dtype != like.dtype
+            or t.device != like.device or not t.is_contiguous()):
+        raise ValueError(f"{name}: {what} must be a contiguous {like.dtype} tensor of shape "
+                         f"{tuple(like.shape)} on {like.device}.")
+    return t
+
+
+def _rms_fwd(args, eps, offset, name, out=None, residual_out=None, save=False, code=None):
+    x, weight, residual, rows, D, dt, rdt, wdt = args
+    if residual is None and residual_out is not None:
+        raise ValueError(f"{name}: residual_out needs a residual.")
+    y = _rms_out(out, x, name, "out") if code is None else torch.empty_like(x, dtype=code)
+    h = None if residual is None else _rms_out(residual_out, residual, name, "residual_out")
+    dev = x.device
+    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if save else None
+    scale = None if code is None else torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    _native.check(_native.on_device(
+        dev, _native.lib().gdn_rms_norm_fwd, x.data_ptr(), _ptr(residual), _ptr(weight), y.data_ptr(),
+        _ptr(h), _ptr(rstd), _ptr(scale), rows, D, float(eps), float(offset), dt, rdt, wdt,
+        dt if code is None else _CODES[code], _stream(dev)), name)
+    return y, h, rstd, scale
+
+
+def rms_norm_fwd_save(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6, *,
+                      residual: Optional[torch.Tensor] = None, offset: float = 0.0):
+    """Training forward: ``(y, h, rstd)``, h (x itself, contiguous, without a
+    residual) and rstd (fp32, one per row) being what ``rms_norm_bwd`` takes."""
+    name = "rms_norm_fwd_save"
+    args = _rms_args(x, weight, residual, name)
+    y, h, rstd, _ = _rms_fwd(args, eps, offset, name, save=True)
+    return y, args[0] if h is None else h, rstd
+
+
+def rms_norm_bwd(h: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Tensor,
+                 rstd: torch.Tensor, dh: Optional[torch.Tensor] = None, *, offset: float = 0.0):
+    """Gradients of ``rms_norm``: ``(dx, dweight, dresidual)`` from dy = dL/dy
+    (its type is x's) and dh = dL/dh (h's type; None where nothing else reads h).
+
+    dresidual is dx itself where h has x's type; with an fp32 residual the same
+    values in fp32.  dweight (None without a weight) has the weight's type and is
+    summed over the rows in fp32 in a fixed order.
+    """
+    name = "rms_norm_bwd"
+    if not isinstance(dy, torch.Tensor) or not isinstance(h, torch.Tensor):
+        raise ValueError(f"{name}: h and dy must be tensors.")
+    dy, weight, h, *sizes = _rms_args(dy, weight, h, name)
+    dx, dw, dr = _rms_bwd(dy, weight, h, sizes, rstd, dh, offset, weight is not None, True, name)
+    return dx, dw, dr
+
+
+def _rms_bwd(dy, weight, h, sizes, rstd, dh, offset, want_w, want_r, name):
+    """On ``_rms_args``' (dy, weight, h, sizes)."""
+    rows, D, dt, hdt, wdt = sizes
+    dev = dy.device
+    if (not isinstance(rstd, torch.Tensor) or rstd.shape != (rows,) or rstd.device != dev
+            or rstd.dtype is not torch.float32):
+        raise ValueError(f"{name}: rstd must be torch.float32 of shape {(rows,)} on {dev}.")
+    if dh is not None:
+        if (not isinstance(dh, torch.Tensor) or dh.shape != h.shape or dh.dtype != h.dtype
+                or dh.device != dev):
+            raise ValueError(f"{name}: dh must be a {h.dtype} tensor of shape {tuple(h.shape)} on {dev}.")
+        dh = dh.contiguous()
+    rstd = rstd.contiguous()
+    dx = torch.empty_like(dy)
+    dr = torch.empty_like(h) if want_r and hdt != dt else None
+    dw = torch.empty_like(weight) if want_w else None
+    lib = _native.lib()
+    ws, nbytes = None, 0
+    if want_w:
+        nbytes = _native.on_device(dev, lib.gdn_rms_norm_bwd_workspace_bytes, rows, D, dt)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _native.check(_native.on_device(
+        dev, lib.gdn_rms_norm_bwd, h.data_ptr(), _ptr(weight), dy.data_ptr(), _ptr(dh),
+        rstd.data_ptr(), dx.data_ptr(), _ptr(dr), _ptr(dw), rows, D, float(offset), dt, hdt, wdt,
+        _ptr(ws), nbytes, _stream(dev)), name)
+    return dx, dw, dr if dr is not None else dx if want_r else None
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps, offset):
+        args = _rms_args(x, weight, residual, "rms_norm")
+        y, h, rstd, _ = _rms_fwd(args, eps, offset, "rms_norm", save=True)
+        ctx.save_for_backward(args[0] if h is None else h, args[1], rstd)
+        ctx.offset, ctx.x_type = offset, x.dtype
+        ctx.set_materialize_grads(False)
+        return y if h is None else (y, h)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight, rstd = ctx.saved_tensors
+        name = "rms_norm"
+        want_x, want_w, want_r = ctx.needs_input_grad[:3]
+        if dy is None:
+            # (y unused: h's gradient alone)
+            dr = dh if want_r else None
+            dx = None if not want_x or dh is None else dh.to(ctx.x_type)
+            dw = torch.zeros_like(weight) if want_w and weight is not None else None
+            return dx, dw, dr, None, None
+        # (checked again: a hook on saved tensors may return others of another layout)
+        dy, weight, h, *sizes = _rms_args(dy, weight, h, name)
+        dx, dw, dr = _rms_bwd(dy, weight, h, sizes, rstd, dh, ctx.offset,
+                              want_w and weight is not None, want_r, name)
+        return dx, dw, dr, None, None
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6, *,
+             residual: Optional[torch.Tensor] = None, offset: float = 0.0,
+             out: Optional[torch.Tensor] = None, residual_out: Optional[torch.Tensor] = None):
+    """RMS norm of ``x`` (fp32, bf16 or fp16) over its last axis:
+    ``y = h * rsqrt(mean(h^2, -1) + eps) * (weight + offset)``.
+
+    Without a ``residual`` h is x, and y is returned.  With one (x's shape; x's
+    type or fp32) ``h = x + residual`` in the residual's type, and ``(y, h)`` is
+    returned: h is what the next layer adds to, and y is the norm of h as
+    returned.  ``weight`` (optional, any of the three types) has the last axis'
+    shape; ``offset`` 1 is for weights stored about zero.  ``out`` (may be x)
+    and ``residual_out`` (may be the residual, or x where the types are the same)
+    avoid allocation; both contiguous.
+
+    Differentiable in x, weight and residual (``rms_norm_bwd``, the gradient of h
+    included); the forward then keeps h and 4 bytes per row.
+    """
+    if torch.is_grad_enabled() and (_grad(x) or _grad(weight) or _grad(residual)):
+        if out is not None or residual_out is not None:
+            raise ValueError("rms_norm: out / residual_out are not supported when gradients are "
+                             "required.")
+        return _RmsNorm.apply(x, weight, residual, eps, offset)
+    y, h, _, _ = _rms_fwd(_rms_args(x, weight, residual, "rms_norm"), eps, offset, "rms_norm", out,
+                          residual_out)
+    return y if h is None else (y, h)
+
+
+def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6, *,
+                   residual: Optional[torch.Tensor] = None, offset: float = 0.0,
+                   dtype: torch.dtype = torch.float8_e4m3fn,
+                   residual_out: Optional[torch.Tensor] = None):
+    """``rms_norm`` with its output in 8 bits: ``(codes, scale)``, with a residual
+    ``(codes, scale, h)``; y is ``codes * scale[..., None]``.
+
+    ``dtype`` is torch.float8_e4m3fn (M = 448) or torch.int8 (M = 127); scale
+    (fp32, one per row) is max |y| / M and codes are y / scale, rounded to nearest
+    with ties to even: half a step off y (e4m3 2^-4 of it, int8 scale / 2).  A row of
+    zeros has scale 0; one of less than 2^-100 is stored as if it reached that; one
+    that is not finite has a scale of NaN.  Not differentiable.
+    """
+    name = "rms_norm_quant"
+    if dtype not in _CODES:
+        raise ValueError(f"{name}: dtype must be torch.float8_e4m3fn or torch.int8, got {dtype}.")
+    y, h, _, scale = _rms_fwd(_rms_args(x, weight, residual, name), eps, offset, name, None,
+                              residual_out, code=dtype)
+    return (y, scale) if h is None else (y, scale, h)
