@@ -19,6 +19,8 @@
 // the lengths (read on the device: nothing here depends on a host copy of them).
 // A share that holds a whole (sequence, kv-head) writes its output; parts leave
 // m, the sum and o in the workspace and a second launch joins them.
+#include <type_traits>
+
 #include "gdn_bits8.h"
 #include "gdn_norm_rows.h"
 
@@ -42,6 +44,7 @@ struct PagedAttnArgs {
   int4* desc;
   int N, L, Hq, Hkv, G, R, RG, rows;   // R = L G rows per kv-head in RG groups of at most `rows`
   int num_pages, page, cap, window;
+  int by_item;    // desc has an entry per (sequence, kv-head, group of rows), not per workgroup
   float scale2;   // scale log2(e)
 };
 
@@ -57,14 +60,34 @@ __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int n) {
   return s;
 }
 
+// x and its value 16 (32) lanes further, in every lane of both: v_permlane swaps
+// of two copies, no LDS.
+typedef uint32_t u32x2s __attribute__((ext_vector_type(2)));
+template <int OFF>
+__device__ __forceinline__ void both(float x, float& a, float& b) {
+  const uint32_t u = __float_as_uint(x);
+  u32x2s r;
+  if constexpr (OFF == 16) r = __builtin_bit_cast(u32x2s, __builtin_amdgcn_permlane16_swap(u, u, false, false));
+  else r = __builtin_bit_cast(u32x2s, __builtin_amdgcn_permlane32_swap(u, u, false, false));
+  const uint32_t lo = r[0], hi = r[1];
+  a = __uint_as_float(lo);
+  b = __uint_as_float(hi);
+}
+// Largest value, sum over the four groups of 16 lanes.
 __device__ __forceinline__ float xmax16(float x) {
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+  float a, b;
+  both<16>(x, a, b);
+  both<32>(fmaxf(a, b), a, b);
+  return fmaxf(a, b);
 }
 __device__ __forceinline__ float xsum16(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+  float a, b;
+  both<16>(x, a, b);
+  both<32>(a + b, a, b);
+  return a + b;
 }
+// 2^x in one instruction (results under 2^-126 are 0).
+__device__ __forceinline__ float exp2i(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // What the MFMAs run in: bf16 over a bf16 cache; fp16 else (8-bit codes are
 // exact there, and two conversions cheaper than in bf16).
@@ -78,10 +101,24 @@ __device__ __forceinline__ uint16_t from_f(float f) {
   if constexpr (BF) return f2bf(f);
   else return f2h(f);
 }
-template <bool BF>
-__device__ __forceinline__ float to_f(uint16_t h) {
-  if constexpr (BF) return bf2f(h);
-  else return static_cast<float>(__builtin_bit_cast(_Float16, h));
+// Eight values as an operand, and what it leaves of them as another.
+template <bool BF, bool LO>
+__device__ __forceinline__ void operands(const f32x4 (&p)[2], u16x8& hi, u16x8& lo) {
+  u16x4 h[2], l[2];
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    if constexpr (BF) {
+      split_bf4(p[s], h[s], l[s]);
+    } else {
+      h[s] = f2h4(p[s]);
+      if constexpr (LO) l[s] = f2h4(p[s] - __builtin_convertvector(__builtin_bit_cast(f16x4, h[s]), f32x4));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    hi[i] = h[i / 4][i % 4];
+    if constexpr (LO) lo[i] = l[i / 4][i % 4];
+  }
 }
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -118,7 +155,7 @@ __device__ __forceinline__ u16x8 codes_operand(uint32_t w0, uint32_t w1) {
 
 // RW: waves of a workgroup that take rows apart (16 each); the others take tokens apart.
 template <int QT, int CT, int D, int RW>
-__global__ __launch_bounds__(256, D == 256 && (CT == GDN_DTYPE_BF16 || CT == GDN_DTYPE_F16) ? 1 : 2)
+__global__ __launch_bounds__(256, D == 256 ? 1 : 2)
 void paged_attn_kernel(PagedAttnArgs a) {
   constexpr bool BF = CT == GDN_DTYPE_BF16;                        // bf16 products
   constexpr bool C8 = CT == GDN_DTYPE_E4M3 || CT == GDN_DTYPE_I8;  // codes with scales
@@ -164,7 +201,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
     share = (total + gridDim.x - 1) / gridDim.x;
     u0 = min((int)blockIdx.x * share, total);
     u1 = min(u0 + share, total);
-    if (tid == 0) a.desc[blockIdx.x] = int4{0, 0, 0, 0};
+    if (tid == 0 && !a.by_item) a.desc[blockIdx.x] = int4{0, 0, 0, 0};
     if (u0 >= u1) return;
     int at = incl - sum;
     if (at * HG <= u0 && u0 < incl * HG) {
@@ -262,7 +299,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
         const int off = min(c16, valid(it, s) - 1) * ROW + 16 * g;
 #pragma unroll
         for (int k = 0; k < KL; ++k) kr[s][k] = *reinterpret_cast<const u32x4w*>(p + (off + 64 * k));
-        if constexpr (C8) kscale[s] = *reinterpret_cast<const f32x4*>(a.ks + row + 4 * g);
+        if constexpr (C8) kscale[s] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(a.ks + row) + 16u * g);
       }
     };
     auto load_v = [&](const long long (&rv)[2], int it) {
@@ -290,7 +327,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
             }
           }
         }
-        if constexpr (C8) vscale[s] = *reinterpret_cast<const f32x4*>(a.vs + row + 4 * g);
+        if constexpr (C8) vscale[s] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(a.vs + row) + 16u * g);
       }
     };
 
@@ -367,70 +404,76 @@ void paged_attn_kernel(PagedAttnArgs a) {
         }
       }
       if (__any(mx > m) || (C8 && grow != 1.f)) {
-        const float f = exp2f(m - ref);   // (m = -inf: 0)
+        const float f = exp2i(m - ref);   // (m = -inf: 0)
         sum *= f;
 #pragma unroll
         for (int j = 0; j < E; ++j) acc[j] *= f * grow;
         m = mx;
       }
-      u16x8 hi, lo;
+      f32x4 p[2];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        float p = exp2f(S[i / 4][i % 4] - ref);
-        sum += p;
+        float x = exp2i(S[i / 4][i % 4] - ref);
+        sum += x;
         if constexpr (C8) {
-          p *= vscale[i / 4][i % 4] * vinv;
-          if (part && !seen[i / 4][i % 4]) p = 0.f;
+          x *= vscale[i / 4][i % 4] * vinv;
+          if (part && !seen[i / 4][i % 4]) x = 0.f;
         }
-        hi[i] = from_f<BF>(p);
-        if constexpr (LO) lo[i] = from_f<BF>(p - to_f<BF>(hi[i]));
+        p[i / 4][i % 4] = x;
       }
-      u16x8 ones;
-      if (mixed) {
+      u16x8 hi, lo;
+      operands<BF, LO>(p, hi, lo);
+      // O^T += V^T P^T;  with `mixed` a value that is not finite reaches only the rows that see its token
+      auto add_v = [&](auto some) {
+        constexpr bool MIX = decltype(some)::value;
+        u16x8 ones;
+        if constexpr (MIX) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) ones[i] = seen[i / 4][i % 4] ? from_f<BF>(1.f) : (uint16_t)0;
-      }
-#pragma unroll
-      for (int j = 0; j < E; ++j) {
-        u32x4w vf;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          if constexpr (CT == GDN_DTYPE_E4M3) {
-            const uint32_t w = __builtin_amdgcn_perm(vr[2 * t + 1][j / 4], vr[2 * t][j / 4],
-                                                     j % 4 < 2 ? 0x05010400u : 0x07030602u);
-            vf[t] = j % 2 ? e4m3_pair<true>(w) : e4m3_pair<false>(w);
-          } else if constexpr (CT == GDN_DTYPE_I8) {
-            constexpr uint32_t sel[4] = {0x0c040c00u, 0x0c050c01u, 0x0c060c02u, 0x0c070c03u};
-            vf[t] = i8_pair(__builtin_amdgcn_perm(vr[2 * t + 1][j / 4] ^ 0x80808080u,
-                                                  vr[2 * t][j / 4] ^ 0x80808080u, sel[j % 4]));
-          } else {
-            vf[t] = __builtin_amdgcn_perm(vr[2 * t + 1][j / 2], vr[2 * t][j / 2],
-                                          j % 2 ? 0x07060302u : 0x05040100u);
-          }
+          for (int i = 0; i < 8; ++i) ones[i] = seen[i / 4][i % 4] ? from_f<BF>(1.f) : (uint16_t)0;
         }
-        u16x8 v = __builtin_bit_cast(u16x8, vf);
-        if (mixed) {
-          // a value that is not finite reaches only the rows that see its token
-          constexpr uint16_t kExp = BF ? 0x7f80 : 0x7c00;
-          u16x8 ind;
-          bool any = false;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const bool x = (v[i] & kExp) == kExp;
-            any |= x;
-            ind[i] = x ? from_f<BF>(1.f) : (uint16_t)0;
-            v[i] = x ? (uint16_t)0 : v[i];
-          }
-          if (__any(any)) {
-            const f32x4 hit = mfma_t<BF>(ind, ones, zero4());
+        for (int j = 0; j < E; ++j) {
+          u32x4w vf;
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (hit[r] > 0.f) acc[j][r] = __builtin_nanf("");
+          for (int t = 0; t < 4; ++t) {
+            if constexpr (CT == GDN_DTYPE_E4M3) {
+              const uint32_t w = __builtin_amdgcn_perm(vr[2 * t + 1][j / 4], vr[2 * t][j / 4],
+                                                       j % 4 < 2 ? 0x05010400u : 0x07030602u);
+              vf[t] = j % 2 ? e4m3_pair<true>(w) : e4m3_pair<false>(w);
+            } else if constexpr (CT == GDN_DTYPE_I8) {
+              constexpr uint32_t sel[4] = {0x0c040c00u, 0x0c050c01u, 0x0c060c02u, 0x0c070c03u};
+              vf[t] = i8_pair(__builtin_amdgcn_perm(vr[2 * t + 1][j / 4] ^ 0x80808080u,
+                                                    vr[2 * t][j / 4] ^ 0x80808080u, sel[j % 4]));
+            } else {
+              vf[t] = __builtin_amdgcn_perm(vr[2 * t + 1][j / 2], vr[2 * t][j / 2],
+                                            j % 2 ? 0x07060302u : 0x05040100u);
+            }
           }
+          u16x8 v = __builtin_bit_cast(u16x8, vf);
+          if constexpr (MIX) {
+            constexpr uint16_t kExp = BF ? 0x7f80 : 0x7c00;
+            u16x8 ind;
+            bool any = false;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const bool x = (v[i] & kExp) == kExp;
+              any |= x;
+              ind[i] = x ? from_f<BF>(1.f) : (uint16_t)0;
+              v[i] = x ? (uint16_t)0 : v[i];
+            }
+            if (__any(any)) {
+              const f32x4 hit = mfma_t<BF>(ind, ones, zero4());
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (hit[r] > 0.f) acc[j][r] = __builtin_nanf("");
+            }
+          }
+          acc[j] = mfma_t<BF>(v, hi, acc[j]);
+          if constexpr (LO) acc[j] = mfma_t<BF>(v, lo, acc[j]);
         }
-        acc[j] = mfma_t<BF>(v, hi, acc[j]);
-        if constexpr (LO) acc[j] = mfma_t<BF>(v, lo, acc[j]);
-      }
+      };
+      if (mixed) add_v(std::true_type{});
+      else add_v(std::false_type{});
       if (it + 1 < tiles) {
         rv[0] = rows[0];
         rv[1] = rows[1];
@@ -470,7 +513,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
       f32x4 o = zero4();
 #pragma unroll
       for (int w = 0; w < TW; ++w) {
-        const float f = exp2f(sm[w0 + w * RW][c] - ref);
+        const float f = exp2i(sm[w0 + w * RW][c] - ref);
         s += f * sl[w0 + w * RW][c];
         o += f * *reinterpret_cast<const f32x4*>(&buf[w0 + w * RW][c][d]);
       }
@@ -491,8 +534,10 @@ void paged_attn_kernel(PagedAttnArgs a) {
         }
       }
     }
-    if (!whole && start == 0 && tid == 0)
-      a.desc[blockIdx.x] = int4{n, item, slot, 1 + (sp.units - len + share - 1) / share};
+    // what the joining launch has to do: {sequence, item, first part's slot, parts}
+    if (start == 0 && tid == 0 && (!whole || a.by_item))
+      a.desc[a.by_item ? n * HG + item : blockIdx.x] =
+          int4{n, item, slot, whole ? 0 : 1 + (sp.units - len + share - 1) / share};
     u += len;
     if (item == HG - 1 && start + len == sp.units) {
       prefix += sp.units;
@@ -502,48 +547,67 @@ void paged_attn_kernel(PagedAttnArgs a) {
   }
 }
 
-// Parts of one (sequence, kv-head) joined: block (w, row, 64 columns) takes the one
-// that begins in workgroup w's share and ends in another's.
-template <int QT, int D>
-__global__ __launch_bounds__(256) void paged_attn_join_kernel(PagedAttnArgs a) {
-  __shared__ float red[4];
-  __shared__ float acc[4][64];
+// Parts of one (sequence, kv-head) joined: block (entry of desc, row).  D / 4 lanes
+// hold a row of a part, NT / (D / 4) parts are added at a time.
+constexpr int kMostParts = 1024;   // workgroups at most
+template <int QT, int D, int NT>
+__global__ __launch_bounds__(NT) void paged_attn_join_kernel(PagedAttnArgs a) {
+  constexpr int LP = D / 4, GR = NT / LP, NW = NT / 64;
+  __shared__ float w[kMostParts];
+  __shared__ float red[2][NW];
+  __shared__ f32x4 acc[GR][LP];
   const int4 ds = a.desc[blockIdx.x];
-  const int pieces = ds.w;
-  if (pieces == 0) return;
+  const int parts = ds.w;
+  if (parts == 0) return;
   const int kvh = ds.y / a.RG, rg = ds.y % a.RG, row = blockIdx.y;
   const int orow = rg * a.rows + row;
   if (orow >= a.R) return;
-  const int tid = threadIdx.x, col = tid % 64, grp = tid / 64, d = blockIdx.z * 64 + col;
+  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, col = tid % LP, grp = tid / LP;
   const size_t each = (size_t)a.rows * (D + 2);
-  // piece p's part: its workgroup's first, but for the one that begins here
-  auto at = [&](int p) { return a.part + (p == 0 ? ds.z : 2 * (blockIdx.x + p)) * each; };
+  // part p: its workgroup's first, but for the one that begins here
+  const int wg = ds.z / 2;
+  auto at = [&](int p) { return a.part + (p == 0 ? ds.z : 2 * (wg + p)) * each; };
   float M = -INFINITY;
-  for (int p = tid; p < pieces; p += 256) M = fmaxf(M, at(p)[a.rows * D + row]);
+  for (int p = tid; p < parts; p += NT) {
+    const float m = at(p)[a.rows * D + row];
+    w[p] = m;
+    M = fmaxf(M, m);
+  }
 #pragma unroll
   for (int off = 1; off < 64; off *= 2) M = fmaxf(M, __shfl_xor(M, off));
-  if (col == 0) red[grp] = M;
+  if (lane == 0) red[0][wave] = M;
   __syncthreads();
-  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+#pragma unroll
+  for (int i = 0; i < NW; ++i) M = fmaxf(M, red[0][i]);
   const float ref = M == -INFINITY ? 0.f : M;
-  float s = 0.f, o = 0.f;
-#pragma unroll 4
-  for (int p = grp; p < pieces; p += 4) {
-    const float* x = at(p);
-    const float f = exp2f(x[a.rows * D + row] - ref);
-    s += f * x[a.rows * (D + 1) + row];
-    o += f * x[row * D + d];
+  float s = 0.f;
+  for (int p = tid; p < parts; p += NT) {
+    const float f = exp2i(w[p] - ref);
+    w[p] = f;
+    s += f * at(p)[a.rows * (D + 1) + row];
   }
+#pragma unroll
+  for (int off = 1; off < 64; off *= 2) s += __shfl_xor(s, off);
+  if (lane == 0) red[1][wave] = s;
+  __syncthreads();
+  f32x4 o = zero4();
+#pragma unroll 8
+  for (int p = grp; p < parts; p += GR) o += w[p] * *reinterpret_cast<const f32x4*>(at(p) + row * D + 4 * col);
   acc[grp][col] = o;
   __syncthreads();
-  if (col == 0) red[grp] = s;
-  __syncthreads();
-  if (grp) return;
-  o = acc[0][col] + acc[1][col] + acc[2][col] + acc[3][col];
-  s = red[0] + red[1] + red[2] + red[3];
+  if (tid >= LP) return;
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) s += red[1][i];
+#pragma unroll
+  for (int i = 1; i < GR; ++i) o += acc[i][col];
+  o *= s == 0.f ? 0.f : 1.f / s;
   const long long out = ((long long)ds.x * a.L + orow / a.G) * a.Hq + kvh * a.G + orow % a.G;
-  ste<QT>(a.o, out * D + d, s == 0.f ? 0.f : o / s);
-  if (a.lse && d == 0) a.lse[out] = s == 0.f ? -INFINITY : (M + log2f(s)) * 0.69314718055994530942f;
+  u16x4 h;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) h[j] = Elt<QT>::from_f(o[j]);
+  *reinterpret_cast<u16x4*>(static_cast<uint16_t*>(a.o) + out * D + 4 * col) = h;
+  if (a.lse && tid == 0) a.lse[out] = s == 0.f ? -INFINITY : (M + log2f(s)) * 0.69314718055994530942f;
 }
 
 }  // namespace gdn
@@ -558,7 +622,8 @@ namespace {
 // Workgroups, and how the rows of a kv-head are laid over their waves.
 struct AttnPlan {
   int rw, rg, rows;
-  long long wgs;
+  long long wgs, items;
+  bool split;   // some work may be cut
   size_t desc, bytes;
 };
 int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_length, AttnPlan& p) {
@@ -578,7 +643,10 @@ int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_le
   const long long most = (units ? units : 1) * N * Hkv * p.rg;
   if (most >= (1LL << 30))
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
+  p.items = (long long)N * Hkv * p.rg;
+  p.split = units > 1;
   p.wgs = 2LL * gdn::device_cus();
+  if (p.wgs > gdn::kMostParts) p.wgs = gdn::kMostParts;
   if (p.wgs > most) p.wgs = most;
   p.desc = (size_t)p.wgs * 16;
   p.bytes = p.desc + (size_t)p.wgs * 2 * p.rows * (D + 2) * sizeof(float);
@@ -661,6 +729,7 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long long q_seq, long long q_to
   a.num_pages = num_pages;
   a.page = page_size;
   a.cap = max_length;
+  a.by_item = p.items <= p.wgs;
   a.window = window > (1 << 30) ? 1 << 30 : window;
   a.scale2 = scale * 1.44269504088896340736f;
   auto st = static_cast<hipStream_t>(stream);
@@ -684,10 +753,16 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long long q_seq, long long q_to
 #undef GDN_PA
   if (!done)
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": the cache must be of q's type or have 8 bits");
-  const dim3 grid((unsigned)p.wgs, (unsigned)p.rows, (unsigned)(D / 64));
+  if (!p.split) return gdn_host::check_launch(name);
+  const dim3 grid((unsigned)(a.by_item ? p.items : p.wgs), (unsigned)p.rows);
+  // few outputs of many parts each: a CU's worth of lanes to each (131072 tokens of
+  // one sequence, 256 parts: see the kernel's figures)
+  const bool wide = (long long)grid.x * grid.y <= gdn::device_cus();
 #define GDN_PJ(QQ, DD)                                                                            \
-  if (dtype == QQ && D == DD)                                                                     \
-    hipLaunchKernelGGL((gdn::paged_attn_join_kernel<QQ, DD>), grid, dim3(256), 0, st, a);
+  if (dtype == QQ && D == DD) {                                                                   \
+    if (wide) hipLaunchKernelGGL((gdn::paged_attn_join_kernel<QQ, DD, 1024>), grid, dim3(1024), 0, st, a); \
+    else hipLaunchKernelGGL((gdn::paged_attn_join_kernel<QQ, DD, 256>), grid, dim3(256), 0, st, a); \
+  }
   GDN_PJ(GDN_DTYPE_BF16, 64) GDN_PJ(GDN_DTYPE_BF16, 128) GDN_PJ(GDN_DTYPE_BF16, 256)
   GDN_PJ(GDN_DTYPE_F16, 64) GDN_PJ(GDN_DTYPE_F16, 128) GDN_PJ(GDN_DTYPE_F16, 256)
 #undef GDN_PJ
