@@ -26,7 +26,7 @@
 
 namespace gdn {
 
-constexpr int kUnit = 128;   // tokens of a unit of work
+constexpr int kUnit = 128;   // least tokens of a unit of work
 
 struct PagedAttnArgs {
   const void* q;
@@ -52,11 +52,12 @@ struct PagedAttnArgs {
 struct Span {
   int lo, hi, units;
 };
+template <int UNIT>
 __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int n) {
   Span s;
   s.hi = min(max(a.lens[n], 0), a.cap);
   s.lo = a.window > 0 ? max(0, s.hi - a.L + 1 - a.window) & ~15 : 0;
-  s.units = max(1, (s.hi - s.lo + kUnit - 1) / kUnit);
+  s.units = max(1, (s.hi - s.lo + UNIT - 1) / UNIT);
   return s;
 }
 
@@ -86,6 +87,19 @@ __device__ __forceinline__ float xsum16(float x) {
   both<32>(a + b, a, b);
   return a + b;
 }
+// The value of lane R of each four.
+template <int R>
+__device__ __forceinline__ float of_four(float x) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), R * 0x55, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float of_four(float x, int r) {
+  return r == 0 ? of_four<0>(x) : r == 1 ? of_four<1>(x) : r == 2 ? of_four<2>(x) : of_four<3>(x);
+}
+// Largest value of each four lanes.
+__device__ __forceinline__ float xmax4(float x) {
+  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xb1, 0xf, 0xf, true)));
+  return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4e, 0xf, 0xf, true)));
+}
 // 2^x in one instruction (results under 2^-126 are 0).
 __device__ __forceinline__ float exp2i(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -103,15 +117,17 @@ __device__ __forceinline__ uint16_t from_f(float f) {
 }
 // Eight values as an operand, and what it leaves of them as another.
 template <bool BF, bool LO>
-__device__ __forceinline__ void operands(const f32x4 (&p)[2], u16x8& hi, u16x8& lo) {
+__device__ __forceinline__ void operands(f32x4 p, f32x4 q, u16x8& hi, u16x8& lo) {
   u16x4 h[2], l[2];
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    if constexpr (BF) {
-      split_bf4(p[s], h[s], l[s]);
-    } else {
-      h[s] = f2h4(p[s]);
-      if constexpr (LO) l[s] = f2h4(p[s] - __builtin_convertvector(__builtin_bit_cast(f16x4, h[s]), f32x4));
+  if constexpr (BF) {
+    split_bf4(p, h[0], l[0]);
+    split_bf4(q, h[1], l[1]);
+  } else {
+    h[0] = f2h4(p);
+    h[1] = f2h4(q);
+    if constexpr (LO) {
+      l[0] = f2h4(p - __builtin_convertvector(__builtin_bit_cast(f16x4, h[0]), f32x4));
+      l[1] = f2h4(q - __builtin_convertvector(__builtin_bit_cast(f16x4, h[1]), f32x4));
     }
   }
 #pragma unroll
@@ -153,6 +169,16 @@ __device__ __forceinline__ u16x8 codes_operand(uint32_t w0, uint32_t w1) {
   return __builtin_bit_cast(u16x8, r);
 }
 
+// Sixteens of tokens that a wave takes at a time, by the bytes of a row: 8 KiB of K and
+// as much of V on their way at once (16 KiB where rows are 512 bytes).  An e4m3 cache of
+// 128 elements, 256 sequences of 4.2 thousand tokens: 415 us, 430 with two sixteens.
+__host__ __device__ constexpr int sixteens(int row_bytes) { return row_bytes <= 128 ? 4 : 2; }
+// Tokens of a unit of work: a step of all the waves that take tokens apart.
+__host__ __device__ constexpr int unit_of(int row_bytes, int rw) {
+  const int t = 16 * sixteens(row_bytes) * (4 / rw);
+  return t > kUnit ? t : kUnit;
+}
+
 // RW: waves of a workgroup that take rows apart (16 each); the others take tokens apart.
 template <int QT, int CT, int D, int RW>
 __global__ __launch_bounds__(256, D == 256 ? 1 : 2)
@@ -160,11 +186,12 @@ void paged_attn_kernel(PagedAttnArgs a) {
   constexpr bool BF = CT == GDN_DTYPE_BF16;                        // bf16 products
   constexpr bool C8 = CT == GDN_DTYPE_E4M3 || CT == GDN_DTYPE_I8;  // codes with scales
   constexpr int ES = C8 ? 1 : 2, ROW = D * ES;                     // bytes of an element, of a row
-  constexpr int TW = 4 / RW;                                       // waves that take tokens apart
+  constexpr int TW = 4 / RW, UNIT = unit_of(ROW, RW);                                       // waves that take tokens apart
   constexpr int KL = ROW / 64;                                     // 16-byte pieces of K per lane and 16 tokens
   constexpr int E = D / 16;                                        // elements of V per lane and token
   constexpr int VD = E * ES / 4;                                   // words of them
   constexpr int CH = E * ES > 16 ? 16 / ES : E;                    // elements of one piece
+  constexpr int NS = sixteens(ROW), TT = 16 * NS;                  // tokens that a wave takes at a time
   constexpr bool LO = BF || QT == GDN_DTYPE_F16;   // P in two parts: 2^-9 (bf16), 2^-12 of one would show in o
   __shared__ float buf[4][16][D + 4];
   __shared__ float sm[4][16], sl[4][16];
@@ -182,7 +209,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
   {
     const int per = (a.N + 255) / 256, first = tid * per, last = min(first + per, a.N);
     int sum = 0;
-    for (int i = first; i < last; ++i) sum += span_of(a, i).units;
+    for (int i = first; i < last; ++i) sum += span_of<UNIT>(a, i).units;
     int incl = sum;
 #pragma unroll
     for (int off = 1; off < 64; off *= 2) {
@@ -207,7 +234,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
     if (at * HG <= u0 && u0 < incl * HG) {
       int i = first;
       for (;; ++i) {
-        const int un = span_of(a, i).units;
+        const int un = span_of<UNIT>(a, i).units;
         if (u0 < (at + un) * HG) break;
         at += un;
       }
@@ -220,11 +247,11 @@ void paged_attn_kernel(PagedAttnArgs a) {
   }
 
   for (int u = u0; u < u1;) {
-    const Span sp = span_of(a, n);
+    const Span sp = span_of<UNIT>(a, n);
     const int rel = u - prefix * HG, item = rel / sp.units, start = rel % sp.units;
     const int len = min(sp.units - start, u1 - u);
     const int kvh = item / a.RG, rg = item % a.RG;
-    const int t0 = sp.lo + start * kUnit, t1 = min(t0 + len * kUnit, sp.hi);
+    const int t0 = sp.lo + start * UNIT, t1 = min(t0 + len * UNIT, sp.hi);
 
     // the rows' queries: column c16 of the operand is row 16 (rg RW + rw) + c16
     const int rr = 16 * (rg * RW + rw) + c16, l = rr / a.G;
@@ -266,45 +293,46 @@ void paged_attn_kernel(PagedAttnArgs a) {
     }
 
     // rows (in the cache) of the next 64 sixteens of this wave's tokens, one per lane
-    const int step = 32 * TW;
-    const int tiles = t1 > t0 + 32 * ts ? (t1 - t0 - 32 * ts + step - 1) / step : 0;
+    constexpr int step = TT * TW;
+    const int begin = t0 + TT * ts;
+    const int tiles = t1 > begin ? (t1 - begin + step - 1) / step : 0;
     long long row64 = 0;
     auto look_up = [&](int it) {
-      int t = t0 + 32 * ts + (it + lane / 2) * step + 16 * (lane % 2);
+      int t = begin + (it + lane / NS) * step + 16 * (lane % NS);
       t = min(t, (t1 - 1) & ~15);
       const int pg = a.table[n * a.table_stride + t / a.page];
       const bool ok = pg >= 0 && pg < a.num_pages;
       row64 = ok ? ((long long)pg * a.Hkv + kvh) * a.page + t % a.page : -1;
     };
     auto row_at = [&](int it, int s) {
-      const int i = 2 * (it % 32) + s;
+      const int i = NS * (it % (64 / NS)) + s;
       const uint32_t lo = __builtin_amdgcn_readlane((int)row64, i);
       const uint32_t hi = __builtin_amdgcn_readlane((int)(row64 >> 32), i);
       return (long long)((uint64_t)hi << 32 | lo);
     };
 
-    u32x4w kr[2][KL];
-    uint32_t vr[8][VD];
-    f32x4 kscale[2], vscale[2];
-    long long rows[2];   // of the tile whose K is loaded
+    u32x4w kr[NS][KL];
+    uint32_t vr[4 * NS][VD];
+    float kscale[NS], vscale[NS];   // of token 4 g + c16 % 4 of a sixteen
+    long long rows[NS];   // of the tile whose K is loaded
     auto valid = [&](int it, int s) {   // tokens of a sixteen that there are
-      return min(max(t1 - (t0 + 32 * ts + it * step + 16 * s), 1), 16);
+      return min(max(t1 - (begin + it * step + 16 * s), 1), 16);
     };
     auto load_k = [&](int it) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+      for (int s = 0; s < NS; ++s) {
         rows[s] = row_at(it, s);
         const long long row = max(rows[s], 0ll);
         const char* p = kc + row * ROW;
         const int off = min(c16, valid(it, s) - 1) * ROW + 16 * g;
 #pragma unroll
         for (int k = 0; k < KL; ++k) kr[s][k] = *reinterpret_cast<const u32x4w*>(p + (off + 64 * k));
-        if constexpr (C8) kscale[s] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(a.ks + row) + 16u * g);
+        if constexpr (C8) kscale[s] = *(a.ks + row + (4u * g + c16 % 4));
       }
     };
-    auto load_v = [&](const long long (&rv)[2], int it) {
+    auto load_v = [&](const long long (&rv)[NS], int it) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+      for (int s = 0; s < NS; ++s) {
         const long long row = max(rv[s], 0ll);
         const char* p = vc + row * ROW;
         const int most = valid(it, s) - 1;
@@ -327,7 +355,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
             }
           }
         }
-        if constexpr (C8) vscale[s] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const char*>(a.vs + row) + 16u * g);
+        if constexpr (C8) vscale[s] = *(a.vs + row + (4u * g + c16 % 4));
       }
     };
 
@@ -335,19 +363,19 @@ void paged_attn_kernel(PagedAttnArgs a) {
 #pragma unroll
     for (int j = 0; j < E; ++j) acc[j] = zero4();
     float m = -INFINITY, sum = 0.f, vref = 0.f, vinv = 1.f;
-    long long rv[2];
+    long long rv[NS];
     if (tiles > 0) {
       look_up(0);
       load_k(0);
-      rv[0] = rows[0];
-      rv[1] = rows[1];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) rv[s] = rows[s];
       load_v(rv, 0);
     }
     for (int it = 0; it < tiles; ++it) {
-      const int tb = t0 + 32 * ts + it * step;
-      f32x4 S[2];
+      const int tb = begin + it * step;
+      f32x4 S[NS];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
+      for (int s = 0; s < NS; ++s) {
         S[s] = zero4();
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
@@ -355,34 +383,37 @@ void paged_attn_kernel(PagedAttnArgs a) {
           if constexpr (C8) kf = codes_operand<CT>(kr[s][k / 2][2 * (k % 2)], kr[s][k / 2][2 * (k % 2) + 1]);
           else kf = __builtin_bit_cast(u16x8, kr[s][k]);
           S[s] = mfma_t<BF>(kf, qf[k], S[s]);
+          if (C8 && k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) S[s][r] *= C8 ? qscale * kscale[s][r] : qscale;
+        for (int r = 0; r < 4; ++r) S[s][r] *= C8 ? qscale * of_four(kscale[s], r) : qscale;
       }
-      const bool bad = rows[0] < 0 || rows[1] < 0;
-      const bool here[2] = {rows[0] < 0, rows[1] < 0};
+      bool bad = false, here[NS];
+#pragma unroll
+      for (int s = 0; s < NS; ++s) {
+        here[s] = rows[s] < 0;
+        bad |= here[s];
+      }
       if (it + 1 < tiles) {
-        if ((it + 1) % 32 == 0) look_up(it + 1);
+        if ((it + 1) % (64 / NS) == 0) look_up(it + 1);
         load_k(it + 1);
       }
       // tokens that some row of this wave does not see
-      const bool mixed = (a.L > 1 && tb + 31 > sp.hi - a.L) || (a.window > 0 && tb <= sp.hi - 1 - a.window);
-      const bool part = mixed || bad || tb + 32 > t1;
-      bool seen[2][4];
+      const bool mixed = (a.L > 1 && tb + TT - 1 > sp.hi - a.L) || (a.window > 0 && tb <= sp.hi - 1 - a.window);
+      const bool part = mixed || bad || tb + TT > t1;
       if (part) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int s = 0; s < NS; ++s)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int t = tb + 16 * s + 4 * g + r;
-            seen[s][r] = t < t1 && t <= pos && (a.window == 0 || t > pos - a.window);
             if (here[s]) S[s][r] = __builtin_nanf("");
-            if (!seen[s][r]) S[s][r] = -INFINITY;
+            if (t >= t1 || t > pos || (a.window > 0 && t <= pos - a.window)) S[s][r] = -INFINITY;
           }
       }
       float mx = S[0][0];
 #pragma unroll
-      for (int i = 1; i < 8; ++i) mx = fmaxf(mx, S[i / 4][i % 4]);
+      for (int i = 1; i < 4 * NS; ++i) mx = fmaxf(mx, S[i / 4][i % 4]);
       mx = fmaxf(m, xmax16(mx));
       const float ref = mx == -INFINITY ? 0.f : mx;
       float grow = 1.f;
@@ -391,11 +422,11 @@ void paged_attn_kernel(PagedAttnArgs a) {
         // fp16's range
         float big = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (part && !(tb + 16 * (i / 4) + 4 * g + i % 4 < t1)) vscale[i / 4][i % 4] = 0.f;
-          big = fmaxf(big, vscale[i / 4][i % 4]);
+        for (int s = 0; s < NS; ++s) {
+          if (part && tb + 16 * s + 4 * g + c16 % 4 >= t1) vscale[s] = 0.f;
+          big = fmaxf(big, vscale[s]);
         }
-        big = xmax16(big);
+        big = xmax16(xmax4(big));
         if (big > vref) {
           const float next = __uint_as_float(min((__float_as_uint(big) & 0x7f800000u) + 0x800000u, 0x7e800000u));
           grow = vref * (1.f / next);
@@ -410,73 +441,85 @@ void paged_attn_kernel(PagedAttnArgs a) {
         for (int j = 0; j < E; ++j) acc[j] *= f * grow;
         m = mx;
       }
-      f32x4 p[2];
+      f32x4 p[NS];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4 * NS; ++i) {
         float x = exp2i(S[i / 4][i % 4] - ref);
         sum += x;
         if constexpr (C8) {
-          x *= vscale[i / 4][i % 4] * vinv;
-          if (part && !seen[i / 4][i % 4]) x = 0.f;
+          // (a token that is not seen may have any scale)
+          const float y = x * (of_four(vscale[i / 4], i % 4) * vinv);
+          x = x == 0.f ? 0.f : y;
         }
         p[i / 4][i % 4] = x;
       }
-      u16x8 hi, lo;
-      operands<BF, LO>(p, hi, lo);
+      u16x8 hi[NS / 2], lo[NS / 2];
+#pragma unroll
+      for (int h = 0; h < NS / 2; ++h) operands<BF, LO>(p[2 * h], p[2 * h + 1], hi[h], lo[h]);
       // O^T += V^T P^T;  with `mixed` a value that is not finite reaches only the rows that see its token
       auto add_v = [&](auto some) {
         constexpr bool MIX = decltype(some)::value;
-        u16x8 ones;
+        u16x8 ones[NS / 2];
         if constexpr (MIX) {
+          // (kept apart from the other branch's conversions, which the compiler would
+          // else form ahead of both and hold in registers all at once)
 #pragma unroll
-          for (int i = 0; i < 8; ++i) ones[i] = seen[i / 4][i % 4] ? from_f<BF>(1.f) : (uint16_t)0;
+          for (int t = 0; t < 4 * NS; ++t)
+#pragma unroll
+            for (int w = 0; w < VD; ++w) asm volatile("" : "+v"(vr[t][w]));
+#pragma unroll
+          for (int i = 0; i < 4 * NS; ++i) ones[i / 8][i % 8] = S[i / 4][i % 4] == -INFINITY ? (uint16_t)0 : from_f<BF>(1.f);
         }
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          u32x4w vf;
 #pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            if constexpr (CT == GDN_DTYPE_E4M3) {
-              const uint32_t w = __builtin_amdgcn_perm(vr[2 * t + 1][j / 4], vr[2 * t][j / 4],
-                                                       j % 4 < 2 ? 0x05010400u : 0x07030602u);
-              vf[t] = j % 2 ? e4m3_pair<true>(w) : e4m3_pair<false>(w);
-            } else if constexpr (CT == GDN_DTYPE_I8) {
-              constexpr uint32_t sel[4] = {0x0c040c00u, 0x0c050c01u, 0x0c060c02u, 0x0c070c03u};
-              vf[t] = i8_pair(__builtin_amdgcn_perm(vr[2 * t + 1][j / 4] ^ 0x80808080u,
-                                                    vr[2 * t][j / 4] ^ 0x80808080u, sel[j % 4]));
-            } else {
-              vf[t] = __builtin_amdgcn_perm(vr[2 * t + 1][j / 2], vr[2 * t][j / 2],
-                                            j % 2 ? 0x07060302u : 0x05040100u);
+          for (int h = 0; h < NS / 2; ++h) {
+            u32x4w vf;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+              const uint32_t* x = vr[8 * h + 2 * t];
+              const uint32_t* y = vr[8 * h + 2 * t + 1];
+              if constexpr (CT == GDN_DTYPE_E4M3) {
+                const uint32_t w = __builtin_amdgcn_perm(y[j / 4], x[j / 4], j % 4 < 2 ? 0x05010400u : 0x07030602u);
+                vf[t] = j % 2 ? e4m3_pair<true>(w) : e4m3_pair<false>(w);
+              } else if constexpr (CT == GDN_DTYPE_I8) {
+                constexpr uint32_t sel[4] = {0x0c040c00u, 0x0c050c01u, 0x0c060c02u, 0x0c070c03u};
+                vf[t] = i8_pair(__builtin_amdgcn_perm(y[j / 4] ^ 0x80808080u, x[j / 4] ^ 0x80808080u, sel[j % 4]));
+              } else {
+                vf[t] = __builtin_amdgcn_perm(y[j / 2], x[j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+              }
             }
+            u16x8 v = __builtin_bit_cast(u16x8, vf);
+            if constexpr (MIX) {
+              constexpr uint16_t kExp = BF ? 0x7f80 : 0x7c00;
+              u16x8 ind;
+              bool any = false;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const bool x = (v[i] & kExp) == kExp;
+                any |= x;
+                ind[i] = x ? from_f<BF>(1.f) : (uint16_t)0;
+                v[i] = x ? (uint16_t)0 : v[i];
+              }
+              if (__any(any)) {
+                const f32x4 hit = mfma_t<BF>(ind, ones[h], zero4());
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if (hit[r] > 0.f) acc[j][r] = __builtin_nanf("");
+              }
+            }
+            acc[j] = mfma_t<BF>(v, hi[h], acc[j]);
+            if constexpr (LO) acc[j] = mfma_t<BF>(v, lo[h], acc[j]);
           }
-          u16x8 v = __builtin_bit_cast(u16x8, vf);
-          if constexpr (MIX) {
-            constexpr uint16_t kExp = BF ? 0x7f80 : 0x7c00;
-            u16x8 ind;
-            bool any = false;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const bool x = (v[i] & kExp) == kExp;
-              any |= x;
-              ind[i] = x ? from_f<BF>(1.f) : (uint16_t)0;
-              v[i] = x ? (uint16_t)0 : v[i];
-            }
-            if (__any(any)) {
-              const f32x4 hit = mfma_t<BF>(ind, ones, zero4());
-#pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (hit[r] > 0.f) acc[j][r] = __builtin_nanf("");
-            }
-          }
-          acc[j] = mfma_t<BF>(v, hi, acc[j]);
-          if constexpr (LO) acc[j] = mfma_t<BF>(v, lo, acc[j]);
+          // (conversions beside their products, not all ahead of them: registers)
+          if (j % 2) __builtin_amdgcn_sched_barrier(0);
         }
       };
       if (mixed) add_v(std::true_type{});
       else add_v(std::false_type{});
       if (it + 1 < tiles) {
-        rv[0] = rows[0];
-        rv[1] = rows[1];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) rv[s] = rows[s];
         load_v(rv, it + 1);
       }
     }
@@ -626,7 +669,7 @@ struct AttnPlan {
   bool split;   // some work may be cut
   size_t desc, bytes;
 };
-int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_length, AttnPlan& p) {
+int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_length, int row_bytes, AttnPlan& p) {
   if (N < 0 || L < 1 || Hq < 1 || Hkv < 1 || max_length < 0)
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": sizes must be non-negative (L, Hq, Hkv > 0)");
   if (Hq % Hkv)
@@ -639,7 +682,8 @@ int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_le
   p.rw = R <= 16 ? 1 : R <= 32 ? 2 : 4;
   p.rg = (int)((R + 16 * p.rw - 1) / (16 * p.rw));
   p.rows = (int)(R < 16 * p.rw ? R : 16 * p.rw);
-  const long long units = ((long long)max_length + gdn::kUnit - 1) / gdn::kUnit;
+  const int unit = row_bytes ? gdn::unit_of(row_bytes, p.rw) : gdn::kUnit;   // (0: the smallest)
+  const long long units = ((long long)max_length + unit - 1) / unit;
   const long long most = (units ? units : 1) * N * Hkv * p.rg;
   if (most >= (1LL << 30))
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
@@ -658,7 +702,7 @@ int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_le
 
 extern "C" size_t gdn_paged_attn_workspace_bytes(int N, int L, int Hq, int Hkv, int D, int max_length) {
   AttnPlan p{};
-  if (attn_plan("gdn_paged_attn_workspace_bytes", N, L, Hq, Hkv, D, max_length, p)) return 0;
+  if (attn_plan("gdn_paged_attn_workspace_bytes", N, L, Hq, Hkv, D, max_length, 0, p)) return 0;
   return p.bytes;
 }
 
@@ -672,7 +716,8 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long long q_seq, long long q_to
                                   size_t workspace_bytes, void* stream) {
   const char* name = "gdn_paged_attn_fwd";
   AttnPlan p{};
-  if (const int rc = attn_plan(name, N, L, Hq, Hkv, D, max_length, p)) return rc;
+  const bool bits8 = cache_dtype == GDN_DTYPE_E4M3 || cache_dtype == GDN_DTYPE_I8;
+  if (const int rc = attn_plan(name, N, L, Hq, Hkv, D, max_length, D * (bits8 ? 1 : 2), p)) return rc;
   if (const int rc = gdn_host::check_cache(name, k_cache, v_cache, k_scale, v_scale, Hkv, D, num_pages, page_size,
                                            cache_dtype))
     return rc;
