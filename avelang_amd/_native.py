@@ -249,9 +249,9 @@ def lib():
             + [_ll, _i, _f, _i, _i, _i, _vp, _sz, _vp])
         h.gdn_rotary.restype = _i
         h.gdn_rotary.argtypes = (
-            [_vp] * 6                         # x y and their strides, heads, positions
-            + [_i, _ll, _vp]                  # int64, batch stride, inv_freq
-            + [_i] * 4 + [_f, _i, _i, _i, _vp])   # B T D R magnitude near inverse dtype stream
+            [_vp] * 5 + [_i] * 5              # q k and their outputs, strides, B T Hq Hk D
+            + [_vp, _i, _ll, _vp]             # positions, int64, batch stride, inv_freq
+            + [_i, _f, _i, _i, _i, _vp])      # R magnitude interleaved inverse dtype stream
         h.gdn_paged_write.restype = _i
         h.gdn_paged_write.argtypes = (
             [_vp, _vp] + [_ll] * 4 + [_vp, _i]   # k v strides slots int64

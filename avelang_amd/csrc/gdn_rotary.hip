@@ -119,37 +119,38 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
 
 }  // namespace gdn
 
-extern "C" int gdn_rotary(const void* const* x, void* const* y, const long long* xs,
-                          const long long* ys, const int* heads, const void* positions,
-                          int pos_int64, long long pos_batch, const double* inv_freq, int B, int T,
-                          int D, int R, float magnitude, int interleaved, int inverse, int dtype,
-                          void* stream) {
+extern "C" int gdn_rotary(const void* q, const void* k, void* q_out, void* k_out,
+                          const long long* strides, int B, int T, int Hq, int Hk, int D,
+                          const void* positions, int pos_int64, long long pos_batch,
+                          const double* inv_freq, int R, float magnitude, int interleaved,
+                          int inverse, int dtype, void* stream) {
   const char* name = "gdn_rotary";
-  if (!x || !y || !xs || !ys || !heads)
-    return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": x, y, their strides and heads must be non-NULL");
-  if (B < 0 || T < 0 || heads[0] < 1 || heads[1] < 0)
-    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": sizes must be non-negative (heads[0] > 0)");
+  if (!k) Hk = 0;
+  if (B < 0 || T < 0 || Hq < 1 || Hk < 0)
+    return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": sizes must be non-negative (Hq > 0)");
   if (D < 2 || D > 512 || D % 2 || R < 2 || R > D || R % 2)
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": D and R must be even, 2 <= R <= D <= 512");
   if (!gdn::dtype_ok(dtype))
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": unsupported dtype code");
-  if ((long long)heads[0] + heads[1] > (1 << 20) || (long long)B * T >= (1LL << 31))
+  if (Hq > (1 << 20) || Hk > (1 << 20) || (long long)B * T >= (1LL << 31))
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
   if ((long long)B * T == 0) return GDN_OK;
-  if (!positions || !inv_freq || !x[0] || !y[0] || (heads[1] && (!x[1] || !y[1])))
-    return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": x, y, positions and inv_freq must be non-NULL");
-  const int two = heads[1] > 0 ? 2 : 1;
-  bool inplace = true;
-  for (int k = 0; k < two; ++k) {
-    const bool same = x[k] == y[k];
-    for (int i = 0; i < 3; ++i) {
-      if (xs[3 * k + i] < 0 || ys[3 * k + i] < 0)
+  if (!positions || !inv_freq || !strides || !q || !q_out || (Hk && !k_out))
+    return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": q, its output, strides, positions and inv_freq must be "
+                                                            "non-NULL, and k's output with k");
+  const void* x[2] = {q, k};
+  void* y[2] = {q_out, k_out};
+  const int heads[2] = {Hq, Hk}, two = Hk > 0 ? 2 : 1;
+  const long long *xs = strides, *ys = strides + 6;
+  const bool inplace = q == q_out;
+  for (int i = 0; i < two; ++i) {
+    for (int j = 0; j < 3; ++j) {
+      if (xs[3 * i + j] < 0 || ys[3 * i + j] < 0)
         return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": strides must be non-negative");
-      if (same && xs[3 * k + i] != ys[3 * k + i])
-        return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": in place x and y must have the same strides");
+      if (inplace && xs[3 * i + j] != ys[3 * i + j])
+        return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": in place both must have the same strides");
     }
-    inplace = inplace && same;
-    if (same != (x[0] == y[0]))
+    if (inplace != (x[i] == y[i]))
       return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": both tensors in place, or none");
   }
   if (two == 2 && y[0] == y[1])
@@ -161,13 +162,13 @@ extern "C" int gdn_rotary(const void* const* x, void* const* y, const long long*
   for (const int v : {full, 2})
     if (vec == 1 && R % (2 * v) == 0 && D % (2 * v) == 0) vec = v;
   gdn::RotaryArgs a{};
-  for (int k = 0; k < two; ++k) {
-    a.x[k] = x[k];
-    a.y[k] = y[k];
-    a.heads[k] = heads[k];
-    for (int i = 0; i < 3; ++i) {
-      a.xs[k][i] = xs[3 * k + i];
-      a.ys[k][i] = ys[3 * k + i];
+  for (int i = 0; i < two; ++i) {
+    a.x[i] = x[i];
+    a.y[i] = y[i];
+    a.heads[i] = heads[i];
+    for (int j = 0; j < 3; ++j) {
+      a.xs[i][j] = xs[3 * i + j];
+      a.ys[i][j] = ys[3 * i + j];
     }
   }
   a.pos = positions;
@@ -184,7 +185,7 @@ extern "C" int gdn_rotary(const void* const* x, void* const* y, const long long*
   a.sign = inverse ? -1.f : 1.f;
   // groups of lanes per token: as many heads to a group as leave every CU eight
   // workgroups, eight at most
-  const int total = heads[0] + heads[1];
+  const int total = Hq + Hk;
   const long long want = 8LL * gdn::device_cus() * a.per_wg;
   long long split = (want + a.rows - 1) / a.rows;
   if (split < (total + 7) / 8) split = (total + 7) / 8;

@@ -15,6 +15,7 @@ follow its kernel-library convention
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -259,6 +260,12 @@ def rms_norm_bwd(h: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Tens
     return dx, dw, dr
 
 
+@functools.lru_cache(maxsize=256)
+def _rms_bytes(device, rows, D, dt):
+    return _native.on_device(torch.device("cuda", device), _native.lib().gdn_rms_norm_bwd_workspace_bytes,
+                             rows, D, dt)
+
+
 def _rms_bwd(dy, weight, h, sizes, rstd, dh, offset, want_w, want_r, name):
     """On ``_rms_args``' (dy, weight, h, sizes)."""
     rows, D, dt, hdt, wdt = sizes
@@ -278,7 +285,7 @@ def _rms_bwd(dy, weight, h, sizes, rstd, dh, offset, want_w, want_r, name):
     lib = _native.lib()
     ws, nbytes = None, 0
     if want_w:
-        nbytes = _native.on_device(dev, lib.gdn_rms_norm_bwd_workspace_bytes, rows, D, dt)
+        nbytes = _rms_bytes(dev.index, rows, D, dt)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _native.check(_native.on_device(
         dev, lib.gdn_rms_norm_bwd, h.data_ptr(), _ptr(weight), dy.data_ptr(), _ptr(dh),

@@ -13,6 +13,7 @@ its kernel-library convention (python/avelang_kernels/amdgpu_gemm.py:458-494).
 """
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -24,6 +25,7 @@ __all__ = ["PagedKVCache", "paged_cache_write", "paged_cache_read", "paged_atten
            "paged_attention_workspace_bytes"]
 
 _SIZES = (64, 128, 256)
+_HALF = (torch.bfloat16, torch.float16)
 _CODES = {torch.float8_e4m3fn: _native.GDN_DTYPE_E4M3, torch.int8: _native.GDN_DTYPE_I8}
 _TYPES = {torch.bfloat16: _native.GDN_DTYPE_BF16, torch.float16: _native.GDN_DTYPE_F16, **_CODES}
 
@@ -42,27 +44,34 @@ class PagedKVCache:
         if not isinstance(k, torch.Tensor) or k.dim() != 4 or k.dtype not in _TYPES:
             raise ValueError(f"{name}: k must be a 4-D tensor [num_pages, kv_heads, page_size, "
                              "head_size] in bf16, fp16, float8_e4m3fn or int8.")
-        shape, dev = k.shape, k.device
-        if shape[1] < 1 or shape[2] < 1 or shape[3] not in _SIZES:
+        dtype, dev, shape = k.dtype, k.device, k.shape
+        pages, heads, page, size = shape
+        if heads < 1 or page < 1 or size not in _SIZES:
             raise ValueError(f"{name}: kv_heads and page_size must be at least 1 and head_size one of "
                              f"{_SIZES}, got {tuple(shape)}.")
-        if not isinstance(v, torch.Tensor) or v.shape != shape or v.dtype != k.dtype or v.device != dev:
-            raise ValueError(f"{name}: v must be like k, {k.dtype} of shape {tuple(shape)} on {dev}.")
-        if not k.is_contiguous() or not v.is_contiguous() or (k.data_ptr() | v.data_ptr()) % 16:
+        if not isinstance(v, torch.Tensor) or v.shape != shape or v.dtype is not dtype or v.device != dev:
+            raise ValueError(f"{name}: v must be like k, {dtype} of shape {tuple(shape)} on {dev}.")
+        pk, pv = k.data_ptr(), v.data_ptr()
+        if not k.is_contiguous() or not v.is_contiguous() or (pk | pv) % 16:
             raise ValueError(f"{name}: k and v must be contiguous and 16-byte aligned.")
-        if k.dtype in _CODES:
-            for nm, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-                if (not isinstance(t, torch.Tensor) or t.shape != shape[:3] or t.device != dev
-                        or t.dtype is not torch.float32 or not t.is_contiguous()
-                        or t.data_ptr() % 16):
-                    raise ValueError(f"{name}: {nm} must be a contiguous, 16-byte aligned "
-                                     f"torch.float32 tensor of shape {tuple(shape[:3])} on {dev}.")
+        sk = sv = None
+        if dtype in _CODES:
+            sk = self._scale(k_scale, shape[:3], dev, "k_scale")
+            sv = self._scale(v_scale, shape[:3], dev, "v_scale")
         elif k_scale is not None or v_scale is not None:
-            raise ValueError(f"{name}: a cache in {k.dtype} has no scales.")
+            raise ValueError(f"{name}: a cache in {dtype} has no scales.")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.ptrs = k.data_ptr(), v.data_ptr(), _ptr(k_scale), _ptr(v_scale)
-        self.sizes = shape[1], shape[3], shape[0], shape[2]   # H, D, pages, page
-        self.code = _TYPES[k.dtype]
+        self.ptrs = pk, pv, sk, sv
+        self.sizes = heads, size, pages, page
+        self.code = _TYPES[dtype]
+
+    @staticmethod
+    def _scale(t, shape, dev, what):
+        if (not isinstance(t, torch.Tensor) or t.shape != shape or t.device != dev
+                or t.dtype is not torch.float32 or not t.is_contiguous() or t.data_ptr() % 16):
+            raise ValueError(f"PagedKVCache: {what} must be a contiguous, 16-byte aligned "
+                             f"torch.float32 tensor of shape {tuple(shape)} on {dev}.")
+        return t.data_ptr()
 
     @classmethod
     def zeros(cls, num_pages: int, page_size: int, kv_heads: int, head_size: int,
@@ -114,15 +123,20 @@ def paged_cache_write(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
     H, D, pages, page = _cache(cache, name).sizes
     dev = cache.k.device
     slots = _slots(slots, cache, name, True)
-    for nm, t in (("k", k), ("v", v)):
-        if (not isinstance(t, torch.Tensor) or t.shape != slots.shape + (H, D) or t.device != dev
-                or t.dtype != k.dtype or t.dtype not in (torch.bfloat16, torch.float16)):
-            raise ValueError(f"{name}: {nm} must be a bf16 or fp16 tensor of shape "
-                             f"{tuple(slots.shape) + (H, D)} on {dev}, k and v alike.")
-    if cache.k.dtype != k.dtype and cache.k.dtype not in _CODES:
+    shape = slots.shape + (H, D)
+    if (not isinstance(k, torch.Tensor) or not isinstance(v, torch.Tensor) or k.shape != shape
+            or v.shape != shape or k.device != dev or v.device != dev or v.dtype is not k.dtype
+            or k.dtype not in _HALF):
+        raise ValueError(f"{name}: k and v must be bf16 or fp16 tensors of one type and shape "
+                         f"{tuple(shape)} on {dev}.")
+    if cache.k.dtype is not k.dtype and cache.k.dtype not in _CODES:
         raise ValueError(f"{name}: a cache in {cache.k.dtype} takes rows of its type, got {k.dtype}.")
-    k, v = (t if t.dim() == 3 else t.reshape(-1, H, D) for t in (k, v))
-    k, v = (t if t.stride(2) == 1 and min(t.stride()) >= 0 else t.contiguous() for t in (k, v))
+    if len(shape) != 3:
+        k, v = k.reshape(-1, H, D), v.reshape(-1, H, D)
+    if k.stride(2) != 1:
+        k = k.contiguous()
+    if v.stride(2) != 1:
+        v = v.contiguous()
     sk, sv = k.stride(), v.stride()
     _native.check(_native.on_device(
         dev, _native.lib().gdn_paged_write, k.data_ptr(), v.data_ptr(), sk[0], sk[1], sv[0], sv[1],
@@ -141,11 +155,12 @@ def paged_cache_read(cache: PagedKVCache, slots: torch.Tensor,
     slots = _slots(slots, cache, name, False)
     if dtype is None:
         dtype = torch.bfloat16 if cache.k.dtype in _CODES else cache.k.dtype
-    if dtype not in (torch.bfloat16, torch.float16) or (cache.k.dtype not in _CODES
+    if dtype not in _HALF or (cache.k.dtype not in _CODES
                                                         and dtype != cache.k.dtype):
         raise ValueError(f"{name}: dtype must be bf16 or fp16, and the cache's unless it has 8 bits, "
                          f"got {dtype}.")
-    k, v = (torch.empty(slots.shape + (H, D), dtype=dtype, device=dev) for _ in "kv")
+    k = torch.empty(slots.shape + (H, D), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
     _native.check(_native.on_device(
         dev, _native.lib().gdn_paged_read, *cache.ptrs, slots.data_ptr(),
         slots.dtype is torch.int64, k.data_ptr(), v.data_ptr(), slots.numel(), H, D, pages, page,
@@ -157,6 +172,11 @@ def paged_attention_workspace_bytes(N: int, L: int, Hq: int, Hkv: int, D: int, m
     """Device scratch bytes ``paged_attention`` needs for N sequences of L new tokens each and
     lengths up to ``max_length``, or for any fewer or shorter with the same L and heads."""
     return int(_native.lib().gdn_paged_attn_workspace_bytes(N, L, Hq, Hkv, D, max_length))
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(device, *sizes):
+    return _native.on_device(torch.device("cuda", device), _native.lib().gdn_paged_attn_workspace_bytes, *sizes)
 
 
 def paged_attention(
@@ -195,7 +215,7 @@ def paged_attention(
     H, D, pages, page = _cache(cache, name).sizes
     dev = cache.k.device
     if (not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[3] != D or q.device != dev
-            or q.dtype not in (torch.bfloat16, torch.float16)):
+            or q.dtype not in _HALF):
         raise ValueError(f"{name}: q must be a bf16 or fp16 tensor [N, L, Hq, {D}] on {dev}.")
     N, L, Hq, _ = q.shape
     if L < 1 or Hq < 1 or Hq % H:
@@ -223,8 +243,9 @@ def paged_attention(
     elif not 0 <= max_length <= held:
         raise ValueError(f"{name}: max_length must be within the block table's {held} tokens.")
     # (strides of an axis of one mean nothing)
-    sn, sl, sh, se = (0 if n == 1 else t for n, t in zip(q.shape, q.stride()))
-    if se != 1 or (sn | sl | sh) % 8 or min(sn, sl, sh) < 0 or q.data_ptr() % 16:
+    sn, sl, sh, se = q.stride()
+    sn, sl, sh = sn if N > 1 else 0, sl if L > 1 else 0, sh if Hq > 1 else 0
+    if se != 1 or (sn | sl | sh) % 8 or q.data_ptr() % 16:
         q = q.contiguous()
         q = q if q.data_ptr() % 16 == 0 else q.clone()
         sn, sl, sh = L * Hq * D, Hq * D, D
@@ -237,7 +258,7 @@ def paged_attention(
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if return_lse else None
     lib = _native.lib()
     if workspace is None:
-        nbytes = _native.on_device(dev, lib.gdn_paged_attn_workspace_bytes, N, L, Hq, H, D, max_length)
+        nbytes = _workspace_bytes(dev.index, N, L, Hq, H, D, max_length)
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     elif workspace.device != dev or not workspace.is_contiguous():   # (its size is checked by the entry point)
         raise ValueError(f"{name}: workspace must be contiguous on {dev}.")

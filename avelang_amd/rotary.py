@@ -22,11 +22,22 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .layer_ops import _dt, _stream
+from .layer_ops import _dt, _ptr, _stream
+from .norm import _grad
 
 __all__ = ["rotary_embedding", "rotary_frequencies"]
 
-_P2, _L6, _I2 = ctypes.c_void_p * 2, ctypes.c_longlong * 6, ctypes.c_int * 2
+_STRIDES = ctypes.c_longlong * 12
+
+
+def _apart(t) -> bool:
+    """No two elements of t share memory (as far as strides in their order tell)."""
+    reach = 0
+    for stride, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+        if stride <= reach:
+            return False
+        reach += stride * (n - 1)
+    return True
 
 
 def rotary_frequencies(dim: int, base: float = 10000.0, *, factor: float = 1.0, original: int = 0,
@@ -58,101 +69,98 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, factor: float = 1.0, 
     return f.to(device) if device is not None else f, size
 
 
-def _apart(t) -> bool:
-    """No two elements of t share memory (as far as strides in their order tell)."""
-    reach = 0
-    for stride, n in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
-        if stride <= reach:
-            return False
-        reach += stride * (n - 1)
-    return True
-
-
 def _args(q, k, positions, inv_freq, name):
-    """Checked q and k as 4-D views, positions with their batch stride, fp64 frequencies."""
-    xs = []
-    for nm, t in (("q", q), ("k", k)):
-        if t is None and nm == "k":
-            continue
-        if not isinstance(t, torch.Tensor) or t.dim() not in (3, 4):
-            raise ValueError(f"{name}: {nm} must be a tensor [B, T, H, D] or [T, H, D].")
-        xs.append(t if t.dim() == 4 else t[None])
-    q4 = xs[0]
-    dt = _dt(q4, name, "q")
-    dev, (B, T, _, D) = q4.device, q4.shape
+    """Checked q and k as 4-D tensors with contiguous elements, positions, fp64 frequencies and
+    the type's code."""
+    if not isinstance(q, torch.Tensor) or not 3 <= q.dim() <= 4:
+        raise ValueError(f"{name}: q must be a tensor [B, T, H, D] or [T, H, D].")
+    dt, dev = _dt(q, name, "q"), q.device
+    if k is not None and (not isinstance(k, torch.Tensor) or k.dim() != q.dim()
+                          or k.dtype is not q.dtype or k.device != dev):
+        raise ValueError(f"{name}: k must be a {q.dtype} tensor like q on {dev}.")
+    if q.dim() == 3:
+        q, k = q[None], None if k is None else k[None]
     if dev.type != "cuda":
         raise ValueError(f"{name}: tensors must be on a ROCm (cuda) device, got {dev}.")
-    if len(xs) == 2:
-        k4 = xs[1]
-        if (k.dim() != q.dim() or k4.shape[:2] != (B, T) or k4.shape[3] != D or k4.dtype != q4.dtype
-                or k4.device != dev):
-            raise ValueError(f"{name}: k must be {q4.dtype} like q on {dev}, with q's axes but heads.")
-    if any(t.shape[2] < 1 for t in xs):
-        raise ValueError(f"{name}: q and k must have at least one head.")
-    if D < 2 or D > 512 or D % 2:
-        raise ValueError(f"{name}: head size must be even and at most 512, got {D}.")
+    B, T, H, D = q.shape
+    if H < 1 or D < 2 or D > 512 or D % 2:
+        raise ValueError(f"{name}: q must have at least one head, and heads of an even size of at "
+                         f"most 512, got {H} of {D}.")
+    if k is not None and (k.shape[0] != B or k.shape[1] != T or k.shape[3] != D or k.shape[2] < 1):
+        raise ValueError(f"{name}: k must have q's axes but heads (at least one), got {tuple(k.shape)} "
+                         f"beside {tuple(q.shape)}.")
     if (not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1 or not inv_freq.is_floating_point()
-            or inv_freq.device != dev or not 1 <= inv_freq.numel() <= D // 2):
+            or inv_freq.device != dev or not 1 <= inv_freq.shape[0] <= D // 2):
         raise ValueError(f"{name}: inv_freq must be a 1-D floating point tensor on {dev} of 1 to "
                          f"{D // 2} frequencies.")
     if (not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64)
-            or positions.device != dev or tuple(positions.shape) not in ((T,), (B, T))):
+            or positions.device != dev or positions.shape != (B, T) and positions.shape != (T,)):
         raise ValueError(f"{name}: positions must be int32 or int64 of shape ({T},) or ({B}, {T}) on "
                          f"{dev}.")
-    batch = T if positions.dim() == 2 else 0
-    xs = [t if t.stride(3) == 1 else t.contiguous() for t in xs]
-    return xs, positions.contiguous(), batch, inv_freq.double().contiguous(), dt
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    if k is not None and k.stride(3) != 1:
+        k = k.contiguous()
+    return q, k, positions.contiguous(), inv_freq.double().contiguous(), dt
 
 
-def _turn(xs, ys, positions, batch, freq, dt, magnitude, interleaved, inverse, name):
-    """ys (4-D, of xs' shapes) from xs."""
-    B, T, _, D = xs[0].shape
-    x, y, heads = _P2(), _P2(), _I2()
-    sx, sy = _L6(), _L6()
-    for i, (a, b) in enumerate(zip(xs, ys)):
-        x[i], y[i], heads[i] = a.data_ptr(), b.data_ptr(), a.shape[2]
-        sx[3 * i:3 * i + 3] = a.stride()[:3]
-        sy[3 * i:3 * i + 3] = b.stride()[:3]
-    dev = xs[0].device
+def _turn(q, k, qo, ko, positions, freq, dt, magnitude, interleaved, inverse, name):
+    """qo, ko (4-D, q's and k's shapes) from q and k."""
+    B, T, Hq, D = q.shape
+    a, b = q.stride(), qo.stride()
+    if k is None:
+        Hk, strides = 0, _STRIDES(a[0], a[1], a[2], 0, 0, 0, b[0], b[1], b[2])
+    else:
+        c, d = k.stride(), ko.stride()
+        Hk = k.shape[2]
+        strides = _STRIDES(a[0], a[1], a[2], c[0], c[1], c[2], b[0], b[1], b[2], d[0], d[1], d[2])
+    dev = q.device
     _native.check(_native.on_device(
-        dev, _native.lib().gdn_rotary, x, y, sx, sy, heads, positions.data_ptr(),
-        positions.dtype is torch.int64, batch, freq.data_ptr(), B, T, D, 2 * freq.numel(),
-        float(magnitude), bool(interleaved), bool(inverse), dt, _stream(dev)), name)
+        dev, _native.lib().gdn_rotary, q.data_ptr(), _ptr(k), qo.data_ptr(), _ptr(ko), strides, B, T,
+        Hq, Hk, D, positions.data_ptr(), positions.dtype is torch.int64,
+        T if positions.dim() == 2 else 0, freq.data_ptr(), 2 * freq.shape[0], magnitude, interleaved,
+        inverse, dt, _stream(dev)), name)
 
 
-def _new(xs):
-    return [torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in xs]
+def _new(t):
+    return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, magnitude, interleaved):
         name = "rotary_embedding"
-        xs, pos, batch, freq, dt = _args(q, k, positions, inv_freq, name)
-        ys = _new(xs)
-        _turn(xs, ys, pos, batch, freq, dt, magnitude, interleaved, False, name)
+        q4, k4, pos, freq, dt = _args(q, k, positions, inv_freq, name)
+        qo, ko = _new(q4), _new(k4)
+        _turn(q4, k4, qo, ko, pos, freq, dt, magnitude, interleaved, False, name)
         ctx.save_for_backward(positions, inv_freq)
-        ctx.rest = magnitude, interleaved, [t.shape for t in (q, k) if t is not None]
+        ctx.rest = magnitude, interleaved
         ctx.set_materialize_grads(False)
-        ys = [y.view(s) for y, s in zip(ys, ctx.rest[2])]
-        return ys[0] if k is None else tuple(ys)
+        if q.dim() == 3:
+            qo, ko = qo[0], None if ko is None else ko[0]
+        return qo if k is None else (qo, ko)
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, *grads):
+    def backward(ctx, dq, dk=None):
         positions, inv_freq = ctx.saved_tensors
-        magnitude, interleaved, _ = ctx.rest
+        magnitude, interleaved = ctx.rest
         name = "rotary_embedding"
-        out = [None, None]
-        at = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[i]]
-        if at:
-            g = [grads[i] for i in at]
-            xs, pos, batch, freq, dt = _args(g[0], g[1] if len(g) > 1 else None, positions, inv_freq, name)
-            ys = _new(xs)
-            _turn(xs, ys, pos, batch, freq, dt, magnitude, interleaved, True, name)
-            for i, y in zip(at, ys):
-                out[i] = y.view(grads[i].shape)
-        return out[0], out[1], None, None, None, None
+        want_q, want_k = ctx.needs_input_grad[:2]
+        a = dq if want_q else None
+        b = dk if want_k else None
+        if a is None:
+            a, b = b, None
+        if a is None:
+            return None, None, None, None, None, None
+        x, y, pos, freq, dt = _args(a, b, positions, inv_freq, name)
+        xo, yo = _new(x), _new(y)
+        _turn(x, y, xo, yo, pos, freq, dt, magnitude, interleaved, True, name)
+        if a.dim() == 3:
+            xo, yo = xo[0], None if yo is None else yo[0]
+        if not want_q or dq is None:
+            xo, yo = None, xo
+        return xo, yo, None, None, None, None
 
 
 def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
@@ -169,20 +177,22 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     turned back), not in place.
     """
     name = "rotary_embedding"
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k)):
+    if torch.is_grad_enabled() and (_grad(q) or _grad(k)):
         if inplace:
             raise ValueError(f"{name}: inplace is not supported when gradients are required.")
         return _Rotary.apply(q, k, positions, inv_freq, float(magnitude), bool(interleaved))
-    xs, pos, batch, freq, dt = _args(q, k, positions, inv_freq, name)
+    q4, k4, pos, freq, dt = _args(q, k, positions, inv_freq, name)
     if inplace:
-        if any(t.stride(-1) != 1 or not _apart(t) for t in (q, k) if t is not None):
-            raise ValueError(f"{name}: in place q and k must have contiguous heads and elements of "
-                             "their own.")
-        ys = xs
+        for t in (q, k):
+            if t is not None and (t.stride(-1) != 1 or not _apart(t)):
+                raise ValueError(f"{name}: in place q and k must have contiguous heads and elements "
+                                 "of their own.")
+        qo, ko = q4, k4
     else:
-        ys = _new(xs)
-    _turn(xs, ys, pos, batch, freq, dt, magnitude, interleaved, False, name)
+        qo, ko = _new(q4), _new(k4)
+    _turn(q4, k4, qo, ko, pos, freq, dt, float(magnitude), bool(interleaved), False, name)
     if inplace:
-        return q if k is None else (q, k)
-    ys = [y if t.dim() == 4 else y[0] for y, t in zip(ys, (q, k))]
-    return ys[0] if k is None else (ys[0], ys[1])
+        qo, ko = q, k
+    elif q.dim() == 3:
+        qo, ko = qo[0], None if ko is None else ko[0]
+    return qo if k is None else (qo, ko)

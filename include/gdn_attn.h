@@ -62,15 +62,16 @@ int gdn_rms_norm_bwd(const void* h, const void* weight, const void* dy, const vo
  *     (a, b) -> magnitude (a cos - b sin, b cos + a sin)
  * pairs (j, j + R / 2), or with `interleaved` (2 j, 2 j + 1); elements R .. D - 1
  * are copied.  `inverse` turns the other way (the gradient).
- * x, y: up to two tensors (a query's and a key's; heads[1] may be 0) of
- * [B, T, heads, D] with strides in elements of batch, token and head (xs, ys:
- * 3 each), elements contiguous; y may be x (the same strides: in place).
+ * q, k (nullable) [B, T, Hq | Hk, D] into q_out, k_out, elements contiguous:
+ * strides holds the elements from one batch, token and head to the next, of q,
+ * k, q_out and k_out (3 each).  q_out may be q and k_out k (the same strides: in
+ * place, both or none).
  * positions [B, T]: int32, or int64 with pos_int64; pos_batch: from one batch's
  * to the next's (0: the same positions).
  */
-int gdn_rotary(const void* const* x, void* const* y, const long long* xs, const long long* ys,
-               const int* heads, const void* positions, int pos_int64, long long pos_batch,
-               const double* inv_freq, int B, int T, int D, int R, float magnitude,
+int gdn_rotary(const void* q, const void* k, void* q_out, void* k_out, const long long* strides,
+               int B, int T, int Hq, int Hk, int D, const void* positions, int pos_int64,
+               long long pos_batch, const double* inv_freq, int R, float magnitude,
                int interleaved, int inverse, int dtype, void* stream);
 
 /*
