@@ -8,6 +8,8 @@
 // in fp32 for 16-bit x (M = 448 = 7 * 64, 127), the quotient is brought to the
 // nearest fp32 value by one fused correction, and no 16-bit x and max bring it
 // within 2^-16 of a border between codes but exactly onto it.
+#include <type_traits>
+
 #include "gdn_bits8.h"
 #include "gdn_norm_rows.h"
 
@@ -19,18 +21,20 @@ struct PagedArgs {
   float* scale[2];
   long long token[2], head[2];   // strides of k, v
   const void* slots;
-  long long rows;   // T H
   long long num_slots;
-  int H, page, slots64;
+  int T, H, page, slots64;
 };
 
 __device__ __forceinline__ long long slot_at(const PagedArgs& a, long long t) {
   return a.slots64 ? static_cast<const long long*>(a.slots)[t]
                    : (long long)static_cast<const int*>(a.slots)[t];
 }
-// Row (token, head) of the cache, in rows.
+// Row (slot, head) of the cache, in rows.  (64-bit divisions, 100 instructions each,
+// only where a cache has that many slots.)
 __device__ __forceinline__ long long cache_row(const PagedArgs& a, long long slot, int h) {
-  return (slot / a.page * a.H + h) * a.page + slot % a.page;
+  const bool few = a.num_slots < (1LL << 31);
+  const long long p = few ? (uint32_t)slot / (uint32_t)a.page : slot / a.page;
+  return (p * a.H + h) * a.page + (slot - p * a.page);
 }
 
 // Eight codes of a row, x in fp32 (16-bit values): exact quotients, rounded.
@@ -52,33 +56,60 @@ __device__ __forceinline__ u32x2b codes8(const float (&x)[8], float most) {
     return u32x2b{int8_4(q[0], q[1], q[2], q[3]), int8_4(q[4], q[5], q[6], q[7])};
 }
 
-template <int DT, int CT, int D>
+// Largest value over the LPR lanes of a row (8, 16 or 32), without LDS.
+template <int LPR>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
+  auto dpp = [](uint32_t v, auto c) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(c)::value, 0xf, 0xf, true);
+  };
+  x = max(x, dpp(x, std::integral_constant<int, 0xb1>{}));    // lanes of a pair changed
+  x = max(x, dpp(x, std::integral_constant<int, 0x4e>{}));    // pairs
+  x = max(x, dpp(x, std::integral_constant<int, 0x141>{}));   // eight lanes mirrored
+  if constexpr (LPR >= 16) x = max(x, dpp(x, std::integral_constant<int, 0x140>{}));   // sixteen
+  if constexpr (LPR == 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(r[0], r[1]);
+  }
+  return x;
+}
+
+// A workgroup takes 256 / LPR * U tokens of one head (blockIdx.y) of k or v
+// (blockIdx.z): what it writes of codes and scales is in one piece.  U rows are on
+// their way to a group of lanes: 4 where that leaves workgroups enough (20011 tokens
+// of 8 heads of 128: MEASURED), 1 else (256 tokens of 2 heads: MEASURED).
+template <int DT, int CT, int D, int U>
 __global__ __launch_bounds__(256) void paged_write_kernel(PagedArgs a) {
-  constexpr int LPR = D / 8;
-  const int l = threadIdx.x % LPR, k = blockIdx.y;
-  const long long r = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  if (r >= a.rows) return;
-  const long long t = r / a.H;
-  const int h = (int)(r % a.H);
-  const long long slot = slot_at(a, t);
-  if (slot < 0 || slot >= a.num_slots) return;
-  const long long dst = cache_row(a, slot, h);
-  const long long src = t * a.token[k] + h * a.head[k] + 8 * l;
-  if constexpr (CT == DT) {
-    reinterpret_cast<u32x4e*>(a.out[k])[dst * LPR + l] =
-        *reinterpret_cast<const u32x4e*>(static_cast<const uint16_t*>(a.in[k]) + src);
-  } else {
-    float x[8];
-    ldn<DT, 8>(a.in[k], src, x);
-    uint32_t m = 0;
+  constexpr int LPR = D / 8, GR = 256 / LPR;
+  const int l = threadIdx.x % LPR, h = blockIdx.y, k = blockIdx.z;
+  const long long t0 = (long long)blockIdx.x * (GR * U) + threadIdx.x / LPR;
+  u32x4e raw[U];
+  long long dst[U];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, abs_bits(x[j]));
+  for (int i = 0; i < U; ++i) {
+    const long long t = t0 + i * GR;
+    dst[i] = -1;
+    if (t >= a.T) continue;
+    const long long slot = slot_at(a, t);
+    raw[i] = *reinterpret_cast<const u32x4e*>(static_cast<const uint16_t*>(a.in[k]) + t * a.token[k] +
+                                              h * a.head[k] + 8 * l);
+    if (slot >= 0 && slot < a.num_slots) dst[i] = cache_row(a, slot, h);
+  }
 #pragma unroll
-    for (int off = 1; off < LPR; off *= 2) m = max(m, (uint32_t)__shfl_xor((int)m, off));
-    const Row8 q = row8(m, CT);
-    if (l == 0) a.scale[k][dst] = q.scale;
-    reinterpret_cast<u32x2b*>(a.out[k])[dst * LPR + l] =
-        codes8<CT>(x, fmaxf(__uint_as_float(m), 0x1p-100f));
+  for (int i = 0; i < U; ++i) {
+    if (dst[i] < 0) continue;   // (the lanes of a row together)
+    if constexpr (CT == DT) {
+      reinterpret_cast<u32x4e*>(a.out[k])[dst[i] * LPR + l] = raw[i];
+    } else {
+      float x[8];
+      unpack<DT>(raw[i], x);
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, abs_bits(x[j]));
+      m = lanes_max<LPR>(m);
+      if (l == 0) a.scale[k][dst[i]] = row8(m, CT).scale;
+      reinterpret_cast<u32x2b*>(a.out[k])[dst[i] * LPR + l] =
+          codes8<CT>(x, fmaxf(__uint_as_float(m), 0x1p-100f));
+    }
   }
 }
 
@@ -98,30 +129,52 @@ __device__ __forceinline__ void values4(uint32_t w, float* f) {
   }
 }
 
-template <int DT, int CT, int D>
+template <int DT, int CT, int D, int U>
 __global__ __launch_bounds__(256) void paged_read_kernel(PagedArgs a) {
-  constexpr int LPR = D / 8;
-  const int l = threadIdx.x % LPR, k = blockIdx.y;
-  const long long r = (long long)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  if (r >= a.rows) return;
-  const long long slot = slot_at(a, r / a.H);
-  float f[8];
+  constexpr int LPR = D / 8, GR = 256 / LPR;
+  constexpr bool C8 = CT == GDN_DTYPE_E4M3 || CT == GDN_DTYPE_I8;
+  const int l = threadIdx.x % LPR, h = blockIdx.y, k = blockIdx.z;
+  const long long t0 = (long long)blockIdx.x * (GR * U) + threadIdx.x / LPR;
+  u32x4e raw[U];
+  u32x2b code[U];
+  float scale[U];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = 0.f;
-  if (slot >= 0 && slot < a.num_slots) {
-    const long long src = cache_row(a, slot, (int)(r % a.H));
-    if constexpr (CT == GDN_DTYPE_E4M3 || CT == GDN_DTYPE_I8) {
-      const u32x2b w = reinterpret_cast<const u32x2b*>(a.in[k])[src * LPR + l];
-      const float s = a.scale[k][src];
-      values4<CT>(w[0], f);
-      values4<CT>(w[1], f + 4);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] *= s;
+  for (int i = 0; i < U; ++i) {
+    const long long t = t0 + i * GR;
+    raw[i] = u32x4e{0, 0, 0, 0};
+    code[i] = u32x2b{0, 0};
+    scale[i] = 0.f;
+    if (t >= a.T) continue;
+    const long long slot = slot_at(a, t);
+    if (slot < 0 || slot >= a.num_slots) continue;
+    const long long src = cache_row(a, slot, h);
+    if constexpr (C8) {
+      code[i] = reinterpret_cast<const u32x2b*>(a.in[k])[src * LPR + l];
+      scale[i] = a.scale[k][src];
     } else {
-      ldn<CT, 8>(a.in[k], src * D + 8 * l, f);
+      raw[i] = reinterpret_cast<const u32x4e*>(a.in[k])[src * LPR + l];
     }
   }
-  stn<DT, 8>(a.out[k], r * D + 8 * l, f);
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const long long t = t0 + i * GR;
+    if (t >= a.T) continue;
+    const long long at = t * a.H + h;
+    if constexpr (C8) {
+      float f[8];
+      values4<CT>(code[i][0], f);
+      values4<CT>(code[i][1], f + 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        f[j] *= scale[i];
+        asm("" : "+v"(f[j]));   // (rounded to fp32 first, not in one step with the conversion to fp16)
+      }
+      stn<DT, 8>(a.out[k], at * D + 8 * l, f);
+    } else {
+      static_assert(DT == CT, "16-bit rows as they are");
+      reinterpret_cast<u32x4e*>(a.out[k])[at * LPR + l] = raw[i];
+    }
+  }
 }
 
 }  // namespace gdn
@@ -138,7 +191,7 @@ int check_cache(const char* name, const void* k_cache, const void* v_cache, cons
     return fail(GDN_ERR_SHAPE, std::string(name) + ": H and page_size must be >= 1, num_pages >= 0");
   if (D != 64 && D != 128 && D != 256)
     return fail(GDN_ERR_SHAPE, std::string(name) + ": D must be 64, 128 or 256");
-  if (H > (1 << 16) || page_size > (1 << 20) || (long long)num_pages * page_size >= (1LL << 40))
+  if (H >= (1 << 16) || page_size > (1 << 20) || (long long)num_pages * page_size >= (1LL << 40))
     return fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
   if (num_pages > 0 && (!k_cache || !v_cache || (bits8 && (!k_scale || !v_scale))))
     return fail(GDN_ERR_NULL, std::string(name) + ": caches, and scales with 8 bits, must be non-NULL");
@@ -154,14 +207,21 @@ namespace {
 int launch_paged(const char* name, bool write, const gdn::PagedArgs& a, int D, int dtype, int cache_dtype,
                  hipStream_t st) {
   const int per = 256 / (D / 8);
-  const long long wgs = (a.rows + per - 1) / per;
-  if (const int fit = gdn_host::check_lanes(name, wgs, 256)) return fit;
-  const dim3 grid((unsigned)wgs, 2);
+  const bool four = (a.T + 4LL * per - 1) / (4 * per) * a.H * 2 >= 4LL * gdn::device_cus();
+  const int tokens = four ? 4 * per : per;
+  const dim3 grid((unsigned)((a.T + (long long)tokens - 1) / tokens), (unsigned)a.H, 2);
+  if (const int fit = gdn_host::check_lanes(name, grid.x, 256)) return fit;
   gdn_host::launch_begin();
+#define GDN_PAGED_U(TT, CC, DD, UU)                                                          \
+  if (write) hipLaunchKernelGGL((gdn::paged_write_kernel<TT, CC, DD, UU>), grid, dim3(256), 0, st, a); \
+  else hipLaunchKernelGGL((gdn::paged_read_kernel<TT, CC, DD, UU>), grid, dim3(256), 0, st, a);
 #define GDN_PAGED(TT, CC, DD)                                                                \
   if (dtype == TT && cache_dtype == CC && D == DD) {                                         \
-    if (write) hipLaunchKernelGGL((gdn::paged_write_kernel<TT, CC, DD>), grid, dim3(256), 0, st, a); \
-    else hipLaunchKernelGGL((gdn::paged_read_kernel<TT, CC, DD>), grid, dim3(256), 0, st, a); \
+    if (four) {                                                                              \
+      GDN_PAGED_U(TT, CC, DD, 4)                                                             \
+    } else {                                                                                 \
+      GDN_PAGED_U(TT, CC, DD, 1)                                                             \
+    }                                                                                        \
     return gdn_host::check_launch(name);                                                     \
   }
 #define GDN_PAGED_D(TT, CC) GDN_PAGED(TT, CC, 64) GDN_PAGED(TT, CC, 128) GDN_PAGED(TT, CC, 256)
@@ -170,6 +230,7 @@ int launch_paged(const char* name, bool write, const gdn::PagedArgs& a, int D, i
   GDN_PAGED_D(GDN_DTYPE_F16, GDN_DTYPE_E4M3) GDN_PAGED_D(GDN_DTYPE_F16, GDN_DTYPE_I8)
 #undef GDN_PAGED_D
 #undef GDN_PAGED
+#undef GDN_PAGED_U
   return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": dtype must be bf16 or f16, and the cache's unless it "
                                                            "has 8 bits");
 }
@@ -191,7 +252,7 @@ extern "C" int gdn_paged_write(const void* k, const void* v, long long k_token, 
   if (!k || !v || !slots)
     return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": k, v and slots must be non-NULL");
   const gdn::PagedArgs a{{k, v}, {k_cache, v_cache}, {k_scale, v_scale}, {k_token, v_token}, {k_head, v_head}, slots,
-                         (long long)T * H, (long long)num_pages * page_size, H, page_size, slots_int64};
+                         (long long)num_pages * page_size, T, H, page_size, slots_int64};
   return launch_paged(name, true, a, D, dtype, cache_dtype, static_cast<hipStream_t>(stream));
 }
 
@@ -208,7 +269,6 @@ extern "C" int gdn_paged_read(const void* k_cache, const void* v_cache, const fl
   if (!k || !v || !slots)
     return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": k, v and slots must be non-NULL");
   const gdn::PagedArgs a{{k_cache, v_cache}, {k, v}, {const_cast<float*>(k_scale), const_cast<float*>(v_scale)},
-                         {0, 0}, {0, 0}, slots, (long long)T * H, (long long)num_pages * page_size, H, page_size,
-                         slots_int64};
+                         {0, 0}, {0, 0}, slots, (long long)num_pages * page_size, T, H, page_size, slots_int64};
   return launch_paged(name, false, a, D, dtype, cache_dtype, static_cast<hipStream_t>(stream));
 }

@@ -46,8 +46,11 @@ __device__ __forceinline__ void st_unit(void* p, long long i, const float (&f)[V
   }
 }
 
+constexpr int kRotaryBatch = 4;   // heads whose loads a lane has on their way
+
 template <int DT, int VEC, bool NEAR>
 __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
+  constexpr int U = kRotaryBatch;
   const int slot = threadIdx.x / a.units, u = threadIdx.x % a.units;
   const long long id = (long long)blockIdx.x * a.per_wg + slot;
   if (slot >= a.per_wg || id >= (long long)a.rows * a.split) return;
@@ -58,6 +61,26 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
   // offsets of the unit's two halves in a head
   const int lo = NEAR || !turn ? 2 * VEC * u : VEC * u;
   const int hi = NEAR || !turn ? lo + VEC : lo + a.R / 2;
+  const int total = a.heads[0] + a.heads[1];
+  long long in[2], out[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    in[k] = b * a.xs[k][0] + t * a.xs[k][1];
+    out[k] = b * a.ys[k][0] + t * a.ys[k][1];
+  }
+  float x[U][VEC], y[U][VEC];
+  auto load = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int head = h + i * a.split;
+      if (head >= total) break;
+      const int k = head >= a.heads[0], hh = k ? head - a.heads[0] : head;
+      const long long at = in[k] + hh * a.xs[k][2];
+      ld_unit<DT, VEC>(a.x[k], at + lo, x[i]);
+      ld_unit<DT, VEC>(a.x[k], at + hi, y[i]);
+    }
+  };
+  load(h0);
   float c[VEC], s[VEC];
   if (turn) {
     const long long pi = b * a.pos_batch + t;
@@ -75,45 +98,46 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
       s[j] *= a.mag * a.sign;
     }
   }
-  const int total = a.heads[0] + a.heads[1];
-  for (int h = h0; h < total; h += a.split) {
-    const int k = h >= a.heads[0], hh = k ? h - a.heads[0] : h;
-    const long long in = b * a.xs[k][0] + t * a.xs[k][1] + hh * a.xs[k][2];
-    const long long out = b * a.ys[k][0] + t * a.ys[k][1] + hh * a.ys[k][2];
-    float x[VEC], y[VEC];
-    ld_unit<DT, VEC>(a.x[k], in + lo, x);
-    ld_unit<DT, VEC>(a.x[k], in + hi, y);
-    if (turn) {
-      if constexpr (NEAR) {
-        // neighbours: pair j is elements 2 j and 2 j + 1 of x and y together
-        float z[2 * VEC];
+  for (int h = h0; h < total; h += U * a.split) {
+    if (h != h0) load(h);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          z[j] = x[j];
-          z[VEC + j] = y[j];
-        }
+    for (int i = 0; i < U; ++i) {
+      const int head = h + i * a.split;
+      if (head >= total) break;
+      if (turn) {
+        if constexpr (NEAR) {
+          // neighbours: pair j is elements 2 j and 2 j + 1 of x and y together
+          float z[2 * VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float p = z[2 * j], q = z[2 * j + 1];
-          z[2 * j] = p * c[j] - q * s[j];
-          z[2 * j + 1] = q * c[j] + p * s[j];
-        }
+          for (int j = 0; j < VEC; ++j) {
+            z[j] = x[i][j];
+            z[VEC + j] = y[i][j];
+          }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          x[j] = z[j];
-          y[j] = z[VEC + j];
-        }
-      } else {
+          for (int j = 0; j < VEC; ++j) {
+            const float p = z[2 * j], q = z[2 * j + 1];
+            z[2 * j] = p * c[j] - q * s[j];
+            z[2 * j + 1] = q * c[j] + p * s[j];
+          }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float p = x[j], q = y[j];
-          x[j] = p * c[j] - q * s[j];
-          y[j] = q * c[j] + p * s[j];
+          for (int j = 0; j < VEC; ++j) {
+            x[i][j] = z[j];
+            y[i][j] = z[VEC + j];
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < VEC; ++j) {
+            const float p = x[i][j], q = y[i][j];
+            x[i][j] = p * c[j] - q * s[j];
+            y[i][j] = q * c[j] + p * s[j];
+          }
         }
       }
+      const int k = head >= a.heads[0], hh = k ? head - a.heads[0] : head;
+      const long long at = out[k] + hh * a.ys[k][2];
+      st_unit<DT, VEC>(a.y[k], at + lo, x[i]);
+      st_unit<DT, VEC>(a.y[k], at + hi, y[i]);
     }
-    st_unit<DT, VEC>(a.y[k], out + lo, x);
-    st_unit<DT, VEC>(a.y[k], out + hi, y);
   }
 }
 
@@ -186,7 +210,7 @@ extern "C" int gdn_rotary(const void* q, const void* k, void* q_out, void* k_out
   // groups of lanes per token: as many heads to a group as leave every CU eight
   // workgroups, eight at most
   const int total = Hq + Hk;
-  const long long want = 8LL * gdn::device_cus() * a.per_wg;
+  const long long want = 4LL * gdn::device_cus() * a.per_wg;
   long long split = (want + a.rows - 1) / a.rows;
   if (split < (total + 7) / 8) split = (total + 7) / 8;
   a.split = (int)(split < total ? split : total);
