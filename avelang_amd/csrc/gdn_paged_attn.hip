@@ -179,9 +179,13 @@ __host__ __device__ constexpr int unit_of(int row_bytes, int rw) {
   return t > kUnit ? t : kUnit;
 }
 
+// Workgroups of a CU, all there are of a call: 256 elements take the registers of
+// two (131072 tokens of bf16 in two rounds of half the length: 55 us, in one 50).
+__host__ __device__ constexpr int resident(int D) { return D == 256 ? 1 : 2; }
+
 // RW: waves of a workgroup that take rows apart (16 each); the others take tokens apart.
 template <int QT, int CT, int D, int RW>
-__global__ __launch_bounds__(256, D == 256 ? 1 : 2)
+__global__ __launch_bounds__(256, resident(D))
 void paged_attn_kernel(PagedAttnArgs a) {
   constexpr bool BF = CT == GDN_DTYPE_BF16;                        // bf16 products
   constexpr bool C8 = CT == GDN_DTYPE_E4M3 || CT == GDN_DTYPE_I8;  // codes with scales
@@ -689,7 +693,7 @@ int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_le
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
   p.items = (long long)N * Hkv * p.rg;
   p.split = units > 1;
-  p.wgs = 2LL * gdn::device_cus();
+  p.wgs = (long long)gdn::resident(D) * gdn::device_cus();
   if (p.wgs > gdn::kMostParts) p.wgs = gdn::kMostParts;
   if (p.wgs > most) p.wgs = most;
   p.desc = (size_t)p.wgs * 16;
