@@ -19,8 +19,6 @@
 // the lengths (read on the device: nothing here depends on a host copy of them).
 // A share that holds a whole (sequence, kv-head) writes its output; parts leave
 // m, the sum and o in the workspace and a second launch joins them.
-#include <type_traits>
-
 #include "gdn_bits8.h"
 #include "gdn_norm_rows.h"
 
@@ -154,6 +152,24 @@ __device__ __forceinline__ uint32_t e4m3_pair(uint32_t w) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI));
 }
 
+// A word's elements of cache type CT that are not finite: 1 at the lowest bit of each.
+template <int CT>
+__device__ __forceinline__ uint32_t broken(uint32_t w) {
+  if constexpr (CT == GDN_DTYPE_E4M3) {
+    return ((w & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u;   // (0x7f alone carries)
+  } else {
+    // (an exponent of ones carries into the sign's place)
+    constexpr uint32_t exp = CT == GDN_DTYPE_BF16 ? 0x7f807f80u : 0x7c007c00u, one = CT == GDN_DTYPE_BF16 ? 0x00800080u : 0x04000400u;
+    return ((w & exp) + one) >> 15 & 0x00010001u;
+  }
+}
+
+// x, of which nothing computed before is kept.
+__device__ __forceinline__ uint32_t again(uint32_t x) {
+  asm("" : "+v"(x));
+  return x;
+}
+
 // Eight codes as an operand.
 template <int CT>
 __device__ __forceinline__ u16x8 codes_operand(uint32_t w0, uint32_t w1) {
@@ -169,13 +185,14 @@ __device__ __forceinline__ u16x8 codes_operand(uint32_t w0, uint32_t w1) {
   return __builtin_bit_cast(u16x8, r);
 }
 
-// Sixteens of tokens that a wave takes at a time, by the bytes of a row: 8 KiB of K and
-// as much of V on their way at once (16 KiB where rows are 512 bytes).  An e4m3 cache of
-// 128 elements, 256 sequences of 4.2 thousand tokens: 415 us, 430 with two sixteens.
-__host__ __device__ constexpr int sixteens(int row_bytes) { return row_bytes <= 128 ? 4 : 2; }
+// Sixteens of tokens that a wave takes at a time, by the bytes of a row and the row tiles
+// (of 16) that it works on: 8 KiB of K and as much of V on their way at once (16 KiB
+// where rows are 512 bytes).  An e4m3 cache of 128 elements, 256 sequences of 4.2
+// thousand tokens: 415 us, 430 with two sixteens.
+__host__ __device__ constexpr int sixteens(int row_bytes, int nt) { return row_bytes <= 128 && nt == 1 ? 4 : 2; }
 // Tokens of a unit of work: a step of all the waves that take tokens apart.
-__host__ __device__ constexpr int unit_of(int row_bytes, int rw) {
-  const int t = 16 * sixteens(row_bytes) * (4 / rw);
+__host__ __device__ constexpr int unit_of(int row_bytes, int nt, int rw) {
+  const int t = 16 * sixteens(row_bytes, nt) * (4 / rw);
   return t > kUnit ? t : kUnit;
 }
 
@@ -183,22 +200,24 @@ __host__ __device__ constexpr int unit_of(int row_bytes, int rw) {
 // two (131072 tokens of bf16 in two rounds of half the length: 55 us, in one 50).
 __host__ __device__ constexpr int resident(int D) { return D == 256 ? 1 : 2; }
 
-// RW: waves of a workgroup that take rows apart (16 each); the others take tokens apart.
-template <int QT, int CT, int D, int RW>
+// NT: tiles of 16 rows that a wave works on with the same K and V; RW: waves of a workgroup
+// that take rows apart, the others take tokens apart.  (32 rows in two waves that both read
+// K and V: 48 sequences of 3 thousand tokens of 128 elements 76 us; in one MEASURED.)
+template <int QT, int CT, int D, int NT, int RW>
 __global__ __launch_bounds__(256, resident(D))
 void paged_attn_kernel(PagedAttnArgs a) {
   constexpr bool BF = CT == GDN_DTYPE_BF16;                        // bf16 products
   constexpr bool C8 = CT == GDN_DTYPE_E4M3 || CT == GDN_DTYPE_I8;  // codes with scales
   constexpr int ES = C8 ? 1 : 2, ROW = D * ES;                     // bytes of an element, of a row
-  constexpr int TW = 4 / RW, UNIT = unit_of(ROW, RW);                                       // waves that take tokens apart
+  constexpr int TW = 4 / RW, UNIT = unit_of(ROW, NT, RW);                                       // waves that take tokens apart
   constexpr int KL = ROW / 64;                                     // 16-byte pieces of K per lane and 16 tokens
   constexpr int E = D / 16;                                        // elements of V per lane and token
   constexpr int VD = E * ES / 4;                                   // words of them
   constexpr int CH = E * ES > 16 ? 16 / ES : E;                    // elements of one piece
-  constexpr int NS = sixteens(ROW), TT = 16 * NS;                  // tokens that a wave takes at a time
+  constexpr int NS = sixteens(ROW, NT), TT = 16 * NS;                  // tokens that a wave takes at a time
   constexpr bool LO = BF || QT == GDN_DTYPE_F16;   // P in two parts: 2^-9 (bf16), 2^-12 of one would show in o
-  __shared__ float buf[4][16][D + 4];
-  __shared__ float sm[4][16], sl[4][16];
+  __shared__ float buf[4][16 * NT][D + 4];
+  __shared__ float sm[4][16 * NT], sl[4][16 * NT];
   __shared__ int wave_sum[4];
   __shared__ int found[2];
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
@@ -257,12 +276,16 @@ void paged_attn_kernel(PagedAttnArgs a) {
     const int kvh = item / a.RG, rg = item % a.RG;
     const int t0 = sp.lo + start * UNIT, t1 = min(t0 + len * UNIT, sp.hi);
 
-    // the rows' queries: column c16 of the operand is row 16 (rg RW + rw) + c16
-    const int rr = 16 * (rg * RW + rw) + c16, l = rr / a.G;
-    const int pos = sp.hi - a.L + l;   // its own place in the sequence
-    u16x8 qf[D / 32];
-    float qscale = a.scale2;
-    {
+    // the rows' queries: column c16 of tile n's operand is row row_of(n)
+    auto row_of = [&](int i) { return 16 * ((rg * RW + rw) * NT + i) + c16; };
+    int pos[NT];   // its own place in the sequence
+    u16x8 qf[NT][D / 32];
+    float qscale[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const int rr = row_of(i), l = rr / a.G;
+      pos[i] = sp.hi - a.L + l;
+      qscale[i] = a.scale2;
       float f[D / 32][8];
       uint32_t m = 0;
       const long long base = n * a.sn + l * a.sl + (kvh * a.G + rr % a.G) * a.sh;
@@ -271,9 +294,9 @@ void paged_attn_kernel(PagedAttnArgs a) {
         const int d = C8 ? 64 * (k / 2) + 16 * g + 8 * (k % 2) : 32 * k + 8 * g;
         if (rr < a.R) {
           if constexpr (C8) ldn<QT, 8>(a.q, base + d, f[k]);
-          else qf[k] = *reinterpret_cast<const u16x8*>(static_cast<const uint16_t*>(a.q) + base + d);
+          else qf[i][k] = *reinterpret_cast<const u16x8*>(static_cast<const uint16_t*>(a.q) + base + d);
         } else {
-          qf[k] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
+          qf[i][k] = u16x8{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
           for (int j = 0; j < 8; ++j) f[k][j] = 0.f;
         }
@@ -291,8 +314,8 @@ void paged_attn_kernel(PagedAttnArgs a) {
 #pragma unroll
         for (int k = 0; k < D / 32; ++k)
 #pragma unroll
-          for (int j = 0; j < 8; ++j) qf[k][j] = f2h(ldexpf(f[k][j], 14 - e));
-        qscale = ldexpf(a.scale2 * (CT == GDN_DTYPE_I8 ? kI8 : 1.f), e - 14);
+          for (int j = 0; j < 8; ++j) qf[i][k][j] = f2h(ldexpf(f[k][j], 14 - e));
+        qscale[i] = ldexpf(a.scale2 * (CT == GDN_DTYPE_I8 ? kI8 : 1.f), e - 14);
       }
     }
 
@@ -363,10 +386,15 @@ void paged_attn_kernel(PagedAttnArgs a) {
       }
     };
 
-    f32x4 acc[E];
+    f32x4 acc[NT][E];
+    float m[NT], sum[NT], vref = 0.f, vinv = 1.f;
 #pragma unroll
-    for (int j = 0; j < E; ++j) acc[j] = zero4();
-    float m = -INFINITY, sum = 0.f, vref = 0.f, vinv = 1.f;
+    for (int i = 0; i < NT; ++i) {
+      m[i] = -INFINITY;
+      sum[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < E; ++j) acc[i][j] = zero4();
+    }
     long long rv[NS];
     if (tiles > 0) {
       look_up(0);
@@ -377,30 +405,30 @@ void paged_attn_kernel(PagedAttnArgs a) {
     }
     for (int it = 0; it < tiles; ++it) {
       const int tb = begin + it * step;
-      f32x4 S[NS];
+      f32x4 S[NT][NS];
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
-        S[s] = zero4();
+#pragma unroll
+        for (int i = 0; i < NT; ++i) S[i][s] = zero4();
 #pragma unroll
         for (int k = 0; k < D / 32; ++k) {
           u16x8 kf;
           if constexpr (C8) kf = codes_operand<CT>(kr[s][k / 2][2 * (k % 2)], kr[s][k / 2][2 * (k % 2) + 1]);
           else kf = __builtin_bit_cast(u16x8, kr[s][k]);
-          S[s] = mfma_t<BF>(kf, qf[k], S[s]);
+#pragma unroll
+          for (int i = 0; i < NT; ++i) S[i][s] = mfma_t<BF>(kf, qf[i][k], S[i][s]);
           if (C8 && k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) S[s][r] *= C8 ? qscale * of_four(kscale[s], r) : qscale;
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) S[i][s][r] *= C8 ? qscale[i] * of_four(kscale[s], r) : qscale[i];
       }
       bool bad = false, here[NS];
 #pragma unroll
       for (int s = 0; s < NS; ++s) {
         here[s] = rows[s] < 0;
         bad |= here[s];
-      }
-      if (it + 1 < tiles) {
-        if ((it + 1) % (64 / NS) == 0) look_up(it + 1);
-        load_k(it + 1);
       }
       // tokens that some row of this wave does not see
       const bool mixed = (a.L > 1 && tb + TT - 1 > sp.hi - a.L) || (a.window > 0 && tb <= sp.hi - 1 - a.window);
@@ -411,15 +439,62 @@ void paged_attn_kernel(PagedAttnArgs a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int t = tb + 16 * s + 4 * g + r;
-            if (here[s]) S[s][r] = __builtin_nanf("");
-            if (t >= t1 || t > pos || (a.window > 0 && t <= pos - a.window)) S[s][r] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+              if (here[s]) S[i][s][r] = __builtin_nanf("");
+              if (t >= t1 || t > pos[i] || (a.window > 0 && t <= pos[i] - a.window)) S[i][s][r] = -INFINITY;
+            }
           }
       }
-      float mx = S[0][0];
+      if constexpr (CT != GDN_DTYPE_I8) {
+        // Where not all rows see all tokens a value of V that is not finite must reach
+        // only those that do (its product with a weight of 0 is NaN): it is taken out, and
+        // its column of theirs is NaN from here on.
+        bool any = false;
+        if (mixed) {
 #pragma unroll
-      for (int i = 1; i < 4 * NS; ++i) mx = fmaxf(mx, S[i / 4][i % 4]);
-      mx = fmaxf(m, xmax16(mx));
-      const float ref = mx == -INFINITY ? 0.f : mx;
+          for (int t = 0; t < 4 * NS; ++t)
+#pragma unroll
+            for (int w = 0; w < VD; ++w) any |= broken<CT>(vr[t][w]) != 0;
+        }
+        if (mixed && __any(any)) {
+#pragma unroll
+          for (int h = 0; h < NS / 2; ++h) {
+            u16x8 ones[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i)
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                ones[i][j] = S[i][2 * h + j / 4][j % 4] == -INFINITY ? (uint16_t)0 : from_f<BF>(1.f);
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+              constexpr int PER = 4 / ES;   // elements of a word
+              u16x8 ind;
+#pragma unroll
+              for (int t = 0; t < 8; ++t) {
+                const uint32_t x = broken<CT>(again(vr[8 * h + t][j / PER])) >> (8 * ES * (j % PER));
+                ind[t] = x & 1 ? from_f<BF>(1.f) : (uint16_t)0;
+              }
+#pragma unroll
+              for (int i = 0; i < NT; ++i) {
+                const f32x4 hit = mfma_t<BF>(ind, ones[i], zero4());
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                  if (hit[r] > 0.f) acc[i][j][r] = __builtin_nanf("");
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int t = 8 * h; t < 8 * h + 8; ++t)
+#pragma unroll
+              for (int w = 0; w < VD; ++w) vr[t][w] &= ~(broken<CT>(again(vr[t][w])) * (ES == 1 ? 0xffu : 0xffffu));
+          }
+        }
+      }
+      if (it + 1 < tiles) {
+        if ((it + 1) % (64 / NS) == 0) look_up(it + 1);
+        load_k(it + 1);
+      }
       float grow = 1.f;
       if constexpr (C8) {
         // V's scales over a power of two no smaller than any so far: P stays in
@@ -438,120 +513,97 @@ void paged_attn_kernel(PagedAttnArgs a) {
           vinv = 1.f / next;
         }
       }
-      if (__any(mx > m) || (C8 && grow != 1.f)) {
-        const float f = exp2i(m - ref);   // (m = -inf: 0)
-        sum *= f;
+      u16x8 hi[NT][NS / 2], lo[NT][NS / 2];
 #pragma unroll
-        for (int j = 0; j < E; ++j) acc[j] *= f * grow;
-        m = mx;
-      }
-      f32x4 p[NS];
+      for (int i = 0; i < NT; ++i) {
+        float mx = S[i][0][0];
 #pragma unroll
-      for (int i = 0; i < 4 * NS; ++i) {
-        float x = exp2i(S[i / 4][i % 4] - ref);
-        sum += x;
-        if constexpr (C8) {
-          // (a token that is not seen may have any scale)
-          const float y = x * (of_four(vscale[i / 4], i % 4) * vinv);
-          x = x == 0.f ? 0.f : y;
+        for (int j = 1; j < 4 * NS; ++j) mx = fmaxf(mx, S[i][j / 4][j % 4]);
+        mx = fmaxf(m[i], xmax16(mx));
+        const float ref = mx == -INFINITY ? 0.f : mx;
+        if (__any(mx > m[i]) || (C8 && grow != 1.f)) {
+          const float f = exp2i(m[i] - ref);   // (m = -inf: 0)
+          sum[i] *= f;
+#pragma unroll
+          for (int j = 0; j < E; ++j) acc[i][j] *= f * grow;
+          m[i] = mx;
         }
-        p[i / 4][i % 4] = x;
-      }
-      u16x8 hi[NS / 2], lo[NS / 2];
+        f32x4 p[NS];
 #pragma unroll
-      for (int h = 0; h < NS / 2; ++h) operands<BF, LO>(p[2 * h], p[2 * h + 1], hi[h], lo[h]);
-      // O^T += V^T P^T;  with `mixed` a value that is not finite reaches only the rows that see its token
-      auto add_v = [&](auto some) {
-        constexpr bool MIX = decltype(some)::value;
-        u16x8 ones[NS / 2];
-        if constexpr (MIX) {
-          // (kept apart from the other branch's conversions, which the compiler would
-          // else form ahead of both and hold in registers all at once)
-#pragma unroll
-          for (int t = 0; t < 4 * NS; ++t)
-#pragma unroll
-            for (int w = 0; w < VD; ++w) asm volatile("" : "+v"(vr[t][w]));
-#pragma unroll
-          for (int i = 0; i < 4 * NS; ++i) ones[i / 8][i % 8] = S[i / 4][i % 4] == -INFINITY ? (uint16_t)0 : from_f<BF>(1.f);
-        }
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-#pragma unroll
-          for (int h = 0; h < NS / 2; ++h) {
-            u32x4w vf;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-              const uint32_t* x = vr[8 * h + 2 * t];
-              const uint32_t* y = vr[8 * h + 2 * t + 1];
-              if constexpr (CT == GDN_DTYPE_E4M3) {
-                const uint32_t w = __builtin_amdgcn_perm(y[j / 4], x[j / 4], j % 4 < 2 ? 0x05010400u : 0x07030602u);
-                vf[t] = j % 2 ? e4m3_pair<true>(w) : e4m3_pair<false>(w);
-              } else if constexpr (CT == GDN_DTYPE_I8) {
-                constexpr uint32_t sel[4] = {0x0c040c00u, 0x0c050c01u, 0x0c060c02u, 0x0c070c03u};
-                vf[t] = i8_pair(__builtin_amdgcn_perm(y[j / 4] ^ 0x80808080u, x[j / 4] ^ 0x80808080u, sel[j % 4]));
-              } else {
-                vf[t] = __builtin_amdgcn_perm(y[j / 2], x[j / 2], j % 2 ? 0x07060302u : 0x05040100u);
-              }
-            }
-            u16x8 v = __builtin_bit_cast(u16x8, vf);
-            if constexpr (MIX) {
-              constexpr uint16_t kExp = BF ? 0x7f80 : 0x7c00;
-              u16x8 ind;
-              bool any = false;
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const bool x = (v[i] & kExp) == kExp;
-                any |= x;
-                ind[i] = x ? from_f<BF>(1.f) : (uint16_t)0;
-                v[i] = x ? (uint16_t)0 : v[i];
-              }
-              if (__any(any)) {
-                const f32x4 hit = mfma_t<BF>(ind, ones[h], zero4());
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                  if (hit[r] > 0.f) acc[j][r] = __builtin_nanf("");
-              }
-            }
-            acc[j] = mfma_t<BF>(v, hi[h], acc[j]);
-            if constexpr (LO) acc[j] = mfma_t<BF>(v, lo[h], acc[j]);
+        for (int j = 0; j < 4 * NS; ++j) {
+          float x = exp2i(S[i][j / 4][j % 4] - ref);
+          sum[i] += x;
+          if constexpr (C8) {
+            // (a token that is not seen may have any scale)
+            const float y = x * (of_four(vscale[j / 4], j % 4) * vinv);
+            x = x == 0.f ? 0.f : y;
           }
-          // (conversions beside their products, not all ahead of them: registers)
-          if (j % 2) __builtin_amdgcn_sched_barrier(0);
+          p[j / 4][j % 4] = x;
         }
-      };
-      if (mixed) add_v(std::true_type{});
-      else add_v(std::false_type{});
+#pragma unroll
+        for (int h = 0; h < NS / 2; ++h) operands<BF, LO>(p[2 * h], p[2 * h + 1], hi[i][h], lo[i][h]);
+      }
+      // O^T += V^T P^T
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+#pragma unroll
+        for (int h = 0; h < NS / 2; ++h) {
+          u32x4w vf;
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const uint32_t* x = vr[8 * h + 2 * t];
+            const uint32_t* y = vr[8 * h + 2 * t + 1];
+            if constexpr (CT == GDN_DTYPE_E4M3) {
+              const uint32_t w = __builtin_amdgcn_perm(y[j / 4], x[j / 4], j % 4 < 2 ? 0x05010400u : 0x07030602u);
+              vf[t] = j % 2 ? e4m3_pair<true>(w) : e4m3_pair<false>(w);
+            } else if constexpr (CT == GDN_DTYPE_I8) {
+              constexpr uint32_t sel[4] = {0x0c040c00u, 0x0c050c01u, 0x0c060c02u, 0x0c070c03u};
+              vf[t] = i8_pair(__builtin_amdgcn_perm(y[j / 4] ^ 0x80808080u, x[j / 4] ^ 0x80808080u, sel[j % 4]));
+            } else {
+              vf[t] = __builtin_amdgcn_perm(y[j / 2], x[j / 2], j % 2 ? 0x07060302u : 0x05040100u);
+            }
+          }
+          const u16x8 v = __builtin_bit_cast(u16x8, vf);
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            acc[i][j] = mfma_t<BF>(v, hi[i][h], acc[i][j]);
+            if constexpr (LO) acc[i][j] = mfma_t<BF>(v, lo[i][h], acc[i][j]);
+          }
+        }
+        // (conversions beside their products, not all ahead of them: registers)
+        if (j % 2) __builtin_amdgcn_sched_barrier(0);
+      }
       if (it + 1 < tiles) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) rv[s] = rows[s];
         load_v(rv, it + 1);
       }
     }
-    sum = xsum16(sum);
-    if constexpr (C8) {
+    // the waves' parts joined: D's element of lane (c16, g), r of acc[i][j] is
+    // (j / CH) 16 CH + (4 g + r) CH + j % CH of row c16 of tile i
 #pragma unroll
-      for (int j = 0; j < E; ++j) acc[j] *= vref * (CT == GDN_DTYPE_I8 ? kI8 : 1.f);
-    }
-
-    // the waves' parts joined: D's element of lane (c16, g), r of acc[j] is
-    // (j / CH) 16 CH + (4 g + r) CH + j % CH of row c16
-    if (g == 0) {
-      sm[wave][c16] = m;
-      sl[wave][c16] = sum;
-    }
-    if (rr < a.R) {
+    for (int i = 0; i < NT; ++i) {
+      sum[i] = xsum16(sum[i]);
+      if (g == 0) {
+        sm[wave][16 * i + c16] = m[i];
+        sl[wave][16 * i + c16] = sum[i];
+      }
+      if (row_of(i) < a.R) {
 #pragma unroll
-      for (int j = 0; j < E; ++j)
+        for (int j = 0; j < E; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) buf[wave][c16][(j / CH) * 16 * CH + (4 * g + r) * CH + j % CH] = acc[j][r];
+          for (int r = 0; r < 4; ++r)
+            buf[wave][16 * i + c16][(j / CH) * 16 * CH + (4 * g + r) * CH + j % CH] =
+                acc[i][j][r] * (C8 ? vref * (CT == GDN_DTYPE_I8 ? kI8 : 1.f) : 1.f);
+      }
     }
     __syncthreads();
     const bool whole = len == sp.units;
     const int slot = u == u0 ? 2 * blockIdx.x : 2 * blockIdx.x + 1;
     float* const part = a.part + (size_t)slot * a.rows * (D + 2);
-    const int here = min(a.R - 16 * RW * rg, 16 * RW);   // rows of this group
+    const int group = 16 * RW * NT, here = min(a.R - group * rg, group);   // rows of this group
     for (int i = tid; i < here * (D / 4); i += 256) {
-      const int row = i / (D / 4), d = 4 * (i % (D / 4)), w0 = row / 16, c = row % 16;
+      const int row = i / (D / 4), d = 4 * (i % (D / 4)), w0 = row / (16 * NT), c = row % (16 * NT);
       float M = sm[w0][c];
 #pragma unroll
       for (int w = 1; w < TW; ++w) M = fmaxf(M, sm[w0 + w * RW][c]);
@@ -564,7 +616,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
         s += f * sl[w0 + w * RW][c];
         o += f * *reinterpret_cast<const f32x4*>(&buf[w0 + w * RW][c][d]);
       }
-      const int orow = 16 * RW * rg + row;
+      const int orow = group * rg + row;
       const long long at = ((long long)n * a.L + orow / a.G) * a.Hq + kvh * a.G + orow % a.G;
       if (whole) {
         o *= s == 0.f ? 0.f : 1.f / s;
@@ -668,7 +720,7 @@ namespace {
 
 // Workgroups, and how the rows of a kv-head are laid over their waves.
 struct AttnPlan {
-  int rw, rg, rows;
+  int nt, rw, rg, rows;
   long long wgs, items;
   bool split;   // some work may be cut
   size_t desc, bytes;
@@ -683,10 +735,12 @@ int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_le
   const long long R = (long long)L * (Hq / Hkv);
   if (R > (1 << 20) || max_length > (1 << 30) || Hq > (1 << 20))
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
-  p.rw = R <= 16 ? 1 : R <= 32 ? 2 : 4;
-  p.rg = (int)((R + 16 * p.rw - 1) / (16 * p.rw));
-  p.rows = (int)(R < 16 * p.rw ? R : 16 * p.rw);
-  const int unit = row_bytes ? gdn::unit_of(row_bytes, p.rw) : gdn::kUnit;   // (0: the smallest)
+  p.nt = R <= 16 ? 1 : 2;
+  p.rw = R <= 32 ? 1 : 2;
+  const int group = 16 * p.nt * p.rw;
+  p.rg = (int)((R + group - 1) / group);
+  p.rows = (int)(R < group ? R : group);
+  const int unit = row_bytes ? gdn::unit_of(row_bytes, p.nt, p.rw) : gdn::kUnit;   // (0: the smallest)
   const long long units = ((long long)max_length + unit - 1) / unit;
   const long long most = (units ? units : 1) * N * Hkv * p.rg;
   if (most >= (1LL << 30))
@@ -784,12 +838,12 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long long q_seq, long long q_to
   auto st = static_cast<hipStream_t>(stream);
   gdn_host::launch_begin();
   bool done = false;
-#define GDN_PA(QQ, CC, DD, WW)                                                                    \
-  if (dtype == QQ && cache_dtype == CC && D == DD && p.rw == WW) {                                \
-    hipLaunchKernelGGL((gdn::paged_attn_kernel<QQ, CC, DD, WW>), dim3((unsigned)p.wgs), dim3(256), 0, st, a); \
+#define GDN_PA(QQ, CC, DD, TT, WW)                                                                \
+  if (dtype == QQ && cache_dtype == CC && D == DD && p.nt == TT && p.rw == WW) {                  \
+    hipLaunchKernelGGL((gdn::paged_attn_kernel<QQ, CC, DD, TT, WW>), dim3((unsigned)p.wgs), dim3(256), 0, st, a); \
     done = true;                                                                                  \
   }
-#define GDN_PA_W(QQ, CC, DD) GDN_PA(QQ, CC, DD, 1) GDN_PA(QQ, CC, DD, 2) GDN_PA(QQ, CC, DD, 4)
+#define GDN_PA_W(QQ, CC, DD) GDN_PA(QQ, CC, DD, 1, 1) GDN_PA(QQ, CC, DD, 2, 1) GDN_PA(QQ, CC, DD, 2, 2)
 #define GDN_PA_D(QQ, CC) GDN_PA_W(QQ, CC, 64) GDN_PA_W(QQ, CC, 128) GDN_PA_W(QQ, CC, 256)
   GDN_PA_D(GDN_DTYPE_BF16, GDN_DTYPE_BF16)
   GDN_PA_D(GDN_DTYPE_F16, GDN_DTYPE_F16)
