@@ -202,7 +202,8 @@ __host__ __device__ constexpr int resident(int D) { return D == 256 ? 1 : 2; }
 
 // NT: tiles of 16 rows that a wave works on with the same K and V; RW: waves of a workgroup
 // that take rows apart, the others take tokens apart.  (32 rows in two waves that both read
-// K and V: 48 sequences of 3 thousand tokens of 128 elements 76 us; in one MEASURED.)
+// K and V, or in one: 48 sequences of 125 to 6000 tokens of 128 elements 76 us either way; the
+// one leaves the other registers' worth of loads on their way.)
 template <int QT, int CT, int D, int NT, int RW>
 __global__ __launch_bounds__(256, resident(D))
 void paged_attn_kernel(PagedAttnArgs a) {
@@ -228,7 +229,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
 
   // this workgroup's share of all units
   const int HG = a.Hkv * a.RG;
-  int total, u0, u1, share, n, prefix;
+  int u0, u1, share, n, prefix, extra;
   {
     const int per = (a.N + 255) / 256, first = tid * per, last = min(first + per, a.N);
     int sum = 0;
@@ -241,23 +242,28 @@ void paged_attn_kernel(PagedAttnArgs a) {
     }
     if (lane == 63) wave_sum[wave] = incl;
     __syncthreads();
-    total = 0;
+    int units = 0;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       if (w < wave) incl += wave_sum[w];
-      total += wave_sum[w];
+      units += wave_sum[w];
     }
-    total = __builtin_amdgcn_readfirstlane(total) * HG;
+    units = __builtin_amdgcn_readfirstlane(units);
+    // a workgroup's queries, first loads and output take about a unit's time: where
+    // shares are of several units each (sequence, kv-head) counts one more, ahead of
+    // its own.  (48 sequences of 125 to 6000 tokens: 95 us, with it 76.)
+    extra = units * HG > (int)gridDim.x;
+    const int total = (units + extra * a.N) * HG;
     share = (total + gridDim.x - 1) / gridDim.x;
     u0 = min((int)blockIdx.x * share, total);
     u1 = min(u0 + share, total);
     if (tid == 0 && !a.by_item) a.desc[blockIdx.x] = int4{0, 0, 0, 0};
     if (u0 >= u1) return;
-    int at = incl - sum;
-    if (at * HG <= u0 && u0 < incl * HG) {
+    int at = incl - sum + extra * min(first, a.N);
+    if (at * HG <= u0 && u0 < (incl + extra * last) * HG) {
       int i = first;
       for (;; ++i) {
-        const int un = span_of<UNIT>(a, i).units;
+        const int un = span_of<UNIT>(a, i).units + extra;
         if (u0 < (at + un) * HG) break;
         at += un;
       }
@@ -271,10 +277,11 @@ void paged_attn_kernel(PagedAttnArgs a) {
 
   for (int u = u0; u < u1;) {
     const Span sp = span_of<UNIT>(a, n);
-    const int rel = u - prefix * HG, item = rel / sp.units, start = rel % sp.units;
-    const int len = min(sp.units - start, u1 - u);
+    const int cost = sp.units + extra;
+    const int rel = u - prefix * HG, item = rel / cost, start = rel % cost;
+    const int len = min(cost - start, u1 - u);
     const int kvh = item / a.RG, rg = item % a.RG;
-    const int t0 = sp.lo + start * UNIT, t1 = min(t0 + len * UNIT, sp.hi);
+    const int t0 = sp.lo + max(start - extra, 0) * UNIT, t1 = min(sp.lo + (start + len - extra) * UNIT, sp.hi);
 
     // the rows' queries: column c16 of tile n's operand is row row_of(n)
     auto row_of = [&](int i) { return 16 * ((rg * RW + rw) * NT + i) + c16; };
@@ -598,7 +605,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
       }
     }
     __syncthreads();
-    const bool whole = len == sp.units;
+    const bool whole = len == cost;
     const int slot = u == u0 ? 2 * blockIdx.x : 2 * blockIdx.x + 1;
     float* const part = a.part + (size_t)slot * a.rows * (D + 2);
     const int group = 16 * RW * NT, here = min(a.R - group * rg, group);   // rows of this group
@@ -636,10 +643,10 @@ void paged_attn_kernel(PagedAttnArgs a) {
     // what the joining launch has to do: {sequence, item, first part's slot, parts}
     if (start == 0 && tid == 0 && (!whole || a.by_item))
       a.desc[a.by_item ? n * HG + item : blockIdx.x] =
-          int4{n, item, slot, whole ? 0 : 1 + (sp.units - len + share - 1) / share};
+          int4{n, item, slot, whole ? 0 : 1 + (cost - len + share - 1) / share};
     u += len;
-    if (item == HG - 1 && start + len == sp.units) {
-      prefix += sp.units;
+    if (item == HG - 1 && start + len == cost) {
+      prefix += cost;
       ++n;
     }
     __syncthreads();
@@ -649,6 +656,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
 // Parts of one (sequence, kv-head) joined: block (entry of desc, row).  D / 4 lanes
 // hold a row of a part, NT / (D / 4) parts are added at a time.
 constexpr int kMostParts = 1024;   // workgroups at most
+constexpr int kFewParts = 6;
 template <int QT, int D, int NT>
 __global__ __launch_bounds__(NT) void paged_attn_join_kernel(PagedAttnArgs a) {
   constexpr int LP = D / 4, GR = NT / LP, NW = NT / 64;
@@ -659,13 +667,51 @@ __global__ __launch_bounds__(NT) void paged_attn_join_kernel(PagedAttnArgs a) {
   const int parts = ds.w;
   if (parts == 0) return;
   const int kvh = ds.y / a.RG, rg = ds.y % a.RG, row = blockIdx.y;
-  const int orow = rg * a.rows + row;
-  if (orow >= a.R) return;
   const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, col = tid % LP, grp = tid / LP;
   const size_t each = (size_t)a.rows * (D + 2);
   // part p: its workgroup's first, but for the one that begins here
   const int wg = ds.z / 2;
   auto at = [&](int p) { return a.part + (p == 0 ? ds.z : 2 * (wg + p)) * each; };
+  auto put = [&](int orow, float M, float s, f32x4 o) {
+    o *= s == 0.f ? 0.f : 1.f / s;
+    const long long out = ((long long)ds.x * a.L + orow / a.G) * a.Hq + kvh * a.G + orow % a.G;
+    u16x4 h;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) h[j] = Elt<QT>::from_f(o[j]);
+    *reinterpret_cast<u16x4*>(static_cast<uint16_t*>(a.o) + out * D + 4 * col) = h;
+    if (a.lse && col == 0) a.lse[out] = s == 0.f ? -INFINITY : (M + log2f(s)) * 0.69314718055994530942f;
+  };
+  if (parts <= kFewParts) {
+    // few parts: a row to each group of lanes, the groups' rows with the first one's block
+    const int r = row + grp, orow = rg * a.rows + r;
+    if (row % GR || r >= a.rows || orow >= a.R) return;
+    float m[kFewParts], l[kFewParts], M = -INFINITY;
+    f32x4 x[kFewParts];
+#pragma unroll
+    for (int p = 0; p < kFewParts; ++p) {
+      if (p >= parts) break;
+      m[p] = at(p)[a.rows * D + r];
+      l[p] = at(p)[a.rows * (D + 1) + r];
+      x[p] = *reinterpret_cast<const f32x4*>(at(p) + r * D + 4 * col);
+    }
+#pragma unroll
+    for (int p = 0; p < kFewParts; ++p)
+      if (p < parts) M = fmaxf(M, m[p]);
+    const float ref = M == -INFINITY ? 0.f : M;
+    float s = 0.f;
+    f32x4 o = zero4();
+#pragma unroll
+    for (int p = 0; p < kFewParts; ++p) {
+      if (p >= parts) break;
+      const float f = exp2i(m[p] - ref);
+      s += f * l[p];
+      o += f * x[p];
+    }
+    put(orow, M, s, o);
+    return;
+  }
+  const int orow = rg * a.rows + row;
+  if (orow >= a.R) return;
   float M = -INFINITY;
   for (int p = tid; p < parts; p += NT) {
     const float m = at(p)[a.rows * D + row];
@@ -700,13 +746,7 @@ __global__ __launch_bounds__(NT) void paged_attn_join_kernel(PagedAttnArgs a) {
   for (int i = 0; i < NW; ++i) s += red[1][i];
 #pragma unroll
   for (int i = 1; i < GR; ++i) o += acc[i][col];
-  o *= s == 0.f ? 0.f : 1.f / s;
-  const long long out = ((long long)ds.x * a.L + orow / a.G) * a.Hq + kvh * a.G + orow % a.G;
-  u16x4 h;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) h[j] = Elt<QT>::from_f(o[j]);
-  *reinterpret_cast<u16x4*>(static_cast<uint16_t*>(a.o) + out * D + 4 * col) = h;
-  if (a.lse && tid == 0) a.lse[out] = s == 0.f ? -INFINITY : (M + log2f(s)) * 0.69314718055994530942f;
+  put(orow, M, s, o);
 }
 
 }  // namespace gdn
@@ -743,7 +783,7 @@ int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_le
   const int unit = row_bytes ? gdn::unit_of(row_bytes, p.nt, p.rw) : gdn::kUnit;   // (0: the smallest)
   const long long units = ((long long)max_length + unit - 1) / unit;
   const long long most = (units ? units : 1) * N * Hkv * p.rg;
-  if (most >= (1LL << 30))
+  if (most + (long long)N * Hkv * p.rg >= (1LL << 30))
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
   p.items = (long long)N * Hkv * p.rg;
   p.split = units > 1;
