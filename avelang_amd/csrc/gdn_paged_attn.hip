@@ -166,7 +166,7 @@ __device__ __forceinline__ uint32_t broken(uint32_t w) {
 
 // x, of which nothing computed before is kept.
 __device__ __forceinline__ uint32_t again(uint32_t x) {
-  asm("" : "+v"(x));
+  asm volatile("" : "+v"(x));
   return x;
 }
 
