@@ -179,6 +179,15 @@ extern "C" int gdn_rotary(const void* q, const void* k, void* q_out, void* k_out
   }
   if (two == 2 && y[0] == y[1])
     return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": the two outputs must not be one");
+  const int es = dtype == GDN_DTYPE_F32 ? 4 : 2;
+  auto bytes = [&](const long long* st, int h) {
+    return (size_t)((B - 1) * st[0] + (T - 1) * st[1] + (h - 1) * st[2] + D) * es;
+  };
+  if (!inplace)
+    for (int i = 0; i < two; ++i)
+      for (int j = 0; j < two; ++j)
+        if (gdn_host::overlaps(y[i], bytes(ys + 3 * i, heads[i]), x[j], bytes(xs + 3 * j, heads[j])))
+          return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": outputs must not overlap an input, but in place");
   // the widest units that divide both parts of a head: 16 bytes of each half, 2
   // elements, or 1
   const int full = dtype == GDN_DTYPE_F32 ? 4 : 8;
