@@ -42,6 +42,7 @@ struct PagedAttnArgs {
   int4* desc;
   int N, L, Hq, Hkv, G, R, RG, rows;   // R = L G rows per kv-head in RG groups of at most `rows`
   int num_pages, page, cap, window;
+  int split;      // work may be cut (else there is no second launch)
   int by_item;    // desc has an entry per (sequence, kv-head, group of rows), not per workgroup
   float scale2;   // scale log2(e)
 };
@@ -252,7 +253,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
     // a workgroup's queries, first loads and output take about a unit's time: where
     // shares are of several units each (sequence, kv-head) counts one more, ahead of
     // its own.  (48 sequences of 125 to 6000 tokens: 95 us, with it 76.)
-    extra = units * HG > (int)gridDim.x;
+    extra = a.split && units * HG > (int)gridDim.x;
     const int total = (units + extra * a.N) * HG;
     share = (total + gridDim.x - 1) / gridDim.x;
     u0 = min((int)blockIdx.x * share, total);
@@ -872,6 +873,7 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long long q_seq, long long q_to
   a.num_pages = num_pages;
   a.page = page_size;
   a.cap = max_length;
+  a.split = p.split;
   a.by_item = p.items <= p.wgs;
   a.window = window > (1 << 30) ? 1 << 30 : window;
   a.scale2 = scale * 1.44269504088896340736f;

@@ -97,6 +97,16 @@ def test_long_and_uneven(rocm_device, t, code):
     _check(o, lse, q, cache, table, n)
 
 
+@pytest.mark.parametrize("t,code", CODES)
+@pytest.mark.parametrize("most", [18, 100, 400, 900])
+def test_many_short(rocm_device, most, t, code):
+    """More sequences than workgroups, of a few units each or of one."""
+    lens = [(7 * i) % most + (i % 5 != 0) for i in range(400)]
+    q, cache, table, n = _case(lens, 1, 4, 2, 128, 16, t, code, seed=3)
+    o, lse = ave.paged_attention(q, cache, table, n, return_lse=True)
+    _check(o, lse, q, cache, table, n)
+
+
 @pytest.mark.parametrize("L,Hq,H", [(16, 8, 2), (64, 4, 1), (40, 16, 2)])
 def test_many_rows(rocm_device, L, Hq, H):
     """More rows to a kv-head than the waves of one workgroup take."""
