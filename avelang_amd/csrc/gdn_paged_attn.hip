@@ -211,27 +211,32 @@ void paged_attn_kernel(PagedAttnArgs a) {
   constexpr bool BF = CT == GDN_DTYPE_BF16;                        // bf16 products
   constexpr bool C8 = CT == GDN_DTYPE_E4M3 || CT == GDN_DTYPE_I8;  // codes with scales
   constexpr int ES = C8 ? 1 : 2, ROW = D * ES;                     // bytes of an element, of a row
-  constexpr int TW = 4 / RW, UNIT = unit_of(ROW, NT, RW);                                       // waves that take tokens apart
+  constexpr bool EACH = RW == 0;                                   // every wave on its own
+  constexpr int RWS = EACH ? 1 : RW, TW = EACH ? 1 : 4 / RW;       // waves that take tokens apart
+  constexpr int UNIT = unit_of(ROW, NT, RWS);
   constexpr int KL = ROW / 64;                                     // 16-byte pieces of K per lane and 16 tokens
   constexpr int E = D / 16;                                        // elements of V per lane and token
   constexpr int VD = E * ES / 4;                                   // words of them
   constexpr int CH = E * ES > 16 ? 16 / ES : E;                    // elements of one piece
-  constexpr int NS = sixteens(ROW, NT), TT = 16 * NS;                  // tokens that a wave takes at a time
+  constexpr int NS = sixteens(ROW, NT), TT = 16 * NS;              // tokens that a wave takes at a time
   constexpr bool LO = BF || QT == GDN_DTYPE_F16;   // P in two parts: 2^-9 (bf16), 2^-12 of one would show in o
-  __shared__ float buf[4][16 * NT][D + 4];
+  __shared__ float buf[EACH ? 1 : 4][EACH ? 1 : 16 * NT][D + 4];
   __shared__ float sm[4][16 * NT], sl[4][16 * NT];
   __shared__ int wave_sum[4];
   __shared__ int found[2];
   const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const int c16 = lane % 16, g = lane / 16;
-  const int ts = wave / RW, rw = wave % RW;
+  const int ts = EACH ? 0 : wave / RWS, rw = EACH ? 0 : wave % RWS;
   const char* const kc = static_cast<const char*>(a.kc);
   const char* const vc = static_cast<const char*>(a.vc);
 
   // this workgroup's share of all units
   const int HG = a.Hkv * a.RG;
-  int u0, u1, share, n, prefix, extra;
-  {
+  int u0, u1, share = 1, n = 0, prefix = 0, extra = 0;
+  if constexpr (EACH) {
+    u0 = blockIdx.x * 4 + wave;
+    u1 = a.N * HG;
+  } else {
     const int per = (a.N + 255) / 256, first = tid * per, last = min(first + per, a.N);
     int sum = 0;
     for (int i = first; i < last; ++i) sum += span_of<UNIT>(a, i).units;
@@ -277,15 +282,16 @@ void paged_attn_kernel(PagedAttnArgs a) {
   }
 
   for (int u = u0; u < u1;) {
+    if constexpr (EACH) n = u / HG;
     const Span sp = span_of<UNIT>(a, n);
     const int cost = sp.units + extra;
-    const int rel = u - prefix * HG, item = rel / cost, start = rel % cost;
-    const int len = min(cost - start, u1 - u);
+    const int rel = u - prefix * HG, item = EACH ? u % HG : rel / cost, start = EACH ? 0 : rel % cost;
+    const int len = EACH ? cost : min(cost - start, u1 - u);
     const int kvh = item / a.RG, rg = item % a.RG;
     const int t0 = sp.lo + max(start - extra, 0) * UNIT, t1 = min(sp.lo + (start + len - extra) * UNIT, sp.hi);
 
     // the rows' queries: column c16 of tile n's operand is row row_of(n)
-    auto row_of = [&](int i) { return 16 * ((rg * RW + rw) * NT + i) + c16; };
+    auto row_of = [&](int i) { return 16 * ((rg * RWS + rw) * NT + i) + c16; };
     int pos[NT];   // its own place in the sequence
     u16x8 qf[NT][D / 32];
     float qscale[NT];
@@ -587,8 +593,32 @@ void paged_attn_kernel(PagedAttnArgs a) {
         load_v(rv, it + 1);
       }
     }
-    // the waves' parts joined: D's element of lane (c16, g), r of acc[i][j] is
-    // (j / CH) 16 CH + (4 g + r) CH + j % CH of row c16 of tile i
+    // D's element of lane (c16, g), r of acc[i][j] is (j / CH) 16 CH + (4 g + r) CH +
+    // j % CH of row c16 of tile i
+    if constexpr (EACH) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const float s = xsum16(sum[i]);
+        const float f = s == 0.f ? 0.f : 1.f / s * (C8 ? vref * (CT == GDN_DTYPE_I8 ? kI8 : 1.f) : 1.f);
+        const int orow = row_of(i);
+        if (orow >= a.R) continue;
+        const long long at = ((long long)n * a.L + orow / a.G) * a.Hq + kvh * a.G + orow % a.G;
+#pragma unroll
+        for (int j = 0; j < E; j += 4)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            u16x4 h;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) h[x] = Elt<QT>::from_f(acc[i][j + x][r] * f);
+            *reinterpret_cast<u16x4*>(static_cast<uint16_t*>(a.o) + at * D + (j / CH) * 16 * CH + (4 * g + r) * CH +
+                                      j % CH) = h;
+          }
+        if (a.lse && g == 0) a.lse[at] = s == 0.f ? -INFINITY : (m[i] + log2f(s)) * 0.69314718055994530942f;
+      }
+      u += 4 * gridDim.x;
+      continue;
+    }
+    // the waves' parts joined
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       sum[i] = xsum16(sum[i]);
@@ -609,20 +639,20 @@ void paged_attn_kernel(PagedAttnArgs a) {
     const bool whole = len == cost;
     const int slot = u == u0 ? 2 * blockIdx.x : 2 * blockIdx.x + 1;
     float* const part = a.part + (size_t)slot * a.rows * (D + 2);
-    const int group = 16 * RW * NT, here = min(a.R - group * rg, group);   // rows of this group
+    const int group = 16 * RWS * NT, here = min(a.R - group * rg, group);   // rows of this group
     for (int i = tid; i < here * (D / 4); i += 256) {
       const int row = i / (D / 4), d = 4 * (i % (D / 4)), w0 = row / (16 * NT), c = row % (16 * NT);
       float M = sm[w0][c];
 #pragma unroll
-      for (int w = 1; w < TW; ++w) M = fmaxf(M, sm[w0 + w * RW][c]);
+      for (int w = 1; w < TW; ++w) M = fmaxf(M, sm[w0 + w * RWS][c]);
       const float ref = M == -INFINITY ? 0.f : M;
       float s = 0.f;
       f32x4 o = zero4();
 #pragma unroll
       for (int w = 0; w < TW; ++w) {
-        const float f = exp2i(sm[w0 + w * RW][c] - ref);
-        s += f * sl[w0 + w * RW][c];
-        o += f * *reinterpret_cast<const f32x4*>(&buf[w0 + w * RW][c][d]);
+        const float f = exp2i(sm[w0 + w * RWS][c] - ref);
+        s += f * sl[w0 + w * RWS][c];
+        o += f * *reinterpret_cast<const f32x4*>(&buf[w0 + w * RWS][c][d]);
       }
       const int orow = group * rg + row;
       const long long at = ((long long)n * a.L + orow / a.G) * a.Hq + kvh * a.G + orow % a.G;
@@ -759,11 +789,14 @@ int check_cache(const char* name, const void* k_cache, const void* v_cache, cons
 
 namespace {
 
+constexpr int kEachMost = 1024;
+
 // Workgroups, and how the rows of a kv-head are laid over their waves.
 struct AttnPlan {
   int nt, rw, rg, rows;
   long long wgs, items;
   bool split;   // some work may be cut
+  bool each;    // every wave on its own
   size_t desc, bytes;
 };
 int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_length, int row_bytes, AttnPlan& p) {
@@ -787,10 +820,16 @@ int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_le
   if (most + (long long)N * Hkv * p.rg >= (1LL << 30))
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
   p.items = (long long)N * Hkv * p.rg;
-  p.split = units > 1;
+  // short sequences in numbers: a wave to each (sequence, kv-head), as many at once as
+  // there are waves, nothing joined.  256 sequences of 8 heads of 128: e4m3, 2 to 600
+  // tokens 43 us (in shares 56), to 100 tokens 12.5 (25.6), to 1000 69 (76); bf16 to 500
+  // 62 either way; rows of 512 bytes leave half of the waves (380, in shares 368).
+  p.each = row_bytes && row_bytes <= 256 && p.nt == 1 && p.items >= 4LL * gdn::device_cus() && max_length <= kEachMost;
+  p.split = units > 1 && !p.each;
   p.wgs = (long long)gdn::resident(D) * gdn::device_cus();
   if (p.wgs > gdn::kMostParts) p.wgs = gdn::kMostParts;
   if (p.wgs > most) p.wgs = most;
+  if (p.each && p.wgs > (p.items + 3) / 4) p.wgs = (p.items + 3) / 4;
   p.desc = (size_t)p.wgs * 16;
   p.bytes = p.desc + (size_t)p.wgs * 2 * p.rows * (D + 2) * sizeof(float);
   p.bytes = (p.bytes + 255) / 256 * 256;
@@ -881,11 +920,11 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long long q_seq, long long q_to
   gdn_host::launch_begin();
   bool done = false;
 #define GDN_PA(QQ, CC, DD, TT, WW)                                                                \
-  if (dtype == QQ && cache_dtype == CC && D == DD && p.nt == TT && p.rw == WW) {                  \
+  if (dtype == QQ && cache_dtype == CC && D == DD && p.nt == TT && (p.each ? 0 : p.rw) == WW) {   \
     hipLaunchKernelGGL((gdn::paged_attn_kernel<QQ, CC, DD, TT, WW>), dim3((unsigned)p.wgs), dim3(256), 0, st, a); \
     done = true;                                                                                  \
   }
-#define GDN_PA_W(QQ, CC, DD) GDN_PA(QQ, CC, DD, 1, 1) GDN_PA(QQ, CC, DD, 2, 1) GDN_PA(QQ, CC, DD, 2, 2)
+#define GDN_PA_W(QQ, CC, DD) GDN_PA(QQ, CC, DD, 1, 0) GDN_PA(QQ, CC, DD, 1, 1) GDN_PA(QQ, CC, DD, 2, 1) GDN_PA(QQ, CC, DD, 2, 2)
 #define GDN_PA_D(QQ, CC) GDN_PA_W(QQ, CC, 64) GDN_PA_W(QQ, CC, 128) GDN_PA_W(QQ, CC, 256)
   GDN_PA_D(GDN_DTYPE_BF16, GDN_DTYPE_BF16)
   GDN_PA_D(GDN_DTYPE_F16, GDN_DTYPE_F16)

@@ -98,13 +98,30 @@ def test_long_and_uneven(rocm_device, t, code):
 
 
 @pytest.mark.parametrize("t,code", CODES)
-@pytest.mark.parametrize("most", [18, 100, 400, 900])
-def test_many_short(rocm_device, most, t, code):
-    """More sequences than workgroups, of a few units each or of one."""
-    lens = [(7 * i) % most + (i % 5 != 0) for i in range(400)]
-    q, cache, table, n = _case(lens, 1, 4, 2, 128, 16, t, code, seed=3)
+@pytest.mark.parametrize("D,most", [(128, 18), (64, 100), (128, 400), (256, 100), (128, 1100)])
+def test_many_short(rocm_device, D, most, t, code):
+    """More sequences than workgroups, of a few units each or of one, a wave to each or in shares."""
+    lens = [(7 * i) % most + (i % 5 != 0) for i in range(530)]
+    q, cache, table, n = _case(lens, 1, 4, 2, D, 16, t, code, seed=3)
     o, lse = ave.paged_attention(q, cache, table, n, return_lse=True)
     _check(o, lse, q, cache, table, n)
+
+
+@pytest.mark.parametrize("t,code", [(BF16, BF16), (F16, I8), (BF16, E4M3)])
+@pytest.mark.parametrize("L,window", [(3, 0), (2, 40)])
+def test_many_short_drafts(rocm_device, L, window, t, code):
+    lens = [(11 * i) % 150 for i in range(520)]
+    q, cache, table, n = _case(lens, L, 8, 2, 64, 16, t, code, seed=6)
+    o, lse = ave.paged_attention(q, cache, table, n, window=window, return_lse=True)
+    _check(o, lse, q, cache, table, n, None, window)
+    # a draft's value that is not finite stays out of the rows ahead of it
+    if code in (BF16, F16):
+        base = ave.paged_attention(q, cache, table, n)
+        at = [i for i, ln in enumerate(lens) if ln >= L]
+        for i in at:
+            cache.v[int(table[i, (lens[i] - 1) // 16]), 1, (lens[i] - 1) % 16, 7] = torch.nan
+        o = ave.paged_attention(q, cache, table, n)
+        assert torch.equal(o[at][:, :-1], base[at][:, :-1]) and o[at][:, -1, 4:, 7].isnan().all()
 
 
 @pytest.mark.parametrize("L,Hq,H", [(16, 8, 2), (64, 4, 1), (40, 16, 2)])
