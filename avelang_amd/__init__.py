@@ -50,7 +50,6 @@ from .norm import (  # noqa: F401
     layer_norm_fwd_save,
     rms_norm,
     rms_norm_bwd,
-    rms_norm_fwd_save,
     rms_norm_quant,
 )
 from .paged_attention import (  # noqa: F401
@@ -87,7 +86,6 @@ __all__ = [
     "layer_norm_fwd_save",
     "rms_norm",
     "rms_norm_bwd",
-    "rms_norm_fwd_save",
     "rms_norm_quant",
     "rotary_embedding",
     "rotary_frequencies",

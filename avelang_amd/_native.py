@@ -239,14 +239,14 @@ def lib():
             + [_ll, _i, _i, _i, _i, _vp, _sz, _vp])
         h.gdn_rms_norm_fwd.restype = _i
         h.gdn_rms_norm_fwd.argtypes = (
-            [_vp] * 7                         # x residual weight y h rstd scale
+            [_vp] * 6                         # x residual weight y h scale
             + [_ll, _i, _f, _f, _i, _i, _i, _i, _vp])   # rows D eps offset types stream
         h.gdn_rms_norm_bwd_workspace_bytes.restype = _sz
         h.gdn_rms_norm_bwd_workspace_bytes.argtypes = [_ll, _i, _i]
         h.gdn_rms_norm_bwd.restype = _i
         h.gdn_rms_norm_bwd.argtypes = (
-            [_vp] * 8                         # h weight dy dh rstd dx dr dweight
-            + [_ll, _i, _f, _i, _i, _i, _vp, _sz, _vp])
+            [_vp] * 7                         # h weight dy dh dx dr dweight
+            + [_ll, _i, _f, _f, _i, _i, _i, _vp, _sz, _vp])
         h.gdn_rotary.restype = _i
         h.gdn_rotary.argtypes = (
             [_vp] * 5 + [_i] * 5              # q k and their outputs, strides, B T Hq Hk D

@@ -36,7 +36,6 @@ struct RmsArgs {
   const void* w;
   void* y;
   void* h;
-  float* rstd;
   float* scale;
   long long rows;
   int D;
@@ -116,7 +115,6 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(RmsArgs a) {
     for (int j = 0; j < VEC; ++j) s += f[i][j] * f[i][j];   // (past the row's end 0)
   s = row_sum<LPR>(s, red);
   const float rstd = 1.f / sqrtf(s / a.D + a.eps);
-  if (a.rstd && l == 0) a.rstd[r] = rstd;
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
@@ -161,7 +159,6 @@ __global__ __launch_bounds__(256) void rms_fwd_long_kernel(RmsArgs a) {
   }
   s = row_sum<256>(s, red);
   const float rstd = 1.f / sqrtf(s / a.D + a.eps);
-  if (a.rstd && threadIdx.x == 0) a.rstd[r] = rstd;
   // (a lane reads again what itself has written)
   auto load = [&](int c) {
     if (a.res) ld_row<RT, VEC>(a.h, base, c, a.D, f);
@@ -195,13 +192,13 @@ struct RmsBwdArgs {
   const void* w;
   const void* dy;
   const void* dh;
-  const float* rstd;
   void* dx;
   void* dr;
-  float* pw;   // [parts][D] partial sums of dweight (NULL: not wanted)
+  float* pw;     // [parts][D] partial sums of dweight (NULL: not wanted)
+  float* rstd;   // rows longer than registers hold: [rows] (NULL: not wanted)
   long long rows;
   int D;
-  float offset;
+  float eps, offset;
   int wt, groups;   // groups walking the rows
 };
 
@@ -212,14 +209,40 @@ __device__ __forceinline__ void st_grads(const RmsBwdArgs& a, long long base, in
   if (a.dr) st_row<RT, VEC>(a.dr, base, c, a.D, f);
 }
 
+// Two sums over the lanes of a row at once (as row_sum).
+template <int LPR>
+__device__ __forceinline__ void row_sum2(float& x, float& y, float (*red)[4]) {
+#pragma unroll
+  for (int off = 1; off < (LPR < 64 ? LPR : 64); off *= 2) {
+    x += __shfl_xor(x, off);
+    y += __shfl_xor(y, off);
+  }
+  if constexpr (LPR > 64) {
+    if (threadIdx.x % 64 == 0) {
+      red[0][threadIdx.x / 64] = x;
+      red[1][threadIdx.x / 64] = y;
+    }
+    __syncthreads();
+    x = red[0][0];
+    y = red[1][0];
+#pragma unroll
+    for (int w = 1; w < LPR / 64; ++w) {
+      x += red[0][w];
+      y += red[1][w];
+    }
+  }
+}
+
 // A group of LPR lanes walks the rows gid, gid + groups, ..., its columns'
 // weights and partial sums of dweight in registers, with the next row loaded
 // while the current one is reduced; the groups of a workgroup are summed in LDS.
+// (rstd is formed again with the other sum of the row, not read: nothing is kept
+// of a forward but h.)
 template <int DT, int RT, int LPR, int VPT>
 __global__ __launch_bounds__(256) void rms_bwd_kernel(RmsBwdArgs a) {
   constexpr int VEC = Elt<DT>::VEC, RV = VEC / Elt<RT>::VEC;   // 16-byte loads of RT per one of DT
   constexpr int GPW = 256 / LPR;
-  __shared__ float red[2][4];
+  __shared__ float red[2][2][4];
   extern __shared__ float part[];   // [GPW][D] where groups are summed
   const int l = threadIdx.x % LPR, gi = threadIdx.x / LPR;
   const int gid = blockIdx.x * GPW + gi;
@@ -236,7 +259,6 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(RmsBwdArgs a) {
   }
   // the next row's bits, on their way while this one is reduced
   u32x4e rx[VPT][RV], rh[VPT][RV], ry[VPT];
-  float nr = 0.f;
   auto load = [&](long long r) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -248,7 +270,6 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(RmsBwdArgs a) {
         rh[i][u] = a.dh ? ld_raw<RT>(a.dh, r * a.D, c + u * Elt<RT>::VEC, a.D) : u32x4e{0, 0, 0, 0};
       }
     }
-    nr = a.rstd[r];
   };
   const float inv_d = 1.f / a.D;
   int ph = 0;
@@ -264,23 +285,26 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(RmsBwdArgs a) {
         unpack<RT>(rh[i][u], dh[i] + u * Elt<RT>::VEC);
       }
     }
-    const float rstd = nr;
     if (r + a.groups < a.rows) load(r + a.groups);
-    float s = 0.f;
+    float ss = 0.f, s = 0.f;
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        x[i][j] *= rstd;
-        dw[i][j] += dy[i][j] * x[i][j];
-        dy[i][j] *= w[i][j];
-        s += dy[i][j] * x[i][j];
+        ss += x[i][j] * x[i][j];
+        s += dy[i][j] * w[i][j] * x[i][j];
       }
-    s = row_sum<LPR>(s, red[ph]) * inv_d;
+    row_sum2<LPR>(ss, s, red[ph]);
+    const float rstd = 1.f / sqrtf(ss / a.D + a.eps);
+    s *= rstd * inv_d;   // mean(e hh)
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) x[i][j] = rstd * (dy[i][j] - x[i][j] * s) + dh[i][j];
+      for (int j = 0; j < VEC; ++j) {
+        x[i][j] *= rstd;
+        dw[i][j] += dy[i][j] * x[i][j];
+        x[i][j] = rstd * (dy[i][j] * w[i][j] - x[i][j] * s) + dh[i][j];
+      }
       const int c = (l + LPR * i) * VEC;
       if (c < a.D) st_grads<DT, RT, VEC>(a, r * a.D, c, x[i]);
     }
@@ -309,36 +333,39 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(RmsBwdArgs a) {
   }
 }
 
-// Rows longer than registers hold: dx alone; the sums by rms_cols_kernel.
+// Rows longer than registers hold: dx and rstd; the sums by rms_cols_kernel.
 template <int DT, int RT>
 __global__ __launch_bounds__(256) void rms_bwd_long_kernel(RmsBwdArgs a) {
   constexpr int VEC = Elt<DT>::VEC;
-  __shared__ float red[4];
+  __shared__ float red[2][4];
   const long long r = blockIdx.x, base = r * a.D;
-  const float rstd = a.rstd[r];
-  float x[VEC], dy[VEC], w[VEC], s = 0.f;
+  float x[VEC], dy[VEC], w[VEC], ss = 0.f, s = 0.f;
   auto load = [&](int c) {
     ld_row<RT, VEC>(a.h, base, c, a.D, x);
     ld_row<DT, VEC>(a.dy, base, c, a.D, dy);
     if (a.w) ld_par<VEC>(a.w, 0, c, a.D, a.wt, w);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-      x[j] *= rstd;
+    for (int j = 0; j < VEC; ++j)
       if (a.w) dy[j] *= w[j] + a.offset;
-    }
   };
   for (int c = threadIdx.x * VEC; c < a.D; c += 256 * VEC) {
     load(c);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) s += dy[j] * x[j];
+    for (int j = 0; j < VEC; ++j) {
+      ss += x[j] * x[j];
+      s += dy[j] * x[j];
+    }
   }
-  s = row_sum<256>(s, red) / a.D;
+  row_sum2<256>(ss, s, red);
+  const float rstd = 1.f / sqrtf(ss / a.D + a.eps);
+  s *= rstd / a.D;
+  if (a.rstd && threadIdx.x == 0) a.rstd[r] = rstd;
   for (int c = threadIdx.x * VEC; c < a.D; c += 256 * VEC) {
     load(c);
     float dh[VEC];
     if (a.dh) ld_row<RT, VEC>(a.dh, base, c, a.D, dh);
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) x[j] = rstd * (dy[j] - x[j] * s) + (a.dh ? dh[j] : 0.f);
+    for (int j = 0; j < VEC; ++j) x[j] = rstd * (dy[j] - x[j] * rstd * s) + (a.dh ? dh[j] : 0.f);
     st_grads<DT, RT, VEC>(a, base, c, x);
   }
 }
@@ -431,8 +458,7 @@ int check_rms(const char* name, long long rows, int D, int dtype, int r_dtype, i
   LONG(GDN_DTYPE_F32, GDN_DTYPE_F32)
 
 extern "C" int gdn_rms_norm_fwd(const void* x, const void* residual, const void* weight, void* y,
-                                void* h, float* rstd, float* scale, long long rows, int D,
-                                float eps, float offset, int dtype, int r_dtype, int w_dtype,
+                                void* h, float* scale, long long rows, int D, float eps, float offset, int dtype, int r_dtype, int w_dtype,
                                 int out_dtype, void* stream) {
   const char* name = "gdn_rms_norm_fwd";
   if (const int rc = check_rms(name, rows, D, dtype, r_dtype, w_dtype)) return rc;
@@ -459,7 +485,7 @@ extern "C" int gdn_rms_norm_fwd(const void* x, const void* residual, const void*
                                                              "but as a whole of the same element size");
   gdn_host::launch_begin();
   auto st = static_cast<hipStream_t>(stream);
-  const gdn::RmsArgs a{x, residual, weight, y, h, rstd, bits8 ? scale : nullptr, rows, D, eps, offset, w_dtype, out_dtype};
+  const gdn::RmsArgs a{x, residual, weight, y, h, bits8 ? scale : nullptr, rows, D, eps, offset, w_dtype, out_dtype};
 #define GDN_RF(TT, RR, LL, VV)                                                                   \
   if (dtype == TT && r_dtype == RR && f.lpr == LL && f.vpt == VV) {                              \
     hipLaunchKernelGGL((gdn::rms_fwd_kernel<TT, RR, LL, VV>), dim3((unsigned)((rows + per - 1) / per)), \
@@ -480,18 +506,18 @@ extern "C" int gdn_rms_norm_fwd(const void* x, const void* residual, const void*
 extern "C" size_t gdn_rms_norm_bwd_workspace_bytes(long long rows, int D, int dtype) {
   if (check_rms("gdn_rms_norm_bwd_workspace_bytes", rows, D, dtype, dtype, GDN_DTYPE_F32) || rows == 0)
     return 0;
-  return (size_t)rms_plan(rows, D, dtype).parts * D * sizeof(float);
+  const RmsPlan p = rms_plan(rows, D, dtype);
+  return ((size_t)p.parts * D + (p.f.lpr ? 0 : rows)) * sizeof(float);
 }
 
 extern "C" int gdn_rms_norm_bwd(const void* h, const void* weight, const void* dy, const void* dh,
-                                const float* rstd, void* dx, void* dr, void* dweight,
-                                long long rows, int D, float offset, int dtype, int h_dtype,
-                                int w_dtype, void* workspace, size_t workspace_bytes,
-                                void* stream) {
+                                void* dx, void* dr, void* dweight, long long rows, int D, float eps,
+                                float offset, int dtype, int h_dtype, int w_dtype, void* workspace,
+                                size_t workspace_bytes, void* stream) {
   const char* name = "gdn_rms_norm_bwd";
   if (const int rc = check_rms(name, rows, D, dtype, h_dtype, w_dtype)) return rc;
-  if (rows > 0 && (!h || !dy || !rstd || !dx))
-    return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": h, dy, rstd and dx must be non-NULL");
+  if (rows > 0 && (!h || !dy || !dx))
+    return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": h, dy and dx must be non-NULL");
   if (dweight)
     if (const int fit = gdn_host::check_lanes(name, ((long long)D + 63) / 64, 1024)) return fit;
   RmsPlan p{};
@@ -510,7 +536,7 @@ extern "C" int gdn_rms_norm_bwd(const void* h, const void* weight, const void* d
     if (!p.f.lpr)
       if (const int fit = gdn_host::check_lanes(name, rows, 256)) return fit;
     if (dweight) {
-      const size_t need = (size_t)p.parts * D * sizeof(float);
+      const size_t need = ((size_t)p.parts * D + (p.f.lpr ? 0 : rows)) * sizeof(float);
       if (!workspace || workspace_bytes < need)
         return gdn_host::fail(GDN_ERR_WORKSPACE, std::string(name) + ": workspace needs " +
                                                      std::to_string(need) + " bytes, got " +
@@ -522,7 +548,8 @@ extern "C" int gdn_rms_norm_bwd(const void* h, const void* weight, const void* d
   gdn_host::launch_begin();
   auto st = static_cast<hipStream_t>(stream);
   if (rows > 0) {
-    const gdn::RmsBwdArgs a{h, weight, dy, dh, rstd, dx, dr, pw, rows, D, offset, w_dtype, (int)p.groups};
+    const gdn::RmsBwdArgs a{h, weight, dy, dh, dx, dr, pw, pw && !p.f.lpr ? pw + p.parts * D : nullptr, rows, D, eps, offset,
+                            w_dtype, (int)p.groups};
     const int gpw = p.f.lpr ? 256 / p.f.lpr : 1;
     const size_t lds = gpw > 1 && pw ? (size_t)gpw * D * sizeof(float) : 0;
 #define GDN_RB(TT, RR, LL, VV)                                                                   \

@@ -27,7 +27,7 @@ from .layer_ops import _DTYPES, _dt, _ptr, _stream
 _CODES = {torch.float8_e4m3fn: _native.GDN_DTYPE_E4M3, torch.int8: _native.GDN_DTYPE_I8}
 
 __all__ = ["layer_norm", "layer_norm_fwd_save", "layer_norm_bwd",
-           "rms_norm", "rms_norm_quant", "rms_norm_fwd_save", "rms_norm_bwd"]
+           "rms_norm", "rms_norm_quant", "rms_norm_bwd"]
 
 
 def _args(x, weight, bias, name):
@@ -188,8 +188,8 @@ def _rms_args(x, weight, residual, name):
     """Checked, contiguous x, weight and residual, with rows, D and type codes."""
     if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{name}: x must be a tensor with a last axis of at least 1.")
-    dt = rdt = _dt(x, name, "x")
-    wdt, dev, D = dt, x.device, x.shape[-1]
+    dt = rdt = wdt = _dt(x, name, "x")
+    dev, D = x.device, x.shape[-1]
     if dev.type != "cuda":
         raise ValueError(f"{name}: tensors must be on a ROCm (cuda) device, got {dev}.")
     if weight is not None:
@@ -208,8 +208,6 @@ def _rms_args(x, weight, residual, name):
 
 
 def _rms_out(t, like, name, what):
-    if t is None:
-        return torch.empty_like(like)
     if (not isinstance(t, torch.Tensor) or t.shape != like.shape or t.dtype != like.dtype
             or t.device != like.device or not t.is_contiguous()):
         raise ValueError(f"{name}: {what} must be a contiguous {like.dtype} tensor of shape "
@@ -217,36 +215,31 @@ def _rms_out(t, like, name, what):
     return t
 
 
-def _rms_fwd(args, eps, offset, name, out=None, residual_out=None, save=False, code=None):
+def _rms_fwd(args, eps, offset, name, out=None, residual_out=None, code=None):
     x, weight, residual, rows, D, dt, rdt, wdt = args
-    if residual is None and residual_out is not None:
+    dev, scale, ydt = x.device, None, dt
+    if code is not None:
+        y, ydt = torch.empty_like(x, dtype=code), _CODES[code]
+        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    else:
+        y = torch.empty_like(x) if out is None else _rms_out(out, x, name, "out")
+    h = None
+    if residual is not None:
+        h = (torch.empty_like(residual) if residual_out is None
+             else _rms_out(residual_out, residual, name, "residual_out"))
+    elif residual_out is not None:
         raise ValueError(f"{name}: residual_out needs a residual.")
-    y = _rms_out(out, x, name, "out") if code is None else torch.empty_like(x, dtype=code)
-    h = None if residual is None else _rms_out(residual_out, residual, name, "residual_out")
-    dev = x.device
-    rstd = torch.empty(rows, dtype=torch.float32, device=dev) if save else None
-    scale = None if code is None else torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
     _native.check(_native.on_device(
         dev, _native.lib().gdn_rms_norm_fwd, x.data_ptr(), _ptr(residual), _ptr(weight), y.data_ptr(),
-        _ptr(h), _ptr(rstd), _ptr(scale), rows, D, float(eps), float(offset), dt, rdt, wdt,
-        dt if code is None else _CODES[code], _stream(dev)), name)
-    return y, h, rstd, scale
-
-
-def rms_norm_fwd_save(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6, *,
-                      residual: Optional[torch.Tensor] = None, offset: float = 0.0):
-    """Training forward: ``(y, h, rstd)``, h (x itself, contiguous, without a
-    residual) and rstd (fp32, one per row) being what ``rms_norm_bwd`` takes."""
-    name = "rms_norm_fwd_save"
-    args = _rms_args(x, weight, residual, name)
-    y, h, rstd, _ = _rms_fwd(args, eps, offset, name, save=True)
-    return y, args[0] if h is None else h, rstd
+        _ptr(h), _ptr(scale), rows, D, eps, offset, dt, rdt, wdt, ydt, _stream(dev)), name)
+    return y, h, scale
 
 
 def rms_norm_bwd(h: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Tensor,
-                 rstd: torch.Tensor, dh: Optional[torch.Tensor] = None, *, offset: float = 0.0):
-    """Gradients of ``rms_norm``: ``(dx, dweight, dresidual)`` from dy = dL/dy
-    (its type is x's) and dh = dL/dh (h's type; None where nothing else reads h).
+                 dh: Optional[torch.Tensor] = None, eps: float = 1e-6, *, offset: float = 0.0):
+    """Gradients of ``rms_norm``: ``(dx, dweight, dresidual)`` from h (x itself without a
+    residual), dy = dL/dy (its type is x's) and dh = dL/dh (h's type; None where nothing
+    else reads h).
 
     dresidual is dx itself where h has x's type; with an fp32 residual the same
     values in fp32.  dweight (None without a weight) has the weight's type and is
@@ -255,9 +248,8 @@ def rms_norm_bwd(h: torch.Tensor, weight: Optional[torch.Tensor], dy: torch.Tens
     name = "rms_norm_bwd"
     if not isinstance(dy, torch.Tensor) or not isinstance(h, torch.Tensor):
         raise ValueError(f"{name}: h and dy must be tensors.")
-    dy, weight, h, *sizes = _rms_args(dy, weight, h, name)
-    dx, dw, dr = _rms_bwd(dy, weight, h, sizes, rstd, dh, offset, weight is not None, True, name)
-    return dx, dw, dr
+    return _rms_bwd(_rms_args(dy, weight, h, name), dh, float(eps), float(offset),
+                    weight is not None, True, name)
 
 
 @functools.lru_cache(maxsize=256)
@@ -266,60 +258,52 @@ def _rms_bytes(device, rows, D, dt):
                              rows, D, dt)
 
 
-def _rms_bwd(dy, weight, h, sizes, rstd, dh, offset, want_w, want_r, name):
-    """On ``_rms_args``' (dy, weight, h, sizes)."""
-    rows, D, dt, hdt, wdt = sizes
+def _rms_bwd(args, dh, eps, offset, want_w, want_r, name):
+    """On ``_rms_args`` of dy, weight and h."""
+    dy, weight, h, rows, D, dt, hdt, wdt = args
     dev = dy.device
-    if (not isinstance(rstd, torch.Tensor) or rstd.shape != (rows,) or rstd.device != dev
-            or rstd.dtype is not torch.float32):
-        raise ValueError(f"{name}: rstd must be torch.float32 of shape {(rows,)} on {dev}.")
     if dh is not None:
-        if (not isinstance(dh, torch.Tensor) or dh.shape != h.shape or dh.dtype != h.dtype
+        if (not isinstance(dh, torch.Tensor) or dh.shape != h.shape or dh.dtype is not h.dtype
                 or dh.device != dev):
             raise ValueError(f"{name}: dh must be a {h.dtype} tensor of shape {tuple(h.shape)} on {dev}.")
         dh = dh.contiguous()
-    rstd = rstd.contiguous()
-    dx = torch.empty_like(dy)
-    dr = torch.empty_like(h) if want_r and hdt != dt else None
-    dw = torch.empty_like(weight) if want_w else None
-    lib = _native.lib()
-    ws, nbytes = None, 0
+    dx, dw, dr, ws, nbytes = torch.empty_like(dy), None, None, None, 0
+    if want_r and hdt != dt:
+        dr = torch.empty_like(h)
     if want_w:
+        dw = torch.empty_like(weight)
         nbytes = _rms_bytes(dev.index, rows, D, dt)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _native.check(_native.on_device(
-        dev, lib.gdn_rms_norm_bwd, h.data_ptr(), _ptr(weight), dy.data_ptr(), _ptr(dh),
-        rstd.data_ptr(), dx.data_ptr(), _ptr(dr), _ptr(dw), rows, D, float(offset), dt, hdt, wdt,
-        _ptr(ws), nbytes, _stream(dev)), name)
-    return dx, dw, dr if dr is not None else dx if want_r else None
+        dev, _native.lib().gdn_rms_norm_bwd, h.data_ptr(), _ptr(weight), dy.data_ptr(), _ptr(dh),
+        dx.data_ptr(), _ptr(dr), _ptr(dw), rows, D, eps, offset, dt, hdt, wdt, _ptr(ws), nbytes,
+        _stream(dev)), name)
+    return dx, dw, (dr if dr is not None else dx) if want_r else None
 
 
 class _RmsNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps, offset):
         args = _rms_args(x, weight, residual, "rms_norm")
-        y, h, rstd, _ = _rms_fwd(args, eps, offset, "rms_norm", save=True)
-        ctx.save_for_backward(args[0] if h is None else h, args[1], rstd)
-        ctx.offset, ctx.x_type = offset, x.dtype
+        y, h, _ = _rms_fwd(args, eps, offset, "rms_norm")
+        ctx.save_for_backward(args[0] if h is None else h, args[1])
+        ctx.rest = eps, offset, x.dtype
         ctx.set_materialize_grads(False)
         return y if h is None else (y, h)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh=None):
-        h, weight, rstd = ctx.saved_tensors
-        name = "rms_norm"
-        want_x, want_w, want_r = ctx.needs_input_grad[:3]
+        h, weight = ctx.saved_tensors
+        eps, offset, x_type = ctx.rest
+        want_x, want_w, want_r, _, _ = ctx.needs_input_grad
         if dy is None:
             # (y unused: h's gradient alone)
-            dr = dh if want_r else None
-            dx = None if not want_x or dh is None else dh.to(ctx.x_type)
-            dw = torch.zeros_like(weight) if want_w and weight is not None else None
-            return dx, dw, dr, None, None
+            return (dh.to(x_type) if want_x and dh is not None else None,
+                    torch.zeros_like(weight) if want_w else None, dh if want_r else None, None, None)
         # (checked again: a hook on saved tensors may return others of another layout)
-        dy, weight, h, *sizes = _rms_args(dy, weight, h, name)
-        dx, dw, dr = _rms_bwd(dy, weight, h, sizes, rstd, dh, ctx.offset,
-                              want_w and weight is not None, want_r, name)
+        name = "rms_norm"
+        dx, dw, dr = _rms_bwd(_rms_args(dy, weight, h, name), dh, eps, offset, want_w, want_r, name)
         return dx, dw, dr, None, None
 
 
@@ -338,15 +322,15 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float 
     avoid allocation; both contiguous.
 
     Differentiable in x, weight and residual (``rms_norm_bwd``, the gradient of h
-    included); the forward then keeps h and 4 bytes per row.
+    included); the forward then keeps h alone.
     """
     if torch.is_grad_enabled() and (_grad(x) or _grad(weight) or _grad(residual)):
         if out is not None or residual_out is not None:
             raise ValueError("rms_norm: out / residual_out are not supported when gradients are "
                              "required.")
-        return _RmsNorm.apply(x, weight, residual, eps, offset)
-    y, h, _, _ = _rms_fwd(_rms_args(x, weight, residual, "rms_norm"), eps, offset, "rms_norm", out,
-                          residual_out)
+        return _RmsNorm.apply(x, weight, residual, float(eps), float(offset))
+    y, h, _ = _rms_fwd(_rms_args(x, weight, residual, "rms_norm"), eps, offset, "rms_norm", out,
+                       residual_out)
     return y if h is None else (y, h)
 
 
@@ -366,6 +350,6 @@ def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: 
     name = "rms_norm_quant"
     if dtype not in _CODES:
         raise ValueError(f"{name}: dtype must be torch.float8_e4m3fn or torch.int8, got {dtype}.")
-    y, h, _, scale = _rms_fwd(_rms_args(x, weight, residual, name), eps, offset, name, None,
-                              residual_out, code=dtype)
+    y, h, scale = _rms_fwd(_rms_args(x, weight, residual, name), eps, offset, name, None,
+                           residual_out, code=dtype)
     return (y, scale) if h is None else (y, scale, h)

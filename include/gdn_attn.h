@@ -31,16 +31,16 @@ extern "C" {
  *     y = h rstd (weight + offset),   rstd = 1 / sqrt(mean(h^2) + eps)
  * in fp32.  dtype: x's type; r_dtype: the residual's and h's, x's or fp32;
  * weight [D] (w_dtype; nullable: y = h rstd).  h is written with a residual
- * (it may be x of the same type, or residual); rstd (nullable, fp32 [rows]) is what
- * gdn_rms_norm_bwd reads.  out_dtype is dtype, or an 8-bit type:
+ * (it may be x of the same type, or residual).  out_dtype is dtype, or an 8-bit type:
  *     scale[row] = max |y| / M,  y's codes are y / scale rounded (M = 448, 127)
  * A row of zeros has scale 0 and codes 0; one under 2^-100 has the scale of
  * 2^-100; one that is not finite (or whose squares overflow fp32) has a scale
- * of NaN.  y may be x where the types are the same.
+ * of NaN.  y may be x where the types are the same.  (h of 2^64 or more: its square
+ * overflows fp32, and y is 0 or NaN.)
  */
 int gdn_rms_norm_fwd(const void* x, const void* residual, const void* weight, void* y, void* h,
-                     float* rstd, float* scale, long long rows, int D, float eps, float offset,
-                     int dtype, int r_dtype, int w_dtype, int out_dtype, void* stream);
+                     float* scale, long long rows, int D, float eps, float offset, int dtype,
+                     int r_dtype, int w_dtype, int out_dtype, void* stream);
 
 /*
  * Its gradients, from h (h_dtype: dtype, or fp32 where the residual was), dy
@@ -50,10 +50,10 @@ int gdn_rms_norm_fwd(const void* x, const void* residual, const void* weight, vo
  * summed over the rows in a fixed order.
  */
 size_t gdn_rms_norm_bwd_workspace_bytes(long long rows, int D, int dtype);
-int gdn_rms_norm_bwd(const void* h, const void* weight, const void* dy, const void* dh,
-                     const float* rstd, void* dx, void* dr, void* dweight, long long rows, int D,
-                     float offset, int dtype, int h_dtype, int w_dtype, void* workspace,
-                     size_t workspace_bytes, void* stream);
+int gdn_rms_norm_bwd(const void* h, const void* weight, const void* dy, const void* dh, void* dx,
+                     void* dr, void* dweight, long long rows, int D, float eps, float offset,
+                     int dtype, int h_dtype, int w_dtype, void* workspace, size_t workspace_bytes,
+                     void* stream);
 
 /*
  * Rotary positions of the first R (even) of D elements of every head: pair j at

@@ -26,9 +26,9 @@ def test_exports_are_the_headers():
 
 
 # ------------------------------------------------------------------ norms ----
-def rms(x=P[0], res=P[1], w=P[2], y=P[3], h=P[4], rstd=P[5], scale=None, rows=4, D=64, dt=BF, rt=BF, wt=F32,
+def rms(x=P[0], res=P[1], w=P[2], y=P[3], h=P[4], scale=None, rows=4, D=64, dt=BF, rt=BF, wt=F32,
         out=BF):
-    return _native.lib().gdn_rms_norm_fwd(x, res, w, y, h, rstd, scale, rows, D, 1e-6, 0.0, dt, rt, wt, out, None)
+    return _native.lib().gdn_rms_norm_fwd(x, res, w, y, h, scale, rows, D, 1e-6, 0.0, dt, rt, wt, out, None)
 
 
 @pytest.mark.parametrize("kw,code", [
@@ -45,11 +45,11 @@ def test_rms_refusals(kw, code):
 
 
 def test_rms_backward_refusals():
-    def bwd(h=P[0], dy=P[1], dh=P[2], rstd=P[3], dx=P[4], dr=None, dw=P[6], rows=4, D=64, dt=BF, ht=BF, wt=F32,
+    def bwd(h=P[0], dy=P[1], dh=P[2], dx=P[4], dr=None, dw=P[6], rows=4, D=64, dt=BF, ht=BF, wt=F32,
             ws=P[7], nbytes=1 << 40):
-        return _native.lib().gdn_rms_norm_bwd(h, P[8], dy, dh, rstd, dx, dr, dw, rows, D, 0.0, dt, ht, wt, ws,
-                                              nbytes, None)
-    for kw in (dict(h=None), dict(dy=None), dict(rstd=None), dict(dx=None)):
+        return _native.lib().gdn_rms_norm_bwd(h, P[8], dy, dh, dx, dr, dw, rows, D, 1e-6, 0.0, dt, ht, wt,
+                                              ws, nbytes, None)
+    for kw in (dict(h=None), dict(dy=None), dict(dx=None)):
         assert bwd(**kw) == -1
     for kw in (dict(dx=P[0]), dict(dx=P[1] + 2), dict(dx=P[2]), dict(dr=P[4] + 4), dict(dr=P[0], ht=F32)):
         assert bwd(**kw) == -5

@@ -119,8 +119,8 @@ def test_wrappers_refuse(rocm_device):
             lambda: ave.rms_norm(x, residual=r[:2]), lambda: ave.rms_norm(r, residual=x), lambda: ave.rms_norm(x.half(), residual=x),
             lambda: ave.rms_norm(x, r[0].cpu()), lambda: ave.rms_norm(x, out=r), lambda: ave.rms_norm(x, residual_out=x),
             lambda: ave.rms_norm(x, residual=x, out=x, residual_out=x),
-            lambda: ave.rms_norm_quant(x, dtype=torch.uint8), lambda: ave.rms_norm_bwd(x, None, x, r[0]),
-            lambda: ave.rms_norm_bwd(x, None, x, r[:, 0].contiguous(), dh=r),
+            lambda: ave.rms_norm_quant(x, dtype=torch.uint8), lambda: ave.rms_norm_bwd(r, None, x, x),
+            lambda: ave.rms_norm_bwd(x, None, x, r), lambda: ave.rms_norm_bwd(x, None, r),
             lambda: ave.rotary_embedding(q, None, pos[:2], f), lambda: ave.rotary_embedding(q, None, pos.float(), f),
             lambda: ave.rotary_embedding(q, None, pos, f.long()), lambda: ave.rotary_embedding(q, None, pos, torch.ones(33, **dev)),
             lambda: ave.rotary_embedding(q, q[:2], pos, f), lambda: ave.rotary_embedding(q, q.half(), pos, f),
