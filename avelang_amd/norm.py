@@ -20,6 +20,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _native
 from .layer_ops import _DTYPES, _dt, _ptr, _stream
@@ -190,6 +191,8 @@ def _rms_args(x, weight, residual, name):
         raise ValueError(f"{name}: x must be a tensor with a last axis of at least 1.")
     dt = rdt = wdt = _dt(x, name, "x")
     dev, D = x.device, x.shape[-1]
+    if D >= 2 ** 31:
+        raise ValueError(f"{name}: rows must be shorter than 2^31, got {D}.")
     if dev.type != "cuda":
         raise ValueError(f"{name}: tensors must be on a ROCm (cuda) device, got {dev}.")
     if weight is not None:
@@ -212,6 +215,8 @@ def _rms_out(t, like, name, what):
             or t.device != like.device or not t.is_contiguous()):
         raise ValueError(f"{name}: {what} must be a contiguous {like.dtype} tensor of shape "
                          f"{tuple(like.shape)} on {like.device}.")
+    if not t.is_inference():
+        increment_version(t)   # (it may be x or the residual, which autograd may have kept)
     return t
 
 

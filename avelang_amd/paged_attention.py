@@ -34,9 +34,9 @@ class PagedKVCache:
     """The tensors of a cache: ``k``, ``v`` [num_pages, kv_heads, page_size,
     head_size] (contiguous, 16-byte aligned; bf16, fp16, float8_e4m3fn or int8) and,
     in 8 bits, ``k_scale``, ``v_scale`` [num_pages, kv_heads, page_size] fp32.
-    ``PagedKVCache.zeros`` allocates them."""
+    ``PagedKVCache.zeros`` allocates them; they are not replaced or resized later."""
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "ptrs", "sizes", "code")
+    __slots__ = ("_held", "sizes", "code")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
                  v_scale: Optional[torch.Tensor] = None):
@@ -54,24 +54,30 @@ class PagedKVCache:
         pk, pv = k.data_ptr(), v.data_ptr()
         if not k.is_contiguous() or not v.is_contiguous() or (pk | pv) % 16:
             raise ValueError(f"{name}: k and v must be contiguous and 16-byte aligned.")
-        sk = sv = None
         if dtype in _CODES:
-            sk = self._scale(k_scale, shape[:3], dev, "k_scale")
-            sv = self._scale(v_scale, shape[:3], dev, "v_scale")
+            self._check_scale(k_scale, shape[:3], dev, "k_scale")
+            self._check_scale(v_scale, shape[:3], dev, "v_scale")
         elif k_scale is not None or v_scale is not None:
             raise ValueError(f"{name}: a cache in {dtype} has no scales.")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.ptrs = pk, pv, sk, sv
+        self._held = k, v, k_scale, v_scale
         self.sizes = heads, size, pages, page
         self.code = _TYPES[dtype]
 
+    k = property(lambda self: self._held[0])
+    v = property(lambda self: self._held[1])
+    k_scale = property(lambda self: self._held[2])
+    v_scale = property(lambda self: self._held[3])
+
+    @property
+    def ptrs(self):
+        return [None if t is None else t.data_ptr() for t in self._held]
+
     @staticmethod
-    def _scale(t, shape, dev, what):
+    def _check_scale(t, shape, dev, what):
         if (not isinstance(t, torch.Tensor) or t.shape != shape or t.device != dev
                 or t.dtype is not torch.float32 or not t.is_contiguous() or t.data_ptr() % 16):
             raise ValueError(f"PagedKVCache: {what} must be a contiguous, 16-byte aligned "
                              f"torch.float32 tensor of shape {tuple(shape)} on {dev}.")
-        return t.data_ptr()
 
     @classmethod
     def zeros(cls, num_pages: int, page_size: int, kv_heads: int, head_size: int,
@@ -98,6 +104,8 @@ def _slots(slots, cache, name, distinct):
     if (not isinstance(slots, torch.Tensor) or slots.dtype not in (torch.int32, torch.int64)
             or slots.device not in (dev, torch.device("cpu"))):
         raise ValueError(f"{name}: slots must be int32 or int64 on {dev} or the CPU.")
+    if slots.numel() >= 2 ** 31:
+        raise ValueError(f"{name}: more than 2^31 - 1 slots in a call.")
     if slots.device.type == "cpu" and slots.numel():
         if distinct:
             used = slots[(slots >= 0) & (slots < cache.sizes[2] * cache.sizes[3])]
@@ -155,8 +163,7 @@ def paged_cache_read(cache: PagedKVCache, slots: torch.Tensor,
     slots = _slots(slots, cache, name, False)
     if dtype is None:
         dtype = torch.bfloat16 if cache.k.dtype in _CODES else cache.k.dtype
-    if dtype not in _HALF or (cache.k.dtype not in _CODES
-                                                        and dtype != cache.k.dtype):
+    if dtype not in _HALF or (cache.k.dtype not in _CODES and dtype != cache.k.dtype):
         raise ValueError(f"{name}: dtype must be bf16 or fp16, and the cache's unless it has 8 bits, "
                          f"got {dtype}.")
     k = torch.empty(slots.shape + (H, D), dtype=dtype, device=dev)
@@ -221,6 +228,8 @@ def paged_attention(
     if L < 1 or Hq < 1 or Hq % H:
         raise ValueError(f"{name}: q must have at least one token, and heads ({Hq}) a multiple of the "
                          f"cache's ({H}).")
+    if max(N, L, Hq) >= 2 ** 31:
+        raise ValueError(f"{name}: q's axes must be under 2^31, got {tuple(q.shape)}.")
     if cache.k.dtype != q.dtype and cache.k.dtype not in _CODES:
         raise ValueError(f"{name}: a cache in {cache.k.dtype} takes queries of its type, got {q.dtype}.")
     if pages < 1 or page % 16:
@@ -242,6 +251,8 @@ def paged_attention(
         max_length = held
     elif not 0 <= max_length <= held:
         raise ValueError(f"{name}: max_length must be within the block table's {held} tokens.")
+    if max_length > 1 << 30:
+        raise ValueError(f"{name}: lengths of more than 2^30 tokens are not supported.")
     # (strides of an axis of one mean nothing)
     sn, sl, sh, se = q.stride()
     sn, sl, sh = sn if N > 1 else 0, sl if L > 1 else 0, sh if Hq > 1 else 0
@@ -264,8 +275,8 @@ def paged_attention(
         raise ValueError(f"{name}: workspace must be contiguous on {dev}.")
     _native.check(_native.on_device(
         dev, lib.gdn_paged_attn_fwd, q.data_ptr(), sn, sl, sh, *cache.ptrs, block_table.data_ptr(),
-        max(block_table.stride(0), block_table.shape[1]), lengths.contiguous().data_ptr(), out.data_ptr(), _ptr(lse), N, L, Hq, H,
-        D, pages, page, max_length, int(window), D ** -0.5 if scale is None else float(scale),
+        max(block_table.stride(0), block_table.shape[1]), lengths.contiguous().data_ptr(), out.data_ptr(),
+        _ptr(lse), N, L, Hq, H, D, pages, page, max_length, min(int(window), 1 << 30), D ** -0.5 if scale is None else float(scale),
         _DTYPES[q.dtype], cache.code, workspace.data_ptr(),
         workspace.numel() * workspace.element_size(), _stream(dev)), name)
     return (out, lse) if return_lse else out

@@ -20,6 +20,7 @@ from typing import Optional, Tuple
 
 import torch
 from torch.autograd.function import once_differentiable
+from torch.autograd.graph import increment_version
 
 from . import _native
 from .layer_ops import _dt, _ptr, _stream
@@ -83,6 +84,8 @@ def _args(q, k, positions, inv_freq, name):
     if dev.type != "cuda":
         raise ValueError(f"{name}: tensors must be on a ROCm (cuda) device, got {dev}.")
     B, T, H, D = q.shape
+    if B * T >= 2 ** 31 or max(H, 0 if k is None else k.shape[2]) > 1 << 20:
+        raise ValueError(f"{name}: at most 2^31 - 1 tokens and 2^20 heads, got {tuple(q.shape)}.")
     if H < 1 or D < 2 or D > 512 or D % 2:
         raise ValueError(f"{name}: q must have at least one head, and heads of an even size of at "
                          f"most 512, got {H} of {D}.")
@@ -193,6 +196,8 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     _turn(q4, k4, qo, ko, pos, freq, dt, float(magnitude), bool(interleaved), False, name)
     if inplace:
         qo, ko = q, k
+        # (autograd, where it kept them, sees that they changed)
+        increment_version([t for t in (q, k) if t is not None and not t.is_inference()])
     elif q.dim() == 3:
         qo, ko = qo[0], None if ko is None else ko[0]
     return qo if k is None else (qo, ko)

@@ -142,3 +142,42 @@ def test_wrappers_refuse(rocm_device):
             lambda: ave.paged_attention(q4, c, t, n, workspace=torch.empty(1 << 20, dtype=torch.uint8))):
         with pytest.raises(ValueError):
             call()
+
+
+def test_wrappers_refuse_sizes(rocm_device):
+    """Sizes past 32 bits, by expanded tensors without memory, are refused and not cut."""
+    big, dev = 2 ** 32 + 3, dict(device=rocm_device)
+    x, f = torch.zeros(1, **dev), torch.ones(1, **dev)
+    pos, n = torch.zeros(1, dtype=torch.int64, **dev), torch.ones(1, dtype=torch.int32, **dev)
+    c = ave.PagedKVCache.zeros(1, 16, 1, 64, torch.bfloat16)
+    row = torch.zeros(1, 1, 64, **dev).bfloat16()
+    for call in (
+            lambda: ave.rms_norm(x.expand(big)), lambda: ave.rms_norm_quant(x.expand(1, big)),
+            lambda: ave.rotary_embedding(x.expand(big, 1, 2), None, pos.expand(big), f),
+            lambda: ave.rotary_embedding(x.expand(1, big, 2), None, pos, f),
+            lambda: ave.paged_cache_write(c, row.expand(big, 1, 64), row.expand(big, 1, 64), pos.expand(big)),
+            lambda: ave.paged_cache_read(c, pos.expand(big)),
+            lambda: ave.paged_attention(row[None].expand(1, big, 1, 64), c, n[None], n),
+            lambda: ave.paged_attention(row[None].expand(big, 1, 1, 64), c, n[None].expand(big, 1), n.expand(big)),
+            lambda: ave.paged_attention(row[None], c, n[None].expand(1, big), n)):
+        with pytest.raises(ValueError):
+            call()
+    n.fill_(16)
+    q, t = torch.randn(1, 2, 1, 64, **dev).bfloat16(), torch.zeros(1, 1, dtype=torch.int32, **dev)
+    c.v.normal_()
+    assert torch.equal(ave.paged_attention(q, c, t, n, window=2 ** 32 + 1), ave.paged_attention(q, c, t, n))
+
+
+def test_cache_tensors(rocm_device):
+    """The cache's tensors are found where they are at a call, and cannot be exchanged for others."""
+    c = ave.PagedKVCache.zeros(3, 16, 1, 64, torch.int8)
+    with pytest.raises(AttributeError):
+        c.k = c.v
+    kv = torch.randn(2, 20, 1, 64, device=rocm_device).bfloat16()
+    slots = torch.arange(20, device=rocm_device)
+    ave.paged_cache_write(c, kv[0], kv[1], slots)
+    before = ave.paged_cache_read(c, slots)
+    old = c.k.data
+    c.k.data = old.clone()
+    old.zero_()
+    assert all(torch.equal(a, b) for a, b in zip(ave.paged_cache_read(c, slots), before))

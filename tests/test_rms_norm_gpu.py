@@ -229,3 +229,21 @@ def test_same_bits_every_time(rocm_device):
     x.requires_grad_()
     w.requires_grad_()
     assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(ave.rms_norm(x, w), [x, w], dy), first))
+
+
+@pytest.mark.parametrize("of", ["x", "residual"])
+def test_in_place_is_seen(rocm_device, of):
+    """Autograd refuses a backward that needs a tensor that was written over since."""
+    w = torch.randn(4, 64, device=rocm_device, requires_grad=True)
+    x, r = torch.randn(4, 64, device=rocm_device), torch.randn(4, 64, device=rocm_device)
+    y = (w * (x if of == "x" else r)).sum()
+    if of == "x":
+        ave.rms_norm(x, out=x)
+    else:
+        ave.rms_norm(x, residual=r, residual_out=r)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    with torch.inference_mode():
+        z = torch.randn(4, 64, device=rocm_device)
+        want = ave.rms_norm(z)
+        assert torch.equal(ave.rms_norm(z, out=z), want)

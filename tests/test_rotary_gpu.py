@@ -108,3 +108,18 @@ def test_empty(rocm_device):
     assert y.shape == q.shape and torch.autograd.grad(y.sum(), [q])[0].shape == q.shape
     with pytest.raises(ValueError, match="inplace"):
         ave.rotary_embedding(q, None, torch.empty(0, device="cuda", dtype=torch.int64), freq, inplace=True)
+
+
+def test_in_place_is_seen(rocm_device):
+    """Autograd refuses a backward that needs a tensor that was turned in place since."""
+    w = torch.randn(4, 1, 64, device=rocm_device, requires_grad=True)
+    x = torch.randn(4, 1, 64, device=rocm_device)
+    y = (w * x).sum()
+    pos, f = torch.arange(4, device=rocm_device), torch.ones(32, dtype=torch.float64, device=rocm_device)
+    ave.rotary_embedding(x, None, pos, f, inplace=True)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    with torch.inference_mode():
+        z = torch.randn(4, 1, 64, device=rocm_device)
+        want = ave.rotary_embedding(z, None, pos, f)
+        assert torch.equal(ave.rotary_embedding(z, None, pos, f, inplace=True), want)
