@@ -194,7 +194,8 @@ struct RmsBwdArgs {
   const void* dh;
   void* dx;
   void* dr;
-  float* pw;     // [parts][D] partial sums of dweight (NULL: not wanted)
+  float* pw;     // [parts][D] partial sums of dweight (NULL: not wanted, or no parts)
+  void* dw;      // [D] dweight of the weight's type where one workgroup takes all rows (else NULL)
   float* rstd;   // rows longer than registers hold: [rows] (NULL: not wanted)
   long long rows;
   int D;
@@ -207,6 +208,13 @@ template <int DT, int RT, int VEC>
 __device__ __forceinline__ void st_grads(const RmsBwdArgs& a, long long base, int c, const float (&f)[VEC]) {
   st_row<DT, VEC>(a.dx, base, c, a.D, f);
   if (a.dr) st_row<RT, VEC>(a.dr, base, c, a.D, f);
+}
+
+// Element c of dweight, of type wt.
+__device__ __forceinline__ void st_weight(void* dw, long long c, float s, int wt) {
+  if (wt == GDN_DTYPE_F32) ste<GDN_DTYPE_F32>(dw, c, s);
+  else if (wt == GDN_DTYPE_BF16) ste<GDN_DTYPE_BF16>(dw, c, s);
+  else ste<GDN_DTYPE_F16>(dw, c, s);
 }
 
 // Two sums over the lanes of a row at once (as row_sum).
@@ -309,7 +317,7 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(RmsBwdArgs a) {
       if (c < a.D) st_grads<DT, RT, VEC>(a, r * a.D, c, x[i]);
     }
   }
-  if (!a.pw) return;
+  if (!a.pw && !a.dw) return;
   if constexpr (GPW > 1) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
@@ -322,13 +330,20 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(RmsBwdArgs a) {
     for (int c = threadIdx.x; c < a.D; c += 256) {
       float s = part[c];
       for (int g = 1; g < GPW; ++g) s += part[g * a.D + c];
-      a.pw[(long long)blockIdx.x * a.D + c] = s;
+      if (a.dw) st_weight(a.dw, c, s, a.wt);
+      else a.pw[(long long)blockIdx.x * a.D + c] = s;
     }
   } else {
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = (l + LPR * i) * VEC;
-      if (c < a.D) st_row<GDN_DTYPE_F32, VEC>(a.pw, (long long)gid * a.D, c, a.D, dw[i]);
+      if (a.dw) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j)
+          if (c + j < a.D) st_weight(a.dw, c + j, dw[i][j], a.wt);
+      } else if (c < a.D) {
+        st_row<GDN_DTYPE_F32, VEC>(a.pw, (long long)gid * a.D, c, a.D, dw[i]);
+      }
     }
   }
 }
@@ -398,9 +413,7 @@ __global__ __launch_bounds__(1024) void rms_sum_kernel(const float* part, void* 
   if (sl == 0 && c < D) {
 #pragma unroll
     for (int i = 1; i < 16; ++i) s += red[i][l];
-    if (wt == GDN_DTYPE_F32) ste<GDN_DTYPE_F32>(dw, c, s);
-    else if (wt == GDN_DTYPE_BF16) ste<GDN_DTYPE_BF16>(dw, c, s);
-    else ste<GDN_DTYPE_F16>(dw, c, s);
+    st_weight(dw, c, s, wt);
   }
 }
 
@@ -408,12 +421,16 @@ __global__ __launch_bounds__(1024) void rms_sum_kernel(const float* part, void* 
 
 namespace {
 
-// Groups that walk the rows of the backward, and the partial sums they leave:
-// two workgroups per CU, no more groups than rows.
+// Groups that walk the rows of the backward, and the partial sums they leave (0:
+// none): two workgroups per CU, no more groups than rows; a few rows take one
+// workgroup, which writes the weight's gradient itself (replayed, 4 rows of 1024
+// bf16: 4.4 us, with a second launch 6.2; 8, two to a group: 5.5 and 6.2; 16, four
+// to a group: 7.6 and 6.3; a call's host time is 8 us less without).
 struct RmsPlan {
   gdn::RowForm f;
   long long groups, parts, span;
 };
+constexpr int kRmsFew = 2;   // rows per group of that one
 RmsPlan rms_plan(long long rows, int D, int dtype) {
   RmsPlan p{gdn::row_form(D, dtype), 0, 0, 0};
   if (!p.f.lpr) {
@@ -424,7 +441,10 @@ RmsPlan rms_plan(long long rows, int D, int dtype) {
   const int gpw = 256 / p.f.lpr;
   p.groups = 2LL * gdn::device_cus() * gpw;
   if (p.groups > rows) p.groups = rows;
-  if (p.groups < 1) p.groups = 1;
+  if (rows <= (long long)kRmsFew * gpw) {
+    if (p.groups > gpw) p.groups = gpw;
+    return p;
+  }
   p.parts = (p.groups + gpw - 1) / gpw;
   return p;
 }
@@ -458,8 +478,9 @@ int check_rms(const char* name, long long rows, int D, int dtype, int r_dtype, i
   LONG(GDN_DTYPE_F32, GDN_DTYPE_F32)
 
 extern "C" int gdn_rms_norm_fwd(const void* x, const void* residual, const void* weight, void* y,
-                                void* h, float* scale, long long rows, int D, float eps, float offset, int dtype, int r_dtype, int w_dtype,
-                                int out_dtype, void* stream) {
+                                void* h, float* scale, long long rows, int D, float eps,
+                                float offset, int dtype, int r_dtype, int w_dtype, int out_dtype,
+                                void* stream) {
   const char* name = "gdn_rms_norm_fwd";
   if (const int rc = check_rms(name, rows, D, dtype, r_dtype, w_dtype)) return rc;
   const bool bits8 = out_dtype == GDN_DTYPE_E4M3 || out_dtype == GDN_DTYPE_I8;
@@ -537,21 +558,22 @@ extern "C" int gdn_rms_norm_bwd(const void* h, const void* weight, const void* d
       if (const int fit = gdn_host::check_lanes(name, rows, 256)) return fit;
     if (dweight) {
       const size_t need = ((size_t)p.parts * D + (p.f.lpr ? 0 : rows)) * sizeof(float);
-      if (!workspace || workspace_bytes < need)
+      if (need && (!workspace || workspace_bytes < need))
         return gdn_host::fail(GDN_ERR_WORKSPACE, std::string(name) + ": workspace needs " +
                                                      std::to_string(need) + " bytes, got " +
                                                      std::to_string(workspace_bytes));
-      pw = static_cast<float*>(workspace);
+      if (need) pw = static_cast<float*>(workspace);
     }
   }
   if (rows == 0 && !dweight) return GDN_OK;
   gdn_host::launch_begin();
   auto st = static_cast<hipStream_t>(stream);
   if (rows > 0) {
-    const gdn::RmsBwdArgs a{h, weight, dy, dh, dx, dr, pw, pw && !p.f.lpr ? pw + p.parts * D : nullptr, rows, D, eps, offset,
-                            w_dtype, (int)p.groups};
+    const gdn::RmsBwdArgs a{h, weight, dy, dh, dx, dr, pw, pw ? nullptr : dweight,
+                            pw && !p.f.lpr ? pw + p.parts * D : nullptr, rows, D, eps, offset, w_dtype,
+                            (int)p.groups};
     const int gpw = p.f.lpr ? 256 / p.f.lpr : 1;
-    const size_t lds = gpw > 1 && pw ? (size_t)gpw * D * sizeof(float) : 0;
+    const size_t lds = gpw > 1 && dweight ? (size_t)gpw * D * sizeof(float) : 0;
 #define GDN_RB(TT, RR, LL, VV)                                                                   \
   if (dtype == TT && h_dtype == RR && p.f.lpr == LL && p.f.vpt == VV)                            \
     hipLaunchKernelGGL((gdn::rms_bwd_kernel<TT, RR, LL, VV>),                                    \
@@ -568,7 +590,7 @@ extern "C" int gdn_rms_norm_bwd(const void* h, const void* weight, const void* d
 #undef GDN_RBL
   }
   // (no rows: the sum over nothing is zero)
-  if (dweight)
+  if (dweight && (pw || rows == 0))
     hipLaunchKernelGGL(gdn::rms_sum_kernel, dim3((unsigned)((D + 63) / 64)), dim3(1024), 0, st, pw,
                        dweight, (int)p.parts, D, w_dtype);
   return gdn_host::check_launch(name);

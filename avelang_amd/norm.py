@@ -278,7 +278,7 @@ def _rms_bwd(args, dh, eps, offset, want_w, want_r, name):
     if want_w:
         dw = torch.empty_like(weight)
         nbytes = _rms_bytes(dev.index, rows, D, dt)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _native.check(_native.on_device(
         dev, _native.lib().gdn_rms_norm_bwd, h.data_ptr(), _ptr(weight), dy.data_ptr(), _ptr(dh),
         dx.data_ptr(), _ptr(dr), _ptr(dw), rows, D, eps, offset, dt, hdt, wdt, _ptr(ws), nbytes,

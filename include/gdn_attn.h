@@ -47,7 +47,8 @@ int gdn_rms_norm_fwd(const void* x, const void* residual, const void* weight, vo
  * (dtype) and, nullable, dh (h_dtype; dL/dh from what else reads h):
  *     dx = rstd (e - hh mean(e hh)) + dh,  e = dy (weight + offset), hh = h rstd
  * in x's type, dr (nullable) the same in h_dtype, dweight (w_dtype; nullable)
- * summed over the rows in a fixed order.
+ * summed over the rows in a fixed order.  workspace: as many bytes where dweight
+ * is wanted (0 for few rows).
  */
 size_t gdn_rms_norm_bwd_workspace_bytes(long long rows, int D, int dtype);
 int gdn_rms_norm_bwd(const void* h, const void* weight, const void* dy, const void* dh, void* dx,

@@ -53,12 +53,12 @@ def test_rms_backward_refusals():
         assert bwd(**kw) == -1
     for kw in (dict(dx=P[0]), dict(dx=P[1] + 2), dict(dx=P[2]), dict(dr=P[4] + 4), dict(dr=P[0], ht=F32)):
         assert bwd(**kw) == -5
-    assert bwd(nbytes=8) == -4 and bwd(ws=None) == -4
+    assert bwd(rows=400, nbytes=8) == -4 and bwd(rows=400, ws=None) == -4
     assert bwd(dt=4) == -2 and bwd(ht=F16) == -2 and bwd(rows=-1) == -2 and bwd(D=1 << 28) == -2
     assert bwd(rows=1 << 24, D=40000, dw=None) == -2
     assert bwd(rows=0, dw=None) == 0 and rms(rows=0, x=None, y=None) == 0
     f = _native.lib().gdn_rms_norm_bwd_workspace_bytes
-    assert f(0, 64, BF) == 0 and 0 < f(1, 64, BF) <= f(4096, 64, BF) and f(5, 64, 9) == 0
+    assert f(0, 64, BF) == f(1, 64, BF) == 0 < f(400, 64, BF) <= f(4096, 64, BF) and f(5, 64, 9) == 0
 
 
 # ----------------------------------------------------------------- rotary ----

@@ -247,3 +247,25 @@ def test_in_place_is_seen(rocm_device, of):
         z = torch.randn(4, 64, device=rocm_device)
         want = ave.rms_norm(z)
         assert torch.equal(ave.rms_norm(z, out=z), want)
+
+
+@pytest.mark.parametrize("t", [BF16, F32])
+@pytest.mark.parametrize("D", [96, 250, 1000, 2500, 8000])
+@pytest.mark.parametrize("rows", [1, 2, 3, 8, 9, 16, 17, 32, 33])
+def test_few_rows_gradients(rocm_device, rows, D, t):
+    """One workgroup's rows and one more: the weight's gradient with and without a second launch."""
+    gen = torch.Generator().manual_seed(rows * D)
+    x, dy = (torch.randn(rows, D, generator=gen).to(t) for _ in "xy")
+    w = torch.randn(D, generator=gen).to(BF16 if rows % 2 else F32)
+    dx, dw, _ = ave.rms_norm_bwd(x.cuda(), w.cuda(), dy.cuda(), eps=1e-5, offset=1.0)
+    leaves = [v.double().requires_grad_() for v in (x, w)]
+    h, weight = leaves
+    y = h * (h.square().mean(-1, keepdim=True) + 1e-5).rsqrt() * (weight + 1)
+    want = torch.autograd.grad(y, leaves, dy.double())
+    # sums in fp32: under (D / 64 + 16) steps of 2^-24 of the terms' sizes; rows up to 2^3 large
+    eps = 2.0 ** -24 * (D / 64 + 32)
+    ax = want[0].abs() * torch.finfo(t).eps / 2 + eps * 8 * (1 + want[0].abs().amax(-1, keepdim=True))
+    xh = (h / (h.square().mean(-1, keepdim=True) + 1e-5).sqrt()).detach()
+    aw = want[1].abs() * torch.finfo(w.dtype).eps / 2 + 4 * eps * (dy.double() * xh).abs().sum(0)
+    assert ((dx.cpu().double() - want[0]).abs() <= ax).all()
+    assert ((dw.cpu().double() - want[1]).abs() <= aw).all()
