@@ -70,100 +70,93 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, factor: float = 1.0, 
     return f.to(device) if device is not None else f, size
 
 
-def _args(q, k, positions, inv_freq, name):
-    """Checked q and k as 4-D tensors with contiguous elements, positions, fp64 frequencies and
-    the type's code."""
-    if not isinstance(q, torch.Tensor) or not 3 <= q.dim() <= 4:
+def _turn(q, k, positions, inv_freq, magnitude, interleaved, inverse, inplace, name):
+    """q and k (or None) turned: new contiguous tensors, or with ``inplace`` themselves."""
+    if not isinstance(q, torch.Tensor) or not 3 <= (dims := q.dim()) <= 4:
         raise ValueError(f"{name}: q must be a tensor [B, T, H, D] or [T, H, D].")
-    dt, dev = _dt(q, name, "q"), q.device
-    if k is not None and (not isinstance(k, torch.Tensor) or k.dim() != q.dim()
-                          or k.dtype is not q.dtype or k.device != dev):
-        raise ValueError(f"{name}: k must be a {q.dtype} tensor like q on {dev}.")
-    if q.dim() == 3:
-        q, k = q[None], None if k is None else k[None]
+    dt, dev, shape = _dt(q, name, "q"), q.device, q.shape
     if dev.type != "cuda":
         raise ValueError(f"{name}: tensors must be on a ROCm (cuda) device, got {dev}.")
-    B, T, H, D = q.shape
-    if B * T >= 2 ** 31 or max(H, 0 if k is None else k.shape[2]) > 1 << 20:
-        raise ValueError(f"{name}: at most 2^31 - 1 tokens and 2^20 heads, got {tuple(q.shape)}.")
+    B, T, H, D = shape if dims == 4 else (1, *shape)
     if H < 1 or D < 2 or D > 512 or D % 2:
         raise ValueError(f"{name}: q must have at least one head, and heads of an even size of at "
                          f"most 512, got {H} of {D}.")
-    if k is not None and (k.shape[0] != B or k.shape[1] != T or k.shape[3] != D or k.shape[2] < 1):
-        raise ValueError(f"{name}: k must have q's axes but heads (at least one), got {tuple(k.shape)} "
-                         f"beside {tuple(q.shape)}.")
+    Hk = 0
+    if k is not None:
+        if (not isinstance(k, torch.Tensor) or k.dim() != dims or k.dtype is not q.dtype
+                or k.device != dev):
+            raise ValueError(f"{name}: k must be a {q.dtype} tensor like q on {dev}.")
+        Hk = k.shape[-2]
+        if k.shape[:-2] != shape[:-2] or k.shape[-1] != D or Hk < 1:
+            raise ValueError(f"{name}: k must have q's axes but heads (at least one), got "
+                             f"{tuple(k.shape)} beside {tuple(shape)}.")
+    if B * T >= 2 ** 31 or max(H, Hk) > 1 << 20:
+        raise ValueError(f"{name}: at most 2^31 - 1 tokens and 2^20 heads, got {tuple(shape)}.")
     if (not isinstance(inv_freq, torch.Tensor) or inv_freq.dim() != 1 or not inv_freq.is_floating_point()
-            or inv_freq.device != dev or not 1 <= inv_freq.shape[0] <= D // 2):
+            or inv_freq.device != dev or not 1 <= (R := inv_freq.shape[0]) <= D // 2):
         raise ValueError(f"{name}: inv_freq must be a 1-D floating point tensor on {dev} of 1 to "
                          f"{D // 2} frequencies.")
     if (not isinstance(positions, torch.Tensor) or positions.dtype not in (torch.int32, torch.int64)
             or positions.device != dev or positions.shape != (B, T) and positions.shape != (T,)):
         raise ValueError(f"{name}: positions must be int32 or int64 of shape ({T},) or ({B}, {T}) on "
                          f"{dev}.")
-    if q.stride(3) != 1:
-        q = q.contiguous()
-    if k is not None and k.stride(3) != 1:
-        k = k.contiguous()
-    return q, k, positions.contiguous(), inv_freq.double().contiguous(), dt
-
-
-def _turn(q, k, qo, ko, positions, freq, dt, magnitude, interleaved, inverse, name):
-    """qo, ko (4-D, q's and k's shapes) from q and k."""
-    B, T, Hq, D = q.shape
-    a, b = q.stride(), qo.stride()
-    if k is None:
-        Hk, strides = 0, _STRIDES(a[0], a[1], a[2], 0, 0, 0, b[0], b[1], b[2])
+    if inplace:
+        for t in (q, k):
+            if t is not None and (t.stride(-1) != 1 or not _apart(t)):
+                raise ValueError(f"{name}: in place q and k must have contiguous heads and elements "
+                                 "of their own.")
+        qo, ko = q, k
     else:
-        c, d = k.stride(), ko.stride()
-        Hk = k.shape[2]
-        strides = _STRIDES(a[0], a[1], a[2], c[0], c[1], c[2], b[0], b[1], b[2], d[0], d[1], d[2])
-    dev = q.device
+        qo, ko = _new(q), None if k is None else _new(k)
+    a, c = q.stride(), (0,) * 4 if k is None else k.stride()
+    if a[-1] != 1:
+        q = q.contiguous()
+        a = q.stride()
+    if k is not None and c[-1] != 1:
+        k = k.contiguous()
+        c = k.stride()
+    a, c = (a[:3], c[:3]) if dims == 4 else ((0, *a[:2]), (0, *c[:2]))
+    b, d = (a, c) if inplace else ((T * H * D, H * D, D), (T * Hk * D, Hk * D, D))
+    positions, inv_freq = positions.contiguous(), inv_freq.double().contiguous()
     _native.check(_native.on_device(
-        dev, _native.lib().gdn_rotary, q.data_ptr(), _ptr(k), qo.data_ptr(), _ptr(ko), strides, B, T,
-        Hq, Hk, D, positions.data_ptr(), positions.dtype is torch.int64,
-        T if positions.dim() == 2 else 0, freq.data_ptr(), 2 * freq.shape[0], magnitude, interleaved,
-        inverse, dt, _stream(dev)), name)
+        dev, _native.lib().gdn_rotary, q.data_ptr(), _ptr(k), qo.data_ptr(), _ptr(ko),
+        _STRIDES(*a, *c, *b, *d), B, T, H, Hk, D, positions.data_ptr(), positions.dtype is torch.int64,
+        T if positions.dim() == 2 else 0, inv_freq.data_ptr(), 2 * R, magnitude, interleaved, inverse,
+        dt, _stream(dev)), name)
+    if inplace:
+        # (autograd, where it kept them, sees that they changed)
+        increment_version([t for t in (q, k) if t is not None and not t.is_inference()])
+    return qo, ko
 
 
 def _new(t):
-    return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
 
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, magnitude, interleaved):
-        name = "rotary_embedding"
-        q4, k4, pos, freq, dt = _args(q, k, positions, inv_freq, name)
-        qo, ko = _new(q4), _new(k4)
-        _turn(q4, k4, qo, ko, pos, freq, dt, magnitude, interleaved, False, name)
+        qo, ko = _turn(q, k, positions, inv_freq, magnitude, interleaved, False, False,
+                       "rotary_embedding")
         ctx.save_for_backward(positions, inv_freq)
         ctx.rest = magnitude, interleaved
         ctx.set_materialize_grads(False)
-        if q.dim() == 3:
-            qo, ko = qo[0], None if ko is None else ko[0]
         return qo if k is None else (qo, ko)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dq, dk=None):
         positions, inv_freq = ctx.saved_tensors
-        magnitude, interleaved = ctx.rest
-        name = "rotary_embedding"
         want_q, want_k = ctx.needs_input_grad[:2]
-        a = dq if want_q else None
-        b = dk if want_k else None
-        if a is None:
-            a, b = b, None
+        if not want_q:
+            dq = None
+        if not want_k:
+            dk = None
+        a, b = (dk, None) if dq is None else (dq, dk)
         if a is None:
             return None, None, None, None, None, None
-        x, y, pos, freq, dt = _args(a, b, positions, inv_freq, name)
-        xo, yo = _new(x), _new(y)
-        _turn(x, y, xo, yo, pos, freq, dt, magnitude, interleaved, True, name)
-        if a.dim() == 3:
-            xo, yo = xo[0], None if yo is None else yo[0]
-        if not want_q or dq is None:
-            xo, yo = None, xo
-        return xo, yo, None, None, None, None
+        a, b = _turn(a, b, positions, inv_freq, *ctx.rest, True, False, "rotary_embedding")
+        return (*((None, a) if dq is None else (a, b)), None, None, None, None)
 
 
 def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor,
@@ -184,20 +177,5 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
         if inplace:
             raise ValueError(f"{name}: inplace is not supported when gradients are required.")
         return _Rotary.apply(q, k, positions, inv_freq, float(magnitude), bool(interleaved))
-    q4, k4, pos, freq, dt = _args(q, k, positions, inv_freq, name)
-    if inplace:
-        for t in (q, k):
-            if t is not None and (t.stride(-1) != 1 or not _apart(t)):
-                raise ValueError(f"{name}: in place q and k must have contiguous heads and elements "
-                                 "of their own.")
-        qo, ko = q4, k4
-    else:
-        qo, ko = _new(q4), _new(k4)
-    _turn(q4, k4, qo, ko, pos, freq, dt, float(magnitude), bool(interleaved), False, name)
-    if inplace:
-        qo, ko = q, k
-        # (autograd, where it kept them, sees that they changed)
-        increment_version([t for t in (q, k) if t is not None and not t.is_inference()])
-    elif q.dim() == 3:
-        qo, ko = qo[0], None if ko is None else ko[0]
-    return qo if k is None else (qo, ko)
+    q, k = _turn(q, k, positions, inv_freq, float(magnitude), bool(interleaved), False, inplace, name)
+    return q if k is None else (q, k)
