@@ -15,9 +15,13 @@ Linear attention with a decay for each head (``linear_attention``):
     fused_recurrent_linear_attn
 Layer norm (``norm``):
     layer_norm (differentiable; layer_norm_bwd)
+What stands around a hybrid model's attention layers (``norm``, ``rotary``, ``paged_attention``):
+    rms_norm (residual added; differentiable; rms_norm_bwd), rms_norm_quant (8 bits),
+    rotary_embedding (differentiable), rotary_frequencies,
+    PagedKVCache, paged_cache_write, paged_cache_read, paged_attention
 
-All call hand-written HIP kernels through the C ABI in include/gdn.h,
-include/gdn_layer.h and include/gdn_linear.h (``libgdn.so``, built by ``python -m avelang_amd.build``).
+All call hand-written HIP kernels through the C ABI in include/gdn.h, include/gdn_layer.h,
+include/gdn_linear.h and include/gdn_attn.h (``libgdn.so``, built by ``python -m avelang_amd.build``).
 """
 from .gated_delta_rule import (  # noqa: F401
     chunk_bwd_workspace_bytes,

@@ -73,33 +73,48 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
   return x;
 }
 
-// A workgroup takes 256 / LPR tokens of one head (blockIdx.y) of k or v
-// (blockIdx.z): what it writes of codes and scales is in one piece.  One row per
-// group of lanes: four on their way to each measured 29 us for 20011 tokens of 8
-// heads of 128 in e4m3 (one: 26 us, 4.8 TB/s read and written; read back 22 us
-// either way, 5.6 TB/s) and 5.0 us for 256 tokens of 2 heads of 256 (one: 3.0).
-template <int DT, int CT, int D>
+// A workgroup takes U 256 / LPR tokens of one head (blockIdx.y) of k or v
+// (blockIdx.z): what it writes of codes and scales is in one piece.  U rows are on
+// their way to a group of lanes: with 8-bit rows 2 where there are workgroups by the
+// dozen to a CU (their launch, and what each lane works out ahead of its row, shows:
+// 40000 tokens of 8 heads of 128 in e4m3 are written in 58 us, 4.2 TB/s read and
+// written, and read in 50, 4.9 TB/s; one row 64 and 58, four 61 and 51), else 1 (256
+// tokens of 2 heads of 256 3.0 and 2.8 us, two rows 3.6 and 3.3; 20011 of 8 heads of
+// 128 in bf16 34 and 30 either way).
+template <int DT, int CT, int D, int U>
 __global__ __launch_bounds__(256) void paged_write_kernel(PagedArgs a) {
   constexpr int LPR = D / 8, GR = 256 / LPR;
   const int l = threadIdx.x % LPR, h = blockIdx.y, k = blockIdx.z;
-  const long long t = (long long)blockIdx.x * GR + threadIdx.x / LPR;
-  if (t >= a.T) return;   // (the lanes of a row together, here and below)
-  const long long slot = slot_at(a, t);
-  const u32x4e raw = *reinterpret_cast<const u32x4e*>(static_cast<const uint16_t*>(a.in[k]) + t * a.token[k] +
-                                                      h * a.head[k] + 8 * l);
-  if (slot < 0 || slot >= a.num_slots) return;
-  const long long dst = cache_row(a, slot, h);
-  if constexpr (CT == DT) {
-    reinterpret_cast<u32x4e*>(a.out[k])[dst * LPR + l] = raw;
-  } else {
-    float x[8];
-    unpack<DT>(raw, x);
-    uint32_t m = 0;
+  const long long t0 = (long long)blockIdx.x * (GR * U) + threadIdx.x / LPR;
+  u32x4e raw[U];
+  long long dst[U];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) m = max(m, abs_bits(x[j]));
-    m = lanes_max<LPR>(m);
-    if (l == 0) a.scale[k][dst] = row8(m, CT).scale;
-    reinterpret_cast<u32x2b*>(a.out[k])[dst * LPR + l] = codes8<CT>(x, fmaxf(__uint_as_float(m), 0x1p-100f));
+  for (int i = 0; i < U; ++i) {
+    const long long t = t0 + i * GR;
+    dst[i] = -1;
+    if (t >= a.T) break;   // (the lanes of a row together, here and below)
+    const long long slot = slot_at(a, t);
+    raw[i] = *reinterpret_cast<const u32x4e*>(static_cast<const uint16_t*>(a.in[k]) + t * a.token[k] +
+                                              h * a.head[k] + 8 * l);
+    if (slot >= 0 && slot < a.num_slots) dst[i] = cache_row(a, slot, h);
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    if (t0 + i * GR >= a.T) return;
+    if (dst[i] < 0) continue;
+    if constexpr (CT == DT) {
+      reinterpret_cast<u32x4e*>(a.out[k])[dst[i] * LPR + l] = raw[i];
+    } else {
+      float x[8];
+      unpack<DT>(raw[i], x);
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) m = max(m, abs_bits(x[j]));
+      m = lanes_max<LPR>(m);
+      if (l == 0) a.scale[k][dst[i]] = row8(m, CT).scale;
+      reinterpret_cast<u32x2b*>(a.out[k])[dst[i] * LPR + l] =
+          codes8<CT>(x, fmaxf(__uint_as_float(m), 0x1p-100f));
+    }
   }
 }
 
@@ -119,35 +134,50 @@ __device__ __forceinline__ void values4(uint32_t w, float* f) {
   }
 }
 
-template <int DT, int CT, int D>
+template <int DT, int CT, int D, int U>
 __global__ __launch_bounds__(256) void paged_read_kernel(PagedArgs a) {
   constexpr int LPR = D / 8, GR = 256 / LPR;
+  constexpr bool C8 = CT == GDN_DTYPE_E4M3 || CT == GDN_DTYPE_I8;
   const int l = threadIdx.x % LPR, h = blockIdx.y, k = blockIdx.z;
-  const long long t = (long long)blockIdx.x * GR + threadIdx.x / LPR;
-  if (t >= a.T) return;
-  const long long slot = slot_at(a, t), at = t * a.H + h;
-  const bool there = slot >= 0 && slot < a.num_slots;
-  const long long src = there ? cache_row(a, slot, h) : 0;
-  if constexpr (CT == GDN_DTYPE_E4M3 || CT == GDN_DTYPE_I8) {
-    u32x2b code{0, 0};
-    float scale = 0.f, f[8];
-    if (there) {
-      code = reinterpret_cast<const u32x2b*>(a.in[k])[src * LPR + l];
-      scale = a.scale[k][src];
-    }
-    values4<CT>(code[0], f);
-    values4<CT>(code[1], f + 4);
+  const long long t0 = (long long)blockIdx.x * (GR * U) + threadIdx.x / LPR;
+  u32x4e raw[U];
+  u32x2b code[U];
+  float scale[U];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      f[j] *= scale;
-      asm("" : "+v"(f[j]));   // (rounded to fp32 first, not in one step with the conversion to fp16)
+  for (int i = 0; i < U; ++i) {
+    const long long t = t0 + i * GR;
+    raw[i] = u32x4e{0, 0, 0, 0};
+    code[i] = u32x2b{0, 0};
+    scale[i] = 0.f;
+    if (t >= a.T) break;
+    const long long slot = slot_at(a, t);
+    if (slot < 0 || slot >= a.num_slots) continue;
+    const long long src = cache_row(a, slot, h);
+    if constexpr (C8) {
+      code[i] = reinterpret_cast<const u32x2b*>(a.in[k])[src * LPR + l];
+      scale[i] = a.scale[k][src];
+    } else {
+      raw[i] = reinterpret_cast<const u32x4e*>(a.in[k])[src * LPR + l];
     }
-    stn<DT, 8>(a.out[k], at * D + 8 * l, f);
-  } else {
-    static_assert(DT == CT, "16-bit rows as they are");
-    u32x4e raw{0, 0, 0, 0};
-    if (there) raw = reinterpret_cast<const u32x4e*>(a.in[k])[src * LPR + l];
-    reinterpret_cast<u32x4e*>(a.out[k])[at * LPR + l] = raw;
+  }
+#pragma unroll
+  for (int i = 0; i < U; ++i) {
+    const long long t = t0 + i * GR, at = t * a.H + h;
+    if (t >= a.T) return;
+    if constexpr (C8) {
+      float f[8];
+      values4<CT>(code[i][0], f);
+      values4<CT>(code[i][1], f + 4);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        f[j] *= scale[i];
+        asm("" : "+v"(f[j]));   // (rounded to fp32 first, not in one step with the conversion to fp16)
+      }
+      stn<DT, 8>(a.out[k], at * D + 8 * l, f);
+    } else {
+      static_assert(DT == CT, "16-bit rows as they are");
+      reinterpret_cast<u32x4e*>(a.out[k])[at * LPR + l] = raw[i];
+    }
   }
 }
 
@@ -181,13 +211,23 @@ namespace {
 int launch_paged(const char* name, bool write, const gdn::PagedArgs& a, int D, int dtype, int cache_dtype,
                  hipStream_t st) {
   const int per = 256 / (D / 8);
-  const dim3 grid((unsigned)((a.T + (long long)per - 1) / per), (unsigned)a.H, 2);
+  const bool two = cache_dtype != dtype && (long long)a.T * a.H * 2 / per >= 32LL * gdn::device_cus();
+  const int tokens = two ? 2 * per : per;
+  const dim3 grid((unsigned)((a.T + (long long)tokens - 1) / tokens), (unsigned)a.H, 2);
   if (const int fit = gdn_host::check_lanes(name, grid.x, 256)) return fit;
   gdn_host::launch_begin();
+#define GDN_PAGED_U(TT, CC, DD, UU)                                                                        \
+  if (write) hipLaunchKernelGGL((gdn::paged_write_kernel<TT, CC, DD, UU>), grid, dim3(256), 0, st, a);     \
+  else hipLaunchKernelGGL((gdn::paged_read_kernel<TT, CC, DD, UU>), grid, dim3(256), 0, st, a);
 #define GDN_PAGED(TT, CC, DD)                                                                              \
   if (dtype == TT && cache_dtype == CC && D == DD) {                                                       \
-    if (write) hipLaunchKernelGGL((gdn::paged_write_kernel<TT, CC, DD>), grid, dim3(256), 0, st, a);       \
-    else hipLaunchKernelGGL((gdn::paged_read_kernel<TT, CC, DD>), grid, dim3(256), 0, st, a);              \
+    if constexpr (TT != CC) {                                                                              \
+      if (two) {                                                                                           \
+        GDN_PAGED_U(TT, CC, DD, 2)                                                                         \
+        return gdn_host::check_launch(name);                                                               \
+      }                                                                                                    \
+    }                                                                                                      \
+    GDN_PAGED_U(TT, CC, DD, 1)                                                                             \
     return gdn_host::check_launch(name);                                                                   \
   }
 #define GDN_PAGED_D(TT, CC) GDN_PAGED(TT, CC, 64) GDN_PAGED(TT, CC, 128) GDN_PAGED(TT, CC, 256)
@@ -196,6 +236,7 @@ int launch_paged(const char* name, bool write, const gdn::PagedArgs& a, int D, i
   GDN_PAGED_D(GDN_DTYPE_F16, GDN_DTYPE_E4M3) GDN_PAGED_D(GDN_DTYPE_F16, GDN_DTYPE_I8)
 #undef GDN_PAGED_D
 #undef GDN_PAGED
+#undef GDN_PAGED_U
   return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": dtype must be bf16 or f16, and the cache's unless it "
                                                            "has 8 bits");
 }

