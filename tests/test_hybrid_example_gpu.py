@@ -181,3 +181,105 @@ def test_cache_tensors(rocm_device):
     c.k.data = old.clone()
     old.zero_()
     assert all(torch.equal(a, b) for a, b in zip(ave.paged_cache_read(c, slots), before))
+
+
+@pytest.mark.parametrize("code", [torch.bfloat16, torch.float8_e4m3fn, torch.int8])
+def test_captured_decode_step(rocm_device, code):
+    """Norm, rotation in place, cache write, attention and the 8-bit norm in one graph, replayed token by
+    token beside the same calls run eagerly on a copy of the cache."""
+    N, Hq, H, D, page, dev = 5, 8, 2, 128, 16, dict(device=rocm_device)
+    gen = torch.Generator(rocm_device).manual_seed(3)
+    rand = lambda *s: torch.randn(*s, generator=gen, **dev).bfloat16()  # noqa: E731
+    x, res, w = rand(N, (Hq + 2 * H) * D), rand(N, (Hq + 2 * H) * D), rand((Hq + 2 * H) * D)
+    f, size = ave.rotary_frequencies(D // 2, factor=4.0, original=2048, device=rocm_device)
+    caches = [ave.PagedKVCache.zeros(64, page, H, D, code) for _ in "ab"]
+    table = torch.randperm(64, generator=gen, **dev).int()[:N * 8].view(N, 8)
+    lens = torch.tensor([0, 15, 16, 31, 100], dtype=torch.int32, **dev)
+    first = int(lens.max())
+    for c in caches:
+        for t in (c.k, c.v):
+            t.view(torch.uint8).fill_(0x30)
+        for t in (c.k_scale, c.v_scale):
+            if t is not None:
+                t.fill_(0.01)
+
+    def step(c, n):
+        y, h = ave.rms_norm(x, w, residual=res, offset=1.0)
+        q, k, v = (t.view(N, 1, -1, D) for t in y.split([Hq * D, H * D, H * D], -1))
+        pos = n.long()[:, None]
+        ave.rotary_embedding(q, k, pos, f, magnitude=size, inplace=True)
+        slots = table.gather(1, pos // page).long() * page + pos % page
+        ave.paged_cache_write(c, k, v, slots)
+        o, lse = ave.paged_attention(q, c, table, n + 1, return_lse=True)
+        return (h, o, lse) + ave.rms_norm_quant(o.flatten(2), dtype=torch.int8)
+
+    spare = ave.PagedKVCache.zeros(64, page, H, D, code)
+    step(spare, lens)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(caches[0], lens)
+    for i in range(4):
+        x.normal_(generator=gen)
+        res.normal_(generator=gen)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, step(caches[1], lens)):
+            assert torch.equal(a, b)
+        assert torch.equal(caches[0].k.view(torch.uint8), caches[1].k.view(torch.uint8))
+        assert torch.equal(caches[0].v.view(torch.uint8), caches[1].v.view(torch.uint8))
+        lens += 1
+    assert int(lens.max()) == first + 4
+
+
+@pytest.mark.parametrize("rows,D,t", [(3, 256, torch.bfloat16), (700, 1000, torch.float32), (40, 9000, torch.bfloat16)])
+def test_captured_gradients(rocm_device, rows, D, t):
+    """The norm's and the rotation's gradients in one graph, replayed with new inputs."""
+    dev = dict(device=rocm_device)
+    x, r, dy, dh = (torch.randn(rows, D, **dev).to(t) for _ in range(4))
+    w = torch.randn(D, **dev)
+    q, dq = (torch.randn(rows, 2, 64, **dev).to(t) for _ in "qd")
+    pos, f = torch.arange(rows, **dev), torch.ones(32, dtype=torch.float64, **dev)
+
+    def work():
+        y, h = ave.rms_norm(x, w, residual=r)
+        return (y, h) + ave.rms_norm_bwd(h, w, dy, dh) + (ave.rotary_embedding(q, None, pos, f),)
+
+    work()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = work()
+    for _ in range(3):
+        for a in (x, r, dy, dh, w, q):
+            a.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, work()):
+            assert torch.equal(a, b)
+
+
+def test_on_another_stream(rocm_device):
+    """Inputs of the current stream, calls and gradients on another."""
+    dev = dict(device=rocm_device)
+    x, dy = (torch.randn(300, 512, **dev).bfloat16() for _ in "xy")
+    w = torch.randn(512, **dev)
+    q, dq = (torch.randn(300, 4, 64, **dev).bfloat16() for _ in "qd")
+    pos, f = torch.arange(300, **dev), torch.ones(32, dtype=torch.float64, **dev)
+
+    def work():
+        a, b, c = (t.clone().requires_grad_() for t in (x, w, q))
+        y = ave.rms_norm(a, b)
+        z = ave.rotary_embedding(c, None, pos, f)
+        c8 = ave.PagedKVCache.zeros(20, 16, 4, 64, torch.int8)
+        ave.paged_cache_write(c8, z.detach(), dq, pos)
+        return [y, z, *torch.autograd.grad([y, z], [a, b, c], [dy, dq]), *ave.paged_cache_read(c8, pos)]
+
+    want = work()
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        got = work()
+    st.synchronize()
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
