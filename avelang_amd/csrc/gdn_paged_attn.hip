@@ -49,6 +49,7 @@ struct PagedAttnArgs {
   int N, L, Hq, Hkv, G, R, RG, rows;   // R = L G rows per kv-head in RG groups of at most `rows`
   int num_pages, page, cap, window;
   int split;      // work may be cut (else there is no second launch)
+  int whole;      // every (sequence, kv-head) is one unit, however long
   int by_item;    // desc has an entry per (sequence, kv-head, group of rows), not per workgroup
   float scale2;   // scale log2(e)
 };
@@ -62,7 +63,7 @@ __device__ __forceinline__ Span span_of(const PagedAttnArgs& a, int n) {
   Span s;
   s.hi = min(max(a.lens[n], 0), a.cap);
   s.lo = a.window > 0 ? max(0, s.hi - a.L + 1 - a.window) & ~15 : 0;
-  s.units = max(1, (s.hi - s.lo + UNIT - 1) / UNIT);
+  s.units = a.whole ? 1 : max(1, (s.hi - s.lo + UNIT - 1) / UNIT);
   return s;
 }
 
@@ -294,7 +295,8 @@ void paged_attn_kernel(PagedAttnArgs a) {
     const int rel = u - prefix * HG, item = EACH ? u % HG : rel / cost, start = EACH ? 0 : rel % cost;
     const int len = EACH ? cost : min(cost - start, u1 - u);
     const int kvh = item / a.RG, rg = item % a.RG;
-    const int t0 = sp.lo + max(start - extra, 0) * UNIT, t1 = min(sp.lo + (start + len - extra) * UNIT, sp.hi);
+    const int t0 = sp.lo + max(start - extra, 0) * UNIT;
+    const int t1 = a.whole ? sp.hi : min(sp.lo + (start + len - extra) * UNIT, sp.hi);
 
     // the rows' queries: column c16 of tile n's operand is row row_of(n)
     auto row_of = [&](int i) { return 16 * ((rg * RWS + rw) * NT + i) + c16; };
@@ -803,6 +805,7 @@ struct AttnPlan {
   long long wgs, items;
   bool split;   // some work may be cut
   bool each;    // every wave on its own
+  bool whole;   // every (sequence, kv-head) one unit
   size_t desc, bytes;
 };
 int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_length, int row_bytes, AttnPlan& p) {
@@ -831,10 +834,17 @@ int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_le
   // tokens 43 us (in shares 56), to 100 tokens 12.5 (25.6), to 1000 69 (76); bf16 to 500
   // 62 either way; rows of 512 bytes leave half of the waves (380, in shares 368).
   p.each = row_bytes && row_bytes <= 256 && p.nt == 1 && p.items >= 4LL * gdn::device_cus() && max_length <= kEachMost;
-  p.split = units > 1 && !p.each;
   p.wgs = (long long)gdn::resident(D) * gdn::device_cus();
   if (p.wgs > gdn::kMostParts) p.wgs = gdn::kMostParts;
+  // few units each are not cut: a join costs what two units do, and shares gain the
+  // less the more workgroups there are without.  8 heads of 128, whole against cut:
+  // 60 ragged sequences to 250, 700, 2000 tokens of bf16 11.0, 19.9, 55.8 us (15.1,
+  // 23.4, 55.4), to 449, 1500 of e4m3 13.7, 26.8 (19.6, 29.3); 16 to 250, 700 of bf16
+  // 7.7, 13.6 (9.1, 12.5); one of 250, 449 tokens 7.6, 9.6 (8.6, 8.7).
+  p.whole = p.each || (row_bytes && p.items <= p.wgs && (units - 2) * p.wgs <= 6 * p.items);
   if (p.wgs > most) p.wgs = most;
+  p.split = units > 1 && !p.whole;
+  if (p.whole && p.wgs > p.items) p.wgs = p.items;
   if (p.each && p.wgs > (p.items + 3) / 4) p.wgs = (p.items + 3) / 4;
   p.desc = (size_t)p.wgs * 16;
   p.bytes = p.desc + (size_t)p.wgs * 2 * p.rows * (D + 2) * sizeof(float);
@@ -919,6 +929,7 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long long q_seq, long long q_to
   a.page = page_size;
   a.cap = max_length;
   a.split = p.split;
+  a.whole = p.whole;
   a.by_item = p.items <= p.wgs;
   a.window = window > (1 << 30) ? 1 << 30 : window;
   a.scale2 = scale * 1.44269504088896340736f;

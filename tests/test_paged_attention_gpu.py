@@ -124,6 +124,26 @@ def test_many_short_drafts(rocm_device, L, window, t, code):
         assert torch.equal(o[at][:, :-1], base[at][:, :-1]) and o[at][:, -1, 4:, 7].isnan().all()
 
 
+@pytest.mark.parametrize("t,code", CODES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("L,Hq,window", [(1, 8, 0), (3, 8, 0), (5, 8, 33), (9, 8, 0), (20, 4, 70)])
+def test_few_units(rocm_device, L, Hq, window, D, t, code):
+    """Sequences of two units at most, which one workgroup takes whole."""
+    q, cache, table, n = _case([256, 0, 129, 128, 1, 2, 17, 255, 200], L, Hq, 2, D, 16, t, code, seed=9)
+    o, lse = ave.paged_attention(q, cache, table, n, window=window, return_lse=True)
+    _check(o, lse, q, cache, table, n, None, window)
+
+
+@pytest.mark.parametrize("t,code", CODES)
+@pytest.mark.parametrize("D,N", [(64, 61), (128, 61), (256, 30)])
+def test_whole_sequences(rocm_device, D, N, t, code):
+    """Several units each, as many sequences as leave nothing to share out."""
+    lens = [(197 * i) % 880 + 1 for i in range(N)]
+    q, cache, table, n = _case(lens, 1, 16, 8, D, 16, t, code, seed=4)
+    o, lse = ave.paged_attention(q, cache, table, n, return_lse=True)
+    _check(o, lse, q, cache, table, n)
+
+
 @pytest.mark.parametrize("L,Hq,H", [(16, 8, 2), (64, 4, 1), (40, 16, 2)])
 def test_many_rows(rocm_device, L, Hq, H):
     """More rows to a kv-head than the waves of one workgroup take."""
