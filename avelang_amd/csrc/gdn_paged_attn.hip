@@ -25,6 +25,8 @@
 // 48 of 1 to 6000, 4 heads of 128 in bf16, 4 newest tokens 67 + 5, 4.5 TB/s (the
 // shares' starts and ends, and the last tokens' masks); one of 449 8.6 + 2.7: a chain
 // of latencies, lengths, table, K, softmax, the waves' join.
+#include <algorithm>
+
 #include "gdn_bits8.h"
 #include "gdn_norm_rows.h"
 
@@ -48,8 +50,7 @@ struct PagedAttnArgs {
   int4* desc;
   int N, L, Hq, Hkv, G, R, RG, rows;   // R = L G rows per kv-head in RG groups of at most `rows`
   int num_pages, page, cap, window;
-  int split;      // work may be cut (else there is no second launch)
-  int whole;      // every (sequence, kv-head) is one unit, however long
+  int whole;      // every (sequence, kv-head) is one unit, however long (no second launch)
   int by_item;    // desc has an entry per (sequence, kv-head, group of rows), not per workgroup
   float scale2;   // scale log2(e)
 };
@@ -243,6 +244,11 @@ void paged_attn_kernel(PagedAttnArgs a) {
   if constexpr (EACH) {
     u0 = blockIdx.x * 4 + wave;
     u1 = a.N * HG;
+  } else if (a.whole) {
+    share = (a.N * HG + gridDim.x - 1) / gridDim.x;
+    u0 = min((int)blockIdx.x * share, a.N * HG);
+    u1 = min(u0 + share, a.N * HG);
+    n = prefix = u0 / HG;
   } else {
     const int per = (a.N + 255) / 256, first = tid * per, last = min(first + per, a.N);
     int sum = 0;
@@ -265,12 +271,12 @@ void paged_attn_kernel(PagedAttnArgs a) {
     // a workgroup's queries, first loads and output take about a unit's time: where
     // shares are of several units each (sequence, kv-head) counts one more, ahead of
     // its own.  (48 sequences of 125 to 6000 tokens: 95 us, with it 76.)
-    extra = a.split && units * HG > (int)gridDim.x;
+    extra = units * HG > (int)gridDim.x;
     const int total = (units + extra * a.N) * HG;
     share = (total + gridDim.x - 1) / gridDim.x;
     u0 = min((int)blockIdx.x * share, total);
     u1 = min(u0 + share, total);
-    if (tid == 0 && !a.by_item) a.desc[blockIdx.x] = int4{0, 0, 0, 0};
+    if (!a.by_item && tid == 0) a.desc[blockIdx.x] = int4{0, 0, 0, 0};
     if (u0 >= u1) return;
     int at = incl - sum + extra * min(first, a.N);
     if (at * HG <= u0 && u0 < (incl + extra * last) * HG) {
@@ -680,7 +686,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
       }
     }
     // what the joining launch has to do: {sequence, item, first part's slot, parts}
-    if (start == 0 && tid == 0 && (!whole || a.by_item))
+    if (!a.whole && start == 0 && tid == 0 && (!whole || a.by_item))
       a.desc[a.by_item ? n * HG + item : blockIdx.x] =
           int4{n, item, slot, whole ? 0 : 1 + (cost - len + share - 1) / share};
     u += len;
@@ -797,15 +803,12 @@ int check_cache(const char* name, const void* k_cache, const void* v_cache, cons
 
 namespace {
 
-constexpr int kEachMost = 1024;
-
 // Workgroups, and how the rows of a kv-head are laid over their waves.
 struct AttnPlan {
   int nt, rw, rg, rows;
-  long long wgs, items;
-  bool split;   // some work may be cut
+  long long wgs, grid, items;   // workgroups where work is cut, launched
   bool each;    // every wave on its own
-  bool whole;   // every (sequence, kv-head) one unit
+  bool whole;   // every (sequence, kv-head) one unit: nothing is cut
   size_t desc, bytes;
 };
 int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_length, int row_bytes, AttnPlan& p) {
@@ -829,23 +832,22 @@ int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_le
   if (most + (long long)N * Hkv * p.rg >= (1LL << 30))
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": problem too large");
   p.items = (long long)N * Hkv * p.rg;
-  // short sequences in numbers: a wave to each (sequence, kv-head), as many at once as
-  // there are waves, nothing joined.  256 sequences of 8 heads of 128: e4m3, 2 to 600
-  // tokens 43 us (in shares 56), to 100 tokens 12.5 (25.6), to 1000 69 (76); bf16 to 500
-  // 62 either way; rows of 512 bytes leave half of the waves (380, in shares 368).
-  p.each = row_bytes && row_bytes <= 256 && p.nt == 1 && p.items >= 4LL * gdn::device_cus() && max_length <= kEachMost;
   p.wgs = (long long)gdn::resident(D) * gdn::device_cus();
   if (p.wgs > gdn::kMostParts) p.wgs = gdn::kMostParts;
-  // few units each are not cut: a join costs what two units do, and shares gain the
-  // less the more workgroups there are without.  8 heads of 128, whole against cut:
-  // 60 ragged sequences to 250, 700, 2000 tokens of bf16 11.0, 19.9, 55.8 us (15.1,
-  // 23.4, 55.4), to 449, 1500 of e4m3 13.7, 26.8 (19.6, 29.3); 16 to 250, 700 of bf16
-  // 7.7, 13.6 (9.1, 12.5); one of 250, 449 tokens 7.6, 9.6 (8.6, 8.7).
-  p.whole = p.each || (row_bytes && p.items <= p.wgs && (units - 2) * p.wgs <= 6 * p.items);
+  // Short sequences in numbers: a wave to each (sequence, kv-head), nothing joined, up
+  // to 64 KiB of K and V each for every `wgs` of them.  8 heads of 128, ragged, in us
+  // (each a wave / each a workgroup / shares): 256 sequences of e4m3 to 250 tokens 20 /
+  // 34 / 32, to 1000 68 / 71 / 75, to 2000 126 / 112 / 120; of bf16 to 250 27 / 33 / 35,
+  // to 700 80 / 76 / 82; 85 of e4m3 to 250 14.9 / 16.6 / 16.8, to 1000 38 / 26 / 30.
+  p.each = row_bytes && p.nt == 1 && (long long)max_length * row_bytes * p.wgs <= 32768 * p.items;
+  // Else few units each are not cut: a join costs what two units do, and shares gain
+  // the less the more workgroups there are without.  bf16 as above, in us: one sequence
+  // of 250 tokens 6.8 (cut 8.6); 16 to 250, 700 6.9, 12.7 (9.1, 12.5); 60 to 449 13.9
+  // (19.4); 85 to 700, 3000 24, 111 (27, 111); 256 of 4 heads, 4 newest tokens, to 1000
+  // 63 (76).  24 units at most: one long sequence among short ones is one workgroup's.
+  p.whole = p.each || (row_bytes && units <= 24 && (units - 2) * p.wgs <= 6 * p.items);
   if (p.wgs > most) p.wgs = most;
-  p.split = units > 1 && !p.whole;
-  if (p.whole && p.wgs > p.items) p.wgs = p.items;
-  if (p.each && p.wgs > (p.items + 3) / 4) p.wgs = (p.items + 3) / 4;
+  p.grid = p.each ? std::min(p.wgs, (p.items + 3) / 4) : p.whole ? std::min(p.items, 1LL << 20) : p.wgs;
   p.desc = (size_t)p.wgs * 16;
   p.bytes = p.desc + (size_t)p.wgs * 2 * p.rows * (D + 2) * sizeof(float);
   p.bytes = (p.bytes + 255) / 256 * 256;
@@ -928,7 +930,6 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long long q_seq, long long q_to
   a.num_pages = num_pages;
   a.page = page_size;
   a.cap = max_length;
-  a.split = p.split;
   a.whole = p.whole;
   a.by_item = p.items <= p.wgs;
   a.window = window > (1 << 30) ? 1 << 30 : window;
@@ -938,7 +939,7 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long long q_seq, long long q_to
   bool done = false;
 #define GDN_PA(QQ, CC, DD, TT, WW)                                                                \
   if (dtype == QQ && cache_dtype == CC && D == DD && p.nt == TT && (p.each ? 0 : p.rw) == WW) {   \
-    hipLaunchKernelGGL((gdn::paged_attn_kernel<QQ, CC, DD, TT, WW>), dim3((unsigned)p.wgs), dim3(256), 0, st, a); \
+    hipLaunchKernelGGL((gdn::paged_attn_kernel<QQ, CC, DD, TT, WW>), dim3((unsigned)p.grid), dim3(256), 0, st, a); \
     done = true;                                                                                  \
   }
 #define GDN_PA_W(QQ, CC, DD) GDN_PA(QQ, CC, DD, 1, 0) GDN_PA(QQ, CC, DD, 1, 1) GDN_PA(QQ, CC, DD, 2, 1) GDN_PA(QQ, CC, DD, 2, 2)
@@ -954,7 +955,7 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long long q_seq, long long q_to
 #undef GDN_PA
   if (!done)
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": the cache must be of q's type or have 8 bits");
-  if (!p.split) return gdn_host::check_launch(name);
+  if (p.whole) return gdn_host::check_launch(name);
   const dim3 grid((unsigned)(a.by_item ? p.items : p.wgs), (unsigned)p.rows);
   // few outputs of many parts each: a CU's worth of lanes to each (131072 tokens of
   // one sequence, 256 parts: see the kernel's figures)

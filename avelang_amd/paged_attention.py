@@ -212,7 +212,8 @@ def paged_attention(
     Returns o like q (contiguous), with ``return_lse`` ``(o, lse)``, lse fp32
     [N, L, Hq] the log of the softmax's sum.  A row that sees no token (lengths
     under L, or 0) is 0 with an lse of -inf.  ``max_length`` (default: what the
-    table holds) bounds the lengths; a larger one counts as this.  Pages outside
+    table holds) bounds the lengths; a larger one counts as this.  How work is laid
+    out follows from it: a tight one is faster where all are short.  Pages outside
     the cache give NaN; entries behind a sequence's last page are not read.
     ``out`` and ``workspace`` (uint8, ``paged_attention_workspace_bytes``; two
     captured graphs that may run at once need one each) avoid allocation.
