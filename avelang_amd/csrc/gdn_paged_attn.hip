@@ -227,7 +227,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
   constexpr int VD = E * ES / 4;                                   // words of them
   constexpr int CH = E * ES > 16 ? 16 / ES : E;                    // elements of one piece
   constexpr int NS = sixteens(ROW, NT), TT = 16 * NS;              // tokens that a wave takes at a time
-  constexpr bool LO = BF || QT == GDN_DTYPE_F16;   // P in two parts: 2^-9 (bf16), 2^-12 of one would show in o
+  constexpr bool LO = BF || QT == GDN_DTYPE_F16;   // P in two parts: 2^-8 (bf16), 2^-11 of one would show in o
   __shared__ float buf[EACH ? 1 : 4][EACH ? 1 : 16 * NT][D + 4];
   __shared__ float sm[4][16 * NT], sl[4][16 * NT];
   __shared__ int wave_sum[4];
