@@ -34,6 +34,9 @@ __device__ __forceinline__ uint32_t row_max(uint32_t x, uint32_t* red) {
   return x;
 }
 
+// 1 / sqrt(mean + eps) of a row's sum of squares.
+__device__ __forceinline__ float rstd_of(float s, int D, float eps) { return rsqrtf(s * (1.f / D) + eps); }
+
 struct RmsArgs {
   const void* x;
   const void* res;
@@ -47,16 +50,22 @@ struct RmsArgs {
   int wt, code;   // code: the output's type where it is one of 8 bits
 };
 
-// Codes of VEC values from element c of a row of D (at byte base).
+// Codes of VEC values from element c of a row of D (at byte base): the nearest fp32
+// quotients by the scale (one correction), rounded.
 template <int VEC>
 __device__ __forceinline__ void st_codes(void* p, long long base, int c, int D, const float (&f)[VEC],
-                                         float inv, int code) {
+                                         const Row8& r, int code) {
   uint32_t w[VEC / 4];
+  float q[VEC];
+#pragma unroll
+  for (int j = 0; j < VEC; ++j) {
+    q[j] = f[j] * r.inv;
+    q[j] = fmaf(fmaf(-q[j], r.scale, f[j]), r.inv, q[j]);
+  }
 #pragma unroll
   for (int u = 0; u < VEC / 4; ++u)
-    w[u] = code == GDN_DTYPE_E4M3
-               ? e4m3_4(f[4 * u] * inv, f[4 * u + 1] * inv, f[4 * u + 2] * inv, f[4 * u + 3] * inv)
-               : int8_4(f[4 * u] * inv, f[4 * u + 1] * inv, f[4 * u + 2] * inv, f[4 * u + 3] * inv);
+    w[u] = code == GDN_DTYPE_E4M3 ? e4m3_4(q[4 * u], q[4 * u + 1], q[4 * u + 2], q[4 * u + 3])
+                                  : int8_4(q[4 * u], q[4 * u + 1], q[4 * u + 2], q[4 * u + 3]);
   uint8_t* dst = static_cast<uint8_t*>(p) + base + c;
   if (c + VEC <= D) {
     if constexpr (VEC == 8)
@@ -118,7 +127,7 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(RmsArgs a) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) s += f[i][j] * f[i][j];   // (past the row's end 0)
   s = row_sum<LPR>(s, red);
-  const float rstd = 1.f / sqrtf(s / a.D + a.eps);
+  const float rstd = rstd_of(s, a.D, a.eps);
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
@@ -139,7 +148,7 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(RmsArgs a) {
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int c = (l + LPR * i) * VEC;
-    if (c < a.D) st_codes<VEC>(a.y, base, c, a.D, f[i], q.inv, a.code);
+    if (c < a.D) st_codes<VEC>(a.y, base, c, a.D, f[i], q, a.code);
   }
 }
 
@@ -162,7 +171,7 @@ __global__ __launch_bounds__(256) void rms_fwd_long_kernel(RmsArgs a) {
     for (int j = 0; j < VEC; ++j) s += f[j] * f[j];
   }
   s = row_sum<256>(s, red);
-  const float rstd = 1.f / sqrtf(s / a.D + a.eps);
+  const float rstd = rstd_of(s, a.D, a.eps);
   // (a lane reads again what itself has written)
   auto load = [&](int c) {
     if (a.res) ld_row<RT, VEC>(a.h, base, c, a.D, f);
@@ -187,7 +196,7 @@ __global__ __launch_bounds__(256) void rms_fwd_long_kernel(RmsArgs a) {
   if (threadIdx.x == 0) a.scale[r] = q.scale;
   for (int c = threadIdx.x * VEC; c < a.D; c += 256 * VEC) {
     load(c);
-    st_codes<VEC>(a.y, base, c, a.D, f, q.inv, a.code);
+    st_codes<VEC>(a.y, base, c, a.D, f, q, a.code);
   }
 }
 
@@ -307,7 +316,7 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(RmsBwdArgs a) {
         s += dy[i][j] * w[i][j] * x[i][j];
       }
     row_sum2<LPR>(ss, s, red[ph]);
-    const float rstd = 1.f / sqrtf(ss / a.D + a.eps);
+    const float rstd = rstd_of(ss, a.D, a.eps);
     s *= rstd * inv_d;   // mean(e hh)
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
@@ -376,7 +385,7 @@ __global__ __launch_bounds__(256) void rms_bwd_long_kernel(RmsBwdArgs a) {
     }
   }
   row_sum2<256>(ss, s, red);
-  const float rstd = 1.f / sqrtf(ss / a.D + a.eps);
+  const float rstd = rstd_of(ss, a.D, a.eps);
   s *= rstd / a.D;
   if (a.rstd && threadIdx.x == 0) a.rstd[r] = rstd;
   for (int c = threadIdx.x * VEC; c < a.D; c += 256 * VEC) {

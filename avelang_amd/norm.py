@@ -9,9 +9,9 @@ head's row by itself with parameters of its own (the norm of an attention's
 output).  The RMS norm also adds the residual stream and can leave its output in
 8 bits with a scale per row (``rms_norm_quant``).
 HIP kernels of ``csrc/gdn_norm.hip`` behind ``include/gdn_linear.h`` and of
-``csrc/gdn_rms.hip`` behind ``include/gdn_attn.h``; there is no fallback path.  The reference repository has no counterpart; the wrappers
-follow its kernel-library convention
-(python/avelang_kernels/amdgpu_gemm.py:458-494).
+``csrc/gdn_rms.hip`` behind ``include/gdn_attn.h``; there is no fallback path.
+The reference repository has no counterpart; the wrappers follow its
+kernel-library convention (python/avelang_kernels/amdgpu_gemm.py:458-494).
 """
 from __future__ import annotations
 
