@@ -283,3 +283,17 @@ def test_on_another_stream(rocm_device):
     st.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+def test_no_gradients_of_gradients(rocm_device):
+    """Gradients with a graph of their own are right, and refuse to be differentiated again."""
+    dev = dict(device=rocm_device)
+    x, w, q = torch.randn(5, 64, **dev), torch.randn(64, **dev), torch.randn(5, 2, 32, **dev)
+    pos, f = torch.arange(5, **dev), torch.ones(16, dtype=torch.float64, **dev)
+    for call, leaves in ((lambda a, b: ave.rms_norm(a, b), (x, w)), (lambda a: ave.rotary_embedding(a, None, pos, f), (q,))):
+        leaves = [t.clone().requires_grad_() for t in leaves]
+        want = torch.autograd.grad(call(*leaves).square().sum(), leaves)
+        got = torch.autograd.grad(call(*leaves).square().sum(), leaves, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            got[0].sum().backward()
