@@ -21,9 +21,9 @@
 // m, the sum and o in the workspace and a second launch joins them.
 //
 // Measured, kernel and join: 256 sequences of 100 to 8192 tokens, 8 heads of 128 in
-// e4m3 395 + 5 us, 5.7 TB/s; one of 131072, 2 heads of 256 in bf16 50 + 6, 5.4 TB/s;
+// e4m3 395 + 5 us, 5.7 TB/s; one of 131072, 2 heads of 256 in bf16 50 + 5, 5.4 TB/s;
 // 48 of 1 to 6000, 4 heads of 128 in bf16, 4 newest tokens 67 + 5, 4.5 TB/s (the
-// shares' starts and ends, and the last tokens' masks); one of 449 8.6 + 2.7: a chain
+// shares' starts and ends, and the last tokens' masks); one of 449 8.7 + 2.5: a chain
 // of latencies, lengths, table, K, softmax, the waves' join.
 #include <algorithm>
 
@@ -698,21 +698,23 @@ void paged_attn_kernel(PagedAttnArgs a) {
   }
 }
 
-// Parts of one (sequence, kv-head) joined: block (entry of desc, row).  D / 4 lanes
-// hold a row of a part, NT / (D / 4) parts are added at a time.
+// Parts of one (sequence, kv-head) joined: block (entry of desc, row, columns).  LP
+// lanes hold 4 LP columns of a row of a part, NT / LP parts are added at a time.
 constexpr int kMostParts = 1024;   // workgroups at most
 constexpr int kFewParts = 6;
-template <int QT, int D, int NT>
+template <int QT, int D, int NT, int LP>
 __global__ __launch_bounds__(NT) void paged_attn_join_kernel(PagedAttnArgs a) {
-  constexpr int LP = D / 4, GR = NT / LP, NW = NT / 64;
+  constexpr int GR = NT / LP, NW = NT / 64;
+  static_assert(LP <= 64, "a row's lanes are of one wave");
   __shared__ float w[kMostParts];
   __shared__ float red[2][NW];
-  __shared__ f32x4 acc[GR][LP];
+  __shared__ f32x4 acc[NW][LP];
   const int4 ds = a.desc[blockIdx.x];
   const int parts = ds.w;
   if (parts == 0) return;
   const int kvh = ds.y / a.RG, rg = ds.y % a.RG, row = blockIdx.y;
-  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, col = tid % LP, grp = tid / LP;
+  const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, grp = tid / LP;
+  const int col = blockIdx.z * LP + tid % LP;
   const size_t each = (size_t)a.rows * (D + 2);
   // part p: its workgroup's first, but for the one that begins here
   const int wg = ds.z / 2;
@@ -783,14 +785,18 @@ __global__ __launch_bounds__(NT) void paged_attn_join_kernel(PagedAttnArgs a) {
   f32x4 o = zero4();
 #pragma unroll 8
   for (int p = grp; p < parts; p += GR) o += w[p] * *reinterpret_cast<const f32x4*>(at(p) + row * D + 4 * col);
-  acc[grp][col] = o;
+#pragma unroll
+  for (int off = LP; off < 64; off *= 2)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] += __shfl_xor(o[j], off);
+  if (lane < LP) acc[wave][lane] = o;
   __syncthreads();
   if (tid >= LP) return;
   s = 0.f;
 #pragma unroll
   for (int i = 0; i < NW; ++i) s += red[1][i];
 #pragma unroll
-  for (int i = 1; i < GR; ++i) o += acc[i][col];
+  for (int i = 1; i < NW; ++i) o += acc[i][tid];
   put(orow, M, s, o);
 }
 
@@ -957,13 +963,15 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long long q_seq, long long q_to
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": the cache must be of q's type or have 8 bits");
   if (p.whole) return gdn_host::check_launch(name);
   const dim3 grid((unsigned)(a.by_item ? p.items : p.wgs), (unsigned)p.rows);
-  // few outputs of many parts each: a CU's worth of lanes to each (131072 tokens of
-  // one sequence, 256 parts: see the kernel's figures)
+  // few outputs of many parts each: a CU's worth of lanes to 64 columns of each
+  // (131072 tokens of one sequence, 256 parts of 16 rows of 256: 4.8 us, 6.2 with a CU
+  // to a whole row)
   const bool wide = (long long)grid.x * grid.y <= gdn::device_cus();
 #define GDN_PJ(QQ, DD)                                                                            \
   if (dtype == QQ && D == DD) {                                                                   \
-    if (wide) hipLaunchKernelGGL((gdn::paged_attn_join_kernel<QQ, DD, 1024>), grid, dim3(1024), 0, st, a); \
-    else hipLaunchKernelGGL((gdn::paged_attn_join_kernel<QQ, DD, 256>), grid, dim3(256), 0, st, a); \
+    if (wide) hipLaunchKernelGGL((gdn::paged_attn_join_kernel<QQ, DD, 1024, 16>), dim3(grid.x, grid.y, DD / 64), \
+                                 dim3(1024), 0, st, a);                                           \
+    else hipLaunchKernelGGL((gdn::paged_attn_join_kernel<QQ, DD, 256, DD / 4>), grid, dim3(256), 0, st, a); \
   }
   GDN_PJ(GDN_DTYPE_BF16, 64) GDN_PJ(GDN_DTYPE_BF16, 128) GDN_PJ(GDN_DTYPE_BF16, 256)
   GDN_PJ(GDN_DTYPE_F16, 64) GDN_PJ(GDN_DTYPE_F16, 128) GDN_PJ(GDN_DTYPE_F16, 256)
