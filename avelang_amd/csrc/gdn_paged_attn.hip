@@ -102,11 +102,6 @@ __device__ __forceinline__ float of_four(float x) {
 __device__ __forceinline__ float of_four(float x, int r) {
   return r == 0 ? of_four<0>(x) : r == 1 ? of_four<1>(x) : r == 2 ? of_four<2>(x) : of_four<3>(x);
 }
-// Largest value of each four lanes.
-__device__ __forceinline__ float xmax4(float x) {
-  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xb1, 0xf, 0xf, true)));
-  return fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4e, 0xf, 0xf, true)));
-}
 // 2^x in one instruction (results under 2^-126 are 0).
 __device__ __forceinline__ float exp2i(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -151,6 +146,9 @@ typedef uint32_t u32x4w __attribute__((ext_vector_type(4)));
 // as an fp16 denormal u 2^-24, times 2^15, less 128 2^-9: the value times 2^-9,
 // exactly.
 constexpr float kI8 = 512.f;
+// What the largest product of a row and V's scale becomes in fp16, up to twice as much:
+// 2^15 of 65504 at the top, 28 bits of normal values below it.
+constexpr float kTop = 0x1p14f;
 __device__ __forceinline__ uint32_t i8_pair(uint32_t u) {
   const f16x2 x = __builtin_bit_cast(f16x2, u);
   const f16x2 k = {(_Float16)32768.f, (_Float16)32768.f}, b = {(_Float16)-0.25f, (_Float16)-0.25f};
@@ -227,6 +225,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
   constexpr int VD = E * ES / 4;                                   // words of them
   constexpr int CH = E * ES > 16 ? 16 / ES : E;                    // elements of one piece
   constexpr int NS = sixteens(ROW, NT), TT = 16 * NS;              // tokens that a wave takes at a time
+  constexpr float BACK = (CT == GDN_DTYPE_I8 ? kI8 : 1.f) / kTop;   // C8: of acc, beside its unit
   constexpr bool LO = BF || QT == GDN_DTYPE_F16;   // P in two parts: 2^-8 (bf16), 2^-11 of one would show in o
   __shared__ float buf[EACH ? 1 : 4][EACH ? 1 : 16 * NT][D + 4];
   __shared__ float sm[4][16 * NT], sl[4][16 * NT];
@@ -416,11 +415,11 @@ void paged_attn_kernel(PagedAttnArgs a) {
     };
 
     f32x4 acc[NT][E];
-    float m[NT], sum[NT], vref = 0.f, vinv = 1.f;
+    float m[NT], sum[NT], unit[NT];   // C8: acc holds products with V in units of 2^m unit
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
       m[i] = -INFINITY;
-      sum[i] = 0.f;
+      sum[i] = unit[i] = 0.f;
 #pragma unroll
       for (int j = 0; j < E; ++j) acc[i][j] = zero4();
     }
@@ -524,24 +523,6 @@ void paged_attn_kernel(PagedAttnArgs a) {
         if ((it + 1) % (64 / NS) == 0) look_up(it + 1);
         load_k(it + 1);
       }
-      float grow = 1.f;
-      if constexpr (C8) {
-        // V's scales over a power of two no smaller than any so far: P stays in
-        // fp16's range
-        float big = 0.f;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-          if (part && tb + 16 * s + 4 * g + c16 % 4 >= t1) vscale[s] = 0.f;
-          big = fmaxf(big, vscale[s]);
-        }
-        big = xmax16(xmax4(big));
-        if (big > vref) {
-          const float next = __uint_as_float(min((__float_as_uint(big) & 0x7f800000u) + 0x800000u, 0x7e800000u));
-          grow = vref * (1.f / next);
-          vref = next;
-          vinv = 1.f / next;
-        }
-      }
       u16x8 hi[NT][NS / 2], lo[NT][NS / 2];
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
@@ -550,24 +531,50 @@ void paged_attn_kernel(PagedAttnArgs a) {
         for (int j = 1; j < 4 * NS; ++j) mx = fmaxf(mx, S[i][j / 4][j % 4]);
         mx = fmaxf(m[i], xmax16(mx));
         const float ref = mx == -INFINITY ? 0.f : mx;
-        if (__any(mx > m[i]) || (C8 && grow != 1.f)) {
+        if (__any(mx > m[i])) {
           const float f = exp2i(m[i] - ref);   // (m = -inf: 0)
           sum[i] *= f;
+          if constexpr (C8) {
+            unit[i] *= f;
+          } else {
 #pragma unroll
-          for (int j = 0; j < E; ++j) acc[i][j] *= f * grow;
+            for (int j = 0; j < E; ++j) acc[i][j] *= f;
+          }
           m[i] = mx;
         }
         f32x4 p[NS];
+        float big = 0.f;
 #pragma unroll
         for (int j = 0; j < 4 * NS; ++j) {
           float x = exp2i(S[i][j / 4][j % 4] - ref);
           sum[i] += x;
           if constexpr (C8) {
             // (a token that is not seen may have any scale)
-            const float y = x * (of_four(vscale[j / 4], j % 4) * vinv);
+            const float y = x * of_four(vscale[j / 4], j % 4);
             x = x == 0.f ? 0.f : y;
+            big = fmaxf(big, x);
           }
           p[j / 4][j % 4] = x;
+        }
+        if constexpr (C8) {
+          // P times V's scale, over a unit of the row's own: within a factor of two of the
+          // largest that it has formed, in units of 2^m, so that what other rows see, or what
+          // has no weight, cannot push this row's products out of fp16's range.  2^-110 at
+          // least (no row has a smaller scale): the quotient stays in fp32's.
+          big = xmax16(big);
+          big = big > 0.f ? fmaxf(big, 0x1p-110f) : 0.f;
+          const float was = unit[i];
+          const bool more = big > 2.f * was;
+          const bool any = __any(more);
+          if (any) unit[i] = more ? big : was;
+          const float inv = __builtin_amdgcn_rcpf(fmaxf(unit[i], 0x1p-111f) * (1.f / kTop));
+          if (any) {
+            const float f = more ? was * (1.f / kTop) * inv : 1.f;
+#pragma unroll
+            for (int j = 0; j < E; ++j) acc[i][j] *= f;
+          }
+#pragma unroll
+          for (int s = 0; s < NS; ++s) p[s] *= inv;
         }
 #pragma unroll
         for (int h = 0; h < NS / 2; ++h) operands<BF, LO>(p[2 * h], p[2 * h + 1], hi[i][h], lo[i][h]);
@@ -614,7 +621,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const float s = xsum16(sum[i]);
-        const float f = s == 0.f ? 0.f : 1.f / s * (C8 ? vref * (CT == GDN_DTYPE_I8 ? kI8 : 1.f) : 1.f);
+        const float f = s == 0.f ? 0.f : 1.f / s * (C8 ? unit[i] * BACK : 1.f);
         const int orow = row_of(i);
         if (orow >= a.R) continue;
         const long long at = ((long long)n * a.L + orow / a.G) * a.Hq + kvh * a.G + orow % a.G;
@@ -647,7 +654,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
 #pragma unroll
           for (int r = 0; r < 4; ++r)
             buf[wave][16 * i + c16][(j / CH) * 16 * CH + (4 * g + r) * CH + j % CH] =
-                acc[i][j][r] * (C8 ? vref * (CT == GDN_DTYPE_I8 ? kI8 : 1.f) : 1.f);
+                acc[i][j][r] * (C8 ? unit[i] * BACK : 1.f);
       }
     }
     __syncthreads();
