@@ -529,7 +529,11 @@ void paged_attn_kernel(PagedAttnArgs a) {
         float mx = S[i][0][0];
 #pragma unroll
         for (int j = 1; j < 4 * NS; ++j) mx = fmaxf(mx, S[i][j / 4][j % 4]);
-        mx = fmaxf(m[i], xmax16(mx));
+        mx = xmax16(mx);
+        // (P in fp16 as it is: up to 2^15, 29 bits of normal values; a score of 2^20 or more,
+        // of which 15 is not exact, up to 1)
+        if constexpr (CT == GDN_DTYPE_F16) mx -= fabsf(mx) < 0x1p20f ? 15.f : 0.f;
+        mx = fmaxf(m[i], mx);
         const float ref = mx == -INFINITY ? 0.f : mx;
         if (__any(mx > m[i])) {
           const float f = exp2i(m[i] - ref);   // (m = -inf: 0)

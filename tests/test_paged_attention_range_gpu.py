@@ -13,7 +13,7 @@ import torch
 
 import avelang_amd as ave
 from oracle import attn_ref as R
-from test_paged_attention_gpu import BF16, E4M3, F16, I8, _case
+from test_paged_attention_gpu import BF16, CODES, E4M3, F16, I8, _case
 
 pytestmark = pytest.mark.gpu
 C8 = [(BF16, E4M3), (F16, E4M3), (BF16, I8), (F16, I8)]
@@ -46,7 +46,7 @@ def _place(cache, table, i, t, k, v):
     ave.paged_cache_write(cache, k[None], v[None], torch.tensor([page * cache.k.shape[2] + row]))
 
 
-@pytest.mark.parametrize("t,code", [(BF16, BF16)] + C8)
+@pytest.mark.parametrize("t,code", CODES)
 @pytest.mark.parametrize("D,H,N,most", [(64, 2, 600, 300), (128, 8, 30, 880), (64, 1, 1, 9000)])
 def test_a_token_that_takes_nearly_all(rocm_device, D, H, N, most, t, code):
     """The first token takes 99.9 % of the softmax and has a small value: what is left is the other tokens'."""
@@ -59,6 +59,27 @@ def test_a_token_that_takes_nearly_all(rocm_device, D, H, N, most, t, code):
         k = k * (torch.log(torch.tensor(999.0 * m)) * D ** 0.5 / k.square().sum(-1, keepdim=True))
         _place(cache, table, i, 0, k.to(t), 1e-3 * torch.randn(H, D, device="cuda").to(t))
     _check(ave.paged_attention(q, cache, table, n), q, cache, table, n)
+
+
+@pytest.mark.parametrize("code", [F16, I8])
+@pytest.mark.parametrize("size", [1e3, 2.0 ** 18, 1e6, 1e8])
+def test_large_scores(rocm_device, size, code):
+    """Scores of such a size: one token takes all of the softmax, or tokens of the same key share it."""
+    q, cache, table, n = _case([300, 1, 40], 1, 4, 2, 64, 16, F16, code, seed=30)
+    for sign in (1, -1):
+        k = sign * q[:, 0, ::2].float()
+        scale = size / k.square().sum(-1).amin().item()
+        for i, ln in enumerate(n.tolist()):
+            for at in range(ln):
+                page, row = _token(cache, table, i, at)
+                if at % 3 == 0:
+                    _place(cache, table, i, at, k[i].half(), torch.full((2, 64), 2.0, device="cuda").half())
+                else:   # (a third of the key: far below, or far above, the others)
+                    _place(cache, table, i, at, (k[i] / 3).half(), torch.full((2, 64), 1.0, device="cuda").half())
+        o = ave.paged_attention(q, cache, table, n, scale)
+        # heads 0 and 2 have their own query in the keys; a sequence of one token sees that alone
+        want = torch.tensor([2.0, 2.0, 2.0] if sign > 0 else [1.0, 2.0, 1.0], device="cuda")
+        assert ((o[:, 0, ::2].float() - want[:, None, None]).abs() <= 2 ** -10).all()
 
 
 @pytest.mark.parametrize("t,code", C8)
