@@ -18,7 +18,7 @@
 // has; all units in a row are cut into equal shares, one per workgroup, whatever
 // the lengths (read on the device: nothing here depends on a host copy of them).
 // A share that holds a whole (sequence, kv-head) writes its output; parts leave
-// m, the sum and o in the workspace and a second launch joins them.
+// m, the sum and o over it in the workspace and a second launch joins them.
 //
 // Measured, kernel and join: 256 sequences of 100 to 8192 tokens, 8 heads of 128 in
 // e4m3 395 + 5 us, 5.7 TB/s; one of 131072, 2 heads of 256 in bf16 50 + 5, 5.4 TB/s;
@@ -652,13 +652,15 @@ void paged_attn_kernel(PagedAttnArgs a) {
         sm[wave][16 * i + c16] = m[i];
         sl[wave][16 * i + c16] = sum[i];
       }
+      // (each divided by its own sum: values near fp32's largest do not leave its range when
+      // they are added up)
+      const float f = sum[i] == 0.f ? 0.f : 1.f / sum[i] * (C8 ? unit[i] * BACK : 1.f);
       if (row_of(i) < a.R) {
 #pragma unroll
         for (int j = 0; j < E; ++j)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            buf[wave][16 * i + c16][(j / CH) * 16 * CH + (4 * g + r) * CH + j % CH] =
-                acc[i][j][r] * (C8 ? unit[i] * BACK : 1.f);
+            buf[wave][16 * i + c16][(j / CH) * 16 * CH + (4 * g + r) * CH + j % CH] = acc[i][j][r] * f;
       }
     }
     __syncthreads();
@@ -672,18 +674,20 @@ void paged_attn_kernel(PagedAttnArgs a) {
 #pragma unroll
       for (int w = 1; w < TW; ++w) M = fmaxf(M, sm[w0 + w * RWS][c]);
       const float ref = M == -INFINITY ? 0.f : M;
-      float s = 0.f;
+      float s = 0.f, f[TW];
       f32x4 o = zero4();
 #pragma unroll
       for (int w = 0; w < TW; ++w) {
-        const float f = exp2i(sm[w0 + w * RWS][c] - ref);
-        s += f * sl[w0 + w * RWS][c];
-        o += f * *reinterpret_cast<const f32x4*>(&buf[w0 + w * RWS][c][d]);
+        f[w] = exp2i(sm[w0 + w * RWS][c] - ref) * sl[w0 + w * RWS][c];
+        s += f[w];
       }
+      const float inv = s == 0.f ? 0.f : 1.f / s;
+#pragma unroll
+      for (int w = 0; w < TW; ++w)
+        o += f[w] * inv * *reinterpret_cast<const f32x4*>(&buf[w0 + w * RWS][c][d]);
       const int orow = group * rg + row;
       const long long at = ((long long)n * a.L + orow / a.G) * a.Hq + kvh * a.G + orow % a.G;
       if (whole) {
-        o *= s == 0.f ? 0.f : 1.f / s;
         u16x4 h;
 #pragma unroll
         for (int j = 0; j < 4; ++j) h[j] = Elt<QT>::from_f(o[j]);
@@ -732,7 +736,6 @@ __global__ __launch_bounds__(NT) void paged_attn_join_kernel(PagedAttnArgs a) {
   const int wg = ds.z / 2;
   auto at = [&](int p) { return a.part + (p == 0 ? ds.z : 2 * (wg + p)) * each; };
   auto put = [&](int orow, float M, float s, f32x4 o) {
-    o *= s == 0.f ? 0.f : 1.f / s;
     const long long out = ((long long)ds.x * a.L + orow / a.G) * a.Hq + kvh * a.G + orow % a.G;
     u16x4 h;
 #pragma unroll
@@ -762,9 +765,14 @@ __global__ __launch_bounds__(NT) void paged_attn_join_kernel(PagedAttnArgs a) {
 #pragma unroll
     for (int p = 0; p < kFewParts; ++p) {
       if (p >= parts) break;
-      const float f = exp2i(m[p] - ref);
-      s += f * l[p];
-      o += f * x[p];
+      l[p] *= exp2i(m[p] - ref);
+      s += l[p];
+    }
+    const float inv = s == 0.f ? 0.f : 1.f / s;
+#pragma unroll
+    for (int p = 0; p < kFewParts; ++p) {
+      if (p >= parts) break;
+      o += l[p] * inv * x[p];
     }
     put(orow, M, s, o);
     return;
@@ -786,17 +794,21 @@ __global__ __launch_bounds__(NT) void paged_attn_join_kernel(PagedAttnArgs a) {
   const float ref = M == -INFINITY ? 0.f : M;
   float s = 0.f;
   for (int p = tid; p < parts; p += NT) {
-    const float f = exp2i(w[p] - ref);
+    const float f = exp2i(w[p] - ref) * at(p)[a.rows * (D + 1) + row];
     w[p] = f;
-    s += f * at(p)[a.rows * (D + 1) + row];
+    s += f;
   }
 #pragma unroll
   for (int off = 1; off < 64; off *= 2) s += __shfl_xor(s, off);
   if (lane == 0) red[1][wave] = s;
   __syncthreads();
+  s = 0.f;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) s += red[1][i];
+  const float inv = s == 0.f ? 0.f : 1.f / s;
   f32x4 o = zero4();
 #pragma unroll 8
-  for (int p = grp; p < parts; p += GR) o += w[p] * *reinterpret_cast<const f32x4*>(at(p) + row * D + 4 * col);
+  for (int p = grp; p < parts; p += GR) o += w[p] * inv * *reinterpret_cast<const f32x4*>(at(p) + row * D + 4 * col);
 #pragma unroll
   for (int off = LP; off < 64; off *= 2)
 #pragma unroll
@@ -804,9 +816,6 @@ __global__ __launch_bounds__(NT) void paged_attn_join_kernel(PagedAttnArgs a) {
   if (lane < LP) acc[wave][lane] = o;
   __syncthreads();
   if (tid >= LP) return;
-  s = 0.f;
-#pragma unroll
-  for (int i = 0; i < NW; ++i) s += red[1][i];
 #pragma unroll
   for (int i = 1; i < NW; ++i) o += acc[i][tid];
   put(orow, M, s, o);

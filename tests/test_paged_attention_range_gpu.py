@@ -121,3 +121,16 @@ def test_a_large_value_of_no_weight(rocm_device, power, lens, D, t, code):
             page, row = _token(cache, table, i, at)
             cache.v_scale[page, :, row] *= 2.0 ** power
     _check(ave.paged_attention(q, cache, table, n), q, cache, table, n)
+
+
+@pytest.mark.parametrize("code", [E4M3, I8])
+@pytest.mark.parametrize("D,H,lens", [(128, 2, [1, 40, 300, 9000]), (256, 1, [5000]), (64, 2, [250] * 560)])
+@pytest.mark.parametrize("top", [125, -100])
+def test_far_scales(rocm_device, top, D, H, lens, code):
+    """Values up to 2^top: neither their sum over the tokens nor a factor on its way leaves fp32's range."""
+    q, cache, table, n = _case(lens, 1, 2 * H, H, D, 16, BF16, code, seed=7)
+    page = cache.k.shape[2]
+    for i, ln in enumerate(lens):   # (the rows that tokens have; the others stay NaN)
+        for p in range(-(-ln // page)):
+            cache.v_scale[int(table[i, p]), :, :min(page, ln - p * page)].mul_(2.0 ** (top - 3))   # |v| < 8
+    _check(ave.paged_attention(q, cache, table, n), q, cache, table, n)
