@@ -247,6 +247,7 @@ def paged_attention(
         raise ValueError(f"{name}: window must not be negative.")
     if block_table.stride(1) != 1 or block_table.stride(0) < block_table.shape[1]:
         block_table = block_table.contiguous()
+    lengths = lengths.contiguous()   # (a copy lives until the launch)
     held = block_table.shape[1] * page
     if max_length is None:
         max_length = held
@@ -276,7 +277,7 @@ def paged_attention(
         raise ValueError(f"{name}: workspace must be contiguous on {dev}.")
     _native.check(_native.on_device(
         dev, lib.gdn_paged_attn_fwd, q.data_ptr(), sn, sl, sh, *cache.ptrs, block_table.data_ptr(),
-        max(block_table.stride(0), block_table.shape[1]), lengths.contiguous().data_ptr(), out.data_ptr(),
+        max(block_table.stride(0), block_table.shape[1]), lengths.data_ptr(), out.data_ptr(),
         _ptr(lse), N, L, Hq, H, D, pages, page, max_length, min(int(window), 1 << 30),
         D ** -0.5 if scale is None else float(scale), _DTYPES[q.dtype], cache.code, workspace.data_ptr(),
         workspace.numel() * workspace.element_size(), _stream(dev)), name)
