@@ -601,7 +601,7 @@ def _recurrent_indexed(q, k, v, g, beta, scale, pool, output_final_state, cu_seq
         raise ValueError(f"{name}: ssm_state_indices must be int32 of shape ({N},) on {dev} "
                          "or the CPU.")
     _check_distinct_slots(idx, pool.shape[0], name)
-    idx = idx.to(dev)
+    idx = idx.to(dev).contiguous()
     if scale is None:
         scale = K ** -0.5
     o = _out(v, out, name)
@@ -610,18 +610,18 @@ def _recurrent_indexed(q, k, v, g, beta, scale, pool, output_final_state, cu_seq
         rc = _native.lib().gdn_recurrent_fwd_rows(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), *rows,
             *_rows_gates(gate, g, beta, Hv, dev, name), pool.data_ptr(), _ptr(ht), o.data_ptr(),
-            _ptr(cu), idx.contiguous().data_ptr(), B, T, Hqk, Hv, K, V, N, pool.shape[0],
+            _ptr(cu), idx.data_ptr(), B, T, Hqk, Hv, K, V, N, pool.shape[0],
             float(scale), int(bool(use_qk_l2norm_in_kernel)), _stream_ptr(dev))
     elif gate is not None:
         rc = _native.lib().gdn_recurrent_fwd_gating(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), *_gate_ptrs(gate, g, beta, Hv, dev, name),
-            pool.data_ptr(), _ptr(ht), o.data_ptr(), _ptr(cu), idx.contiguous().data_ptr(),
+            pool.data_ptr(), _ptr(ht), o.data_ptr(), _ptr(cu), idx.data_ptr(),
             B, T, Hqk, Hv, K, V, N, pool.shape[0], float(scale),
             int(bool(use_qk_l2norm_in_kernel)), _stream_ptr(dev))
     else:
         rc = _native.lib().gdn_recurrent_fwd_indexed(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), g.data_ptr(), beta.data_ptr(),
-            pool.data_ptr(), _ptr(ht), o.data_ptr(), _ptr(cu), idx.contiguous().data_ptr(),
+            pool.data_ptr(), _ptr(ht), o.data_ptr(), _ptr(cu), idx.data_ptr(),
             B, T, Hqk, Hv, K, V, N, pool.shape[0], float(scale),
             int(bool(use_qk_l2norm_in_kernel)), _stream_ptr(dev))
     _native.check(rc, name)
@@ -685,9 +685,15 @@ def _recurrent_spec(q, k, v, g, beta, scale, pool, cu_seqlens, use_qk_l2norm_in_
 
 
 # ------------------------------------------------ gating fused into the core
+def _gate(A_log, dt_bias, beta, threshold):
+    """The gating parameters, contiguous (the caller holds copies until its launch)."""
+    A_log, dt_bias = (t.contiguous() if isinstance(t, torch.Tensor) else t for t in (A_log, dt_bias))
+    return A_log, dt_bias, beta, threshold
+
+
 def _gate_ptrs(gate, a, b, Hv, dev, name):
     """Pointer / code arguments of the *_gating entry points, after checking
-    A_log, dt_bias ([Hv], one dtype) and the gating inputs a, b."""
+    A_log, dt_bias ([Hv], one dtype; of ``_gate``) and the gating inputs a, b."""
     from .layer_ops import _dt
     A_log, dt_bias, spb, spt = gate
     for nm, t in (("A_log", A_log), ("dt_bias", dt_bias)):
@@ -698,8 +704,8 @@ def _gate_ptrs(gate, a, b, Hv, dev, name):
     if not spb > 0:
         raise ValueError(f"{name}: softplus beta must be > 0.")
     adt, bdt, pdt = _dt(a, name, "a"), _dt(b, name, "b"), _dt(A_log, name, "A_log")
-    return (A_log.contiguous().data_ptr(), a.data_ptr(), b.data_ptr(),
-            dt_bias.contiguous().data_ptr(), adt, bdt, pdt, float(spb), float(spt))
+    return (A_log.data_ptr(), a.data_ptr(), b.data_ptr(), dt_bias.data_ptr(), adt, bdt, pdt,
+            float(spb), float(spt))
 
 
 def _rows_gates(gate, g, beta, Hv, dev, name):
@@ -760,7 +766,7 @@ def chunk_gated_delta_rule_gated(
                                       save_for_backward=save_for_backward)
     return _chunk_fwd(q, k, v, a, b, scale, initial_state, output_final_state, cu_seqlens,
                       use_qk_l2norm_in_kernel, workspace=workspace, out=out,
-                      gate=(A_log, dt_bias, softplus_beta, softplus_threshold),
+                      gate=_gate(A_log, dt_bias, softplus_beta, softplus_threshold),
                       name="chunk_gated_delta_rule_gated")
 
 
@@ -789,7 +795,7 @@ def fused_recurrent_gated_delta_rule_gated(
     kernel forms g and beta from ``a``, ``b``, ``A_log``, ``dt_bias`` per
     token (see ``chunk_gated_delta_rule_gated``)."""
     name = "fused_recurrent_gated_delta_rule_gated"
-    gate = (A_log, dt_bias, softplus_beta, softplus_threshold)
+    gate = _gate(A_log, dt_bias, softplus_beta, softplus_threshold)
     if ssm_state_indices is not None:
         if ssm_state_indices.dim() != 1:
             raise ValueError(f"{name}: ssm_state_indices must be 1-D [N].")
