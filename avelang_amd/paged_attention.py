@@ -17,6 +17,7 @@ import functools
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _native
 from .layer_ops import _DTYPES, _ptr, _stream
@@ -36,7 +37,7 @@ class PagedKVCache:
     in 8 bits, ``k_scale``, ``v_scale`` [num_pages, kv_heads, page_size] fp32.
     ``PagedKVCache.zeros`` allocates them; they are not replaced or resized later."""
 
-    __slots__ = ("_held", "sizes", "code")
+    __slots__ = ("_held", "_versions", "sizes", "code")
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None,
                  v_scale: Optional[torch.Tensor] = None):
@@ -60,6 +61,7 @@ class PagedKVCache:
         elif k_scale is not None or v_scale is not None:
             raise ValueError(f"{name}: a cache in {dtype} has no scales.")
         self._held = k, v, k_scale, v_scale
+        self._versions = [t for t in self._held if t is not None and not t.is_inference()]
         self.sizes = heads, size, pages, page
         self.code = _TYPES[dtype]
 
@@ -150,6 +152,7 @@ def paged_cache_write(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
         dev, _native.lib().gdn_paged_write, k.data_ptr(), v.data_ptr(), sk[0], sk[1], sv[0], sv[1],
         slots.data_ptr(), slots.dtype is torch.int64, *cache.ptrs, slots.numel(), H, D, pages, page,
         _DTYPES[k.dtype], cache.code, _stream(dev)), name)
+    increment_version(cache._versions)   # (autograd, where it kept them, sees that they changed)
 
 
 def paged_cache_read(cache: PagedKVCache, slots: torch.Tensor,
@@ -268,6 +271,8 @@ def paged_attention(
           or out.device != dev or not out.is_contiguous() or out.data_ptr() % 16):
         raise ValueError(f"{name}: out must be a contiguous, 16-byte aligned {q.dtype} tensor of shape "
                          f"{tuple(q.shape)} on {dev}.")
+    elif not out.is_inference():
+        increment_version(out)   # (autograd may have kept it)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if return_lse else None
     lib = _native.lib()
     if workspace is None:
