@@ -11,6 +11,8 @@
 //
 // bf16: 8192 tokens of 40 heads of 128 38 us, 4.4 TB/s read and written; 256 tokens
 // of 18 heads of 256, a quarter turned, 5.3 us: a round trip behind the angles.
+#include <algorithm>
+
 #include "gdn_norm_rows.h"
 #include "../../include/gdn_attn.h"
 
@@ -146,6 +148,57 @@ __global__ __launch_bounds__(256) void rotary_kernel(RotaryArgs a) {
 
 }  // namespace gdn
 
+namespace {
+
+// Whether sum x_i stride_i = rem has a solution with lo_i <= x_i <= hi_i, strides falling: of
+// each only the x that leave what the rest can reach (one or two where strides nest; `steps`
+// bounds what others may take, and what is not settled by then counts as a solution).
+struct Term {
+  long long stride, lo, hi;
+};
+bool solvable(const Term* t, int n, long long rem, int& steps) {
+  if (n == 0) return rem == 0;
+  if (--steps < 0) return true;
+  long long least = 0, most = 0;   // of the rest
+  for (int i = 1; i < n; ++i) {
+    least += t[i].lo * t[i].stride;
+    most += t[i].hi * t[i].stride;
+  }
+  auto floor_div = [](long long a, long long b) { return a >= 0 ? a / b : -((b - 1 - a) / b); };
+  const long long from = std::max(t->lo, -floor_div(most - rem, t->stride));
+  const long long to = std::min(t->hi, floor_div(rem - least, t->stride));
+  for (long long x = from; x <= to; ++x)
+    if (solvable(t + 1, n - 1, rem - x * t->stride, steps)) return true;
+  return false;
+}
+
+// Whether two tensors [n0, n1, n2, D] (strides in elements of es bytes, the last 1) share a byte.
+bool share(const void* a, const long long* as, const long long (&an)[3], const void* b, const long long* bs,
+           const long long (&bn)[3], int D, int es) {
+  Term t[7];
+  int n = 0;
+  auto add = [&](long long stride, long long lo, long long hi) {
+    if (stride == 0 || lo == hi) return;
+    int i = 0;
+    while (i < n && t[i].stride > stride) ++i;
+    if (i == n || t[i].stride != stride) {
+      for (int j = n++; j > i; --j) t[j] = t[j - 1];
+      t[i] = Term{stride, 0, 0};
+    }
+    t[i].lo += lo;
+    t[i].hi += hi;
+  };
+  for (int j = 0; j < 3; ++j) {
+    add(as[j] * es, 0, an[j] - 1);
+    add(bs[j] * es, 1 - bn[j], 0);
+  }
+  add(1, 1 - D * es, D * es - 1);
+  int steps = 1 << 16;
+  return solvable(t, n, (long long)(reinterpret_cast<intptr_t>(b) - reinterpret_cast<intptr_t>(a)), steps);
+}
+
+}  // namespace
+
 extern "C" int gdn_rotary(const void* q, const void* k, void* q_out, void* k_out,
                           const long long* strides, int B, int T, int Hq, int Hk, int D,
                           const void* positions, int pos_int64, long long pos_batch,
@@ -180,12 +233,12 @@ extern "C" int gdn_rotary(const void* q, const void* k, void* q_out, void* k_out
     if (inplace != (x[i] == y[i]))
       return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": both tensors in place, or none");
   }
-  if (two == 2 && y[0] == y[1])
-    return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": the two outputs must not be one");
   const int es = dtype == GDN_DTYPE_F32 ? 4 : 2;
   auto bytes = [&](const long long* st, int h) {
     return (size_t)((B - 1) * st[0] + (T - 1) * st[1] + (h - 1) * st[2] + D) * es;
   };
+  if (two == 2 && share(y[0], ys, {B, T, Hq}, y[1], ys + 3, {B, T, Hk}, D, es))
+    return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": the two outputs must share no element");
   if (!inplace)
     for (int i = 0; i < two; ++i)
       for (int j = 0; j < two; ++j)

@@ -168,9 +168,9 @@ def rotary_embedding(q: torch.Tensor, k: Optional[torch.Tensor], positions: torc
     ``positions`` (int32 / int64, [T] or [B, T]) may be any integers; the first
     ``2 * len(inv_freq)`` elements of a head turn (``rotary_frequencies``; fp64 keeps
     far positions' angles), the rest is copied.  Strided inputs (column slices of a
-    projection) are read in place; outputs are contiguous.  With ``inplace`` q and k
-    themselves are turned and returned.  Differentiable in q and k (the gradient is
-    turned back), not in place.
+    projection) are read in place; outputs are contiguous.  With ``inplace`` q and k,
+    which share no element, are turned themselves and returned.  Differentiable in q
+    and k (the gradient is turned back), not in place.
     """
     name = "rotary_embedding"
     if torch.is_grad_enabled() and (_grad(q) or _grad(k)):

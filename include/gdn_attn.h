@@ -66,7 +66,7 @@ int gdn_rms_norm_bwd(const void* h, const void* weight, const void* dy, const vo
  * q, k (nullable) [B, T, Hq | Hk, D] into q_out, k_out, elements contiguous:
  * strides holds the elements from one batch, token and head to the next, of q,
  * k, q_out and k_out (3 each).  q_out may be q and k_out k (the same strides: in
- * place, both or none; q and k share no element), else they overlap neither.
+ * place, both or none), else they overlap neither; q_out and k_out share no element.
  * positions [B, T]: int32, or int64 with pos_int64; pos_batch: from one batch's
  * to the next's (0: the same positions).
  */
