@@ -49,6 +49,7 @@ struct PagedAttnArgs {
   float* part;
   int4* desc;
   int N, L, Hq, Hkv, G, R, RG, rows;   // R = L G rows per kv-head in RG groups of at most `rows`
+  int part_size;  // floats of a part: o [rows][D], m, sums [rows], 16-byte aligned
   int num_pages, page, cap, window;
   int whole;      // every (sequence, kv-head) is one unit, however long (no second launch)
   int by_item;    // desc has an entry per (sequence, kv-head, group of rows), not per workgroup
@@ -666,7 +667,7 @@ void paged_attn_kernel(PagedAttnArgs a) {
     __syncthreads();
     const bool whole = len == cost;
     const int slot = u == u0 ? 2 * blockIdx.x : 2 * blockIdx.x + 1;
-    float* const part = a.part + (size_t)slot * a.rows * (D + 2);
+    float* const part = a.part + (size_t)slot * a.part_size;
     const int group = 16 * RWS * NT, here = min(a.R - group * rg, group);   // rows of this group
     for (int i = tid; i < here * (D / 4); i += 256) {
       const int row = i / (D / 4), d = 4 * (i % (D / 4)), w0 = row / (16 * NT), c = row % (16 * NT);
@@ -731,10 +732,9 @@ __global__ __launch_bounds__(NT) void paged_attn_join_kernel(PagedAttnArgs a) {
   const int kvh = ds.y / a.RG, rg = ds.y % a.RG, row = blockIdx.y;
   const int tid = threadIdx.x, wave = tid / 64, lane = tid % 64, grp = tid / LP;
   const int col = blockIdx.z * LP + tid % LP;
-  const size_t each = (size_t)a.rows * (D + 2);
   // part p: its workgroup's first, but for the one that begins here
   const int wg = ds.z / 2;
-  auto at = [&](int p) { return a.part + (p == 0 ? ds.z : 2 * (wg + p)) * each; };
+  auto at = [&](int p) { return a.part + (size_t)(p == 0 ? ds.z : 2 * (wg + p)) * a.part_size; };
   auto put = [&](int orow, float M, float s, f32x4 o) {
     const long long out = ((long long)ds.x * a.L + orow / a.G) * a.Hq + kvh * a.G + orow % a.G;
     u16x4 h;
@@ -832,7 +832,7 @@ namespace {
 
 // Workgroups, and how the rows of a kv-head are laid over their waves.
 struct AttnPlan {
-  int nt, rw, rg, rows;
+  int nt, rw, rg, rows, part_size;
   long long wgs, grid, items;   // workgroups where work is cut, launched
   bool each;    // every wave on its own
   bool whole;   // every (sequence, kv-head) one unit: nothing is cut
@@ -875,8 +875,9 @@ int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_le
   p.whole = p.each || (row_bytes && units <= 24 && (units - 2) * p.wgs <= 6 * p.items);
   if (p.wgs > most) p.wgs = most;
   p.grid = p.each ? std::min(p.wgs, (p.items + 3) / 4) : p.whole ? std::min(p.items, 1LL << 20) : p.wgs;
+  p.part_size = (p.rows * (D + 2) + 3) / 4 * 4;
   p.desc = (size_t)p.wgs * 16;
-  p.bytes = p.desc + (size_t)p.wgs * 2 * p.rows * (D + 2) * sizeof(float);
+  p.bytes = p.desc + (size_t)p.wgs * 2 * p.part_size * sizeof(float);
   p.bytes = (p.bytes + 255) / 256 * 256;
   return GDN_OK;
 }
@@ -954,6 +955,7 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long long q_seq, long long q_to
   a.R = (int)R;
   a.RG = p.rg;
   a.rows = p.rows;
+  a.part_size = p.part_size;
   a.num_pages = num_pages;
   a.page = page_size;
   a.cap = max_length;
