@@ -11,7 +11,8 @@ import ctypes
 import threading
 from pathlib import Path
 
-import torch  # noqa: F401  (load torch's HIP runtime before libgdn.so)
+import torch  # (loads torch's HIP runtime before libgdn.so)
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "libgdn.so"
 
@@ -279,6 +280,14 @@ def on_device(dev, fn, *args):
         return fn(*args)
     with torch.cuda.device(dev):
         return fn(*args)
+
+
+def no_tangents(name: str, *tensors) -> None:
+    """Refuse tensors with a forward-mode tangent, which no operator here carries on."""
+    if forward_ad._current_level < 0:
+        return
+    if any(isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name}: forward-mode differentiation is not supported.")
 
 
 def last_error() -> str:

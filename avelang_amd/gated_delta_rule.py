@@ -105,6 +105,7 @@ def _cu_on_device(c32: torch.Tensor, dev: torch.device) -> torch.Tensor:
 
 def _check_inputs(q, k, v, g, beta, initial_state, cu_seqlens, name, convert_gates=True,
                   contiguous=True):
+    _native.no_tangents(name, q, k, v, g, beta, initial_state)
     for nm, t in (("q", q), ("k", k), ("v", v)):
         if not isinstance(t, torch.Tensor):
             raise ValueError(f"{name}: {nm} must be a torch.Tensor")
@@ -233,6 +234,7 @@ def chunk_gated_delta_rule_bwd(
     raw q and k.
     """
     name = "chunk_gated_delta_rule_bwd"
+    _native.no_tangents(name, do, dht)
     q, k, v, g, beta, cu, (B, T, Hqk, Hv, K, V, N) = _check_inputs(
         q, k, v, g, beta, initial_state, cu_seqlens, name)
     if scale is None:
@@ -696,6 +698,7 @@ def _gate_ptrs(gate, a, b, Hv, dev, name):
     A_log, dt_bias ([Hv], one dtype; of ``_gate``) and the gating inputs a, b."""
     from .layer_ops import _dt
     A_log, dt_bias, spb, spt = gate
+    _native.no_tangents(name, A_log, dt_bias)
     for nm, t in (("A_log", A_log), ("dt_bias", dt_bias)):
         if not isinstance(t, torch.Tensor) or tuple(t.shape) != (Hv,) or t.device != dev:
             raise ValueError(f"{name}: {nm} must be a tensor of shape ({Hv},) on {dev}.")

@@ -111,6 +111,7 @@ def fused_gdn_gating(
 
 def _gating_args(A_log, a, b, dt_bias, beta, name):
     """Validated, contiguous (A_log, a, b, dt_bias) and their dtype codes."""
+    _native.no_tangents(name, A_log, a, b, dt_bias)
     for nm, t in (("A_log", A_log), ("a", a), ("b", b), ("dt_bias", dt_bias)):
         if not isinstance(t, torch.Tensor):
             raise ValueError(f"{name}: {nm} must be a torch.Tensor")
@@ -166,6 +167,7 @@ def fused_gdn_gating_bwd(
     ``db`` is None when ``dbeta`` is.
     """
     name = "fused_gdn_gating_bwd"
+    _native.no_tangents(name, dg, dbeta)
     A_log, a, b, dt_bias, adt, bdt, pdt = _gating_args(A_log, a, b, dt_bias, beta, name)
     H = a.shape[-1]
     dev = a.device
@@ -221,6 +223,7 @@ def l2norm_fwd(x: torch.Tensor, eps: float = 1e-6,
     ``out`` may be ``x`` itself.
     """
     name = "l2norm_fwd"
+    _native.no_tangents(name, x)
     if not isinstance(x, torch.Tensor) or x.dim() < 1:
         raise ValueError(f"{name}: x must be a tensor with at least one axis.")
     D = x.shape[-1]
@@ -263,6 +266,7 @@ def causal_conv1d_fn(
     given).  The output has ``x``'s layout and dtype.
     """
     name = "causal_conv1d_fn"
+    _native.no_tangents(name, x, weight, bias, initial_states)
     if not isinstance(x, torch.Tensor) or x.dim() != 3:
         raise ValueError(f"{name}: x must be a 3-D tensor [B, D, T].")
     B, D, T = x.shape
@@ -327,6 +331,7 @@ def causal_conv1d_update(
     Returns the output with ``x``'s shape and dtype.
     """
     name = "causal_conv1d_update"
+    _native.no_tangents(name, x, conv_state, weight, bias)
     if not isinstance(x, torch.Tensor) or x.dim() not in (2, 3):
         raise ValueError(f"{name}: x must be [B, D] or [B, D, L].")
     squeeze = x.dim() == 2
@@ -382,6 +387,7 @@ def rms_norm_gated(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor,
     ``weight`` has ``x``'s dtype), times ``silu(z)`` in fp32, rounded.
     """
     name = "rms_norm_gated"
+    _native.no_tangents(name, x, z, weight)
     if not isinstance(x, torch.Tensor) or not isinstance(z, torch.Tensor) or x.dim() < 1:
         raise ValueError(f"{name}: x and z must be tensors.")
     if x.shape != z.shape or x.dtype != z.dtype:

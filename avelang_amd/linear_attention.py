@@ -45,6 +45,7 @@ def _inputs(q, k, v, g, cu_seqlens, name, out=None):
     """Checked q, k, v (as the kernels take them), g, cu_seqlens on the device,
     the token strides and the sizes (B, T, Hqk, Hv, K, V, N)."""
     bf16 = torch.bfloat16
+    _native.no_tangents(name, q, k, v, g)
     for nm, t in (("q", q), ("k", k), ("v", v)):
         if not isinstance(t, torch.Tensor):
             raise ValueError(f"{name}: {nm} must be a torch.Tensor")
@@ -105,6 +106,7 @@ def _cu(cu_seqlens, B, T, dev, name):
 
 
 def _state(t, shape, dev, what, name):
+    _native.no_tangents(name, t)
     if (not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype is not torch.float32
             or t.device != dev):
         raise ValueError(f"{name}: {what} must be torch.float32 of shape {shape} on {dev}.")
@@ -207,6 +209,7 @@ def _chunk_bwd(inputs, do, dht, scale, initial_state, want_dh0, states, workspac
     q, k, v, g, cu, rows, dims = inputs
     B, T, Hqk, Hv, K, V, N = dims
     dev = q.device
+    _native.no_tangents(name, do)
     if (not isinstance(do, torch.Tensor) or do.shape != v.shape or do.dtype != torch.bfloat16
             or do.device != dev):
         raise ValueError(f"{name}: do must be a bf16 tensor of shape {tuple(v.shape)} on {dev}.")
@@ -355,6 +358,7 @@ def fused_recurrent_linear_attn(
     dev = q.device
     o = _out(v, out, name)
     h0, ht, idx, slots = initial_state, None, None, N
+    _native.no_tangents(name, h0)
     if ssm_state_indices is not None:
         idx = ssm_state_indices
         if not isinstance(h0, torch.Tensor) or h0.dim() != 4:

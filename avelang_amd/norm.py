@@ -33,6 +33,7 @@ __all__ = ["layer_norm", "layer_norm_fwd_save", "layer_norm_bwd",
 
 def _args(x, weight, bias, name):
     """Checked, contiguous x and parameters, with rows, heads, D and type codes."""
+    _native.no_tangents(name, x, weight, bias)
     if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{name}: x must be a tensor with a last axis of at least 1.")
     dt = _dt(x, name, "x")
@@ -128,6 +129,7 @@ def _stats(stats, rows, dev, name):
 
 
 def _bwd(x, weight, dy, stats, rows, heads, D, dt, wdt, dw, db, name):
+    _native.no_tangents(name, dy)
     dy = dy.contiguous()
     dx = torch.empty_like(x)
     lib = _native.lib()
@@ -187,6 +189,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
 
 def _rms_args(x, weight, residual, name):
     """Checked, contiguous x, weight and residual, with rows, D and type codes."""
+    _native.no_tangents(name, x, weight, residual)
     if not isinstance(x, torch.Tensor) or x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{name}: x must be a tensor with a last axis of at least 1.")
     dt = rdt = wdt = _dt(x, name, "x")
@@ -265,6 +268,7 @@ def _rms_bytes(device, rows, D, dt):
 
 def _rms_bwd(args, dh, eps, offset, want_w, want_r, name):
     """On ``_rms_args`` of dy, weight and h."""
+    _native.no_tangents(name, dh)
     dy, weight, h, rows, D, dt, hdt, wdt = args
     dev = dy.device
     if dh is not None:

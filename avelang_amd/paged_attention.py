@@ -130,6 +130,7 @@ def paged_cache_write(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor,
     reached that, and one that is not finite has a scale of NaN.
     """
     name = "paged_cache_write"
+    _native.no_tangents(name, k, v)
     H, D, pages, page = _cache(cache, name).sizes
     dev = cache.k.device
     slots = _slots(slots, cache, name, True)
@@ -161,6 +162,7 @@ def paged_cache_read(cache: PagedKVCache, slots: torch.Tensor,
     hold, codes times their scales rounded to ``dtype`` (bf16 or fp16; default the
     cache's own, bf16 in 8 bits).  A slot outside the cache gives zeros."""
     name = "paged_cache_read"
+    _native.no_tangents(name, *getattr(cache, "_held", ()))
     H, D, pages, page = _cache(cache, name).sizes
     dev = cache.k.device
     slots = _slots(slots, cache, name, False)
@@ -223,6 +225,7 @@ def paged_attention(
     Deterministic.  Not differentiable.
     """
     name = "paged_attention"
+    _native.no_tangents(name, q, *getattr(cache, "_held", ()))
     H, D, pages, page = _cache(cache, name).sizes
     dev = cache.k.device
     if (not isinstance(q, torch.Tensor) or q.dim() != 4 or q.shape[3] != D or q.device != dev

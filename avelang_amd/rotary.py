@@ -72,6 +72,7 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, factor: float = 1.0, 
 
 def _turn(q, k, positions, inv_freq, magnitude, interleaved, inverse, inplace, name):
     """q and k (or None) turned: new contiguous tensors, or with ``inplace`` themselves."""
+    _native.no_tangents(name, q, k, inv_freq)
     if not isinstance(q, torch.Tensor) or not 3 <= (dims := q.dim()) <= 4:
         raise ValueError(f"{name}: q must be a tensor [B, T, H, D] or [T, H, D].")
     dt, dev, shape = _dt(q, name, "q"), q.device, q.shape
