@@ -257,6 +257,17 @@ extern "C" int gdn_paged_write(const void* k, const void* v, long long k_token, 
   if (T == 0 || num_pages == 0) return GDN_OK;
   if (!k || !v || !slots)
     return gdn_host::fail(GDN_ERR_NULL, std::string(name) + ": k, v and slots must be non-NULL");
+  // (all four are written or read by workgroups of their own)
+  const bool bits8 = cache_dtype == GDN_DTYPE_E4M3 || cache_dtype == GDN_DTYPE_I8;
+  const size_t rows = (size_t)num_pages * H * page_size, cb = rows * D * (bits8 ? 1 : 2);
+  auto bytes = [&](long long token, long long head) { return ((size_t)(T - 1) * token + (H - 1) * head + D) * 2; };
+  bool apart = !gdn_host::overlaps(k_cache, cb, v_cache, cb) &&
+               !(bits8 && gdn_host::overlaps(k_scale, rows * 4, v_scale, rows * 4));
+  for (const void* c : {k_cache, v_cache})
+    apart = apart && !gdn_host::overlaps(c, cb, k, bytes(k_token, k_head)) &&
+            !gdn_host::overlaps(c, cb, v, bytes(v_token, v_head));
+  if (!apart)
+    return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": the caches must not overlap each other, k or v");
   const gdn::PagedArgs a{{k, v}, {k_cache, v_cache}, {k_scale, v_scale}, {k_token, v_token}, {k_head, v_head}, slots,
                          (long long)num_pages * page_size, T, H, page_size, slots_int64};
   return launch_paged(name, true, a, D, dtype, cache_dtype, static_cast<hipStream_t>(stream));

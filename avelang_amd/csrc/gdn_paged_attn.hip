@@ -925,8 +925,10 @@ extern "C" int gdn_paged_attn_fwd(const void* q, long long q_seq, long long q_to
     return gdn_host::fail(GDN_ERR_SHAPE, std::string(name) + ": scales must be 16-byte aligned");
   const size_t ob = (size_t)N * L * Hq * D * 2;
   const size_t qb = ((size_t)(N - 1) * q_seq + (size_t)(L - 1) * q_token + (size_t)(Hq - 1) * q_head + D) * 2;
-  if (gdn_host::overlaps(o, ob, q, qb))
-    return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": o must not overlap q");
+  const size_t cb = (size_t)num_pages * Hkv * page_size * D * (bits8 ? 1 : 2);
+  if (gdn_host::overlaps(o, ob, q, qb) || gdn_host::overlaps(o, ob, k_cache, cb) ||
+      gdn_host::overlaps(o, ob, v_cache, cb))
+    return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": o must not overlap q or the caches");
   if (!workspace || workspace_bytes < p.bytes || reinterpret_cast<uintptr_t>(workspace) % 16)
     return gdn_host::fail(GDN_ERR_WORKSPACE, std::string(name) + ": workspace needs " + std::to_string(p.bytes) +
                                                  " bytes, 16-byte aligned, got " + std::to_string(workspace_bytes));

@@ -507,11 +507,15 @@ extern "C" int gdn_rms_norm_fwd(const void* x, const void* residual, const void*
   const int per = f.lpr ? 256 / f.lpr : 1;   // rows per workgroup
   if (const int fit = gdn_host::check_lanes(name, (rows + per - 1) / per, 256)) return fit;
   const size_t n = (size_t)rows * D, xb = dtype == GDN_DTYPE_F32 ? 4 : 2, rb = r_dtype == GDN_DTYPE_F32 ? 4 : 2;
-  const size_t yb = bits8 ? 1 : xb;
+  const size_t yb = bits8 ? 1 : xb, wb = (size_t)D * (w_dtype == GDN_DTYPE_F32 ? 4 : 2);
   // (a lane writes where it has read, of the same width)
   auto apart = [&](const void* out, size_t ob, const void* in, size_t ib) {
     return !in || (out == in && ob == ib) || !gdn_host::overlaps(out, n * ob, in, n * ib);
   };
+  // (the weight is read behind h's stores; of a single row y may be the weight)
+  auto over = [&](const void* out, size_t ob) { return weight && gdn_host::overlaps(out, n * ob, weight, wb); };
+  if ((over(y, yb) && !(rows == 1 && y == weight && yb * D == wb)) || (residual && over(h, rb)))
+    return gdn_host::fail(GDN_ERR_ALIAS, std::string(name) + ": outputs must not overlap the weight");
   if (!apart(y, yb, x, xb) || !apart(y, yb, residual, rb) ||
       (residual && (!apart(h, rb, x, xb) || !apart(h, rb, residual, rb) ||
                     gdn_host::overlaps(h, n * rb, y, n * yb))))

@@ -35,7 +35,8 @@ extern "C" {
  *     scale[row] = max |y| / M,  y's codes are y / scale rounded (M = 448, 127)
  * A row of zeros has scale 0 and codes 0; one under 2^-100 has the scale of
  * 2^-100; one that is not finite (or whose squares overflow fp32) has a scale
- * of NaN.  y may be x where the types are the same.  (h of 2^64 or more: its square
+ * of NaN.  y may be x where the types are the same; neither overlaps the weight (y of
+ * a single row may be it, of its type).  (h of 2^64 or more: its square
  * overflows fp32, and y is 0 or NaN.)
  */
 int gdn_rms_norm_fwd(const void* x, const void* residual, const void* weight, void* y, void* h,
@@ -86,7 +87,7 @@ int gdn_rotary(const void* q, const void* k, void* q_out, void* k_out, const lon
  * (cache_dtype == dtype) or as codes round(x M / max |x|), ties to even, with
  * scale max |x| / M (gdn_rms_norm_fwd's M and limits).  A slot outside the cache
  * is a padding token's: skipped.  What a slot that two tokens name holds
- * afterwards is not defined.
+ * afterwards is not defined.  The caches overlap neither each other nor k, v.
  * read: the rows of `slots`, codes times their scales in fp32, rounded to
  * dtype, into k, v [T, H, D] contiguous; a slot outside the cache gives zeros.
  */
@@ -104,7 +105,7 @@ int gdn_paged_read(const void* k_cache, const void* v_cache, const float* k_scal
  * Attention of every sequence's newest L tokens over the cache (page_size a
  * multiple of 16): q, o [N, L, Hq, D] of dtype (bf16, f16; q_seq, q_token,
  * q_head: q's strides in elements, multiples of 8, elements contiguous; o
- * contiguous), lengths [N] int32: tokens that sequence n has cached, the
+ * contiguous, overlapping neither q nor the caches), lengths [N] int32: tokens that sequence n has cached, the
  * newest L among them; token t of it is row t % page_size of page
  * block_table[n * table_row + t / page_size] (int32).  q-head h reads kv-head
  * h / (Hq / Hkv); row i stands at position p = lengths[n] - L + i and sees the
