@@ -6,16 +6,16 @@
 // one pass (in base 2).
 //
 // The path reads the cache once (2 D elements per token and kv-head against 4 D
-// flops per row: up to 16 rows share a read) and is bound by HBM.  A wave takes
-// 32 tokens at a time straight from HBM into the registers of its MFMA operands,
-// no LDS in between: S^T = K Q^T with tokens as rows leaves P^T in the layout in
+// flops per row: up to 32 rows share a read) and is bound by HBM.  A wave takes
+// 32 tokens at a time (64 where rows are short) straight from HBM into the registers
+// of its MFMA operands, no LDS in between: S^T = K Q^T with tokens as rows leaves P^T in the layout in
 // which it is the operand of O^T = V^T P^T, whose V^T a lane forms in its own
 // registers from eight tokens' 16-byte pieces (one v_perm per word).  The next
 // tokens' K is on its way while these' softmax and V are worked on, and the other
 // way round.
 //
-// Work: every (sequence, kv-head) is as many units of 128 tokens as its length
-// has; all units in a row are cut into equal shares, one per workgroup, whatever
+// Work: every (sequence, kv-head) is as many units of 128 tokens (256 where a wave
+// takes 64) as its length has; all units in a row are cut into equal shares, one per workgroup, whatever
 // the lengths (read on the device: nothing here depends on a host copy of them).
 // A share that holds a whole (sequence, kv-head) writes its output; parts leave
 // m, the sum and o over it in the workspace and a second launch joins them.
@@ -23,8 +23,13 @@
 // Measured, kernel and join: 256 sequences of 100 to 8192 tokens, 8 heads of 128 in
 // e4m3 395 + 5 us, 5.7 TB/s; one of 131072, 2 heads of 256 in bf16 50 + 5, 5.4 TB/s;
 // 48 of 1 to 6000, 4 heads of 128 in bf16, 4 newest tokens 67 + 5, 4.5 TB/s (the
-// shares' starts and ends, and the last tokens' masks); one of 449 8.7 + 2.5: a chain
+// shares' starts and ends, and the last tokens' masks); one of 449 9.0 + 2.5: a chain
 // of latencies, lengths, table, K, softmax, the waves' join.
+//
+// Many newest tokens are taken in groups of 64 rows, each of which reads all of the
+// sequence for itself, tokens past its own rows included (they are masked): 512 of
+// 8192, 8 q-heads to each of 4 kv-heads of 128 in bf16, 189 us, 2048 of them 626, where
+// their products alone are 54 and 195 at a large product's rate.
 #include <algorithm>
 
 #include "gdn_bits8.h"
@@ -194,8 +199,9 @@ __device__ __forceinline__ u16x8 codes_operand(uint32_t w0, uint32_t w1) {
 }
 
 // Sixteens of tokens that a wave takes at a time, by the bytes of a row and the row tiles
-// (of 16) that it works on: 8 KiB of K and as much of V on their way at once (16 KiB
-// where rows are 512 bytes).  An e4m3 cache of 8 heads of 128 elements, 256 ragged
+// (of 16) that it works on: 8 KiB of K and as much of V on their way at once where rows
+// are 128 bytes of one tile, or 256 (4 KiB where they are 64 of one tile, or 128 of two; 2
+// where 64 of two; 16 where 512).  An e4m3 cache of 8 heads of 128 elements, 256 ragged
 // sequences to 8192 tokens: 398 us, 465 with two sixteens.
 __host__ __device__ constexpr int sixteens(int row_bytes, int nt) { return row_bytes <= 128 && nt == 1 ? 4 : 2; }
 // Tokens of a unit of work: a step of all the waves that take tokens apart.
@@ -227,7 +233,11 @@ void paged_attn_kernel(PagedAttnArgs a) {
   constexpr int CH = E * ES > 16 ? 16 / ES : E;                    // elements of one piece
   constexpr int NS = sixteens(ROW, NT), TT = 16 * NS;              // tokens that a wave takes at a time
   constexpr float BACK = (CT == GDN_DTYPE_I8 ? kI8 : 1.f) / kTop;   // C8: of acc, beside its unit
-  constexpr bool LO = BF || QT == GDN_DTYPE_F16;   // P in two parts: 2^-8 (bf16), 2^-11 of one would show in o
+  // P in two parts: 2^-8 (bf16), 2^-11 of one would show in o.  (bf16 queries over 8 bits
+  // take one, an eighth of o's half step: 256 ragged sequences of e4m3 to 8192 tokens are
+  // 1.671e-3 from 64 bits in the norm, with two 1.661e-3, and 395 us, with two 397; 300 of 8
+  // heads of 64 in int8 to 4000 139 and 150.)
+  constexpr bool LO = BF || QT == GDN_DTYPE_F16;
   __shared__ float buf[EACH ? 1 : 4][EACH ? 1 : 16 * NT][D + 4];
   __shared__ float sm[4][16 * NT], sl[4][16 * NT];
   __shared__ int wave_sum[4];
@@ -870,7 +880,7 @@ int attn_plan(const char* name, int N, int L, int Hq, int Hkv, int D, int max_le
   // Else few units each are not cut: a join costs what two units do, and shares gain
   // the less the more workgroups there are without.  bf16 as above, in us: one sequence
   // of 250 tokens 6.8 (cut 8.6); 16 to 250, 700 6.9, 12.7 (9.1, 12.5); 60 to 449 13.9
-  // (19.4); 85 to 700, 3000 24, 111 (27, 111); 256 of 4 heads, 4 newest tokens, to 1000
+  // (19.6; in e4m3 13.0, 20.0); 85 to 700, 3000 24, 111 (27, 111); 256 of 4 heads, 4 newest tokens, to 1000
   // 63 (76).  24 units at most: one long sequence among short ones is one workgroup's.
   p.whole = p.each || (row_bytes && units <= 24 && (units - 2) * p.wgs <= 6 * p.items);
   if (p.wgs > most) p.wgs = most;

@@ -9,8 +9,10 @@
 // formed in 64 bits and reduced there, so far positions lose nothing, and no
 // position is out of a table's range.
 //
-// bf16: 8192 tokens of 40 heads of 128 38 us, 4.4 TB/s read and written; 256 tokens
-// of 18 heads of 256, a quarter turned, 5.3 us: a round trip behind the angles.
+// bf16: 8192 tokens of 40 heads of 128, neighbours, 38 us, 4.4 TB/s read and written (a
+// lane's two pieces lie side by side, so that the lanes of one instruction take 16 bytes of
+// every 32); 256 tokens of 18 heads of 256, a quarter turned, 5.3 us: a round trip behind
+// the angles.
 #include <algorithm>
 
 #include "gdn_norm_rows.h"
@@ -272,7 +274,7 @@ extern "C" int gdn_rotary(const void* q, const void* k, void* q_out, void* k_out
   a.inplace = inplace;
   a.mag = magnitude;
   a.sign = inverse ? -1.f : 1.f;
-  // groups of lanes per token: as many heads to a group as leave every CU eight
+  // groups of lanes per token: as many heads to a group as leave every CU four
   // workgroups, eight at most
   const int total = Hq + Hk;
   const long long want = 4LL * gdn::device_cus() * a.per_wg;

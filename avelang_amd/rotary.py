@@ -50,8 +50,11 @@ def rotary_frequencies(dim: int, base: float = 10000.0, *, factor: float = 1.0, 
     With ``original`` = 0 every frequency is divided by ``factor`` and the
     magnitude is 1.  Else ``original`` is the trained context: pairs that turn
     less than ``slow`` times over it are divided by the factor, those that turn
-    more than ``fast`` times keep theirs, a linear ramp lies between, and the
-    magnitude is 0.1 ln(factor) + 1.
+    more than ``fast`` times keep theirs, a ramp that is linear in the number of
+    turns lies between, and the magnitude is 0.1 ln(factor) + 1 (the formulas of
+    arXiv 2309.00071, "YaRN", 3.2 and 3.4).  Programs whose ramp is linear in the
+    pair's index instead, between two borders rounded to whole pairs, get other
+    frequencies there: give ``rotary_embedding`` theirs.
     """
     name = "rotary_frequencies"
     if dim < 2 or dim % 2 or not base > 0 or not factor > 0 or original < 0:

@@ -71,7 +71,8 @@ class HybridBlock(torch.nn.Module):
         return F.linear(o.flatten(2), self.lin_out), state
 
     def attention_layer(self, y, positions, slots, pages):
-        """y [N, T, width] of new tokens, T at most 64."""
+        """y [N, T, width] of new tokens, any T (every 64 rows of T tokens and a kv-head's q-heads read the whole
+        cache: pieces of some dozens of tokens are what the operator is made for)."""
         N, T, _ = y.shape
         q, k, v = F.linear(y, self.att_in).split(self.att_widths, -1)
         q, k, v = (t.view(N, T, -1, self.size) for t in (q, k, v))
