@@ -1,5 +1,5 @@
-"""Outputs that overlap what other workgroups still read or write are refused by the entry points (on the CPU: every
-call below is refused, or stops at a check behind)."""
+"""Outputs that overlap what other workgroups still read or write are refused by the entry points (on the CPU: no
+call below launches anything)."""
 import pytest
 
 from avelang_amd import _native
